@@ -332,6 +332,76 @@ int32_t infr_cuda_rmsnorm(infr_cuda_ctx* ctx, const infr_cuda_buf* x, const infr
 int32_t infr_cuda_add(infr_cuda_ctx* ctx, const infr_cuda_buf* a, const infr_cuda_buf* b, infr_cuda_buf* dst,
                       size_t n);
 
+/* ---- the attention half of a layer: rotary rows into a cache, attention over it --------------------
+ *
+ * What runs between two MoE calls, so that a layer's rows stay on this backend: Linear makes q, k and v rows,
+ * infr_cuda_rope_kv rotates q and k and puts k and v into the cache, infr_cuda_attention reads the cache, Linear and
+ * Add bring the result back to the residual stream.
+ *
+ * Rows are f32, as everywhere here; the cache is f16, in one of two layouts:
+ *   pages   k, v: [n_pages, n_kv, page_size, head_dim]; page_table: [n_seq, max_pages] i32, token i of sequence s is token
+ *           i % page_size of page page_table[s, i / page_size].  Pages may be shared by sequences that read them.
+ *   packed  k, v: [rows, n_kv, head_dim], the call's own rows in their order; page_table and kv_len are NULL.  For prompts
+ *           that need no cache (each row sees the rows before it of its own sequence).
+ * A batch is n_seq sequences: cu_q [n_seq + 1] i32, ascending, rows cu_q[s] .. cu_q[s + 1] - 1 are the new tokens of sequence s;
+ * kv_len [n_seq] i32 its tokens in the cache with the new ones, which are the last: row i of q_len has position
+ * kv_len - q_len + i (packed: i).  A sequence may have no rows.  Rows outside cu_q[0] .. cu_q[n_seq] - 1 are not read
+ * and their results stay as they were.  A row with a negative position (kv_len < q_len) writes nothing to the cache, its q stays
+ * as it was, and its attention is zero.
+ *
+ * All of these arrays are read on the device when the call runs, so a recorded plan follows new lengths and tables written into the same
+ * buffers.  What they say is checked there: a row number outside the call, a length past max_pages * page_size or a page outside
+ * [0, n_pages) is forced into range (a page that is not there is read as page 0, and not written), and the next infr_cuda_sync /
+ * download fails with INVALID_ARG.  Page table entries past a sequence's length are not read.
+ *
+ * head_dim: a multiple of 16 up to 256.  n_head: a multiple of n_kv, up to 128 query heads to each; query head h reads kv head
+ * h / (n_head / n_kv).  page_size: a multiple of 16.  Strides are in values between rows, a multiple of 4, 0 for rows side by side (as
+ * many values as heads x head_dim): the parts of one wide q/k/v row are buffers wrapped at their first value. */
+#define INFR_CUDA_ROPE_HALVES 0      /* pairs (i, i + n_rot / 2)  */
+#define INFR_CUDA_ROPE_INTERLEAVED 1 /* pairs (2 i, 2 i + 1)      */
+typedef struct infr_cuda_rope_kv_desc {
+  const infr_cuda_buf* q;            /* [rows, n_head, head_dim] f32, rows q_stride apart                     */
+  const infr_cuda_buf* k;            /* [rows, n_kv, head_dim] f32, rows k_stride apart                       */
+  const infr_cuda_buf* v;            /* [rows, n_kv, head_dim] f32, rows v_stride apart                       */
+  infr_cuda_buf* q_out;              /* [rows, n_head, head_dim] f32, rows q_out_stride apart; may be q itself
+                                        (same handle or address, same stride), else apart from q, k and v     */
+  infr_cuda_buf *k_cache, *v_cache;  /* f16, see above                                                        */
+  const infr_cuda_buf *cu_q, *kv_len, *page_table;
+  const infr_cuda_buf *q_norm, *k_norm; /* [head_dim] f32: RmsNorm over each head of q / k first, or NULL    */
+  const infr_cuda_buf* freq_factors; /* [n_rot / 2] f32: pair i's frequency is divided by it, or NULL
+                                        (GGUF rope_freqs.weight)                                              */
+  uint32_t rows, n_seq, n_head, n_kv, head_dim;
+  uint32_t n_pages, page_size, max_pages;              /* 0 for packed rows                                   */
+  uint32_t q_stride, k_stride, v_stride, q_out_stride;
+  uint32_t n_rot;                    /* leading values of a head that are rotated: a multiple of 8, 0 = none  */
+  uint32_t style;                    /* INFR_CUDA_ROPE_*                                                      */
+  float rope_base;                   /* pair i turns by position * rope_scale * rope_base^(-2 i / n_rot)      */
+  float rope_scale;                  /* 1 for plain rotary embedding                                          */
+  float norm_eps;
+} infr_cuda_rope_kv_desc;
+int32_t infr_cuda_rope_kv(infr_cuda_ctx* ctx, const infr_cuda_rope_kv_desc* desc);
+
+/* out[r, h, :] = sum_j w_j v_j,  w = softmax_j(scale * q[r, h, :] . k_j)  over the keys j of the row's sequence with
+ * position(r) - window < j <= position(r)  (window 0: all j <= position(r)); a row that sees no key gets zeros.
+ * f32 accuracy: q and the weights enter the tensor cores as two f16 pieces each, sums are f32.  Keys and values that a row may not
+ * see do not reach it, whatever bits they hold. */
+typedef struct infr_cuda_attention_desc {
+  const infr_cuda_buf* q;            /* [rows, n_head, head_dim] f32, rows q_stride apart                     */
+  const infr_cuda_buf *k, *v;        /* f16, pages or packed rows                                             */
+  infr_cuda_buf* out;                /* [rows, n_head, head_dim] f32, rows out_stride apart; not q, k or v    */
+  const infr_cuda_buf *cu_q, *kv_len, *page_table;
+  uint32_t rows, n_seq, n_head, n_kv, head_dim;
+  uint32_t n_pages, page_size, max_pages;              /* 0 for packed rows                                   */
+  uint32_t q_stride, out_stride;
+  uint32_t max_q;                    /* rows of a sequence at most, as far as the caller knows (0: `rows`).  Only
+                                        the choice of kernel goes by it: results do not                       */
+  uint32_t window;                   /* keys that a row sees at most; 0 = all before it                       */
+  float scale;                       /* usually head_dim^-0.5                                                 */
+  uint32_t path;                     /* 0 = choose; 1 = the few-rows kernel (up to 16 query heads to a kv head);
+                                        2 = the tensor-memory kernel                                          */
+} infr_cuda_attention_desc;
+int32_t infr_cuda_attention(infr_cuda_ctx* ctx, const infr_cuda_attention_desc* desc);
+
 /* ---- expert parallelism (crates/infr-vulkan/src/ep.rs:1-53, 156-505) ---------------------------- */
 
 /* The reference's ExpertParallelBackend gives rank r the contiguous expert band

@@ -30,6 +30,7 @@ EXPORTS = [
     "infr_cuda_gguf_open", "infr_cuda_gguf_close", "infr_cuda_gguf_tensor_count", "infr_cuda_gguf_tensor_name", "infr_cuda_gguf_find",
     "infr_cuda_gguf_meta_u64", "infr_cuda_gguf_meta_f64", "infr_cuda_gguf_meta_str", "infr_cuda_gguf_upload",
     "infr_cuda_sync", "infr_cuda_moe_ffn", "infr_cuda_moe_route", "infr_cuda_linear",
+    "infr_cuda_rope_kv", "infr_cuda_attention",
     "infr_cuda_gated_act", "infr_cuda_moe_shared_add", "infr_cuda_rmsnorm", "infr_cuda_add",
     "infr_cuda_moe_expert_rows", "infr_cuda_launch_count", "infr_cuda_em_down_ctas_per_sm",
     "infr_cuda_graph_begin", "infr_cuda_graph_end", "infr_cuda_graph_launch", "infr_cuda_graph_free", "infr_cuda_set_trace", "infr_cuda_moe_route_noalloc", "infr_cuda_moe_combine", "infr_cuda_umma_selftest",
@@ -124,6 +125,18 @@ class _Desc(C.Structure):
     ]
 
 
+class _RopeKvDesc(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v", "q_out", "k_cache", "v_cache", "cu_q", "kv_len", "page_table", "q_norm", "k_norm", "freq_factors")] + [
+        (n, C.c_uint32) for n in ("rows", "n_seq", "n_head", "n_kv", "head_dim", "n_pages", "page_size", "max_pages", "q_stride", "k_stride", "v_stride",
+                                  "q_out_stride", "n_rot", "style")] + [(n, C.c_float) for n in ("rope_base", "rope_scale", "norm_eps")]
+
+
+class _AttentionDesc(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v", "out", "cu_q", "kv_len", "page_table")] + [
+        (n, C.c_uint32) for n in ("rows", "n_seq", "n_head", "n_kv", "head_dim", "n_pages", "page_size", "max_pages", "q_stride", "out_stride", "max_q",
+                                  "window")] + [("scale", C.c_float), ("path", C.c_uint32)]
+
+
 class Config(C.Structure):
     """`infr_cuda_config`: the context's tuning switches (the reference's typed kernel config,
     crates/infr-core/src/config/mod.rs:1-29)."""
@@ -185,6 +198,8 @@ def load_library(path: Optional[str] = None):
     L.infr_cuda_moe_ffn.argtypes = [vp, C.POINTER(_Desc)]
     L.infr_cuda_moe_route.argtypes = [vp, C.POINTER(_Desc)]
     L.infr_cuda_linear.argtypes = [vp, i32, vp, vp, vp, u32, u32, u32]
+    L.infr_cuda_rope_kv.argtypes = [vp, C.POINTER(_RopeKvDesc)]
+    L.infr_cuda_attention.argtypes = [vp, C.POINTER(_AttentionDesc)]
     L.infr_cuda_gated_act.argtypes = [vp, vp, vp, vp, sz]
     L.infr_cuda_moe_shared_add.argtypes = [vp, vp, vp, vp, vp, u32, u32]
     L.infr_cuda_rmsnorm.argtypes = [vp, vp, vp, vp, u32, u32, C.c_float]
@@ -339,6 +354,85 @@ class MoeFfn:
         d.fused_gate_up = int(bool(self.fused_gate_up))
         d._op = self  # the descriptor holds raw handle pointers: the op (and its Buffer objects) must outlive it
         return d
+
+
+def _fill(desc, op, names):
+    """The named fields of an op into its descriptor: handles for buffers, numbers as they are."""
+    for n in names:
+        x = getattr(op, n)
+        setattr(desc, n, x.handle if isinstance(x, Buffer) else x)
+    return desc
+
+
+@dataclass(frozen=True)
+class RopeKv:
+    """New q, k and v rows of a batch on their way to attention: per-head RmsNorm (where the weights are given), rotary embedding of q and k,
+    k and v into the f16 cache - pages where `page_table` is given, packed rows otherwise (`infr_cuda_rope_kv_desc` in
+    include/infr_cuda.h says what each field is).  Frozen: the descriptor is made once and serves every call."""
+    q: Buffer
+    k: Buffer
+    v: Buffer
+    q_out: Buffer
+    k_cache: Buffer
+    v_cache: Buffer
+    cu_q: Buffer
+    rows: int
+    n_seq: int
+    n_head: int
+    n_kv: int
+    head_dim: int
+    kv_len: Optional[Buffer] = None
+    page_table: Optional[Buffer] = None
+    n_pages: int = 0
+    page_size: int = 0
+    max_pages: int = 0
+    q_stride: int = 0
+    k_stride: int = 0
+    v_stride: int = 0
+    q_out_stride: int = 0
+    n_rot: int = 0
+    interleaved: bool = False
+    rope_base: float = 1e4
+    rope_scale: float = 1.0
+    freq_factors: Optional[Buffer] = None
+    q_norm: Optional[Buffer] = None
+    k_norm: Optional[Buffer] = None
+    norm_eps: float = 1e-6
+
+    def __post_init__(self):
+        d = _fill(_RopeKvDesc(), self, [n for n, _ in _RopeKvDesc._fields_ if n != "style"])
+        d.style = int(bool(self.interleaved))
+        object.__setattr__(self, "_desc", d)
+
+
+@dataclass(frozen=True)
+class Attention:
+    """Causal attention of a batch's new rows over its cache, or over packed f16 rows where `page_table` is not given
+    (`infr_cuda_attention_desc` in include/infr_cuda.h says what each field is).  Frozen: the descriptor is made once and serves every call."""
+    q: Buffer
+    k: Buffer
+    v: Buffer
+    out: Buffer
+    cu_q: Buffer
+    rows: int
+    n_seq: int
+    n_head: int
+    n_kv: int
+    head_dim: int
+    scale: float
+    kv_len: Optional[Buffer] = None
+    page_table: Optional[Buffer] = None
+    n_pages: int = 0
+    page_size: int = 0
+    max_pages: int = 0
+    q_stride: int = 0
+    out_stride: int = 0
+    max_q: int = 0  # longest sequence of new rows, as far as known: picks the kernel, not the results
+    window: int = 0
+    path: int = 0  # 0 auto, 1 few-rows kernel, 2 tensor-memory kernel
+
+    def __post_init__(self):
+        object.__setattr__(self, "_desc", _fill(_AttentionDesc(), self, [n for n, _ in _AttentionDesc._fields_]))
 
 
 class CudaBackend:
@@ -565,6 +659,12 @@ class CudaBackend:
 
     def linear(self, dtype: DType, w: Buffer, x: Buffer, y: Buffer, m: int, in_f: int, out_f: int) -> None:
         self._check(self._lib.infr_cuda_linear(self._ctx, int(dtype), w.handle, x.handle, y.handle, m, in_f, out_f))
+
+    def rope_kv(self, op: RopeKv) -> None:
+        self._check(self._lib.infr_cuda_rope_kv(self._ctx, op._desc))
+
+    def attention(self, op: Attention) -> None:
+        self._check(self._lib.infr_cuda_attention(self._ctx, op._desc))
 
     def gated_act(self, gate: Buffer, up: Buffer, dst: Buffer, n: int) -> None:
         self._check(self._lib.infr_cuda_gated_act(self._ctx, gate.handle, up.handle, dst.handle, n))

@@ -1,4 +1,5 @@
 // C ABI: context, buffers, descriptor validation and dispatch (see include/infr_cuda.h).
+#include <cmath>
 #include <cstdio>
 #include <chrono>
 #include <cstring>
@@ -7,6 +8,7 @@
 #include <new>
 #include <tuple>
 
+#include "attn.cuh"
 #include "formats.cuh"
 #include "kernels.cuh"
 
@@ -179,6 +181,9 @@ int32_t drain_and_poll(infr_cuda_ctx* ctx, const char* what) {
       std::snprintf(msg, sizeof msg, "a bounded device-side wait ran out (kernel tag %d); outputs of that call are invalid", tag);
       return fail(ctx, INFR_CUDA_ERR_TIMEOUT, msg);
     }
+    if (bad == 2)
+      return fail(ctx, INFR_CUDA_ERR_INVALID_ARG,
+                  "a page, a row or a length outside its range reached an attention kernel and was forced into it; outputs of that call are invalid");
     return fail(ctx, INFR_CUDA_ERR_INVALID_ARG,
                 "an expert id outside [0, n_expert) reached a kernel and was served as another expert; outputs of that call are invalid");
   }
@@ -212,7 +217,9 @@ int32_t infr_cuda_create(int32_t device, infr_cuda_ctx** out) {
       cudaHostAlloc(reinterpret_cast<void**>(&ctx->status_host), HOST_WORDS_BYTES, cudaHostAllocMapped) != cudaSuccess ||
       cudaHostGetDevicePointer(reinterpret_cast<void**>(&ctx->status), ctx->status_host, 0) != cudaSuccess ||
       cudaMalloc(&ctx->route_logits, ROUTE_LOGIT_BYTES) != cudaSuccess ||
-      cudaMemset(ctx->route_logits, 0xFF, ROUTE_LOGIT_BYTES) != cudaSuccess) {
+      cudaMemset(ctx->route_logits, 0xFF, ROUTE_LOGIT_BYTES) != cudaSuccess ||
+      cudaMalloc(&ctx->attn_count, ATTN_MAX_CTAS * sizeof(int)) != cudaSuccess ||
+      cudaMemset(ctx->attn_count, 0, ATTN_MAX_CTAS * sizeof(int)) != cudaSuccess) {
     infr_cuda_destroy(ctx);
     return INFR_CUDA_ERR_CUDA;
   }
@@ -238,6 +245,7 @@ void infr_cuda_destroy(infr_cuda_ctx* ctx) {
   if (ctx->scratch) cudaFree(ctx->scratch);
   if (ctx->status_host) cudaFreeHost(ctx->status_host);
   if (ctx->route_logits) cudaFree(ctx->route_logits);
+  if (ctx->attn_count) cudaFree(ctx->attn_count);
   if (ctx->own_stream) cudaStreamDestroy(ctx->own_stream);
   delete ctx;
 }
@@ -1030,6 +1038,162 @@ int32_t infr_cuda_add(infr_cuda_ctx* ctx, const infr_cuda_buf* a, const infr_cud
   if (!n) return INFR_CUDA_OK;
   DeviceGuard g(ctx->device);
   return launch_add(ctx, static_cast<const float*>(a->ptr), static_cast<const float*>(b->ptr), static_cast<float*>(dst->ptr), n);
+}
+
+// ---- the attention half of a layer ----------------------------------------------------------------
+
+}  // extern "C"
+
+namespace {
+
+template <class Desc>
+AttnSizes attn_sizes(const Desc* d) {
+  return {d->rows, d->n_seq, d->n_head, d->n_kv, d->head_dim, d->n_pages, d->page_size, d->max_pages, d->page_table != nullptr};
+}
+
+// Bytes of the cache that a call's rows or pages take.
+uint64_t attn_cache_bytes(const AttnSizes& s) {
+  return (s.paged ? (uint64_t)s.n_pages * s.page_size : (uint64_t)s.rows) * s.n_kv * s.head_dim * 2;
+}
+
+// What both calls check of a batch and its cache.
+template <class Desc>
+int32_t attn_check_batch(infr_cuda_ctx* ctx, const char* op, const Desc* d, const infr_cuda_buf* k, const infr_cuda_buf* v) {
+  const AttnSizes s = attn_sizes(d);
+  bool unsupported = false;
+  const std::string name = std::string(op) + ": ";
+  if (const char* why = attn_sizes_error(s, &unsupported)) return fail(ctx, unsupported ? INFR_CUDA_ERR_UNSUPPORTED : INFR_CUDA_ERR_INVALID_ARG, name + why);
+  if ((d->kv_len != nullptr) != s.paged) return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, name + "kv_len and page_table come together");
+  if (!fits(d->cu_q, ((size_t)d->n_seq + 1) * 4) || (s.paged && (!fits(d->kv_len, (size_t)d->n_seq * 4) || !fits(d->page_table, (size_t)d->n_seq * d->max_pages * 4))))
+    return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, name + "cu_q, kv_len or page_table missing or too small");
+  if (!fits(k, attn_cache_bytes(s)) || !fits(v, attn_cache_bytes(s))) return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, name + "cache buffer missing or too small");
+  return INFR_CUDA_OK;
+}
+
+// A matrix of rows: its stride (0 = rows side by side) and whether the buffer holds it.
+int32_t attn_check_rows(infr_cuda_ctx* ctx, const char* what, const infr_cuda_buf* b, uint32_t rows, uint32_t stride, uint32_t wide, long long* out) {
+  const uint32_t s = stride ? stride : wide;
+  if (s < wide || s % 4) return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, std::string(what) + ": a row stride is a multiple of 4 and at least a row");
+  if (!fits(b, attn_span(rows, s, wide) * 4)) return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, std::string(what) + ": buffer missing or too small");
+  *out = s;
+  return INFR_CUDA_OK;
+}
+
+bool overlap(const infr_cuda_buf* a, uint64_t na, const infr_cuda_buf* b, uint64_t nb) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a->ptr), y = reinterpret_cast<uintptr_t>(b->ptr);
+  return x < y + nb && y < x + na;
+}
+
+template <class Params, class Desc>
+void attn_batch_params(Params& p, infr_cuda_ctx* ctx, const Desc* d) {
+  const bool paged = d->page_table != nullptr;
+  p.cu_q = static_cast<const int*>(d->cu_q->ptr);
+  p.kv_len = paged ? static_cast<const int*>(d->kv_len->ptr) : nullptr;
+  p.page_table = paged ? static_cast<const int*>(d->page_table->ptr) : nullptr;
+  p.status = ctx->status;
+  // pages: [page][kv head][token][value]; packed rows: [row][kv head][value]
+  p.row_pitch = paged ? d->head_dim : (size_t)d->n_kv * d->head_dim;
+  p.head_pitch = paged ? (size_t)d->page_size * d->head_dim : d->head_dim;
+  p.page_pitch = paged ? (size_t)d->n_kv * d->page_size * d->head_dim : (size_t)d->rows * d->n_kv * d->head_dim;
+  p.rows = (int)d->rows;
+  p.n_seq = (int)d->n_seq;
+  p.n_kv = (int)d->n_kv;
+  p.hd = (int)d->head_dim;
+  p.page_size = (int)d->page_size;
+  p.max_pages = (int)d->max_pages;
+  p.n_pages = (int)d->n_pages;
+  p.cap = (int)(d->max_pages * d->page_size);
+}
+
+}  // namespace
+
+extern "C" {
+
+int32_t infr_cuda_rope_kv(infr_cuda_ctx* ctx, const infr_cuda_rope_kv_desc* d) {
+  if (!ctx) return INFR_CUDA_ERR_INVALID_ARG;
+  if (!d) return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "rope_kv: null descriptor");
+  int32_t rc = attn_check_batch(ctx, "rope_kv", d, d->k_cache, d->v_cache);
+  if (rc) return rc;
+  if (d->n_rot % 8 || d->n_rot > d->head_dim) return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "rope_kv: n_rot must be a multiple of 8, at most head_dim");
+  if (d->style > INFR_CUDA_ROPE_INTERLEAVED) return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "rope_kv: unknown style");
+  if (d->n_rot && !(d->rope_base > 0.f && std::isfinite(d->rope_base) && std::isfinite(d->rope_scale)))
+    return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "rope_kv: rope_base must be positive, rope_base and rope_scale finite");
+  if ((d->q_norm && !fits(d->q_norm, (size_t)d->head_dim * 4)) || (d->k_norm && !fits(d->k_norm, (size_t)d->head_dim * 4)))
+    return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "rope_kv: norm weight too small");
+  if ((d->q_norm || d->k_norm) && !(d->norm_eps >= 0.f && std::isfinite(d->norm_eps)))
+    return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "rope_kv: norm_eps must be finite and not negative");
+  if (d->freq_factors && !fits(d->freq_factors, (size_t)d->n_rot * 2)) return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "rope_kv: freq_factors too small");
+  RopeParams p = {};
+  const uint32_t wide_q = d->n_head * d->head_dim, wide_kv = d->n_kv * d->head_dim;
+  if ((rc = attn_check_rows(ctx, "rope_kv: q", d->q, d->rows, d->q_stride, wide_q, &p.q_stride)) ||
+      (rc = attn_check_rows(ctx, "rope_kv: k", d->k, d->rows, d->k_stride, wide_kv, &p.k_stride)) ||
+      (rc = attn_check_rows(ctx, "rope_kv: v", d->v, d->rows, d->v_stride, wide_kv, &p.v_stride)) ||
+      (rc = attn_check_rows(ctx, "rope_kv: q_out", d->q_out, d->rows, d->q_out_stride, wide_q, &p.qo_stride)))
+    return rc;
+  if (!d->rows) return INFR_CUDA_OK;
+  const uint64_t nq = attn_span(d->rows, p.qo_stride, wide_q) * 4, nc = attn_cache_bytes(attn_sizes(d));
+  const bool in_place = d->q_out->ptr == d->q->ptr && p.qo_stride == p.q_stride;
+  if (!in_place && (overlap(d->q_out, nq, d->q, attn_span(d->rows, p.q_stride, wide_q) * 4) || overlap(d->q_out, nq, d->k, attn_span(d->rows, p.k_stride, wide_kv) * 4) ||
+                    overlap(d->q_out, nq, d->v, attn_span(d->rows, p.v_stride, wide_kv) * 4)))
+    return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "rope_kv: q_out overlaps q, k or v without being q itself");
+  if (overlap(d->k_cache, nc, d->v_cache, nc) || overlap(d->k_cache, nc, d->q_out, nq) || overlap(d->v_cache, nc, d->q_out, nq))
+    return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "rope_kv: k_cache, v_cache and q_out must not overlap");
+  DeviceGuard g(ctx->device);
+  attn_batch_params(p, ctx, d);
+  p.q = static_cast<const float*>(d->q->ptr);
+  p.k = static_cast<const float*>(d->k->ptr);
+  p.v = static_cast<const float*>(d->v->ptr);
+  p.q_out = static_cast<float*>(d->q_out->ptr);
+  p.k_cache = static_cast<__half*>(d->k_cache->ptr);
+  p.v_cache = static_cast<__half*>(d->v_cache->ptr);
+  p.q_norm = d->q_norm ? static_cast<const float*>(d->q_norm->ptr) : nullptr;
+  p.k_norm = d->k_norm ? static_cast<const float*>(d->k_norm->ptr) : nullptr;
+  p.freq_factors = d->freq_factors ? static_cast<const float*>(d->freq_factors->ptr) : nullptr;
+  p.turns0 = (double)d->rope_scale / (2.0 * 3.14159265358979323846);
+  p.ratio = d->n_rot ? std::pow((double)d->rope_base, -2.0 / d->n_rot) : 1.0;
+  p.norm_eps = d->norm_eps;
+  p.n_head = (int)d->n_head;
+  p.n_rot = (int)d->n_rot;
+  p.interleaved = d->style == INFR_CUDA_ROPE_INTERLEAVED;
+  return launch_rope_kv(ctx, p);
+}
+
+int32_t infr_cuda_attention(infr_cuda_ctx* ctx, const infr_cuda_attention_desc* d) {
+  if (!ctx) return INFR_CUDA_ERR_INVALID_ARG;
+  if (!d) return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "attention: null descriptor");
+  int32_t rc = attn_check_batch(ctx, "attention", d, d->k, d->v);
+  if (rc) return rc;
+  if (!std::isfinite(d->scale)) return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "attention: scale must be finite");
+  if (d->path > 2) return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "attention: unknown path");
+  if (d->window > 0x7FFFFFFFu) return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "attention: window is past 31 bits");
+  const uint32_t g = d->n_head / d->n_kv, wide = d->n_head * d->head_dim;
+  if (d->path == 1 && g > (uint32_t)ATTN_ROWS_LIMIT) return fail(ctx, INFR_CUDA_ERR_UNSUPPORTED, "attention: path 1 takes up to 16 query heads to a kv head");
+  AttnParams p = {};
+  if ((rc = attn_check_rows(ctx, "attention: q", d->q, d->rows, d->q_stride, wide, &p.q_stride)) ||
+      (rc = attn_check_rows(ctx, "attention: out", d->out, d->rows, d->out_stride, wide, &p.out_stride)))
+    return rc;
+  if (!d->rows) return INFR_CUDA_OK;
+  const uint64_t no = attn_span(d->rows, p.out_stride, wide) * 4, nc = attn_cache_bytes(attn_sizes(d));
+  if (overlap(d->out, no, d->q, attn_span(d->rows, p.q_stride, wide) * 4) || overlap(d->out, no, d->k, nc) || overlap(d->out, no, d->v, nc))
+    return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "attention: out must not overlap q, k or v");
+  DeviceGuard guard(ctx->device);
+  attn_batch_params(p, ctx, d);
+  p.q = static_cast<const float*>(d->q->ptr);
+  p.out = static_cast<float*>(d->out->ptr);
+  p.v = static_cast<const __half*>(d->v->ptr);
+  p.g = (int)g;
+  p.window = (int)d->window;
+  p.scale_log2 = (float)((double)d->scale * 1.4426950408889634);
+  p.count = ctx->attn_count;
+  const uint64_t max_rows = (uint64_t)(d->max_q && d->max_q < d->rows ? d->max_q : d->rows) * g;
+  const bool few = d->path ? d->path == 1 : max_rows <= (uint64_t)ATTN_ROWS_LIMIT;
+  const size_t item_rows = few ? ATTN_ROWS_LIMIT : ATTN_TILE_ROWS, slots = 2 * (size_t)ctx->sm_count;
+  const size_t part = align_up(slots * item_rows * 256 * 4, 256);
+  if ((rc = ensure_scratch(ctx, part + slots * item_rows * 8))) return rc;
+  p.part = static_cast<float*>(ctx->scratch);
+  p.part_ml = reinterpret_cast<float2*>(static_cast<char*>(ctx->scratch) + part);
+  const __half* k = static_cast<const __half*>(d->k->ptr);
+  return few ? launch_attn_rows(ctx, p, k, (int)(max_rows < 1024 ? max_rows : 1024)) : launch_attn_tiles(ctx, p, k);
 }
 
 int32_t infr_cuda_moe_expert_rows(infr_cuda_ctx* ctx, const infr_cuda_buf* x_rows, const infr_cuda_buf* seg_off,

@@ -1,0 +1,252 @@
+// What the two attention kernels share: parameters, the line of units and a CTA's walk along it, joining of partial results.
+#pragma once
+#include <math_constants.h>
+
+#include "attn_shape.h"
+#include "kernels.cuh"
+#include "tma.cuh"
+
+namespace infr {
+
+struct AttnParams {
+  const float* q;
+  float* out;
+  const int *cu_q, *kv_len, *page_table;  // kv_len, page_table: null where the keys are packed rows
+  const __half* v;                        // for what the tiles' products leave out (values that are not finite)
+  size_t page_pitch, head_pitch, row_pitch;  // of the cache, in values
+  long long q_stride, out_stride;
+  float* part;      // [2 CTAs][rows of an item][HD] sums, not yet divided
+  float2* part_ml;  // [2 CTAs][rows of an item] reference and weight
+  int* count;       // [CTAs] partial results in, per item by its first CTA; zero between launches
+  DeviceStatus* status;
+  float scale_log2;  // scale * log2(e)
+  int rows, n_seq, n_kv, g, hd, page_size, max_pages, n_pages, window;
+  int tb;            // tokens of an item
+  int cap;           // max_pages * page_size
+};
+
+// Weights are 2^(x - reference + ATTN_BIAS): the reference follows the running maximum only when that has grown by ATTN_SLACK, so
+// they stay below 2^15 and fit f16; a weight of 2^-32 of the largest still has a bit in f16's subnormals.
+constexpr float ATTN_BIAS = 7.f, ATTN_SLACK = 8.f;
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// 2^(a - b) where a <= b, either possibly "no key yet" (-inf).
+__device__ __forceinline__ float exp2_rel(float a, float b) { return a == -CUDART_INF_F ? 0.f : exp2_approx(a - b); }
+
+__device__ __forceinline__ void tma_load_4d(void* smem_dst, const CUtensorMap* tm, int x, int y, int z, int w, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(
+          smem_u32(smem_dst)),
+      "l"(reinterpret_cast<uint64_t>(tm)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
+}
+
+__device__ __forceinline__ AttnSeq attn_load_seq(const AttnParams& p, int s) {
+  bool bad = false;
+  const AttnSeq r = attn_seq(__ldcg(p.cu_q + s), __ldcg(p.cu_q + s + 1), p.kv_len != nullptr ? __ldcg(p.kv_len + s) : 0, p.kv_len == nullptr, p.rows, p.cap, &bad);
+  if (bad) p.status->bad_index = 2;
+  return r;
+}
+
+__device__ __forceinline__ int attn_page(const AttnParams& p, int s, int page) {
+  const int id = __ldcg(p.page_table + (size_t)s * p.max_pages + page);
+  if ((unsigned)id < (unsigned)p.n_pages) return id;
+  p.status->bad_index = 2;  // read as page 0, reported at the next sync
+  return 0;
+}
+
+// Where the values of a key and head begin; the keys behind it follow row_pitch apart up to its page's end.
+__device__ __forceinline__ const __half* attn_value(const AttnParams& p, int s, int q0, int head, int key) {
+  const size_t at = p.page_table == nullptr ? (size_t)(q0 + key) * p.row_pitch
+                                            : (size_t)attn_page(p, s, key / p.page_size) * p.page_pitch + (size_t)(key % p.page_size) * p.row_pitch;
+  return p.v + at + (size_t)head * p.head_pitch;
+}
+
+// The first unit's place of a CTA, and the line's length.
+struct AttnStart {
+  long long units, u0, u1, ub;  // ub: first unit of the block's first head
+  int s, b, ctas;               // ctas: those with units
+};
+
+// Inclusive sum over the block's threads; s_warp: one word per warp.
+template <int THREADS>
+__device__ __forceinline__ long long block_scan(long long v, long long* s_warp) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long t = __shfl_up_sync(0xFFFFFFFFu, v, o);
+    if (lane >= o) v += t;
+  }
+  __syncthreads();
+  if (lane == 31) s_warp[warp] = v;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w)
+    if (w < warp) v += s_warp[w];
+  return v;
+}
+
+// Every CTA works the whole line out for itself (a sequence and a few blocks per thread), which costs less than a launch for it.
+// pre: n_seq + 1 words of shared memory, free again after the call.  All threads take part.
+template <int THREADS, int LOG2_TILE>
+__device__ void attn_plan(const AttnParams& p, int* pre, long long* s_warp, AttnStart* st) {
+  const int tid = threadIdx.x;
+  long long carry = 0;
+  for (int s0 = 0; s0 < p.n_seq; s0 += THREADS) {
+    const int s = s0 + tid;
+    const int n = s < p.n_seq ? attn_blocks(attn_load_seq(p, s).q_len, p.tb) : 0;
+    const long long sum = carry + block_scan<THREADS>(n, s_warp);
+    if (s < p.n_seq) pre[s + 1] = (int)sum;
+    if (s0 == 0 && tid == 0) pre[0] = 0;
+    if (s0 + THREADS < p.n_seq) {
+      __syncthreads();
+      carry = pre[s0 + THREADS];
+    }
+  }
+  __syncthreads();
+  const int F = pre[p.n_seq];
+  const int f0 = (int)((long long)tid * F / THREADS), f1 = (int)((long long)(tid + 1) * F / THREADS);
+  int s = 0;
+  for (int hi = p.n_seq; hi - s > 1;) {  // the last sequence that begins at or before block f0
+    const int mid = (s + hi) / 2;
+    if (pre[mid] <= f0) s = mid;
+    else hi = mid;
+  }
+  long long mine = 0;
+  if (f0 < f1) {
+    int at = s;
+    AttnSeq q = attn_load_seq(p, at);
+    for (int f = f0; f < f1; ++f) {
+      while (f >= pre[at + 1]) q = attn_load_seq(p, ++at);
+      mine += attn_block(q, f - pre[at], p.tb, LOG2_TILE, p.window).ntile;
+    }
+  }
+  const long long end = block_scan<THREADS>(mine, s_warp);
+  if (tid == THREADS - 1) {
+    st->units = end * p.n_kv;
+    st->ctas = (int)(st->units < (long long)gridDim.x ? st->units : (long long)gridDim.x);
+    const bool idle = (int)blockIdx.x >= st->ctas;
+    st->u0 = idle ? 0 : attn_begin(blockIdx.x, st->units, st->ctas);
+    st->u1 = idle ? 0 : attn_begin(blockIdx.x + 1, st->units, st->ctas);
+  }
+  __syncthreads();
+  long long ub = (end - mine) * p.n_kv;
+  const long long u0 = st->u0;
+  if (mine > 0 && u0 >= ub && u0 < end * p.n_kv) {
+    int at = s;
+    AttnSeq q = attn_load_seq(p, at);
+    for (int f = f0; f < f1; ++f) {
+      while (f >= pre[at + 1]) q = attn_load_seq(p, ++at);
+      const long long n = (long long)attn_block(q, f - pre[at], p.tb, LOG2_TILE, p.window).ntile * p.n_kv;
+      if (u0 < ub + n) {
+        st->s = at;
+        st->b = f - pre[at];
+        st->ub = ub;
+        break;
+      }
+      ub += n;
+    }
+  }
+  __syncthreads();
+}
+
+// One item after the other from a CTA's first.
+template <int LOG2_TILE>
+struct AttnCursor {
+  AttnSeq seq;
+  AttnBlock blk;
+  long long ub;  // the item's first unit
+  int s, b, head;
+
+  __device__ __forceinline__ void start(const AttnParams& p, const AttnStart& st) {
+    s = st.s, b = st.b;
+    seq = attn_load_seq(p, s);
+    blk = attn_block(seq, b, p.tb, LOG2_TILE, p.window);
+    head = (int)((st.u0 - st.ub) / blk.ntile);
+    ub = st.ub + (long long)head * blk.ntile;
+  }
+  __device__ __forceinline__ void next(const AttnParams& p) {
+    ub += blk.ntile;
+    if (++head < p.n_kv) return;
+    head = 0;
+    ++b;
+    while (b >= attn_blocks(seq.q_len, p.tb)) {
+      if (s + 1 >= p.n_seq) return;  // past the line's end: nobody asks for more
+      seq = attn_load_seq(p, ++s);
+      b = 0;
+    }
+    blk = attn_block(seq, b, p.tb, LOG2_TILE, p.window);
+  }
+};
+
+// Whose partial results an item has: those of the CTAs first .. last, the first one's in its second slot, the others' in their first.
+struct AttnShare {
+  int first, last;
+};
+__device__ __forceinline__ AttnShare attn_share(long long ub, int ntile, const AttnStart& st) {
+  return {attn_cta_of(ub, st.units, st.ctas), attn_cta_of(ub + ntile - 1, st.units, st.ctas)};
+}
+__device__ __forceinline__ int attn_slot(int cta, const AttnShare& sh) { return 2 * cta + (cta == sh.first ? 1 : 0); }
+
+// After all threads have written their CTA's part: whether this CTA is the item's last and joins it.  Counting is by atomics, the join
+// itself is in the order of the CTAs: the sums do not depend on who came last.
+__device__ __forceinline__ bool attn_arrive(const AttnParams& p, const AttnShare& sh, int* s_last, int threads_bar, int threads) {
+  __threadfence();
+  asm volatile("bar.sync %0, %1;" ::"r"(threads_bar), "r"(threads) : "memory");
+  if (threadIdx.x == 0) {
+    const int n = atomicAdd(p.count + sh.first, 1);
+    *s_last = n == sh.last - sh.first;
+    if (n == sh.last - sh.first) p.count[sh.first] = 0;
+    __threadfence();
+  }
+  asm volatile("bar.sync %0, %1;" ::"r"(threads_bar), "r"(threads) : "memory");
+  return *s_last != 0;
+}
+
+// Four values of row r of the joined item, divided by its weight (zero where no row was seen).
+template <int HD>
+__device__ __forceinline__ float4 attn_join4(const AttnParams& p, const AttnShare& sh, int item_rows, int r, int i) {
+  float M = -CUDART_INF_F;
+  for (int c = sh.first; c <= sh.last; ++c) M = fmaxf(M, __ldcg(&p.part_ml[(size_t)attn_slot(c, sh) * item_rows + r]).x);
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  float L = 0.f;
+#pragma unroll 4
+  for (int c = sh.first; c <= sh.last; ++c) {
+    const size_t at = (size_t)attn_slot(c, sh) * item_rows + r;
+    const float2 ml = __ldcg(&p.part_ml[at]);
+    const float4 v = __ldcg(reinterpret_cast<const float4*>(p.part + at * HD + i));
+    const float w = exp2_rel(ml.x, M);
+    if (w != 0.f) {  // (a part that saw nothing holds nothing)
+      L += w * ml.y;
+      o.x += w * v.x, o.y += w * v.y, o.z += w * v.z, o.w += w * v.w;
+    }
+  }
+  const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);  // NaN stays
+  return make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+}
+
+// Maps of a cache for boxes of 64 values x box_rows keys of one head: dimensions (values, keys of a page or packed rows, kv heads, pages).
+bool attn_cache_map(CUtensorMap* tm, const __half* base, const AttnParams& p, int box_rows);
+
+struct RopeParams {
+  const float *q, *k, *v, *q_norm, *k_norm, *freq_factors;
+  float* q_out;
+  __half *k_cache, *v_cache;
+  const int *cu_q, *kv_len, *page_table;
+  DeviceStatus* status;
+  size_t page_pitch, head_pitch, row_pitch;
+  long long q_stride, k_stride, v_stride, qo_stride;
+  double turns0, ratio;  // turns per token of pair 0, and of each pair relative to the one before
+  float norm_eps;
+  int rows, n_seq, n_head, n_kv, hd, page_size, max_pages, n_pages, cap, n_rot, interleaved;
+};
+int32_t launch_rope_kv(infr_cuda_ctx* ctx, const RopeParams& p);
+
+int32_t launch_attn_rows(infr_cuda_ctx* ctx, AttnParams p, const __half* k, int max_rows);
+int32_t launch_attn_tiles(infr_cuda_ctx* ctx, AttnParams p, const __half* k);
+
+}  // namespace infr

@@ -1,0 +1,442 @@
+// Attention of a few rows per (sequence, kv head): single tokens and speculative windows, up to 16 rows (tokens x query heads of a kv head)
+// to an item.  One pass over the keys: what bounds it is reading K and V once.
+//
+// A CTA takes key tiles of 16 keys per warp; each warp streams its own 16-key slices of K and V through a ring of its own (tiled copies, no
+// barrier between warps) and keeps its own running maximum, weight and sums, joined at the item's end.  Both products are transposed so that
+// the tensor cores' 16 rows are keys or head values, and the 8 columns the rows of the item:
+//   S^T[16 keys, 8 rows] = K[16, hd] q^T[hd, 8],    O^T[hd, 8 rows] += V^T[hd, 16 keys] P^T[16 keys, 8 rows]
+// The scores' fragments become P^T's through a transposition of 8 x 8 matrices in registers.  q and P go in as two f16 pieces each (22 bits;
+// q scaled by a power of two per row so that f16's range holds it): f32 results stay f32 results.
+#include "attn.cuh"
+
+namespace infr {
+namespace {
+
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t movm(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+// a and b as f16 pairs: the rounded values, and what the rounding left.
+__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
+  const __half2 h = __floats2half2_rn(a, b);
+  const float2 f = __half22float2(h);
+  const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
+  hi = *reinterpret_cast<const uint32_t*>(&h);
+  lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+
+template <int HD, int NT>
+struct RowsShape {
+  static constexpr int WARPS = HD > 128 ? 4 : 8, THREADS = WARPS * 32, RB = 8 * NT;
+  static constexpr int LOG2_TILE = HD > 128 ? 6 : 7;  // 16 keys a warp
+  static constexpr int SLICE = 2 * 16 * HD * 2;       // bytes of 16 keys of K and V
+  static constexpr int PITCH = HD + 4;                // words: the fragments' columns fall on different banks
+  static constexpr int MERGE = WARPS * RB * PITCH * 4, STATS = 2 * WARPS * RB * 4;
+  static constexpr int FIT = (232448 - 1024 - 1024 - MERGE - STATS) / (WARPS * SLICE);
+  static constexpr int STAGES = FIT > 6 ? 6 : FIT;
+  static constexpr int SMEM = 1024 + WARPS * STAGES * SLICE + MERGE + STATS + WARPS * STAGES * 8;
+};
+
+template <int HD, int NT>
+__global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
+    k_attn_rows(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const AttnParams p) {
+  using Sh = RowsShape<HD, NT>;
+  constexpr int WARPS = Sh::WARPS, THREADS = Sh::THREADS, RB = Sh::RB, STAGES = Sh::STAGES, SLICE = Sh::SLICE, PITCH = Sh::PITCH;
+  constexpr int SLABS = HD / 64, KST = HD / 16;
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ long long s_scan[WARPS];
+  __shared__ AttnStart s_start;
+  __shared__ int s_last;
+  unsigned char* ring_all = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  float* s_o = reinterpret_cast<float*>(ring_all + WARPS * STAGES * SLICE);
+  float* s_m = s_o + WARPS * RB * PITCH;
+  float* s_l = s_m + WARPS * RB;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(s_l + WARPS * RB);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  unsigned char* ring = ring_all + warp * STAGES * SLICE;
+  uint64_t* full = bars + warp * STAGES;
+
+  if (lane == 0)
+    for (int i = 0; i < STAGES; ++i) mbar_init(full + i, 1);
+  mbar_fence_init();
+  pdl_wait();
+  attn_plan<THREADS, Sh::LOG2_TILE>(p, reinterpret_cast<int*>(ring_all), s_scan, &s_start);
+  const AttnStart st = s_start;
+  if (st.u0 >= st.u1) return;
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the plan's words lay where the copies go
+  __syncthreads();
+
+  const bool packed = p.page_table == nullptr;
+  // ---- what the warp asks for: its slices of the CTA's tiles, one after the other, STAGES of them ahead of their use
+  AttnCursor<Sh::LOG2_TILE> ahead;
+  ahead.start(p, st);
+  long long au = st.u0;                 // unit of the next slice to ask for
+  int a_key = -1, a_page = 0;           // its first key (-1: none left) and its page
+  uint32_t asked = 0;
+  auto find = [&]() {                   // the next unit of which this warp has keys, from au on
+    while (au < st.u1) {
+      if (au >= ahead.ub + ahead.blk.ntile) {
+        ahead.next(p);
+        continue;
+      }
+      const int ks = ((ahead.blk.tile0 + (int)(au - ahead.ub)) << Sh::LOG2_TILE) + warp * 16;
+      if (ks < ahead.blk.hi && ks + 16 > ahead.blk.lo) {
+        a_key = ks;
+        if (!packed) a_page = attn_page(p, ahead.s, ks / p.page_size);
+        return;
+      }
+      ++au;
+    }
+    a_key = -1;
+  };
+  auto ask = [&]() {
+    if (a_key < 0) return;
+    if (lane == 0) {
+      const int stage = asked % STAGES;
+      unsigned char* dst = ring + stage * SLICE;
+      mbar_arrive_expect_tx(full + stage, SLICE);
+      const int y = packed ? ahead.seq.q0 + a_key : a_key % p.page_size, w = packed ? 0 : a_page;
+#pragma unroll
+      for (int s = 0; s < SLABS; ++s) {
+        tma_load_4d(dst + s * 2048, &kmap, 64 * s, y, ahead.head, w, full + stage);
+        tma_load_4d(dst + SLICE / 2 + s * 2048, &vmap, 64 * s, y, ahead.head, w, full + stage);
+      }
+    }
+    ++asked;
+    ++au;
+    find();
+  };
+  find();
+  for (int i = 0; i < STAGES; ++i) ask();
+
+  AttnCursor<Sh::LOG2_TILE> cur;
+  cur.start(p, st);
+  uint32_t used = 0;
+  bool alive = true;
+  const int c0 = 2 * (lane & 3);  // this thread's columns (rows of the item): c0, c0 + 1 of every eight
+  for (long long u = st.u0; u < st.u1;) {
+    if (u >= cur.ub + cur.blk.ntile) cur.next(p);
+    const AttnBlock& blk = cur.blk;
+    const int first_tile = (int)(u - cur.ub), n_rows = blk.nt * p.g;
+    const int end_tile = (int)(st.u1 - cur.ub < blk.ntile ? st.u1 - cur.ub : blk.ntile);
+
+    // ---- q: B fragments of q^T, rows scaled by a power of two, as two f16 pieces
+    uint32_t qh[NT][KST][2], ql[NT][KST][2];
+    float f[NT][2];  // of the thread's columns: score -> log2 units
+    int lim[NT][2];  // and the last key their row sees
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int r = 8 * n + (lane >> 2);
+      const bool has = r < n_rows;
+      const float* src = p.q + (size_t)(cur.seq.q0 + blk.t0 + (has ? r / p.g : 0)) * p.q_stride + (size_t)(cur.head * p.g + (has ? r % p.g : 0)) * p.hd;
+      float2 v[KST][2];
+      float big = 0.f;
+#pragma unroll
+      for (int k = 0; k < KST; ++k)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int i = 16 * k + 8 * j + c0;
+          v[k][j] = has && i < p.hd ? __ldcg(reinterpret_cast<const float2*>(src + i)) : make_float2(0.f, 0.f);
+          big = fmaxf(big, fmaxf(fabsf(v[k][j].x), fabsf(v[k][j].y)));
+        }
+      big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 1));
+      big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 2));
+      // the largest value to [2^7, 2^8); exponents kept where 2^-e and 2^e are both normal
+      int e = (int)((__float_as_uint(big) >> 23) & 255u) - 134;
+      e = big > 0.f && big < CUDART_INF_F ? max(-126, e) : 0;
+      const float down = __uint_as_float((uint32_t)(127 - e) << 23), up = __uint_as_float((uint32_t)(127 + e) << 23);
+#pragma unroll
+      for (int k = 0; k < KST; ++k)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) split2(v[k][j].x * down, v[k][j].y * down, qh[n][k][j], ql[n][k][j]);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        f[n][j] = __shfl_sync(0xFFFFFFFFu, up, (c0 + j) * 4) * p.scale_log2;
+        const int rr = 8 * n + c0 + j;
+        lim[n][j] = cur.seq.past + blk.t0 + (rr < n_rows ? rr / p.g : blk.nt - 1);
+      }
+    }
+    const int full_hi = cur.seq.past + blk.t0 + 1;  // keys below are seen by every row, but for the window's
+    const int full_lo = p.window > 0 ? cur.seq.past + blk.t0 + blk.nt - p.window : 0;
+
+    float o[KST][NT][4], m[NT][2], l[NT][2];
+#pragma unroll
+    for (int k = 0; k < KST; ++k)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[k][n][i] = 0.f;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) m[n][0] = m[n][1] = -CUDART_INF_F, l[n][0] = l[n][1] = 0.f;
+
+    bool odd = false;  // values that are not finite were left out
+    for (int t = first_tile; t < end_tile; ++t) {
+      const int ks = ((blk.tile0 + t) << Sh::LOG2_TILE) + warp * 16;
+      if (ks >= blk.hi || ks + 16 <= blk.lo) continue;
+      const int stage = used % STAGES;
+      if (alive) {
+        alive = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(full + stage, (used / STAGES) & 1));
+        if (!alive && lane == 0) atomicExch(&p.status->timeout, 10);
+      }
+      if (alive) {
+        const uint32_t kb = smem_u32(ring + stage * SLICE), vb = kb + SLICE / 2;
+        const int i4 = lane >> 3, r8 = lane & 7;
+        // ---- scores
+        float s[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+        for (int k = 0; k < KST; ++k) {
+          uint32_t a[4];
+          ldsm4(a, kb + (k >> 2) * 2048 + ((i4 & 1) * 8 + r8) * 128 + (((2 * (k & 3) + (i4 >> 1)) ^ r8) << 4));
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            mma16816(s[n], a, qh[n][k][0], qh[n][k][1]);
+            mma16816(s[n], a, ql[n][k][0], ql[n][k][1]);
+          }
+        }
+        const bool masked = ks + 16 > full_hi || ks < full_lo;
+        const int key = ks + (lane >> 2);
+        float mx[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            s[n][j] *= f[n][j];
+            s[n][2 + j] *= f[n][j];
+            if (masked) {
+              const int to = lim[n][j], from = p.window > 0 ? to - p.window : -1;
+              if (key > to || key <= from) s[n][j] = -CUDART_INF_F;
+              if (key + 8 > to || key + 8 <= from) s[n][2 + j] = -CUDART_INF_F;
+            }
+            mx[n][j] = fmaxf(s[n][j], s[n][2 + j]);
+          }
+        bool grows = false;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) mx[n][j] = fmaxf(mx[n][j], __shfl_xor_sync(0xFFFFFFFFu, mx[n][j], x));
+            grows |= mx[n][j] > m[n][j] + ATTN_SLACK;
+          }
+        if (__any_sync(0xFFFFFFFFu, grows)) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const float to = mx[n][j] > m[n][j] + ATTN_SLACK ? mx[n][j] : m[n][j];
+              const float w = to == m[n][j] ? 1.f : exp2_rel(m[n][j], to);
+              m[n][j] = to;
+              l[n][j] *= w;
+#pragma unroll
+              for (int k = 0; k < KST; ++k) o[k][n][j] *= w, o[k][n][2 + j] *= w;
+            }
+        }
+        // ---- weights, transposed into B fragments
+        uint32_t ph[NT][2], pl[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float e[4];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float off = ATTN_BIAS - (m[n][j] == -CUDART_INF_F ? 0.f : m[n][j]);
+            e[j] = exp2_approx(s[n][j] + off);
+            e[2 + j] = exp2_approx(s[n][2 + j] + off);
+            l[n][j] += e[j] + e[2 + j];
+          }
+          split2(e[0], e[1], ph[n][0], pl[n][0]);
+          split2(e[2], e[3], ph[n][1], pl[n][1]);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) ph[n][i] = movm(ph[n][i]), pl[n][i] = movm(pl[n][i]);
+        }
+        // ---- sums.  Where some row does not see some key, 0 x value must be 0 whatever the value: keys that no row sees count as
+        // zeros, and values that are not finite wait for the item's end.
+        const int vk = ks + c0;  // this thread's keys of V^T: vk, vk + 1 and eight further on
+#pragma unroll
+        for (int k = 0; k < KST; ++k) {
+          uint32_t a[4];
+          ldsm4_t(a, vb + (k >> 2) * 2048 + ((i4 >> 1) * 8 + r8) * 128 + (((2 * (k & 3) + (i4 & 1)) ^ r8) << 4));
+          if (masked) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int kk = vk + 8 * (i >> 1);
+              if (kk >= blk.hi || kk < blk.lo) a[i] &= 0xFFFF0000u;
+              if (kk + 1 >= blk.hi || kk + 1 < blk.lo) a[i] &= 0x0000FFFFu;
+              if ((a[i] & 0x7C00u) == 0x7C00u) a[i] &= 0xFFFF0000u, odd = true;
+              if ((a[i] & 0x7C000000u) == 0x7C000000u) a[i] &= 0x0000FFFFu, odd = true;
+            }
+          }
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            mma16816(o[k][n], a, ph[n][0], ph[n][1]);
+            mma16816(o[k][n], a, pl[n][0], pl[n][1]);
+          }
+        }
+        __syncwarp();
+        ++used;
+        ask();
+      }
+    }
+
+    // ---- values that are not finite: a product of pieces makes NaN of them (inf times a piece of the other sign, or of zero), so what the
+    // rows that see them get is put together by itself.  Ordinary calls only look.
+#pragma unroll
+    for (int k = 0; k < KST; ++k)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) odd |= !(fabsf(o[k][n][i]) < CUDART_INF_F);
+    if (__any_sync(0xFFFFFFFFu, odd)) {
+#pragma unroll
+      for (int k = 0; k < KST; ++k)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const int i = 16 * k + 8 * half + (lane >> 2);
+          float add[NT][2] = {};
+          bool has[NT][2] = {};
+          for (int t = first_tile; t < end_tile && i < p.hd; ++t) {
+            const int ks = ((blk.tile0 + t) << Sh::LOG2_TILE) + warp * 16;
+            if (ks >= blk.hi || ks + 16 <= blk.lo) continue;
+            const __half* at = attn_value(p, cur.s, cur.seq.q0, cur.head, ks) + i;
+            for (int key = max(ks, blk.lo); key < min(ks + 16, blk.hi); ++key) {
+              const float x = __half2float(at[(size_t)(key - ks) * p.row_pitch]);
+              if (fabsf(x) < CUDART_INF_F) continue;
+#pragma unroll
+              for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+                  if (key <= lim[n][j] && (p.window == 0 || key > lim[n][j] - p.window)) add[n][j] += x, has[n][j] = true;
+            }
+          }
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+              if (has[n][j]) o[k][n][2 * half + j] = add[n][j];
+        }
+    }
+
+    // ---- the warps' parts of the item
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) l[n][j] += __shfl_xor_sync(0xFFFFFFFFu, l[n][j], x);
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        if (m[n][j] == -CUDART_INF_F && l[n][j] != 0.f) m[n][j] = 0.f;  // nothing but NaN: a part that counts, not one without keys
+    __syncthreads();  // the last item's parts have been read
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int r = 8 * n + c0 + j;
+        if (lane < 4) s_m[warp * RB + r] = m[n][j], s_l[warp * RB + r] = l[n][j];
+#pragma unroll
+        for (int k = 0; k < KST; ++k) {
+          float* at = s_o + (warp * RB + r) * PITCH + 16 * k + (lane >> 2);
+          at[0] = o[k][n][j];
+          at[8] = o[k][n][2 + j];
+        }
+      }
+    }
+    __syncthreads();
+    const bool whole = first_tile == 0 && end_tile == blk.ntile;
+    const AttnShare share = attn_share(cur.ub, blk.ntile, st);
+    auto store = [&](int r, int i, float4 v) {
+      float* dst = p.out + (size_t)(cur.seq.q0 + blk.t0 + r / p.g) * p.out_stride + (size_t)(cur.head * p.g + r % p.g) * p.hd + i;
+      *reinterpret_cast<float4*>(dst) = v;
+    };
+    for (int e = tid; e < RB * (HD / 4); e += THREADS) {
+      const int r = e / (HD / 4), i = 4 * (e % (HD / 4));
+      if (r >= n_rows) continue;
+      float M = -CUDART_INF_F, L = 0.f;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) M = fmaxf(M, s_m[w * RB + r]);
+      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) {
+        const float wt = exp2_rel(s_m[w * RB + r], M);
+        const float4 v = *reinterpret_cast<const float4*>(s_o + (w * RB + r) * PITCH + i);
+        if (wt != 0.f) {
+          L += wt * s_l[w * RB + r];
+          sum.x += wt * v.x, sum.y += wt * v.y, sum.z += wt * v.z, sum.w += wt * v.w;
+        }
+      }
+      if (whole) {
+        const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
+        if (i < p.hd) store(r, i, make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv));
+      } else {
+        const size_t at = (size_t)attn_slot(blockIdx.x, share) * RB + r;
+        __stcg(reinterpret_cast<float4*>(p.part + at * HD + i), sum);
+        if (i == 0) __stcg(p.part_ml + at, make_float2(M, L));
+      }
+    }
+    if (!whole && attn_arrive(p, share, &s_last, 0, THREADS)) {
+      for (int e = tid; e < RB * (HD / 4); e += THREADS) {
+        const int r = e / (HD / 4), i = 4 * (e % (HD / 4));
+        if (r < n_rows && i < p.hd) store(r, i, attn_join4<HD>(p, share, RB, r, i));
+      }
+    }
+    u = cur.ub + end_tile;
+  }
+  // a warp that gave up has copies in flight: they land before its shared memory is somebody else's
+  if (!alive)
+    for (; used < asked; ++used) mbar_wait_bounded(full + used % STAGES, (used / STAGES) & 1);
+}
+
+template <int HD, int NT>
+cudaError_t run_rows(infr_cuda_ctx* ctx, const CUtensorMap& km, const CUtensorMap& vm, const AttnParams& p) {
+  using Sh = RowsShape<HD, NT>;
+  const cudaError_t e = ensure_smem(reinterpret_cast<const void*>(&k_attn_rows<HD, NT>), Sh::SMEM);
+  if (e != cudaSuccess) return e;
+  return launch_ex(k_attn_rows<HD, NT>, dim3(ctx->sm_count), dim3(Sh::THREADS), Sh::SMEM, ctx->stream, true, km, vm, p);
+}
+
+}  // namespace
+
+bool attn_cache_map(CUtensorMap* tm, const __half* base, const AttnParams& p, int box_rows) {
+  EncodeTiledFn enc = encode_tiled_fn();
+  if (!enc) return false;
+  const bool packed = p.page_table == nullptr;
+  const cuuint64_t dims[4] = {(cuuint64_t)p.hd, (cuuint64_t)(packed ? p.rows : p.page_size), (cuuint64_t)p.n_kv, (cuuint64_t)(packed ? 1 : p.n_pages)};
+  const cuuint64_t strides[3] = {p.row_pitch * 2, p.head_pitch * 2, p.page_pitch * 2};
+  const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1}, estr[4] = {1, 1, 1, 1};
+  return enc(tm, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<__half*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// max_rows: rows (tokens x heads of a kv head) that a sequence's new tokens make at most, as far as the caller knows; longer ones are
+// cut into more items.
+int32_t launch_attn_rows(infr_cuda_ctx* ctx, AttnParams p, const __half* k, int max_rows) {
+  CUtensorMap km, vm;
+  if (!attn_cache_map(&km, k, p, 16) || !attn_cache_map(&vm, p.v, p, 16)) return fail(ctx, INFR_CUDA_ERR_CUDA, "attention: cuTensorMapEncodeTiled failed");
+  const int nt = p.g <= 8 && max_rows <= 8 ? 1 : 2;
+  p.tb = 8 * nt / p.g;
+  cudaError_t e;
+  if (p.hd <= 64) e = nt == 1 ? run_rows<64, 1>(ctx, km, vm, p) : run_rows<64, 2>(ctx, km, vm, p);
+  else if (p.hd <= 128) e = nt == 1 ? run_rows<128, 1>(ctx, km, vm, p) : run_rows<128, 2>(ctx, km, vm, p);
+  else if (p.hd <= 192) e = nt == 1 ? run_rows<192, 1>(ctx, km, vm, p) : run_rows<192, 2>(ctx, km, vm, p);
+  else e = nt == 1 ? run_rows<256, 1>(ctx, km, vm, p) : run_rows<256, 2>(ctx, km, vm, p);
+  if (e != cudaSuccess) return check_cuda(ctx, e, "k_attn_rows launch");
+  ctx->launches += 1;
+  return check_cuda(ctx, cudaGetLastError(), "k_attn_rows launch");
+}
+
+}  // namespace infr

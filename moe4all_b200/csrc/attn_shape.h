@@ -1,0 +1,97 @@
+// How an attention call is cut into work (attn_rows.cu, attn_tiles.cu), and what its sizes have to satisfy: plain arithmetic, the same on
+// the host and in the kernels.
+//
+// An item is a block of consecutive new tokens of one sequence with the query heads of one kv head; its work is the key tiles that some row
+// of it sees.  Items in order (sequence, block, kv head) and their tiles in order form one line of units, which the CTAs of the launch share
+// evenly: CTA c of C takes the units [c U / C, (c + 1) U / C).  An item that crosses a border is joined from its CTAs' partial results, in
+// their order, by whichever finishes last.
+#pragma once
+#include <cstddef>
+#include <cstdint>
+
+#ifdef __CUDACC__
+#define INFR_ATTN_HD __host__ __device__ __forceinline__
+#else
+#define INFR_ATTN_HD inline
+#endif
+
+namespace infr {
+
+constexpr int ATTN_MAX_SEQ = 16384;    // sequences per call: the blocks' prefix sums fit where the key tiles go later
+constexpr int ATTN_MAX_CTAS = 1024;    // join counters of a context
+constexpr int ATTN_ROWS_LIMIT = 16;    // rows (tokens x heads of a kv head) of an item of the few-rows kernel
+constexpr int ATTN_TILE_ROWS = 128;    // and of the tensor-memory kernel
+
+struct AttnSeq {
+  int q0, q_len;  // rows of the call
+  int past;       // tokens in the cache before them (negative: that many rows at the front see nothing)
+};
+struct AttnBlock {
+  int t0, nt;        // its tokens
+  int lo, hi;        // keys that some row sees
+  int tile0, ntile;  // key tiles, at least one: a block without keys still has its zeros to write
+};
+
+// Sequence from cu_q[s], cu_q[s + 1] and the cache's length, forced into the call's rows and the page table; *bad where that changed them.
+INFR_ATTN_HD AttnSeq attn_seq(int a, int b, int kv, bool packed, int rows, int cap, bool* bad) {
+  const int q0 = a < 0 ? 0 : (a > rows ? rows : a);
+  const int q1 = b < q0 ? q0 : (b > rows ? rows : b);
+  int n = q1 - q0;
+  bool off = q0 != a || q1 != b;
+  if (!packed) {
+    n = kv < 0 ? 0 : (kv > cap ? cap : kv);
+    off = off || n != kv;
+  }
+  if (off) *bad = true;
+  return {q0, q1 - q0, n - (q1 - q0)};
+}
+
+INFR_ATTN_HD int attn_blocks(int q_len, int tb) { return (q_len + tb - 1) / tb; }
+
+INFR_ATTN_HD AttnBlock attn_block(const AttnSeq& s, int b, int tb, int log2_tile, int window) {
+  AttnBlock r;
+  r.t0 = b * tb;
+  r.nt = s.q_len - r.t0 < tb ? s.q_len - r.t0 : tb;
+  const int last = s.past + r.t0 + r.nt, first = s.past + r.t0 - window + 1;
+  r.hi = last > 0 ? last : 0;
+  r.lo = window > 0 && first > 0 ? first : 0;
+  r.tile0 = r.lo >> log2_tile;
+  const int end = (r.hi + (1 << log2_tile) - 1) >> log2_tile;
+  r.ntile = end > r.tile0 ? end - r.tile0 : 1;
+  return r;
+}
+
+// Where CTA c of C begins in a line of u units, and which CTA has unit i.
+INFR_ATTN_HD long long attn_begin(int c, long long u, int C) { return (long long)c * u / C; }
+INFR_ATTN_HD int attn_cta_of(long long i, long long u, int C) { return (int)(((i + 1) * C - 1) / u); }
+
+// What a call gives, as numbers.
+struct AttnSizes {
+  uint32_t rows, n_seq, n_head, n_kv, head_dim;
+  uint32_t n_pages, page_size, max_pages;  // 0 where the keys are packed rows
+  bool paged;
+};
+
+// nullptr, or what is wrong with the sizes; *unsupported: right, but not covered.
+inline const char* attn_sizes_error(const AttnSizes& s, bool* unsupported) {
+  *unsupported = false;
+  if (!s.n_seq || !s.n_head || !s.n_kv || !s.head_dim) return "zero dimension";
+  if (s.n_head % s.n_kv) return "n_head must be a multiple of n_kv";
+  if (s.paged && (!s.n_pages || !s.page_size || !s.max_pages)) return "a page table needs n_pages, page_size and max_pages";
+  if (!s.paged && (s.n_pages || s.page_size || s.max_pages)) return "n_pages, page_size and max_pages need a page table";
+  if (s.paged && (uint64_t)s.max_pages * s.page_size > 0x7FFF0000u) return "max_pages * page_size is past 31 bits";
+  *unsupported = true;
+  if (s.head_dim % 16 || s.head_dim > 256) return "head_dim must be a multiple of 16, at most 256";
+  if (s.n_head / s.n_kv > (uint32_t)ATTN_TILE_ROWS) return "more than 128 query heads to a kv head";
+  if (s.n_seq > (uint32_t)ATTN_MAX_SEQ) return "more than 16384 sequences per call";
+  if (s.rows > (1u << 22) || s.n_head > 1024) return "more than 2^22 rows or 1024 heads";
+  if (s.paged && s.page_size % 16) return "page_size must be a multiple of 16";
+  if (s.paged && s.n_pages > (1u << 30)) return "more than 2^30 pages";
+  *unsupported = false;
+  return nullptr;
+}
+
+// Values a buffer needs for `rows` rows of `wide` values that are `stride` apart.
+inline uint64_t attn_span(uint64_t rows, uint64_t stride, uint64_t wide) { return rows ? (rows - 1) * stride + wide : 0; }
+
+}  // namespace infr

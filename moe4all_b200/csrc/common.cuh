@@ -26,7 +26,7 @@ constexpr uint32_t QK = 256;
 // Device-visible status word written by kernels whose bounded waits ran out.
 struct DeviceStatus {
   int timeout;      // != 0: a bounded wait gave up (value identifies the kernel)
-  int bad_index;    // != 0: an expert id outside [0, n_expert) was clamped
+  int bad_index;    // 1: an expert id outside [0, n_expert) was clamped; 2: a page, row or length of an attention batch
 };
 
 }  // namespace infr
@@ -75,6 +75,7 @@ struct infr_cuda_ctx {
   unsigned long long* done_dev = nullptr;
   float* route_logits = nullptr;              // device memory: the whole-row router kernel's logit buffer, all words
                                               // "not written yet" between launches (see ROUTE_LOGIT_EMPTY)
+  int* attn_count = nullptr;                  // device memory: join counters of the attention kernels, zero between launches
   unsigned long long* trace = nullptr;        // optional phase stamps (see trace_stamp)
   infr_cuda_config cfg = {};                  // tuning switches (infr_cuda_set_config)
   infr::EpState* ep = nullptr;                // expert-parallel communicator and buffers, or null
