@@ -66,6 +66,31 @@ __device__ __forceinline__ const __half* attn_value(const AttnParams& p, int s, 
   return p.v + at + (size_t)head * p.head_pitch;
 }
 
+// Powers of two that bring a row whose largest magnitude is `big` to [2^7, 2^8), and back; both normal numbers.
+__device__ __forceinline__ void attn_row_scale(float big, float& down, float& up) {
+  int e = (int)((__float_as_uint(big) >> 23) & 255u) - 134;
+  e = big > 0.f && big < CUDART_INF_F ? max(-126, e) : 0;
+  down = __uint_as_float((uint32_t)(127 - e) << 23);
+  up = __uint_as_float((uint32_t)(127 + e) << 23);
+}
+
+// a and b as f16 pairs: the rounded values, and what the rounding left.
+__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
+  const __half2 h = __floats2half2_rn(a, b);
+  const float2 f = __half22float2(h);
+  const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
+  hi = *reinterpret_cast<const uint32_t*>(&h);
+  lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+
+// Pairs of f16 bits: whether one is not finite, and the same with those as zeros.
+__device__ __forceinline__ bool any_odd(uint32_t x) { return (x & 0x7C00u) == 0x7C00u || (x & 0x7C000000u) == 0x7C000000u; }
+__device__ __forceinline__ uint32_t only_finite(uint32_t x) {
+  if ((x & 0x7C00u) == 0x7C00u) x &= 0xFFFF0000u;
+  if ((x & 0x7C000000u) == 0x7C000000u) x &= 0x0000FFFFu;
+  return x;
+}
+
 // The first unit's place of a CTA, and the line's length.
 struct AttnStart {
   long long units, u0, u1, ub;  // ub: first unit of the block's first head
@@ -154,6 +179,12 @@ __device__ void attn_plan(const AttnParams& p, int* pre, long long* s_warp, Attn
   __syncthreads();
 }
 
+// Keys below full_hi and from full_lo on are seen by every row of the item.
+__device__ __forceinline__ int attn_full_hi(const AttnSeq& seq, const AttnBlock& blk) { return seq.past + blk.t0 + 1; }
+__device__ __forceinline__ int attn_full_lo(const AttnParams& p, const AttnSeq& seq, const AttnBlock& blk) {
+  return p.window > 0 ? seq.past + blk.t0 + blk.nt - p.window : 0;
+}
+
 // One item after the other from a CTA's first.
 template <int LOG2_TILE>
 struct AttnCursor {
@@ -183,6 +214,28 @@ struct AttnCursor {
   }
 };
 
+// Some value that this row sees may not be finite: what the products of pieces made of it (inf times a piece of the other sign, or of zero, is
+// NaN), or left out, in columns col0 .. of the result or part at dst, is put right: the sum of such values.  Columns that came out finite
+// can only miss values of tiles with hidden keys, where they count as zeros.
+// key0 .. key1: the keys of this part; full_lo .. full_hi: tiles inside have no hidden keys; to: the row's last key.
+static __device__ __noinline__ void attn_odd_values(const AttnParams& p, int s, int q0, int head, int key0, int key1, int tile, int full_lo, int full_hi, int to,
+                                             int col0, int cols, float* dst) {
+  const int from = p.window > 0 ? to - p.window : -1;
+  for (int i = 0; i < cols && col0 + i < p.hd; ++i) {
+    const bool came_finite = fabsf(__ldcg(dst + i)) < CUDART_INF_F;
+    float add = 0.f;
+    bool has = false;
+    for (int ks = key0; ks < key1 && !(add != add); ks += tile) {
+      if (came_finite && ks + tile <= full_hi && ks >= full_lo) continue;
+      for (int key = max(ks, from + 1); key < ks + tile && key <= to; ++key) {
+        const float x = __half2float(attn_value(p, s, q0, head, key)[col0 + i]);
+        if (!(fabsf(x) < CUDART_INF_F)) add += x, has = true;
+      }
+    }
+    if (has) __stcg(dst + i, add);
+  }
+}
+
 // Whose partial results an item has: those of the CTAs first .. last, the first one's in its second slot, the others' in their first.
 struct AttnShare {
   int first, last;
@@ -194,10 +247,10 @@ __device__ __forceinline__ int attn_slot(int cta, const AttnShare& sh) { return 
 
 // After all threads have written their CTA's part: whether this CTA is the item's last and joins it.  Counting is by atomics, the join
 // itself is in the order of the CTAs: the sums do not depend on who came last.
-__device__ __forceinline__ bool attn_arrive(const AttnParams& p, const AttnShare& sh, int* s_last, int threads_bar, int threads) {
+__device__ __forceinline__ bool attn_arrive(const AttnParams& p, const AttnShare& sh, int* s_last, bool leader, int threads_bar, int threads) {
   __threadfence();
   asm volatile("bar.sync %0, %1;" ::"r"(threads_bar), "r"(threads) : "memory");
-  if (threadIdx.x == 0) {
+  if (leader) {
     const int n = atomicAdd(p.count + sh.first, 1);
     *s_last = n == sh.last - sh.first;
     if (n == sh.last - sh.first) p.count[sh.first] = 0;

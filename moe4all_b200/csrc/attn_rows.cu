@@ -28,15 +28,6 @@ __device__ __forceinline__ uint32_t movm(uint32_t a) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
 }
-// a and b as f16 pairs: the rounded values, and what the rounding left.
-__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
-  const __half2 h = __floats2half2_rn(a, b);
-  const float2 f = __half22float2(h);
-  const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
-  hi = *reinterpret_cast<const uint32_t*>(&h);
-  lo = *reinterpret_cast<const uint32_t*>(&l);
-}
-
 template <int HD, int NT>
 struct RowsShape {
   static constexpr int WARPS = HD > 128 ? 4 : 8, THREADS = WARPS * 32, RB = 8 * NT;
@@ -51,7 +42,7 @@ struct RowsShape {
 
 template <int HD, int NT>
 __global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
-    k_attn_rows(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const AttnParams p) {
+    k_attn_rows(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ AttnParams p) {
   using Sh = RowsShape<HD, NT>;
   constexpr int WARPS = Sh::WARPS, THREADS = Sh::THREADS, RB = Sh::RB, STAGES = Sh::STAGES, SLICE = Sh::SLICE, PITCH = Sh::PITCH;
   constexpr int SLABS = HD / 64, KST = HD / 16;
@@ -153,10 +144,8 @@ __global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
         }
       big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 1));
       big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 2));
-      // the largest value to [2^7, 2^8); exponents kept where 2^-e and 2^e are both normal
-      int e = (int)((__float_as_uint(big) >> 23) & 255u) - 134;
-      e = big > 0.f && big < CUDART_INF_F ? max(-126, e) : 0;
-      const float down = __uint_as_float((uint32_t)(127 - e) << 23), up = __uint_as_float((uint32_t)(127 + e) << 23);
+      float down, up;
+      attn_row_scale(big, down, up);
 #pragma unroll
       for (int k = 0; k < KST; ++k)
 #pragma unroll
@@ -168,8 +157,7 @@ __global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
         lim[n][j] = cur.seq.past + blk.t0 + (rr < n_rows ? rr / p.g : blk.nt - 1);
       }
     }
-    const int full_hi = cur.seq.past + blk.t0 + 1;  // keys below are seen by every row, but for the window's
-    const int full_lo = p.window > 0 ? cur.seq.past + blk.t0 + blk.nt - p.window : 0;
+    const int full_hi = attn_full_hi(cur.seq, blk), full_lo = attn_full_lo(p, cur.seq, blk);
 
     float o[KST][NT][4], m[NT][2], l[NT][2];
 #pragma unroll
@@ -388,7 +376,7 @@ __global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
         if (i == 0) __stcg(p.part_ml + at, make_float2(M, L));
       }
     }
-    if (!whole && attn_arrive(p, share, &s_last, 0, THREADS)) {
+    if (!whole && attn_arrive(p, share, &s_last, tid == 0, 0, THREADS)) {
       for (int e = tid; e < RB * (HD / 4); e += THREADS) {
         const int r = e / (HD / 4), i = 4 * (e % (HD / 4));
         if (r < n_rows && i < p.hd) store(r, i, attn_join4<HD>(p, share, RB, r, i));
