@@ -22,6 +22,7 @@ struct AttnParams {
   float scale_log2;  // scale * log2(e)
   int rows, n_seq, n_kv, g, hd, page_size, max_pages, n_pages, window;
   int tb;            // tokens of an item
+  uint32_t g_inv;    // ceil(2^16 / g): r / g = r * g_inv >> 16 for the rows r of an item
   int cap;           // max_pages * page_size
 };
 
@@ -57,6 +58,13 @@ __device__ __forceinline__ int attn_page(const AttnParams& p, int s, int page) {
   if ((unsigned)id < (unsigned)p.n_pages) return id;
   p.status->bad_index = 2;  // read as page 0, reported at the next sync
   return 0;
+}
+
+// Token (of the item) and query head (of the kv head) of row r < 128: the error of g_inv adds less than 1 / 512.
+__device__ __forceinline__ int attn_row_token(const AttnParams& p, int r) { return (int)((uint32_t)r * p.g_inv >> 16); }
+__device__ __forceinline__ size_t attn_row_offset(const AttnParams& p, int token0, int head, int r, long long stride) {
+  const int t = attn_row_token(p, r);
+  return (size_t)(token0 + t) * stride + (size_t)(head * p.g + (r - t * p.g)) * p.hd;
 }
 
 // Where the values of a key and head begin; the keys behind it follow row_pitch apart up to its page's end.

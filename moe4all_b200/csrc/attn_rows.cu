@@ -131,7 +131,7 @@ __global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
     for (int n = 0; n < NT; ++n) {
       const int r = 8 * n + (lane >> 2);
       const bool has = r < n_rows;
-      const float* src = p.q + (size_t)(cur.seq.q0 + blk.t0 + (has ? r / p.g : 0)) * p.q_stride + (size_t)(cur.head * p.g + (has ? r % p.g : 0)) * p.hd;
+      const float* src = p.q + attn_row_offset(p, cur.seq.q0 + blk.t0, cur.head, has ? r : 0, p.q_stride);
       float2 v[KST][2];
       float big = 0.f;
 #pragma unroll
@@ -154,7 +154,7 @@ __global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
       for (int j = 0; j < 2; ++j) {
         f[n][j] = __shfl_sync(0xFFFFFFFFu, up, (c0 + j) * 4) * p.scale_log2;
         const int rr = 8 * n + c0 + j;
-        lim[n][j] = cur.seq.past + blk.t0 + (rr < n_rows ? rr / p.g : blk.nt - 1);
+        lim[n][j] = cur.seq.past + blk.t0 + (rr < n_rows ? attn_row_token(p, rr) : blk.nt - 1);
       }
     }
     const int full_hi = attn_full_hi(cur.seq, blk), full_lo = attn_full_lo(p, cur.seq, blk);
@@ -348,8 +348,7 @@ __global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
     const bool whole = first_tile == 0 && end_tile == blk.ntile;
     const AttnShare share = attn_share(cur.ub, blk.ntile, st);
     auto store = [&](int r, int i, float4 v) {
-      float* dst = p.out + (size_t)(cur.seq.q0 + blk.t0 + r / p.g) * p.out_stride + (size_t)(cur.head * p.g + r % p.g) * p.hd + i;
-      *reinterpret_cast<float4*>(dst) = v;
+      *reinterpret_cast<float4*>(p.out + attn_row_offset(p, cur.seq.q0 + blk.t0, cur.head, r, p.out_stride) + i) = v;
     };
     for (int e = tid; e < RB * (HD / 4); e += THREADS) {
       const int r = e / (HD / 4), i = 4 * (e % (HD / 4));

@@ -4,13 +4,16 @@
 // a pair (row, key) costs 8 hd operations at the f16 rate.
 //
 // One CTA per SM, roles by warpgroup:
-//   weights   a thread per row: scores S from tensor memory -> running maximum -> weights P, back over S as f16 pieces
-//   sums      a thread per row: the f32 sums in registers.  Each tile's P V starts from zero in tensor memory and is added here, times
-//             the maximum's correction: an accumulation over thousands of steps in the tensor cores, which truncate, would lose
-//             an f32 result's last bits (measured: 1.3e-8 of the result per step), and the correction is part of the same FMA
-//   control   a warp for the copies, a warp for the MMAs, two that turn q into f16 pieces and look after tiles with hidden keys
+//   weights   a thread per row: scores S from tensor memory -> running maximum -> weights P, back over S as f16 pieces.  Two groups (one for
+//             heads wider than 128, whose products take longer) take the tiles in turn, each with a maximum and a weight of its own; the
+//             group that has an item's first tile turns the item's q into f16 pieces, while the other still has the last item's end
+//   sums      a thread per row: the f32 sums in registers.  Each tile's P V starts from zero in tensor memory and is added here, brought
+//             to a common maximum: an accumulation over thousands of steps in the tensor cores, which truncate, would lose an f32
+//             result's last bits (measured: 1.3e-8 of the result per step)
+//   control   a warp for the copies, a warp for the MMAs, two that look after tiles with hidden keys
 // S and P of two tiles, and the sums of two (one for heads wider than 192), fill tensor memory: while a tile's weights are made the
-// tensor cores work on the next tile's scores and the last one's sums.
+// tensor cores work on the next tile's scores and the last one's sums.  Loops are kept rolled: with every tile's code straight-line the
+// roles together left the instruction cache (60% hits, 4.6 ms for an 8192-token prompt instead of 4.1).
 #include "attn.cuh"
 #include "umma.cuh"
 
@@ -18,42 +21,51 @@ namespace infr {
 namespace {
 
 constexpr float TILE_BIAS = 15.f;  // weights are 2^(x - maximum + 15): below f16's limit, 2^-40 of the largest still has a bit
-constexpr int ALPHA_RING = 4, ITEM_RING = 16;
+constexpr int RING = 4;            // tiles' and items' words in shared memory: the roles are never further apart
 
 template <int HD>
 struct TilesShape {
   static constexpr int LOG2_TILE = HD <= 128 ? 7 : 6, BK = 1 << LOG2_TILE;
-  static constexpr int SUM_GROUPS = HD <= 128 ? 1 : 2, COLS = HD / SUM_GROUPS;  // columns of a sums thread
-  static constexpr int THREADS = 128 * (2 + SUM_GROUPS);
+  static constexpr int W_GROUPS = HD <= 128 ? 2 : 1;
+  static constexpr int S_GROUPS = 3 - W_GROUPS, COLS = HD / S_GROUPS;  // columns of a sums thread
+  static constexpr int THREADS = 512;
   static constexpr int SLABS = HD / 64, TILE = BK * HD * 2, QPIECE = 128 * HD * 2;
   static constexpr int STAGES = HD == 64 ? 8 : HD == 128 ? 4 : HD == 192 ? 4 : 2;
   static constexpr int OBUFS = HD <= 192 ? 2 : 1;
   static constexpr uint32_t O_COL = 2 * BK;
-  static constexpr int SMALL = ALPHA_RING * 128 * 4 + ITEM_RING * 128 * 8 + 4 * 128 * 4;  // corrections, (maximum, weight), score factors
+  static constexpr int SMALL = RING * 128 * 4 + 2 * 2 * RING * 128 * 8 + RING * 128 * 4;  // tiles' maxima, (maximum, weight), score factors
   static constexpr int SMEM = 1024 + 2 * QPIECE + STAGES * TILE + SMALL;
   static_assert(SMEM + 1024 <= 232448, "more shared memory than a CTA has");
-  // registers by role; together no more than the launch has
-  static constexpr int REG_W = HD <= 128 ? 160 : 136, REG_S = HD <= 128 ? 208 : 152, REG_C = HD <= 128 ? 136 : 72;
+  // registers by role: together as many as the launch has
+  static constexpr int REG_W = HD == 64 ? 128 : HD == 128 ? 104 : 136, REG_S = HD == 64 ? 144 : HD == 128 ? 200 : 152, REG_C = HD == 64 ? 112 : HD == 128 ? 104 : 72;
+  static_assert(REG_W * W_GROUPS + REG_S * S_GROUPS + REG_C <= 512, "more registers than the launch has");
 };
 
 template <int N>
-__device__ __forceinline__ void regs_less() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
-template <int N>
-__device__ __forceinline__ void regs_more() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+__device__ __forceinline__ void set_regs() {  // from the launch's 128
+  if constexpr (N < 128) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+  if constexpr (N > 128) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
 
 struct TileBars {
-  uint64_t full[8], empty[8];   // tiles of K and V, in the order K0 K1 V0 K2 V1 ...
+  uint64_t full[8], empty[8];  // tiles of K and V, in the order K0 K1 V0 K2 V1 ...
   uint64_t s_full[2], p_full[2];
   uint64_t o_full[2], o_empty[2];
-  uint64_t a_full[ALPHA_RING];  // a tile's corrections (and, at an item's last, maximum and weight)
-  uint64_t f_full[4];           // an item's score factors
-  uint64_t q_full, q_empty;
-  uint64_t v_ask, v_ok;         // a V tile with hidden keys: there, and looked after
+  uint64_t a_full[RING];       // a tile's maxima (and, at an item's end, maximum and weight)
+  uint64_t f_full[RING];       // an item's score factors
+  uint64_t q_full, q_empty[RING];
+  uint64_t v_ask, v_ok;        // a V tile with hidden keys: there, and looked after
 };
 
 // Whether some row of the item does not see some key of [ks, ks + n).
 __device__ __forceinline__ bool tile_masked(const AttnParams& p, const AttnSeq& seq, const AttnBlock& blk, int ks, int n) {
   return ks + n > attn_full_hi(seq, blk) || ks < attn_full_lo(p, seq, blk);
+}
+
+// Bit i: whether the key k0 + i is in (from, to].
+__device__ __forceinline__ uint32_t seen_keys(int k0, int from, int to) {
+  const int lo = max(0, from + 1 - k0), n = min(32, to + 1 - k0);  // bits lo .. n - 1
+  return n <= lo ? 0u : (~0u >> (32 - (n - lo))) << lo;
 }
 
 template <int HD>
@@ -66,24 +78,23 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
   __shared__ long long s_scan[Sh::THREADS / 32];
   __shared__ AttnStart s_start;
   __shared__ uint32_t s_tmem;
-  __shared__ int s_last, s_odd[ITEM_RING];
+  __shared__ int s_last, s_odd[2 * RING];
   unsigned char* s_q = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   unsigned char* s_kv = s_q + 2 * Sh::QPIECE;
-  float* s_alpha = reinterpret_cast<float*>(s_kv + STAGES * TILE);           // [ALPHA_RING][128]
-  float2* s_ml = reinterpret_cast<float2*>(s_alpha + ALPHA_RING * 128);      // [ITEM_RING][128]
-  float* s_fac = reinterpret_cast<float*>(s_ml + ITEM_RING * 128);           // [4][128]
+  float* s_ref = reinterpret_cast<float*>(s_kv + STAGES * TILE);        // [RING][128]
+  float* s_fac = s_ref + RING * 128;                                    // [RING][128]
+  float2* s_ml = reinterpret_cast<float2*>(s_fac + RING * 128);         // [2 RING][2][128]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int wg = warp >> 2, control = 1 + Sh::SUM_GROUPS, role = wg == control ? 4 + (warp & 3) : wg;  // 4: copies, 5: MMAs
+  const int wg = warp >> 2, role = wg == 3 ? 3 + (warp & 3) : wg < Sh::W_GROUPS ? 0 : 1;  // 0 weights, 1 sums, 3 copies, 4 MMAs, 5 and 6 hidden keys
 
   if (tid == 0) {
     for (int i = 0; i < 8; ++i) mbar_init(bars.full + i, 1), mbar_init(bars.empty + i, 1);
-    for (int i = 0; i < 2; ++i) mbar_init(bars.s_full + i, 1), mbar_init(bars.p_full + i, 4), mbar_init(bars.o_full + i, 1), mbar_init(bars.o_empty + i, 4 * Sh::SUM_GROUPS);
-    for (int i = 0; i < ALPHA_RING; ++i) mbar_init(bars.a_full + i, 4);
-    for (int i = 0; i < 4; ++i) mbar_init(bars.f_full + i, 2);
-    mbar_init(&bars.q_full, 2), mbar_init(&bars.q_empty, 1), mbar_init(&bars.v_ask, 1), mbar_init(&bars.v_ok, 2);
+    for (int i = 0; i < 2; ++i) mbar_init(bars.s_full + i, 1), mbar_init(bars.p_full + i, 4), mbar_init(bars.o_full + i, 1), mbar_init(bars.o_empty + i, 4 * Sh::S_GROUPS);
+    for (int i = 0; i < RING; ++i) mbar_init(bars.a_full + i, 4), mbar_init(bars.f_full + i, 4), mbar_init(bars.q_empty + i, 1);
+    mbar_init(&bars.q_full, 4), mbar_init(&bars.v_ask, 1), mbar_init(&bars.v_ok, 2);
     mbar_fence_init();
   }
-  if (tid < ITEM_RING) s_odd[tid] = 0;
+  if (tid < 2 * RING) s_odd[tid] = 0;
   if (warp == 0) umma::tmem_alloc(&s_tmem);
   pdl_wait();
   attn_plan<Sh::THREADS, Sh::LOG2_TILE>(p, reinterpret_cast<int*>(s_q), s_scan, &s_start);
@@ -96,10 +107,10 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
   const int N = (int)(st.u1 - st.u0);  // tiles of this CTA
   bool ok = true;
 
-  if (N > 0 && wg == control) regs_less<Sh::REG_C>();
+  if (N > 0 && wg == 3) set_regs<Sh::REG_C>();
   if (N == 0) {
     // nothing to do
-  } else if (role == 4) {
+  } else if (role == 3) {
     // ---- copies
     AttnCursor<Sh::LOG2_TILE> kc, vc;
     kc.start(p, st);
@@ -141,7 +152,7 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
       // copies in flight land before the shared memory is somebody else's
       for (int i = max(0, asked - STAGES); i < asked; ++i) mbar_wait_bounded(bars.full + i % STAGES, (i / STAGES) & 1);
     }
-  } else if (role == 5) {
+  } else if (role == 4) {
     // ---- MMAs
     AttnCursor<Sh::LOG2_TILE> ic, cc;  // of the tile whose scores come next, and of the one whose sums do
     ic.start(p, st);
@@ -175,7 +186,7 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
             }
           umma::commit1(bars.empty + stage);
           umma::commit1(bars.s_full + (issued & 1));
-          if (last) umma::commit1(&bars.q_empty);
+          if (last) umma::commit1(bars.q_empty + ((items - 1) & (RING - 1)));
         }
         __syncwarp();
         ++issued;
@@ -212,204 +223,211 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
       __syncwarp();
     }
     if (!ok && lane == 0) atomicExch(&p.status->timeout, 11);
-  } else if (role > 5) {
-    // ---- q into two f16 pieces, and V tiles with hidden keys
-    const int at = (warp & 1) * 32 + lane, l8 = lane & 7;
+  } else if (role > 4) {
+    // ---- V tiles with hidden keys.  0 x value has to be 0 where a row does not see the key: keys that no row sees become zeros, and so do
+    // values that are not finite; the item's end adds these to the rows that see them
+    const int at = (warp & 1) * 32 + lane;
     AttnCursor<Sh::LOG2_TILE> c;
     c.start(p, st);
     int asks = 0, item = 0;
-    for (int n = 0; n < N && ok; ++item) {
-      const long long u = st.u0 + n;
-      while (u >= c.ub + c.blk.ntile) c.next(p);
-      const int end = (int)((c.ub + c.blk.ntile < st.u1 ? c.ub + c.blk.ntile : st.u1) - st.u0), n_rows = c.blk.nt * p.g;
-      if (at == 0) s_odd[(item + 8) % ITEM_RING] = 0;
-      if (item > 0) ok = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(&bars.q_empty, (item - 1) & 1));
-      if (!ok) break;
-      // eight lanes a row, four rows a warp at once; rows past the item's are zeros
-#pragma unroll(HD <= 128 ? 2 : 1)
-      for (int r0 = 0; r0 < 128; r0 += 8) {
-        const int r = r0 + (at >> 3);
-        const bool has = r < n_rows;
-        const float* src = p.q + (size_t)(c.seq.q0 + c.blk.t0 + (has ? r / p.g : 0)) * p.q_stride + (size_t)(c.head * p.g + (has ? r % p.g : 0)) * p.hd;
-        float4 v[HD / 32];
-        float big = 0.f;
-#pragma unroll
-        for (int j = 0; j < HD / 32; ++j) {
-          const int i = 4 * (l8 + 8 * j);
-          v[j] = has && i < p.hd ? __ldcg(reinterpret_cast<const float4*>(src + i)) : make_float4(0.f, 0.f, 0.f, 0.f);
-          big = fmaxf(big, fmaxf(fmaxf(fabsf(v[j].x), fabsf(v[j].y)), fmaxf(fabsf(v[j].z), fabsf(v[j].w))));
-        }
-#pragma unroll
-        for (int x = 1; x < 8; x <<= 1) big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, x));
-        float down, up;
-        attn_row_scale(big, down, up);
-        if (p.scale_log2 < 0.f) down = -down;
-#pragma unroll
-        for (int j = 0; j < HD / 32; ++j) {
-          const int i = 4 * (l8 + 8 * j);
-          uint2 hi, lo;
-          split2(v[j].x * down, v[j].y * down, hi.x, lo.x);
-          split2(v[j].z * down, v[j].w * down, hi.y, lo.y);
-          unsigned char* dst = s_q + (i >> 6) * 16384 + r * 128 + ((((i >> 3) & 7) ^ (r & 7)) << 4) + ((i & 4) << 1);
-          *reinterpret_cast<uint2*>(dst) = hi;
-          *reinterpret_cast<uint2*>(dst + Sh::QPIECE) = lo;
-        }
-        // (not 0: hidden keys' -inf times it stays -inf)
-        if (l8 == 0) s_fac[(item & 3) * 128 + r] = fmaxf(up * fabsf(p.scale_log2), 1.2e-38f);
-      }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars.q_full), mbar_arrive(bars.f_full + (item & 3));
-      for (; n < end && ok; ++n) {
-        const int ks = (c.blk.tile0 + (int)(st.u0 + n - c.ub)) << Sh::LOG2_TILE;
-        if (!tile_masked(p, c.seq, c.blk, ks, BK)) continue;
-        // 0 x value has to be 0 where a row does not see the key: keys that no row sees become zeros, and so do values that are not
-        // finite; the item's end adds these to the rows that see them
-        ok = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(&bars.v_ask, asks & 1));
-        ++asks;
-        if (!ok) break;
-        const int i = n + 1 < N ? 2 * n + 2 : 2 * N - 1;
-        bool odd = false;
-        for (int row = at; row < BK; row += 64) {
-          const bool seen = ks + row >= c.blk.lo && ks + row < c.blk.hi;
-#pragma unroll
-          for (int s = 0; s < SLABS; ++s) {
-            unsigned char* base = s_kv + (i % STAGES) * TILE + s * (BK * 128) + row * 128;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              uint4* w = reinterpret_cast<uint4*>(base + (((j + row) & 7) << 4));
-              if (!seen) {
-                *w = make_uint4(0, 0, 0, 0);
-                continue;
-              }
-              const uint4 x = *w;
-              if (any_odd(x.x) || any_odd(x.y) || any_odd(x.z) || any_odd(x.w)) {
-                *w = make_uint4(only_finite(x.x), only_finite(x.y), only_finite(x.z), only_finite(x.w));
-                odd = true;
-              }
-            }
-          }
-        }
-        if (odd) s_odd[item % ITEM_RING] = 1;
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bars.v_ok);
-      }
-    }
-    if (!ok && lane == 0) atomicExch(&p.status->timeout, 11);
-  } else if (wg == 0) {
-    // ---- weights: thread = row
-    if (Sh::REG_W < 160) regs_more<Sh::REG_W>();
-    else regs_less<Sh::REG_W>();
-    AttnCursor<Sh::LOG2_TILE> c;
-    c.start(p, st);
-    const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
-    int item = -1;
-    float m = -CUDART_INF_F, l = 0.f, f = 0.f;
-    int to = 0, from = 0, n_rows = 0;  // the row sees the keys (from, to]
     for (int n = 0; n < N && ok; ++n) {
       const long long u = st.u0 + n;
-      if (n == 0 || u >= c.ub + c.blk.ntile) {
+      if (u >= c.ub + c.blk.ntile) {
         while (u >= c.ub + c.blk.ntile) c.next(p);
         ++item;
-        n_rows = c.blk.nt * p.g;
-        to = c.seq.past + c.blk.t0 + (tid < n_rows ? tid / p.g : c.blk.nt - 1);
-        from = p.window > 0 ? to - p.window : -1;
-        m = -CUDART_INF_F, l = 0.f;
-        ok = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(bars.f_full + (item & 3), (item >> 2) & 1));
-        f = s_fac[(item & 3) * 128 + tid];
+        if (at == 0) s_odd[(item + RING) % (2 * RING)] = 0;
       }
       const int ks = (c.blk.tile0 + (int)(u - c.ub)) << Sh::LOG2_TILE;
-      const bool masked = tile_masked(p, c.seq, c.blk, ks, BK);
-      ok = ok && __all_sync(0xFFFFFFFFu, mbar_wait_bounded(bars.s_full + (n & 1), (n >> 1) & 1));
+      if (!tile_masked(p, c.seq, c.blk, ks, BK)) continue;
+      ok = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(&bars.v_ask, asks & 1));
+      ++asks;
       if (!ok) break;
-      umma::fence_after_sync();
-      float alpha = 1.f;
-      if (warp * 32 < n_rows) {  // (other rows' weights are whatever is there: they reach those rows' sums only)
-        const uint32_t sa = lanes + (n & 1) * BK;
-        float top = -CUDART_INF_F;
+      const int i = n + 1 < N ? 2 * n + 2 : 2 * N - 1;
+      bool odd = false;
+#pragma unroll 1
+      for (int row = at; row < BK * SLABS; row += 64) {
+        const int key = ks + (row & (BK - 1));
+        const bool seen = key >= c.blk.lo && key < c.blk.hi;
+        unsigned char* base = s_kv + (i % STAGES) * TILE + row * 128;
 #pragma unroll
-        for (int j = 0; j < BK / 32; ++j) {
-          float s[32];
-          umma::tmem_ld_32x32(sa + 32 * j, s);
-          umma::tmem_ld_wait(s);
-          if (masked) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (ks + 32 * j + i <= to && ks + 32 * j + i > from) top = fmaxf(top, s[i]);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) top = fmaxf(top, s[i]);
+        for (int j = 0; j < 8; ++j) {
+          uint4* w = reinterpret_cast<uint4*>(base + (((j + row) & 7) << 4));
+          const uint4 x = *w;
+          if (!seen) *w = make_uint4(0, 0, 0, 0);
+          else if (any_odd(x.x) || any_odd(x.y) || any_odd(x.z) || any_odd(x.w)) {
+            *w = make_uint4(only_finite(x.x), only_finite(x.y), only_finite(x.z), only_finite(x.w));
+            odd = true;
           }
         }
-        const float now = fmaxf(m, top * f);
-        alpha = exp2_rel(m, now);
-        m = now;
-        const float off = TILE_BIAS - (now == -CUDART_INF_F ? 0.f : now);
-        float sum0 = 0.f, sum1 = 0.f;
-#pragma unroll
-        for (int j = 0; j < BK / 32; ++j) {
-          float s[32];
-          umma::tmem_ld_32x32(sa + 32 * j, s);
-          umma::tmem_ld_wait(s);
-          if (masked) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (!(ks + 32 * j + i <= to && ks + 32 * j + i > from)) s[i] = -CUDART_INF_F;
-          }
-          uint32_t w[32];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float a = exp2_approx(fmaf(s[2 * i], f, off)), b = exp2_approx(fmaf(s[2 * i + 1], f, off));
-            sum0 += a, sum1 += b;
-            split2(a, b, w[i], w[16 + i]);
-          }
-          umma::tmem_st_32x32_async(sa + 32 * j, w);
-        }
-        l = l * alpha + (sum0 + sum1);
-        umma::tmem_st_wait();
       }
-      umma::fence_before_sync();
-      s_alpha[(n & (ALPHA_RING - 1)) * 128 + tid] = alpha;
-      if (u + 1 >= c.ub + c.blk.ntile || n + 1 == N) {
-        if (m == -CUDART_INF_F && l != 0.f) m = 0.f;  // nothing but NaN: a part that counts
-        s_ml[(item % ITEM_RING) * 128 + tid] = make_float2(m, l);
-      }
+      if (odd) s_odd[item % (2 * RING)] = 1;
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
-      if (lane == 0) mbar_arrive(bars.p_full + (n & 1)), mbar_arrive(bars.a_full + (n & (ALPHA_RING - 1)));
+      if (lane == 0) mbar_arrive(&bars.v_ok);
+    }
+    if (!ok && lane == 0) atomicExch(&p.status->timeout, 11);
+  } else if (role == 0) {
+    // ---- weights: thread = row, every W_GROUPS-th tile
+    set_regs<Sh::REG_W>();
+    AttnCursor<Sh::LOG2_TILE> c;
+    c.start(p, st);
+    const int row = tid & 127;
+    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    for (int n0 = 0, item = 0; n0 < N && ok; ++item) {
+      while (st.u0 + n0 >= c.ub + c.blk.ntile) c.next(p);
+      const int n1 = (int)((c.ub + c.blk.ntile < st.u1 ? c.ub + c.blk.ntile : st.u1) - st.u0), n_rows = c.blk.nt * p.g;
+      const int slot = item & (RING - 1);
+      if (Sh::W_GROUPS == 1 || (n0 & 1) == wg) {
+        // q into two f16 pieces: eight lanes a row; rows past the item's are zeros
+        if (item > 0) ok = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(bars.q_empty + ((item - 1) & (RING - 1)), ((item - 1) / RING) & 1));
+        if (!ok) break;
+        const int l8 = lane & 7;
+#pragma unroll(HD == 64 ? 4 : HD == 128 ? 2 : 1)
+        for (int r0 = 0; r0 < 128; r0 += 16) {
+          const int r = r0 + (row >> 3);
+          const bool has = r < n_rows;
+          const float* src = p.q + attn_row_offset(p, c.seq.q0 + c.blk.t0, c.head, has ? r : 0, p.q_stride);
+          float4 v[HD / 32];
+          float big = 0.f;
+#pragma unroll
+          for (int j = 0; j < HD / 32; ++j) {
+            const int i = 4 * (l8 + 8 * j);
+            v[j] = has && i < p.hd ? __ldcg(reinterpret_cast<const float4*>(src + i)) : make_float4(0.f, 0.f, 0.f, 0.f);
+          }
+#pragma unroll
+          for (int j = 0; j < HD / 32; ++j) big = fmaxf(big, fmaxf(fmaxf(fabsf(v[j].x), fabsf(v[j].y)), fmaxf(fabsf(v[j].z), fabsf(v[j].w))));
+#pragma unroll
+          for (int x = 1; x < 8; x <<= 1) big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, x));
+          float down, up;
+          attn_row_scale(big, down, up);
+          if (p.scale_log2 < 0.f) down = -down;
+#pragma unroll
+          for (int j = 0; j < HD / 32; ++j) {
+            const int i = 4 * (l8 + 8 * j);
+            uint2 hi, lo;
+            split2(v[j].x * down, v[j].y * down, hi.x, lo.x);
+            split2(v[j].z * down, v[j].w * down, hi.y, lo.y);
+            unsigned char* dst = s_q + (i >> 6) * 16384 + r * 128 + ((((i >> 3) & 7) ^ (r & 7)) << 4) + ((i & 4) << 1);
+            *reinterpret_cast<uint2*>(dst) = hi;
+            *reinterpret_cast<uint2*>(dst + Sh::QPIECE) = lo;
+          }
+          // (not 0: hidden keys' -inf times it stays -inf)
+          if (l8 == 0) s_fac[slot * 128 + r] = fmaxf(up * fabsf(p.scale_log2), 1.2e-38f);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.q_full), mbar_arrive(bars.f_full + slot);
+      }
+      int n = n0;
+      if (Sh::W_GROUPS == 2 && (n & 1) != wg) ++n;
+      if (n < n1) ok = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(bars.f_full + slot, (item / RING) & 1));
+      const float f = s_fac[slot * 128 + row];
+      const int to = c.seq.past + c.blk.t0 + (row < n_rows ? attn_row_token(p, row) : c.blk.nt - 1);  // the row sees the keys (from, to]
+      const int from = p.window > 0 ? to - p.window : -1;
+      float m = -CUDART_INF_F, l = 0.f;
+      for (; n < n1 && ok; n += Sh::W_GROUPS) {
+        const int ks = (c.blk.tile0 + (int)(st.u0 + n - c.ub)) << Sh::LOG2_TILE;
+        const bool masked = tile_masked(p, c.seq, c.blk, ks, BK);
+        ok = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(bars.s_full + (n & 1), (n >> 1) & 1));
+        if (!ok) break;
+        umma::fence_after_sync();
+        if ((warp & 3) * 32 < n_rows) {  // (other rows' weights are whatever is there: they reach those rows' sums only)
+          const uint32_t sa = lanes + (n & 1) * BK;
+          float top = -CUDART_INF_F;
+#pragma unroll 1
+          for (int j = 0; j < BK / 32; ++j) {
+            float s[32];
+            umma::tmem_ld_32x32(sa + 32 * j, s);
+            const uint32_t seen = masked ? seen_keys(ks + 32 * j, from, to) : ~0u;
+            umma::tmem_ld_wait(s);
+            if (seen != ~0u) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) s[i] = (seen >> i) & 1u ? s[i] : -CUDART_INF_F;
+            }
+            float t[4] = {top, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) t[(i >> 1) & 3] = fmaxf(fmaxf(t[(i >> 1) & 3], s[i]), s[i + 1]);
+            top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+          }
+          const float now = fmaxf(m, top * f);
+          l *= exp2_rel(m, now);
+          m = now;
+          const float off = TILE_BIAS - (now == -CUDART_INF_F ? 0.f : now);
+          const float2 f2 = make_float2(f, f), off2 = make_float2(off, off), minus = make_float2(-1.f, -1.f);
+          float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll 1
+          for (int j = 0; j < BK / 32; ++j) {
+            float s[32];
+            umma::tmem_ld_32x32(sa + 32 * j, s);
+            const uint32_t seen = masked ? seen_keys(ks + 32 * j, from, to) : ~0u;
+            umma::tmem_ld_wait(s);
+            if (seen != ~0u) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) s[i] = (seen >> i) & 1u ? s[i] : -CUDART_INF_F;
+            }
+            uint32_t w[32];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float2 x = __ffma2_rn(make_float2(s[2 * i], s[2 * i + 1]), f2, off2);
+              const float2 e = make_float2(exp2_approx(x.x), exp2_approx(x.y));
+              sum[i & 1] = __fadd2_rn(sum[i & 1], e);
+              // the piece that f16 holds (below 2^-14, 2^-29 of the largest, rounded once more), and the rest
+              const float2 h = make_float2(__uint_as_float(__float_as_uint(e.x) & 0xFFFFE000u), __uint_as_float(__float_as_uint(e.y) & 0xFFFFE000u));
+              const float2 r = __ffma2_rn(h, minus, e);
+              const __half2 hh = __floats2half2_rn(h.x, h.y), rr = __floats2half2_rn(r.x, r.y);
+              w[i] = *reinterpret_cast<const uint32_t*>(&hh);
+              w[16 + i] = *reinterpret_cast<const uint32_t*>(&rr);
+            }
+            umma::tmem_st_32x32_async(sa + 32 * j, w);
+          }
+          l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+          umma::tmem_st_wait();
+        }
+        umma::fence_before_sync();
+        s_ref[(n & (RING - 1)) * 128 + row] = m;
+        if (n + Sh::W_GROUPS >= n1) s_ml[((item % (2 * RING)) * 2 + (n & (Sh::W_GROUPS - 1))) * 128 + row] = make_float2(m, l);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bars.p_full + (n & 1)), mbar_arrive(bars.a_full + (n & (RING - 1)));
+      }
+      n0 = n1;
     }
     if (!ok && lane == 0) atomicExch(&p.status->timeout, 11);
   } else {
     // ---- sums: thread = row, COLS of its columns
-    regs_more<Sh::REG_S>();
+    set_regs<Sh::REG_S>();
     AttnCursor<Sh::LOG2_TILE> c;
     c.start(p, st);
-    const int row = tid & 127, col0 = (wg - 1) * Sh::COLS;
+    const int row = tid & 127, group = wg - Sh::W_GROUPS, col0 = group * Sh::COLS;
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16) + Sh::O_COL + col0;
-    float o[Sh::COLS];
+    float2 o[Sh::COLS / 2];
+    float M = -CUDART_INF_F;
     int item = 0, first = 0;
     for (int n = 0; n < N && ok; ++n) {
       const long long u = st.u0 + n;
       while (u >= c.ub + c.blk.ntile) c.next(p);
       if (n == first) {
+        M = -CUDART_INF_F;
 #pragma unroll
-        for (int i = 0; i < Sh::COLS; ++i) o[i] = 0.f;
+        for (int i = 0; i < Sh::COLS / 2; ++i) o[i] = make_float2(0.f, 0.f);
       }
       const int n_rows = c.blk.nt * p.g;
       const bool mine = (warp & 3) * 32 < n_rows;
-      ok = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(bars.a_full + (n & (ALPHA_RING - 1)), (n / ALPHA_RING) & 1));
-      const float alpha = s_alpha[(n & (ALPHA_RING - 1)) * 128 + row];
+      ok = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(bars.a_full + (n & (RING - 1)), (n / RING) & 1));
+      const float ref = s_ref[(n & (RING - 1)) * 128 + row], now = fmaxf(M, ref);
+      const float a = exp2_rel(M, now), b = exp2_rel(ref, now);
+      M = now;
       ok = ok && __all_sync(0xFFFFFFFFu, mbar_wait_bounded(bars.o_full + n % OBUFS, (n / OBUFS) & 1));
       if (!ok) break;
       umma::fence_after_sync();
       if (mine) {
+        const float2 a2 = make_float2(a, a), b2 = make_float2(b, b), zero = make_float2(0.f, 0.f);
 #pragma unroll
         for (int j = 0; j < Sh::COLS / 32; ++j) {
           float t[32];
           umma::tmem_ld_32x32(lanes + (n % OBUFS) * HD + 32 * j, t);
           umma::tmem_ld_wait(t);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[32 * j + i] = fmaf(o[32 * j + i], alpha, t[i]);
+          for (int i = 0; i < 16; ++i) o[16 * j + i] = __ffma2_rn(o[16 * j + i], a2, __ffma2_rn(make_float2(t[2 * i], t[2 * i + 1]), b2, zero));
         }
       }
       umma::fence_before_sync();
@@ -420,32 +438,37 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
       // ---- the item's end
       const bool whole = u + 1 >= c.ub + c.blk.ntile && st.u0 + first <= c.ub;
       const AttnShare share = attn_share(c.ub, c.blk.ntile, st);
-      const bool odd_tiles = *reinterpret_cast<volatile int*>(s_odd + item % ITEM_RING) != 0;
-      const float2 ml = s_ml[(item % ITEM_RING) * 128 + row];
+      const bool odd_tiles = *reinterpret_cast<volatile int*>(s_odd + item % (2 * RING)) != 0;
+      float L = 0.f;  // the groups' weights, brought to one maximum
+#pragma unroll
+      for (int w = 0; w < Sh::W_GROUPS; ++w)
+        if (n > first || w == (n & (Sh::W_GROUPS - 1))) {
+          const float2 ml = s_ml[((item % (2 * RING)) * 2 + w) * 128 + row];
+          L += ml.y * (ml.y == ml.y ? exp2_rel(ml.x, M) : 1.f);
+        }
+      const float2 ml = make_float2(M == -CUDART_INF_F && L != 0.f ? 0.f : M, L);  // (nothing but NaN is a part that counts)
       const size_t slot = (size_t)attn_slot(blockIdx.x, share) * 128 + row;
       const bool mine_row = row < n_rows;
-      float* dst = whole ? p.out + (size_t)(c.seq.q0 + c.blk.t0 + (mine_row ? row / p.g : 0)) * p.out_stride + (size_t)(c.head * p.g + (mine_row ? row % p.g : 0)) * p.hd + col0
-                         : p.part + slot * HD + col0;
+      float* dst = whole ? p.out + attn_row_offset(p, c.seq.q0 + c.blk.t0, c.head, mine_row ? row : 0, p.out_stride) + col0 : p.part + slot * HD + col0;
       if (mine_row) {
-        const float inv = !whole ? 1.f : ml.y > 0.f ? 1.f / ml.y : (ml.y == 0.f ? 0.f : ml.y);
+        const float inv = !whole ? 1.f : L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
         bool odd = odd_tiles;
 #pragma unroll
         for (int i = 0; i < Sh::COLS; i += 4) {
-          const float4 v = make_float4(o[i] * inv, o[i + 1] * inv, o[i + 2] * inv, o[i + 3] * inv);
-          odd |= !(fabsf(o[i]) < CUDART_INF_F && fabsf(o[i + 1]) < CUDART_INF_F && fabsf(o[i + 2]) < CUDART_INF_F && fabsf(o[i + 3]) < CUDART_INF_F);
-          if (col0 + i < p.hd) __stcg(reinterpret_cast<float4*>(dst + i), v);
+          const float4 v = make_float4(o[i / 2].x, o[i / 2].y, o[i / 2 + 1].x, o[i / 2 + 1].y);
+          odd |= !(fabsf(v.x) < CUDART_INF_F && fabsf(v.y) < CUDART_INF_F && fabsf(v.z) < CUDART_INF_F && fabsf(v.w) < CUDART_INF_F);
+          if (col0 + i < p.hd) __stcg(reinterpret_cast<float4*>(dst + i), make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
         }
-        if (!whole && wg == 1) __stcg(p.part_ml + slot, ml);
-        if (odd && ml.y == ml.y) attn_odd_values(p, c.s, c.seq.q0, c.head, (c.blk.tile0 + (int)(max(st.u0 + first, c.ub) - c.ub)) << Sh::LOG2_TILE,
-                                                      (c.blk.tile0 + (int)(u + 1 - c.ub)) << Sh::LOG2_TILE, BK, attn_full_lo(p, c.seq, c.blk), attn_full_hi(c.seq, c.blk),
-                                                      c.seq.past + c.blk.t0 + row / p.g, col0, Sh::COLS, dst);
+        if (!whole && group == 0) __stcg(p.part_ml + slot, ml);
+        if (odd && L == L)
+          attn_odd_values(p, c.s, c.seq.q0, c.head, (c.blk.tile0 + (int)(st.u0 + first - c.ub)) << Sh::LOG2_TILE, (c.blk.tile0 + (int)(u + 1 - c.ub)) << Sh::LOG2_TILE,
+                          BK, attn_full_lo(p, c.seq, c.blk), attn_full_hi(c.seq, c.blk), c.seq.past + c.blk.t0 + attn_row_token(p, row), col0, Sh::COLS, dst);
       }
-      if (!whole && attn_arrive(p, share, &s_last, tid == 128, 1, 128 * Sh::SUM_GROUPS)) {
-        for (int e = tid - 128; e < n_rows * (HD / 4); e += 128 * Sh::SUM_GROUPS) {
+      if (!whole && attn_arrive(p, share, &s_last, tid == 128 * Sh::W_GROUPS, 1, 128 * Sh::S_GROUPS)) {
+        for (int e = tid - 128 * Sh::W_GROUPS; e < n_rows * (HD / 4); e += 128 * Sh::S_GROUPS) {
           const int r = e / (HD / 4), i = 4 * (e % (HD / 4));
           if (i < p.hd)
-            *reinterpret_cast<float4*>(p.out + (size_t)(c.seq.q0 + c.blk.t0 + r / p.g) * p.out_stride + (size_t)(c.head * p.g + r % p.g) * p.hd + i) =
-                attn_join4<HD>(p, share, 128, r, i);
+            *reinterpret_cast<float4*>(p.out + attn_row_offset(p, c.seq.q0 + c.blk.t0, c.head, r, p.out_stride) + i) = attn_join4<HD>(p, share, 128, r, i);
         }
       }
       first = n + 1;
