@@ -129,6 +129,7 @@ template <int THREADS, int LOG2_TILE>
 __device__ void attn_plan(const AttnParams& p, int* pre, long long* s_warp, AttnStart* st) {
   const int tid = threadIdx.x;
   long long carry = 0;
+#pragma unroll 1
   for (int s0 = 0; s0 < p.n_seq; s0 += THREADS) {
     const int s = s0 + tid;
     const int n = s < p.n_seq ? attn_blocks(attn_load_seq(p, s).q_len, p.tb) : 0;
@@ -144,6 +145,7 @@ __device__ void attn_plan(const AttnParams& p, int* pre, long long* s_warp, Attn
   const int F = pre[p.n_seq];
   const int f0 = (int)((long long)tid * F / THREADS), f1 = (int)((long long)(tid + 1) * F / THREADS);
   int s = 0;
+#pragma unroll 1
   for (int hi = p.n_seq; hi - s > 1;) {  // the last sequence that begins at or before block f0
     const int mid = (s + hi) / 2;
     if (pre[mid] <= f0) s = mid;
@@ -153,6 +155,7 @@ __device__ void attn_plan(const AttnParams& p, int* pre, long long* s_warp, Attn
   if (f0 < f1) {
     int at = s;
     AttnSeq q = attn_load_seq(p, at);
+#pragma unroll 1
     for (int f = f0; f < f1; ++f) {
       while (f >= pre[at + 1]) q = attn_load_seq(p, ++at);
       mine += attn_block(q, f - pre[at], p.tb, LOG2_TILE, p.window).ntile;
@@ -172,6 +175,7 @@ __device__ void attn_plan(const AttnParams& p, int* pre, long long* s_warp, Attn
   if (mine > 0 && u0 >= ub && u0 < end * p.n_kv) {
     int at = s;
     AttnSeq q = attn_load_seq(p, at);
+#pragma unroll 1
     for (int f = f0; f < f1; ++f) {
       while (f >= pre[at + 1]) q = attn_load_seq(p, ++at);
       const long long n = (long long)attn_block(q, f - pre[at], p.tb, LOG2_TILE, p.window).ntile * p.n_kv;
@@ -213,6 +217,7 @@ struct AttnCursor {
     if (++head < p.n_kv) return;
     head = 0;
     ++b;
+#pragma unroll 1
     while (b >= attn_blocks(seq.q_len, p.tb)) {
       if (s + 1 >= p.n_seq) return;  // past the line's end: nobody asks for more
       seq = attn_load_seq(p, ++s);
@@ -229,12 +234,15 @@ struct AttnCursor {
 static __device__ __noinline__ void attn_odd_values(const AttnParams& p, int s, int q0, int head, int key0, int key1, int tile, int full_lo, int full_hi, int to,
                                              int col0, int cols, float* dst) {
   const int from = p.window > 0 ? to - p.window : -1;
+#pragma unroll 1
   for (int i = 0; i < cols && col0 + i < p.hd; ++i) {
     const bool came_finite = fabsf(__ldcg(dst + i)) < CUDART_INF_F;
     float add = 0.f;
     bool has = false;
+#pragma unroll 1
     for (int ks = key0; ks < key1 && !(add != add); ks += tile) {
       if (came_finite && ks + tile <= full_hi && ks >= full_lo) continue;
+#pragma unroll 1
       for (int key = max(ks, from + 1); key < ks + tile && key <= to; ++key) {
         const float x = __half2float(attn_value(p, s, q0, head, key)[col0 + i]);
         if (!(fabsf(x) < CUDART_INF_F)) add += x, has = true;
@@ -272,6 +280,7 @@ __device__ __forceinline__ bool attn_arrive(const AttnParams& p, const AttnShare
 template <int HD>
 __device__ __forceinline__ float4 attn_join4(const AttnParams& p, const AttnShare& sh, int item_rows, int r, int i) {
   float M = -CUDART_INF_F;
+#pragma unroll 1
   for (int c = sh.first; c <= sh.last; ++c) M = fmaxf(M, __ldcg(&p.part_ml[(size_t)attn_slot(c, sh) * item_rows + r]).x);
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   float L = 0.f;

@@ -31,8 +31,11 @@ struct TilesShape {
   static constexpr int THREADS = 512;
   static constexpr int SLABS = HD / 64, TILE = BK * HD * 2, QPIECE = 128 * HD * 2;
   static constexpr int STAGES = HD == 64 ? 8 : HD == 128 ? 4 : HD == 192 ? 4 : 2;
-  static constexpr int OBUFS = HD <= 192 ? 2 : 1;
-  static constexpr uint32_t O_COL = 2 * BK;
+  static constexpr int OBUFS = HD == 64 ? 2 : 1;
+  // columns of tensor memory: scores of two tiles, sums, q's pieces (of heads wider than 192 the first)
+  static constexpr uint32_t O_COL = 2 * BK, Q_COL = O_COL + OBUFS * HD;
+  static constexpr int Q_TMEM = HD <= 192 ? 2 : 1;
+  static_assert(Q_COL + Q_TMEM * HD / 2 <= 512, "more columns than tensor memory has");
   static constexpr int SMALL = RING * 128 * 4 + 2 * 2 * RING * 128 * 8 + RING * 128 * 4;  // tiles' maxima, (maximum, weight), score factors
   static constexpr int SMEM = 1024 + 2 * QPIECE + STAGES * TILE + SMALL;
   static_assert(SMEM + 1024 <= 232448, "more shared memory than a CTA has");
@@ -47,7 +50,17 @@ __device__ __forceinline__ void set_regs() {  // from the launch's 128
   if constexpr (N > 128) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
 }
 
+// An item as the roles see it: its tiles here, n0 .. n1 - 1 of the CTA's.
+struct __align__(16) TileItem {
+  int n0, n1, row0, n_rows;          // first row of the call, rows (tokens x heads)
+  int key0, lo, hi, pos0;            // first key of its first tile here; keys that some row sees; position of its first token
+  int full_lo, full_hi, head, s;     // keys that every row sees
+  int q0, whole, first_cta, last_cta;  // the sequence's first row; no other CTA has tiles of it; the CTAs that have
+};
+constexpr int ITEMS = 16;  // the copies are at most nine items ahead of the sums
+
 struct TileBars {
+  uint64_t i_full[ITEMS];
   uint64_t full[8], empty[8];  // tiles of K and V, in the order K0 K1 V0 K2 V1 ...
   uint64_t s_full[2], p_full[2];
   uint64_t o_full[2], o_empty[2];
@@ -58,9 +71,9 @@ struct TileBars {
 };
 
 // Whether some row of the item does not see some key of [ks, ks + n).
-__device__ __forceinline__ bool tile_masked(const AttnParams& p, const AttnSeq& seq, const AttnBlock& blk, int ks, int n) {
-  return ks + n > attn_full_hi(seq, blk) || ks < attn_full_lo(p, seq, blk);
-}
+__device__ __forceinline__ bool tile_masked(const TileItem& it, int ks, int n) { return ks + n > it.full_hi || ks < it.full_lo; }
+
+__device__ __forceinline__ bool wait_all(uint64_t* bar, int phase) { return __all_sync(0xFFFFFFFFu, mbar_wait_bounded(bar, (uint32_t)phase & 1)); }
 
 // Bit i: whether the key k0 + i is in (from, to].
 __device__ __forceinline__ uint32_t seen_keys(int k0, int from, int to) {
@@ -75,6 +88,7 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
   constexpr int BK = Sh::BK, SLABS = Sh::SLABS, STAGES = Sh::STAGES, OBUFS = Sh::OBUFS, TILE = Sh::TILE;
   extern __shared__ unsigned char smem_raw[];
   __shared__ TileBars bars;
+  __shared__ TileItem s_item[ITEMS];
   __shared__ long long s_scan[Sh::THREADS / 32];
   __shared__ AttnStart s_start;
   __shared__ uint32_t s_tmem;
@@ -88,6 +102,7 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
   const int wg = warp >> 2, role = wg == 3 ? 3 + (warp & 3) : wg < Sh::W_GROUPS ? 0 : 1;  // 0 weights, 1 sums, 3 copies, 4 MMAs, 5 and 6 hidden keys
 
   if (tid == 0) {
+    for (int i = 0; i < ITEMS; ++i) mbar_init(bars.i_full + i, 1);
     for (int i = 0; i < 8; ++i) mbar_init(bars.full + i, 1), mbar_init(bars.empty + i, 1);
     for (int i = 0; i < 2; ++i) mbar_init(bars.s_full + i, 1), mbar_init(bars.p_full + i, 4), mbar_init(bars.o_full + i, 1), mbar_init(bars.o_empty + i, 4 * Sh::S_GROUPS);
     for (int i = 0; i < RING; ++i) mbar_init(bars.a_full + i, 4), mbar_init(bars.f_full + i, 4), mbar_init(bars.q_empty + i, 1);
@@ -111,25 +126,23 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
   if (N == 0) {
     // nothing to do
   } else if (role == 3) {
-    // ---- copies
-    AttnCursor<Sh::LOG2_TILE> kc, vc;
-    kc.start(p, st);
-    vc = kc;
+    // ---- copies, and the items' words
+    AttnCursor<Sh::LOG2_TILE> c;
+    c.start(p, st);
     const int pieces = BK / granule;
     const bool packed = p.page_table == nullptr;
-    int asked = 0;
-    auto load = [&](AttnCursor<Sh::LOG2_TILE>& c, int n, const CUtensorMap* map) {
-      const long long u = st.u0 + n;
-      while (u >= c.ub + c.blk.ntile) c.next(p);
-      const int ks = (c.blk.tile0 + (int)(u - c.ub)) << Sh::LOG2_TILE, key = ks + lane * granule;
-      const bool has = lane < pieces && key < c.blk.hi && key + granule > c.blk.lo;
-      int y = c.seq.q0 + key, w = 0;
+    int asked = 0, k_item = -1, v_item = 0;
+    auto load = [&](const TileItem& it, int n, const CUtensorMap* map) {
+      const int key = it.key0 + ((n - it.n0) << Sh::LOG2_TILE) + lane * granule;
+      const bool has = lane < pieces && key < it.hi && key + granule > it.lo;
+      int y = it.q0 + key, w = 0;
       if (has && !packed) {
-        w = attn_page(p, c.s, key / p.page_size);
-        y = key % p.page_size;
+        const int page = key / p.page_size;
+        w = attn_page(p, it.s, page);
+        y = key - page * p.page_size;
       }
       const int stage = asked % STAGES;
-      if (asked >= STAGES) ok = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(bars.empty + stage, (asked / STAGES - 1) & 1));
+      if (asked >= STAGES) ok = wait_all(bars.empty + stage, asked / STAGES - 1);
       if (!ok) return;
       const int count = __popc(__ballot_sync(0xFFFFFFFFu, has));
       if (lane == 0) mbar_arrive_expect_tx(bars.full + stage, (uint32_t)(count * granule * 128 * SLABS));
@@ -137,15 +150,37 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
       if (has) {
         unsigned char* dst = s_kv + stage * TILE + lane * granule * 128;
 #pragma unroll
-        for (int s = 0; s < SLABS; ++s) tma_load_4d(dst + s * (BK * 128), map, 64 * s, y, c.head, w, bars.full + stage);
+        for (int s = 0; s < SLABS; ++s) tma_load_4d(dst + s * (BK * 128), map, 64 * s, y, it.head, w, bars.full + stage);
       }
       __syncwarp();
       ++asked;
     };
-    load(kc, 0, &kmap);
-    for (int n = 0; n < N && ok; ++n) {
-      if (n + 1 < N) load(kc, n + 1, &kmap);
-      if (ok) load(vc, n, &vmap);
+#pragma unroll 1
+    for (int n = -1; n < N && ok; ++n) {  // K of tile n + 1, V of tile n
+      if (n + 1 < N) {
+        const long long u = st.u0 + n + 1;
+        if (k_item < 0 || u >= c.ub + c.blk.ntile) {
+          if (k_item >= 0) c.next(p);
+          ++k_item;
+          if (lane == 0) {
+            TileItem& it = s_item[k_item % ITEMS];
+            const long long end = c.ub + c.blk.ntile;
+            const AttnShare sh = attn_share(c.ub, c.blk.ntile, st);
+            it.n0 = n + 1, it.n1 = (int)((end < st.u1 ? end : st.u1) - st.u0);
+            it.row0 = c.seq.q0 + c.blk.t0, it.n_rows = c.blk.nt * p.g;
+            it.key0 = (c.blk.tile0 + (int)(u - c.ub)) << Sh::LOG2_TILE, it.lo = c.blk.lo, it.hi = c.blk.hi, it.pos0 = c.seq.past + c.blk.t0;
+            it.full_lo = attn_full_lo(p, c.seq, c.blk), it.full_hi = attn_full_hi(c.seq, c.blk), it.head = c.head, it.s = c.s;
+            it.q0 = c.seq.q0, it.whole = sh.first == sh.last, it.first_cta = sh.first, it.last_cta = sh.last;
+            mbar_arrive(bars.i_full + k_item % ITEMS);
+          }
+          __syncwarp();
+        }
+        load(s_item[k_item % ITEMS], n + 1, &kmap);
+      }
+      if (n >= 0 && ok) {
+        if (n == s_item[v_item % ITEMS].n1) ++v_item;
+        load(s_item[v_item % ITEMS], n, &vmap);
+      }
     }
     if (!ok) {
       if (lane == 0) atomicExch(&p.status->timeout, 11);
@@ -153,66 +188,83 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
       for (int i = max(0, asked - STAGES); i < asked; ++i) mbar_wait_bounded(bars.full + i % STAGES, (i / STAGES) & 1);
     }
   } else if (role == 4) {
-    // ---- MMAs
-    AttnCursor<Sh::LOG2_TILE> ic, cc;  // of the tile whose scores come next, and of the one whose sums do
-    ic.start(p, st);
-    cc = ic;
+    // ---- MMAs.  Scores run one tile ahead of the sums; their accumulators are free by then, since MMAs of one thread go in order
     const uint32_t idesc_s = umma::idesc_f16_f32(128, BK), idesc_o = umma::idesc_f16_f32(128, HD) | umma::IDESC_B_MN_MAJOR;
-    const uint32_t kva = smem_u32(s_kv);
-    int issued = 0, items = 0, asks = 0;
-    bool starts = true;  // the next tile of scores is its item's first here
+    const uint32_t kva = smem_u32(s_kv), tq = tmem + Sh::Q_COL;
+    const uint64_t qdesc = umma::smem_desc_k_major_swz128(s_q, 0), kdesc = umma::smem_desc_k_major_swz128(s_kv, 0);
+    const uint64_t vdesc = umma::smem_desc_mn_major_swz128(kva, 0, BK * 128);
+    int issued = 0, s_it = 0, v_it = 0, asks = 0;
+    int s_end = 0, v_end = 0, key = 0, full_lo = 0, full_hi = 0;  // ends of the items that scores and sums are in
+#pragma unroll 1
     for (int n = 0; n < N && ok; ++n) {
-      // scores: one tile ahead, but not into the next item, whose q may still be on its way while this one's sums are due
-      while (issued < N && issued <= n + 1 && (issued == n || !starts)) {
-        if (starts) {
-          ok = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(&bars.q_full, items & 1));
-          ++items;
+#pragma unroll 1
+      while (issued < N && issued <= n + 1) {
+        // (not into the next item while this one's sums are due and its q is not there)
+        if (issued == s_end) {
+          if (issued > n && !mbar_try_wait(&bars.q_full, s_it & 1)) break;
+          ok = wait_all(bars.i_full + s_it % ITEMS, s_it / ITEMS) && wait_all(&bars.q_full, s_it);
+          if (!ok) break;
+          s_end = s_item[s_it % ITEMS].n1;
+          ++s_it;
+          umma::fence_after_sync();
+          if (umma::elect_one()) {
+#pragma unroll 1
+            for (int piece = 0; piece < Sh::Q_TMEM; ++piece)
+#pragma unroll 4
+              for (int k = 0; k < HD / 16; ++k)
+                umma::copy1_128x256b(tq + piece * (HD / 2) + 8 * k, qdesc + (uint64_t)((piece * Sh::QPIECE + (k >> 2) * 16384 + (k & 3) * 32) >> 4));
+            if (Sh::Q_TMEM == 2) umma::commit1(bars.q_empty + ((s_it - 1) & (RING - 1)));
+          }
+          __syncwarp();
         }
         const int i = issued == 0 ? 0 : 2 * issued - 1, stage = i % STAGES;
-        ok = ok && __all_sync(0xFFFFFFFFu, mbar_wait_bounded(bars.full + stage, (i / STAGES) & 1));
+        ok = wait_all(bars.full + stage, i / STAGES);
         if (!ok) break;
         umma::fence_after_sync();
-        const long long u = st.u0 + issued;
-        const bool last = u + 1 >= ic.ub + ic.blk.ntile || issued + 1 == N;
         if (umma::elect_one()) {
           const uint32_t d = tmem + (issued & 1) * BK;
-#pragma unroll
+          const uint64_t kd = kdesc + (uint64_t)((stage * TILE) >> 4);
+#pragma unroll 1
           for (int piece = 0; piece < 2; ++piece)
-#pragma unroll
+#pragma unroll 4
             for (int k = 0; k < HD / 16; ++k) {
-              const uint64_t a = umma::smem_desc_k_major_swz128(s_q + piece * Sh::QPIECE + (k >> 2) * 16384, k & 3);
-              const uint64_t b = umma::smem_desc_k_major_swz128(s_kv + stage * TILE + (k >> 2) * (BK * 128), k & 3);
-              umma::mma1_f16_ss(d, a, b, idesc_s, piece + k > 0 ? 1u : 0u);
+              const uint64_t b = kd + (uint64_t)(((k >> 2) * (BK * 128) + (k & 3) * 32) >> 4);
+              if (piece < Sh::Q_TMEM) umma::mma1_f16_ts(d, tq + piece * (HD / 2) + 8 * k, b, idesc_s, piece + k > 0 ? 1u : 0u);
+              else umma::mma1_f16_ss(d, qdesc + (uint64_t)((piece * Sh::QPIECE + (k >> 2) * 16384 + (k & 3) * 32) >> 4), b, idesc_s, 1u);
             }
           umma::commit1(bars.empty + stage);
           umma::commit1(bars.s_full + (issued & 1));
-          if (last) umma::commit1(bars.q_empty + ((items - 1) & (RING - 1)));
+          if (Sh::Q_TMEM == 1 && issued + 1 == s_end) umma::commit1(bars.q_empty + ((s_it - 1) & (RING - 1)));
         }
         __syncwarp();
         ++issued;
-        starts = last;
-        if (u + 1 >= ic.ub + ic.blk.ntile && issued < N) ic.next(p);
       }
       if (!ok) break;
-      const long long u = st.u0 + n;
-      while (u >= cc.ub + cc.blk.ntile) cc.next(p);
+      if (n == v_end) {
+        const TileItem& it = s_item[v_it % ITEMS];
+        ok = wait_all(bars.i_full + v_it % ITEMS, v_it / ITEMS);
+        v_end = it.n1, key = it.key0, full_lo = it.full_lo, full_hi = it.full_hi;
+        ++v_it;
+      }
       const int i = n + 1 < N ? 2 * n + 2 : 2 * N - 1, stage = i % STAGES;
-      const bool masked = tile_masked(p, cc.seq, cc.blk, (cc.blk.tile0 + (int)(u - cc.ub)) << Sh::LOG2_TILE, BK);
-      ok = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(bars.full + stage, (i / STAGES) & 1));
-      if (ok && masked && lane == 0) mbar_arrive(&bars.v_ask);
-      ok = ok && __all_sync(0xFFFFFFFFu, mbar_wait_bounded(bars.p_full + (n & 1), (n >> 1) & 1));
-      if (n >= OBUFS) ok = ok && __all_sync(0xFFFFFFFFu, mbar_wait_bounded(bars.o_empty + n % OBUFS, (n / OBUFS - 1) & 1));
-      if (masked) {
-        ok = ok && __all_sync(0xFFFFFFFFu, mbar_wait_bounded(&bars.v_ok, asks & 1));
+      ok = ok && wait_all(bars.full + stage, i / STAGES);
+      const bool masked = key + BK > full_hi || key < full_lo;
+      key += BK;
+      if (masked && ok) {
+        if (lane == 0) mbar_arrive(&bars.v_ask);
+        ok = wait_all(&bars.v_ok, asks);
         ++asks;
       }
+      ok = ok && wait_all(bars.p_full + (n & 1), n >> 1);
+      if (n >= OBUFS) ok = ok && wait_all(bars.o_empty + n % OBUFS, n / OBUFS - 1);
       if (!ok) break;
       umma::fence_after_sync();
       if (umma::elect_one()) {
         const uint32_t d = tmem + Sh::O_COL + (n % OBUFS) * HD, a = tmem + (n & 1) * BK;
-#pragma unroll
+        const uint64_t vd = vdesc + (uint64_t)((stage * TILE) >> 4);
+#pragma unroll 2
         for (int k = 0; k < BK / 16; ++k) {
-          const uint64_t b = umma::smem_desc_mn_major_swz128(kva + stage * TILE, k, BK * 128);
+          const uint64_t b = vd + (uint64_t)((k * 2048) >> 4);
           const uint32_t ak = a + (k >> 1) * 32 + (k & 1) * 8;  // 32 keys: 16 columns of their weights, 16 of the rest
           umma::mma1_f16_ts(d, ak, b, idesc_o, k > 0 ? 1u : 0u);
           umma::mma1_f16_ts(d, ak + 16, b, idesc_o, 1u);
@@ -227,19 +279,21 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
     // ---- V tiles with hidden keys.  0 x value has to be 0 where a row does not see the key: keys that no row sees become zeros, and so do
     // values that are not finite; the item's end adds these to the rows that see them
     const int at = (warp & 1) * 32 + lane;
-    AttnCursor<Sh::LOG2_TILE> c;
-    c.start(p, st);
-    int asks = 0, item = 0;
+    int asks = 0, item = -1, end = 0;
+    TileItem it;
+#pragma unroll 1
     for (int n = 0; n < N && ok; ++n) {
-      const long long u = st.u0 + n;
-      if (u >= c.ub + c.blk.ntile) {
-        while (u >= c.ub + c.blk.ntile) c.next(p);
+      if (n == end) {
         ++item;
+        ok = wait_all(bars.i_full + item % ITEMS, item / ITEMS);
+        if (!ok) break;
+        it = s_item[item % ITEMS];
+        end = it.n1;
         if (at == 0) s_odd[(item + RING) % (2 * RING)] = 0;
       }
-      const int ks = (c.blk.tile0 + (int)(u - c.ub)) << Sh::LOG2_TILE;
-      if (!tile_masked(p, c.seq, c.blk, ks, BK)) continue;
-      ok = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(&bars.v_ask, asks & 1));
+      const int ks = it.key0 + ((n - it.n0) << Sh::LOG2_TILE);
+      if (!tile_masked(it, ks, BK)) continue;
+      ok = wait_all(&bars.v_ask, asks);
       ++asks;
       if (!ok) break;
       const int i = n + 1 < N ? 2 * n + 2 : 2 * N - 1;
@@ -247,7 +301,7 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
 #pragma unroll 1
       for (int row = at; row < BK * SLABS; row += 64) {
         const int key = ks + (row & (BK - 1));
-        const bool seen = key >= c.blk.lo && key < c.blk.hi;
+        const bool seen = key >= it.lo && key < it.hi;
         unsigned char* base = s_kv + (i % STAGES) * TILE + row * 128;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -269,24 +323,24 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
   } else if (role == 0) {
     // ---- weights: thread = row, every W_GROUPS-th tile
     set_regs<Sh::REG_W>();
-    AttnCursor<Sh::LOG2_TILE> c;
-    c.start(p, st);
     const int row = tid & 127;
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+#pragma unroll 1
     for (int n0 = 0, item = 0; n0 < N && ok; ++item) {
-      while (st.u0 + n0 >= c.ub + c.blk.ntile) c.next(p);
-      const int n1 = (int)((c.ub + c.blk.ntile < st.u1 ? c.ub + c.blk.ntile : st.u1) - st.u0), n_rows = c.blk.nt * p.g;
-      const int slot = item & (RING - 1);
+      ok = wait_all(bars.i_full + item % ITEMS, item / ITEMS);
+      if (!ok) break;
+      const TileItem& it = s_item[item % ITEMS];
+      const int n1 = it.n1, n_rows = it.n_rows, slot = item & (RING - 1);
       if (Sh::W_GROUPS == 1 || (n0 & 1) == wg) {
         // q into two f16 pieces: eight lanes a row; rows past the item's are zeros
-        if (item > 0) ok = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(bars.q_empty + ((item - 1) & (RING - 1)), ((item - 1) / RING) & 1));
+        if (item > 0) ok = wait_all(bars.q_empty + ((item - 1) & (RING - 1)), (item - 1) / RING);
         if (!ok) break;
         const int l8 = lane & 7;
 #pragma unroll(HD == 64 ? 4 : HD == 128 ? 2 : 1)
         for (int r0 = 0; r0 < 128; r0 += 16) {
           const int r = r0 + (row >> 3);
           const bool has = r < n_rows;
-          const float* src = p.q + attn_row_offset(p, c.seq.q0 + c.blk.t0, c.head, has ? r : 0, p.q_stride);
+          const float* src = p.q + attn_row_offset(p, it.row0, it.head, has ? r : 0, p.q_stride);
           float4 v[HD / 32];
           float big = 0.f;
 #pragma unroll
@@ -320,15 +374,16 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
       }
       int n = n0;
       if (Sh::W_GROUPS == 2 && (n & 1) != wg) ++n;
-      if (n < n1) ok = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(bars.f_full + slot, (item / RING) & 1));
+      if (n < n1) ok = wait_all(bars.f_full + slot, item / RING);
       const float f = s_fac[slot * 128 + row];
-      const int to = c.seq.past + c.blk.t0 + (row < n_rows ? attn_row_token(p, row) : c.blk.nt - 1);  // the row sees the keys (from, to]
+      const int to = it.pos0 + (row < n_rows ? attn_row_token(p, row) : 0);  // the row sees the keys (from, to]
       const int from = p.window > 0 ? to - p.window : -1;
       float m = -CUDART_INF_F, l = 0.f;
+#pragma unroll 1
       for (; n < n1 && ok; n += Sh::W_GROUPS) {
-        const int ks = (c.blk.tile0 + (int)(st.u0 + n - c.ub)) << Sh::LOG2_TILE;
-        const bool masked = tile_masked(p, c.seq, c.blk, ks, BK);
-        ok = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(bars.s_full + (n & 1), (n >> 1) & 1));
+        const int ks = it.key0 + ((n - n0) << Sh::LOG2_TILE);
+        const bool masked = tile_masked(it, ks, BK);
+        ok = wait_all(bars.s_full + (n & 1), n >> 1);
         if (!ok) break;
         umma::fence_after_sync();
         if ((warp & 3) * 32 < n_rows) {  // (other rows' weights are whatever is there: they reach those rows' sums only)
@@ -395,28 +450,30 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
   } else {
     // ---- sums: thread = row, COLS of its columns
     set_regs<Sh::REG_S>();
-    AttnCursor<Sh::LOG2_TILE> c;
-    c.start(p, st);
     const int row = tid & 127, group = wg - Sh::W_GROUPS, col0 = group * Sh::COLS;
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16) + Sh::O_COL + col0;
     float2 o[Sh::COLS / 2];
     float M = -CUDART_INF_F;
-    int item = 0, first = 0;
+    int item = -1, first = 0, end = 0, n_rows = 0;
+#pragma unroll 1
     for (int n = 0; n < N && ok; ++n) {
-      const long long u = st.u0 + n;
-      while (u >= c.ub + c.blk.ntile) c.next(p);
+      if (n == end) {
+        ++item;
+        ok = wait_all(bars.i_full + item % ITEMS, item / ITEMS);
+        if (!ok) break;
+        first = n, end = s_item[item % ITEMS].n1, n_rows = s_item[item % ITEMS].n_rows;
+      }
       if (n == first) {
         M = -CUDART_INF_F;
 #pragma unroll
         for (int i = 0; i < Sh::COLS / 2; ++i) o[i] = make_float2(0.f, 0.f);
       }
-      const int n_rows = c.blk.nt * p.g;
       const bool mine = (warp & 3) * 32 < n_rows;
-      ok = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(bars.a_full + (n & (RING - 1)), (n / RING) & 1));
+      ok = wait_all(bars.a_full + (n & (RING - 1)), n / RING);
       const float ref = s_ref[(n & (RING - 1)) * 128 + row], now = fmaxf(M, ref);
       const float a = exp2_rel(M, now), b = exp2_rel(ref, now);
       M = now;
-      ok = ok && __all_sync(0xFFFFFFFFu, mbar_wait_bounded(bars.o_full + n % OBUFS, (n / OBUFS) & 1));
+      ok = ok && wait_all(bars.o_full + n % OBUFS, n / OBUFS);
       if (!ok) break;
       umma::fence_after_sync();
       if (mine) {
@@ -433,11 +490,12 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
       umma::fence_before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive(bars.o_empty + n % OBUFS);
-      if (!(u + 1 >= c.ub + c.blk.ntile || n + 1 == N)) continue;
+      if (n + 1 < end) continue;
 
       // ---- the item's end
-      const bool whole = u + 1 >= c.ub + c.blk.ntile && st.u0 + first <= c.ub;
-      const AttnShare share = attn_share(c.ub, c.blk.ntile, st);
+      const TileItem& it = s_item[item % ITEMS];
+      const bool whole = it.whole;
+      const AttnShare share = {it.first_cta, it.last_cta};
       const bool odd_tiles = *reinterpret_cast<volatile int*>(s_odd + item % (2 * RING)) != 0;
       float L = 0.f;  // the groups' weights, brought to one maximum
 #pragma unroll
@@ -449,7 +507,7 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
       const float2 ml = make_float2(M == -CUDART_INF_F && L != 0.f ? 0.f : M, L);  // (nothing but NaN is a part that counts)
       const size_t slot = (size_t)attn_slot(blockIdx.x, share) * 128 + row;
       const bool mine_row = row < n_rows;
-      float* dst = whole ? p.out + attn_row_offset(p, c.seq.q0 + c.blk.t0, c.head, mine_row ? row : 0, p.out_stride) + col0 : p.part + slot * HD + col0;
+      float* dst = whole ? p.out + attn_row_offset(p, it.row0, it.head, mine_row ? row : 0, p.out_stride) + col0 : p.part + slot * HD + col0;
       if (mine_row) {
         const float inv = !whole ? 1.f : L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
         bool odd = odd_tiles;
@@ -461,18 +519,17 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
         }
         if (!whole && group == 0) __stcg(p.part_ml + slot, ml);
         if (odd && L == L)
-          attn_odd_values(p, c.s, c.seq.q0, c.head, (c.blk.tile0 + (int)(st.u0 + first - c.ub)) << Sh::LOG2_TILE, (c.blk.tile0 + (int)(u + 1 - c.ub)) << Sh::LOG2_TILE,
-                          BK, attn_full_lo(p, c.seq, c.blk), attn_full_hi(c.seq, c.blk), c.seq.past + c.blk.t0 + attn_row_token(p, row), col0, Sh::COLS, dst);
+          attn_odd_values(p, it.s, it.q0, it.head, it.key0, it.key0 + ((end - first) << Sh::LOG2_TILE), BK, it.full_lo, it.full_hi, it.pos0 + attn_row_token(p, row),
+                          col0, Sh::COLS, dst);
       }
       if (!whole && attn_arrive(p, share, &s_last, tid == 128 * Sh::W_GROUPS, 1, 128 * Sh::S_GROUPS)) {
+#pragma unroll 1
         for (int e = tid - 128 * Sh::W_GROUPS; e < n_rows * (HD / 4); e += 128 * Sh::S_GROUPS) {
           const int r = e / (HD / 4), i = 4 * (e % (HD / 4));
           if (i < p.hd)
-            *reinterpret_cast<float4*>(p.out + attn_row_offset(p, c.seq.q0 + c.blk.t0, c.head, r, p.out_stride) + i) = attn_join4<HD>(p, share, 128, r, i);
+            *reinterpret_cast<float4*>(p.out + attn_row_offset(p, it.row0, it.head, r, p.out_stride) + i) = attn_join4<HD>(p, share, 128, r, i);
         }
       }
-      first = n + 1;
-      ++item;
     }
     if (!ok && lane == 0) atomicExch(&p.status->timeout, 11);
   }

@@ -162,6 +162,11 @@ __device__ __forceinline__ void commit1(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
+// 128 rows x 32 bytes of a K-major tile into 8 columns of tensor memory (lane = row), in order with this thread's MMAs.
+__device__ __forceinline__ void copy1_128x256b(uint32_t taddr, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::1.128x256b [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+
 // 32 consecutive columns of every lane's row, asked for; they are there after tmem_ld_wait (which names them, so that no use moves above it).
 __device__ __forceinline__ void tmem_ld_32x32(uint32_t taddr, float (&r)[32]) {
   asm volatile(
