@@ -91,8 +91,7 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t&
   lo = *reinterpret_cast<const uint32_t*>(&l);
 }
 
-// Pairs of f16 bits: whether one is not finite, and the same with those as zeros.
-__device__ __forceinline__ bool any_odd(uint32_t x) { return (x & 0x7C00u) == 0x7C00u || (x & 0x7C000000u) == 0x7C000000u; }
+// A pair of f16 bits with values that are not finite as zeros.
 __device__ __forceinline__ uint32_t only_finite(uint32_t x) {
   if ((x & 0x7C00u) == 0x7C00u) x &= 0xFFFF0000u;
   if ((x & 0x7C000000u) == 0x7C000000u) x &= 0x0000FFFFu;

@@ -4,9 +4,9 @@
 // a pair (row, key) costs 8 hd operations at the f16 rate.
 //
 // One CTA per SM, roles by warpgroup:
-//   weights   a thread per row: scores S from tensor memory -> running maximum -> weights P, back over S as f16 pieces.  Two groups (one for
-//             heads wider than 128, whose products take longer) take the tiles in turn, each with a maximum and a weight of its own; the
-//             group that has an item's first tile turns the item's q into f16 pieces, while the other still has the last item's end
+//   weights   a thread per row and 64 keys (two groups for tiles of 128): scores S from tensor memory -> running maximum -> weights P, back
+//             over S as f16 pieces.  Both groups on one tile: what the MMAs wait for is a tile's weights, and with a tile to each
+//             group these took twice as long (3.3 against 1.7 thousand cycles; the tensor cores' part of a tile is 2.1)
 //   sums      a thread per row: the f32 sums in registers.  Each tile's P V starts from zero in tensor memory and is added here, brought
 //             to a common maximum: an accumulation over thousands of steps in the tensor cores, which truncate, would lose an f32
 //             result's last bits (measured: 1.3e-8 of the result per step)
@@ -26,21 +26,21 @@ constexpr int RING = 4;            // tiles' and items' words in shared memory: 
 template <int HD>
 struct TilesShape {
   static constexpr int LOG2_TILE = HD <= 128 ? 7 : 6, BK = 1 << LOG2_TILE;
-  static constexpr int W_GROUPS = HD <= 128 ? 2 : 1;
+  static constexpr int W_GROUPS = BK / 64;
   static constexpr int S_GROUPS = 3 - W_GROUPS, COLS = HD / S_GROUPS;  // columns of a sums thread
   static constexpr int THREADS = 512;
   static constexpr int SLABS = HD / 64, TILE = BK * HD * 2, QPIECE = 128 * HD * 2;
-  static constexpr int STAGES = HD == 64 ? 8 : HD == 128 ? 4 : HD == 192 ? 4 : 2;
+  static constexpr int STAGES = HD == 64 ? 4 : HD <= 192 ? 2 : 1;  // of V of a tile and K of the next but one, which are used one after the other
   static constexpr int OBUFS = HD == 64 ? 2 : 1;
   // columns of tensor memory: scores of two tiles, sums, q's pieces (of heads wider than 192 the first)
   static constexpr uint32_t O_COL = 2 * BK, Q_COL = O_COL + OBUFS * HD;
   static constexpr int Q_TMEM = HD <= 192 ? 2 : 1;
   static_assert(Q_COL + Q_TMEM * HD / 2 <= 512, "more columns than tensor memory has");
-  static constexpr int SMALL = RING * 128 * 4 + 2 * 2 * RING * 128 * 8 + RING * 128 * 4;  // tiles' maxima, (maximum, weight), score factors
-  static constexpr int SMEM = 1024 + 2 * QPIECE + STAGES * TILE + SMALL;
+  static constexpr int SMALL = (2 * RING + 2 * RING + 2 * W_GROUPS + 2 * RING * W_GROUPS) * 128 * 4;  // rows' words, see the kernel
+  static constexpr int SMEM = 1024 + 2 * QPIECE + STAGES * 2 * TILE + SMALL;
   static_assert(SMEM + 1024 <= 232448, "more shared memory than a CTA has");
   // registers by role: together as many as the launch has
-  static constexpr int REG_W = HD == 64 ? 128 : HD == 128 ? 104 : 136, REG_S = HD == 64 ? 144 : HD == 128 ? 200 : 152, REG_C = HD == 64 ? 112 : HD == 128 ? 104 : 72;
+  static constexpr int REG_W = HD == 64 ? 136 : HD == 128 ? 120 : 136, REG_S = HD == 64 ? 128 : HD == 128 ? 192 : 152, REG_C = HD == 64 ? 104 : 72;
   static_assert(REG_W * W_GROUPS + REG_S * S_GROUPS + REG_C <= 512, "more registers than the launch has");
 };
 
@@ -61,10 +61,10 @@ constexpr int ITEMS = 16;  // the copies are at most nine items ahead of the sum
 
 struct TileBars {
   uint64_t i_full[ITEMS];
-  uint64_t full[8], empty[8];  // tiles of K and V, in the order K0 K1 V0 K2 V1 ...
-  uint64_t s_full[2], p_full[2];
-  uint64_t o_full[2], o_empty[2];
-  uint64_t a_full[RING];       // a tile's maxima (and, at an item's end, maximum and weight)
+  uint64_t full[4], empty[4];  // stages of K and V
+  uint64_t s_full[2], ready[2];  // scores; weights there and the sums' columns free
+  uint64_t o_full[2];
+  uint64_t a_full[RING];       // a tile's maxima (and, at an item's end, weights)
   uint64_t f_full[RING];       // an item's score factors
   uint64_t q_full, q_empty[RING];
   uint64_t v_ask, v_ok;        // a V tile with hidden keys: there, and looked after
@@ -95,18 +95,20 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
   __shared__ int s_last, s_odd[2 * RING];
   unsigned char* s_q = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   unsigned char* s_kv = s_q + 2 * Sh::QPIECE;
-  float* s_ref = reinterpret_cast<float*>(s_kv + STAGES * TILE);        // [RING][128]
-  float* s_fac = s_ref + RING * 128;                                    // [RING][128]
-  float2* s_ml = reinterpret_cast<float2*>(s_fac + RING * 128);         // [2 RING][2][128]
+  float* s_ref = reinterpret_cast<float*>(s_kv + STAGES * 2 * TILE);   // [RING][128] running maximum after a tile
+  float* s_fac = s_ref + RING * 128;                               // [RING][128] score factors by item
+  float* s_end = s_fac + RING * 128;                               // [2 RING][128] running maximum at an item's end
+  float* s_l = s_end + 2 * RING * 128;                             // [2 RING][W_GROUPS][128] weights then
+  float* s_max = s_l + 2 * RING * Sh::W_GROUPS * 128;              // [2][W_GROUPS][128] a tile's maxima by group
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int wg = warp >> 2, role = wg == 3 ? 3 + (warp & 3) : wg < Sh::W_GROUPS ? 0 : 1;  // 0 weights, 1 sums, 3 copies, 4 MMAs, 5 and 6 hidden keys
 
   if (tid == 0) {
     for (int i = 0; i < ITEMS; ++i) mbar_init(bars.i_full + i, 1);
-    for (int i = 0; i < 8; ++i) mbar_init(bars.full + i, 1), mbar_init(bars.empty + i, 1);
-    for (int i = 0; i < 2; ++i) mbar_init(bars.s_full + i, 1), mbar_init(bars.p_full + i, 4), mbar_init(bars.o_full + i, 1), mbar_init(bars.o_empty + i, 4 * Sh::S_GROUPS);
-    for (int i = 0; i < RING; ++i) mbar_init(bars.a_full + i, 4), mbar_init(bars.f_full + i, 4), mbar_init(bars.q_empty + i, 1);
-    mbar_init(&bars.q_full, 4), mbar_init(&bars.v_ask, 1), mbar_init(&bars.v_ok, 2);
+    for (int i = 0; i < 4; ++i) mbar_init(bars.full + i, 1), mbar_init(bars.empty + i, 1);
+    for (int i = 0; i < 2; ++i) mbar_init(bars.s_full + i, 1), mbar_init(bars.ready + i, 4 * (Sh::W_GROUPS + Sh::S_GROUPS)), mbar_init(bars.o_full + i, 1);
+    for (int i = 0; i < RING; ++i) mbar_init(bars.a_full + i, 4 * Sh::W_GROUPS), mbar_init(bars.f_full + i, 4 * Sh::W_GROUPS), mbar_init(bars.q_empty + i, 1);
+    mbar_init(&bars.q_full, 4 * Sh::W_GROUPS), mbar_init(&bars.v_ask, 1), mbar_init(&bars.v_ok, 2);
     mbar_fence_init();
   }
   if (tid < 2 * RING) s_odd[tid] = 0;
@@ -131,34 +133,23 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
     c.start(p, st);
     const int pieces = BK / granule;
     const bool packed = p.page_table == nullptr;
-    int asked = 0, k_item = -1, v_item = 0;
-    auto load = [&](const TileItem& it, int n, const CUtensorMap* map) {
+    int k_item = -1, v_item = 0, asked = 0;
+    auto place = [&](const TileItem& it, int n, bool& has, int& y, int& w) {  // where this lane's keys of tile n are
       const int key = it.key0 + ((n - it.n0) << Sh::LOG2_TILE) + lane * granule;
-      const bool has = lane < pieces && key < it.hi && key + granule > it.lo;
-      int y = it.q0 + key, w = 0;
+      has = lane < pieces && key < it.hi && key + granule > it.lo;
+      y = it.q0 + key, w = 0;
       if (has && !packed) {
         const int page = key / p.page_size;
         w = attn_page(p, it.s, page);
         y = key - page * p.page_size;
       }
-      const int stage = asked % STAGES;
-      if (asked >= STAGES) ok = wait_all(bars.empty + stage, asked / STAGES - 1);
-      if (!ok) return;
-      const int count = __popc(__ballot_sync(0xFFFFFFFFu, has));
-      if (lane == 0) mbar_arrive_expect_tx(bars.full + stage, (uint32_t)(count * granule * 128 * SLABS));
-      __syncwarp();
-      if (has) {
-        unsigned char* dst = s_kv + stage * TILE + lane * granule * 128;
-#pragma unroll
-        for (int s = 0; s < SLABS; ++s) tma_load_4d(dst + s * (BK * 128), map, 64 * s, y, it.head, w, bars.full + stage);
-      }
-      __syncwarp();
-      ++asked;
     };
 #pragma unroll 1
-    for (int n = -1; n < N && ok; ++n) {  // K of tile n + 1, V of tile n
-      if (n + 1 < N) {
-        const long long u = st.u0 + n + 1;
+    for (int n = -2; n < N && ok; ++n) {  // K of tile n + 2, V of tile n
+      bool has_k = false, has_v = false;
+      int ky = 0, kw = 0, vy = 0, vw = 0, k_head = 0, v_head = 0;
+      if (n + 2 < N) {
+        const long long u = st.u0 + n + 2;
         if (k_item < 0 || u >= c.ub + c.blk.ntile) {
           if (k_item >= 0) c.next(p);
           ++k_item;
@@ -166,21 +157,46 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
             TileItem& it = s_item[k_item % ITEMS];
             const long long end = c.ub + c.blk.ntile;
             const AttnShare sh = attn_share(c.ub, c.blk.ntile, st);
-            it.n0 = n + 1, it.n1 = (int)((end < st.u1 ? end : st.u1) - st.u0);
+            it.n0 = n + 2, it.n1 = (int)((end < st.u1 ? end : st.u1) - st.u0);
             it.row0 = c.seq.q0 + c.blk.t0, it.n_rows = c.blk.nt * p.g;
             it.key0 = (c.blk.tile0 + (int)(u - c.ub)) << Sh::LOG2_TILE, it.lo = c.blk.lo, it.hi = c.blk.hi, it.pos0 = c.seq.past + c.blk.t0;
             it.full_lo = attn_full_lo(p, c.seq, c.blk), it.full_hi = attn_full_hi(c.seq, c.blk), it.head = c.head, it.s = c.s;
             it.q0 = c.seq.q0, it.whole = sh.first == sh.last, it.first_cta = sh.first, it.last_cta = sh.last;
             mbar_arrive(bars.i_full + k_item % ITEMS);
           }
+          // its q on the way to L2, a few tiles before it is turned into pieces
+          for (int t = lane; t < c.blk.nt; t += 32)
+            asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p.q + (size_t)(c.seq.q0 + c.blk.t0 + t) * p.q_stride + (size_t)c.head * p.g * p.hd),
+                         "r"(p.g * p.hd * 4) : "memory");
           __syncwarp();
         }
-        load(s_item[k_item % ITEMS], n + 1, &kmap);
+        const TileItem& it = s_item[k_item % ITEMS];
+        place(it, n + 2, has_k, ky, kw);
+        k_head = it.head;
       }
-      if (n >= 0 && ok) {
+      if (n >= 0) {
         if (n == s_item[v_item % ITEMS].n1) ++v_item;
-        load(s_item[v_item % ITEMS], n, &vmap);
+        const TileItem& it = s_item[v_item % ITEMS];
+        place(it, n, has_v, vy, vw);
+        v_head = it.head;
       }
+      const int stage = asked % STAGES;
+      if (asked >= STAGES) ok = wait_all(bars.empty + stage, asked / STAGES - 1);
+      if (!ok) break;
+      const int count = __popc(__ballot_sync(0xFFFFFFFFu, has_k)) + __popc(__ballot_sync(0xFFFFFFFFu, has_v));
+      if (lane == 0) mbar_arrive_expect_tx(bars.full + stage, (uint32_t)(count * granule * 128 * SLABS));
+      __syncwarp();
+      unsigned char* dst = s_kv + stage * 2 * TILE + lane * granule * 128;
+      if (has_v) {
+#pragma unroll
+        for (int s = 0; s < SLABS; ++s) tma_load_4d(dst + TILE + s * (BK * 128), &vmap, 64 * s, vy, v_head, vw, bars.full + stage);
+      }
+      if (has_k) {
+#pragma unroll
+        for (int s = 0; s < SLABS; ++s) tma_load_4d(dst + s * (BK * 128), &kmap, 64 * s, ky, k_head, kw, bars.full + stage);
+      }
+      __syncwarp();
+      ++asked;
     }
     if (!ok) {
       if (lane == 0) atomicExch(&p.status->timeout, 11);
@@ -192,17 +208,49 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
     const uint32_t idesc_s = umma::idesc_f16_f32(128, BK), idesc_o = umma::idesc_f16_f32(128, HD) | umma::IDESC_B_MN_MAJOR;
     const uint32_t kva = smem_u32(s_kv), tq = tmem + Sh::Q_COL;
     const uint64_t qdesc = umma::smem_desc_k_major_swz128(s_q, 0), kdesc = umma::smem_desc_k_major_swz128(s_kv, 0);
-    const uint64_t vdesc = umma::smem_desc_mn_major_swz128(kva, 0, BK * 128);
-    int issued = 0, s_it = 0, v_it = 0, asks = 0;
+    const uint64_t vdesc = umma::smem_desc_mn_major_swz128(kva + TILE, 0, BK * 128);
+    int s_it = 0, v_it = 0, asks = 0;
     int s_end = 0, v_end = 0, key = 0, full_lo = 0, full_hi = 0;  // ends of the items that scores and sums are in
+    // Step n: the sums of tile n, then the scores of tile n + 2, whose accumulators are free by then: MMAs of one thread go in order.  What
+    // is not there before a step is waited for behind the last step's MMAs.
 #pragma unroll 1
-    for (int n = 0; n < N && ok; ++n) {
-#pragma unroll 1
-      while (issued < N && issued <= n + 1) {
-        // (not into the next item while this one's sums are due and its q is not there)
-        if (issued == s_end) {
-          if (issued > n && !mbar_try_wait(&bars.q_full, s_it & 1)) break;
-          ok = wait_all(bars.i_full + s_it % ITEMS, s_it / ITEMS) && wait_all(&bars.q_full, s_it);
+    for (int n = -2; n < N && ok; ++n) {
+      const int stage = (n + 2) % STAGES;
+      ok = wait_all(bars.full + stage, (n + 2) / STAGES);
+      if (n >= 0) {
+        if (n == v_end) {
+          const TileItem& it = s_item[v_it % ITEMS];
+          v_end = it.n1, key = it.key0, full_lo = it.full_lo, full_hi = it.full_hi;
+          ++v_it;
+        }
+        const bool masked = key + BK > full_hi || key < full_lo;
+        key += BK;
+        if (masked && ok) {
+          if (lane == 0) mbar_arrive(&bars.v_ask);
+          ok = wait_all(&bars.v_ok, asks);
+          ++asks;
+        }
+        ok = ok && wait_all(bars.ready + (n & 1), n >> 1);
+        if (!ok) break;
+        umma::fence_after_sync();
+        if (umma::elect_one()) {
+          const uint32_t d = tmem + Sh::O_COL + (n % OBUFS) * HD, a = tmem + (n & 1) * BK;
+          const uint64_t vd = vdesc + (uint64_t)((stage * 2 * TILE) >> 4);
+#pragma unroll 2
+          for (int k = 0; k < BK / 16; ++k) {
+            const uint64_t b = vd + (uint64_t)((k * 2048) >> 4);
+            const uint32_t ak = a + (k >> 1) * 32 + (k & 1) * 8;  // 32 keys: 16 columns of their weights, 16 of the rest
+            umma::mma1_f16_ts(d, ak, b, idesc_o, k > 0 ? 1u : 0u);
+            umma::mma1_f16_ts(d, ak + 16, b, idesc_o, 1u);
+          }
+          umma::commit1(bars.o_full + n % OBUFS);
+        }
+        __syncwarp();
+      }
+      const int next = n + 2;
+      if (next < N) {
+        if (next == s_end) {  // an item's q, into tensor memory behind the last item's scores
+          ok = ok && wait_all(bars.i_full + s_it % ITEMS, s_it / ITEMS) && wait_all(&bars.q_full, s_it);
           if (!ok) break;
           s_end = s_item[s_it % ITEMS].n1;
           ++s_it;
@@ -210,20 +258,18 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
           if (umma::elect_one()) {
 #pragma unroll 1
             for (int piece = 0; piece < Sh::Q_TMEM; ++piece)
-#pragma unroll 4
+#pragma unroll 2
               for (int k = 0; k < HD / 16; ++k)
                 umma::copy1_128x256b(tq + piece * (HD / 2) + 8 * k, qdesc + (uint64_t)((piece * Sh::QPIECE + (k >> 2) * 16384 + (k & 3) * 32) >> 4));
             if (Sh::Q_TMEM == 2) umma::commit1(bars.q_empty + ((s_it - 1) & (RING - 1)));
           }
           __syncwarp();
         }
-        const int i = issued == 0 ? 0 : 2 * issued - 1, stage = i % STAGES;
-        ok = wait_all(bars.full + stage, i / STAGES);
         if (!ok) break;
         umma::fence_after_sync();
         if (umma::elect_one()) {
-          const uint32_t d = tmem + (issued & 1) * BK;
-          const uint64_t kd = kdesc + (uint64_t)((stage * TILE) >> 4);
+          const uint32_t d = tmem + (next & 1) * BK;
+          const uint64_t kd = kdesc + (uint64_t)((stage * 2 * TILE) >> 4);
 #pragma unroll 1
           for (int piece = 0; piece < 2; ++piece)
 #pragma unroll 4
@@ -232,46 +278,12 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
               if (piece < Sh::Q_TMEM) umma::mma1_f16_ts(d, tq + piece * (HD / 2) + 8 * k, b, idesc_s, piece + k > 0 ? 1u : 0u);
               else umma::mma1_f16_ss(d, qdesc + (uint64_t)((piece * Sh::QPIECE + (k >> 2) * 16384 + (k & 3) * 32) >> 4), b, idesc_s, 1u);
             }
-          umma::commit1(bars.empty + stage);
-          umma::commit1(bars.s_full + (issued & 1));
-          if (Sh::Q_TMEM == 1 && issued + 1 == s_end) umma::commit1(bars.q_empty + ((s_it - 1) & (RING - 1)));
+          umma::commit1(bars.s_full + (next & 1));
+          if (Sh::Q_TMEM == 1 && next + 1 == s_end) umma::commit1(bars.q_empty + ((s_it - 1) & (RING - 1)));
         }
         __syncwarp();
-        ++issued;
       }
-      if (!ok) break;
-      if (n == v_end) {
-        const TileItem& it = s_item[v_it % ITEMS];
-        ok = wait_all(bars.i_full + v_it % ITEMS, v_it / ITEMS);
-        v_end = it.n1, key = it.key0, full_lo = it.full_lo, full_hi = it.full_hi;
-        ++v_it;
-      }
-      const int i = n + 1 < N ? 2 * n + 2 : 2 * N - 1, stage = i % STAGES;
-      ok = ok && wait_all(bars.full + stage, i / STAGES);
-      const bool masked = key + BK > full_hi || key < full_lo;
-      key += BK;
-      if (masked && ok) {
-        if (lane == 0) mbar_arrive(&bars.v_ask);
-        ok = wait_all(&bars.v_ok, asks);
-        ++asks;
-      }
-      ok = ok && wait_all(bars.p_full + (n & 1), n >> 1);
-      if (n >= OBUFS) ok = ok && wait_all(bars.o_empty + n % OBUFS, n / OBUFS - 1);
-      if (!ok) break;
-      umma::fence_after_sync();
-      if (umma::elect_one()) {
-        const uint32_t d = tmem + Sh::O_COL + (n % OBUFS) * HD, a = tmem + (n & 1) * BK;
-        const uint64_t vd = vdesc + (uint64_t)((stage * TILE) >> 4);
-#pragma unroll 2
-        for (int k = 0; k < BK / 16; ++k) {
-          const uint64_t b = vd + (uint64_t)((k * 2048) >> 4);
-          const uint32_t ak = a + (k >> 1) * 32 + (k & 1) * 8;  // 32 keys: 16 columns of their weights, 16 of the rest
-          umma::mma1_f16_ts(d, ak, b, idesc_o, k > 0 ? 1u : 0u);
-          umma::mma1_f16_ts(d, ak + 16, b, idesc_o, 1u);
-        }
-        umma::commit1(bars.empty + stage);
-        umma::commit1(bars.o_full + n % OBUFS);
-      }
+      if (umma::elect_one()) umma::commit1(bars.empty + stage);
       __syncwarp();
     }
     if (!ok && lane == 0) atomicExch(&p.status->timeout, 11);
@@ -296,21 +308,32 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
       ok = wait_all(&bars.v_ask, asks);
       ++asks;
       if (!ok) break;
-      const int i = n + 1 < N ? 2 * n + 2 : 2 * N - 1;
       bool odd = false;
+      unsigned char* v = s_kv + ((n + 2) % STAGES) * 2 * TILE + TILE;
 #pragma unroll 1
       for (int row = at; row < BK * SLABS; row += 64) {
         const int key = ks + (row & (BK - 1));
         const bool seen = key >= it.lo && key < it.hi;
-        unsigned char* base = s_kv + (i % STAGES) * TILE + row * 128;
+        uint4* w = reinterpret_cast<uint4*>(v + row * 128);
+        uint4 x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = w[(j + row) & 7];
+        __half2 sum = __float2half2_rn(0.f);  // of 0 x value: NaN as soon as one is not finite
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          uint4* w = reinterpret_cast<uint4*>(base + (((j + row) & 7) << 4));
-          const uint4 x = *w;
-          if (!seen) *w = make_uint4(0, 0, 0, 0);
-          else if (any_odd(x.x) || any_odd(x.y) || any_odd(x.z) || any_odd(x.w)) {
-            *w = make_uint4(only_finite(x.x), only_finite(x.y), only_finite(x.z), only_finite(x.w));
-            odd = true;
+          const __half2* h = reinterpret_cast<const __half2*>(x + j);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sum = __hfma2(h[i], __float2half2_rn(0.f), sum);
+        }
+        if (!seen) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) w[(j + row) & 7] = make_uint4(0, 0, 0, 0);
+        } else if (__hisnan(__low2half(sum)) || __hisnan(__high2half(sum))) {
+          odd = true;
+#pragma unroll 1
+          for (int j = 0; j < 8; ++j) {
+            const uint4 y = w[j];
+            w[j] = make_uint4(only_finite(y.x), only_finite(y.y), only_finite(y.z), only_finite(y.w));
           }
         }
       }
@@ -321,109 +344,113 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
     }
     if (!ok && lane == 0) atomicExch(&p.status->timeout, 11);
   } else if (role == 0) {
-    // ---- weights: thread = row, every W_GROUPS-th tile
+    // ---- weights: thread = row, 64 keys of each tile
     set_regs<Sh::REG_W>();
+    constexpr int GROUPS = Sh::W_GROUPS;
     const int row = tid & 127;
-    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t mine = tmem + ((uint32_t)((warp & 3) * 32) << 16) + 64 * wg;
 #pragma unroll 1
-    for (int n0 = 0, item = 0; n0 < N && ok; ++item) {
+    for (int n = 0, item = 0; n < N && ok; ++item) {
       ok = wait_all(bars.i_full + item % ITEMS, item / ITEMS);
       if (!ok) break;
       const TileItem& it = s_item[item % ITEMS];
       const int n1 = it.n1, n_rows = it.n_rows, slot = item & (RING - 1);
-      if (Sh::W_GROUPS == 1 || (n0 & 1) == wg) {
-        // q into two f16 pieces: eight lanes a row; rows past the item's are zeros
-        if (item > 0) ok = wait_all(bars.q_empty + ((item - 1) & (RING - 1)), (item - 1) / RING);
-        if (!ok) break;
-        const int l8 = lane & 7;
-#pragma unroll(HD == 64 ? 4 : HD == 128 ? 2 : 1)
-        for (int r0 = 0; r0 < 128; r0 += 16) {
-          const int r = r0 + (row >> 3);
-          const bool has = r < n_rows;
-          const float* src = p.q + attn_row_offset(p, it.row0, it.head, has ? r : 0, p.q_stride);
-          float4 v[HD / 32];
-          float big = 0.f;
+      // q into two f16 pieces: eight lanes a row, the next rows on their way meanwhile (a rolled loop: code that runs once an item
+      // comes from far away).  What is left in the rows past the item's reaches these rows' sums only.
+      const int l8 = lane & 7;
+      const float* q_item = p.q + (size_t)it.row0 * p.q_stride + (size_t)it.head * p.g * p.hd + 4 * l8;
+      auto load = [&](float4 (&v)[HD / 32], int r) {
+        const float* src = q_item + attn_row_offset(p, 0, 0, r, p.q_stride);
 #pragma unroll
-          for (int j = 0; j < HD / 32; ++j) {
-            const int i = 4 * (l8 + 8 * j);
-            v[j] = has && i < p.hd ? __ldcg(reinterpret_cast<const float4*>(src + i)) : make_float4(0.f, 0.f, 0.f, 0.f);
-          }
+        for (int j = 0; j < HD / 32; ++j)
+          v[j] = r < n_rows && 4 * (l8 + 8 * j) < p.hd ? __ldcg(reinterpret_cast<const float4*>(src + 32 * j)) : make_float4(0.f, 0.f, 0.f, 0.f);
+      };
+      float4 ahead[HD / 32];
+      load(ahead, tid >> 3);
+      if (item > 0) ok = wait_all(bars.q_empty + ((item - 1) & (RING - 1)), (item - 1) / RING);
+      if (!ok) break;
+#pragma unroll 1
+      for (int r = tid >> 3; r - (int)(tid >> 3) < n_rows; r += 16 * GROUPS) {
+        float4 v[HD / 32];
+        float big = 0.f;
 #pragma unroll
-          for (int j = 0; j < HD / 32; ++j) big = fmaxf(big, fmaxf(fmaxf(fabsf(v[j].x), fabsf(v[j].y)), fmaxf(fabsf(v[j].z), fabsf(v[j].w))));
-#pragma unroll
-          for (int x = 1; x < 8; x <<= 1) big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, x));
-          float down, up;
-          attn_row_scale(big, down, up);
-          if (p.scale_log2 < 0.f) down = -down;
-#pragma unroll
-          for (int j = 0; j < HD / 32; ++j) {
-            const int i = 4 * (l8 + 8 * j);
-            uint2 hi, lo;
-            split2(v[j].x * down, v[j].y * down, hi.x, lo.x);
-            split2(v[j].z * down, v[j].w * down, hi.y, lo.y);
-            unsigned char* dst = s_q + (i >> 6) * 16384 + r * 128 + ((((i >> 3) & 7) ^ (r & 7)) << 4) + ((i & 4) << 1);
-            *reinterpret_cast<uint2*>(dst) = hi;
-            *reinterpret_cast<uint2*>(dst + Sh::QPIECE) = lo;
-          }
-          // (not 0: hidden keys' -inf times it stays -inf)
-          if (l8 == 0) s_fac[slot * 128 + r] = fmaxf(up * fabsf(p.scale_log2), 1.2e-38f);
+        for (int j = 0; j < HD / 32; ++j) {
+          v[j] = ahead[j];
+          big = fmaxf(big, fmaxf(fmaxf(fabsf(v[j].x), fabsf(v[j].y)), fmaxf(fabsf(v[j].z), fabsf(v[j].w))));
         }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bars.q_full), mbar_arrive(bars.f_full + slot);
+        if (r + 16 * GROUPS < 128) load(ahead, r + 16 * GROUPS);
+#pragma unroll
+        for (int x = 1; x < 8; x <<= 1) big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, x));
+        float down, up;
+        attn_row_scale(big, down, up);
+        if (p.scale_log2 < 0.f) down = -down;
+#pragma unroll
+        for (int j = 0; j < HD / 32; ++j) {
+          uint2 hi, lo;
+          split2(v[j].x * down, v[j].y * down, hi.x, lo.x);
+          split2(v[j].z * down, v[j].w * down, hi.y, lo.y);
+          unsigned char* dst = s_q + (j >> 1) * 16384 + r * 128 + ((((l8 >> 1) + 4 * (j & 1)) ^ (r & 7)) << 4) + ((l8 & 1) << 3);
+          *reinterpret_cast<uint2*>(dst) = hi;
+          *reinterpret_cast<uint2*>(dst + Sh::QPIECE) = lo;
+        }
+        // (not 0: hidden keys' -inf times it stays -inf)
+        if (l8 == 0) s_fac[slot * 128 + r] = fmaxf(up * fabsf(p.scale_log2), 1.2e-38f);
       }
-      int n = n0;
-      if (Sh::W_GROUPS == 2 && (n & 1) != wg) ++n;
-      if (n < n1) ok = wait_all(bars.f_full + slot, item / RING);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars.q_full), mbar_arrive(bars.f_full + slot);
+      ok = wait_all(bars.f_full + slot, item / RING);
       const float f = s_fac[slot * 128 + row];
       const int to = it.pos0 + (row < n_rows ? attn_row_token(p, row) : 0);  // the row sees the keys (from, to]
       const int from = p.window > 0 ? to - p.window : -1;
+      const bool busy = (warp & 3) * 32 < n_rows;  // (other rows' weights are whatever is there: they reach those rows' sums only)
       float m = -CUDART_INF_F, l = 0.f;
+      int ks = it.key0 + 64 * wg;
 #pragma unroll 1
-      for (; n < n1 && ok; n += Sh::W_GROUPS) {
-        const int ks = it.key0 + ((n - n0) << Sh::LOG2_TILE);
-        const bool masked = tile_masked(it, ks, BK);
+      for (; n < n1 && ok; ++n, ks += BK) {
         ok = wait_all(bars.s_full + (n & 1), n >> 1);
         if (!ok) break;
         umma::fence_after_sync();
-        if ((warp & 3) * 32 < n_rows) {  // (other rows' weights are whatever is there: they reach those rows' sums only)
-          const uint32_t sa = lanes + (n & 1) * BK;
-          float top = -CUDART_INF_F;
-#pragma unroll 1
-          for (int j = 0; j < BK / 32; ++j) {
-            float s[32];
-            umma::tmem_ld_32x32(sa + 32 * j, s);
-            const uint32_t seen = masked ? seen_keys(ks + 32 * j, from, to) : ~0u;
-            umma::tmem_ld_wait(s);
-            if (seen != ~0u) {
+        const uint32_t sa = mine + (n & 1) * BK;
+        float s[2][32];
+        float top = -CUDART_INF_F;
+        if (busy) {
+          umma::tmem_ld_32x32(sa, s[0]);
+          umma::tmem_ld_32x32(sa + 32, s[1]);
+          umma::tmem_ld_wait(s[0]);
+          umma::tmem_ld_wait(s[1]);
+          if (ks + 64 > it.full_hi || ks < it.full_lo) {
+            const uint32_t seen0 = seen_keys(ks, from, to), seen1 = seen_keys(ks + 32, from, to);
 #pragma unroll
-              for (int i = 0; i < 32; ++i) s[i] = (seen >> i) & 1u ? s[i] : -CUDART_INF_F;
+            for (int i = 0; i < 32; ++i) {
+              s[0][i] = (seen0 >> i) & 1u ? s[0][i] : -CUDART_INF_F;
+              s[1][i] = (seen1 >> i) & 1u ? s[1][i] : -CUDART_INF_F;
             }
-            float t[4] = {top, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
-#pragma unroll
-            for (int i = 0; i < 32; i += 2) t[(i >> 1) & 3] = fmaxf(fmaxf(t[(i >> 1) & 3], s[i]), s[i + 1]);
-            top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
           }
-          const float now = fmaxf(m, top * f);
-          l *= exp2_rel(m, now);
-          m = now;
+          float t[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
+#pragma unroll
+          for (int i = 0; i < 32; ++i) t[i & 3] = fmaxf(fmaxf(t[i & 3], s[0][i]), s[1][i]);
+          top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+        }
+        if constexpr (GROUPS == 2) {
+          float* at = s_max + (n & 1) * 256 + row;
+          at[128 * wg] = top;
+          asm volatile("bar.sync 2, 256;" ::: "memory");
+          top = fmaxf(top, at[128 * (wg ^ 1)]);
+        }
+        const float now = fmaxf(m, top * f);
+        l *= exp2_rel(m, now);
+        m = now;
+        if (busy) {
           const float off = TILE_BIAS - (now == -CUDART_INF_F ? 0.f : now);
           const float2 f2 = make_float2(f, f), off2 = make_float2(off, off), minus = make_float2(-1.f, -1.f);
           float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll 1
-          for (int j = 0; j < BK / 32; ++j) {
-            float s[32];
-            umma::tmem_ld_32x32(sa + 32 * j, s);
-            const uint32_t seen = masked ? seen_keys(ks + 32 * j, from, to) : ~0u;
-            umma::tmem_ld_wait(s);
-            if (seen != ~0u) {
 #pragma unroll
-              for (int i = 0; i < 32; ++i) s[i] = (seen >> i) & 1u ? s[i] : -CUDART_INF_F;
-            }
+          for (int j = 0; j < 2; ++j) {
             uint32_t w[32];
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-              const float2 x = __ffma2_rn(make_float2(s[2 * i], s[2 * i + 1]), f2, off2);
+              const float2 x = __ffma2_rn(make_float2(s[j][2 * i], s[j][2 * i + 1]), f2, off2);
               const float2 e = make_float2(exp2_approx(x.x), exp2_approx(x.y));
               sum[i & 1] = __fadd2_rn(sum[i & 1], e);
               // the piece that f16 holds (below 2^-14, 2^-29 of the largest, rounded once more), and the rest
@@ -439,12 +466,14 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
           umma::tmem_st_wait();
         }
         umma::fence_before_sync();
-        s_ref[(n & (RING - 1)) * 128 + row] = m;
-        if (n + Sh::W_GROUPS >= n1) s_ml[((item % (2 * RING)) * 2 + (n & (Sh::W_GROUPS - 1))) * 128 + row] = make_float2(m, l);
+        if (wg == 0) s_ref[(n & (RING - 1)) * 128 + row] = m;
+        if (n + 1 == n1) {
+          s_l[((item % (2 * RING)) * GROUPS + wg) * 128 + row] = l;
+          if (wg == 0) s_end[(item % (2 * RING)) * 128 + row] = m;
+        }
         __syncwarp();
-        if (lane == 0) mbar_arrive(bars.p_full + (n & 1)), mbar_arrive(bars.a_full + (n & (RING - 1)));
+        if (lane == 0) mbar_arrive(bars.ready + (n & 1)), mbar_arrive(bars.a_full + (n & (RING - 1)));
       }
-      n0 = n1;
     }
     if (!ok && lane == 0) atomicExch(&p.status->timeout, 11);
   } else {
@@ -453,8 +482,10 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
     const int row = tid & 127, group = wg - Sh::W_GROUPS, col0 = group * Sh::COLS;
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16) + Sh::O_COL + col0;
     float2 o[Sh::COLS / 2];
-    float M = -CUDART_INF_F;
+    float m = -CUDART_INF_F;
     int item = -1, first = 0, end = 0, n_rows = 0;
+    for (int n = 0; n < OBUFS && n < N; ++n)
+      if (lane == 0) mbar_arrive(bars.ready + (n & 1));
 #pragma unroll 1
     for (int n = 0; n < N && ok; ++n) {
       if (n == end) {
@@ -462,34 +493,31 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
         ok = wait_all(bars.i_full + item % ITEMS, item / ITEMS);
         if (!ok) break;
         first = n, end = s_item[item % ITEMS].n1, n_rows = s_item[item % ITEMS].n_rows;
-      }
-      if (n == first) {
-        M = -CUDART_INF_F;
+        m = -CUDART_INF_F;
 #pragma unroll
         for (int i = 0; i < Sh::COLS / 2; ++i) o[i] = make_float2(0.f, 0.f);
       }
       const bool mine = (warp & 3) * 32 < n_rows;
       ok = wait_all(bars.a_full + (n & (RING - 1)), n / RING);
-      const float ref = s_ref[(n & (RING - 1)) * 128 + row], now = fmaxf(M, ref);
-      const float a = exp2_rel(M, now), b = exp2_rel(ref, now);
-      M = now;
+      const float now = s_ref[(n & (RING - 1)) * 128 + row], a = exp2_rel(m, now);
+      m = now;
       ok = ok && wait_all(bars.o_full + n % OBUFS, n / OBUFS);
       if (!ok) break;
       umma::fence_after_sync();
       if (mine) {
-        const float2 a2 = make_float2(a, a), b2 = make_float2(b, b), zero = make_float2(0.f, 0.f);
+        const float2 a2 = make_float2(a, a);
 #pragma unroll
         for (int j = 0; j < Sh::COLS / 32; ++j) {
           float t[32];
           umma::tmem_ld_32x32(lanes + (n % OBUFS) * HD + 32 * j, t);
           umma::tmem_ld_wait(t);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) o[16 * j + i] = __ffma2_rn(o[16 * j + i], a2, __ffma2_rn(make_float2(t[2 * i], t[2 * i + 1]), b2, zero));
+          for (int i = 0; i < 16; ++i) o[16 * j + i] = __ffma2_rn(o[16 * j + i], a2, make_float2(t[2 * i], t[2 * i + 1]));
         }
       }
       umma::fence_before_sync();
       __syncwarp();
-      if (lane == 0) mbar_arrive(bars.o_empty + n % OBUFS);
+      if (lane == 0 && n + OBUFS < N) mbar_arrive(bars.ready + ((n + OBUFS) & 1));
       if (n + 1 < end) continue;
 
       // ---- the item's end
@@ -497,14 +525,12 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
       const bool whole = it.whole;
       const AttnShare share = {it.first_cta, it.last_cta};
       const bool odd_tiles = *reinterpret_cast<volatile int*>(s_odd + item % (2 * RING)) != 0;
-      float L = 0.f;  // the groups' weights, brought to one maximum
+      float L = 0.f;
 #pragma unroll
-      for (int w = 0; w < Sh::W_GROUPS; ++w)
-        if (n > first || w == (n & (Sh::W_GROUPS - 1))) {
-          const float2 ml = s_ml[((item % (2 * RING)) * 2 + w) * 128 + row];
-          L += ml.y * (ml.y == ml.y ? exp2_rel(ml.x, M) : 1.f);
-        }
-      const float2 ml = make_float2(M == -CUDART_INF_F && L != 0.f ? 0.f : M, L);  // (nothing but NaN is a part that counts)
+      for (int w = 0; w < Sh::W_GROUPS; ++w) L += s_l[((item % (2 * RING)) * Sh::W_GROUPS + w) * 128 + row];
+      float at_end = s_end[(item % (2 * RING)) * 128 + row];
+      if (at_end == -CUDART_INF_F && L != 0.f) at_end = 0.f;  // nothing but NaN is a part that counts
+      const float2 ml = make_float2(at_end, L);
       const size_t slot = (size_t)attn_slot(blockIdx.x, share) * 128 + row;
       const bool mine_row = row < n_rows;
       float* dst = whole ? p.out + attn_row_offset(p, it.row0, it.head, mine_row ? row : 0, p.out_stride) + col0 : p.part + slot * HD + col0;
