@@ -46,6 +46,18 @@ __device__ __forceinline__ void tma_load_4d(void* smem_dst, const CUtensorMap* t
       : "memory");
 }
 
+// mbar_wait_bounded in a tenth of the instructions (its loop is not unrolled): these kernels wait in many places, and their code has to stay
+// in the instruction cache.
+__device__ __forceinline__ bool attn_wait(uint64_t* bar, int phase) {
+#pragma unroll 1
+  for (uint32_t i = 0; i < (1u << 24); ++i) {
+    if (mbar_try_wait(bar, (uint32_t)phase & 1)) return true;
+    if (i > 4096) __nanosleep(64);
+  }
+  return false;
+}
+__device__ __forceinline__ bool wait_all(uint64_t* bar, int phase) { return __all_sync(0xFFFFFFFFu, attn_wait(bar, phase)); }
+
 __device__ __forceinline__ AttnSeq attn_load_seq(const AttnParams& p, int s) {
   bool bad = false;
   const AttnSeq r = attn_seq(__ldcg(p.cu_q + s), __ldcg(p.cu_q + s + 1), p.kv_len != nullptr ? __ldcg(p.kv_len + s) : 0, p.kv_len == nullptr, p.rows, p.cap, &bad);

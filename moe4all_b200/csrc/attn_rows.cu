@@ -175,7 +175,7 @@ __global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
       if (ks >= blk.hi || ks + 16 <= blk.lo) continue;
       const int stage = used % STAGES;
       if (alive) {
-        alive = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(full + stage, (used / STAGES) & 1));
+        alive = wait_all(full + stage, used / STAGES);
         if (!alive && lane == 0) atomicExch(&p.status->timeout, 10);
       }
       if (alive) {
@@ -385,7 +385,7 @@ __global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
   }
   // a warp that gave up has copies in flight: they land before its shared memory is somebody else's
   if (!alive)
-    for (; used < asked; ++used) mbar_wait_bounded(full + used % STAGES, (used / STAGES) & 1);
+    for (; used < asked; ++used) attn_wait(full + used % STAGES, used / STAGES);
 }
 
 template <int HD, int NT>

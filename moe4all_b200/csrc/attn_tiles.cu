@@ -30,14 +30,14 @@ struct TilesShape {
   static constexpr int S_GROUPS = 3 - W_GROUPS, COLS = HD / S_GROUPS;  // columns of a sums thread
   static constexpr int THREADS = 512;
   static constexpr int SLABS = HD / 64, TILE = BK * HD * 2, QPIECE = 128 * HD * 2;
-  static constexpr int STAGES = HD == 64 ? 4 : HD <= 192 ? 2 : 1;  // of V of a tile and K of the next but one, which are used one after the other
+  static constexpr int BUFS = HD == 64 ? 4 : HD <= 192 ? 2 : 1;  // tiles of K, and of V, in shared memory
   static constexpr int OBUFS = HD == 64 ? 2 : 1;
   // columns of tensor memory: scores of two tiles, sums, q's pieces (of heads wider than 192 the first)
   static constexpr uint32_t O_COL = 2 * BK, Q_COL = O_COL + OBUFS * HD;
   static constexpr int Q_TMEM = HD <= 192 ? 2 : 1;
   static_assert(Q_COL + Q_TMEM * HD / 2 <= 512, "more columns than tensor memory has");
   static constexpr int SMALL = (2 * RING + 2 * RING + 2 * W_GROUPS + 2 * RING * W_GROUPS) * 128 * 4;  // rows' words, see the kernel
-  static constexpr int SMEM = 1024 + 2 * QPIECE + STAGES * 2 * TILE + SMALL;
+  static constexpr int SMEM = 1024 + 2 * QPIECE + 2 * BUFS * TILE + SMALL;
   static_assert(SMEM + 1024 <= 232448, "more shared memory than a CTA has");
   // registers by role: together as many as the launch has
   static constexpr int REG_W = HD == 64 ? 136 : HD == 128 ? 120 : 136, REG_S = HD == 64 ? 128 : HD == 128 ? 192 : 152, REG_C = HD == 64 ? 104 : 72;
@@ -61,7 +61,7 @@ constexpr int ITEMS = 16;  // the copies are at most nine items ahead of the sum
 
 struct TileBars {
   uint64_t i_full[ITEMS];
-  uint64_t full[4], empty[4];  // stages of K and V
+  uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4];
   uint64_t s_full[2], ready[2];  // scores; weights there and the sums' columns free
   uint64_t o_full[2];
   uint64_t a_full[RING];       // a tile's maxima (and, at an item's end, weights)
@@ -73,8 +73,6 @@ struct TileBars {
 // Whether some row of the item does not see some key of [ks, ks + n).
 __device__ __forceinline__ bool tile_masked(const TileItem& it, int ks, int n) { return ks + n > it.full_hi || ks < it.full_lo; }
 
-__device__ __forceinline__ bool wait_all(uint64_t* bar, int phase) { return __all_sync(0xFFFFFFFFu, mbar_wait_bounded(bar, (uint32_t)phase & 1)); }
-
 // Bit i: whether the key k0 + i is in (from, to].
 __device__ __forceinline__ uint32_t seen_keys(int k0, int from, int to) {
   const int lo = max(0, from + 1 - k0), n = min(32, to + 1 - k0);  // bits lo .. n - 1
@@ -85,7 +83,7 @@ template <int HD>
 __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
     k_attn_tiles(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ AttnParams p, const int granule) {
   using Sh = TilesShape<HD>;
-  constexpr int BK = Sh::BK, SLABS = Sh::SLABS, STAGES = Sh::STAGES, OBUFS = Sh::OBUFS, TILE = Sh::TILE;
+  constexpr int BK = Sh::BK, SLABS = Sh::SLABS, BUFS = Sh::BUFS, OBUFS = Sh::OBUFS, TILE = Sh::TILE;
   extern __shared__ unsigned char smem_raw[];
   __shared__ TileBars bars;
   __shared__ TileItem s_item[ITEMS];
@@ -94,8 +92,8 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
   __shared__ uint32_t s_tmem;
   __shared__ int s_last, s_odd[2 * RING];
   unsigned char* s_q = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  unsigned char* s_kv = s_q + 2 * Sh::QPIECE;
-  float* s_ref = reinterpret_cast<float*>(s_kv + STAGES * 2 * TILE);   // [RING][128] running maximum after a tile
+  unsigned char *s_k = s_q + 2 * Sh::QPIECE, *s_v = s_k + BUFS * TILE;
+  float* s_ref = reinterpret_cast<float*>(s_v + BUFS * TILE);   // [RING][128] running maximum after a tile
   float* s_fac = s_ref + RING * 128;                               // [RING][128] score factors by item
   float* s_end = s_fac + RING * 128;                               // [2 RING][128] running maximum at an item's end
   float* s_l = s_end + 2 * RING * 128;                             // [2 RING][W_GROUPS][128] weights then
@@ -105,7 +103,7 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
 
   if (tid == 0) {
     for (int i = 0; i < ITEMS; ++i) mbar_init(bars.i_full + i, 1);
-    for (int i = 0; i < 4; ++i) mbar_init(bars.full + i, 1), mbar_init(bars.empty + i, 1);
+    for (int i = 0; i < 4; ++i) mbar_init(bars.k_full + i, 1), mbar_init(bars.k_empty + i, 1), mbar_init(bars.v_full + i, 1), mbar_init(bars.v_empty + i, 1);
     for (int i = 0; i < 2; ++i) mbar_init(bars.s_full + i, 1), mbar_init(bars.ready + i, 4 * (Sh::W_GROUPS + Sh::S_GROUPS)), mbar_init(bars.o_full + i, 1);
     for (int i = 0; i < RING; ++i) mbar_init(bars.a_full + i, 4 * Sh::W_GROUPS), mbar_init(bars.f_full + i, 4 * Sh::W_GROUPS), mbar_init(bars.q_empty + i, 1);
     mbar_init(&bars.q_full, 4 * Sh::W_GROUPS), mbar_init(&bars.v_ask, 1), mbar_init(&bars.v_ok, 2);
@@ -133,91 +131,93 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
     c.start(p, st);
     const int pieces = BK / granule;
     const bool packed = p.page_table == nullptr;
-    int k_item = -1, v_item = 0, asked = 0;
-    auto place = [&](const TileItem& it, int n, bool& has, int& y, int& w) {  // where this lane's keys of tile n are
-      const int key = it.key0 + ((n - it.n0) << Sh::LOG2_TILE) + lane * granule;
-      has = lane < pieces && key < it.hi && key + granule > it.lo;
-      y = it.q0 + key, w = 0;
-      if (has && !packed) {
-        const int page = key / p.page_size;
-        w = attn_page(p, it.s, page);
-        y = key - page * p.page_size;
-      }
+    int item = -1;
+    struct Place {
+      int y, w, head;  // of this lane's keys of a tile; y < 0: none
     };
-#pragma unroll 1
-    for (int n = -2; n < N && ok; ++n) {  // K of tile n + 2, V of tile n
-      bool has_k = false, has_v = false;
-      int ky = 0, kw = 0, vy = 0, vw = 0, k_head = 0, v_head = 0;
-      if (n + 2 < N) {
-        const long long u = st.u0 + n + 2;
-        if (k_item < 0 || u >= c.ub + c.blk.ntile) {
-          if (k_item >= 0) c.next(p);
-          ++k_item;
-          if (lane == 0) {
-            TileItem& it = s_item[k_item % ITEMS];
-            const long long end = c.ub + c.blk.ntile;
-            const AttnShare sh = attn_share(c.ub, c.blk.ntile, st);
-            it.n0 = n + 2, it.n1 = (int)((end < st.u1 ? end : st.u1) - st.u0);
-            it.row0 = c.seq.q0 + c.blk.t0, it.n_rows = c.blk.nt * p.g;
-            it.key0 = (c.blk.tile0 + (int)(u - c.ub)) << Sh::LOG2_TILE, it.lo = c.blk.lo, it.hi = c.blk.hi, it.pos0 = c.seq.past + c.blk.t0;
-            it.full_lo = attn_full_lo(p, c.seq, c.blk), it.full_hi = attn_full_hi(c.seq, c.blk), it.head = c.head, it.s = c.s;
-            it.q0 = c.seq.q0, it.whole = sh.first == sh.last, it.first_cta = sh.first, it.last_cta = sh.last;
-            mbar_arrive(bars.i_full + k_item % ITEMS);
-          }
-          // its q on the way to L2, a few tiles before it is turned into pieces
-          for (int t = lane; t < c.blk.nt; t += 32)
-            asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p.q + (size_t)(c.seq.q0 + c.blk.t0 + t) * p.q_stride + (size_t)c.head * p.g * p.hd),
-                         "r"(p.g * p.hd * 4) : "memory");
-          __syncwarp();
+    // Where tile n is.  Asked a step before its K is due, so that the page's number is there by then; V follows two steps later.
+    auto place = [&](int n) {
+      Place at = {-1, 0, 0};
+      if (n >= N) return at;
+      const long long u = st.u0 + n;
+      if (item < 0 || u >= c.ub + c.blk.ntile) {
+        if (item >= 0) c.next(p);
+        ++item;
+        if (lane == 0) {
+          TileItem& it = s_item[item % ITEMS];
+          const long long end = c.ub + c.blk.ntile;
+          const AttnShare sh = attn_share(c.ub, c.blk.ntile, st);
+          it.n0 = n, it.n1 = (int)((end < st.u1 ? end : st.u1) - st.u0);
+          it.row0 = c.seq.q0 + c.blk.t0, it.n_rows = c.blk.nt * p.g;
+          it.key0 = (c.blk.tile0 + (int)(u - c.ub)) << Sh::LOG2_TILE, it.lo = c.blk.lo, it.hi = c.blk.hi, it.pos0 = c.seq.past + c.blk.t0;
+          it.full_lo = attn_full_lo(p, c.seq, c.blk), it.full_hi = attn_full_hi(c.seq, c.blk), it.head = c.head, it.s = c.s;
+          it.q0 = c.seq.q0, it.whole = sh.first == sh.last, it.first_cta = sh.first, it.last_cta = sh.last;
+          mbar_arrive(bars.i_full + item % ITEMS);
         }
-        const TileItem& it = s_item[k_item % ITEMS];
-        place(it, n + 2, has_k, ky, kw);
-        k_head = it.head;
+        // its q on the way to L2, a few tiles before it is turned into pieces
+#pragma unroll 1
+        for (int t = lane; t < c.blk.nt; t += 32)
+          asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p.q + (size_t)(c.seq.q0 + c.blk.t0 + t) * p.q_stride + (size_t)c.head * p.g * p.hd),
+                       "r"(p.g * p.hd * 4) : "memory");
+        __syncwarp();
       }
-      if (n >= 0) {
-        if (n == s_item[v_item % ITEMS].n1) ++v_item;
-        const TileItem& it = s_item[v_item % ITEMS];
-        place(it, n, has_v, vy, vw);
-        v_head = it.head;
+      at.head = c.head;
+      const int key = ((c.blk.tile0 + (int)(u - c.ub)) << Sh::LOG2_TILE) + lane * granule;
+      if (lane < pieces && key < c.blk.hi && key + granule > c.blk.lo) {
+        at.y = c.seq.q0 + key;
+        if (!packed) {
+          const int page = key / p.page_size;
+          at.w = attn_page(p, c.s, page);
+          at.y = key - page * p.page_size;
+        }
       }
-      const int stage = asked % STAGES;
-      if (asked >= STAGES) ok = wait_all(bars.empty + stage, asked / STAGES - 1);
-      if (!ok) break;
-      const int count = __popc(__ballot_sync(0xFFFFFFFFu, has_k)) + __popc(__ballot_sync(0xFFFFFFFFu, has_v));
-      if (lane == 0) mbar_arrive_expect_tx(bars.full + stage, (uint32_t)(count * granule * 128 * SLABS));
+      return at;
+    };
+    auto load = [&](const Place& at, int n, const CUtensorMap* map, unsigned char* bufs, uint64_t* full, uint64_t* empty) {
+      const int buf = n % BUFS;
+      const int count = __popc(__ballot_sync(0xFFFFFFFFu, at.y >= 0));
+      if (n >= BUFS) ok = wait_all(empty + buf, n / BUFS - 1);
+      if (!ok) return;
+      if (lane == 0) mbar_arrive_expect_tx(full + buf, (uint32_t)(count * granule * 128 * SLABS));
       __syncwarp();
-      unsigned char* dst = s_kv + stage * 2 * TILE + lane * granule * 128;
-      if (has_v) {
+      if (at.y >= 0) {
+        unsigned char* dst = bufs + buf * TILE + lane * granule * 128;
 #pragma unroll
-        for (int s = 0; s < SLABS; ++s) tma_load_4d(dst + TILE + s * (BK * 128), &vmap, 64 * s, vy, v_head, vw, bars.full + stage);
-      }
-      if (has_k) {
-#pragma unroll
-        for (int s = 0; s < SLABS; ++s) tma_load_4d(dst + s * (BK * 128), &kmap, 64 * s, ky, k_head, kw, bars.full + stage);
+        for (int s = 0; s < SLABS; ++s) tma_load_4d(dst + s * (BK * 128), map, 64 * s, at.y, at.head, at.w, full + buf);
       }
       __syncwarp();
-      ++asked;
+    };
+    // V of tile n, K of tile n + 2: the order in which they are used, and in which buffers come free
+    Place v0 = {}, v1 = {}, k = place(0);
+#pragma unroll 1
+    for (int n = -2; n < N && ok; ++n) {
+      if (n >= 0) load(v0, n, &vmap, s_v, bars.v_full, bars.v_empty);
+      v0 = v1, v1 = k;
+      if (n + 2 < N && ok) {
+        load(k, n + 2, &kmap, s_k, bars.k_full, bars.k_empty);
+        k = place(n + 3);
+      }
     }
     if (!ok) {
       if (lane == 0) atomicExch(&p.status->timeout, 11);
-      // copies in flight land before the shared memory is somebody else's
-      for (int i = max(0, asked - STAGES); i < asked; ++i) mbar_wait_bounded(bars.full + i % STAGES, (i / STAGES) & 1);
+      // copies in flight land before the shared memory is somebody else's (waits for what has landed pass; each has its limit)
+      for (int i = 0; i < 2 * BUFS; ++i) attn_wait(bars.k_full + i / 2, i), attn_wait(bars.v_full + i / 2, i);
     }
   } else if (role == 4) {
     // ---- MMAs.  Scores run one tile ahead of the sums; their accumulators are free by then, since MMAs of one thread go in order
     const uint32_t idesc_s = umma::idesc_f16_f32(128, BK), idesc_o = umma::idesc_f16_f32(128, HD) | umma::IDESC_B_MN_MAJOR;
-    const uint32_t kva = smem_u32(s_kv), tq = tmem + Sh::Q_COL;
-    const uint64_t qdesc = umma::smem_desc_k_major_swz128(s_q, 0), kdesc = umma::smem_desc_k_major_swz128(s_kv, 0);
-    const uint64_t vdesc = umma::smem_desc_mn_major_swz128(kva + TILE, 0, BK * 128);
+    const uint32_t tq = tmem + Sh::Q_COL;
+    const uint64_t qdesc = umma::smem_desc_k_major_swz128(s_q, 0), kdesc = umma::smem_desc_k_major_swz128(s_k, 0);
+    const uint64_t vdesc = umma::smem_desc_mn_major_swz128(smem_u32(s_v), 0, BK * 128);
     int s_it = 0, v_it = 0, asks = 0;
     int s_end = 0, v_end = 0, key = 0, full_lo = 0, full_hi = 0;  // ends of the items that scores and sums are in
     // Step n: the sums of tile n, then the scores of tile n + 2, whose accumulators are free by then: MMAs of one thread go in order.  What
     // is not there before a step is waited for behind the last step's MMAs.
 #pragma unroll 1
     for (int n = -2; n < N && ok; ++n) {
-      const int stage = (n + 2) % STAGES;
-      ok = wait_all(bars.full + stage, (n + 2) / STAGES);
       if (n >= 0) {
+        const int buf = n % BUFS;
+        ok = wait_all(bars.v_full + buf, n / BUFS);
         if (n == v_end) {
           const TileItem& it = s_item[v_it % ITEMS];
           v_end = it.n1, key = it.key0, full_lo = it.full_lo, full_hi = it.full_hi;
@@ -235,7 +235,7 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
         umma::fence_after_sync();
         if (umma::elect_one()) {
           const uint32_t d = tmem + Sh::O_COL + (n % OBUFS) * HD, a = tmem + (n & 1) * BK;
-          const uint64_t vd = vdesc + (uint64_t)((stage * 2 * TILE) >> 4);
+          const uint64_t vd = vdesc + (uint64_t)((buf * TILE) >> 4);
 #pragma unroll 2
           for (int k = 0; k < BK / 16; ++k) {
             const uint64_t b = vd + (uint64_t)((k * 2048) >> 4);
@@ -244,6 +244,7 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
             umma::mma1_f16_ts(d, ak + 16, b, idesc_o, 1u);
           }
           umma::commit1(bars.o_full + n % OBUFS);
+          umma::commit1(bars.v_empty + buf);
         }
         __syncwarp();
       }
@@ -265,11 +266,13 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
           }
           __syncwarp();
         }
+        const int buf = next % BUFS;
+        ok = ok && wait_all(bars.k_full + buf, next / BUFS);
         if (!ok) break;
         umma::fence_after_sync();
         if (umma::elect_one()) {
           const uint32_t d = tmem + (next & 1) * BK;
-          const uint64_t kd = kdesc + (uint64_t)((stage * 2 * TILE) >> 4);
+          const uint64_t kd = kdesc + (uint64_t)((buf * TILE) >> 4);
 #pragma unroll 1
           for (int piece = 0; piece < 2; ++piece)
 #pragma unroll 4
@@ -279,12 +282,11 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
               else umma::mma1_f16_ss(d, qdesc + (uint64_t)((piece * Sh::QPIECE + (k >> 2) * 16384 + (k & 3) * 32) >> 4), b, idesc_s, 1u);
             }
           umma::commit1(bars.s_full + (next & 1));
+          umma::commit1(bars.k_empty + buf);
           if (Sh::Q_TMEM == 1 && next + 1 == s_end) umma::commit1(bars.q_empty + ((s_it - 1) & (RING - 1)));
         }
         __syncwarp();
       }
-      if (umma::elect_one()) umma::commit1(bars.empty + stage);
-      __syncwarp();
     }
     if (!ok && lane == 0) atomicExch(&p.status->timeout, 11);
   } else if (role > 4) {
@@ -309,7 +311,7 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
       ++asks;
       if (!ok) break;
       bool odd = false;
-      unsigned char* v = s_kv + ((n + 2) % STAGES) * 2 * TILE + TILE;
+      unsigned char* v = s_v + (n % BUFS) * TILE;
 #pragma unroll 1
       for (int row = at; row < BK * SLABS; row += 64) {
         const int key = ks + (row & (BK - 1));
