@@ -50,7 +50,7 @@ __device__ __forceinline__ void tma_load_4d(void* smem_dst, const CUtensorMap* t
 // in the instruction cache.
 __device__ __forceinline__ bool attn_wait(uint64_t* bar, int phase) {
 #pragma unroll 1
-  for (uint32_t i = 0; i < (1u << 24); ++i) {
+  for (uint32_t i = 0; i < (1u << 22); ++i) {
     if (mbar_try_wait(bar, (uint32_t)phase & 1)) return true;
     if (i > 4096) __nanosleep(64);
   }
@@ -240,26 +240,37 @@ struct AttnCursor {
 
 // Some value that this row sees may not be finite: what the products of pieces made of it (inf times a piece of the other sign, or of zero, is
 // NaN), or left out, in columns col0 .. of the result or part at dst, is put right: the sum of such values.  Columns that came out finite
-// can only miss values of tiles with hidden keys, where they count as zeros.
+// can only miss values of tiles with hidden keys, where they count as zeros.  (Key by key, eight columns at a time: other warps of the CTA
+// wait meanwhile, and their waits have a limit.)
 // key0 .. key1: the keys of this part; full_lo .. full_hi: tiles inside have no hidden keys; to: the row's last key.
 static __device__ __noinline__ void attn_odd_values(const AttnParams& p, int s, int q0, int head, int key0, int key1, int tile, int full_lo, int full_hi, int to,
-                                             int col0, int cols, float* dst) {
+                                                    int col0, int cols, float* dst) {
   const int from = p.window > 0 ? to - p.window : -1;
+  const int n = min(cols, p.hd - col0);
+  bool came_finite = true;
 #pragma unroll 1
-  for (int i = 0; i < cols && col0 + i < p.hd; ++i) {
-    const bool came_finite = fabsf(__ldcg(dst + i)) < CUDART_INF_F;
-    float add = 0.f;
-    bool has = false;
+  for (int i = 0; i < n; ++i) came_finite &= fabsf(__ldcg(dst + i)) < CUDART_INF_F;
+  uint32_t placed[8] = {};  // columns whose result is such a sum by now
 #pragma unroll 1
-    for (int ks = key0; ks < key1 && !(add != add); ks += tile) {
-      if (came_finite && ks + tile <= full_hi && ks >= full_lo) continue;
+  for (int ks = key0; ks < key1; ks += tile) {
+    if (came_finite && ks + tile <= full_hi && ks >= full_lo) continue;
 #pragma unroll 1
-      for (int key = max(ks, from + 1); key < ks + tile && key <= to; ++key) {
-        const float x = __half2float(attn_value(p, s, q0, head, key)[col0 + i]);
-        if (!(fabsf(x) < CUDART_INF_F)) add += x, has = true;
+    for (int key = max(ks, from + 1); key < ks + tile && key <= to; ++key) {
+      const __half* v = attn_value(p, s, q0, head, key) + col0;
+#pragma unroll 1
+      for (int i = 0; i < n; i += 8) {
+        const uint4 x = *reinterpret_cast<const uint4*>(v + i);
+        if (only_finite(x.x) == x.x && only_finite(x.y) == x.y && only_finite(x.z) == x.z && only_finite(x.w) == x.w) continue;
+#pragma unroll 1
+        for (int j = i; j < i + 8; ++j) {
+          const float y = __half2float(v[j]);
+          if (fabsf(y) < CUDART_INF_F) continue;
+          const uint32_t bit = 1u << (j & 31);
+          __stcg(dst + j, placed[j >> 5] & bit ? __ldcg(dst + j) + y : y);
+          placed[j >> 5] |= bit;
+        }
       }
     }
-    if (has) __stcg(dst + i, add);
   }
 }
 

@@ -36,9 +36,12 @@ struct TilesShape {
   static constexpr uint32_t O_COL = 2 * BK, Q_COL = O_COL + OBUFS * HD;
   static constexpr int Q_TMEM = HD <= 192 ? 2 : 1;
   static_assert(Q_COL + Q_TMEM * HD / 2 <= 512, "more columns than tensor memory has");
-  static constexpr int SMALL = (2 * RING + 2 * RING + 2 * W_GROUPS + 2 * RING * W_GROUPS) * 128 * 4;  // rows' words, see the kernel
-  static constexpr int SMEM = 1024 + 2 * QPIECE + 2 * BUFS * TILE + SMALL;
-  static_assert(SMEM + 1024 <= 232448, "more shared memory than a CTA has");
+  // items' words are read at their end, tiles' before: with two sums' buffers the weights may be that far ahead
+  static constexpr int ENDS = OBUFS == 1 ? RING : 2 * RING;
+  static constexpr int OUT_COLS = S_GROUPS == 1 ? 32 : 16, OUT = 4 * S_GROUPS * 32 * OUT_COLS * 4;  // results on their way out, by warp
+  static constexpr int SMALL = (2 * RING + ENDS + 2 * W_GROUPS + ENDS * W_GROUPS) * 128 * 4;          // rows' words, see the kernel
+  static constexpr int SMEM = 1024 + 2 * QPIECE + 2 * BUFS * TILE + OUT + SMALL;
+  static_assert(SMEM + 2048 <= 232448, "more shared memory than a CTA has");
   // registers by role: together as many as the launch has
   static constexpr int REG_W = HD == 64 ? 136 : HD == 128 ? 120 : 136, REG_S = HD == 64 ? 128 : HD == 128 ? 192 : 152, REG_C = HD == 64 ? 104 : 72;
   static_assert(REG_W * W_GROUPS + REG_S * S_GROUPS + REG_C <= 512, "more registers than the launch has");
@@ -62,12 +65,12 @@ constexpr int ITEMS = 16;  // the copies are at most nine items ahead of the sum
 struct TileBars {
   uint64_t i_full[ITEMS];
   uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4];
+  uint64_t v_ok[4];            // a V tile is there and has been looked after
   uint64_t s_full[2], ready[2];  // scores; weights there and the sums' columns free
   uint64_t o_full[2];
   uint64_t a_full[RING];       // a tile's maxima (and, at an item's end, weights)
   uint64_t f_full[RING];       // an item's score factors
   uint64_t q_full, q_empty[RING];
-  uint64_t v_ask, v_ok;        // a V tile with hidden keys: there, and looked after
 };
 
 // Whether some row of the item does not see some key of [ks, ks + n).
@@ -90,26 +93,27 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
   __shared__ long long s_scan[Sh::THREADS / 32];
   __shared__ AttnStart s_start;
   __shared__ uint32_t s_tmem;
-  __shared__ int s_last, s_odd[2 * RING];
+  __shared__ int s_last, s_odd[4 * RING];
   unsigned char* s_q = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   unsigned char *s_k = s_q + 2 * Sh::QPIECE, *s_v = s_k + BUFS * TILE;
-  float* s_ref = reinterpret_cast<float*>(s_v + BUFS * TILE);   // [RING][128] running maximum after a tile
-  float* s_fac = s_ref + RING * 128;                               // [RING][128] score factors by item
-  float* s_end = s_fac + RING * 128;                               // [2 RING][128] running maximum at an item's end
-  float* s_l = s_end + 2 * RING * 128;                             // [2 RING][W_GROUPS][128] weights then
-  float* s_max = s_l + 2 * RING * Sh::W_GROUPS * 128;              // [2][W_GROUPS][128] a tile's maxima by group
+  unsigned char* s_out = s_v + BUFS * TILE;
+  float* s_ref = reinterpret_cast<float*>(s_out + Sh::OUT);   // [RING][128] running maximum after a tile
+  float* s_fac = s_ref + RING * 128;                          // [RING][128] score factors by item
+  float* s_end = s_fac + RING * 128;                          // [ENDS][128] running maximum at an item's end
+  float* s_l = s_end + Sh::ENDS * 128;                        // [ENDS][W_GROUPS][128] weights then
+  float* s_max = s_l + Sh::ENDS * Sh::W_GROUPS * 128;         // [2][W_GROUPS][128] a tile's maxima by group
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int wg = warp >> 2, role = wg == 3 ? 3 + (warp & 3) : wg < Sh::W_GROUPS ? 0 : 1;  // 0 weights, 1 sums, 3 copies, 4 MMAs, 5 and 6 hidden keys
 
   if (tid == 0) {
     for (int i = 0; i < ITEMS; ++i) mbar_init(bars.i_full + i, 1);
-    for (int i = 0; i < 4; ++i) mbar_init(bars.k_full + i, 1), mbar_init(bars.k_empty + i, 1), mbar_init(bars.v_full + i, 1), mbar_init(bars.v_empty + i, 1);
+    for (int i = 0; i < 4; ++i) mbar_init(bars.k_full + i, 1), mbar_init(bars.k_empty + i, 1), mbar_init(bars.v_full + i, 1), mbar_init(bars.v_empty + i, 1), mbar_init(bars.v_ok + i, 2);
     for (int i = 0; i < 2; ++i) mbar_init(bars.s_full + i, 1), mbar_init(bars.ready + i, 4 * (Sh::W_GROUPS + Sh::S_GROUPS)), mbar_init(bars.o_full + i, 1);
     for (int i = 0; i < RING; ++i) mbar_init(bars.a_full + i, 4 * Sh::W_GROUPS), mbar_init(bars.f_full + i, 4 * Sh::W_GROUPS), mbar_init(bars.q_empty + i, 1);
-    mbar_init(&bars.q_full, 4 * Sh::W_GROUPS), mbar_init(&bars.v_ask, 1), mbar_init(&bars.v_ok, 2);
+    mbar_init(&bars.q_full, 4 * Sh::W_GROUPS);
     mbar_fence_init();
   }
-  if (tid < 2 * RING) s_odd[tid] = 0;
+  if (tid < 4 * RING) s_odd[tid] = 0;
   if (warp == 0) umma::tmem_alloc(&s_tmem);
   pdl_wait();
   attn_plan<Sh::THREADS, Sh::LOG2_TILE>(p, reinterpret_cast<int*>(s_q), s_scan, &s_start);
@@ -173,7 +177,8 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
       }
       return at;
     };
-    auto load = [&](const Place& at, int n, const CUtensorMap* map, unsigned char* bufs, uint64_t* full, uint64_t* empty) {
+    int ks = 0, vs = 0;  // copies asked for
+    auto load = [&](const Place& at, int n, int& asked, const CUtensorMap* map, unsigned char* bufs, uint64_t* full, uint64_t* empty) {
       const int buf = n % BUFS;
       const int count = __popc(__ballot_sync(0xFFFFFFFFu, at.y >= 0));
       if (n >= BUFS) ok = wait_all(empty + buf, n / BUFS - 1);
@@ -186,22 +191,24 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
         for (int s = 0; s < SLABS; ++s) tma_load_4d(dst + s * (BK * 128), map, 64 * s, at.y, at.head, at.w, full + buf);
       }
       __syncwarp();
+      asked = n + 1;
     };
     // V of tile n, K of tile n + 2: the order in which they are used, and in which buffers come free
     Place v0 = {}, v1 = {}, k = place(0);
 #pragma unroll 1
     for (int n = -2; n < N && ok; ++n) {
-      if (n >= 0) load(v0, n, &vmap, s_v, bars.v_full, bars.v_empty);
+      if (n >= 0) load(v0, n, vs, &vmap, s_v, bars.v_full, bars.v_empty);
       v0 = v1, v1 = k;
       if (n + 2 < N && ok) {
-        load(k, n + 2, &kmap, s_k, bars.k_full, bars.k_empty);
+        load(k, n + 2, ks, &kmap, s_k, bars.k_full, bars.k_empty);
         k = place(n + 3);
       }
     }
     if (!ok) {
       if (lane == 0) atomicExch(&p.status->timeout, 11);
-      // copies in flight land before the shared memory is somebody else's (waits for what has landed pass; each has its limit)
-      for (int i = 0; i < 2 * BUFS; ++i) attn_wait(bars.k_full + i / 2, i), attn_wait(bars.v_full + i / 2, i);
+      // copies in flight land before the shared memory is somebody else's
+      for (int i = max(0, ks - BUFS); i < ks; ++i) attn_wait(bars.k_full + i % BUFS, i / BUFS);
+      for (int i = max(0, vs - BUFS); i < vs; ++i) attn_wait(bars.v_full + i % BUFS, i / BUFS);
     }
   } else if (role == 4) {
     // ---- MMAs.  Scores run one tile ahead of the sums; their accumulators are free by then, since MMAs of one thread go in order
@@ -209,27 +216,14 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
     const uint32_t tq = tmem + Sh::Q_COL;
     const uint64_t qdesc = umma::smem_desc_k_major_swz128(s_q, 0), kdesc = umma::smem_desc_k_major_swz128(s_k, 0);
     const uint64_t vdesc = umma::smem_desc_mn_major_swz128(smem_u32(s_v), 0, BK * 128);
-    int s_it = 0, v_it = 0, asks = 0;
-    int s_end = 0, v_end = 0, key = 0, full_lo = 0, full_hi = 0;  // ends of the items that scores and sums are in
+    int s_it = 0, s_end = 0;  // items whose scores have begun, and the end of the last one's tiles
     // Step n: the sums of tile n, then the scores of tile n + 2, whose accumulators are free by then: MMAs of one thread go in order.  What
     // is not there before a step is waited for behind the last step's MMAs.
 #pragma unroll 1
     for (int n = -2; n < N && ok; ++n) {
       if (n >= 0) {
         const int buf = n % BUFS;
-        ok = wait_all(bars.v_full + buf, n / BUFS);
-        if (n == v_end) {
-          const TileItem& it = s_item[v_it % ITEMS];
-          v_end = it.n1, key = it.key0, full_lo = it.full_lo, full_hi = it.full_hi;
-          ++v_it;
-        }
-        const bool masked = key + BK > full_hi || key < full_lo;
-        key += BK;
-        if (masked && ok) {
-          if (lane == 0) mbar_arrive(&bars.v_ask);
-          ok = wait_all(&bars.v_ok, asks);
-          ++asks;
-        }
+        ok = wait_all(bars.v_ok + buf, n / BUFS);
         ok = ok && wait_all(bars.ready + (n & 1), n >> 1);
         if (!ok) break;
         umma::fence_after_sync();
@@ -293,7 +287,7 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
     // ---- V tiles with hidden keys.  0 x value has to be 0 where a row does not see the key: keys that no row sees become zeros, and so do
     // values that are not finite; the item's end adds these to the rows that see them
     const int at = (warp & 1) * 32 + lane;
-    int asks = 0, item = -1, end = 0;
+    int item = -1, end = 0;
     TileItem it;
 #pragma unroll 1
     for (int n = 0; n < N && ok; ++n) {
@@ -303,13 +297,15 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
         if (!ok) break;
         it = s_item[item % ITEMS];
         end = it.n1;
-        if (at == 0) s_odd[(item + RING) % (2 * RING)] = 0;
+        if (at == 0) s_odd[(item + 2 * RING) % (4 * RING)] = 0;  // (eight items back: read)
       }
       const int ks = it.key0 + ((n - it.n0) << Sh::LOG2_TILE);
-      if (!tile_masked(it, ks, BK)) continue;
-      ok = wait_all(&bars.v_ask, asks);
-      ++asks;
+      ok = wait_all(bars.v_full + n % BUFS, n / BUFS);
       if (!ok) break;
+      if (!tile_masked(it, ks, BK)) {
+        if (lane == 0) mbar_arrive(bars.v_ok + n % BUFS);
+        continue;
+      }
       bool odd = false;
       unsigned char* v = s_v + (n % BUFS) * TILE;
 #pragma unroll 1
@@ -339,10 +335,10 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
           }
         }
       }
-      if (odd) s_odd[item % (2 * RING)] = 1;
+      if (odd) s_odd[item % (4 * RING)] = 1;
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bars.v_ok);
+      if (lane == 0) mbar_arrive(bars.v_ok + n % BUFS);
     }
     if (!ok && lane == 0) atomicExch(&p.status->timeout, 11);
   } else if (role == 0) {
@@ -361,42 +357,52 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
       // comes from far away).  What is left in the rows past the item's reaches these rows' sums only.
       const int l8 = lane & 7;
       const float* q_item = p.q + (size_t)it.row0 * p.q_stride + (size_t)it.head * p.g * p.hd + 4 * l8;
-      auto load = [&](float4 (&v)[HD / 32], int r) {
-        const float* src = q_item + attn_row_offset(p, 0, 0, r, p.q_stride);
+      constexpr int STEP = 16 * GROUPS, AT_ONCE = HD <= 128 ? 2 : 1;
+      float4 ahead[AT_ONCE][HD / 32];
+      auto load = [&](int r0) {
 #pragma unroll
-        for (int j = 0; j < HD / 32; ++j)
-          v[j] = r < n_rows && 4 * (l8 + 8 * j) < p.hd ? __ldcg(reinterpret_cast<const float4*>(src + 32 * j)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int a = 0; a < AT_ONCE; ++a) {
+          const int r = r0 + a * STEP;
+          const float* src = q_item + attn_row_offset(p, 0, 0, r, p.q_stride);
+#pragma unroll
+          for (int j = 0; j < HD / 32; ++j)
+            ahead[a][j] = r < n_rows && 4 * (l8 + 8 * j) < p.hd ? __ldcg(reinterpret_cast<const float4*>(src + 32 * j)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
       };
-      float4 ahead[HD / 32];
-      load(ahead, tid >> 3);
+      load(tid >> 3);
       if (item > 0) ok = wait_all(bars.q_empty + ((item - 1) & (RING - 1)), (item - 1) / RING);
       if (!ok) break;
 #pragma unroll 1
-      for (int r = tid >> 3; r - (int)(tid >> 3) < n_rows; r += 16 * GROUPS) {
-        float4 v[HD / 32];
-        float big = 0.f;
+      for (int r0 = 0; r0 < n_rows; r0 += AT_ONCE * STEP) {
+        float4 v[AT_ONCE][HD / 32];
 #pragma unroll
-        for (int j = 0; j < HD / 32; ++j) {
-          v[j] = ahead[j];
-          big = fmaxf(big, fmaxf(fmaxf(fabsf(v[j].x), fabsf(v[j].y)), fmaxf(fabsf(v[j].z), fabsf(v[j].w))));
+        for (int a = 0; a < AT_ONCE; ++a)
+#pragma unroll
+          for (int j = 0; j < HD / 32; ++j) v[a][j] = ahead[a][j];
+        if (r0 + AT_ONCE * STEP < n_rows) load(r0 + AT_ONCE * STEP + (tid >> 3));
+#pragma unroll
+        for (int a = 0; a < AT_ONCE; ++a) {
+          const int r = r0 + a * STEP + (tid >> 3);
+          float big = 0.f;
+#pragma unroll
+          for (int j = 0; j < HD / 32; ++j) big = fmaxf(big, fmaxf(fmaxf(fabsf(v[a][j].x), fabsf(v[a][j].y)), fmaxf(fabsf(v[a][j].z), fabsf(v[a][j].w))));
+#pragma unroll
+          for (int x = 1; x < 8; x <<= 1) big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, x));
+          float down, up;
+          attn_row_scale(big, down, up);
+          if (p.scale_log2 < 0.f) down = -down;
+#pragma unroll
+          for (int j = 0; j < HD / 32; ++j) {
+            uint2 hi, lo;
+            split2(v[a][j].x * down, v[a][j].y * down, hi.x, lo.x);
+            split2(v[a][j].z * down, v[a][j].w * down, hi.y, lo.y);
+            unsigned char* dst = s_q + (j >> 1) * 16384 + r * 128 + ((((l8 >> 1) + 4 * (j & 1)) ^ (r & 7)) << 4) + ((l8 & 1) << 3);
+            *reinterpret_cast<uint2*>(dst) = hi;
+            *reinterpret_cast<uint2*>(dst + Sh::QPIECE) = lo;
+          }
+          // (not 0: hidden keys' -inf times it stays -inf)
+          if (l8 == 0) s_fac[slot * 128 + r] = fmaxf(up * fabsf(p.scale_log2), 1.2e-38f);
         }
-        if (r + 16 * GROUPS < 128) load(ahead, r + 16 * GROUPS);
-#pragma unroll
-        for (int x = 1; x < 8; x <<= 1) big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, x));
-        float down, up;
-        attn_row_scale(big, down, up);
-        if (p.scale_log2 < 0.f) down = -down;
-#pragma unroll
-        for (int j = 0; j < HD / 32; ++j) {
-          uint2 hi, lo;
-          split2(v[j].x * down, v[j].y * down, hi.x, lo.x);
-          split2(v[j].z * down, v[j].w * down, hi.y, lo.y);
-          unsigned char* dst = s_q + (j >> 1) * 16384 + r * 128 + ((((l8 >> 1) + 4 * (j & 1)) ^ (r & 7)) << 4) + ((l8 & 1) << 3);
-          *reinterpret_cast<uint2*>(dst) = hi;
-          *reinterpret_cast<uint2*>(dst + Sh::QPIECE) = lo;
-        }
-        // (not 0: hidden keys' -inf times it stays -inf)
-        if (l8 == 0) s_fac[slot * 128 + r] = fmaxf(up * fabsf(p.scale_log2), 1.2e-38f);
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
@@ -470,8 +476,8 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
         umma::fence_before_sync();
         if (wg == 0) s_ref[(n & (RING - 1)) * 128 + row] = m;
         if (n + 1 == n1) {
-          s_l[((item % (2 * RING)) * GROUPS + wg) * 128 + row] = l;
-          if (wg == 0) s_end[(item % (2 * RING)) * 128 + row] = m;
+          s_l[((item % Sh::ENDS) * GROUPS + wg) * 128 + row] = l;
+          if (wg == 0) s_end[(item % Sh::ENDS) * 128 + row] = m;
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(bars.ready + (n & 1)), mbar_arrive(bars.a_full + (n & (RING - 1)));
@@ -526,29 +532,49 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
       const TileItem& it = s_item[item % ITEMS];
       const bool whole = it.whole;
       const AttnShare share = {it.first_cta, it.last_cta};
-      const bool odd_tiles = *reinterpret_cast<volatile int*>(s_odd + item % (2 * RING)) != 0;
+      const bool odd_tiles = *reinterpret_cast<volatile int*>(s_odd + item % (4 * RING)) != 0;
       float L = 0.f;
 #pragma unroll
-      for (int w = 0; w < Sh::W_GROUPS; ++w) L += s_l[((item % (2 * RING)) * Sh::W_GROUPS + w) * 128 + row];
-      float at_end = s_end[(item % (2 * RING)) * 128 + row];
+      for (int w = 0; w < Sh::W_GROUPS; ++w) L += s_l[((item % Sh::ENDS) * Sh::W_GROUPS + w) * 128 + row];
+      float at_end = s_end[(item % Sh::ENDS) * 128 + row];
       if (at_end == -CUDART_INF_F && L != 0.f) at_end = 0.f;  // nothing but NaN is a part that counts
       const float2 ml = make_float2(at_end, L);
       const size_t slot = (size_t)attn_slot(blockIdx.x, share) * 128 + row;
       const bool mine_row = row < n_rows;
-      float* dst = whole ? p.out + attn_row_offset(p, it.row0, it.head, mine_row ? row : 0, p.out_stride) + col0 : p.part + slot * HD + col0;
-      if (mine_row) {
-        const float inv = !whole ? 1.f : L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
-        bool odd = odd_tiles;
+      // (a part's rows lie side by side; the result's are found by the lane that stores them)
+      const float inv = !whole ? 1.f : L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
+      bool odd = odd_tiles;
+      unsigned char* out = s_out + (warp & (4 * Sh::S_GROUPS - 1)) * 32 * Sh::OUT_COLS * 4;
+      constexpr int WORDS = Sh::OUT_COLS / 4, ROWS = 32 / WORDS;  // 16-byte words of a row, rows that a warp stores at once
+      const int first_row = (warp & 3) * 32;
+      if (mine) {
 #pragma unroll
-        for (int i = 0; i < Sh::COLS; i += 4) {
-          const float4 v = make_float4(o[i / 2].x, o[i / 2].y, o[i / 2 + 1].x, o[i / 2 + 1].y);
-          odd |= !(fabsf(v.x) < CUDART_INF_F && fabsf(v.y) < CUDART_INF_F && fabsf(v.z) < CUDART_INF_F && fabsf(v.w) < CUDART_INF_F);
-          if (col0 + i < p.hd) __stcg(reinterpret_cast<float4*>(dst + i), make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+        for (int i0 = 0; i0 < Sh::COLS; i0 += Sh::OUT_COLS) {
+#pragma unroll
+          for (int i = 0; i < Sh::OUT_COLS; i += 4) {
+            const float4 v = make_float4(o[(i0 + i) / 2].x, o[(i0 + i) / 2].y, o[(i0 + i) / 2 + 1].x, o[(i0 + i) / 2 + 1].y);
+            odd |= !(fabsf(v.x) < CUDART_INF_F && fabsf(v.y) < CUDART_INF_F && fabsf(v.z) < CUDART_INF_F && fabsf(v.w) < CUDART_INF_F);
+            *reinterpret_cast<float4*>(out + lane * Sh::OUT_COLS * 4 + ((i / 4 ^ (lane & (WORDS - 1))) << 4)) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+          }
+          __syncwarp();
+          const int word = lane & (WORDS - 1), col = col0 + i0 + 4 * word;
+#pragma unroll 2
+          for (int r = lane / WORDS; r < 32; r += ROWS) {
+            const float4 v = *reinterpret_cast<const float4*>(out + r * Sh::OUT_COLS * 4 + ((word ^ (r & (WORDS - 1))) << 4));
+            const int rr = first_row + r;
+            if (rr < n_rows && col < p.hd)
+              __stcg(reinterpret_cast<float4*>(whole ? p.out + attn_row_offset(p, it.row0, it.head, rr, p.out_stride) + col : p.part + (slot - row + rr) * HD + col), v);
+          }
+          __syncwarp();
         }
-        if (!whole && group == 0) __stcg(p.part_ml + slot, ml);
-        if (odd && L == L)
-          attn_odd_values(p, it.s, it.q0, it.head, it.key0, it.key0 + ((end - first) << Sh::LOG2_TILE), BK, it.full_lo, it.full_hi, it.pos0 + attn_row_token(p, row),
-                          col0, Sh::COLS, dst);
+        if (mine_row && !whole && group == 0) __stcg(p.part_ml + slot, ml);
+        if (__any_sync(0xFFFFFFFFu, mine_row && odd && L == L)) {  // (the rows' stores above are seen by the lanes that put them right)
+          __threadfence();
+          __syncwarp();
+          if (mine_row && odd && L == L)
+            attn_odd_values(p, it.s, it.q0, it.head, it.key0, it.key0 + ((end - first) << Sh::LOG2_TILE), BK, it.full_lo, it.full_hi, it.pos0 + attn_row_token(p, row),
+                            col0, Sh::COLS, whole ? p.out + attn_row_offset(p, it.row0, it.head, row, p.out_stride) + col0 : p.part + slot * HD + col0);
+        }
       }
       if (!whole && attn_arrive(p, share, &s_last, tid == 128 * Sh::W_GROUPS, 1, 128 * Sh::S_GROUPS)) {
 #pragma unroll 1
