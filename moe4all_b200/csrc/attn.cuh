@@ -110,10 +110,11 @@ __device__ __forceinline__ uint32_t only_finite(uint32_t x) {
   return x;
 }
 
-// The first unit's place of a CTA, and the line's length.
+// A CTA's share of the line: its tiles are those at the places [u0, u1).
 struct AttnStart {
-  long long units, u0, u1, ub;  // ub: first unit of the block's first head
-  int s, b, ctas;               // ctas: those with units
+  long long units, u0, u1, ub;  // ub: where the block's first head begins
+  long long before, until;      // tiles ahead of u0 and of u1
+  int s, b, ctas;               // ctas: those that the line is shared by
 };
 
 // Inclusive sum over the block's threads; s_warp: one word per warp.
@@ -136,7 +137,7 @@ __device__ __forceinline__ long long block_scan(long long v, long long* s_warp) 
 
 // Every CTA works the whole line out for itself (a sequence and a few blocks per thread), which costs less than a launch for it.
 // pre: n_seq + 1 words of shared memory, free again after the call.  All threads take part.
-template <int THREADS, int LOG2_TILE>
+template <int THREADS, int LOG2_TILE, int EXTRA>
 __device__ void attn_plan(const AttnParams& p, int* pre, long long* s_warp, AttnStart* st) {
   const int tid = threadIdx.x;
   long long carry = 0;
@@ -174,29 +175,38 @@ __device__ void attn_plan(const AttnParams& p, int* pre, long long* s_warp, Attn
   }
   const long long end = block_scan<THREADS>(mine, s_warp);
   if (tid == THREADS - 1) {
-    st->units = end * p.n_kv;
+    st->units = (end + (long long)EXTRA * F) * p.n_kv;
     st->ctas = (int)(st->units < (long long)gridDim.x ? st->units : (long long)gridDim.x);
     const bool idle = (int)blockIdx.x >= st->ctas;
     st->u0 = idle ? 0 : attn_begin(blockIdx.x, st->units, st->ctas);
     st->u1 = idle ? 0 : attn_begin(blockIdx.x + 1, st->units, st->ctas);
+    st->before = 0;
+    st->until = idle ? 0 : end * p.n_kv;  // (where u1 is the line's end)
   }
   __syncthreads();
-  long long ub = (end - mine) * p.n_kv;
-  const long long u0 = st->u0;
-  if (mine > 0 && u0 >= ub && u0 < end * p.n_kv) {
+  // the blocks that u0 and u1 fall into
+  const long long u0 = st->u0, u1 = st->u1;
+  long long tiles = end - mine, ub = (tiles + (long long)EXTRA * f0) * p.n_kv;
+  const long long ue = (end + (long long)EXTRA * f1) * p.n_kv;
+  if (u0 < u1 && ((u0 >= ub && u0 < ue) || (u1 >= ub && u1 < ue))) {
     int at = s;
     AttnSeq q = attn_load_seq(p, at);
 #pragma unroll 1
     for (int f = f0; f < f1; ++f) {
       while (f >= pre[at + 1]) q = attn_load_seq(p, ++at);
-      const long long n = (long long)attn_block(q, f - pre[at], p.tb, LOG2_TILE, p.window).ntile * p.n_kv;
-      if (u0 < ub + n) {
-        st->s = at;
-        st->b = f - pre[at];
-        st->ub = ub;
-        break;
+      const int nt = attn_block(q, f - pre[at], p.tb, LOG2_TILE, p.window).ntile;
+      const long long n = (long long)(nt + EXTRA) * p.n_kv;
+#pragma unroll 1
+      for (int k = 0; k < 2; ++k) {
+        const long long u = k == 0 ? u0 : u1;
+        if (u < ub || u >= ub + n) continue;
+        const int in = (int)((u - ub) % (nt + EXTRA)) - EXTRA;
+        const long long at_u = tiles * p.n_kv + (u - ub) / (nt + EXTRA) * nt + (in > 0 ? in : 0);
+        if (k == 0) st->s = at, st->b = f - pre[at], st->ub = ub, st->before = at_u;
+        else st->until = at_u;
       }
       ub += n;
+      tiles += nt;
     }
   }
   __syncthreads();
@@ -208,23 +218,23 @@ __device__ __forceinline__ int attn_full_lo(const AttnParams& p, const AttnSeq& 
   return p.window > 0 ? seq.past + blk.t0 + blk.nt - p.window : 0;
 }
 
-// One item after the other from a CTA's first.
-template <int LOG2_TILE>
+// One item after the other from the one that a CTA's share begins in.
+template <int LOG2_TILE, int EXTRA>
 struct AttnCursor {
   AttnSeq seq;
   AttnBlock blk;
-  long long ub;  // the item's first unit
+  long long ub;  // the place of the item's first tile
   int s, b, head;
 
   __device__ __forceinline__ void start(const AttnParams& p, const AttnStart& st) {
     s = st.s, b = st.b;
     seq = attn_load_seq(p, s);
     blk = attn_block(seq, b, p.tb, LOG2_TILE, p.window);
-    head = (int)((st.u0 - st.ub) / blk.ntile);
-    ub = st.ub + (long long)head * blk.ntile;
+    head = (int)((st.u0 - st.ub) / (blk.ntile + EXTRA));
+    ub = st.ub + (long long)head * (blk.ntile + EXTRA) + EXTRA;
   }
   __device__ __forceinline__ void next(const AttnParams& p) {
-    ub += blk.ntile;
+    ub += blk.ntile + EXTRA;
     if (++head < p.n_kv) return;
     head = 0;
     ++b;
@@ -235,6 +245,12 @@ struct AttnCursor {
       b = 0;
     }
     blk = attn_block(seq, b, p.tb, LOG2_TILE, p.window);
+  }
+  // its tiles that the share has: first(), .. end() - 1; none where the share's border lies in the units ahead of them
+  __device__ __forceinline__ int first(const AttnStart& st) const { return st.u0 > ub ? (int)(st.u0 - ub) : 0; }
+  __device__ __forceinline__ int end(const AttnStart& st) const {
+    const long long n = st.u1 - ub;
+    return n >= blk.ntile ? blk.ntile : (n > 0 ? (int)n : 0);
   }
 };
 

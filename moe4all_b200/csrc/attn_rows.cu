@@ -28,6 +28,8 @@ __device__ __forceinline__ uint32_t movm(uint32_t a) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
 }
+constexpr int ROWS_EXTRA = 1;  // tiles' time that an item's beginning and end take
+
 template <int HD, int NT>
 struct RowsShape {
   static constexpr int WARPS = HD > 128 ? 4 : 8, THREADS = WARPS * 32, RB = 8 * NT;
@@ -63,32 +65,33 @@ __global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
     for (int i = 0; i < STAGES; ++i) mbar_init(full + i, 1);
   mbar_fence_init();
   pdl_wait();
-  attn_plan<THREADS, Sh::LOG2_TILE>(p, reinterpret_cast<int*>(ring_all), s_scan, &s_start);
+  attn_plan<THREADS, Sh::LOG2_TILE, ROWS_EXTRA>(p, reinterpret_cast<int*>(ring_all), s_scan, &s_start);
   const AttnStart st = s_start;
-  if (st.u0 >= st.u1) return;
+  if (st.until == st.before) return;
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the plan's words lay where the copies go
   __syncthreads();
 
   const bool packed = p.page_table == nullptr;
   // ---- what the warp asks for: its slices of the CTA's tiles, one after the other, STAGES of them ahead of their use
-  AttnCursor<Sh::LOG2_TILE> ahead;
+  AttnCursor<Sh::LOG2_TILE, ROWS_EXTRA> ahead;
   ahead.start(p, st);
-  long long au = st.u0;                 // unit of the next slice to ask for
-  int a_key = -1, a_page = 0;           // its first key (-1: none left) and its page
+  int at = ahead.first(st);             // tile of its item to look at next
+  int a_key = -1, a_page = 0;           // first key of the slice to ask for (-1: none left) and its page
   uint32_t asked = 0;
-  auto find = [&]() {                   // the next unit of which this warp has keys, from au on
-    while (au < st.u1) {
-      if (au >= ahead.ub + ahead.blk.ntile) {
+  auto find = [&]() {                   // the next tile of which this warp has keys
+    while (ahead.ub < st.u1) {
+      if (at >= ahead.end(st)) {
         ahead.next(p);
+        at = 0;
         continue;
       }
-      const int ks = ((ahead.blk.tile0 + (int)(au - ahead.ub)) << Sh::LOG2_TILE) + warp * 16;
+      const int ks = ((ahead.blk.tile0 + at) << Sh::LOG2_TILE) + warp * 16;
       if (ks < ahead.blk.hi && ks + 16 > ahead.blk.lo) {
         a_key = ks;
         if (!packed) a_page = attn_page(p, ahead.s, ks / p.page_size);
         return;
       }
-      ++au;
+      ++at;
     }
     a_key = -1;
   };
@@ -106,22 +109,21 @@ __global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
       }
     }
     ++asked;
-    ++au;
+    ++at;
     find();
   };
   find();
   for (int i = 0; i < STAGES; ++i) ask();
 
-  AttnCursor<Sh::LOG2_TILE> cur;
+  AttnCursor<Sh::LOG2_TILE, ROWS_EXTRA> cur;
   cur.start(p, st);
   uint32_t used = 0;
   bool alive = true;
   const int c0 = 2 * (lane & 3);  // this thread's columns (rows of the item): c0, c0 + 1 of every eight
-  for (long long u = st.u0; u < st.u1;) {
-    if (u >= cur.ub + cur.blk.ntile) cur.next(p);
+  long long left = st.until - st.before;  // tiles
+  for (;; cur.next(p)) {
     const AttnBlock& blk = cur.blk;
-    const int first_tile = (int)(u - cur.ub), n_rows = blk.nt * p.g;
-    const int end_tile = (int)(st.u1 - cur.ub < blk.ntile ? st.u1 - cur.ub : blk.ntile);
+    const int first_tile = cur.first(st), end_tile = cur.end(st), n_rows = blk.nt * p.g;
 
     // ---- q: B fragments of q^T, rows scaled by a power of two, as two f16 pieces
     uint32_t qh[NT][KST][2], ql[NT][KST][2];
@@ -381,7 +383,8 @@ __global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
         if (r < n_rows && i < p.hd) store(r, i, attn_join4<HD>(p, share, RB, r, i));
       }
     }
-    u = cur.ub + end_tile;
+    left -= end_tile - first_tile;
+    if (left <= 0) break;
   }
   // a warp that gave up has copies in flight: they land before its shared memory is somebody else's
   if (!alive)

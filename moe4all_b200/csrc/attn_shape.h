@@ -2,9 +2,10 @@
 // the host and in the kernels.
 //
 // An item is a block of consecutive new tokens of one sequence with the query heads of one kv head; its work is the key tiles that some row
-// of it sees.  Items in order (sequence, block, kv head) and their tiles in order form one line of units, which the CTAs of the launch share
-// evenly: CTA c of C takes the units [c U / C, (c + 1) U / C).  An item that crosses a border is joined from its CTAs' partial results, in
-// their order, by whichever finishes last.
+// of it sees, and some units more for its beginning and end (its q, its results).  Items in order (sequence, block, kv head), each as
+// `extra` units and then its tiles, form one line, which the CTAs of the launch share evenly: CTA c of C takes the tiles in
+// [c U / C, (c + 1) U / C).  An item whose tiles cross a border is joined from its CTAs' partial results, in their order, by whichever
+// finishes last.
 #pragma once
 #include <cstddef>
 #include <cstdint>
@@ -61,7 +62,7 @@ INFR_ATTN_HD AttnBlock attn_block(const AttnSeq& s, int b, int tb, int log2_tile
   return r;
 }
 
-// Where CTA c of C begins in a line of u units, and which CTA has unit i.
+// Where CTA c of C begins in a line of u units, and which CTA has the tile at place i.
 INFR_ATTN_HD long long attn_begin(int c, long long u, int C) { return (long long)c * u / C; }
 INFR_ATTN_HD int attn_cta_of(long long i, long long u, int C) { return (int)(((i + 1) * C - 1) / u); }
 

@@ -21,6 +21,7 @@ namespace infr {
 namespace {
 
 constexpr float TILE_BIAS = 15.f;  // weights are 2^(x - maximum + 15): below f16's limit, 2^-40 of the largest still has a bit
+constexpr int EXTRA = 2;           // tiles' time that an item's beginning and end take
 constexpr int RING = 4;            // tiles' and items' words in shared memory: the roles are never further apart
 
 template <int HD>
@@ -116,14 +117,14 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
   if (tid < 4 * RING) s_odd[tid] = 0;
   if (warp == 0) umma::tmem_alloc(&s_tmem);
   pdl_wait();
-  attn_plan<Sh::THREADS, Sh::LOG2_TILE>(p, reinterpret_cast<int*>(s_q), s_scan, &s_start);
+  attn_plan<Sh::THREADS, Sh::LOG2_TILE, EXTRA>(p, reinterpret_cast<int*>(s_q), s_scan, &s_start);
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the plan's words lay where tiles go
   umma::fence_before_sync();
   __syncthreads();
   umma::fence_after_sync();
   const AttnStart st = s_start;
   const uint32_t tmem = s_tmem;
-  const int N = (int)(st.u1 - st.u0);  // tiles of this CTA
+  const int N = (int)(st.until - st.before);  // tiles of this CTA
   bool ok = true;
 
   if (N > 0 && wg == 3) set_regs<Sh::REG_C>();
@@ -131,8 +132,9 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
     // nothing to do
   } else if (role == 3) {
     // ---- copies, and the items' words
-    AttnCursor<Sh::LOG2_TILE> c;
+    AttnCursor<Sh::LOG2_TILE, EXTRA> c;
     c.start(p, st);
+    int t = c.first(st), t_end = 0;  // the tile of its item that comes next, and where its tiles end here
     const int pieces = BK / granule;
     const bool packed = p.page_table == nullptr;
     int item = -1;
@@ -143,17 +145,16 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
     auto place = [&](int n) {
       Place at = {-1, 0, 0};
       if (n >= N) return at;
-      const long long u = st.u0 + n;
-      if (item < 0 || u >= c.ub + c.blk.ntile) {
-        if (item >= 0) c.next(p);
+      if (t >= t_end) {
+        if (item >= 0) c.next(p), t = 0;
+        t_end = c.end(st);
         ++item;
         if (lane == 0) {
           TileItem& it = s_item[item % ITEMS];
-          const long long end = c.ub + c.blk.ntile;
           const AttnShare sh = attn_share(c.ub, c.blk.ntile, st);
-          it.n0 = n, it.n1 = (int)((end < st.u1 ? end : st.u1) - st.u0);
+          it.n0 = n, it.n1 = n + t_end - t;
           it.row0 = c.seq.q0 + c.blk.t0, it.n_rows = c.blk.nt * p.g;
-          it.key0 = (c.blk.tile0 + (int)(u - c.ub)) << Sh::LOG2_TILE, it.lo = c.blk.lo, it.hi = c.blk.hi, it.pos0 = c.seq.past + c.blk.t0;
+          it.key0 = (c.blk.tile0 + t) << Sh::LOG2_TILE, it.lo = c.blk.lo, it.hi = c.blk.hi, it.pos0 = c.seq.past + c.blk.t0;
           it.full_lo = attn_full_lo(p, c.seq, c.blk), it.full_hi = attn_full_hi(c.seq, c.blk), it.head = c.head, it.s = c.s;
           it.q0 = c.seq.q0, it.whole = sh.first == sh.last, it.first_cta = sh.first, it.last_cta = sh.last;
           mbar_arrive(bars.i_full + item % ITEMS);
@@ -166,7 +167,7 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
         __syncwarp();
       }
       at.head = c.head;
-      const int key = ((c.blk.tile0 + (int)(u - c.ub)) << Sh::LOG2_TILE) + lane * granule;
+      const int key = ((c.blk.tile0 + t++) << Sh::LOG2_TILE) + lane * granule;
       if (lane < pieces && key < c.blk.hi && key + granule > c.blk.lo) {
         at.y = c.seq.q0 + key;
         if (!packed) {

@@ -1,5 +1,5 @@
 // The line of units of an attention call (attn_shape.h), walked by every CTA as the kernels walk it.
-//   line  tb log2_tile window n_kv ctas cap packed rows  n_seq  cu_q[n_seq + 1]  kv_len[n_seq]    prints "units items joined bad" or what is wrong
+//   line  tb log2_tile window n_kv ctas cap packed rows extra  n_seq  cu_q[n_seq + 1]  kv_len[n_seq]    prints "tiles items joined bad" or what is wrong
 //   sizes rows n_seq n_head n_kv head_dim n_pages page_size max_pages paged            prints "ok", "invalid: ..." or "unsupported: ..."
 #include <cstdio>
 #include <cstdlib>
@@ -15,9 +15,9 @@ using namespace infr;
 static int line(int argc, char** argv) {
   std::vector<long long> v;
   for (int i = 2; i < argc; ++i) v.push_back(std::atoll(argv[i]));
-  const int tb = (int)v[0], log2_tile = (int)v[1], window = (int)v[2], n_kv = (int)v[3], grid = (int)v[4], cap = (int)v[5], rows = (int)v[7], n_seq = (int)v[8];
+  const int tb = (int)v[0], log2_tile = (int)v[1], window = (int)v[2], n_kv = (int)v[3], grid = (int)v[4], cap = (int)v[5], rows = (int)v[7], extra = (int)v[8], n_seq = (int)v[9];
   const bool packed = v[6] != 0;
-  const long long *cu = v.data() + 9, *kv = cu + n_seq + 1;
+  const long long *cu = v.data() + 10, *kv = cu + n_seq + 1;
   struct Item {
     int s, b, head;
     AttnBlock blk;
@@ -26,7 +26,7 @@ static int line(int argc, char** argv) {
   bool bad = false;
   std::vector<Item> items;
   std::set<std::pair<int, int>> written;  // (row, head)
-  long long units = 0;
+  long long units = 0, tiles = 0;
   for (int s = 0; s < n_seq; ++s) {
     const AttnSeq q = attn_seq((int)cu[s], (int)cu[s + 1], (int)kv[s], packed, rows, cap, &bad);
     if (q.q0 < 0 || q.q_len < 0 || q.q0 + q.q_len > rows) return std::puts("rows out of range"), 1;
@@ -41,8 +41,9 @@ static int line(int argc, char** argv) {
           if (pos >= 0 && (lo < k.lo || pos >= k.hi || (lo >> log2_tile) < k.tile0 || (pos >> log2_tile) >= k.tile0 + k.ntile)) return std::puts("key lost"), 1;
           written.insert({q.q0 + t, h});
         }
-        items.push_back({s, b, h, k, units});
-        units += k.ntile;
+        items.push_back({s, b, h, k, units + extra});
+        units += extra + k.ntile;
+        tiles += k.ntile;
       }
   }
   const int C = (int)(units < grid ? units : grid);
@@ -79,7 +80,7 @@ static int line(int argc, char** argv) {
     const int first = attn_cta_of(it.ub, units, C), last = attn_cta_of(it.ub + it.blk.ntile - 1, units, C);
     if (slots.count(it.ub) && (int)slots[it.ub].size() != last - first + 1) return std::puts("parts missing"), 1;
   }
-  std::printf("%lld %zu %zu %d\n", units, items.size(), slots.size(), (int)bad);
+  std::printf("%lld %zu %zu %d\n", tiles, items.size(), slots.size(), (int)bad);
   return 0;
 }
 

@@ -17,8 +17,8 @@ def exe(tmp_path_factory):
     return exe
 
 
-def line(exe, tb, log2_tile, window, n_kv, ctas, cap, packed, rows, cu, kv):
-    args = [exe, "line", tb, log2_tile, window, n_kv, ctas, cap, int(packed), rows, len(kv), *cu, *kv]
+def line(exe, tb, log2_tile, window, n_kv, ctas, cap, packed, rows, cu, kv, extra=1):
+    args = [exe, "line", tb, log2_tile, window, n_kv, ctas, cap, int(packed), rows, extra, len(kv), *cu, *kv]
     r = subprocess.run([str(a) for a in args], capture_output=True, text=True)
     assert r.returncode == 0, (r.stdout, args)
     return [int(x) for x in r.stdout.split()]
@@ -50,7 +50,7 @@ def test_batches(exe, seed):
     kv = list(q) if packed else [max(0, x + r.choice([-2, 0, 5, r.randint(0, 3000)])) for x in q]
     cu = [sum(q[:i]) for i in range(n + 1)]
     units, items, joined, bad = line(exe, r.choice([1, 2, 5, 16, 128]), r.choice([6, 7]), r.choice([0, 0, 1, 60, 1000]), r.choice([1, 3, 8]),
-                                     r.choice([1, 7, 148]), 4096, packed, cu[-1] + r.choice([0, 3]), cu, kv)
+                                     r.choice([1, 7, 148]), 4096, packed, cu[-1] + r.choice([0, 3]), cu, kv, r.choice([0, 1, 2, 5]))
     assert bad == 0 and units >= items
 
 
