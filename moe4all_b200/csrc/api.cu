@@ -1074,6 +1074,7 @@ int32_t attn_check_batch(infr_cuda_ctx* ctx, const char* op, const Desc* d, cons
 int32_t attn_check_rows(infr_cuda_ctx* ctx, const char* what, const infr_cuda_buf* b, uint32_t rows, uint32_t stride, uint32_t wide, long long* out) {
   const uint32_t s = stride ? stride : wide;
   if (s < wide || s % 4) return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, std::string(what) + ": a row stride is a multiple of 4 and at least a row");
+  if (s > (1u << 24)) return fail(ctx, INFR_CUDA_ERR_UNSUPPORTED, std::string(what) + ": a row stride past 2^24 values");
   if (!fits(b, attn_span(rows, s, wide) * 4)) return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, std::string(what) + ": buffer missing or too small");
   *out = s;
   return INFR_CUDA_OK;

@@ -349,30 +349,31 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
     const int row = tid & 127;
     const uint32_t mine = tmem + ((uint32_t)((warp & 3) * 32) << 16) + 64 * wg;
 #pragma unroll 1
-    for (int n = 0, item = 0; n < N && ok; ++item) {
+    // q of an item into two f16 pieces: eight lanes a row, the next rows on their way meanwhile.  What is left in the rows past the item's
+    // reaches these rows' sums only.  (A short rolled loop: code that runs once an item comes from far away.)
+    auto convert = [&](int item) {
       ok = wait_all(bars.i_full + item % ITEMS, item / ITEMS);
-      if (!ok) break;
+      if (!ok) return;
       const TileItem& it = s_item[item % ITEMS];
-      const int n1 = it.n1, n_rows = it.n_rows, slot = item & (RING - 1);
-      // q into two f16 pieces: eight lanes a row, the next rows on their way meanwhile (a rolled loop: code that runs once an item
-      // comes from far away).  What is left in the rows past the item's reaches these rows' sums only.
-      const int l8 = lane & 7;
+      const int n_rows = it.n_rows, l8 = lane & 7, r8 = tid >> 3;
       const float* q_item = p.q + (size_t)it.row0 * p.q_stride + (size_t)it.head * p.g * p.hd + 4 * l8;
+      const int stride = (int)p.q_stride, head_pitch = p.hd, g = p.g;
       constexpr int STEP = 16 * GROUPS, AT_ONCE = HD <= 128 ? 2 : 1;
       float4 ahead[AT_ONCE][HD / 32];
       auto load = [&](int r0) {
 #pragma unroll
         for (int a = 0; a < AT_ONCE; ++a) {
-          const int r = r0 + a * STEP;
-          const float* src = q_item + attn_row_offset(p, 0, 0, r, p.q_stride);
+          const int r = r0 + a * STEP, t = attn_row_token(p, r);
+          const float* src = q_item + (t * stride + (r - t * g) * head_pitch);
 #pragma unroll
           for (int j = 0; j < HD / 32; ++j)
             ahead[a][j] = r < n_rows && 4 * (l8 + 8 * j) < p.hd ? __ldcg(reinterpret_cast<const float4*>(src + 32 * j)) : make_float4(0.f, 0.f, 0.f, 0.f);
         }
       };
-      load(tid >> 3);
+      load(r8);
       if (item > 0) ok = wait_all(bars.q_empty + ((item - 1) & (RING - 1)), (item - 1) / RING);
-      if (!ok) break;
+      if (!ok) return;
+      float* fac = s_fac + (item & (RING - 1)) * 128;
 #pragma unroll 1
       for (int r0 = 0; r0 < n_rows; r0 += AT_ONCE * STEP) {
         float4 v[AT_ONCE][HD / 32];
@@ -380,10 +381,10 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
         for (int a = 0; a < AT_ONCE; ++a)
 #pragma unroll
           for (int j = 0; j < HD / 32; ++j) v[a][j] = ahead[a][j];
-        if (r0 + AT_ONCE * STEP < n_rows) load(r0 + AT_ONCE * STEP + (tid >> 3));
+        if (r0 + AT_ONCE * STEP < n_rows) load(r0 + AT_ONCE * STEP + r8);
 #pragma unroll
         for (int a = 0; a < AT_ONCE; ++a) {
-          const int r = r0 + a * STEP + (tid >> 3);
+          const int r = r0 + a * STEP + r8;
           float big = 0.f;
 #pragma unroll
           for (int j = 0; j < HD / 32; ++j) big = fmaxf(big, fmaxf(fmaxf(fabsf(v[a][j].x), fabsf(v[a][j].y)), fmaxf(fabsf(v[a][j].z), fabsf(v[a][j].w))));
@@ -392,32 +393,47 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
           float down, up;
           attn_row_scale(big, down, up);
           if (p.scale_log2 < 0.f) down = -down;
+          unsigned char* row_at = s_q + r * 128 + ((l8 & 1) << 3);
 #pragma unroll
           for (int j = 0; j < HD / 32; ++j) {
             uint2 hi, lo;
             split2(v[a][j].x * down, v[a][j].y * down, hi.x, lo.x);
             split2(v[a][j].z * down, v[a][j].w * down, hi.y, lo.y);
-            unsigned char* dst = s_q + (j >> 1) * 16384 + r * 128 + ((((l8 >> 1) + 4 * (j & 1)) ^ (r & 7)) << 4) + ((l8 & 1) << 3);
+            unsigned char* dst = row_at + (j >> 1) * 16384 + ((((l8 >> 1) + 4 * (j & 1)) ^ (r & 7)) << 4);
             *reinterpret_cast<uint2*>(dst) = hi;
             *reinterpret_cast<uint2*>(dst + Sh::QPIECE) = lo;
           }
           // (not 0: hidden keys' -inf times it stays -inf)
-          if (l8 == 0) s_fac[slot * 128 + r] = fmaxf(up * fabsf(p.scale_log2), 1.2e-38f);
+          if (l8 == 0) fac[r] = fmaxf(up * fabsf(p.scale_log2), 1.2e-38f);
         }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bars.q_full), mbar_arrive(bars.f_full + slot);
-      ok = wait_all(bars.f_full + slot, item / RING);
-      const float f = s_fac[slot * 128 + row];
+      if (lane == 0) mbar_arrive(&bars.q_full), mbar_arrive(bars.f_full + (item & (RING - 1)));
+    };
+    // an item's q is turned two tiles ahead of its first: its scores then follow the last item's without a break.  (Not earlier: the copies
+    // know of an item three tiles ahead.)
+    int turned = 0;
+#pragma unroll 1
+    for (int n = 0, item = 0; n < N && ok; ++item) {
+      ok = wait_all(bars.i_full + item % ITEMS, item / ITEMS);
+      if (!ok) break;
+      const TileItem& it = s_item[item % ITEMS];
+      const int n1 = it.n1, n_rows = it.n_rows, slot = item & (RING - 1);
+      float f = 0.f;
       const int to = it.pos0 + (row < n_rows ? attn_row_token(p, row) : 0);  // the row sees the keys (from, to]
       const int from = p.window > 0 ? to - p.window : -1;
       const bool busy = (warp & 3) * 32 < n_rows;  // (other rows' weights are whatever is there: they reach those rows' sums only)
       float m = -CUDART_INF_F, l = 0.f;
       int ks = it.key0 + 64 * wg;
 #pragma unroll 1
-      for (; n < n1 && ok; ++n, ks += BK) {
-        ok = wait_all(bars.s_full + (n & 1), n >> 1);
+      for (; n < n1; ++n, ks += BK) {
+        while (turned <= (n + 2 >= n1 && n1 < N ? item + 1 : item) && ok) convert(turned), ++turned;
+        if (n == it.n0) {
+          ok = ok && wait_all(bars.f_full + slot, item / RING);
+          f = s_fac[slot * 128 + row];
+        }
+        ok = ok && wait_all(bars.s_full + (n & 1), n >> 1);
         if (!ok) break;
         umma::fence_after_sync();
         const uint32_t sa = mine + (n & 1) * BK;
@@ -548,6 +564,8 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
       unsigned char* out = s_out + (warp & (4 * Sh::S_GROUPS - 1)) * 32 * Sh::OUT_COLS * 4;
       constexpr int WORDS = Sh::OUT_COLS / 4, ROWS = 32 / WORDS;  // 16-byte words of a row, rows that a warp stores at once
       const int first_row = (warp & 3) * 32;
+      float* base = whole ? p.out + (size_t)it.row0 * p.out_stride + (size_t)it.head * p.g * p.hd : p.part + (slot - row) * HD;
+      const int g = p.g, head_pitch = whole ? p.hd : HD, token_pitch = whole ? (int)p.out_stride : g * HD;
       if (mine) {
 #pragma unroll
         for (int i0 = 0; i0 < Sh::COLS; i0 += Sh::OUT_COLS) {
@@ -558,13 +576,12 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
             *reinterpret_cast<float4*>(out + lane * Sh::OUT_COLS * 4 + ((i / 4 ^ (lane & (WORDS - 1))) << 4)) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
           }
           __syncwarp();
-          const int word = lane & (WORDS - 1), col = col0 + i0 + 4 * word;
-#pragma unroll 2
-          for (int r = lane / WORDS; r < 32; r += ROWS) {
+          const int word = lane & (WORDS - 1), col = col0 + i0 + 4 * word, stored = col < p.hd ? min(32, n_rows - first_row) : 0;
+#pragma unroll 1
+          for (int r = lane / WORDS; r < stored; r += ROWS) {
             const float4 v = *reinterpret_cast<const float4*>(out + r * Sh::OUT_COLS * 4 + ((word ^ (r & (WORDS - 1))) << 4));
-            const int rr = first_row + r;
-            if (rr < n_rows && col < p.hd)
-              __stcg(reinterpret_cast<float4*>(whole ? p.out + attn_row_offset(p, it.row0, it.head, rr, p.out_stride) + col : p.part + (slot - row + rr) * HD + col), v);
+            const int rr = first_row + r, t = attn_row_token(p, rr);
+            __stcg(reinterpret_cast<float4*>(base + col + (t * token_pitch + (rr - t * g) * head_pitch)), v);
           }
           __syncwarp();
         }

@@ -422,7 +422,7 @@ def test_refusals(backend):
                dict(scale=float("nan")), dict(scale=float("inf")), dict(path=3), dict(q_stride=511), dict(q_stride=508), dict(q_stride=514), dict(out=part),
                dict(q=part), dict(k=part), dict(cu_q=part, n_seq=100), dict(out=ok.q), dict(n_pages=10 ** 6), dict(max_pages=10 ** 8), dict(window=1 << 31)):
         refused(BackendError, **kw)
-    for kw in (dict(head_dim=72), dict(head_dim=272, n_head=1, n_kv=1), dict(page_size=24), dict(n_head=32, n_kv=1, head_dim=16, path=1), dict(n_seq=20000)):
+    for kw in (dict(head_dim=72), dict(head_dim=272, n_head=1, n_kv=1), dict(page_size=24), dict(n_head=32, n_kv=1, head_dim=16, path=1), dict(n_seq=20000), dict(q_stride=(1 << 24) + 4)):
         refused(Unsupported, **kw)
     be.attention(dataclasses.replace(ok, rows=0))
     be.attention(ok)
