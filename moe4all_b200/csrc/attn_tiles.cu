@@ -65,9 +65,10 @@ constexpr int ITEMS = 16;  // the copies are at most nine items ahead of the sum
 
 struct TileBars {
   uint64_t i_full[ITEMS];
-  uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4];
-  uint64_t v_ok[4];            // a V tile is there and has been looked after
-  uint64_t s_full[2], ready[2];  // scores; weights there and the sums' columns free
+  uint64_t k_empty[4], v_full[4], v_empty[4];
+  uint64_t s_full[2];
+  uint64_t ready[4];    // all that step n of the MMAs needs: weights of tile n, its V there and looked after, its sums' columns free, K of tile n + 2
+  uint64_t k_first[2];  // K of the first two tiles
   uint64_t o_full[2];
   uint64_t a_full[RING];       // a tile's maxima (and, at an item's end, weights)
   uint64_t f_full[RING];       // an item's score factors
@@ -108,8 +109,8 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
 
   if (tid == 0) {
     for (int i = 0; i < ITEMS; ++i) mbar_init(bars.i_full + i, 1);
-    for (int i = 0; i < 4; ++i) mbar_init(bars.k_full + i, 1), mbar_init(bars.k_empty + i, 1), mbar_init(bars.v_full + i, 1), mbar_init(bars.v_empty + i, 1), mbar_init(bars.v_ok + i, 2);
-    for (int i = 0; i < 2; ++i) mbar_init(bars.s_full + i, 1), mbar_init(bars.ready + i, 4 * (Sh::W_GROUPS + Sh::S_GROUPS)), mbar_init(bars.o_full + i, 1);
+    for (int i = 0; i < 4; ++i) mbar_init(bars.k_empty + i, 1), mbar_init(bars.v_full + i, 1), mbar_init(bars.v_empty + i, 1), mbar_init(bars.ready + i, 4 * (Sh::W_GROUPS + Sh::S_GROUPS) + 3);
+    for (int i = 0; i < 2; ++i) mbar_init(bars.s_full + i, 1), mbar_init(bars.o_full + i, 1), mbar_init(bars.k_first + i, 1);
     for (int i = 0; i < RING; ++i) mbar_init(bars.a_full + i, 4 * Sh::W_GROUPS), mbar_init(bars.f_full + i, 4 * Sh::W_GROUPS), mbar_init(bars.q_empty + i, 1);
     mbar_init(&bars.q_full, 4 * Sh::W_GROUPS);
     mbar_fence_init();
@@ -184,12 +185,12 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
       const int count = __popc(__ballot_sync(0xFFFFFFFFu, at.y >= 0));
       if (n >= BUFS) ok = wait_all(empty + buf, n / BUFS - 1);
       if (!ok) return;
-      if (lane == 0) mbar_arrive_expect_tx(full + buf, (uint32_t)(count * granule * 128 * SLABS));
+      if (lane == 0) mbar_arrive_expect_tx(full, (uint32_t)(count * granule * 128 * SLABS));
       __syncwarp();
       if (at.y >= 0) {
         unsigned char* dst = bufs + buf * TILE + lane * granule * 128;
 #pragma unroll
-        for (int s = 0; s < SLABS; ++s) tma_load_4d(dst + s * (BK * 128), map, 64 * s, at.y, at.head, at.w, full + buf);
+        for (int s = 0; s < SLABS; ++s) tma_load_4d(dst + s * (BK * 128), map, 64 * s, at.y, at.head, at.w, full);
       }
       __syncwarp();
       asked = n + 1;
@@ -198,18 +199,22 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
     Place v0 = {}, v1 = {}, k = place(0);
 #pragma unroll 1
     for (int n = -2; n < N && ok; ++n) {
-      if (n >= 0) load(v0, n, vs, &vmap, s_v, bars.v_full, bars.v_empty);
+      if (n >= 0) load(v0, n, vs, &vmap, s_v, bars.v_full + n % BUFS, bars.v_empty);
       v0 = v1, v1 = k;
       if (n + 2 < N && ok) {
-        load(k, n + 2, ks, &kmap, s_k, bars.k_full, bars.k_empty);
+        load(k, n + 2, ks, &kmap, s_k, n < 0 ? bars.k_first + n + 2 : bars.ready + (n & 3), bars.k_empty);
         k = place(n + 3);
+      } else if (ok && lane == 0) {
+        mbar_arrive(bars.ready + (n & 3));
       }
     }
     if (!ok) {
       if (lane == 0) atomicExch(&p.status->timeout, 11);
       // copies in flight land before the shared memory is somebody else's
-      for (int i = max(0, ks - BUFS); i < ks; ++i) attn_wait(bars.k_full + i % BUFS, i / BUFS);
       for (int i = max(0, vs - BUFS); i < vs; ++i) attn_wait(bars.v_full + i % BUFS, i / BUFS);
+      for (int i = max(0, ks - BUFS); i < min(ks, 2); ++i) attn_wait(bars.k_first + i, 0);
+      // (K's land in barriers that wait for more than copies: their bytes are given the time that copies take at most)
+      __nanosleep(1000000);
     }
   } else if (role == 4) {
     // ---- MMAs.  Scores run one tile ahead of the sums; their accumulators are free by then, since MMAs of one thread go in order
@@ -224,14 +229,13 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
     for (int n = -2; n < N && ok; ++n) {
       if (n >= 0) {
         const int buf = n % BUFS;
-        ok = wait_all(bars.v_ok + buf, n / BUFS);
-        ok = ok && wait_all(bars.ready + (n & 1), n >> 1);
+        ok = wait_all(bars.ready + (n & 3), n >> 2);
         if (!ok) break;
         umma::fence_after_sync();
         if (umma::elect_one()) {
           const uint32_t d = tmem + Sh::O_COL + (n % OBUFS) * HD, a = tmem + (n & 1) * BK;
           const uint64_t vd = vdesc + (uint64_t)((buf * TILE) >> 4);
-#pragma unroll 2
+#pragma unroll 4
           for (int k = 0; k < BK / 16; ++k) {
             const uint64_t b = vd + (uint64_t)((k * 2048) >> 4);
             const uint32_t ak = a + (k >> 1) * 32 + (k & 1) * 8;  // 32 keys: 16 columns of their weights, 16 of the rest
@@ -262,7 +266,7 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
           __syncwarp();
         }
         const int buf = next % BUFS;
-        ok = ok && wait_all(bars.k_full + buf, next / BUFS);
+        if (n < 0) ok = ok && wait_all(bars.k_first + next, 0);
         if (!ok) break;
         umma::fence_after_sync();
         if (umma::elect_one()) {
@@ -270,7 +274,7 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
           const uint64_t kd = kdesc + (uint64_t)((buf * TILE) >> 4);
 #pragma unroll 1
           for (int piece = 0; piece < 2; ++piece)
-#pragma unroll 4
+#pragma unroll 8
             for (int k = 0; k < HD / 16; ++k) {
               const uint64_t b = kd + (uint64_t)(((k >> 2) * (BK * 128) + (k & 3) * 32) >> 4);
               if (piece < Sh::Q_TMEM) umma::mma1_f16_ts(d, tq + piece * (HD / 2) + 8 * k, b, idesc_s, piece + k > 0 ? 1u : 0u);
@@ -304,7 +308,7 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
       ok = wait_all(bars.v_full + n % BUFS, n / BUFS);
       if (!ok) break;
       if (!tile_masked(it, ks, BK)) {
-        if (lane == 0) mbar_arrive(bars.v_ok + n % BUFS);
+        if (lane == 0) mbar_arrive(bars.ready + (n & 3));
         continue;
       }
       bool odd = false;
@@ -339,7 +343,7 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
       if (odd) s_odd[item % (4 * RING)] = 1;
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
-      if (lane == 0) mbar_arrive(bars.v_ok + n % BUFS);
+      if (lane == 0) mbar_arrive(bars.ready + (n & 3));
     }
     if (!ok && lane == 0) atomicExch(&p.status->timeout, 11);
   } else if (role == 0) {
@@ -497,7 +501,7 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
           if (wg == 0) s_end[(item % Sh::ENDS) * 128 + row] = m;
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(bars.ready + (n & 1)), mbar_arrive(bars.a_full + (n & (RING - 1)));
+        if (lane == 0) mbar_arrive(bars.ready + (n & 3)), mbar_arrive(bars.a_full + (n & (RING - 1)));
       }
     }
     if (!ok && lane == 0) atomicExch(&p.status->timeout, 11);
@@ -510,7 +514,7 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
     float m = -CUDART_INF_F;
     int item = -1, first = 0, end = 0, n_rows = 0;
     for (int n = 0; n < OBUFS && n < N; ++n)
-      if (lane == 0) mbar_arrive(bars.ready + (n & 1));
+      if (lane == 0) mbar_arrive(bars.ready + n);
 #pragma unroll 1
     for (int n = 0; n < N && ok; ++n) {
       if (n == end) {
@@ -542,7 +546,7 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
       }
       umma::fence_before_sync();
       __syncwarp();
-      if (lane == 0 && n + OBUFS < N) mbar_arrive(bars.ready + ((n + OBUFS) & 1));
+      if (lane == 0 && n + OBUFS < N) mbar_arrive(bars.ready + ((n + OBUFS) & 3));
       if (n + 1 < end) continue;
 
       // ---- the item's end
