@@ -84,6 +84,11 @@ __device__ __forceinline__ uint32_t seen_keys(int k0, int from, int to) {
   return n <= lo ? 0u : (~0u >> (32 - (n - lo))) << lo;
 }
 
+__device__ __forceinline__ void hide(float (&s)[32], uint32_t seen) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i) s[i] = (seen >> i) & 1u ? s[i] : -CUDART_INF_F;
+}
+
 template <int HD>
 __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
     k_attn_tiles(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ AttnParams p, const int granule) {
@@ -235,7 +240,7 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
         if (umma::elect_one()) {
           const uint32_t d = tmem + Sh::O_COL + (n % OBUFS) * HD, a = tmem + (n & 1) * BK;
           const uint64_t vd = vdesc + (uint64_t)((buf * TILE) >> 4);
-#pragma unroll 4
+#pragma unroll 2
           for (int k = 0; k < BK / 16; ++k) {
             const uint64_t b = vd + (uint64_t)((k * 2048) >> 4);
             const uint32_t ak = a + (k >> 1) * 32 + (k & 1) * 8;  // 32 keys: 16 columns of their weights, 16 of the rest
@@ -274,7 +279,7 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
           const uint64_t kd = kdesc + (uint64_t)((buf * TILE) >> 4);
 #pragma unroll 1
           for (int piece = 0; piece < 2; ++piece)
-#pragma unroll 8
+#pragma unroll 4
             for (int k = 0; k < HD / 16; ++k) {
               const uint64_t b = kd + (uint64_t)(((k >> 2) * (BK * 128) + (k & 3) * 32) >> 4);
               if (piece < Sh::Q_TMEM) umma::mma1_f16_ts(d, tq + piece * (HD / 2) + 8 * k, b, idesc_s, piece + k > 0 ? 1u : 0u);
@@ -362,7 +367,7 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
       const int n_rows = it.n_rows, l8 = lane & 7, r8 = tid >> 3;
       const float* q_item = p.q + (size_t)it.row0 * p.q_stride + (size_t)it.head * p.g * p.hd + 4 * l8;
       const int stride = (int)p.q_stride, head_pitch = p.hd, g = p.g;
-      constexpr int STEP = 16 * GROUPS, AT_ONCE = HD <= 128 ? 2 : 1;
+      constexpr int STEP = 16 * GROUPS, AT_ONCE = 1;
       float4 ahead[AT_ONCE][HD / 32];
       auto load = [&](int r0) {
 #pragma unroll
@@ -441,25 +446,21 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
         if (!ok) break;
         umma::fence_after_sync();
         const uint32_t sa = mine + (n & 1) * BK;
-        float s[2][32];
         float top = -CUDART_INF_F;
+        const bool masked = ks + 64 > it.full_hi || ks < it.full_lo;
         if (busy) {
-          umma::tmem_ld_32x32(sa, s[0]);
-          umma::tmem_ld_32x32(sa + 32, s[1]);
-          umma::tmem_ld_wait(s[0]);
-          umma::tmem_ld_wait(s[1]);
-          if (ks + 64 > it.full_hi || ks < it.full_lo) {
-            const uint32_t seen0 = seen_keys(ks, from, to), seen1 = seen_keys(ks + 32, from, to);
+#pragma unroll 1
+          for (int j = 0; j < 64; j += 32) {
+            float s[32];
+            umma::tmem_ld_32x32(sa + j, s);
+            const uint32_t seen = masked ? seen_keys(ks + j, from, to) : ~0u;
+            umma::tmem_ld_wait(s);
+            if (masked) hide(s, seen);
+            float t[2] = {top, -CUDART_INF_F};
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              s[0][i] = (seen0 >> i) & 1u ? s[0][i] : -CUDART_INF_F;
-              s[1][i] = (seen1 >> i) & 1u ? s[1][i] : -CUDART_INF_F;
-            }
+            for (int i = 0; i < 32; i += 2) t[(i >> 1) & 1] = fmaxf(fmaxf(t[(i >> 1) & 1], s[i]), s[i + 1]);
+            top = fmaxf(t[0], t[1]);
           }
-          float t[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
-#pragma unroll
-          for (int i = 0; i < 32; ++i) t[i & 3] = fmaxf(fmaxf(t[i & 3], s[0][i]), s[1][i]);
-          top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
         }
         if constexpr (GROUPS == 2) {
           float* at = s_max + (n & 1) * 256 + row;
@@ -474,12 +475,17 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
           const float off = TILE_BIAS - (now == -CUDART_INF_F ? 0.f : now);
           const float2 f2 = make_float2(f, f), off2 = make_float2(off, off), minus = make_float2(-1.f, -1.f);
           float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
+#pragma unroll 1
+          for (int j = 0; j < 64; j += 32) {
+            float s[32];
+            umma::tmem_ld_32x32(sa + j, s);
+            const uint32_t seen = masked ? seen_keys(ks + j, from, to) : ~0u;
+            umma::tmem_ld_wait(s);
+            if (masked) hide(s, seen);
             uint32_t w[32];
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-              const float2 x = __ffma2_rn(make_float2(s[j][2 * i], s[j][2 * i + 1]), f2, off2);
+              const float2 x = __ffma2_rn(make_float2(s[2 * i], s[2 * i + 1]), f2, off2);
               const float2 e = make_float2(exp2_approx(x.x), exp2_approx(x.y));
               sum[i & 1] = __fadd2_rn(sum[i & 1], e);
               // the piece that f16 holds (below 2^-14, 2^-29 of the largest, rounded once more), and the rest
@@ -489,7 +495,7 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
               w[i] = *reinterpret_cast<const uint32_t*>(&hh);
               w[16 + i] = *reinterpret_cast<const uint32_t*>(&rr);
             }
-            umma::tmem_st_32x32_async(sa + 32 * j, w);
+            umma::tmem_st_32x32_async(sa + j, w);
           }
           l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
           umma::tmem_st_wait();
