@@ -301,40 +301,66 @@ __device__ __forceinline__ int attn_slot(int cta, const AttnShare& sh) { return 
 
 // After all threads have written their CTA's part: whether this CTA is the item's last and joins it.  Counting is by atomics, the join
 // itself is in the order of the CTAs: the sums do not depend on who came last.
-__device__ __forceinline__ bool attn_arrive(const AttnParams& p, const AttnShare& sh, int* s_last, bool leader, int threads_bar, int threads) {
+// (first, last are read behind the barrier.)
+__device__ __forceinline__ bool attn_arrive(const AttnParams& p, const int& first, const int& last, int* s_last, bool leader, int threads_bar, int threads) {
   __threadfence();
   asm volatile("bar.sync %0, %1;" ::"r"(threads_bar), "r"(threads) : "memory");
   if (leader) {
-    const int n = atomicAdd(p.count + sh.first, 1);
-    *s_last = n == sh.last - sh.first;
-    if (n == sh.last - sh.first) p.count[sh.first] = 0;
+    const int n = atomicAdd(p.count + first, 1);
+    *s_last = n == last - first;
+    if (n == last - first) p.count[first] = 0;
     __threadfence();
   }
   asm volatile("bar.sync %0, %1;" ::"r"(threads_bar), "r"(threads) : "memory");
   return *s_last != 0;
 }
 
-// Four values of row r of the joined item, divided by its weight (zero where no row was seen).
+// Row r of the joined item, divided by its weight (zero where no key was seen), by a warp: the parts' weights by lane, their values eight
+// parts in flight.  (A thread that walked the parts by itself took 24 us for 37 of them.)
 template <int HD>
-__device__ __forceinline__ float4 attn_join4(const AttnParams& p, const AttnShare& sh, int item_rows, int r, int i) {
+__device__ __forceinline__ void attn_join_row(const AttnParams& p, const AttnShare& sh, int item_rows, int r, float* dst) {
+  constexpr int V = (HD + 127) / 128;
+  const int lane = threadIdx.x & 31, parts = sh.last - sh.first + 1;
   float M = -CUDART_INF_F;
 #pragma unroll 1
-  for (int c = sh.first; c <= sh.last; ++c) M = fmaxf(M, __ldcg(&p.part_ml[(size_t)attn_slot(c, sh) * item_rows + r]).x);
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int c = lane; c < parts; c += 32) M = fmaxf(M, __ldcg(&p.part_ml[(size_t)attn_slot(sh.first + c, sh) * item_rows + r]).x);
+  M = warp_max(M);
   float L = 0.f;
-#pragma unroll 4
-  for (int c = sh.first; c <= sh.last; ++c) {
-    const size_t at = (size_t)attn_slot(c, sh) * item_rows + r;
-    const float2 ml = __ldcg(&p.part_ml[at]);
-    const float4 v = __ldcg(reinterpret_cast<const float4*>(p.part + at * HD + i));
-    const float w = exp2_rel(ml.x, M);
-    if (w != 0.f) {  // (a part that saw nothing holds nothing)
-      L += w * ml.y;
-      o.x += w * v.x, o.y += w * v.y, o.z += w * v.z, o.w += w * v.w;
+  float4 o[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) o[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+  for (int c0 = 0; c0 < parts; c0 += 32) {
+    float w = 0.f;
+    if (c0 + lane < parts) {
+      const float2 ml = __ldcg(&p.part_ml[(size_t)attn_slot(sh.first + c0 + lane, sh) * item_rows + r]);
+      w = exp2_rel(ml.x, M);
+      if (w != 0.f) L += w * ml.y;  // (a part that saw nothing holds nothing)
+    }
+#pragma unroll 1
+    for (int k0 = 0; k0 < min(32, parts - c0); k0 += 8) {
+      float4 v[8][V];
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          if (c0 + k0 + k < parts && 4 * lane + 128 * j < HD)
+            v[k][j] = __ldcg(reinterpret_cast<const float4*>(p.part + ((size_t)attn_slot(sh.first + c0 + k0 + k, sh) * item_rows + r) * HD + 4 * lane + 128 * j));
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float wk = __shfl_sync(0xFFFFFFFFu, w, k0 + k);
+        if (c0 + k0 + k < parts && wk != 0.f) {
+#pragma unroll
+          for (int j = 0; j < V; ++j) o[j].x += wk * v[k][j].x, o[j].y += wk * v[k][j].y, o[j].z += wk * v[k][j].z, o[j].w += wk * v[k][j].w;
+        }
+      }
     }
   }
+  L = warp_sum(L);
   const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);  // NaN stays
-  return make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+#pragma unroll
+  for (int j = 0; j < V; ++j)
+    if (4 * lane + 128 * j < p.hd) *reinterpret_cast<float4*>(dst + 4 * lane + 128 * j) = make_float4(o[j].x * inv, o[j].y * inv, o[j].z * inv, o[j].w * inv);
 }
 
 // Maps of a cache for boxes of 64 values x box_rows keys of one head: dimensions (values, keys of a page or packed rows, kv heads, pages).

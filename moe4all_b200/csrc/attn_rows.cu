@@ -377,11 +377,10 @@ __global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
         if (i == 0) __stcg(p.part_ml + at, make_float2(M, L));
       }
     }
-    if (!whole && attn_arrive(p, share, &s_last, tid == 0, 0, THREADS)) {
-      for (int e = tid; e < RB * (HD / 4); e += THREADS) {
-        const int r = e / (HD / 4), i = 4 * (e % (HD / 4));
-        if (r < n_rows && i < p.hd) store(r, i, attn_join4<HD>(p, share, RB, r, i));
-      }
+    if (!whole && attn_arrive(p, share.first, share.last, &s_last, tid == 0, 0, THREADS)) {
+#pragma unroll 1
+      for (int r = warp; r < n_rows; r += WARPS)
+        attn_join_row<HD>(p, share, RB, r, p.out + attn_row_offset(p, cur.seq.q0 + blk.t0, cur.head, r, p.out_stride));
     }
     left -= end_tile - first_tile;
     if (left <= 0) break;

@@ -22,6 +22,7 @@ namespace {
 
 constexpr float TILE_BIAS = 15.f;  // weights are 2^(x - maximum + 15): below f16's limit, 2^-40 of the largest still has a bit
 constexpr int EXTRA = 2;           // tiles' time that an item's beginning and end take
+constexpr int JOIN_PARTS = 32;     // parts of an item that are joined by column; more go row by row
 constexpr int RING = 4;            // tiles' and items' words in shared memory: the roles are never further apart
 
 template <int HD>
@@ -44,7 +45,7 @@ struct TilesShape {
   static constexpr int SMEM = 1024 + 2 * QPIECE + 2 * BUFS * TILE + OUT + SMALL;
   static_assert(SMEM + 2048 <= 232448, "more shared memory than a CTA has");
   // registers by role: together as many as the launch has
-  static constexpr int REG_W = HD == 64 ? 136 : HD == 128 ? 120 : 136, REG_S = HD == 64 ? 128 : HD == 128 ? 192 : 152, REG_C = HD == 64 ? 104 : 72;
+  static constexpr int REG_W = HD <= 128 ? 104 : 112, REG_S = HD == 64 ? 168 : HD == 128 ? 208 : 160, REG_C = HD == 64 ? 128 : HD == 128 ? 96 : 80;
   static_assert(REG_W * W_GROUPS + REG_S * S_GROUPS + REG_C <= 512, "more registers than the launch has");
 };
 
@@ -96,7 +97,7 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
   constexpr int BK = Sh::BK, SLABS = Sh::SLABS, BUFS = Sh::BUFS, OBUFS = Sh::OBUFS, TILE = Sh::TILE;
   extern __shared__ unsigned char smem_raw[];
   __shared__ TileBars bars;
-  __shared__ TileItem s_item[ITEMS];
+  __shared__ TileItem s_item[ITEMS], s_parts[2];
   __shared__ long long s_scan[Sh::THREADS / 32];
   __shared__ AttnStart s_start;
   __shared__ uint32_t s_tmem;
@@ -518,7 +519,7 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16) + Sh::O_COL + col0;
     float2 o[Sh::COLS / 2];
     float m = -CUDART_INF_F;
-    int item = -1, first = 0, end = 0, n_rows = 0;
+    int item = -1, first = 0, end = 0, n_rows = 0, parts = 0;
     for (int n = 0; n < OBUFS && n < N; ++n)
       if (lane == 0) mbar_arrive(bars.ready + n);
 #pragma unroll 1
@@ -542,12 +543,12 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
       if (mine) {
         const float2 a2 = make_float2(a, a);
 #pragma unroll
-        for (int j = 0; j < Sh::COLS / 32; ++j) {
-          float t[32];
-          umma::tmem_ld_32x32(lanes + (n % OBUFS) * HD + 32 * j, t);
+        for (int j = 0; j < Sh::COLS; j += 16) {
+          float t[16];
+          umma::tmem_ld_32x16(lanes + (n % OBUFS) * HD + j, t);
           umma::tmem_ld_wait(t);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) o[16 * j + i] = __ffma2_rn(o[16 * j + i], a2, make_float2(t[2 * i], t[2 * i + 1]));
+          for (int i = 0; i < 8; ++i) o[j / 2 + i] = __ffma2_rn(o[j / 2 + i], a2, make_float2(t[2 * i], t[2 * i + 1]));
         }
       }
       umma::fence_before_sync();
@@ -604,13 +605,60 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
                             col0, Sh::COLS, whole ? p.out + attn_row_offset(p, it.row0, it.head, row, p.out_stride) + col0 : p.part + slot * HD + col0);
         }
       }
-      if (!whole && attn_arrive(p, share, &s_last, tid == 128 * Sh::W_GROUPS, 1, 128 * Sh::S_GROUPS)) {
+      if (!whole) {  // the first and the last at most
+        if (tid == 128 * Sh::W_GROUPS) s_parts[parts] = it;
+        ++parts;
+      }
+    }
+    // ---- items that other CTAs have tiles of: whoever comes last joins them
 #pragma unroll 1
-        for (int e = tid - 128 * Sh::W_GROUPS; e < n_rows * (HD / 4); e += 128 * Sh::S_GROUPS) {
-          const int r = e / (HD / 4), i = 4 * (e % (HD / 4));
-          if (i < p.hd)
-            *reinterpret_cast<float4*>(p.out + attn_row_offset(p, it.row0, it.head, r, p.out_stride) + i) = attn_join4<HD>(p, share, 128, r, i);
+    for (int i = 0; i < parts && ok; ++i) {
+      if (attn_arrive(p, s_parts[i].first_cta, s_parts[i].last_cta, &s_last, tid == 128 * Sh::W_GROUPS, 1, 128 * Sh::S_GROUPS)) {
+        const TileItem& it = s_parts[i];
+        const AttnShare share = {it.first_cta, it.last_cta};
+        const int n = share.last - share.first + 1, n_rows = it.n_rows, at = tid - 128 * Sh::W_GROUPS;
+        float* base = p.out + (size_t)it.row0 * p.out_stride + (size_t)it.head * p.g * p.hd;
+        if (n > JOIN_PARTS) {
+#pragma unroll 1
+          for (int r = at >> 5; r < n_rows; r += 4 * Sh::S_GROUPS) attn_join_row<HD>(p, share, 128, r, base + attn_row_offset(p, 0, 0, r, p.out_stride));
+          continue;
         }
+        // the parts' weights by row, then the sums by four columns, several in flight
+        float* s_w = reinterpret_cast<float*>(s_out);
+        static_assert(JOIN_PARTS * 128 * 4 <= Sh::OUT, "the parts' weights lie where results go");
+        if (at < n_rows) {
+          float M = -CUDART_INF_F, L = 0.f;
+#pragma unroll 4
+          for (int c = 0; c < n; ++c) {
+            const float2 ml = __ldcg(&p.part_ml[(size_t)attn_slot(share.first + c, share) * 128 + at]);
+            s_w[c * 128 + at] = ml.x;
+            M = fmaxf(M, ml.x);
+          }
+#pragma unroll 4
+          for (int c = 0; c < n; ++c) {
+            const float w = exp2_rel(s_w[c * 128 + at], M);
+            if (w != 0.f) L += w * __ldcg(&p.part_ml[(size_t)attn_slot(share.first + c, share) * 128 + at]).y;  // (a part that saw nothing holds nothing)
+            s_w[c * 128 + at] = w;
+          }
+          const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);  // NaN stays
+#pragma unroll 1
+          for (int c = 0; c < n; ++c) s_w[c * 128 + at] *= inv;
+        }
+        asm volatile("bar.sync 1, %0;" ::"n"(128 * Sh::S_GROUPS) : "memory");
+        const int words = p.hd / 4, stride = (int)p.out_stride, head_pitch = p.hd, g = p.g;
+#pragma unroll 4
+        for (int e = at; e < n_rows * words; e += 128 * Sh::S_GROUPS) {
+          const int r = e / words, col = 4 * (e - r * words), t = attn_row_token(p, r);
+          float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
+          for (int c = 0; c < n; ++c) {
+            const float w = s_w[c * 128 + r];
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(p.part + ((size_t)attn_slot(share.first + c, share) * 128 + r) * HD + col));
+            if (w != 0.f) o.x += w * v.x, o.y += w * v.y, o.z += w * v.z, o.w += w * v.w;
+          }
+          *reinterpret_cast<float4*>(base + col + (t * stride + (r - t * g) * head_pitch)) = o;
+        }
+        asm volatile("bar.sync 1, %0;" ::"n"(128 * Sh::S_GROUPS) : "memory");
       }
     }
     if (!ok && lane == 0) atomicExch(&p.status->timeout, 11);
