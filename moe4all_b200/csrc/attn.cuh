@@ -112,9 +112,10 @@ __device__ __forceinline__ uint32_t only_finite(uint32_t x) {
 
 // A CTA's share of the line: its tiles are those at the places [u0, u1).
 struct AttnStart {
-  long long units, u0, u1, ub;  // ub: where the block's first head begins
-  long long before, until;      // tiles ahead of u0 and of u1
-  int s, b, ctas;               // ctas: those that the line is shared by
+  AttnLine line;
+  long long u0, u1, ub;     // ub: where the block's first head begins
+  long long before, until;  // tiles ahead of u0 and of u1
+  int s, b;
 };
 
 // Inclusive sum over the block's threads; s_warp: one word per warp.
@@ -129,33 +130,34 @@ __device__ __forceinline__ long long block_scan(long long v, long long* s_warp) 
   __syncthreads();
   if (lane == 31) s_warp[warp] = v;
   __syncthreads();
-#pragma unroll
-  for (int w = 0; w < THREADS / 32; ++w)
-    if (w < warp) v += s_warp[w];
+#pragma unroll 1
+  for (int w = 0; w < warp; ++w) v += s_warp[w];
   return v;
 }
 
 // Every CTA works the whole line out for itself (a sequence and a few blocks per thread), which costs less than a launch for it.
-// pre: n_seq + 1 words of shared memory, free again after the call.  All threads take part.
+// known: 16 bytes per sequence and one word of shared memory, free again after the call.  All threads take part.
 template <int THREADS, int LOG2_TILE, int EXTRA>
-__device__ void attn_plan(const AttnParams& p, int* pre, long long* s_warp, AttnStart* st) {
+__device__ __forceinline__ void attn_plan(const AttnParams& p, int* known, long long* s_warp, AttnStart* st) {
   const int tid = threadIdx.x;
+  AttnSeq* seqs = reinterpret_cast<AttnSeq*>(known);
+  int* pre = known + 3 * p.n_seq;  // blocks ahead of each sequence
+  if (tid == 0) pre[0] = 0;
   long long carry = 0;
 #pragma unroll 1
   for (int s0 = 0; s0 < p.n_seq; s0 += THREADS) {
     const int s = s0 + tid;
-    const int n = s < p.n_seq ? attn_blocks(attn_load_seq(p, s).q_len, p.tb) : 0;
+    int n = 0;
+    if (s < p.n_seq) {
+      seqs[s] = attn_load_seq(p, s);
+      n = attn_blocks(seqs[s].q_len, p.tb);
+    }
     const long long sum = carry + block_scan<THREADS>(n, s_warp);
     if (s < p.n_seq) pre[s + 1] = (int)sum;
-    if (s0 == 0 && tid == 0) pre[0] = 0;
-    if (s0 + THREADS < p.n_seq) {
-      __syncthreads();
-      carry = pre[s0 + THREADS];
-    }
+    __syncthreads();
+    carry = pre[min(s0 + THREADS, p.n_seq)];
   }
-  __syncthreads();
-  const int F = pre[p.n_seq];
-  const int f0 = (int)((long long)tid * F / THREADS), f1 = (int)((long long)(tid + 1) * F / THREADS);
+  const int F = (int)carry, per = (F + THREADS - 1) / THREADS, f0 = min(tid * per, F), f1 = min(f0 + per, F);
   int s = 0;
 #pragma unroll 1
   for (int hi = p.n_seq; hi - s > 1;) {  // the last sequence that begins at or before block f0
@@ -163,50 +165,47 @@ __device__ void attn_plan(const AttnParams& p, int* pre, long long* s_warp, Attn
     if (pre[mid] <= f0) s = mid;
     else hi = mid;
   }
-  long long mine = 0;
-  if (f0 < f1) {
+  // twice along this thread's blocks: their tiles, then the blocks that the CTA's borders fall into
+  long long mine = 0, end = 0, u0 = 0, u1 = -1;
+#pragma unroll 1
+  for (int pass = 0; pass < 2; ++pass) {
+    long long tiles = end - mine;
     int at = s;
-    AttnSeq q = attn_load_seq(p, at);
 #pragma unroll 1
     for (int f = f0; f < f1; ++f) {
-      while (f >= pre[at + 1]) q = attn_load_seq(p, ++at);
-      mine += attn_block(q, f - pre[at], p.tb, LOG2_TILE, p.window).ntile;
-    }
-  }
-  const long long end = block_scan<THREADS>(mine, s_warp);
-  if (tid == THREADS - 1) {
-    st->units = (end + (long long)EXTRA * F) * p.n_kv;
-    st->ctas = (int)(st->units < (long long)gridDim.x ? st->units : (long long)gridDim.x);
-    const bool idle = (int)blockIdx.x >= st->ctas;
-    st->u0 = idle ? 0 : attn_begin(blockIdx.x, st->units, st->ctas);
-    st->u1 = idle ? 0 : attn_begin(blockIdx.x + 1, st->units, st->ctas);
-    st->before = 0;
-    st->until = idle ? 0 : end * p.n_kv;  // (where u1 is the line's end)
-  }
-  __syncthreads();
-  // the blocks that u0 and u1 fall into
-  const long long u0 = st->u0, u1 = st->u1;
-  long long tiles = end - mine, ub = (tiles + (long long)EXTRA * f0) * p.n_kv;
-  const long long ue = (end + (long long)EXTRA * f1) * p.n_kv;
-  if (u0 < u1 && ((u0 >= ub && u0 < ue) || (u1 >= ub && u1 < ue))) {
-    int at = s;
-    AttnSeq q = attn_load_seq(p, at);
+      while (f >= pre[at + 1]) ++at;
+      const int nt = attn_block(seqs[at], f - pre[at], p.tb, LOG2_TILE, p.window).ntile;
+      if (pass == 1) {
+        const long long ub = (tiles + (long long)EXTRA * f) * p.n_kv, n = (long long)(nt + EXTRA) * p.n_kv;
 #pragma unroll 1
-    for (int f = f0; f < f1; ++f) {
-      while (f >= pre[at + 1]) q = attn_load_seq(p, ++at);
-      const int nt = attn_block(q, f - pre[at], p.tb, LOG2_TILE, p.window).ntile;
-      const long long n = (long long)(nt + EXTRA) * p.n_kv;
-#pragma unroll 1
-      for (int k = 0; k < 2; ++k) {
-        const long long u = k == 0 ? u0 : u1;
-        if (u < ub || u >= ub + n) continue;
-        const int in = (int)((u - ub) % (nt + EXTRA)) - EXTRA;
-        const long long at_u = tiles * p.n_kv + (u - ub) / (nt + EXTRA) * nt + (in > 0 ? in : 0);
-        if (k == 0) st->s = at, st->b = f - pre[at], st->ub = ub, st->before = at_u;
-        else st->until = at_u;
+        for (int k = 0; k < 2; ++k) {
+          const long long u = k == 0 ? u0 : u1;
+          if (u < ub || u >= ub + n) continue;
+          const int head = attn_small_div(u - ub, nt + EXTRA), in = (int)(u - ub - (long long)head * (nt + EXTRA)) - EXTRA;
+          const long long ahead = tiles * p.n_kv + (long long)head * nt + (in > 0 ? in : 0);
+          if (k == 0) st->s = at, st->b = f - pre[at], st->ub = ub, st->before = ahead;
+          else st->until = ahead;
+        }
       }
-      ub += n;
       tiles += nt;
+    }
+    if (pass == 0) {
+      mine = tiles;
+      end = block_scan<THREADS>(mine, s_warp);
+      if (tid == THREADS - 1) {
+        const long long units = (end + (long long)EXTRA * F) * p.n_kv;
+        const int ctas = (int)(units < (long long)gridDim.x ? units : (long long)gridDim.x);
+        const bool idle = (int)blockIdx.x >= ctas;
+        st->line.each = ctas > 0 ? units / ctas : 0;
+        st->line.more = (int)(units - st->line.each * ctas);
+        st->u0 = idle ? 0 : attn_begin(st->line, blockIdx.x);
+        st->u1 = idle ? 0 : attn_begin(st->line, blockIdx.x + 1);
+        st->before = 0;
+        st->until = idle ? 0 : end * p.n_kv;  // (where u1 is the line's end)
+      }
+      __syncthreads();
+      u0 = st->u0, u1 = st->u1;
+      if (u0 >= u1) break;
     }
   }
   __syncthreads();
@@ -230,7 +229,7 @@ struct AttnCursor {
     s = st.s, b = st.b;
     seq = attn_load_seq(p, s);
     blk = attn_block(seq, b, p.tb, LOG2_TILE, p.window);
-    head = (int)((st.u0 - st.ub) / (blk.ntile + EXTRA));
+    head = attn_small_div(st.u0 - st.ub, blk.ntile + EXTRA);
     ub = st.ub + (long long)head * (blk.ntile + EXTRA) + EXTRA;
   }
   __device__ __forceinline__ void next(const AttnParams& p) {
@@ -295,7 +294,7 @@ struct AttnShare {
   int first, last;
 };
 __device__ __forceinline__ AttnShare attn_share(long long ub, int ntile, const AttnStart& st) {
-  return {attn_cta_of(ub, st.units, st.ctas), attn_cta_of(ub + ntile - 1, st.units, st.ctas)};
+  return {attn_cta_of(st.line, ub), attn_cta_of(st.line, ub + ntile - 1)};
 }
 __device__ __forceinline__ int attn_slot(int cta, const AttnShare& sh) { return 2 * cta + (cta == sh.first ? 1 : 0); }
 

@@ -52,6 +52,7 @@ __global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
   __shared__ long long s_scan[WARPS];
   __shared__ AttnStart s_start;
   __shared__ int s_last;
+  __shared__ float s_weight[RB];
   unsigned char* ring_all = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   float* s_o = reinterpret_cast<float*>(ring_all + WARPS * STAGES * SLICE);
   float* s_m = s_o + WARPS * RB * PITCH;
@@ -79,6 +80,7 @@ __global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
   int a_key = -1, a_page = 0;           // first key of the slice to ask for (-1: none left) and its page
   uint32_t asked = 0;
   auto find = [&]() {                   // the next tile of which this warp has keys
+#pragma unroll 1
     while (ahead.ub < st.u1) {
       if (at >= ahead.end(st)) {
         ahead.next(p);
@@ -113,6 +115,7 @@ __global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
     find();
   };
   find();
+#pragma unroll 1
   for (int i = 0; i < STAGES; ++i) ask();
 
   AttnCursor<Sh::LOG2_TILE, ROWS_EXTRA> cur;
@@ -121,6 +124,7 @@ __global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
   bool alive = true;
   const int c0 = 2 * (lane & 3);  // this thread's columns (rows of the item): c0, c0 + 1 of every eight
   long long left = st.until - st.before;  // tiles
+#pragma unroll 1
   for (;; cur.next(p)) {
     const AttnBlock& blk = cur.blk;
     const int first_tile = cur.first(st), end_tile = cur.end(st), n_rows = blk.nt * p.g;
@@ -172,6 +176,7 @@ __global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
     for (int n = 0; n < NT; ++n) m[n][0] = m[n][1] = -CUDART_INF_F, l[n][0] = l[n][1] = 0.f;
 
     bool odd = false;  // values that are not finite were left out
+#pragma unroll 1
     for (int t = first_tile; t < end_tile; ++t) {
       const int ks = ((blk.tile0 + t) << Sh::LOG2_TILE) + warp * 16;
       if (ks >= blk.hi || ks + 16 <= blk.lo) continue;
@@ -183,20 +188,26 @@ __global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
       if (alive) {
         const uint32_t kb = smem_u32(ring + stage * SLICE), vb = kb + SLICE / 2;
         const int i4 = lane >> 3, r8 = lane & 7;
-        // ---- scores
-        float s[NT][4];
+        // ---- scores: pieces and even and odd steps apart, four chains of products instead of one
+        float s[NT][4], part[NT][3][4];
 #pragma unroll
-        for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[n][i] = part[n][0][i] = part[n][1][i] = part[n][2][i] = 0.f;
 #pragma unroll
         for (int k = 0; k < KST; ++k) {
           uint32_t a[4];
           ldsm4(a, kb + (k >> 2) * 2048 + ((i4 & 1) * 8 + r8) * 128 + (((2 * (k & 3) + (i4 >> 1)) ^ r8) << 4));
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            mma16816(s[n], a, qh[n][k][0], qh[n][k][1]);
-            mma16816(s[n], a, ql[n][k][0], ql[n][k][1]);
+            mma16816(k & 1 ? part[n][0] : s[n], a, qh[n][k][0], qh[n][k][1]);
+            mma16816(k & 1 ? part[n][2] : part[n][1], a, ql[n][k][0], ql[n][k][1]);
           }
         }
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[n][i] = (s[n][i] + part[n][0][i]) + (part[n][1][i] + part[n][2][i]);
         const bool masked = ks + 16 > full_hi || ks < full_lo;
         const int key = ks + (lane >> 2);
         float mx[NT][2];
@@ -252,23 +263,27 @@ __global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
 #pragma unroll
           for (int i = 0; i < 2; ++i) ph[n][i] = movm(ph[n][i]), pl[n][i] = movm(pl[n][i]);
         }
-        // ---- sums.  Where some row does not see some key, 0 x value must be 0 whatever the value: keys that no row sees count as
-        // zeros, and values that are not finite wait for the item's end.
-        const int vk = ks + c0;  // this thread's keys of V^T: vk, vk + 1 and eight further on
+        // ---- sums.  Where some row does not see some key, 0 x value must be 0 whatever the value: keys that no row sees become zeros, and
+        // so do values that are not finite, which wait for the item's end.
+        if (masked) {
+          unsigned char* vs = ring + stage * SLICE + SLICE / 2;
+#pragma unroll 1
+          for (int e = lane; e < 16 * SLABS * 8; e += 32) {  // 16-byte words, 128 bytes of a key after the other
+            const int kk = ks + ((e >> 3) & 15);
+            uint4* w = reinterpret_cast<uint4*>(vs) + e;
+            const uint4 x = *w;
+            uint4 y = make_uint4(only_finite(x.x), only_finite(x.y), only_finite(x.z), only_finite(x.w));
+            if (kk >= blk.hi || kk < blk.lo) y = make_uint4(0, 0, 0, 0);
+            else odd |= x.x != y.x || x.y != y.y || x.z != y.z || x.w != y.w;
+            *w = y;
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // (ahead of the slot's next copy)
+          __syncwarp();
+        }
 #pragma unroll
         for (int k = 0; k < KST; ++k) {
           uint32_t a[4];
           ldsm4_t(a, vb + (k >> 2) * 2048 + ((i4 >> 1) * 8 + r8) * 128 + (((2 * (k & 3) + (i4 & 1)) ^ r8) << 4));
-          if (masked) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int kk = vk + 8 * (i >> 1);
-              if (kk >= blk.hi || kk < blk.lo) a[i] &= 0xFFFF0000u;
-              if (kk + 1 >= blk.hi || kk + 1 < blk.lo) a[i] &= 0x0000FFFFu;
-              if ((a[i] & 0x7C00u) == 0x7C00u) a[i] &= 0xFFFF0000u, odd = true;
-              if ((a[i] & 0x7C000000u) == 0x7C000000u) a[i] &= 0x0000FFFFu, odd = true;
-            }
-          }
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             mma16816(o[k][n], a, ph[n][0], ph[n][1]);
@@ -281,43 +296,12 @@ __global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
       }
     }
 
-    // ---- values that are not finite: a product of pieces makes NaN of them (inf times a piece of the other sign, or of zero), so what the
-    // rows that see them get is put together by itself.  Ordinary calls only look.
 #pragma unroll
     for (int k = 0; k < KST; ++k)
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int i = 0; i < 4; ++i) odd |= !(fabsf(o[k][n][i]) < CUDART_INF_F);
-    if (__any_sync(0xFFFFFFFFu, odd)) {
-#pragma unroll
-      for (int k = 0; k < KST; ++k)
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const int i = 16 * k + 8 * half + (lane >> 2);
-          float add[NT][2] = {};
-          bool has[NT][2] = {};
-          for (int t = first_tile; t < end_tile && i < p.hd; ++t) {
-            const int ks = ((blk.tile0 + t) << Sh::LOG2_TILE) + warp * 16;
-            if (ks >= blk.hi || ks + 16 <= blk.lo) continue;
-            const __half* at = attn_value(p, cur.s, cur.seq.q0, cur.head, ks) + i;
-            for (int key = max(ks, blk.lo); key < min(ks + 16, blk.hi); ++key) {
-              const float x = __half2float(at[(size_t)(key - ks) * p.row_pitch]);
-              if (fabsf(x) < CUDART_INF_F) continue;
-#pragma unroll
-              for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-                  if (key <= lim[n][j] && (p.window == 0 || key > lim[n][j] - p.window)) add[n][j] += x, has[n][j] = true;
-            }
-          }
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-              if (has[n][j]) o[k][n][2 * half + j] = add[n][j];
-        }
-    }
 
     // ---- the warps' parts of the item
 #pragma unroll
@@ -346,7 +330,7 @@ __global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
         }
       }
     }
-    __syncthreads();
+    const bool any_odd = __syncthreads_or(odd) != 0;
     const bool whole = first_tile == 0 && end_tile == blk.ntile;
     const AttnShare share = attn_share(cur.ub, blk.ntile, st);
     auto store = [&](int r, int i, float4 v) {
@@ -376,6 +360,15 @@ __global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
         __stcg(reinterpret_cast<float4*>(p.part + at * HD + i), sum);
         if (i == 0) __stcg(p.part_ml + at, make_float2(M, L));
       }
+      if (i == 0) s_weight[r] = L;
+    }
+    if (any_odd) {  // some value that a row sees may not be finite: put together by itself
+      __threadfence();
+      __syncthreads();
+      if (tid < n_rows && s_weight[tid] == s_weight[tid])
+        attn_odd_values(p, cur.s, cur.seq.q0, cur.head, (blk.tile0 + first_tile) << Sh::LOG2_TILE, (blk.tile0 + end_tile) << Sh::LOG2_TILE, 16, full_lo, full_hi,
+                        cur.seq.past + blk.t0 + attn_row_token(p, tid), 0, HD,
+                        whole ? p.out + attn_row_offset(p, cur.seq.q0 + blk.t0, cur.head, tid, p.out_stride) : p.part + ((size_t)attn_slot(blockIdx.x, share) * RB + tid) * HD);
     }
     if (!whole && attn_arrive(p, share.first, share.last, &s_last, tid == 0, 0, THREADS)) {
 #pragma unroll 1

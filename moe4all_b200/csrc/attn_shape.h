@@ -3,8 +3,7 @@
 //
 // An item is a block of consecutive new tokens of one sequence with the query heads of one kv head; its work is the key tiles that some row
 // of it sees, and some units more for its beginning and end (its q, its results).  Items in order (sequence, block, kv head), each as
-// `extra` units and then its tiles, form one line, which the CTAs of the launch share evenly: CTA c of C takes the tiles in
-// [c U / C, (c + 1) U / C).  An item whose tiles cross a border is joined from its CTAs' partial results, in their order, by whichever
+// `extra` units and then its tiles, form one line, which the CTAs of the launch share evenly: a CTA takes the tiles in its piece.  An item whose tiles cross a border is joined from its CTAs' partial results, in their order, by whichever
 // finishes last.
 #pragma once
 #include <cstddef>
@@ -18,7 +17,7 @@
 
 namespace infr {
 
-constexpr int ATTN_MAX_SEQ = 16384;    // sequences per call: the blocks' prefix sums fit where the key tiles go later
+constexpr int ATTN_MAX_SEQ = 4096;     // sequences per call: what is known of them fits where the key tiles go later (16 bytes each)
 constexpr int ATTN_MAX_CTAS = 1024;    // join counters of a context
 constexpr int ATTN_ROWS_LIMIT = 16;    // rows (tokens x heads of a kv head) of an item of the few-rows kernel
 constexpr int ATTN_TILE_ROWS = 128;    // and of the tensor-memory kernel
@@ -62,9 +61,25 @@ INFR_ATTN_HD AttnBlock attn_block(const AttnSeq& s, int b, int tb, int log2_tile
   return r;
 }
 
-// Where CTA c of C begins in a line of u units, and which CTA has the tile at place i.
-INFR_ATTN_HD long long attn_begin(int c, long long u, int C) { return (long long)c * u / C; }
-INFR_ATTN_HD int attn_cta_of(long long i, long long u, int C) { return (int)(((i + 1) * C - 1) / u); }
+// a / b for quotients below 2^20: an estimate in f32 is off by one at most (64-bit divisions are a hundred instructions each).
+INFR_ATTN_HD int attn_small_div(long long a, long long b) {
+  int q = (int)((float)a / (float)b);
+  if ((long long)q * b > a) --q;
+  if ((long long)(q + 1) * b <= a) ++q;
+  return q;
+}
+
+// A line of u units over C CTAs: the first `more` have each + 1, the others `each`.
+struct AttnLine {
+  long long each;
+  int more;
+};
+// Where CTA c begins, and which CTA has the tile at place i.
+INFR_ATTN_HD long long attn_begin(const AttnLine& l, int c) { return c * l.each + (c < l.more ? c : l.more); }
+INFR_ATTN_HD int attn_cta_of(const AttnLine& l, long long i) {
+  const long long wide = l.more * (l.each + 1);
+  return i < wide ? attn_small_div(i, l.each + 1) : l.more + attn_small_div(i - wide, l.each);
+}
 
 // What a call gives, as numbers.
 struct AttnSizes {
@@ -84,7 +99,7 @@ inline const char* attn_sizes_error(const AttnSizes& s, bool* unsupported) {
   *unsupported = true;
   if (s.head_dim % 16 || s.head_dim > 256) return "head_dim must be a multiple of 16, at most 256";
   if (s.n_head / s.n_kv > (uint32_t)ATTN_TILE_ROWS) return "more than 128 query heads to a kv head";
-  if (s.n_seq > (uint32_t)ATTN_MAX_SEQ) return "more than 16384 sequences per call";
+  if (s.n_seq > (uint32_t)ATTN_MAX_SEQ) return "more than 4096 sequences per call";
   if (s.rows > (1u << 22) || s.n_head > 1024) return "more than 2^22 rows or 1024 heads";
   if (s.paged && s.page_size % 16) return "page_size must be a multiple of 16";
   if (s.paged && s.n_pages > (1u << 30)) return "more than 2^30 pages";

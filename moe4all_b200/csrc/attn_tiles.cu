@@ -21,13 +21,13 @@ namespace infr {
 namespace {
 
 constexpr float TILE_BIAS = 15.f;  // weights are 2^(x - maximum + 15): below f16's limit, 2^-40 of the largest still has a bit
-constexpr int EXTRA = 2;           // tiles' time that an item's beginning and end take
 constexpr int JOIN_PARTS = 32;     // parts of an item that are joined by column; more go row by row
 constexpr int RING = 4;            // tiles' and items' words in shared memory: the roles are never further apart
 
 template <int HD>
 struct TilesShape {
   static constexpr int LOG2_TILE = HD <= 128 ? 7 : 6, BK = 1 << LOG2_TILE;
+  static constexpr int EXTRA = HD == 64 ? 2 : 3;  // tiles' time that an item's beginning and end take
   static constexpr int W_GROUPS = BK / 64;
   static constexpr int S_GROUPS = 3 - W_GROUPS, COLS = HD / S_GROUPS;  // columns of a sums thread
   static constexpr int THREADS = 512;
@@ -124,7 +124,7 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
   if (tid < 4 * RING) s_odd[tid] = 0;
   if (warp == 0) umma::tmem_alloc(&s_tmem);
   pdl_wait();
-  attn_plan<Sh::THREADS, Sh::LOG2_TILE, EXTRA>(p, reinterpret_cast<int*>(s_q), s_scan, &s_start);
+  attn_plan<Sh::THREADS, Sh::LOG2_TILE, Sh::EXTRA>(p, reinterpret_cast<int*>(s_q), s_scan, &s_start);
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the plan's words lay where tiles go
   umma::fence_before_sync();
   __syncthreads();
@@ -139,7 +139,7 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
     // nothing to do
   } else if (role == 3) {
     // ---- copies, and the items' words
-    AttnCursor<Sh::LOG2_TILE, EXTRA> c;
+    AttnCursor<Sh::LOG2_TILE, Sh::EXTRA> c;
     c.start(p, st);
     int t = c.first(st), t_end = 0;  // the tile of its item that comes next, and where its tiles end here
     const int pieces = BK / granule;
@@ -358,7 +358,6 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
     constexpr int GROUPS = Sh::W_GROUPS;
     const int row = tid & 127;
     const uint32_t mine = tmem + ((uint32_t)((warp & 3) * 32) << 16) + 64 * wg;
-#pragma unroll 1
     // q of an item into two f16 pieces: eight lanes a row, the next rows on their way meanwhile.  What is left in the rows past the item's
     // reaches these rows' sums only.  (A short rolled loop: code that runs once an item comes from far away.)
     auto convert = [&](int item) {

@@ -47,21 +47,25 @@ static int line(int argc, char** argv) {
       }
   }
   const int C = (int)(units < grid ? units : grid);
+  const AttnLine l = {C ? units / C : 0, C ? (int)(units % C) : 0};
+  for (long long a : {units, 7 * units + 3, units / 3, (1ll << 45) + units})
+    for (long long b : {units + 1, units / 2 + 5, (1ll << 30) + 3})
+      if (a / b < (1 << 20) && attn_small_div(a, b) != a / b) return std::puts("small_div"), 1;
   std::map<long long, std::set<int>> slots;  // by the item's first unit
   std::map<long long, long long> covered;
   std::set<int> used;
   std::map<int, long long> counter;  // join counter -> item
   long long at = 0;
   for (int c = 0; c < C; ++c) {
-    const long long u0 = attn_begin(c, units, C), u1 = attn_begin(c + 1, units, C);
+    const long long u0 = attn_begin(l, c), u1 = attn_begin(l, c + 1);
     if (u0 != at || u1 <= u0) return std::puts("units not shared"), 1;
     at = u1;
     for (const Item& it : items) {
       const long long a = u0 > it.ub ? u0 : it.ub, e = u1 < it.ub + it.blk.ntile ? u1 : it.ub + it.blk.ntile;
       if (a >= e) continue;
       covered[it.ub] += e - a;
-      if (attn_cta_of(a, units, C) != c || attn_cta_of(e - 1, units, C) != c) return std::puts("cta_of"), 1;
-      const int first = attn_cta_of(it.ub, units, C), last = attn_cta_of(it.ub + it.blk.ntile - 1, units, C);
+      if (attn_cta_of(l, a) != c || attn_cta_of(l, e - 1) != c) return std::puts("cta_of"), 1;
+      const int first = attn_cta_of(l, it.ub), last = attn_cta_of(l, it.ub + it.blk.ntile - 1);
       if (a == it.ub && e == it.ub + it.blk.ntile) {
         if (first != c || last != c) return std::puts("a whole item is not whole"), 1;
         continue;
@@ -77,7 +81,7 @@ static int line(int argc, char** argv) {
   if (units && at != units) return std::puts("units left"), 1;
   for (const Item& it : items) {
     if (covered[it.ub] != it.blk.ntile) return std::puts("tiles lost"), 1;
-    const int first = attn_cta_of(it.ub, units, C), last = attn_cta_of(it.ub + it.blk.ntile - 1, units, C);
+    const int first = attn_cta_of(l, it.ub), last = attn_cta_of(l, it.ub + it.blk.ntile - 1);
     if (slots.count(it.ub) && (int)slots[it.ub].size() != last - first + 1) return std::puts("parts missing"), 1;
   }
   std::printf("%lld %zu %zu %d\n", tiles, items.size(), slots.size(), (int)bad);
