@@ -65,12 +65,14 @@ __device__ __forceinline__ AttnSeq attn_load_seq(const AttnParams& p, int s) {
   return r;
 }
 
-__device__ __forceinline__ int attn_page(const AttnParams& p, int s, int page) {
-  const int id = __ldcg(p.page_table + (size_t)s * p.max_pages + page);
+// A page's number as the table has it, and made sure of: apart, so that what lies between hides the load.
+__device__ __forceinline__ int attn_page_entry(const AttnParams& p, int s, int page) { return __ldcg(p.page_table + (size_t)s * p.max_pages + page); }
+__device__ __forceinline__ int attn_page_checked(const AttnParams& p, int id) {
   if ((unsigned)id < (unsigned)p.n_pages) return id;
   p.status->bad_index = 2;  // read as page 0, reported at the next sync
   return 0;
 }
+__device__ __forceinline__ int attn_page(const AttnParams& p, int s, int page) { return attn_page_checked(p, attn_page_entry(p, s, page)); }
 
 // Token (of the item) and query head (of the kv head) of row r < 128: the error of g_inv adds less than 1 / 512.
 __device__ __forceinline__ int attn_row_token(const AttnParams& p, int r) { return (int)((uint32_t)r * p.g_inv >> 16); }

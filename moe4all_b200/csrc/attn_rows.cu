@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
       const int ks = ((ahead.blk.tile0 + at) << Sh::LOG2_TILE) + warp * 16;
       if (ks < ahead.blk.hi && ks + 16 > ahead.blk.lo) {
         a_key = ks;
-        if (!packed) a_page = attn_page(p, ahead.s, ks / p.page_size);
+        if (!packed) a_page = attn_page_entry(p, ahead.s, ks / p.page_size);
         return;
       }
       ++at;
@@ -103,7 +103,7 @@ __global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
       const int stage = asked % STAGES;
       unsigned char* dst = ring + stage * SLICE;
       mbar_arrive_expect_tx(full + stage, SLICE);
-      const int y = packed ? ahead.seq.q0 + a_key : a_key % p.page_size, w = packed ? 0 : a_page;
+      const int y = packed ? ahead.seq.q0 + a_key : a_key % p.page_size, w = packed ? 0 : attn_page_checked(p, a_page);
 #pragma unroll
       for (int s = 0; s < SLABS; ++s) {
         tma_load_4d(dst + s * 2048, &kmap, 64 * s, y, ahead.head, w, full + stage);

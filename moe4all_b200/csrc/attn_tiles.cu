@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
         at.y = c.seq.q0 + key;
         if (!packed) {
           const int page = key / p.page_size;
-          at.w = attn_page(p, c.s, page);
+          at.w = attn_page_entry(p, c.s, page);
           at.y = key - page * p.page_size;
         }
       }
@@ -194,9 +194,10 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
       if (lane == 0) mbar_arrive_expect_tx(full, (uint32_t)(count * granule * 128 * SLABS));
       __syncwarp();
       if (at.y >= 0) {
+        const int w = packed ? 0 : attn_page_checked(p, at.w);
         unsigned char* dst = bufs + buf * TILE + lane * granule * 128;
 #pragma unroll
-        for (int s = 0; s < SLABS; ++s) tma_load_4d(dst + s * (BK * 128), map, 64 * s, at.y, at.head, at.w, full);
+        for (int s = 0; s < SLABS; ++s) tma_load_4d(dst + s * (BK * 128), map, 64 * s, at.y, at.head, w, full);
       }
       __syncwarp();
       asked = n + 1;
