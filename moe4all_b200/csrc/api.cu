@@ -1187,6 +1187,9 @@ int32_t infr_cuda_attention(infr_cuda_ctx* ctx, const infr_cuda_attention_desc* 
   p.window = (int)d->window;
   p.scale_log2 = (float)((double)d->scale * 1.4426950408889634);
   p.count = ctx->attn_count;
+  p.page_shift = -1;
+  for (int i = 4; i < 31; ++i)
+    if (d->page_size == (1u << i)) p.page_shift = i;
   const uint64_t max_rows = (uint64_t)(d->max_q && d->max_q < d->rows ? d->max_q : d->rows) * g;
   const bool few = d->path ? d->path == 1 : max_rows <= (uint64_t)ATTN_ROWS_LIMIT;
   const size_t item_rows = few ? ATTN_ROWS_LIMIT : ATTN_TILE_ROWS, slots = 2 * (size_t)ctx->sm_count;

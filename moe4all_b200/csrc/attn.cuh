@@ -24,6 +24,7 @@ struct AttnParams {
   int tb;            // tokens of an item
   uint32_t g_inv;    // ceil(2^16 / g): r / g = r * g_inv >> 16 for the rows r of an item
   int cap;           // max_pages * page_size
+  int page_shift;    // log2(page_size), or -1
 };
 
 // Weights are 2^(x - reference + ATTN_BIAS): the reference follows the running maximum only when that has grown by ATTN_SLACK, so
@@ -65,6 +66,8 @@ __device__ __forceinline__ AttnSeq attn_load_seq(const AttnParams& p, int s) {
   return r;
 }
 
+// The page that a key is in (a division is a tenth of a slice's instructions).
+__device__ __forceinline__ int attn_page_of(const AttnParams& p, int key) { return p.page_shift >= 0 ? key >> p.page_shift : key / p.page_size; }
 // A page's number as the table has it, and made sure of: apart, so that what lies between hides the load.
 __device__ __forceinline__ int attn_page_entry(const AttnParams& p, int s, int page) { return __ldcg(p.page_table + (size_t)s * p.max_pages + page); }
 __device__ __forceinline__ int attn_page_checked(const AttnParams& p, int id) {
@@ -83,9 +86,9 @@ __device__ __forceinline__ size_t attn_row_offset(const AttnParams& p, int token
 
 // Where the values of a key and head begin; the keys behind it follow row_pitch apart up to its page's end.
 __device__ __forceinline__ const __half* attn_value(const AttnParams& p, int s, int q0, int head, int key) {
-  const size_t at = p.page_table == nullptr ? (size_t)(q0 + key) * p.row_pitch
-                                            : (size_t)attn_page(p, s, key / p.page_size) * p.page_pitch + (size_t)(key % p.page_size) * p.row_pitch;
-  return p.v + at + (size_t)head * p.head_pitch;
+  if (p.page_table == nullptr) return p.v + (size_t)(q0 + key) * p.row_pitch + (size_t)head * p.head_pitch;
+  const int page = attn_page_of(p, key);
+  return p.v + (size_t)attn_page(p, s, page) * p.page_pitch + (size_t)(key - page * p.page_size) * p.row_pitch + (size_t)head * p.head_pitch;
 }
 
 // Powers of two that bring a row whose largest magnitude is `big` to [2^7, 2^8), and back; both normal numbers.

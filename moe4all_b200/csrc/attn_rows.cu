@@ -32,21 +32,26 @@ constexpr int ROWS_EXTRA = 1;  // tiles' time that an item's beginning and end t
 
 template <int HD, int NT>
 struct RowsShape {
-  static constexpr int WARPS = HD > 128 ? 4 : 8, THREADS = WARPS * 32, RB = 8 * NT;
-  static constexpr int LOG2_TILE = HD > 128 ? 6 : 7;  // 16 keys a warp
-  static constexpr int SLICE = 2 * 16 * HD * 2;       // bytes of 16 keys of K and V
-  static constexpr int PITCH = HD + 4;                // words: the fragments' columns fall on different banks
-  static constexpr int MERGE = WARPS * RB * PITCH * 4, STATS = 2 * WARPS * RB * 4;
-  static constexpr int FIT = (232448 - 1024 - 1024 - MERGE - STATS) / (WARPS * SLICE);
-  static constexpr int STAGES = FIT > 6 ? 6 : FIT;
-  static constexpr int SMEM = 1024 + WARPS * STAGES * SLICE + MERGE + STATS + WARPS * STAGES * 8;
+  static constexpr int WARPS = 8, THREADS = WARPS * 32, RB = 8 * NT;
+  static constexpr int LOG2_TILE = 7;              // 16 keys a warp
+  static constexpr int SIDE = 16 * HD * 2;         // bytes of 16 keys of K, or of V
+  // A unit of the ring is both where eight warps' rings hold two of them or more, else (heads wider than 128) one of the two: K's place is
+  // asked for again while V is used.  (Apart, heads of 128 lose: 93 -> 106 us for 64 streams.)
+  static constexpr bool PAIRED = HD <= 128;
+  static constexpr int UNIT = PAIRED ? 2 * SIDE : SIDE;
+  static constexpr int PITCH = HD + 4;             // words: the fragments' columns fall on different banks
+  static constexpr int SLOTS = PAIRED ? WARPS : WARPS / 2;  // wide heads: half of the warps add theirs to the others' first
+  static constexpr int MERGE = SLOTS * RB * PITCH * 4, STATS = 2 * WARPS * RB * 4;
+  static constexpr int FIT = (232448 - 1024 - 1024 - MERGE - STATS) / (WARPS * UNIT);
+  static constexpr int UNITS = FIT > 6 ? 6 : FIT;
+  static constexpr int SMEM = 1024 + WARPS * UNITS * UNIT + MERGE + STATS + WARPS * UNITS * 8;
 };
 
 template <int HD, int NT>
 __global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
     k_attn_rows(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ AttnParams p) {
   using Sh = RowsShape<HD, NT>;
-  constexpr int WARPS = Sh::WARPS, THREADS = Sh::THREADS, RB = Sh::RB, STAGES = Sh::STAGES, SLICE = Sh::SLICE, PITCH = Sh::PITCH;
+  constexpr int WARPS = Sh::WARPS, THREADS = Sh::THREADS, RB = Sh::RB, UNITS = Sh::UNITS, UNIT = Sh::UNIT, SIDE = Sh::SIDE, PITCH = Sh::PITCH, SLOTS = Sh::SLOTS;
   constexpr int SLABS = HD / 64, KST = HD / 16;
   extern __shared__ unsigned char smem_raw[];
   __shared__ long long s_scan[WARPS];
@@ -54,16 +59,16 @@ __global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
   __shared__ int s_last;
   __shared__ float s_weight[RB];
   unsigned char* ring_all = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  float* s_o = reinterpret_cast<float*>(ring_all + WARPS * STAGES * SLICE);
-  float* s_m = s_o + WARPS * RB * PITCH;
+  float* s_o = reinterpret_cast<float*>(ring_all + WARPS * UNITS * UNIT);
+  float* s_m = s_o + SLOTS * RB * PITCH;
   float* s_l = s_m + WARPS * RB;
   uint64_t* bars = reinterpret_cast<uint64_t*>(s_l + WARPS * RB);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  unsigned char* ring = ring_all + warp * STAGES * SLICE;
-  uint64_t* full = bars + warp * STAGES;
+  unsigned char* ring = ring_all + warp * UNITS * UNIT;
+  uint64_t* full = bars + warp * UNITS;
 
   if (lane == 0)
-    for (int i = 0; i < STAGES; ++i) mbar_init(full + i, 1);
+    for (int i = 0; i < UNITS; ++i) mbar_init(full + i, 1);
   mbar_fence_init();
   pdl_wait();
   attn_plan<THREADS, Sh::LOG2_TILE, ROWS_EXTRA>(p, reinterpret_cast<int*>(ring_all), s_scan, &s_start);
@@ -73,11 +78,11 @@ __global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
   __syncthreads();
 
   const bool packed = p.page_table == nullptr;
-  // ---- what the warp asks for: its slices of the CTA's tiles, one after the other, STAGES of them ahead of their use
+  // ---- what the warp asks for: K and V of its slices of the CTA's tiles, one after the other, as many as its ring holds
   AttnCursor<Sh::LOG2_TILE, ROWS_EXTRA> ahead;
   ahead.start(p, st);
   int at = ahead.first(st);             // tile of its item to look at next
-  int a_key = -1, a_page = 0;           // first key of the slice to ask for (-1: none left) and its page
+  int a_key = -1, a_page = 0, a_y = 0;  // first key of the slice to ask for (-1: none left), its page, its place there
   uint32_t asked = 0;
   auto find = [&]() {                   // the next tile of which this warp has keys
 #pragma unroll 1
@@ -90,33 +95,41 @@ __global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
       const int ks = ((ahead.blk.tile0 + at) << Sh::LOG2_TILE) + warp * 16;
       if (ks < ahead.blk.hi && ks + 16 > ahead.blk.lo) {
         a_key = ks;
-        if (!packed) a_page = attn_page_entry(p, ahead.s, ks / p.page_size);
+        a_y = ahead.seq.q0 + ks;
+        if (!packed) {
+          const int page = attn_page_of(p, ks);
+          a_page = attn_page_entry(p, ahead.s, page);
+          a_y = ks - page * p.page_size;
+        }
         return;
       }
       ++at;
     }
     a_key = -1;
   };
-  auto ask = [&]() {
+  auto ask_next = [&]() {  // K and V in turn, or both
     if (a_key < 0) return;
     if (lane == 0) {
-      const int stage = asked % STAGES;
-      unsigned char* dst = ring + stage * SLICE;
-      mbar_arrive_expect_tx(full + stage, SLICE);
-      const int y = packed ? ahead.seq.q0 + a_key : a_key % p.page_size, w = packed ? 0 : attn_page_checked(p, a_page);
+      const int at = asked % UNITS;
+      unsigned char* dst = ring + at * UNIT;
+      mbar_arrive_expect_tx(full + at, UNIT);
+      const int y = a_y, w = packed ? 0 : attn_page_checked(p, a_page);
+      const CUtensorMap* map = Sh::PAIRED || !(asked & 1) ? &kmap : &vmap;
 #pragma unroll
       for (int s = 0; s < SLABS; ++s) {
-        tma_load_4d(dst + s * 2048, &kmap, 64 * s, y, ahead.head, w, full + stage);
-        tma_load_4d(dst + SLICE / 2 + s * 2048, &vmap, 64 * s, y, ahead.head, w, full + stage);
+        tma_load_4d(dst + s * 2048, map, 64 * s, y, ahead.head, w, full + at);
+        if (Sh::PAIRED) tma_load_4d(dst + SIDE + s * 2048, &vmap, 64 * s, y, ahead.head, w, full + at);
       }
     }
     ++asked;
-    ++at;
-    find();
+    if (Sh::PAIRED || !(asked & 1)) {
+      ++at;
+      find();
+    }
   };
   find();
 #pragma unroll 1
-  for (int i = 0; i < STAGES; ++i) ask();
+  for (int i = 0; i < UNITS; ++i) ask_next();
 
   AttnCursor<Sh::LOG2_TILE, ROWS_EXTRA> cur;
   cur.start(p, st);
@@ -180,13 +193,12 @@ __global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
     for (int t = first_tile; t < end_tile; ++t) {
       const int ks = ((blk.tile0 + t) << Sh::LOG2_TILE) + warp * 16;
       if (ks >= blk.hi || ks + 16 <= blk.lo) continue;
-      const int stage = used % STAGES;
       if (alive) {
-        alive = wait_all(full + stage, used / STAGES);
+        alive = wait_all(full + used % UNITS, used / UNITS);
         if (!alive && lane == 0) atomicExch(&p.status->timeout, 10);
       }
       if (alive) {
-        const uint32_t kb = smem_u32(ring + stage * SLICE), vb = kb + SLICE / 2;
+        const uint32_t kb = smem_u32(ring + (used % UNITS) * UNIT);
         const int i4 = lane >> 3, r8 = lane & 7;
         // ---- scores: pieces and even and odd steps apart, four chains of products instead of one
         float s[NT][4], part[NT][3][4];
@@ -208,9 +220,14 @@ __global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int i = 0; i < 4; ++i) s[n][i] = (s[n][i] + part[n][0][i]) + (part[n][1][i] + part[n][2][i]);
+        if (!Sh::PAIRED) {
+          __syncwarp();
+          ++used;
+          ask_next();
+        }
         const bool masked = ks + 16 > full_hi || ks < full_lo;
         const int key = ks + (lane >> 2);
-        float mx[NT][2];
+        bool grows = false;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -222,23 +239,18 @@ __global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
               if (key > to || key <= from) s[n][j] = -CUDART_INF_F;
               if (key + 8 > to || key + 8 <= from) s[n][2 + j] = -CUDART_INF_F;
             }
-            mx[n][j] = fmaxf(s[n][j], s[n][2 + j]);
+            grows |= fmaxf(s[n][j], s[n][2 + j]) > m[n][j] + ATTN_SLACK;
           }
-        bool grows = false;
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-#pragma unroll
-            for (int x = 4; x < 32; x <<= 1) mx[n][j] = fmaxf(mx[n][j], __shfl_xor_sync(0xFFFFFFFFu, mx[n][j], x));
-            grows |= mx[n][j] > m[n][j] + ATTN_SLACK;
-          }
+        // (the maximum is looked for only where a score is past the slack: one vote instead of three rounds of shuffles)
         if (__any_sync(0xFFFFFFFFu, grows)) {
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-              const float to = mx[n][j] > m[n][j] + ATTN_SLACK ? mx[n][j] : m[n][j];
+              float mx = fmaxf(s[n][j], s[n][2 + j]);
+#pragma unroll
+              for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, x));
+              const float to = mx > m[n][j] + ATTN_SLACK ? mx : m[n][j];
               const float w = to == m[n][j] ? 1.f : exp2_rel(m[n][j], to);
               m[n][j] = to;
               l[n][j] *= w;
@@ -265,8 +277,16 @@ __global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
         }
         // ---- sums.  Where some row does not see some key, 0 x value must be 0 whatever the value: keys that no row sees become zeros, and
         // so do values that are not finite, which wait for the item's end.
+        if (!Sh::PAIRED) {
+          alive = wait_all(full + used % UNITS, used / UNITS);
+          if (!alive) {
+            if (lane == 0) atomicExch(&p.status->timeout, 10);
+            continue;
+          }
+        }
+        unsigned char* vs = ring + (used % UNITS) * UNIT + (Sh::PAIRED ? SIDE : 0);
+        const uint32_t vb = smem_u32(vs);
         if (masked) {
-          unsigned char* vs = ring + stage * SLICE + SLICE / 2;
 #pragma unroll 1
           for (int e = lane; e < 16 * SLABS * 8; e += 32) {  // 16-byte words, 128 bytes of a key after the other
             const int kk = ks + ((e >> 3) & 15);
@@ -292,7 +312,7 @@ __global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
         }
         __syncwarp();
         ++used;
-        ask();
+        ask_next();
       }
     }
 
@@ -316,19 +336,41 @@ __global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
       for (int j = 0; j < 2; ++j)
         if (m[n][j] == -CUDART_INF_F && l[n][j] != 0.f) m[n][j] = 0.f;  // nothing but NaN: a part that counts, not one without keys
     __syncthreads();  // the last item's parts have been read
+    // one half of the warps puts its sums down, the other adds its own to them, each brought to the higher maximum
+    if (lane < 4) {
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int r = 8 * n + c0 + j;
-        if (lane < 4) s_m[warp * RB + r] = m[n][j], s_l[warp * RB + r] = l[n][j];
+        for (int j = 0; j < 2; ++j) s_m[warp * RB + 8 * n + c0 + j] = m[n][j], s_l[warp * RB + 8 * n + c0 + j] = l[n][j];
+    }
+    float* mine = s_o + (warp & (SLOTS - 1)) * RB * PITCH + (lane >> 2);
+    if (SLOTS == WARPS || warp >= SLOTS) {
 #pragma unroll
-        for (int k = 0; k < KST; ++k) {
-          float* at = s_o + (warp * RB + r) * PITCH + 16 * k + (lane >> 2);
-          at[0] = o[k][n][j];
-          at[8] = o[k][n][2 + j];
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int k = 0; k < KST; ++k) {
+            float* at = mine + (8 * n + c0 + j) * PITCH + 16 * k;
+            at[0] = o[k][n][j];
+            at[8] = o[k][n][2 + j];
+          }
+    }
+    if constexpr (SLOTS < WARPS) __syncthreads();
+    if (SLOTS < WARPS && warp < SLOTS) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float other = s_m[(warp + SLOTS) % WARPS * RB + 8 * n + c0 + j], to = fmaxf(m[n][j], other);
+          const float a = exp2_rel(m[n][j], to), b = exp2_rel(other, to);
+#pragma unroll
+          for (int k = 0; k < KST; ++k) {
+            float* at = mine + (8 * n + c0 + j) * PITCH + 16 * k;
+            at[0] = (a != 0.f ? a * o[k][n][j] : 0.f) + (b != 0.f ? b * at[0] : 0.f);
+            at[8] = (a != 0.f ? a * o[k][n][2 + j] : 0.f) + (b != 0.f ? b * at[8] : 0.f);
+          }
         }
-      }
     }
     const bool any_odd = __syncthreads_or(odd) != 0;
     const bool whole = first_tile == 0 && end_tile == blk.ntile;
@@ -344,11 +386,14 @@ __global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
       for (int w = 0; w < WARPS; ++w) M = fmaxf(M, s_m[w * RB + r]);
       float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int w = 0; w < WARPS; ++w) {
-        const float wt = exp2_rel(s_m[w * RB + r], M);
+      for (int w = 0; w < SLOTS; ++w) {
+        constexpr bool two = SLOTS < WARPS;  // this slot holds two warps' sums
+        const float m0 = s_m[w * RB + r], m1 = two ? s_m[(w + SLOTS) % WARPS * RB + r] : -CUDART_INF_F;
+        const float wt = exp2_rel(fmaxf(m0, m1), M);
         const float4 v = *reinterpret_cast<const float4*>(s_o + (w * RB + r) * PITCH + i);
         if (wt != 0.f) {
-          L += wt * s_l[w * RB + r];
+          const float w0 = exp2_rel(m0, M), w1 = exp2_rel(m1, M);
+          L += (w0 != 0.f ? w0 * s_l[w * RB + r] : 0.f) + (w1 != 0.f ? w1 * s_l[(w + SLOTS) % WARPS * RB + r] : 0.f);
           sum.x += wt * v.x, sum.y += wt * v.y, sum.z += wt * v.z, sum.w += wt * v.w;
         }
       }
@@ -380,7 +425,7 @@ __global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
   }
   // a warp that gave up has copies in flight: they land before its shared memory is somebody else's
   if (!alive)
-    for (; used < asked; ++used) attn_wait(full + used % STAGES, used / STAGES);
+    for (; used < asked; ++used) attn_wait(full + used % UNITS, used / UNITS);
 }
 
 template <int HD, int NT>

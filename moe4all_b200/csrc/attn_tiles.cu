@@ -178,7 +178,7 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
       if (lane < pieces && key < c.blk.hi && key + granule > c.blk.lo) {
         at.y = c.seq.q0 + key;
         if (!packed) {
-          const int page = key / p.page_size;
+          const int page = attn_page_of(p, key);
           at.w = attn_page_entry(p, c.s, page);
           at.y = key - page * p.page_size;
         }
