@@ -4,13 +4,14 @@
 // Sixteen lanes own a head; a lane takes eight values at a time as two 16-byte words that hold four whole pairs (halves style: the words
 // are half the rotated range apart; interleaved: neighbours), so that a pair never leaves its lane.  The angles are products of a position
 // and a frequency in 64 bits, reduced to a fraction of a turn before they are rounded to 32 (a position of 10^6 times a frequency near 1
-// keeps 4 bits of f32 after the point); a row's sines are worked out once for all of its heads.
+// keeps 4 bits of f32 after the point); a row's sines are worked out once for all of its heads, by as many threads as there are pairs in a
+// few rows.
 #include "attn.cuh"
 
 namespace infr {
 namespace {
 
-constexpr int ROPE_THREADS = 256, ROPE_TEAMS = ROPE_THREADS / 16, ROPE_MAX_PAIRS = 128;
+constexpr int ROPE_THREADS = 256, ROPE_TEAMS = ROPE_THREADS / 16, ROPE_MAX_PAIRS = 128, ROPE_ROWS = 4;
 
 __device__ __forceinline__ float team_sum(float v) {
 #pragma unroll
@@ -29,107 +30,141 @@ __device__ __forceinline__ void store4_f16(__half* dst, const float4& v) {
   *reinterpret_cast<uint2*>(dst) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
 }
 
-__global__ void __launch_bounds__(ROPE_THREADS) k_rope_kv(const RopeParams p) {
-  __shared__ __align__(16) float s_cos[2][ROPE_MAX_PAIRS], s_sin[2][ROPE_MAX_PAIRS];
-  const int tid = threadIdx.x, team = tid >> 4, tl = tid & 15;
-  pdl_wait();
-  const int r0 = (int)((long long)blockIdx.x * p.rows / gridDim.x), r1 = (int)((long long)(blockIdx.x + 1) * p.rows / gridDim.x);
-  // the last sequence that begins at or before the first row (rows ahead of cu_q[0] belong to none)
-  int s = 0;
-  for (int hi = p.n_seq; hi - s > 1;) {
-    const int mid = (s + hi) / 2;
-    if (__ldcg(p.cu_q + mid) <= r0) s = mid;
-    else hi = mid;
+// JS: eight-value chunks of a lane: 1 for heads up to 128, else 2.
+template <int JS>
+__global__ void __launch_bounds__(ROPE_THREADS) k_rope_kv(const __grid_constant__ RopeParams p) {
+  __shared__ __align__(16) float s_cos[ROPE_ROWS * ROPE_MAX_PAIRS], s_sin[ROPE_ROWS * ROPE_MAX_PAIRS];
+  __shared__ int s_pos[ROPE_ROWS], s_first;
+  __shared__ long long s_at[ROPE_ROWS];
+  const int tid = threadIdx.x, team = tid >> 4, tl = tid & 15, lane = tid & 31;
+  const int pairs = p.n_rot / 2, batch = pairs ? min(ROPE_ROWS, ROPE_THREADS / pairs) : ROPE_ROWS;
+  const int my_row = pairs ? tid / pairs : 0, my_pair = pairs ? tid - my_row * pairs : 0;
+  const bool turns_one = pairs && my_row < batch;
+  double turns = p.turns0, x = p.ratio;  // of this thread's pair, per token: turns0 * ratio^pair by squares
+#pragma unroll 1
+  for (int b = my_pair; b; b >>= 1, x *= x)
+    if (b & 1) turns *= x;
+  const int n_vec = p.n_head + 2 * p.n_kv, chunks = p.hd / 8, rot = p.n_rot / 8;
+  int oa[JS], ob[JS];
+#pragma unroll
+  for (int j = 0; j < JS; ++j) {
+    const int c = tl + 16 * j;
+    oa[j] = !p.interleaved && c < rot ? 4 * c : 8 * c;
+    ob[j] = !p.interleaved && c < rot ? p.n_rot / 2 + 4 * c : 8 * c + 4;
   }
+  const int r0 = (int)((long long)blockIdx.x * p.rows / gridDim.x), r1 = (int)((long long)(blockIdx.x + 1) * p.rows / gridDim.x);
+  pdl_wait();
+  if (turns_one && p.freq_factors != nullptr) turns /= (double)p.freq_factors[my_pair];
+  if (tid < 32) {
+    // the last sequence that begins at or before the first row (rows ahead of cu_q[0] belong to none): 32 places at a time
+    int lo = 0, hi = p.n_seq;
+#pragma unroll 1
+    while (hi - lo > 1) {
+      const int step = (hi - lo + 31) / 32, i = lo + lane * step;
+      const int n = __popc(__ballot_sync(0xFFFFFFFFu, i < hi && __ldcg(p.cu_q + i) <= r0));
+      lo += max(n - 1, 0) * step;
+      hi = min(hi, lo + step);
+    }
+    if (lane == 0) s_first = lo;
+  }
+  __syncthreads();
   bool bad = false;
+  int s = s_first;
+  AttnSeq seq = {0, 0, 0};
   auto load = [&](int i) {
     return attn_seq(__ldcg(p.cu_q + i), __ldcg(p.cu_q + i + 1), p.kv_len != nullptr ? __ldcg(p.kv_len + i) : 0, p.kv_len == nullptr, p.rows, p.cap, &bad);
   };
-  AttnSeq seq = load(s);
-  const int pairs = p.n_rot / 2;
-  double turns = 0.0;  // of this thread's pair, per token
-  if (tid < pairs) {
-    turns = p.turns0 * pow(p.ratio, (double)tid);
-    if (p.freq_factors != nullptr) turns /= (double)p.freq_factors[tid];
-  }
-  const int n_vec = p.n_head + 2 * p.n_kv, chunks = p.hd / 8, rot = p.n_rot / 8;
-  int buf = 0;
-  for (int r = r0; r < r1; ++r) {
-    while (s + 1 < p.n_seq && r >= seq.q0 + seq.q_len) seq = load(++s);
-    const int pos = seq.past + r - seq.q0;
-    if (r < seq.q0 || r >= seq.q0 + seq.q_len || pos < 0) continue;  // (the same for the whole CTA)
-    float *co = s_cos[buf], *si = s_sin[buf];  // (two: the other's readers are past the next barrier)
-    buf ^= 1;
-    if (tid < pairs) {
-      const double a = (double)pos * turns;
-      sincospif(2.f * (float)(a - rint(a)), si + tid, co + tid);
+  if (tid < batch) seq = load(s);
+
+  float4 a[JS], b[JS];  // of the head that comes next
+  auto fetch = [&](int row0, int rows, int e) {
+    const int i = e / n_vec, h = e - i * n_vec, r = row0 + i;
+    const bool is_q = h < p.n_head, is_v = h >= p.n_head + p.n_kv;
+    const float* src = is_q ? p.q + (size_t)r * p.q_stride + (size_t)h * p.hd
+                            : (is_v ? p.v + (size_t)r * p.v_stride + (size_t)(h - p.n_head - p.n_kv) * p.hd : p.k + (size_t)r * p.k_stride + (size_t)(h - p.n_head) * p.hd);
+#pragma unroll
+    for (int j = 0; j < JS; ++j) {
+      a[j] = b[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (i < rows && tl + 16 * j < chunks) {
+        a[j] = __ldcg(reinterpret_cast<const float4*>(src + oa[j]));
+        b[j] = __ldcg(reinterpret_cast<const float4*>(src + ob[j]));
+      }
     }
-    size_t at = (size_t)r * p.row_pitch;
-    bool writes = true;
-    if (p.page_table != nullptr) {
-      const int page = pos / p.page_size, id = __ldcg(p.page_table + (size_t)s * p.max_pages + page);
-      writes = (unsigned)id < (unsigned)p.n_pages;  // a page that is not there is not written, and reported at the next sync
-      if (!writes) bad = true;
-      at = (size_t)id * p.page_pitch + (size_t)(pos - page * p.page_size) * p.row_pitch;
+  };
+
+#pragma unroll 1
+  for (int row0 = r0; row0 < r1; row0 += batch) {
+    const int rows = min(batch, r1 - row0);
+    fetch(row0, rows, team);
+    if (tid < rows) {  // positions, and places in the cache (-1: none)
+      const int r = row0 + tid;
+#pragma unroll 1
+      while (s + 1 < p.n_seq && r >= seq.q0 + seq.q_len) seq = load(++s);
+      const int pos = seq.past + r - seq.q0;
+      const bool has = r >= seq.q0 && r < seq.q0 + seq.q_len && pos >= 0;
+      long long at = (long long)r * p.row_pitch;
+      if (has && p.page_table != nullptr) {
+        const int page = pos / p.page_size, id = __ldcg(p.page_table + (size_t)s * p.max_pages + page);
+        at = (unsigned)id < (unsigned)p.n_pages ? (long long)((size_t)id * p.page_pitch + (size_t)(pos - page * p.page_size) * p.row_pitch) : -1;
+        if (at < 0) bad = true;  // a page that is not there is not written, and reported at the next sync
+      }
+      s_pos[tid] = has ? pos : -1;
+      s_at[tid] = at;
     }
     __syncthreads();
-    for (int h0 = 0; h0 < n_vec; h0 += ROPE_TEAMS) {
-      const int h = h0 + team;
-      const bool has = h < n_vec, is_q = h < p.n_head, is_v = h >= p.n_head + p.n_kv;
-      const int kvh = is_q ? 0 : (is_v ? h - p.n_head - p.n_kv : h - p.n_head);
-      const float* src = is_q ? p.q + (size_t)r * p.q_stride + (size_t)h * p.hd
-                              : (is_v ? p.v + (size_t)r * p.v_stride : p.k + (size_t)r * p.k_stride) + (size_t)kvh * p.hd;
+    if (turns_one && my_row < rows) {
+      const double t = (double)s_pos[my_row] * turns;
+      sincospif(2.f * (float)(t - rint(t)), s_sin + my_row * ROPE_MAX_PAIRS + my_pair, s_cos + my_row * ROPE_MAX_PAIRS + my_pair);
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int e0 = 0; e0 < rows * n_vec; e0 += ROPE_TEAMS) {
+      const int e = e0 + team, i = min(e / n_vec, rows - 1), h = e - (e / n_vec) * n_vec, r = row0 + i;
+      const bool is_q = h < p.n_head, is_v = h >= p.n_head + p.n_kv, has = e < rows * n_vec && s_pos[i] >= 0;
       const float* w = is_v ? nullptr : (is_q ? p.q_norm : p.k_norm);
-      float4 a[2], b[2];
-      int oa[2], ob[2];
+      float4 x[JS], y[JS];
       float sq = 0.f;
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int c = tl + 16 * j;
-        oa[j] = 8 * c, ob[j] = 8 * c + 4;
-        if (!p.interleaved && c < rot) oa[j] = 4 * c, ob[j] = p.n_rot / 2 + 4 * c;
-        a[j] = b[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (has && c < chunks) {
-          a[j] = __ldcg(reinterpret_cast<const float4*>(src + oa[j]));
-          b[j] = __ldcg(reinterpret_cast<const float4*>(src + ob[j]));
-        }
-        if (w != nullptr)
-          sq += a[j].x * a[j].x + a[j].y * a[j].y + a[j].z * a[j].z + a[j].w * a[j].w + b[j].x * b[j].x + b[j].y * b[j].y + b[j].z * b[j].z + b[j].w * b[j].w;
+      for (int j = 0; j < JS; ++j) {
+        x[j] = a[j], y[j] = b[j];
+        sq += x[j].x * x[j].x + x[j].y * x[j].y + x[j].z * x[j].z + x[j].w * x[j].w + y[j].x * y[j].x + y[j].y * y[j].y + y[j].z * y[j].z + y[j].w * y[j].w;
       }
-      // (every lane takes part: the warp's other team may have a norm to sum)
-      const float total = team_sum(sq);
+      if (e0 + ROPE_TEAMS < rows * n_vec) fetch(row0, rows, e + ROPE_TEAMS);
+      if (p.q_norm != nullptr || p.k_norm != nullptr) sq = team_sum(sq);  // (every lane takes part)
       if (!has) continue;
-      const float k = w != nullptr ? rsqrtf(total / (float)p.hd + p.norm_eps) : 1.f;
+      const float k = w != nullptr ? rsqrtf(sq / (float)p.hd + p.norm_eps) : 1.f;
+      const long long at = s_at[i];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
+      for (int j = 0; j < JS; ++j) {
         const int c = tl + 16 * j;
         if (c >= chunks) continue;
         if (w != nullptr) {
           const float4 wa = *reinterpret_cast<const float4*>(w + oa[j]), wb = *reinterpret_cast<const float4*>(w + ob[j]);
-          a[j].x *= k * wa.x, a[j].y *= k * wa.y, a[j].z *= k * wa.z, a[j].w *= k * wa.w;
-          b[j].x *= k * wb.x, b[j].y *= k * wb.y, b[j].z *= k * wb.z, b[j].w *= k * wb.w;
+          x[j].x *= k * wa.x, x[j].y *= k * wa.y, x[j].z *= k * wa.z, x[j].w *= k * wa.w;
+          y[j].x *= k * wb.x, y[j].y *= k * wb.y, y[j].z *= k * wb.z, y[j].w *= k * wb.w;
         }
         if (!is_v && c < rot) {
-          const float4 cs = *reinterpret_cast<const float4*>(co + 4 * c), sn = *reinterpret_cast<const float4*>(si + 4 * c);
+          const float4 cs = *reinterpret_cast<const float4*>(s_cos + i * ROPE_MAX_PAIRS + 4 * c), sn = *reinterpret_cast<const float4*>(s_sin + i * ROPE_MAX_PAIRS + 4 * c);
           if (p.interleaved) {
-            turn(a[j].x, a[j].y, cs.x, sn.x), turn(a[j].z, a[j].w, cs.y, sn.y);
-            turn(b[j].x, b[j].y, cs.z, sn.z), turn(b[j].z, b[j].w, cs.w, sn.w);
+            turn(x[j].x, x[j].y, cs.x, sn.x), turn(x[j].z, x[j].w, cs.y, sn.y);
+            turn(y[j].x, y[j].y, cs.z, sn.z), turn(y[j].z, y[j].w, cs.w, sn.w);
           } else {
-            turn(a[j].x, b[j].x, cs.x, sn.x), turn(a[j].y, b[j].y, cs.y, sn.y);
-            turn(a[j].z, b[j].z, cs.z, sn.z), turn(a[j].w, b[j].w, cs.w, sn.w);
+            turn(x[j].x, y[j].x, cs.x, sn.x), turn(x[j].y, y[j].y, cs.y, sn.y);
+            turn(x[j].z, y[j].z, cs.z, sn.z), turn(x[j].w, y[j].w, cs.w, sn.w);
           }
         }
         if (is_q) {
           float* dst = p.q_out + (size_t)r * p.qo_stride + (size_t)h * p.hd;
-          *reinterpret_cast<float4*>(dst + oa[j]) = a[j];
-          *reinterpret_cast<float4*>(dst + ob[j]) = b[j];
-        } else if (writes) {
-          __half* dst = (is_v ? p.v_cache : p.k_cache) + at + (size_t)kvh * p.head_pitch;
-          store4_f16(dst + oa[j], a[j]);
-          store4_f16(dst + ob[j], b[j]);
+          *reinterpret_cast<float4*>(dst + oa[j]) = x[j];
+          *reinterpret_cast<float4*>(dst + ob[j]) = y[j];
+        } else if (at >= 0) {
+          __half* dst = (is_v ? p.v_cache + (size_t)(h - p.n_head - p.n_kv) * p.head_pitch : p.k_cache + (size_t)(h - p.n_head) * p.head_pitch) + at;
+          store4_f16(dst + oa[j], x[j]);
+          store4_f16(dst + ob[j], y[j]);
         }
       }
     }
+    __syncthreads();  // the rows' words have been read
   }
   if (bad) p.status->bad_index = 2;
 }
@@ -137,8 +172,8 @@ __global__ void __launch_bounds__(ROPE_THREADS) k_rope_kv(const RopeParams p) {
 }  // namespace
 
 int32_t launch_rope_kv(infr_cuda_ctx* ctx, const RopeParams& p) {
-  const int most = ctx->sm_count * 8;
-  const cudaError_t e = launch_ex(k_rope_kv, dim3(p.rows < most ? p.rows : most), dim3(ROPE_THREADS), 0, ctx->stream, true, p);
+  const int most = ctx->sm_count * 8;  // as many as an SM's threads allow
+  const cudaError_t e = launch_ex(p.hd <= 128 ? k_rope_kv<1> : k_rope_kv<2>, dim3(p.rows < most ? p.rows : most), dim3(ROPE_THREADS), 0, ctx->stream, true, p);
   if (e != cudaSuccess) return check_cuda(ctx, e, "k_rope_kv launch");
   ctx->launches += 1;
   return check_cuda(ctx, cudaGetLastError(), "k_rope_kv launch");
