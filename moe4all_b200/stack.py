@@ -1,6 +1,11 @@
-"""A stack of MoE FFN sub-layers as the graph builder emits them for a decode step
+"""A stack of layers as the graph builder emits them for a step
 (crates/infr-llama/src/seam/runner.rs:7999-8176; layer shape pinned in
-crates/infr-core/src/fusion.rs:735-737), attention omitted:
+crates/infr-core/src/fusion.rs:735-737): MoE FFN sub-layers, and with `attn` an attention sub-layer ahead of each:
+
+    hn     = RmsNorm(hidden, a_l, eps)                  with attn
+    qkv    = Linear(hn, wqkv_l)
+    q      = RopeKv(qkv) -> k, v into layer l's pages
+    hidden = Add(hidden, Linear(Attention(q), wo_l))
 
     hn     = RmsNorm(hidden, w_l, eps)
     sub    = MoeFfn(hn) (+ shared expert)
@@ -10,19 +15,86 @@ Every op goes through the C ABI; the whole step can be recorded once and replaye
 (`Backend::compile` + decode replay)."""
 from __future__ import annotations
 
+from dataclasses import dataclass, field
 from typing import List, Optional
 
 import torch
 
-from .backend import CudaBackend, MoeFfn
+from .backend import Attention, Buffer, CudaBackend, DType, MoeFfn, RopeKv
+
+
+@dataclass
+class AttnWeights:
+    """One layer's attention: the norm ahead of it, q / k / v in one projection [(n_head + 2 n_kv) head_dim, ne], the output
+    projection [ne, n_head head_dim], both of `dtype`, and the per-head norms of q and k where the model has them."""
+    norm: torch.Tensor
+    wqkv: Buffer
+    wo: Buffer
+    q_norm: Optional[torch.Tensor] = None
+    k_norm: Optional[torch.Tensor] = None
+    dtype: DType = DType.F32
+
+
+@dataclass
+class StackAttention:
+    """The attention of a `MoeStack` over pages that all of its layers address alike: sequence s has kv_len[s] tokens with the step's new
+    ones, which are the stack's rows cu_q[s] .. cu_q[s + 1] - 1.  The three arrays are i32 tensors on the device, read when a step runs: a
+    recorded step follows new lengths and pages written into them.  `caches[l]` are layer l's (k, v), f16 [n_pages, n_kv, page_size, head_dim]."""
+    layers: List[AttnWeights]
+    n_head: int
+    n_kv: int
+    head_dim: int
+    cu_q: torch.Tensor
+    kv_len: torch.Tensor
+    page_table: torch.Tensor
+    page_size: int
+    caches: List[tuple]
+    max_q: int = 0
+    window: int = 0
+    rope_base: float = 1e4
+    n_rot: Optional[int] = None  # whole heads unless given
+    interleaved: bool = False
+    _ops: list = field(default_factory=list, repr=False)
+
+    def bind(self, be: CudaBackend, rows: int, ne: int, eps: float, hidden: Buffer, device) -> None:
+        """Rows between the ops, and the ops over them."""
+        H, K, hd = self.n_head, self.n_kv, self.head_dim
+        wide, w = (H + 2 * K) * hd, be.wrap_tensor
+        self._be, self._shape, self._hidden = be, (rows, ne, eps, wide, H * hd), hidden
+        self._rows = [torch.zeros(rows, n, device=device) for n in (ne, wide, H * hd, H * hd, ne)]
+        self._hn, self._qkv, q, out, self._sub = (w(t) for t in self._rows)
+        self._out = out
+        part = lambda first: be.wrap(self._rows[1].data_ptr() + 4 * first, 4 * (rows * wide - first))
+        n_pages = self.caches[0][0].shape[0]
+        batch = dict(cu_q=w(self.cu_q), kv_len=w(self.kv_len), page_table=w(self.page_table), rows=rows, n_seq=self.kv_len.numel(), n_head=H, n_kv=K,
+                     head_dim=hd, n_pages=n_pages, page_size=self.page_size, max_pages=self.page_table.shape[1])
+        parts = part(0), part(H * hd), part((H + K) * hd)
+        for L, (k, v) in zip(self.layers, self.caches, strict=True):
+            opt = lambda t: None if t is None else w(t)
+            kc, vc = w(k), w(v)
+            self._ops.append((w(L.norm), RopeKv(q=parts[0], k=parts[1], v=parts[2], q_stride=wide, k_stride=wide, v_stride=wide, q_out=q, k_cache=kc, v_cache=vc,
+                                                n_rot=hd if self.n_rot is None else self.n_rot, interleaved=self.interleaved, rope_base=self.rope_base,
+                                                q_norm=opt(L.q_norm), k_norm=opt(L.k_norm), norm_eps=eps, **batch),
+                              Attention(q=q, k=kc, v=vc, out=out, scale=hd ** -0.5, max_q=self.max_q, window=self.window, **batch)))
+
+    def layer(self, li: int) -> None:
+        """One attention sub-layer in place on `hidden`."""
+        be, L, (norm, rope, attention) = self._be, self.layers[li], self._ops[li]
+        rows, ne, eps, wide, n_out = self._shape
+        be.rms_norm(self._hidden, norm, self._hn, rows, ne, eps)
+        be.linear(L.dtype, L.wqkv, self._hn, self._qkv, rows, ne, wide)
+        be.rope_kv(rope)
+        be.attention(attention)
+        be.linear(L.dtype, L.wo, self._out, self._sub, rows, n_out, ne)
+        be.add(self._hidden, self._sub, self._hidden, rows * ne)
 
 
 class MoeStack:
     def __init__(self, be: CudaBackend, layers: List, norm_weights: List[torch.Tensor], rows: int, ne: int, n_expert: int,
-                 n_used: int, n_ff: int, sh_ff: int = 0, eps: float = 1e-6, fused: bool = True, **route_kw):
+                 n_used: int, n_ff: int, sh_ff: int = 0, eps: float = 1e-6, fused: bool = True, attn: Optional[StackAttention] = None, **route_kw):
         """fused: fold RmsNorm and the residual Add into the MoE op (the reference's
         RmsNorm->MoeFfn and MoeFfn->Add peepholes, crates/infr-core/src/fusion.rs:17-25) instead of
-        running them as kernels of their own."""
+        running them as kernels of their own.  attn: an attention sub-layer ahead of every MoE one."""
         assert len(layers) == len(norm_weights)
         self.be, self.layers, self.rows, self.ne, self.eps = be, layers, rows, ne, eps
         dev = norm_weights[0].device
@@ -47,10 +119,15 @@ class MoeStack:
                                    sh_down=b.get("sh_down"), sh_gate_inp=b.get("sh_gate_inp"),
                                    sh_ff=sh_ff if "sh_gate" in b else 0, **fuse, **route_kw))
         self.plan = None
+        self.attn = attn
+        if attn is not None:
+            attn.bind(be, rows, ne, eps, self.b_hidden, dev)
 
     def layer(self, li: int) -> None:
-        """One sub-layer in place on `hidden`."""
+        """One layer in place on `hidden`."""
         be = self.be
+        if self.attn is not None:
+            self.attn.layer(li)
         if self.fused:
             be.moe_ffn(self.ops[li])
             return
