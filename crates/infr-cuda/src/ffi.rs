@@ -102,6 +102,81 @@ impl Default for infr_cuda_moe_ffn_desc {
     }
 }
 
+pub const ROPE_HALVES: u32 = 0;
+pub const ROPE_INTERLEAVED: u32 = 1;
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct infr_cuda_rope_kv_desc {
+    pub q: *const infr_cuda_buf,
+    pub k: *const infr_cuda_buf,
+    pub v: *const infr_cuda_buf,
+    pub q_out: *mut infr_cuda_buf,
+    pub k_cache: *mut infr_cuda_buf,
+    pub v_cache: *mut infr_cuda_buf,
+    pub cu_q: *const infr_cuda_buf,
+    pub kv_len: *const infr_cuda_buf,
+    pub page_table: *const infr_cuda_buf,
+    pub q_norm: *const infr_cuda_buf,
+    pub k_norm: *const infr_cuda_buf,
+    pub freq_factors: *const infr_cuda_buf,
+    pub rows: u32,
+    pub n_seq: u32,
+    pub n_head: u32,
+    pub n_kv: u32,
+    pub head_dim: u32,
+    pub n_pages: u32,
+    pub page_size: u32,
+    pub max_pages: u32,
+    pub q_stride: u32,
+    pub k_stride: u32,
+    pub v_stride: u32,
+    pub q_out_stride: u32,
+    pub n_rot: u32,
+    pub style: u32,
+    pub rope_base: f32,
+    pub rope_scale: f32,
+    pub norm_eps: f32,
+}
+
+impl Default for infr_cuda_rope_kv_desc {
+    fn default() -> Self {
+        unsafe { std::mem::zeroed() }
+    }
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct infr_cuda_attention_desc {
+    pub q: *const infr_cuda_buf,
+    pub k: *const infr_cuda_buf,
+    pub v: *const infr_cuda_buf,
+    pub out: *mut infr_cuda_buf,
+    pub cu_q: *const infr_cuda_buf,
+    pub kv_len: *const infr_cuda_buf,
+    pub page_table: *const infr_cuda_buf,
+    pub rows: u32,
+    pub n_seq: u32,
+    pub n_head: u32,
+    pub n_kv: u32,
+    pub head_dim: u32,
+    pub n_pages: u32,
+    pub page_size: u32,
+    pub max_pages: u32,
+    pub q_stride: u32,
+    pub out_stride: u32,
+    pub max_q: u32,
+    pub window: u32,
+    pub scale: f32,
+    pub path: u32,
+}
+
+impl Default for infr_cuda_attention_desc {
+    fn default() -> Self {
+        unsafe { std::mem::zeroed() }
+    }
+}
+
 #[repr(C)]
 #[derive(Clone, Copy, Default)]
 pub struct infr_cuda_config {
@@ -153,6 +228,8 @@ extern "C" {
                                dst: *mut infr_cuda_buf, n: usize) -> i32;
     pub fn infr_cuda_moe_shared_add(ctx: *mut infr_cuda_ctx, moe: *const infr_cuda_buf, shexp: *const infr_cuda_buf,
                                     gate: *const infr_cuda_buf, dst: *mut infr_cuda_buf, rows: u32, n: u32) -> i32;
+    pub fn infr_cuda_rope_kv(ctx: *mut infr_cuda_ctx, desc: *const infr_cuda_rope_kv_desc) -> i32;
+    pub fn infr_cuda_attention(ctx: *mut infr_cuda_ctx, desc: *const infr_cuda_attention_desc) -> i32;
     pub fn infr_cuda_rmsnorm(ctx: *mut infr_cuda_ctx, x: *const infr_cuda_buf, weight: *const infr_cuda_buf,
                              dst: *mut infr_cuda_buf, rows: u32, dim: u32, eps: f32) -> i32;
     pub fn infr_cuda_add(ctx: *mut infr_cuda_ctx, a: *const infr_cuda_buf, b: *const infr_cuda_buf, dst: *mut infr_cuda_buf, n: usize) -> i32;

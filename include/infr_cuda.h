@@ -354,7 +354,7 @@ int32_t infr_cuda_add(infr_cuda_ctx* ctx, const infr_cuda_buf* a, const infr_cud
  * [0, n_pages) is forced into range (a page that is not there is read as page 0, and not written), and the next infr_cuda_sync /
  * download fails with INVALID_ARG.  Page table entries past a sequence's length are not read.
  *
- * head_dim: a multiple of 16 up to 256.  n_head: a multiple of n_kv, up to 128 query heads to each; query head h reads kv head
+ * n_seq: up to 4096.  head_dim: a multiple of 16 up to 256.  n_head: a multiple of n_kv, up to 128 query heads to each; query head h reads kv head
  * h / (n_head / n_kv).  page_size: a multiple of 16.  Strides are in values between rows, a multiple of 4 up to 2^24, 0 for rows side by side
  * (as many values as heads x head_dim): the parts of one wide q/k/v row are buffers wrapped at their first value. */
 #define INFR_CUDA_ROPE_HALVES 0      /* pairs (i, i + n_rot / 2)  */

@@ -124,6 +124,75 @@ class Plan {
   infr_cuda_graph* g_ = nullptr;
 };
 
+// A batch of sequences over a cache of pages, or over packed rows (page_table and kv_len null): what infr_cuda_rope_kv_desc and
+// infr_cuda_attention_desc have in common (infr_cuda.h says what each field is).
+struct SeqBatch {
+  const Buffer* cu_q = nullptr;
+  const Buffer* kv_len = nullptr;
+  const Buffer* page_table = nullptr;
+  uint32_t rows = 0, n_seq = 0, n_head = 0, n_kv = 0, head_dim = 0;
+  uint32_t n_pages = 0, page_size = 0, max_pages = 0;
+
+  template <class Desc>
+  void fill(Desc& d) const {
+    auto h = [](const Buffer* b) -> infr_cuda_buf* { return b ? b->handle() : nullptr; };
+    d.cu_q = h(cu_q), d.kv_len = h(kv_len), d.page_table = h(page_table);
+    d.rows = rows, d.n_seq = n_seq, d.n_head = n_head, d.n_kv = n_kv, d.head_dim = head_dim;
+    d.n_pages = n_pages, d.page_size = page_size, d.max_pages = max_pages;
+  }
+};
+
+// New rows on their way to attention: per-head norms, rotary embedding, k and v into the cache.
+struct RopeKv {
+  SeqBatch batch;
+  const Buffer* q = nullptr;
+  const Buffer* k = nullptr;
+  const Buffer* v = nullptr;
+  Buffer* q_out = nullptr;
+  Buffer* k_cache = nullptr;
+  Buffer* v_cache = nullptr;
+  const Buffer* q_norm = nullptr;
+  const Buffer* k_norm = nullptr;
+  const Buffer* freq_factors = nullptr;
+  uint32_t q_stride = 0, k_stride = 0, v_stride = 0, q_out_stride = 0, n_rot = 0;
+  bool interleaved = false;
+  float rope_base = 1e4f, rope_scale = 1.f, norm_eps = 1e-6f;
+
+  infr_cuda_rope_kv_desc to_desc() const {
+    infr_cuda_rope_kv_desc d;
+    std::memset(&d, 0, sizeof d);
+    auto h = [](const Buffer* b) -> infr_cuda_buf* { return b ? b->handle() : nullptr; };
+    batch.fill(d);
+    d.q = h(q), d.k = h(k), d.v = h(v), d.q_out = h(q_out), d.k_cache = h(k_cache), d.v_cache = h(v_cache);
+    d.q_norm = h(q_norm), d.k_norm = h(k_norm), d.freq_factors = h(freq_factors);
+    d.q_stride = q_stride, d.k_stride = k_stride, d.v_stride = v_stride, d.q_out_stride = q_out_stride;
+    d.n_rot = n_rot, d.style = interleaved ? INFR_CUDA_ROPE_INTERLEAVED : INFR_CUDA_ROPE_HALVES;
+    d.rope_base = rope_base, d.rope_scale = rope_scale, d.norm_eps = norm_eps;
+    return d;
+  }
+};
+
+// Causal attention of a batch's new rows over its cache.
+struct Attention {
+  SeqBatch batch;
+  const Buffer* q = nullptr;
+  const Buffer* k = nullptr;
+  const Buffer* v = nullptr;
+  Buffer* out = nullptr;
+  uint32_t q_stride = 0, out_stride = 0, max_q = 0, window = 0, path = 0;
+  float scale = 0.f;
+
+  infr_cuda_attention_desc to_desc() const {
+    infr_cuda_attention_desc d;
+    std::memset(&d, 0, sizeof d);
+    auto h = [](const Buffer* b) -> infr_cuda_buf* { return b ? b->handle() : nullptr; };
+    batch.fill(d);
+    d.q = h(q), d.k = h(k), d.v = h(v), d.out = h(out);
+    d.q_stride = q_stride, d.out_stride = out_stride, d.max_q = max_q, d.window = window, d.scale = scale, d.path = path;
+    return d;
+  }
+};
+
 // `Op::MoeFfn` (graph.rs:1259-1352) with bound buffers, in the forms the CUDA kernels cover:
 // split gate/up banks, SiLU, output-side weighting.  Optional members are null pointers.
 struct MoeFfn {
@@ -275,6 +344,14 @@ class Backend {
   }
   Status linear(DType dtype, const Buffer& w, const Buffer& x, Buffer& y, uint32_t m, uint32_t in_f, uint32_t out_f) {
     return st(infr_cuda_linear(ctx_, static_cast<int32_t>(dtype), w.handle(), x.handle(), y.handle(), m, in_f, out_f));
+  }
+  Status rope_kv(const RopeKv& op) {
+    const infr_cuda_rope_kv_desc d = op.to_desc();
+    return st(infr_cuda_rope_kv(ctx_, &d));
+  }
+  Status attention(const Attention& op) {
+    const infr_cuda_attention_desc d = op.to_desc();
+    return st(infr_cuda_attention(ctx_, &d));
   }
   Status gated_act(const Buffer& gate, const Buffer& up, Buffer& dst, size_t n) { return st(infr_cuda_gated_act(ctx_, gate.handle(), up.handle(), dst.handle(), n)); }
   Status moe_shared_expert_add(const Buffer& moe, const Buffer& shexp, const Buffer& gate, Buffer& dst, uint32_t rows, uint32_t n) {
