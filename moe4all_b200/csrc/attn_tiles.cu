@@ -429,86 +429,92 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
       ok = wait_all(bars.i_full + item % ITEMS, item / ITEMS);
       if (!ok) break;
       const TileItem& it = s_item[item % ITEMS];
-      const int n1 = it.n1, n_rows = it.n_rows, slot = item & (RING - 1);
-      float f = 0.f;
+      const int n1 = it.n1, n_rows = it.n_rows;
+      for (; turned <= item && ok; ++turned) convert(turned);
+      ok = ok && wait_all(bars.f_full + (item & (RING - 1)), item / RING);
+      if (!ok) break;
+      const float f = s_fac[(item & (RING - 1)) * 128 + row];
       const int to = it.pos0 + (row < n_rows ? attn_row_token(p, row) : 0);  // the row sees the keys (from, to]
       const int from = p.window > 0 ? to - p.window : -1;
       const bool busy = (warp & 3) * 32 < n_rows;  // (other rows' weights are whatever is there: they reach those rows' sums only)
       float m = -CUDART_INF_F, l = 0.f;
       int ks = it.key0 + 64 * wg;
+      int stop = n1 < N ? max(n, n1 - 2) : n1;  // where the next item's q is turned
 #pragma unroll 1
-      for (; n < n1; ++n, ks += BK) {
-        while (turned <= (n + 2 >= n1 && n1 < N ? item + 1 : item) && ok) convert(turned), ++turned;
-        if (n == it.n0) {
-          ok = ok && wait_all(bars.f_full + slot, item / RING);
-          f = s_fac[slot * 128 + row];
-        }
-        ok = ok && wait_all(bars.s_full + (n & 1), n >> 1);
-        if (!ok) break;
-        umma::fence_after_sync();
-        const uint32_t sa = mine + (n & 1) * BK;
-        float top = -CUDART_INF_F;
-        const bool masked = ks + 64 > it.full_hi || ks < it.full_lo;
-        if (busy) {
+      while (true) {
 #pragma unroll 1
-          for (int j = 0; j < 64; j += 32) {
-            float s[32];
-            umma::tmem_ld_32x32(sa + j, s);
-            const uint32_t seen = masked ? seen_keys(ks + j, from, to) : ~0u;
-            umma::tmem_ld_wait(s);
-            if (masked) hide(s, seen);
-            float t[2] = {top, -CUDART_INF_F};
+        for (; n < stop && ok; ++n, ks += BK) {
+          ok = wait_all(bars.s_full + (n & 1), n >> 1);
+          if (!ok) break;
+          umma::fence_after_sync();
+          const uint32_t sa = mine + (n & 1) * BK;
+          float top = -CUDART_INF_F;
+          const bool masked = ks + 64 > it.full_hi || ks < it.full_lo;
+          if (busy) {
+#pragma unroll 1
+            for (int j = 0; j < 64; j += 32) {
+              float s[32];
+              umma::tmem_ld_32x32(sa + j, s);
+              const uint32_t seen = masked ? seen_keys(ks + j, from, to) : ~0u;
+              umma::tmem_ld_wait(s);
+              if (masked) hide(s, seen);
+              float t[2] = {top, -CUDART_INF_F};
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) t[(i >> 1) & 1] = fmaxf(fmaxf(t[(i >> 1) & 1], s[i]), s[i + 1]);
-            top = fmaxf(t[0], t[1]);
-          }
-        }
-        if constexpr (GROUPS == 2) {
-          float* at = s_max + (n & 1) * 256 + row;
-          at[128 * wg] = top;
-          asm volatile("bar.sync 2, 256;" ::: "memory");
-          top = fmaxf(top, at[128 * (wg ^ 1)]);
-        }
-        const float now = fmaxf(m, top * f);
-        l *= exp2_rel(m, now);
-        m = now;
-        if (busy) {
-          const float off = TILE_BIAS - (now == -CUDART_INF_F ? 0.f : now);
-          const float2 f2 = make_float2(f, f), off2 = make_float2(off, off), minus = make_float2(-1.f, -1.f);
-          float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll 1
-          for (int j = 0; j < 64; j += 32) {
-            float s[32];
-            umma::tmem_ld_32x32(sa + j, s);
-            const uint32_t seen = masked ? seen_keys(ks + j, from, to) : ~0u;
-            umma::tmem_ld_wait(s);
-            if (masked) hide(s, seen);
-            uint32_t w[32];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float2 x = __ffma2_rn(make_float2(s[2 * i], s[2 * i + 1]), f2, off2);
-              const float2 e = make_float2(exp2_approx(x.x), exp2_approx(x.y));
-              sum[i & 1] = __fadd2_rn(sum[i & 1], e);
-              // the piece that f16 holds (below 2^-14, 2^-29 of the largest, rounded once more), and the rest
-              const float2 h = make_float2(__uint_as_float(__float_as_uint(e.x) & 0xFFFFE000u), __uint_as_float(__float_as_uint(e.y) & 0xFFFFE000u));
-              const float2 r = __ffma2_rn(h, minus, e);
-              const __half2 hh = __floats2half2_rn(h.x, h.y), rr = __floats2half2_rn(r.x, r.y);
-              w[i] = *reinterpret_cast<const uint32_t*>(&hh);
-              w[16 + i] = *reinterpret_cast<const uint32_t*>(&rr);
+              for (int i = 0; i < 32; i += 2) t[(i >> 1) & 1] = fmaxf(fmaxf(t[(i >> 1) & 1], s[i]), s[i + 1]);
+              top = fmaxf(t[0], t[1]);
             }
-            umma::tmem_st_32x32_async(sa + j, w);
           }
-          l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-          umma::tmem_st_wait();
+          if constexpr (GROUPS == 2) {
+            float* at = s_max + (n & 1) * 256 + row;
+            at[128 * wg] = top;
+            asm volatile("bar.sync %0, 64;" ::"r"(2 + (warp & 3)) : "memory");  // (the two warps of these rows)
+            top = fmaxf(top, at[128 * (wg ^ 1)]);
+          }
+          const float now = fmaxf(m, top * f);
+          l *= exp2_rel(m, now);
+          m = now;
+          if (busy) {
+            const float off = TILE_BIAS - (now == -CUDART_INF_F ? 0.f : now);
+            const float2 f2 = make_float2(f, f), off2 = make_float2(off, off), minus = make_float2(-1.f, -1.f);
+            float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll 1
+            for (int j = 0; j < 64; j += 32) {
+              float s[32];
+              umma::tmem_ld_32x32(sa + j, s);
+              const uint32_t seen = masked ? seen_keys(ks + j, from, to) : ~0u;
+              umma::tmem_ld_wait(s);
+              if (masked) hide(s, seen);
+              uint32_t w[32];
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const float2 x = __ffma2_rn(make_float2(s[2 * i], s[2 * i + 1]), f2, off2);
+                const float2 e = make_float2(exp2_approx(x.x), exp2_approx(x.y));
+                sum[i & 1] = __fadd2_rn(sum[i & 1], e);
+                // the piece that f16 holds (below 2^-14, 2^-29 of the largest, rounded once more), and the rest
+                const float2 h = make_float2(__uint_as_float(__float_as_uint(e.x) & 0xFFFFE000u), __uint_as_float(__float_as_uint(e.y) & 0xFFFFE000u));
+                const float2 r = __ffma2_rn(h, minus, e);
+                const __half2 hh = __floats2half2_rn(h.x, h.y), rr = __floats2half2_rn(r.x, r.y);
+                w[i] = *reinterpret_cast<const uint32_t*>(&hh);
+                w[16 + i] = *reinterpret_cast<const uint32_t*>(&rr);
+              }
+              umma::tmem_st_32x32_async(sa + j, w);
+            }
+            l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+            umma::tmem_st_wait();
+          }
+          umma::fence_before_sync();
+          if (wg == 0) s_ref[(n & (RING - 1)) * 128 + row] = m;
+          if (n + 1 == n1) {
+            s_l[((item % Sh::ENDS) * GROUPS + wg) * 128 + row] = l;
+            if (wg == 0) s_end[(item % Sh::ENDS) * 128 + row] = m;
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bars.ready + (n & 3)), mbar_arrive(bars.a_full + (n & (RING - 1)));
         }
-        umma::fence_before_sync();
-        if (wg == 0) s_ref[(n & (RING - 1)) * 128 + row] = m;
-        if (n + 1 == n1) {
-          s_l[((item % Sh::ENDS) * GROUPS + wg) * 128 + row] = l;
-          if (wg == 0) s_end[(item % Sh::ENDS) * 128 + row] = m;
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bars.ready + (n & 3)), mbar_arrive(bars.a_full + (n & (RING - 1)));
+        if (n >= n1 || !ok) break;
+        convert(turned);
+        ++turned;
+        stop = n1;
       }
     }
     if (!ok && lane == 0) atomicExch(&p.status->timeout, 11);
