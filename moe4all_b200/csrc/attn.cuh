@@ -120,6 +120,7 @@ struct AttnStart {
   AttnLine line;
   long long u0, u1, ub;     // ub: where the block's first head begins
   long long before, until;  // tiles ahead of u0 and of u1
+  AttnSeq seq;
   int s, b;
 };
 
@@ -188,7 +189,7 @@ __device__ __forceinline__ void attn_plan(const AttnParams& p, int* known, long 
           if (u < ub || u >= ub + n) continue;
           const int head = attn_small_div(u - ub, nt + EXTRA), in = (int)(u - ub - (long long)head * (nt + EXTRA)) - EXTRA;
           const long long ahead = tiles * p.n_kv + (long long)head * nt + (in > 0 ? in : 0);
-          if (k == 0) st->s = at, st->b = f - pre[at], st->ub = ub, st->before = ahead;
+          if (k == 0) st->s = at, st->seq = seqs[at], st->b = f - pre[at], st->ub = ub, st->before = ahead;
           else st->until = ahead;
         }
       }
@@ -231,8 +232,7 @@ struct AttnCursor {
   int s, b, head;
 
   __device__ __forceinline__ void start(const AttnParams& p, const AttnStart& st) {
-    s = st.s, b = st.b;
-    seq = attn_load_seq(p, s);
+    s = st.s, b = st.b, seq = st.seq;
     blk = attn_block(seq, b, p.tb, LOG2_TILE, p.window);
     head = attn_small_div(st.u0 - st.ub, blk.ntile + EXTRA);
     ub = st.ub + (long long)head * (blk.ntile + EXTRA) + EXTRA;

@@ -67,6 +67,7 @@ __global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
   unsigned char* ring = ring_all + warp * UNITS * UNIT;
   uint64_t* full = bars + warp * UNITS;
 
+  pdl_trigger();  // the next kernel may take the SMs that this one leaves free, and do what needs no input of its
   if (lane == 0)
     for (int i = 0; i < UNITS; ++i) mbar_init(full + i, 1);
   mbar_fence_init();
@@ -81,6 +82,7 @@ __global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
   // ---- what the warp asks for: K and V of its slices of the CTA's tiles, one after the other, as many as its ring holds
   AttnCursor<Sh::LOG2_TILE, ROWS_EXTRA> ahead;
   ahead.start(p, st);
+  AttnCursor<Sh::LOG2_TILE, ROWS_EXTRA> cur = ahead;  // what it works on
   int at = ahead.first(st);             // tile of its item to look at next
   int a_key = -1, a_page = 0, a_y = 0;  // first key of the slice to ask for (-1: none left), its page, its place there
   uint32_t asked = 0;
@@ -131,8 +133,6 @@ __global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
 #pragma unroll 1
   for (int i = 0; i < UNITS; ++i) ask_next();
 
-  AttnCursor<Sh::LOG2_TILE, ROWS_EXTRA> cur;
-  cur.start(p, st);
   uint32_t used = 0;
   bool alive = true;
   const int c0 = 2 * (lane & 3);  // this thread's columns (rows of the item): c0, c0 + 1 of every eight
@@ -374,7 +374,8 @@ __global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
     }
     const bool any_odd = __syncthreads_or(odd) != 0;
     const bool whole = first_tile == 0 && end_tile == blk.ntile;
-    const AttnShare share = attn_share(cur.ub, blk.ntile, st);
+    AttnShare share = {0, 0};
+    if (!whole) share = attn_share(cur.ub, blk.ntile, st);
     auto store = [&](int r, int i, float4 v) {
       *reinterpret_cast<float4*>(p.out + attn_row_offset(p, cur.seq.q0 + blk.t0, cur.head, r, p.out_stride) + i) = v;
     };

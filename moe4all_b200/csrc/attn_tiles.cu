@@ -113,6 +113,7 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int wg = warp >> 2, role = wg == 3 ? 3 + (warp & 3) : wg < Sh::W_GROUPS ? 0 : 1;  // 0 weights, 1 sums, 3 copies, 4 MMAs, 5 and 6 hidden keys
 
+  pdl_trigger();  // the next kernel may take the SMs that this one leaves free, and do what needs no input of its
   if (tid == 0) {
     for (int i = 0; i < ITEMS; ++i) mbar_init(bars.i_full + i, 1);
     for (int i = 0; i < 4; ++i) mbar_init(bars.k_empty + i, 1), mbar_init(bars.v_full + i, 1), mbar_init(bars.v_empty + i, 1), mbar_init(bars.ready + i, 4 * (Sh::W_GROUPS + Sh::S_GROUPS) + 3);

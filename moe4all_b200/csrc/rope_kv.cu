@@ -40,6 +40,7 @@ __global__ void __launch_bounds__(ROPE_THREADS) k_rope_kv(const __grid_constant_
   const int pairs = p.n_rot / 2, batch = pairs ? min(ROPE_ROWS, ROPE_THREADS / pairs) : ROPE_ROWS;
   const int my_row = pairs ? tid / pairs : 0, my_pair = pairs ? tid - my_row * pairs : 0;
   const bool turns_one = pairs && my_row < batch;
+  pdl_trigger();
   double turns = p.turns0, x = p.ratio;  // of this thread's pair, per token: turns0 * ratio^pair by squares
 #pragma unroll 1
   for (int b = my_pair; b; b >>= 1, x *= x)
