@@ -176,6 +176,8 @@ int32_t drain_and_poll(infr_cuda_ctx* ctx, const char* what) {
     st->bad_index = 0;
     // a router launch that gave up may have left logits behind: every word back to "not written yet"
     if (tag && ctx->route_logits) cudaMemset(ctx->route_logits, 0xFF, ROUTE_LOGIT_BYTES);
+    // and an attention launch join counters
+    if (tag && ctx->attn_count) cudaMemset(ctx->attn_count, 0, ATTN_MAX_CTAS * sizeof(int));
     if (tag) {
       char msg[96];
       std::snprintf(msg, sizeof msg, "a bounded device-side wait ran out (kernel tag %d); outputs of that call are invalid", tag);
@@ -246,6 +248,7 @@ void infr_cuda_destroy(infr_cuda_ctx* ctx) {
   if (ctx->status_host) cudaFreeHost(ctx->status_host);
   if (ctx->route_logits) cudaFree(ctx->route_logits);
   if (ctx->attn_count) cudaFree(ctx->attn_count);
+  if (ctx->attn_parts) cudaFree(ctx->attn_parts);
   if (ctx->own_stream) cudaStreamDestroy(ctx->own_stream);
   delete ctx;
 }
@@ -1139,6 +1142,10 @@ int32_t infr_cuda_rope_kv(infr_cuda_ctx* ctx, const infr_cuda_rope_kv_desc* d) {
     return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "rope_kv: q_out overlaps q, k or v without being q itself");
   if (overlap(d->k_cache, nc, d->v_cache, nc) || overlap(d->k_cache, nc, d->q_out, nq) || overlap(d->v_cache, nc, d->q_out, nq))
     return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "rope_kv: k_cache, v_cache and q_out must not overlap");
+  for (const infr_cuda_buf* c : {d->k_cache, d->v_cache})
+    if (overlap(c, nc, d->q, attn_span(d->rows, p.q_stride, wide_q) * 4) || overlap(c, nc, d->k, attn_span(d->rows, p.k_stride, wide_kv) * 4) ||
+        overlap(c, nc, d->v, attn_span(d->rows, p.v_stride, wide_kv) * 4))
+      return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "rope_kv: a cache overlaps the rows that go into it");
   DeviceGuard g(ctx->device);
   attn_batch_params(p, ctx, d);
   p.q = static_cast<const float*>(d->q->ptr);
@@ -1192,11 +1199,19 @@ int32_t infr_cuda_attention(infr_cuda_ctx* ctx, const infr_cuda_attention_desc* 
     if (d->page_size == (1u << i)) p.page_shift = i;
   const uint64_t max_rows = (uint64_t)(d->max_q && d->max_q < d->rows ? d->max_q : d->rows) * g;
   const bool few = d->path ? d->path == 1 : max_rows <= (uint64_t)ATTN_ROWS_LIMIT;
-  const size_t item_rows = few ? ATTN_ROWS_LIMIT : ATTN_TILE_ROWS, slots = 2 * (size_t)ctx->sm_count;
-  const size_t part = align_up(slots * item_rows * 256 * 4, 256);
-  if ((rc = ensure_scratch(ctx, part + slots * item_rows * 8))) return rc;
-  p.part = static_cast<float*>(ctx->scratch);
-  p.part_ml = reinterpret_cast<float2*>(static_cast<char*>(ctx->scratch) + part);
+  // two partial results of 128 rows of 256 values for each CTA, their maxima and weights behind them
+  const size_t part = align_up(2 * (size_t)ctx->sm_count * ATTN_TILE_ROWS * 256 * 4, 256);
+  if (!ctx->attn_parts) {
+    if (ctx->capturing) return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "attention: its workspace would have to be made while recording: run the call once un-recorded first");
+    const cudaError_t e = cudaMalloc(&ctx->attn_parts, part + 2 * (size_t)ctx->sm_count * ATTN_TILE_ROWS * 8);
+    if (e != cudaSuccess) {
+      ctx->attn_parts = nullptr;
+      cudaGetLastError();
+      return check_cuda(ctx, e, "attention: workspace");
+    }
+  }
+  p.part = reinterpret_cast<float*>(ctx->attn_parts);
+  p.part_ml = reinterpret_cast<float2*>(ctx->attn_parts + part);
   const __half* k = static_cast<const __half*>(d->k->ptr);
   return few ? launch_attn_rows(ctx, p, k, (int)(max_rows < 1024 ? max_rows : 1024)) : launch_attn_tiles(ctx, p, k);
 }

@@ -434,7 +434,7 @@ cudaError_t run_rows(infr_cuda_ctx* ctx, const CUtensorMap& km, const CUtensorMa
   using Sh = RowsShape<HD, NT>;
   const cudaError_t e = ensure_smem(reinterpret_cast<const void*>(&k_attn_rows<HD, NT>), Sh::SMEM);
   if (e != cudaSuccess) return e;
-  return launch_ex(k_attn_rows<HD, NT>, dim3(ctx->sm_count), dim3(Sh::THREADS), Sh::SMEM, ctx->stream, true, km, vm, p);
+  return launch_ex(k_attn_rows<HD, NT>, dim3(ctx->sm_count < ATTN_MAX_CTAS ? ctx->sm_count : ATTN_MAX_CTAS), dim3(Sh::THREADS), Sh::SMEM, ctx->stream, true, km, vm, p);
 }
 
 }  // namespace

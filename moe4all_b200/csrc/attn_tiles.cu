@@ -681,7 +681,7 @@ cudaError_t run_tiles(infr_cuda_ctx* ctx, const CUtensorMap& km, const CUtensorM
   using Sh = TilesShape<HD>;
   const cudaError_t e = ensure_smem(reinterpret_cast<const void*>(&k_attn_tiles<HD>), Sh::SMEM);
   if (e != cudaSuccess) return e;
-  return launch_ex(k_attn_tiles<HD>, dim3(ctx->sm_count), dim3(Sh::THREADS), Sh::SMEM, ctx->stream, true, km, vm, p, granule);
+  return launch_ex(k_attn_tiles<HD>, dim3(ctx->sm_count < ATTN_MAX_CTAS ? ctx->sm_count : ATTN_MAX_CTAS), dim3(Sh::THREADS), Sh::SMEM, ctx->stream, true, km, vm, p, granule);
 }
 
 }  // namespace

@@ -76,6 +76,8 @@ struct infr_cuda_ctx {
   float* route_logits = nullptr;              // device memory: the whole-row router kernel's logit buffer, all words
                                               // "not written yet" between launches (see ROUTE_LOGIT_EMPTY)
   int* attn_count = nullptr;                  // device memory: join counters of the attention kernels, zero between launches
+  char* attn_parts = nullptr;                 // and their partial results: one block of its final size, so that a recorded
+                                              // plan's address of it holds whatever is called later
   unsigned long long* trace = nullptr;        // optional phase stamps (see trace_stamp)
   infr_cuda_config cfg = {};                  // tuning switches (infr_cuda_set_config)
   infr::EpState* ep = nullptr;                // expert-parallel communicator and buffers, or null

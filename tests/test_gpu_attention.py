@@ -349,6 +349,50 @@ def test_recorded_plan_follows_lengths_and_tables(backend):
         assert float((b.out - want).abs().max()) <= tol and float((c.out - want2).abs().max()) <= tol2
 
 
+def test_recorded_step_outlives_larger_calls(backend):
+    """A decode step recorded by a fresh context, then a prompt of another kernel and size: the plan's workspace is still its own."""
+    import torch
+
+    from moe4all_b200 import BackendError, CudaBackend
+
+    be = CudaBackend(0)
+    b = Batch([1, 1], [3000, 5000], 8, 2, 128, page=16, seed=30)
+    op = b.op(be)
+    be.graph_begin()
+    with pytest.raises(BackendError, match="un-recorded"):
+        be.attention(op)
+    be.graph_end()
+    be.attention(op)
+    be.sync()
+    be.graph_begin()
+    be.attention(op)
+    plan = be.graph_end()
+    c = Batch([700], [4000], 16, 2, 256, page=16, seed=31)
+    check(be, c)
+    keep = [torch.zeros(32 << 20, dtype=torch.uint8, device="cuda") for _ in range(4)]
+    want, tol = b.ref()
+    b.out.zero_()
+    torch.cuda.synchronize()
+    be.execute(plan)
+    be.sync()
+    assert float((b.out - want).abs().max()) <= tol
+    assert not any(bool(x.any()) for x in keep)
+    del plan, op
+    be.close()
+
+
+@pytest.mark.parametrize("path", [1, 2])
+@pytest.mark.parametrize("scale", [0.0, -0.125, 1e-30])
+def test_scales_that_are_zero_negative_or_tiny(backend, path, scale):
+    check(backend, Batch([1, 40, 200], [300, 20, 0], 8, 2, 64, page=16, seed=32), scale=scale, path=path)
+
+
+def test_bound_that_is_too_small(backend):
+    # max_q only picks the kernel: sequences longer than it says are served all the same
+    check(backend, Batch([90, 1, 300], [10, 20, 0], 8, 2, 128, page=16, seed=33), max_q=1)
+    check(backend, Batch([1, 1, 1], [10, 2000, 0], 8, 2, 128, page=16, seed=34), max_q=10 ** 6)
+
+
 def test_on_the_callers_stream(backend):
     import torch
 
@@ -581,7 +625,7 @@ def test_rope_refusals(backend):
     part = be.wrap(r.q_out.data_ptr(), 64)
     for kw in (dict(n_rot=60), dict(n_rot=72), dict(rope_base=0.0), dict(rope_base=-1.0), dict(rope_base=float("inf")), dict(rope_scale=NAN), dict(norm_eps=-1.0),
                dict(q_norm=part), dict(freq_factors=part), dict(q_stride=516 - 2), dict(k_stride=64), dict(q_out=part), dict(v=part), dict(v_cache=ok.k_cache),
-               dict(q_out=ok.q, q_out_stride=516), dict(q_out=ok.k_cache), dict(n_head=7), dict(kv_len=None)):
+               dict(q_out=ok.q, q_out_stride=516), dict(q_out=ok.k_cache), dict(k=ok.k_cache), dict(n_head=7), dict(kv_len=None)):
         with pytest.raises(BackendError) as e:
             be.rope_kv(dataclasses.replace(ok, **kw))
         assert not isinstance(e.value, Unsupported), kw
