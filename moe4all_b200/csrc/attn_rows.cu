@@ -28,7 +28,7 @@ __device__ __forceinline__ uint32_t movm(uint32_t a) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
 }
-constexpr int ROWS_EXTRA = 1;  // tiles' time that an item's beginning and end take
+constexpr int ROWS_EXTRA = 3;  // tiles' time that an item's beginning and end take (64 streams: 1 93.7, 3 86.1, 6 87.0 us)
 
 template <int HD, int NT>
 struct RowsShape {
@@ -53,8 +53,7 @@ __global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
   using Sh = RowsShape<HD, NT>;
   constexpr int WARPS = Sh::WARPS, THREADS = Sh::THREADS, RB = Sh::RB, UNITS = Sh::UNITS, UNIT = Sh::UNIT, SIDE = Sh::SIDE, PITCH = Sh::PITCH, SLOTS = Sh::SLOTS;
   constexpr int SLABS = HD / 64, KST = HD / 16;
-  constexpr bool Q_SHARED = HD > 128;
-  static_assert(!Q_SHARED || NT * KST * 512 <= Sh::MERGE, "q's pieces lie where the sums go");
+  static_assert(NT * KST * 512 <= Sh::MERGE, "q's pieces lie where the sums go");
   extern __shared__ unsigned char smem_raw[];
   __shared__ long long s_scan[WARPS];
   __shared__ AttnStart s_start;
@@ -145,58 +144,48 @@ __global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
     const AttnBlock& blk = cur.blk;
     const int first_tile = cur.first(st), end_tile = cur.end(st), n_rows = blk.nt * p.g;
 
-    // ---- q: B fragments of q^T, rows scaled by a power of two, as two f16 pieces.  Wide heads' would take the registers that the products
-    // need (16 streams, heads of 256: every load waited for, 71 us): one warp puts them down where the sums go at the item's end
-    uint32_t qh[Q_SHARED ? 1 : NT][Q_SHARED ? 1 : KST][2], ql[Q_SHARED ? 1 : NT][Q_SHARED ? 1 : KST][2];
+    // ---- q: B fragments of q^T, rows scaled by a power of two, as two f16 pieces, put down by one warp per eight rows where the sums go
+    // at the item's end (in every warp's registers they took the products' room: heads of 256 71 us instead of 60 for 16 streams, of 128
+    // 93 instead of 90 for 64)
     float f[NT][2];  // of the thread's columns: score -> log2 units
     int lim[NT][2];  // and the last key their row sees
-    if (Q_SHARED) __syncthreads();  // the last item's sums have been read
+    __syncthreads();  // the last item's sums have been read
+    if (warp < NT) {
+      const int r = 8 * warp + (lane >> 2);
+      const bool has = r < n_rows;
+      const float* src = p.q + attn_row_offset(p, cur.seq.q0 + blk.t0, cur.head, has ? r : 0, p.q_stride);
+      float2 v[KST][2];
+      float big = 0.f;
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      if (!Q_SHARED || warp == n) {
-        const int r = 8 * n + (lane >> 2);
-        const bool has = r < n_rows;
-        const float* src = p.q + attn_row_offset(p, cur.seq.q0 + blk.t0, cur.head, has ? r : 0, p.q_stride);
-        float2 v[KST][2];
-        float big = 0.f;
+      for (int k = 0; k < KST; ++k)
 #pragma unroll
-        for (int k = 0; k < KST; ++k)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int i = 16 * k + 8 * j + c0;
-            v[k][j] = has && i < p.hd ? __ldcg(reinterpret_cast<const float2*>(src + i)) : make_float2(0.f, 0.f);
-            big = fmaxf(big, fmaxf(fabsf(v[k][j].x), fabsf(v[k][j].y)));
-          }
-        big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 1));
-        big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 2));
-        float down, up;
-        attn_row_scale(big, down, up);
-#pragma unroll
-        for (int k = 0; k < KST; ++k) {
-          uint4 w;
-          split2(v[k][0].x * down, v[k][0].y * down, w.x, w.z);
-          split2(v[k][1].x * down, v[k][1].y * down, w.y, w.w);
-          if constexpr (Q_SHARED) s_q[(n * KST + k) * 32 + lane] = w;
-          else qh[n][k][0] = w.x, qh[n][k][1] = w.y, ql[n][k][0] = w.z, ql[n][k][1] = w.w;
+        for (int j = 0; j < 2; ++j) {
+          const int i = 16 * k + 8 * j + c0;
+          v[k][j] = has && i < p.hd ? __ldcg(reinterpret_cast<const float2*>(src + i)) : make_float2(0.f, 0.f);
+          big = fmaxf(big, fmaxf(fabsf(v[k][j].x), fabsf(v[k][j].y)));
         }
-        if constexpr (Q_SHARED) {
-          if ((lane & 3) == 0) s_factor[8 * n + (lane >> 2)] = up * p.scale_log2;
-        } else {
+      big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 1));
+      big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 2));
+      float down, up;
+      attn_row_scale(big, down, up);
 #pragma unroll
-          for (int j = 0; j < 2; ++j) f[n][j] = __shfl_sync(0xFFFFFFFFu, up, (c0 + j) * 4) * p.scale_log2;
-        }
+      for (int k = 0; k < KST; ++k) {
+        uint4 w;
+        split2(v[k][0].x * down, v[k][0].y * down, w.x, w.z);
+        split2(v[k][1].x * down, v[k][1].y * down, w.y, w.w);
+        s_q[(warp * KST + k) * 32 + lane] = w;
       }
+      if ((lane & 3) == 0) s_factor[r] = up * p.scale_log2;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const int rr = 8 * n + c0 + j;
+        f[n][j] = s_factor[rr];
         lim[n][j] = cur.seq.past + blk.t0 + (rr < n_rows ? attn_row_token(p, rr) : blk.nt - 1);
       }
-    }
-    if constexpr (Q_SHARED) {
-      __syncthreads();
-#pragma unroll
-      for (int n = 0; n < NT; ++n) f[n][0] = s_factor[8 * n + c0], f[n][1] = s_factor[8 * n + c0 + 1];
-    }
     const int full_hi = attn_full_hi(cur.seq, blk), full_lo = attn_full_lo(p, cur.seq, blk);
 
     float o[KST][NT][4], m[NT][2], l[NT][2];
@@ -233,9 +222,7 @@ __global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
           ldsm4(a, kb + (k >> 2) * 2048 + ((i4 & 1) * 8 + r8) * 128 + (((2 * (k & 3) + (i4 >> 1)) ^ r8) << 4));
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            uint4 w;
-            if constexpr (Q_SHARED) w = s_q[(n * KST + k) * 32 + lane];
-            else w = make_uint4(qh[n][k][0], qh[n][k][1], ql[n][k][0], ql[n][k][1]);
+            const uint4 w = s_q[(n * KST + k) * 32 + lane];
             mma16816(k & 1 ? part[n][0] : s[n], a, w.x, w.y);
             mma16816(k & 1 ? part[n][2] : part[n][1], a, w.z, w.w);
           }
