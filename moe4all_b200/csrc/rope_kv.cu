@@ -78,8 +78,10 @@ __global__ void __launch_bounds__(ROPE_THREADS) k_rope_kv(const __grid_constant_
   if (tid < batch) seq = load(s);
 
   float4 a[JS], b[JS];  // of the head that comes next
-  auto fetch = [&](int row0, int rows, int e) {
-    const int i = e / n_vec, h = e - i * n_vec, r = row0 + i;
+  int fi = 0, fh = 0;   // its row of the batch and its number
+  auto fetch = [&](int row0, int rows) {
+    while (fh >= n_vec) fh -= n_vec, ++fi;
+    const int i = fi, h = fh, r = row0 + i;
     const bool is_q = h < p.n_head, is_v = h >= p.n_head + p.n_kv;
     const float* src = is_q ? p.q + (size_t)r * p.q_stride + (size_t)h * p.hd
                             : (is_v ? p.v + (size_t)r * p.v_stride + (size_t)(h - p.n_head - p.n_kv) * p.hd : p.k + (size_t)r * p.k_stride + (size_t)(h - p.n_head) * p.hd);
@@ -96,7 +98,8 @@ __global__ void __launch_bounds__(ROPE_THREADS) k_rope_kv(const __grid_constant_
 #pragma unroll 1
   for (int row0 = r0; row0 < r1; row0 += batch) {
     const int rows = min(batch, r1 - row0);
-    fetch(row0, rows, team);
+    fi = 0, fh = team;
+    fetch(row0, rows);
     if (tid < rows) {  // positions, and places in the cache (-1: none)
       const int r = row0 + tid;
 #pragma unroll 1
@@ -120,8 +123,8 @@ __global__ void __launch_bounds__(ROPE_THREADS) k_rope_kv(const __grid_constant_
     __syncthreads();
 #pragma unroll 1
     for (int e0 = 0; e0 < rows * n_vec; e0 += ROPE_TEAMS) {
-      const int e = e0 + team, i = min(e / n_vec, rows - 1), h = e - (e / n_vec) * n_vec, r = row0 + i;
-      const bool is_q = h < p.n_head, is_v = h >= p.n_head + p.n_kv, has = e < rows * n_vec && s_pos[i] >= 0;
+      const int i = min(fi, rows - 1), h = fh, r = row0 + i;
+      const bool is_q = h < p.n_head, is_v = h >= p.n_head + p.n_kv, has = fi < rows && s_pos[i] >= 0;
       const float* w = is_v ? nullptr : (is_q ? p.q_norm : p.k_norm);
       float4 x[JS], y[JS];
       float sq = 0.f;
@@ -130,7 +133,8 @@ __global__ void __launch_bounds__(ROPE_THREADS) k_rope_kv(const __grid_constant_
         x[j] = a[j], y[j] = b[j];
         sq += x[j].x * x[j].x + x[j].y * x[j].y + x[j].z * x[j].z + x[j].w * x[j].w + y[j].x * y[j].x + y[j].y * y[j].y + y[j].z * y[j].z + y[j].w * y[j].w;
       }
-      if (e0 + ROPE_TEAMS < rows * n_vec) fetch(row0, rows, e + ROPE_TEAMS);
+      fh += ROPE_TEAMS;
+      if (e0 + ROPE_TEAMS < rows * n_vec) fetch(row0, rows);
       if (p.q_norm != nullptr || p.k_norm != nullptr) sq = team_sum(sq);  // (every lane takes part)
       if (!has) continue;
       const float k = w != nullptr ? rsqrtf(sq / (float)p.hd + p.norm_eps) : 1.f;
