@@ -369,54 +369,46 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
       const int n_rows = it.n_rows, l8 = lane & 7, r8 = tid >> 3;
       const float* q_item = p.q + (size_t)it.row0 * p.q_stride + (size_t)it.head * p.g * p.hd + 4 * l8;
       const int stride = (int)p.q_stride, head_pitch = p.hd, g = p.g;
-      constexpr int STEP = 16 * GROUPS, AT_ONCE = 1;
-      float4 ahead[AT_ONCE][HD / 32];
-      auto load = [&](int r0) {
+      constexpr int STEP = 16 * GROUPS;
+      float4 ahead[HD / 32];
+      auto load = [&](int r) {
+        const int t = attn_row_token(p, r);
+        const float* src = q_item + (t * stride + (r - t * g) * head_pitch);
 #pragma unroll
-        for (int a = 0; a < AT_ONCE; ++a) {
-          const int r = r0 + a * STEP, t = attn_row_token(p, r);
-          const float* src = q_item + (t * stride + (r - t * g) * head_pitch);
-#pragma unroll
-          for (int j = 0; j < HD / 32; ++j)
-            ahead[a][j] = r < n_rows && 4 * (l8 + 8 * j) < p.hd ? __ldcg(reinterpret_cast<const float4*>(src + 32 * j)) : make_float4(0.f, 0.f, 0.f, 0.f);
-        }
+        for (int j = 0; j < HD / 32; ++j)
+          ahead[j] = r < n_rows && 4 * (l8 + 8 * j) < p.hd ? __ldcg(reinterpret_cast<const float4*>(src + 32 * j)) : make_float4(0.f, 0.f, 0.f, 0.f);
       };
       load(r8);
       if (item > 0) ok = wait_all(bars.q_empty + ((item - 1) & (RING - 1)), (item - 1) / RING);
       if (!ok) return;
       float* fac = s_fac + (item & (RING - 1)) * 128;
 #pragma unroll 1
-      for (int r0 = 0; r0 < n_rows; r0 += AT_ONCE * STEP) {
-        float4 v[AT_ONCE][HD / 32];
+      for (int r0 = 0; r0 < n_rows; r0 += STEP) {
+        const int r = r0 + r8;
+        float4 v[HD / 32];
+        float big = 0.f;
 #pragma unroll
-        for (int a = 0; a < AT_ONCE; ++a)
+        for (int j = 0; j < HD / 32; ++j) v[j] = ahead[j];
+        if (r0 + STEP < n_rows) load(r + STEP);
 #pragma unroll
-          for (int j = 0; j < HD / 32; ++j) v[a][j] = ahead[a][j];
-        if (r0 + AT_ONCE * STEP < n_rows) load(r0 + AT_ONCE * STEP + r8);
+        for (int j = 0; j < HD / 32; ++j) big = fmaxf(big, fmaxf(fmaxf(fabsf(v[j].x), fabsf(v[j].y)), fmaxf(fabsf(v[j].z), fabsf(v[j].w))));
 #pragma unroll
-        for (int a = 0; a < AT_ONCE; ++a) {
-          const int r = r0 + a * STEP + r8;
-          float big = 0.f;
+        for (int x = 1; x < 8; x <<= 1) big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, x));
+        float down, up;
+        attn_row_scale(big, down, up);
+        if (p.scale_log2 < 0.f) down = -down;
+        unsigned char* row_at = s_q + r * 128 + ((l8 & 1) << 3);
 #pragma unroll
-          for (int j = 0; j < HD / 32; ++j) big = fmaxf(big, fmaxf(fmaxf(fabsf(v[a][j].x), fabsf(v[a][j].y)), fmaxf(fabsf(v[a][j].z), fabsf(v[a][j].w))));
-#pragma unroll
-          for (int x = 1; x < 8; x <<= 1) big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, x));
-          float down, up;
-          attn_row_scale(big, down, up);
-          if (p.scale_log2 < 0.f) down = -down;
-          unsigned char* row_at = s_q + r * 128 + ((l8 & 1) << 3);
-#pragma unroll
-          for (int j = 0; j < HD / 32; ++j) {
-            uint2 hi, lo;
-            split2(v[a][j].x * down, v[a][j].y * down, hi.x, lo.x);
-            split2(v[a][j].z * down, v[a][j].w * down, hi.y, lo.y);
-            unsigned char* dst = row_at + (j >> 1) * 16384 + ((((l8 >> 1) + 4 * (j & 1)) ^ (r & 7)) << 4);
-            *reinterpret_cast<uint2*>(dst) = hi;
-            *reinterpret_cast<uint2*>(dst + Sh::QPIECE) = lo;
-          }
-          // (not 0: hidden keys' -inf times it stays -inf)
-          if (l8 == 0) fac[r] = fmaxf(up * fabsf(p.scale_log2), 1.2e-38f);
+        for (int j = 0; j < HD / 32; ++j) {
+          uint2 hi, lo;
+          split2(v[j].x * down, v[j].y * down, hi.x, lo.x);
+          split2(v[j].z * down, v[j].w * down, hi.y, lo.y);
+          unsigned char* dst = row_at + (j >> 1) * 16384 + ((((l8 >> 1) + 4 * (j & 1)) ^ (r & 7)) << 4);
+          *reinterpret_cast<uint2*>(dst) = hi;
+          *reinterpret_cast<uint2*>(dst + Sh::QPIECE) = lo;
         }
+        // (not 0: hidden keys' -inf times it stays -inf)
+        if (l8 == 0) fac[r] = fmaxf(up * fabsf(p.scale_log2), 1.2e-38f);
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
