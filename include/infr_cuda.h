@@ -364,7 +364,8 @@ typedef struct infr_cuda_rope_kv_desc {
   const infr_cuda_buf* k;            /* [rows, n_kv, head_dim] f32, rows k_stride apart                       */
   const infr_cuda_buf* v;            /* [rows, n_kv, head_dim] f32, rows v_stride apart                       */
   infr_cuda_buf* q_out;              /* [rows, n_head, head_dim] f32, rows q_out_stride apart; may be q itself
-                                        (same handle or address, same stride), else apart from q, k and v     */
+                                        (same handle or address, same stride; its rows may lie between those
+                                        of k and v), else apart from q, k and v                               */
   infr_cuda_buf *k_cache, *v_cache;  /* f16, see above                                                        */
   const infr_cuda_buf *cu_q, *kv_len, *page_table;
   const infr_cuda_buf *q_norm, *k_norm; /* [head_dim] f32: RmsNorm over each head of q / k first, or NULL    */

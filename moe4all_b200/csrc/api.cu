@@ -1140,6 +1140,10 @@ int32_t infr_cuda_rope_kv(infr_cuda_ctx* ctx, const infr_cuda_rope_kv_desc* d) {
   if (!in_place && (overlap(d->q_out, nq, d->q, attn_span(d->rows, p.q_stride, wide_q) * 4) || overlap(d->q_out, nq, d->k, attn_span(d->rows, p.k_stride, wide_kv) * 4) ||
                     overlap(d->q_out, nq, d->v, attn_span(d->rows, p.v_stride, wide_kv) * 4)))
     return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "rope_kv: q_out overlaps q, k or v without being q itself");
+  if (in_place)
+    for (const auto& [b, stride] : {std::pair{d->k, p.k_stride}, std::pair{d->v, p.v_stride}})
+      if (attn_rows_meet(reinterpret_cast<uintptr_t>(d->q->ptr), wide_q * 4ull, p.q_stride * 4ull, reinterpret_cast<uintptr_t>(b->ptr), wide_kv * 4ull, stride * 4ull, d->rows))
+        return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "rope_kv: q is rotated in place and k or v lies in its rows");
   if (overlap(d->k_cache, nc, d->v_cache, nc) || overlap(d->k_cache, nc, d->q_out, nq) || overlap(d->v_cache, nc, d->q_out, nq))
     return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "rope_kv: k_cache, v_cache and q_out must not overlap");
   for (const infr_cuda_buf* c : {d->k_cache, d->v_cache})

@@ -110,4 +110,13 @@ inline const char* attn_sizes_error(const AttnSizes& s, bool* unsupported) {
 // Values a buffer needs for `rows` rows of `wide` values that are `stride` apart.
 inline uint64_t attn_span(uint64_t rows, uint64_t stride, uint64_t wide) { return rows ? (rows - 1) * stride + wide : 0; }
 
+// Whether two sets of rows (addresses a and b; bytes of a row, bytes between rows) share a byte.  Of one stride they may lie between each
+// other, as the parts of wide rows do; of two, spans that overlap count as shared.
+inline bool attn_rows_meet(uint64_t a, uint64_t wide_a, uint64_t stride_a, uint64_t b, uint64_t wide_b, uint64_t stride_b, uint64_t rows) {
+  if (!(a < b + attn_span(rows, stride_b, wide_b) && b < a + attn_span(rows, stride_a, wide_a))) return false;
+  if (stride_a != stride_b) return true;
+  const uint64_t d = b >= a ? (b - a) % stride_a : (stride_a - (a - b) % stride_a) % stride_a;  // from a row of a to the next row of b
+  return d < wide_a || d + wide_b > stride_a;
+}
+
 }  // namespace infr

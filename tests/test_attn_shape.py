@@ -82,3 +82,19 @@ def test_wrong_arrays_are_forced_into_range(exe, cu, kv):
 def test_sizes(exe, sizes, want):
     out = subprocess.run([exe, "sizes", *map(str, sizes)], capture_output=True, text=True, check=True).stdout
     assert out.split(":")[0].strip() == want, out
+
+
+@pytest.mark.parametrize("seed", range(30))
+def test_rows_that_share_bytes(exe, seed):
+    r = random.Random(seed)
+    for _ in range(8):
+        stride, rows = r.randint(4, 40), r.randint(1, 5)
+        wa, wb = r.randint(1, stride), r.randint(1, stride)
+        a, b = 1000, 1000 + r.randint(-2 * stride, rows * stride + 3)
+        used = lambda at, w: {at + i * stride + j for i in range(rows) for j in range(w)}
+        got = subprocess.run([exe, "meet"] + [str(x) for x in (a, wa, stride, b, wb, stride, rows)], capture_output=True, text=True).stdout
+        assert got == f"{int(bool(used(a, wa) & used(b, wb)))}\n", (a, wa, stride, b, wb, rows)
+    # the parts of wide rows lie between each other; of two strides, spans count
+    meet = lambda *x: subprocess.run([exe, "meet"] + [str(i) for i in x], capture_output=True, text=True).stdout == "1\n"
+    assert not meet(0, 32, 48, 32, 8, 48, 100) and not meet(0, 32, 48, 40, 8, 48, 100) and meet(0, 32, 48, 28, 8, 48, 100)
+    assert meet(0, 32, 48, 32, 8, 44, 100) and not meet(0, 32, 48, 99 * 48 + 32, 8, 44, 100)

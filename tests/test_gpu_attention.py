@@ -592,6 +592,24 @@ def test_rope_in_place(backend):
     assert float(((r.parts[0].double() - want[0]).abs() - 2.0 ** -20 * mag[0]).max()) <= 0
 
 
+def test_rope_in_place_in_wide_rows(backend):
+    from moe4all_b200 import BackendError
+
+    b = Batch([5, 40], [7, 100], 8, 2, 128, page=16, seed=25)
+    r = Rope(b, 128, True, norm=True, factors=False, fused=True)
+    op = r.op(backend)
+    op = dataclasses.replace(op, q_out=op.q, q_out_stride=op.q_stride)
+    for kw in (dict(k=op.q), dict(v=op.q), dict(k_stride=op.k_stride - 12)):  # rows that the call would read and write
+        with pytest.raises(BackendError, match="in place"):
+            backend.rope_kv(dataclasses.replace(op, **kw))
+    rest = r.qkv[:, 8 * 128 :].clone()
+    want, mag = r.ref()
+    backend.rope_kv(op)
+    backend.sync()
+    assert float(((r.parts[0].double() - want[0]).abs() - 2.0 ** -20 * mag[0]).max()) <= 0
+    assert bool((r.qkv[:, 8 * 128 :] == rest).all())
+
+
 def test_rope_negative_positions_and_bad_pages(backend):
     from moe4all_b200 import BackendError
 
