@@ -11,9 +11,15 @@
 //             to a common maximum: an accumulation over thousands of steps in the tensor cores, which truncate, would lose an f32
 //             result's last bits (measured: 1.3e-8 of the result per step)
 //   control   a warp for the copies, a warp for the MMAs, two that look after tiles with hidden keys
-// S and P of two tiles, and the sums of two (one for heads wider than 192), fill tensor memory: while a tile's weights are made the
-// tensor cores work on the next tile's scores and the last one's sums.  Loops are kept rolled: with every tile's code straight-line the
-// roles together left the instruction cache (60% hits, 4.6 ms for an 8192-token prompt instead of 4.1).
+// S and P of two tiles, and the sums of two (one for heads wider than 64), fill tensor memory: while a tile's weights are made the
+// tensor cores work on the next tile's scores and the last one's sums.
+//
+// Measured (us; the tensor cores' floor at 2 x 4 hd operations a pair and the measured 1666 TFLOP/s): 8192 tokens of 32 / 4 heads of 128 1046 (660),
+// four chunks of 512 tokens over up to 16000 keys 576 (366), 8192 tokens in 16 sequences of 64 / 8 heads of 64 235 (51).  What bounds it is
+// the weights: 3.0 thousand cycles a tile of 128 keys (maxima 0.6, powers of two and pieces 1.7, the rest waits), against 2.1 - 2.3 of MMAs.  Short
+// sequences of narrow heads pay per item: q into pieces 3 - 4 thousand cycles, results out 4 - 5, masked tiles on the diagonal.
+// Loops are kept rolled, and waits short: the roles share one instruction cache, and with every tile's code straight-line it hit 60% of
+// the time and the 8192 tokens took 4.6 ms.  (The weights' loop over 32 keys of 64 unrolled: 628 -> 685 us for the chunks as they were then.)
 #include "attn.cuh"
 #include "umma.cuh"
 
@@ -27,7 +33,9 @@ constexpr int RING = 4;            // tiles' and items' words in shared memory: 
 template <int HD>
 struct TilesShape {
   static constexpr int LOG2_TILE = HD <= 128 ? 7 : 6, BK = 1 << LOG2_TILE;
-  static constexpr int EXTRA = HD == 64 ? 2 : 3;  // tiles' time that an item's beginning and end take
+  // tiles' time that an item's beginning and end take (16 sequences of heads of 64: 2 257, 3 269, 4 281 us as they were then; wider heads' tiles are
+  // 64 keys or twice the work, and their results twice the columns and more)
+  static constexpr int EXTRA = HD == 64 ? 2 : 3;
   static constexpr int W_GROUPS = BK / 64;
   static constexpr int S_GROUPS = 3 - W_GROUPS, COLS = HD / S_GROUPS;  // columns of a sums thread
   static constexpr int THREADS = 512;
@@ -231,6 +239,8 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
     const uint64_t qdesc = umma::smem_desc_k_major_swz128(s_q, 0), kdesc = umma::smem_desc_k_major_swz128(s_k, 0);
     const uint64_t vdesc = umma::smem_desc_mn_major_swz128(smem_u32(s_v), 0, BK * 128);
     int s_it = 0, s_end = 0;  // items whose scores have begun, and the end of the last one's tiles
+    // Both products take the smaller pieces first: the tensor cores truncate at every step, and then half of the steps only what is 2^-11
+    // of the result (scores of size 10 in heads of 128: 16 steps' worth of 2^-24 of them would otherwise be on every weight).
     // Step n: the sums of tile n, then the scores of tile n + 2, whose accumulators are free by then: MMAs of one thread go in order.  What
     // is not there before a step is waited for behind the last step's MMAs.
 #pragma unroll 1
@@ -243,13 +253,11 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
         if (umma::elect_one()) {
           const uint32_t d = tmem + Sh::O_COL + (n % OBUFS) * HD, a = tmem + (n & 1) * BK;
           const uint64_t vd = vdesc + (uint64_t)((buf * TILE) >> 4);
+#pragma unroll 1
+          for (int piece = 1; piece >= 0; --piece)  // the small ones first: see above
 #pragma unroll 2
-          for (int k = 0; k < BK / 16; ++k) {
-            const uint64_t b = vd + (uint64_t)((k * 2048) >> 4);
-            const uint32_t ak = a + (k >> 1) * 32 + (k & 1) * 8;  // 32 keys: 16 columns of their weights, 16 of the rest
-            umma::mma1_f16_ts(d, ak, b, idesc_o, k > 0 ? 1u : 0u);
-            umma::mma1_f16_ts(d, ak + 16, b, idesc_o, 1u);
-          }
+            for (int k = 0; k < BK / 16; ++k)  // 32 keys: 16 columns of their weights, 16 of the rest
+              umma::mma1_f16_ts(d, a + (k >> 1) * 32 + (k & 1) * 8 + 16 * piece, vd + (uint64_t)((k * 2048) >> 4), idesc_o, piece == 0 || k > 0 ? 1u : 0u);
           umma::commit1(bars.o_full + n % OBUFS);
           umma::commit1(bars.v_empty + buf);
         }
@@ -281,12 +289,12 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
           const uint32_t d = tmem + (next & 1) * BK;
           const uint64_t kd = kdesc + (uint64_t)((buf * TILE) >> 4);
 #pragma unroll 1
-          for (int piece = 0; piece < 2; ++piece)
+          for (int piece = 1; piece >= 0; --piece)
 #pragma unroll 4
             for (int k = 0; k < HD / 16; ++k) {
               const uint64_t b = kd + (uint64_t)(((k >> 2) * (BK * 128) + (k & 3) * 32) >> 4);
-              if (piece < Sh::Q_TMEM) umma::mma1_f16_ts(d, tq + piece * (HD / 2) + 8 * k, b, idesc_s, piece + k > 0 ? 1u : 0u);
-              else umma::mma1_f16_ss(d, qdesc + (uint64_t)((piece * Sh::QPIECE + (k >> 2) * 16384 + (k & 3) * 32) >> 4), b, idesc_s, 1u);
+              if (piece < Sh::Q_TMEM) umma::mma1_f16_ts(d, tq + piece * (HD / 2) + 8 * k, b, idesc_s, piece == 0 || k > 0 ? 1u : 0u);
+              else umma::mma1_f16_ss(d, qdesc + (uint64_t)((piece * Sh::QPIECE + (k >> 2) * 16384 + (k & 3) * 32) >> 4), b, idesc_s, k > 0 ? 1u : 0u);
             }
           umma::commit1(bars.s_full + (next & 1));
           umma::commit1(bars.k_empty + buf);

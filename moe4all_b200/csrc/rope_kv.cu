@@ -6,6 +6,9 @@
 // and a frequency in 64 bits, reduced to a fraction of a turn before they are rounded to 32 (a position of 10^6 times a frequency near 1
 // keeps 4 bits of f32 after the point); a row's sines are worked out once for all of its heads, by as many threads as there are pairs in a
 // few rows.
+//
+// Measured: 8192 rows of 32 + 2 x 4 heads of 128 59.9 us, 5.3 TB/s of the rows and the cache (0.81 of the copy rate; 62.4 with heads divided
+// out of an index instead of counted on, 64.5 with five CTAs to an SM in place of four); 777 rows 9.9 us, 32 rows 4.8 us: launch, plan, one row's chain.
 #include "attn.cuh"
 
 namespace infr {
