@@ -121,7 +121,7 @@ struct AttnStart {
   long long u0, u1, ub;     // ub: where the block's first head begins
   long long before, until;  // tiles ahead of u0 and of u1
   AttnSeq seq;
-  int s, b;
+  int s, b, most;  // most: tiles of the line's longest item
 };
 
 // Inclusive sum over the block's threads; s_warp: one word per warp.
@@ -143,12 +143,13 @@ __device__ __forceinline__ long long block_scan(long long v, long long* s_warp) 
 
 // Every CTA works the whole line out for itself (a sequence and a few blocks per thread), which costs less than a launch for it.
 // known: 16 bytes per sequence and one word of shared memory, free again after the call.  All threads take part.
-template <int THREADS, int LOG2_TILE, int EXTRA>
+// JOIN: see attn_ctas; 0 where joins cost little.
+template <int THREADS, int LOG2_TILE, int EXTRA, int JOIN>
 __device__ __forceinline__ void attn_plan(const AttnParams& p, int* known, long long* s_warp, AttnStart* st) {
   const int tid = threadIdx.x;
   AttnSeq* seqs = reinterpret_cast<AttnSeq*>(known);
   int* pre = known + 3 * p.n_seq;  // blocks ahead of each sequence
-  if (tid == 0) pre[0] = 0;
+  if (tid == 0) pre[0] = st->most = 0;
   long long carry = 0;
 #pragma unroll 1
   for (int s0 = 0; s0 < p.n_seq; s0 += THREADS) {
@@ -176,7 +177,7 @@ __device__ __forceinline__ void attn_plan(const AttnParams& p, int* known, long 
 #pragma unroll 1
   for (int pass = 0; pass < 2; ++pass) {
     long long tiles = end - mine;
-    int at = s;
+    int at = s, most = 0;
 #pragma unroll 1
     for (int f = f0; f < f1; ++f) {
       while (f >= pre[at + 1]) ++at;
@@ -194,13 +195,15 @@ __device__ __forceinline__ void attn_plan(const AttnParams& p, int* known, long 
         }
       }
       tiles += nt;
+      if (JOIN > 0) most = max(most, nt);
     }
     if (pass == 0) {
       mine = tiles;
+      if (JOIN > 0 && most > 0) atomicMax(&st->most, most);
       end = block_scan<THREADS>(mine, s_warp);
       if (tid == THREADS - 1) {
         const long long units = (end + (long long)EXTRA * F) * p.n_kv;
-        const int ctas = (int)(units < (long long)gridDim.x ? units : (long long)gridDim.x);
+        const int ctas = attn_ctas(units, (int)gridDim.x, JOIN > 0 ? st->most + EXTRA : 0, JOIN);
         const bool idle = (int)blockIdx.x >= ctas;
         st->line.each = ctas > 0 ? units / ctas : 0;
         st->line.more = (int)(units - st->line.each * ctas);

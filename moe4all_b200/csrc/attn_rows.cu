@@ -79,7 +79,7 @@ __global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
     for (int i = 0; i < UNITS; ++i) mbar_init(full + i, 1);
   mbar_fence_init();
   pdl_wait();
-  attn_plan<THREADS, Sh::LOG2_TILE, ROWS_EXTRA>(p, reinterpret_cast<int*>(ring_all), s_scan, &s_start);
+  attn_plan<THREADS, Sh::LOG2_TILE, ROWS_EXTRA, 0>(p, reinterpret_cast<int*>(ring_all), s_scan, &s_start);
   const AttnStart st = s_start;
   if (st.until == st.before) return;
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the plan's words lay where the copies go

@@ -6,6 +6,8 @@
 // `extra` units and then its tiles, form one line, which the CTAs of the launch share evenly: a CTA takes the tiles in its piece.  An item whose tiles cross a border is joined from its CTAs' partial results, in their order, by whichever
 // finishes last.
 #pragma once
+#include <math.h>
+
 #include <cstddef>
 #include <cstdint>
 
@@ -79,6 +81,14 @@ INFR_ATTN_HD long long attn_begin(const AttnLine& l, int c) { return c * l.each 
 INFR_ATTN_HD int attn_cta_of(const AttnLine& l, long long i) {
   const long long wide = l.more * (l.each + 1);
   return i < wide ? attn_small_div(i, l.each + 1) : l.more + attn_small_div(i - wide, l.each);
+}
+
+// How many CTAs share a line of `units` whose longest item has `most`: all, unless joining the parts would take longer than the shares do.
+// A part costs its joiner `join` eighths of a unit, so shares of m units and most / m parts take m + most join / (8 m): least at m^2 = most join / 8.
+INFR_ATTN_HD int attn_ctas(long long units, int grid, int most, int join) {
+  const int m = (int)ceilf(sqrtf(0.125f * (float)join * (float)most));
+  const long long n = m > 1 ? units / m : units;
+  return (int)(units < 1 ? 0 : n < 1 ? 1 : n < grid ? n : grid);
 }
 
 // What a call gives, as numbers.

@@ -27,7 +27,7 @@ namespace infr {
 namespace {
 
 constexpr float TILE_BIAS = 15.f;  // weights are 2^(x - maximum + 15): below f16's limit, 2^-40 of the largest still has a bit
-constexpr int JOIN_PARTS = 32;     // parts of an item that are joined by column; more go row by row
+constexpr int JOIN_PARTS = 160;    // parts that an item can have: CTAs of a launch
 constexpr int RING = 4;            // tiles' and items' words in shared memory: the roles are never further apart
 
 template <int HD>
@@ -36,6 +36,9 @@ struct TilesShape {
   // tiles' time that an item's beginning and end take (16 sequences of heads of 64: 2 257, 3 269, 4 281 us as they were then; wider heads' tiles are
   // 64 keys or twice the work, and their results twice the columns and more)
   static constexpr int EXTRA = HD == 64 ? 2 : 3;
+  // what joining a part of an item takes, in eighths of a tile's time (us with 2, 4, 8 and 16: 9 tokens of 12 / 1 heads of 64
+  // over 42730 keys 34.4, 33.0, 33.1, 37.1; 61 of 10 / 2 heads of 192 over 5855 keys 34.2, 34.2, 45.6, 46.7)
+  static constexpr int JOIN = 4;
   static constexpr int W_GROUPS = BK / 64;
   static constexpr int S_GROUPS = 3 - W_GROUPS, COLS = HD / S_GROUPS;  // columns of a sums thread
   static constexpr int THREADS = 512;
@@ -133,7 +136,7 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
   if (tid < 4 * RING) s_odd[tid] = 0;
   if (warp == 0) umma::tmem_alloc(&s_tmem);
   pdl_wait();
-  attn_plan<Sh::THREADS, Sh::LOG2_TILE, Sh::EXTRA>(p, reinterpret_cast<int*>(s_q), s_scan, &s_start);
+  attn_plan<Sh::THREADS, Sh::LOG2_TILE, Sh::EXTRA, Sh::JOIN>(p, reinterpret_cast<int*>(s_q), s_scan, &s_start);
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the plan's words lay where tiles go
   umma::fence_before_sync();
   __syncthreads();
@@ -625,23 +628,18 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
         const AttnShare share = {it.first_cta, it.last_cta};
         const int n = share.last - share.first + 1, n_rows = it.n_rows, at = tid - 128 * Sh::W_GROUPS;
         float* base = p.out + (size_t)it.row0 * p.out_stride + (size_t)it.head * p.g * p.hd;
-        if (n > JOIN_PARTS) {
-#pragma unroll 1
-          for (int r = at >> 5; r < n_rows; r += 4 * Sh::S_GROUPS) attn_join_row<HD>(p, share, 128, r, base + attn_row_offset(p, 0, 0, r, p.out_stride));
-          continue;
-        }
-        // the parts' weights by row, then the sums by four columns, several in flight
-        float* s_w = reinterpret_cast<float*>(s_out);
-        static_assert(JOIN_PARTS * 128 * 4 <= Sh::OUT, "the parts' weights lie where results go");
+        // the parts' weights by row, then the sums by four columns, sixteen loads in flight (one after the other 11 parts of heads of 128 took 120 us)
+        float* s_w = reinterpret_cast<float*>(s_k);  // (this CTA's products are done)
+        static_assert(JOIN_PARTS * 128 * 4 <= 2 * BUFS * TILE + Sh::OUT, "the parts' weights lie where tiles and results were");
         if (at < n_rows) {
           float M = -CUDART_INF_F, L = 0.f;
-#pragma unroll 4
+#pragma unroll 8
           for (int c = 0; c < n; ++c) {
             const float2 ml = __ldcg(&p.part_ml[(size_t)attn_slot(share.first + c, share) * 128 + at]);
             s_w[c * 128 + at] = ml.x;
             M = fmaxf(M, ml.x);
           }
-#pragma unroll 4
+#pragma unroll 8
           for (int c = 0; c < n; ++c) {
             const float w = exp2_rel(s_w[c * 128 + at], M);
             if (w != 0.f) L += w * __ldcg(&p.part_ml[(size_t)attn_slot(share.first + c, share) * 128 + at]).y;  // (a part that saw nothing holds nothing)
@@ -653,17 +651,37 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
         }
         asm volatile("bar.sync 1, %0;" ::"n"(128 * Sh::S_GROUPS) : "memory");
         const int words = p.hd / 4, stride = (int)p.out_stride, head_pitch = p.hd, g = p.g;
-#pragma unroll 4
-        for (int e = at; e < n_rows * words; e += 128 * Sh::S_GROUPS) {
-          const int r = e / words, col = 4 * (e - r * words), t = attn_row_token(p, r);
-          float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 2
-          for (int c = 0; c < n; ++c) {
-            const float w = s_w[c * 128 + r];
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(p.part + ((size_t)attn_slot(share.first + c, share) * 128 + r) * HD + col));
-            if (w != 0.f) o.x += w * v.x, o.y += w * v.y, o.z += w * v.z, o.w += w * v.w;
+#pragma unroll 1
+        for (int e0 = at; e0 < n_rows * words; e0 += 4 * 128 * Sh::S_GROUPS) {
+          int row[4], col[4];
+          float4 o[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {  // (behind the last row: the last row again)
+            const int e = min(e0 + i * 128 * Sh::S_GROUPS, n_rows * words - 1);
+            row[i] = e / words, col[i] = 4 * (e - row[i] * words), o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
           }
-          *reinterpret_cast<float4*>(base + col + (t * stride + (r - t * g) * head_pitch)) = o;
+#pragma unroll 1
+          for (int c0 = 0; c0 < n; c0 += 4) {
+            float4 v[4][4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const float* part = p.part + (size_t)attn_slot(share.first + min(c0 + c, n - 1), share) * 128 * HD;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) v[c][i] = __ldcg(reinterpret_cast<const float4*>(part + row[i] * HD + col[i]));
+            }
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float w = c0 + c < n ? s_w[(c0 + c) * 128 + row[i]] : 0.f;
+                if (w != 0.f) o[i].x += w * v[c][i].x, o[i].y += w * v[c][i].y, o[i].z += w * v[c][i].z, o[i].w += w * v[c][i].w;
+              }
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int t = attn_row_token(p, row[i]);
+            if (e0 + i * 128 * Sh::S_GROUPS < n_rows * words) *reinterpret_cast<float4*>(base + col[i] + (t * stride + (row[i] - t * g) * head_pitch)) = o[i];
+          }
         }
         asm volatile("bar.sync 1, %0;" ::"n"(128 * Sh::S_GROUPS) : "memory");
       }
@@ -681,7 +699,7 @@ cudaError_t run_tiles(infr_cuda_ctx* ctx, const CUtensorMap& km, const CUtensorM
   using Sh = TilesShape<HD>;
   const cudaError_t e = ensure_smem(reinterpret_cast<const void*>(&k_attn_tiles<HD>), Sh::SMEM);
   if (e != cudaSuccess) return e;
-  return launch_ex(k_attn_tiles<HD>, dim3(ctx->sm_count < ATTN_MAX_CTAS ? ctx->sm_count : ATTN_MAX_CTAS), dim3(Sh::THREADS), Sh::SMEM, ctx->stream, true, km, vm, p, granule);
+  return launch_ex(k_attn_tiles<HD>, dim3(ctx->sm_count < JOIN_PARTS ? ctx->sm_count : JOIN_PARTS), dim3(Sh::THREADS), Sh::SMEM, ctx->stream, true, km, vm, p, granule);
 }
 
 }  // namespace

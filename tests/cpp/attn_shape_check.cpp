@@ -1,5 +1,5 @@
 // The line of units of an attention call (attn_shape.h), walked by every CTA as the kernels walk it.
-//   line  tb log2_tile window n_kv ctas cap packed rows extra  n_seq  cu_q[n_seq + 1]  kv_len[n_seq]    prints "tiles items joined bad" or what is wrong
+//   line  tb log2_tile window n_kv ctas cap packed rows extra join  n_seq  cu_q[n_seq + 1]  kv_len[n_seq]    prints "tiles items joined bad" or what is wrong
 //   meet  a wide_a stride_a b wide_b stride_b rows                                     prints 0 or 1
 //   sizes rows n_seq n_head n_kv head_dim n_pages page_size max_pages paged            prints "ok", "invalid: ..." or "unsupported: ..."
 #include <cstdio>
@@ -16,9 +16,9 @@ using namespace infr;
 static int line(int argc, char** argv) {
   std::vector<long long> v;
   for (int i = 2; i < argc; ++i) v.push_back(std::atoll(argv[i]));
-  const int tb = (int)v[0], log2_tile = (int)v[1], window = (int)v[2], n_kv = (int)v[3], grid = (int)v[4], cap = (int)v[5], rows = (int)v[7], extra = (int)v[8], n_seq = (int)v[9];
+  const int tb = (int)v[0], log2_tile = (int)v[1], window = (int)v[2], n_kv = (int)v[3], grid = (int)v[4], cap = (int)v[5], rows = (int)v[7], extra = (int)v[8], join = (int)v[9], n_seq = (int)v[10];
   const bool packed = v[6] != 0;
-  const long long *cu = v.data() + 10, *kv = cu + n_seq + 1;
+  const long long *cu = v.data() + 11, *kv = cu + n_seq + 1;
   struct Item {
     int s, b, head;
     AttnBlock blk;
@@ -47,7 +47,9 @@ static int line(int argc, char** argv) {
         tiles += k.ntile;
       }
   }
-  const int C = (int)(units < grid ? units : grid);
+  int most = 0;
+  for (const Item& i : items) most = i.blk.ntile + extra > most ? i.blk.ntile + extra : most;
+  const int C = attn_ctas(units, grid, most, join);
   const AttnLine l = {C ? units / C : 0, C ? (int)(units % C) : 0};
   for (long long a : {units, 7 * units + 3, units / 3, (1ll << 45) + units})
     for (long long b : {units + 1, units / 2 + 5, (1ll << 30) + 3})

@@ -17,8 +17,8 @@ def exe(tmp_path_factory):
     return exe
 
 
-def line(exe, tb, log2_tile, window, n_kv, ctas, cap, packed, rows, cu, kv, extra=1):
-    args = [exe, "line", tb, log2_tile, window, n_kv, ctas, cap, int(packed), rows, extra, len(kv), *cu, *kv]
+def line(exe, tb, log2_tile, window, n_kv, ctas, cap, packed, rows, cu, kv, extra=1, join=0):
+    args = [exe, "line", tb, log2_tile, window, n_kv, ctas, cap, int(packed), rows, extra, join, len(kv), *cu, *kv]
     r = subprocess.run([str(a) for a in args], capture_output=True, text=True)
     assert r.returncode == 0, (r.stdout, args)
     return [int(x) for x in r.stdout.split()]
@@ -52,6 +52,14 @@ def test_batches(exe, seed):
     units, items, joined, bad = line(exe, r.choice([1, 2, 5, 16, 128]), r.choice([6, 7]), r.choice([0, 0, 1, 60, 1000]), r.choice([1, 3, 8]),
                                      r.choice([1, 7, 148]), 4096, packed, cu[-1] + r.choice([0, 3]), cu, kv, r.choice([0, 1, 2, 5]))
     assert bad == 0 and units >= items
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_fewer_ctas_where_joins_cost(exe, seed):
+    r = random.Random(seed + 50)
+    q, kv = [r.randint(1, 200), r.choice([0, 3])], [r.randint(200, 40000), 7]
+    args = (r.choice([1, 5, 128]), 7, 0, r.choice([1, 3]), 148, 65536, False, sum(q), [0, q[0], sum(q)], kv, 3)
+    assert line(exe, *args, join=r.choice([2, 4, 100]))[:2] == line(exe, *args, join=0)[:2]  # the same work, by fewer
 
 
 @pytest.mark.parametrize("cu,kv", [([0, 5, 3, 9], [5, 5, 5]), ([-3, 2, 4, 8], [9, 9, 9]), ([0, 100, 200, 300], [400, 400, 400]), ([0, 2, 4, 6], [2, -7, 10 ** 6]),

@@ -295,6 +295,13 @@ def test_many_sequences(backend):
     check(backend, Batch([r.choice([0, 1, 3, 9]) for _ in range(700)], [0] * 700, 4, 2, 64, seed=12))
 
 
+@pytest.mark.parametrize("kv,hd,n,H", [(2000, 64, 9, 12), (140_000, 64, 9, 12), (7000, 128, 3, 40), (30_000, 128, 32, 4), (70_000, 192, 2, 20), (20_000, 256, 20, 6), (70_000, 16, 128, 1)])
+def test_an_item_in_many_parts(backend, kv, hd, n, H):
+    # one item, or two: its parts go up to as many as CTAs pay for, and past 32 for the longest caches
+    check(backend, Batch([n], [kv], H, 1, hd, page=64, seed=hd + n), path=2)
+    check(backend, Batch([n, 2], [kv, 300], H, 1, hd, page=64, seed=hd + n + 1), path=2)
+
+
 @pytest.mark.parametrize("H,K", [(32, 1), (128, 1), (40, 2)])
 def test_many_heads_to_a_kv_head(backend, H, K):
     check(backend, Batch([1, 3, 1], [300, 1000, 5], H, K, 64, page=16, seed=H))
