@@ -14,8 +14,8 @@
 // S and P of two tiles, and the sums of two (one for heads wider than 64), fill tensor memory: while a tile's weights are made the
 // tensor cores work on the next tile's scores and the last one's sums.
 //
-// Measured (us; the tensor cores' floor at 2 x 4 hd operations a pair and the measured 1666 TFLOP/s): 8192 tokens of 32 / 4 heads of 128 1046 (660),
-// four chunks of 512 tokens over up to 16000 keys 576 (366), 8192 tokens in 16 sequences of 64 / 8 heads of 64 235 (51).  What bounds it is
+// Measured (us; the tensor cores' floor at 2 x 4 hd operations a pair and the measured 1666 TFLOP/s): 8192 tokens of 32 / 4 heads of 128 1036 (660),
+// four chunks of 512 tokens over up to 16000 keys 576 (366), 8192 tokens in 16 sequences of 64 / 8 heads of 64 225 (51).  What bounds it is
 // the weights: 3.0 thousand cycles a tile of 128 keys (maxima 0.6, powers of two and pieces 1.7, the rest waits), against 2.1 - 2.3 of MMAs.  Short
 // sequences of narrow heads pay per item: q into pieces 3 - 4 thousand cycles, results out 4 - 5, masked tiles on the diagonal.
 // Loops are kept rolled, and waits short: the roles share one instruction cache, and with every tile's code straight-line it hit 60% of
