@@ -1202,7 +1202,7 @@ int32_t infr_cuda_attention(infr_cuda_ctx* ctx, const infr_cuda_attention_desc* 
   for (int i = 4; i < 31; ++i)
     if (d->page_size == (1u << i)) p.page_shift = i;
   const uint64_t max_rows = (uint64_t)(d->max_q && d->max_q < d->rows ? d->max_q : d->rows) * g;
-  const bool few = d->path ? d->path == 1 : max_rows <= (uint64_t)ATTN_ROWS_LIMIT;
+  const bool few = d->path ? d->path == 1 : attn_few_rows(max_rows, g, (uint64_t)d->n_seq * d->n_kv);
   // two partial results of 128 rows of 256 values for each CTA, their maxima and weights behind them
   const size_t part = align_up(2 * (size_t)ctx->sm_count * ATTN_TILE_ROWS * 256 * 4, 256);
   if (!ctx->attn_parts) {

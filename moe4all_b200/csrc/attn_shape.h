@@ -91,6 +91,14 @@ INFR_ATTN_HD int attn_ctas(long long units, int grid, int most, int join) {
   return (int)(units < 1 ? 0 : n < 1 ? 1 : n < grid ? n : grid);
 }
 
+// Whether the few-rows kernel serves a call of up to max_rows rows (tokens x g heads) to a (sequence, kv head), of which there are `pairs`.  Its
+// time grows with the rows past eight, the tile kernel's does not; but that one's ends are longer, which counts while every pair has many CTAs.
+// Measured (us, few-rows / tile kernel, heads of 128): 32 rows, 4 pairs of 16000 keys 28.9 / 40.7, 8 of 8000 29.3 / 35.7, 16 of 8000 43.2 / 39.0;
+// 16 rows, 16 pairs 31.3 / 33.4, 32 49.2 / 44.7 (heads of 64: 30.8 / 34.9; of 1000 keys 20.3 / 21.8), 128 of 4000 79.3 / 69.6; 8 rows, 128 56.8 / 65.3.
+inline bool attn_few_rows(uint64_t max_rows, uint32_t g, uint64_t pairs) {
+  return g <= (uint32_t)ATTN_ROWS_LIMIT && max_rows <= (pairs <= 8 ? 32u : pairs <= 32 ? 16u : 8u);
+}
+
 // What a call gives, as numbers.
 struct AttnSizes {
   uint32_t rows, n_seq, n_head, n_kv, head_dim;

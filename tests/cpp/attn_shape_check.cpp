@@ -1,6 +1,7 @@
 // The line of units of an attention call (attn_shape.h), walked by every CTA as the kernels walk it.
 //   line  tb log2_tile window n_kv ctas cap packed rows extra join  n_seq  cu_q[n_seq + 1]  kv_len[n_seq]    prints "tiles items joined bad" or what is wrong
 //   meet  a wide_a stride_a b wide_b stride_b rows                                     prints 0 or 1
+//   few   max_rows g pairs                                                             prints 0 or 1
 //   sizes rows n_seq n_head n_kv head_dim n_pages page_size max_pages paged            prints "ok", "invalid: ..." or "unsupported: ..."
 #include <cstdio>
 #include <cstdlib>
@@ -98,6 +99,7 @@ int main(int argc, char** argv) {
     for (int i = 0; i < 7; ++i) x[i] = std::strtoull(argv[i + 2], nullptr, 10);
     return std::printf("%d\n", attn_rows_meet(x[0], x[1], x[2], x[3], x[4], x[5], x[6])), 0;
   }
+  if (argc == 5 && !std::strcmp(argv[1], "few")) return std::printf("%d\n", attn_few_rows(std::strtoull(argv[2], nullptr, 10), (uint32_t)std::atoi(argv[3]), std::strtoull(argv[4], nullptr, 10))), 0;
   if (argc != 11) return 2;
   uint32_t v[9];
   for (int i = 0; i < 9; ++i) v[i] = (uint32_t)std::strtoul(argv[i + 2], nullptr, 10);

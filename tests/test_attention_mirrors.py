@@ -37,7 +37,7 @@ def test_descriptors_have_the_same_fields_everywhere(tmp_path, name, cls):
     assert got == [getattr(mirror, n).offset for n, _ in mirror._fields_] + [C.sizeof(mirror)]
 
 
-def build_checker(tmp_path):
+def build_host(tmp_path):
     from moe4all_b200 import build
 
     lib = build.build()
@@ -49,12 +49,12 @@ def build_checker(tmp_path):
 
 
 def test_cpp_mirror_compiles_and_links(tmp_path):
-    assert os.path.exists(build_checker(tmp_path))
+    assert os.path.exists(build_host(tmp_path))
 
 
 @pytest.mark.gpu
 def test_cpp_mirror_against_the_formula(tmp_path):
-    exe = build_checker(tmp_path)
+    exe = build_host(tmp_path)
     H, K, hd, cu = 4, 2, 64, [0, 13, 40]
     rows = cu[-1]
     rng = np.random.default_rng(3)

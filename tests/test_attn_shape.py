@@ -106,3 +106,9 @@ def test_rows_that_share_bytes(exe, seed):
     meet = lambda *x: subprocess.run([exe, "meet"] + [str(i) for i in x], capture_output=True, text=True).stdout == "1\n"
     assert not meet(0, 32, 48, 32, 8, 48, 100) and not meet(0, 32, 48, 40, 8, 48, 100) and meet(0, 32, 48, 28, 8, 48, 100)
     assert meet(0, 32, 48, 32, 8, 44, 100) and not meet(0, 32, 48, 99 * 48 + 32, 8, 44, 100)
+
+
+@pytest.mark.parametrize("rows,g,pairs,want", [(8, 8, 10 ** 6, 1), (9, 9, 33, 0), (16, 16, 32, 1), (17, 1, 32, 0), (32, 16, 8, 1), (33, 1, 1, 0), (17, 17, 1, 0), (1, 1, 0, 1), (2 ** 40, 4, 1, 0)])
+def test_which_kernel(exe, rows, g, pairs, want):
+    r = subprocess.run([exe, "few", str(rows), str(g), str(pairs)], capture_output=True, text=True)
+    assert r.stdout == f"{want}\n"

@@ -12,7 +12,7 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 SRC = os.path.join(ROOT, "tests", "cpp", "host_mirror_check.cpp")
 
 
-def build_checker(tmp_path):
+def build_host(tmp_path):
     from moe4all_b200 import build
     lib = build.build()
     libdir = os.path.dirname(lib)
@@ -25,7 +25,7 @@ def build_checker(tmp_path):
 
 
 def test_cpp_mirror_compiles_and_links(tmp_path):
-    exe = build_checker(tmp_path)
+    exe = build_host(tmp_path)
     assert os.path.exists(exe)
 
 
@@ -35,7 +35,7 @@ def test_cpp_mirror_layer_matches_oracle(tmp_path, rows):
     from moe4all_b200 import synth
     from helpers import assert_close, near_tie_rows, oracle_layer
 
-    exe = build_checker(tmp_path)
+    exe = build_host(tmp_path)
     ne, E, k, nff = 512, 16, 4, 256
     L = synth.make_layer(41, ne, E, nff, sh_ff=nff, router_std=0.05)
     x = synth.activations(5 + rows, rows, ne)
