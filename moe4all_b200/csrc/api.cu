@@ -1054,11 +1054,6 @@ AttnSizes attn_sizes(const Desc* d) {
   return {d->rows, d->n_seq, d->n_head, d->n_kv, d->head_dim, d->n_pages, d->page_size, d->max_pages, d->page_table != nullptr};
 }
 
-// Bytes of the cache that a call's rows or pages take.
-uint64_t attn_cache_bytes(const AttnSizes& s) {
-  return (s.paged ? (uint64_t)s.n_pages * s.page_size : (uint64_t)s.rows) * s.n_kv * s.head_dim * 2;
-}
-
 // What both calls check of a batch and its cache.
 template <class Desc>
 int32_t attn_check_batch(infr_cuda_ctx* ctx, const char* op, const Desc* d, const infr_cuda_buf* k, const infr_cuda_buf* v) {

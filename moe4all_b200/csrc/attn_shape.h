@@ -125,6 +125,12 @@ inline const char* attn_sizes_error(const AttnSizes& s, bool* unsupported) {
   return nullptr;
 }
 
+// Bytes of the cache that a call's pages or rows take; all ones where that is past 64 bits (accepted sizes go to 2^80).
+inline uint64_t attn_cache_bytes(const AttnSizes& s) {
+  const uint64_t tokens = s.paged ? (uint64_t)s.n_pages * s.page_size : s.rows, each = (uint64_t)s.n_kv * s.head_dim * 2;
+  return tokens > ~0ull / each ? ~0ull : tokens * each;
+}
+
 // Values a buffer needs for `rows` rows of `wide` values that are `stride` apart.
 inline uint64_t attn_span(uint64_t rows, uint64_t stride, uint64_t wide) { return rows ? (rows - 1) * stride + wide : 0; }
 

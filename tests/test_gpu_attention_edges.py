@@ -1,0 +1,22 @@
+"""GPU: rope_kv and attention at the ends of what their arguments may be, against the formulas in 64 bits (tolerances as in
+test_gpu_attention.py unless a test derives its own)."""
+import dataclasses
+
+import pytest
+
+from test_gpu_attention import Batch, Rope
+
+pytestmark = pytest.mark.gpu
+
+
+def test_caches_past_64_bits_are_refused(backend):
+    # pages x tokens x heads x values x 2 bytes are 2^69, 2^65 and 2^68: nothing in 64 bits
+    from moe4all_b200 import BackendError
+
+    b = Batch([1], [20], 16, 16, 16, page=16, seed=1)
+    r = Rope(b, 16, False, norm=False, factors=False, fused=False)
+    for kw in (dict(n_pages=1 << 30, page_size=1 << 30), dict(n_pages=1 << 30, page_size=1 << 30, n_head=1, n_kv=1), dict(n_pages=1 << 29, page_size=1 << 30)):
+        for call, op in ((backend.attention, b.op(backend, max_pages=1)), (backend.rope_kv, r.op(backend, max_pages=1))):
+            with pytest.raises(BackendError, match="cache buffer"):
+                call(dataclasses.replace(op, **kw))
+    backend.sync()
