@@ -160,11 +160,12 @@ __device__ __forceinline__ void attn_plan(const AttnParams& p, int* known, long 
       n = attn_blocks(seqs[s].q_len, p.tb);
     }
     const long long sum = carry + block_scan<THREADS>(n, s_warp);
-    if (s < p.n_seq) pre[s + 1] = (int)sum;
+    if (s < p.n_seq) pre[s + 1] = attn_blocks_on(sum, p.rows);
     __syncthreads();
     carry = pre[min(s0 + THREADS, p.n_seq)];
   }
-  const int F = (int)carry, per = (F + THREADS - 1) / THREADS, f0 = min(tid * per, F), f1 = min(f0 + per, F);
+  const int F = carry > p.rows ? 0 : (int)carry;  // (reported: some sequence ends ahead of its beginning)
+  const int per = (F + THREADS - 1) / THREADS, f0 = min(tid * per, F), f1 = min(f0 + per, F);
   int s = 0;
 #pragma unroll 1
   for (int hi = p.n_seq; hi - s > 1;) {  // the last sequence that begins at or before block f0

@@ -50,6 +50,10 @@ INFR_ATTN_HD AttnSeq attn_seq(int a, int b, int kv, bool packed, int rows, int c
 
 INFR_ATTN_HD int attn_blocks(int q_len, int tb) { return (q_len + tb - 1) / tb; }
 
+// Blocks counted on by a sequence's.  Those of sequences that lie one after the other are at most the call's rows; cu_q out of order can make
+// n_seq x rows of them, past 31 bits: counted as rows + 1, and such a call is served as one without rows.
+INFR_ATTN_HD int attn_blocks_on(long long sum, int rows) { return sum > rows ? rows + 1 : (int)sum; }
+
 INFR_ATTN_HD AttnBlock attn_block(const AttnSeq& s, int b, int tb, int log2_tile, int window) {
   AttnBlock r;
   r.t0 = b * tb;

@@ -1,5 +1,6 @@
 // The far ends of what an attention call may be given (attn_shape.h).
 //   bytes rows n_seq n_head n_kv head_dim n_pages page_size max_pages paged     prints "ok" or what is refused, and the cache's bytes
+//   blocks tb rows n_seq                                     blocks counted where cu_q is 0, rows, 0, rows, ...: their number, or rows + 1; 1 where found bad
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
@@ -16,6 +17,16 @@ int main(int argc, char** argv) {
     bool unsupported = false;
     const char* why = attn_sizes_error(s, &unsupported);
     return std::printf("%s %llu\n", why ? "refused" : "ok", why ? 0ull : (unsigned long long)attn_cache_bytes(s)), 0;
+  }
+  if (argc == 5 && !std::strcmp(argv[1], "blocks")) {
+    const int tb = std::atoi(argv[2]), rows = std::atoi(argv[3]), n_seq = std::atoi(argv[4]);
+    long long carry = 0;
+    bool bad = false;
+    for (int s = 0; s < n_seq; ++s) {
+      carry = attn_blocks_on(carry + attn_blocks(attn_seq(s % 2 ? rows : 0, s % 2 ? 0 : rows, 0, true, rows, 0, &bad).q_len, tb), rows);
+      if (carry < 0 || carry > (long long)rows + 1) return std::puts("lost count"), 1;
+    }
+    return std::printf("%lld %d\n", carry, (int)bad), 0;
   }
   return 2;
 }

@@ -24,3 +24,10 @@ def test_bytes_of_a_cache(ask, pages, page, heads, hd):
 
 def test_bytes_of_packed_rows(ask):
     assert ask("bytes", 1 << 22, 1, 1024, 1024, 256, 0, 0, 0, 0) == ["ok", str((1 << 22) * 1024 * 256 * 2)]
+
+
+@pytest.mark.parametrize("tb,rows,n_seq", [(1, 1 << 22, 4096), (1, 1 << 22, 1025), (2, 1 << 22, 4096), (16, 64, 600), (128, 64, 600), (1, 1, 4096), (1, 5, 2), (4, 9, 1)])
+def test_blocks_of_sequences_out_of_order(ask, tb, rows, n_seq):
+    # every second sequence has all of the rows: 2^33 of them at most
+    blocks = (n_seq + 1) // 2 * -(-rows // tb)
+    assert ask("blocks", tb, rows, n_seq) == [str(min(blocks, rows + 1)), str(int(n_seq > 1))]

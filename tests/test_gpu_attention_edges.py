@@ -4,7 +4,7 @@ import dataclasses
 
 import pytest
 
-from test_gpu_attention import Batch, Rope
+from test_gpu_attention import Batch, Rope, check
 
 pytestmark = pytest.mark.gpu
 
@@ -20,3 +20,22 @@ def test_caches_past_64_bits_are_refused(backend):
             with pytest.raises(BackendError, match="cache buffer"):
                 call(dataclasses.replace(op, **kw))
     backend.sync()
+
+
+@pytest.mark.parametrize("path", [1, 2])
+def test_sequences_out_of_order_are_reported(backend, path):
+    # every second of 4096 sequences has all 64 rows of the call
+    from moe4all_b200 import BackendError
+    import torch
+
+    b = Batch([1] * 64 + [0] * 4032, [0] * 4096, 8, 2, 64, seed=2)
+    r = Rope(b, 64, False, norm=False, factors=False, fused=False)
+    b.cu_t.copy_(torch.tensor([0, 64] * 2048 + [0], dtype=torch.int32))
+    torch.cuda.synchronize()
+    for call, op in ((backend.attention, b.op(backend, path=path)), (backend.rope_kv, r.op(backend))):
+        call(op)
+        with pytest.raises(BackendError, match="attention kernel"):
+            backend.sync()
+    b.cu_t.copy_(torch.tensor(b.cu, dtype=torch.int32))
+    b = Batch([1, 5, 0, 58], [0] * 4, 8, 2, 64, seed=3)
+    check(backend, b, path=path)
