@@ -1190,7 +1190,7 @@ int32_t infr_cuda_attention(infr_cuda_ctx* ctx, const infr_cuda_attention_desc* 
   p.v = static_cast<const __half*>(d->v->ptr);
   p.g = (int)g;
   p.g_inv = (65536 + g - 1) / g;
-  p.window = (int)d->window;
+  p.window = attn_window(d->window, p.kv_len != nullptr ? (uint32_t)p.cap : d->rows);
   p.scale_log2 = (float)((double)d->scale * 1.4426950408889634);
   p.count = ctx->attn_count;
   p.page_shift = -1;

@@ -221,12 +221,6 @@ __device__ __forceinline__ void attn_plan(const AttnParams& p, int* known, long 
   __syncthreads();
 }
 
-// Keys below full_hi and from full_lo on are seen by every row of the item.
-__device__ __forceinline__ int attn_full_hi(const AttnSeq& seq, const AttnBlock& blk) { return seq.past + blk.t0 + 1; }
-__device__ __forceinline__ int attn_full_lo(const AttnParams& p, const AttnSeq& seq, const AttnBlock& blk) {
-  return p.window > 0 ? seq.past + blk.t0 + blk.nt - p.window : 0;
-}
-
 // One item after the other from the one that a CTA's share begins in.
 template <int LOG2_TILE, int EXTRA>
 struct AttnCursor {
@@ -269,7 +263,7 @@ struct AttnCursor {
 // key0 .. key1: the keys of this part; full_lo .. full_hi: tiles inside have no hidden keys; to: the row's last key.
 static __device__ __noinline__ void attn_odd_values(const AttnParams& p, int s, int q0, int head, int key0, int key1, int tile, int full_lo, int full_hi, int to,
                                                     int col0, int cols, float* dst) {
-  const int from = p.window > 0 ? to - p.window : -1;
+  const int from = attn_first_key(to, p.window);
   const int n = min(cols, p.hd - col0);
   bool came_finite = true;
 #pragma unroll 1
@@ -279,7 +273,7 @@ static __device__ __noinline__ void attn_odd_values(const AttnParams& p, int s, 
   for (int ks = key0; ks < key1; ks += tile) {
     if (came_finite && ks + tile <= full_hi && ks >= full_lo) continue;
 #pragma unroll 1
-    for (int key = max(ks, from + 1); key < ks + tile && key <= to; ++key) {
+    for (int key = max(ks, from); key < ks + tile && key <= to; ++key) {
       const __half* v = attn_value(p, s, q0, head, key) + col0;
 #pragma unroll 1
       for (int i = 0; i < n; i += 8) {

@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
         f[n][j] = s_factor[rr];
         lim[n][j] = cur.seq.past + blk.t0 + (rr < n_rows ? attn_row_token(p, rr) : blk.nt - 1);
       }
-    const int full_hi = attn_full_hi(cur.seq, blk), full_lo = attn_full_lo(p, cur.seq, blk);
+    const int full_hi = attn_full_hi(cur.seq, blk), full_lo = attn_full_lo(cur.seq, blk, p.window);
 
     float o[KST][NT][4], m[NT][2], l[NT][2];
 #pragma unroll
@@ -251,9 +251,9 @@ __global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
             s[n][j] *= f[n][j];
             s[n][2 + j] *= f[n][j];
             if (masked) {
-              const int to = lim[n][j], from = p.window > 0 ? to - p.window : -1;
-              if (key > to || key <= from) s[n][j] = -CUDART_INF_F;
-              if (key + 8 > to || key + 8 <= from) s[n][2 + j] = -CUDART_INF_F;
+              const int to = lim[n][j], from = attn_first_key(to, p.window);
+              if (key > to || key < from) s[n][j] = -CUDART_INF_F;
+              if (key + 8 > to || key + 8 < from) s[n][2 + j] = -CUDART_INF_F;
             }
             grows |= fmaxf(s[n][j], s[n][2 + j]) > m[n][j] + ATTN_SLACK;
           }

@@ -54,18 +54,28 @@ INFR_ATTN_HD int attn_blocks(int q_len, int tb) { return (q_len + tb - 1) / tb; 
 // n_seq x rows of them, past 31 bits: counted as rows + 1, and such a call is served as one without rows.
 INFR_ATTN_HD int attn_blocks_on(long long sum, int rows) { return sum > rows ? rows + 1 : (int)sum; }
 
+// The window as the kernels get it: 0 where it leaves nothing out of `most` tokens, so that it always stays below them.
+INFR_ATTN_HD int attn_window(uint32_t window, uint32_t most) { return window < most ? (int)window : 0; }
+// The first key that a row at this position sees: by comparison ahead of any difference, since rows with negative positions (as far as -2^22) and
+// windows near 2^31 have none in 32 bits.  (Rows that see nothing get 0.)
+INFR_ATTN_HD int attn_first_key(int position, int window) { return window > 0 && position >= window ? position - window + 1 : 0; }
+
 INFR_ATTN_HD AttnBlock attn_block(const AttnSeq& s, int b, int tb, int log2_tile, int window) {
   AttnBlock r;
   r.t0 = b * tb;
   r.nt = s.q_len - r.t0 < tb ? s.q_len - r.t0 : tb;
-  const int last = s.past + r.t0 + r.nt, first = s.past + r.t0 - window + 1;
+  const int last = s.past + r.t0 + r.nt;
   r.hi = last > 0 ? last : 0;
-  r.lo = window > 0 && first > 0 ? first : 0;
+  r.lo = attn_first_key(s.past + r.t0, window);
   r.tile0 = r.lo >> log2_tile;
   const int end = (r.hi + (1 << log2_tile) - 1) >> log2_tile;
   r.ntile = end > r.tile0 ? end - r.tile0 : 1;
   return r;
 }
+
+// Keys from the first number and below the second are seen by every row of the block.
+INFR_ATTN_HD int attn_full_lo(const AttnSeq& s, const AttnBlock& b, int window) { return attn_first_key(s.past + b.t0 + b.nt - 1, window); }
+INFR_ATTN_HD int attn_full_hi(const AttnSeq& s, const AttnBlock& b) { return s.past + b.t0 + 1; }
 
 // a / b for quotients below 2^20: an estimate in f32 is off by one at most (64-bit divisions are a hundred instructions each).
 INFR_ATTN_HD int attn_small_div(long long a, long long b) {

@@ -90,9 +90,9 @@ struct TileBars {
 // Whether some row of the item does not see some key of [ks, ks + n).
 __device__ __forceinline__ bool tile_masked(const TileItem& it, int ks, int n) { return ks + n > it.full_hi || ks < it.full_lo; }
 
-// Bit i: whether the key k0 + i is in (from, to].
+// Bit i: whether the key k0 + i is one of from .. to.
 __device__ __forceinline__ uint32_t seen_keys(int k0, int from, int to) {
-  const int lo = max(0, from + 1 - k0), n = min(32, to + 1 - k0);  // bits lo .. n - 1
+  const int lo = max(0, from - k0), n = min(32, to + 1 - k0);  // bits lo .. n - 1
   return n <= lo ? 0u : (~0u >> (32 - (n - lo))) << lo;
 }
 
@@ -174,7 +174,7 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
           it.n0 = n, it.n1 = n + t_end - t;
           it.row0 = c.seq.q0 + c.blk.t0, it.n_rows = c.blk.nt * p.g;
           it.key0 = (c.blk.tile0 + t) << Sh::LOG2_TILE, it.lo = c.blk.lo, it.hi = c.blk.hi, it.pos0 = c.seq.past + c.blk.t0;
-          it.full_lo = attn_full_lo(p, c.seq, c.blk), it.full_hi = attn_full_hi(c.seq, c.blk), it.head = c.head, it.s = c.s;
+          it.full_lo = attn_full_lo(c.seq, c.blk, p.window), it.full_hi = attn_full_hi(c.seq, c.blk), it.head = c.head, it.s = c.s;
           it.q0 = c.seq.q0, it.whole = sh.first == sh.last, it.first_cta = sh.first, it.last_cta = sh.last;
           mbar_arrive(bars.i_full + item % ITEMS);
         }
@@ -438,8 +438,8 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
       ok = ok && wait_all(bars.f_full + (item & (RING - 1)), item / RING);
       if (!ok) break;
       const float f = s_fac[(item & (RING - 1)) * 128 + row];
-      const int to = it.pos0 + (row < n_rows ? attn_row_token(p, row) : 0);  // the row sees the keys (from, to]
-      const int from = p.window > 0 ? to - p.window : -1;
+      const int to = it.pos0 + (row < n_rows ? attn_row_token(p, row) : 0);  // the row sees the keys from .. to
+      const int from = attn_first_key(to, p.window);
       const bool busy = (warp & 3) * 32 < n_rows;  // (other rows' weights are whatever is there: they reach those rows' sums only)
       float m = -CUDART_INF_F, l = 0.f;
       int ks = it.key0 + 64 * wg;

@@ -31,3 +31,10 @@ def test_blocks_of_sequences_out_of_order(ask, tb, rows, n_seq):
     # every second sequence has all of the rows: 2^33 of them at most
     blocks = (n_seq + 1) // 2 * -(-rows // tb)
     assert ask("blocks", tb, rows, n_seq) == [str(min(blocks, rows + 1)), str(int(n_seq > 1))]
+
+
+@pytest.mark.parametrize("past,q_len,most", [(-4, 10, 64), (-5, 16, 64), (-150, 200, 640), (-(1 << 22), (1 << 22) + 0, 16), (0, 300, 300), (1000, 5, 4096), (0x7FFF0000 - 200, 200, 0x7FFF0000)])
+@pytest.mark.parametrize("window", [0, 1, 3, 200, 0x7FFEFFFF, 0x7FFF0000, 2 ** 31 - 5, 2 ** 31 - 1])
+def test_windows_and_negative_positions(ask, past, q_len, most, window):
+    for tb, log2_tile in ((16, 7), (128, 6)) if q_len < 1000 else ((128, 7),):
+        assert ask("window", past, q_len, tb, log2_tile, window, most) == ["ok"]

@@ -39,3 +39,14 @@ def test_sequences_out_of_order_are_reported(backend, path):
     b.cu_t.copy_(torch.tensor(b.cu, dtype=torch.int32))
     b = Batch([1, 5, 0, 58], [0] * 4, 8, 2, 64, seed=3)
     check(backend, b, path=path)
+
+
+@pytest.mark.parametrize("path", [1, 2])
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 4, 640, 639, 3])
+def test_widest_windows_where_rows_in_front_see_nothing(backend, path, window):
+    # fewer tokens in the cache than new rows, and every window that hides nothing, or next to nothing
+    b = Batch([10, 16, 200], [-4, -5, -150], 8, 2, 64, page=16, seed=4)
+    want = check(backend, b, window=window, path=path)
+    assert bool((want[:4] == 0).all()) and bool((want[4:10] != 0).any(1).all())
+    check(backend, Batch([1, 40, 7], [600, 20, 0], 8, 2, 64, page=16, seed=5), window=window, path=path)
+    check(backend, Batch([30, 1, 200], [0, 0, 0], 8, 2, 64, seed=6), window=window, path=path)
