@@ -15,6 +15,7 @@ Every op goes through the C ABI; the whole step can be recorded once and replaye
 (`Backend::compile` + decode replay)."""
 from __future__ import annotations
 
+import weakref
 from dataclasses import dataclass, field
 from typing import List, Optional
 
@@ -39,7 +40,10 @@ class AttnWeights:
 class StackAttention:
     """The attention of a `MoeStack` over pages that all of its layers address alike: sequence s has kv_len[s] tokens with the step's new
     ones, which are the stack's rows cu_q[s] .. cu_q[s + 1] - 1.  The three arrays are i32 tensors on the device, read when a step runs: a
-    recorded step follows new lengths and pages written into them.  `caches[l]` are layer l's (k, v), f16 [n_pages, n_kv, page_size, head_dim]."""
+    recorded step follows new lengths and pages written into them.  `caches[l]` are layer l's (k, v), f16 [n_pages, n_kv, page_size, head_dim].
+
+    Several stacks may have the same one (a stack of prompt chunks and one of single tokens over the same caches): weights, caches and arrays are
+    shared, the rows between the ops are each stack's own."""
     layers: List[AttnWeights]
     n_head: int
     n_kv: int
@@ -54,32 +58,50 @@ class StackAttention:
     rope_base: float = 1e4
     n_rot: Optional[int] = None  # whole heads unless given
     interleaved: bool = False
-    _ops: list = field(default_factory=list, repr=False)
+    _bound: weakref.WeakSet = field(default_factory=weakref.WeakSet, init=False, repr=False, compare=False)
 
-    def bind(self, be: CudaBackend, rows: int, ne: int, eps: float, hidden: Buffer, device) -> None:
-        """Rows between the ops, and the ops over them."""
-        H, K, hd = self.n_head, self.n_kv, self.head_dim
+    def bind(self, be: CudaBackend, rows: int, ne: int, eps: float, hidden: Buffer, device) -> "BoundAttention":
+        """These layers on a stack's rows: the ops, and buffers of the stack's own between them."""
+        bound = BoundAttention(self, be, rows, ne, eps, hidden, device)
+        self._bound.add(bound)
+        return bound
+
+    def layer(self, li: int) -> None:
+        """One attention sub-layer in place on the `hidden` of the stack that this is bound to, where there is one."""
+        bound = list(self._bound)
+        if len(bound) != 1:
+            raise RuntimeError(f"StackAttention.layer: bound to {len(bound)} stacks: call the stack's attn_layer")
+        bound[0].layer(li)
+
+
+class BoundAttention:
+    """A `StackAttention` on the rows of one stack: buffers between the ops, and the ops over them."""
+
+    def __init__(self, attn: StackAttention, be: CudaBackend, rows: int, ne: int, eps: float, hidden: Buffer, device):
+        H, K, hd = attn.n_head, attn.n_kv, attn.head_dim
         wide, w = (H + 2 * K) * hd, be.wrap_tensor
-        self._be, self._shape, self._hidden = be, (rows, ne, eps, wide, H * hd), hidden
+        self._be, self._layers, self._shape, self._hidden = be, attn.layers, (rows, ne, eps, wide, H * hd), hidden
         self._rows = [torch.zeros(rows, n, device=device) for n in (ne, wide, H * hd, H * hd, ne)]
         self._hn, self._qkv, q, out, self._sub = (w(t) for t in self._rows)
         self._out = out
+        # (the parts of the wide rows: their memory is _rows')
         part = lambda first: be.wrap(self._rows[1].data_ptr() + 4 * first, 4 * (rows * wide - first))
-        n_pages = self.caches[0][0].shape[0]
-        batch = dict(cu_q=w(self.cu_q), kv_len=w(self.kv_len), page_table=w(self.page_table), rows=rows, n_seq=self.kv_len.numel(), n_head=H, n_kv=K,
-                     head_dim=hd, n_pages=n_pages, page_size=self.page_size, max_pages=self.page_table.shape[1])
+        n_pages = attn.caches[0][0].shape[0]
+        batch = dict(cu_q=w(attn.cu_q), kv_len=w(attn.kv_len), page_table=w(attn.page_table), rows=rows, n_seq=attn.kv_len.numel(), n_head=H, n_kv=K,
+                     head_dim=hd, n_pages=n_pages, page_size=attn.page_size, max_pages=attn.page_table.shape[1])
         parts = part(0), part(H * hd), part((H + K) * hd)
-        for L, (k, v) in zip(self.layers, self.caches, strict=True):
+        self._ops = []
+        for L, (k, v) in zip(attn.layers, attn.caches, strict=True):
             opt = lambda t: None if t is None else w(t)
             kc, vc = w(k), w(v)
             self._ops.append((w(L.norm), RopeKv(q=parts[0], k=parts[1], v=parts[2], q_stride=wide, k_stride=wide, v_stride=wide, q_out=q, k_cache=kc, v_cache=vc,
-                                                n_rot=hd if self.n_rot is None else self.n_rot, interleaved=self.interleaved, rope_base=self.rope_base,
+                                                n_rot=hd if attn.n_rot is None else attn.n_rot, interleaved=attn.interleaved, rope_base=attn.rope_base,
                                                 q_norm=opt(L.q_norm), k_norm=opt(L.k_norm), norm_eps=eps, **batch),
-                              Attention(q=q, k=kc, v=vc, out=out, scale=hd ** -0.5, max_q=self.max_q, window=self.window, **batch)))
+                              Attention(q=q, k=kc, v=vc, out=out, scale=hd ** -0.5, max_q=attn.max_q, window=attn.window, **batch)))
 
     def layer(self, li: int) -> None:
         """One attention sub-layer in place on `hidden`."""
-        be, L, (norm, rope, attention) = self._be, self.layers[li], self._ops[li]
+        be, L, (norm, rope, attention) = self._be, self._layers[li], self._ops[li]
         rows, ne, eps, wide, n_out = self._shape
         be.rms_norm(self._hidden, norm, self._hn, rows, ne, eps)
         be.linear(L.dtype, L.wqkv, self._hn, self._qkv, rows, ne, wide)
@@ -120,14 +142,17 @@ class MoeStack:
                                    sh_ff=sh_ff if "sh_gate" in b else 0, **fuse, **route_kw))
         self.plan = None
         self.attn = attn
-        if attn is not None:
-            attn.bind(be, rows, ne, eps, self.b_hidden, dev)
+        self._attn = None if attn is None else attn.bind(be, rows, ne, eps, self.b_hidden, dev)
+
+    def attn_layer(self, li: int) -> None:
+        """The attention sub-layer of one layer in place on `hidden`."""
+        self._attn.layer(li)
 
     def layer(self, li: int) -> None:
         """One layer in place on `hidden`."""
         be = self.be
-        if self.attn is not None:
-            self.attn.layer(li)
+        if self._attn is not None:
+            self._attn.layer(li)
         if self.fused:
             be.moe_ffn(self.ops[li])
             return
