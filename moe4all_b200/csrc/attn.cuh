@@ -256,39 +256,66 @@ struct AttnCursor {
   }
 };
 
-// Some value that this row sees may not be finite: what the products of pieces made of it (inf times a piece of the other sign, or of zero, is
-// NaN), or left out, in columns col0 .. of the result or part at dst, is put right: the sum of such values.  Columns that came out finite
-// can only miss values of tiles with hidden keys, where they count as zeros.  (Key by key, eight columns at a time: other warps of the CTA
-// wait meanwhile, and their waits have a limit.)
-// key0 .. key1: the keys of this part; full_lo .. full_hi: tiles inside have no hidden keys; to: the row's last key.
-static __device__ __noinline__ void attn_odd_values(const AttnParams& p, int s, int q0, int head, int key0, int key1, int tile, int full_lo, int full_hi, int to,
-                                                    int col0, int cols, float* dst) {
-  const int from = attn_first_key(to, p.window);
-  const int n = min(cols, p.hd - col0);
-  bool came_finite = true;
+// Which of an f16 pair's values are +inf or NaN (bits 0 and 1), and -inf or NaN (bits 16 and 17).
+__device__ __forceinline__ uint32_t odd_pair(uint32_t x) {
+  uint32_t r = 0;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t h = x >> (16 * i), big = h & 0x7FFFu;
+    if (big >= 0x7C00u) r |= (big > 0x7C00u ? 0x10001u : h & 0x8000u ? 0x10000u : 1u) << i;
+  }
+  return r;
+}
+
+// Some value that a row of this warp sees may not be finite: what the products of pieces made of it (inf times a piece of the other sign, or of
+// zero, is NaN), or left out, in columns col0 .. of the result or part at dst, is put right: the sum of such values, whatever their weights.
+// Columns that came out finite can only miss values of tiles with hidden keys, where they count as zeros.
+// All lanes take part; those with a row are active: `to` its last key.  Keys by lane, 32 columns at a time, what is found noted in two words: other
+// warps of the CTA wait meanwhile, and their waits have a limit.  (A row's lane by itself took 3 - 50 us a key.)
+// key0 .. key1: the keys of this part; full_lo .. full_hi: tiles inside have no hidden keys.
+static __device__ __forceinline__ void attn_odd_values(const AttnParams& p, int s, int q0, int head, int key0, int key1, int tile, int full_lo, int full_hi, bool active,
+                                                    int to, int col0, int cols, float* dst) {
+  const int lane = threadIdx.x & 31, from = attn_first_key(to, p.window);
+  const int lo = max(key0, __reduce_min_sync(0xFFFFFFFFu, active ? from : 0x7FFFFFFF)), hi = min(key1 - 1, __reduce_max_sync(0xFFFFFFFFu, active ? to : -1));
 #pragma unroll 1
-  for (int i = 0; i < n; ++i) came_finite &= fabsf(__ldcg(dst + i)) < CUDART_INF_F;
-  uint32_t placed[8] = {};  // columns whose result is such a sum by now
+  for (int c = 0; c < cols && col0 + c < p.hd; c += 32) {
+    const int n = min(32, p.hd - col0 - c);
+    bool came_finite = true;
 #pragma unroll 1
-  for (int ks = key0; ks < key1; ks += tile) {
-    if (came_finite && ks + tile <= full_hi && ks >= full_lo) continue;
+    for (int i = 0; i < n && active; ++i) came_finite &= fabsf(__ldcg(dst + c + i)) < CUDART_INF_F;
+    const bool all = __any_sync(0xFFFFFFFFu, !came_finite);
+    uint32_t plus = 0, minus = 0;  // columns: the row sees +inf or NaN there, -inf or NaN
 #pragma unroll 1
-    for (int key = max(ks, from); key < ks + tile && key <= to; ++key) {
-      const __half* v = attn_value(p, s, q0, head, key) + col0;
+    for (int ks = key0; ks < key1; ks += tile) {
+      if (ks > hi || ks + tile <= lo || (!all && ks + tile <= full_hi && ks >= full_lo)) continue;
 #pragma unroll 1
-      for (int i = 0; i < n; i += 8) {
-        const uint4 x = *reinterpret_cast<const uint4*>(v + i);
-        if (only_finite(x.x) == x.x && only_finite(x.y) == x.y && only_finite(x.z) == x.z && only_finite(x.w) == x.w) continue;
+      for (int k0 = ks; k0 < ks + tile; k0 += 32) {
+        const int key = k0 + lane;
+        uint32_t mine_plus = 0, mine_minus = 0;
+        if (key >= lo && key <= hi) {
+          const uint4* v = reinterpret_cast<const uint4*>(attn_value(p, s, q0, head, key) + col0 + c);
 #pragma unroll 1
-        for (int j = i; j < i + 8; ++j) {
-          const float y = __half2float(v[j]);
-          if (fabsf(y) < CUDART_INF_F) continue;
-          const uint32_t bit = 1u << (j & 31);
-          __stcg(dst + j, placed[j >> 5] & bit ? __ldcg(dst + j) + y : y);
-          placed[j >> 5] |= bit;
+          for (int j = 0; 8 * j < n; ++j) {
+            const uint4 x = __ldcg(v + j);  // past L1, as all that an earlier kernel wrote: this one may have started beside it
+            const uint32_t odd = odd_pair(x.x) | odd_pair(x.y) << 2 | odd_pair(x.z) << 4 | odd_pair(x.w) << 6;
+            mine_plus |= (odd & 0xFFu) << (8 * j);
+            mine_minus |= (odd >> 16) << (8 * j);
+          }
+        }
+#pragma unroll 1
+        for (uint32_t found = __ballot_sync(0xFFFFFFFFu, (mine_plus | mine_minus) != 0); found; found &= found - 1) {
+          const int i = __ffs(found) - 1;
+          const uint32_t a = __shfl_sync(0xFFFFFFFFu, mine_plus, i), b = __shfl_sync(0xFFFFFFFFu, mine_minus, i);
+          if (active && k0 + i >= from && k0 + i <= to) plus |= a, minus |= b;
         }
       }
     }
+#pragma unroll 1
+    for (uint32_t found = plus | minus; found; found &= found - 1) {
+      const int i = __ffs(found) - 1;
+      __stcg(dst + c + i, !((plus >> i) & 1u) ? -CUDART_INF_F : (minus >> i) & 1u ? CUDART_NAN_F : CUDART_INF_F);
+    }
+    __syncwarp();
   }
 }
 

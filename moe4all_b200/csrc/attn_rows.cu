@@ -427,10 +427,12 @@ __global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
     if (any_odd) {  // some value that a row sees may not be finite: put together by itself
       __threadfence();
       __syncthreads();
-      if (tid < n_rows && s_weight[tid] == s_weight[tid])
-        attn_odd_values(p, cur.s, cur.seq.q0, cur.head, (blk.tile0 + first_tile) << Sh::LOG2_TILE, (blk.tile0 + end_tile) << Sh::LOG2_TILE, 16, full_lo, full_hi,
-                        cur.seq.past + blk.t0 + attn_row_token(p, tid), 0, HD,
-                        whole ? p.out + attn_row_offset(p, cur.seq.q0 + blk.t0, cur.head, tid, p.out_stride) : p.part + ((size_t)attn_slot(blockIdx.x, share) * RB + tid) * HD);
+      const int r = lane < n_rows ? lane : 0;
+#pragma unroll 1
+      for (int col0 = 32 * warp; col0 < p.hd; col0 += 32 * WARPS)
+        attn_odd_values(p, cur.s, cur.seq.q0, cur.head, (blk.tile0 + first_tile) << Sh::LOG2_TILE, (blk.tile0 + end_tile) << Sh::LOG2_TILE, 1 << Sh::LOG2_TILE, full_lo,
+                        full_hi, lane < n_rows && s_weight[r] == s_weight[r], cur.seq.past + blk.t0 + attn_row_token(p, r), col0, 32,
+                        (whole ? p.out + attn_row_offset(p, cur.seq.q0 + blk.t0, cur.head, r, p.out_stride) : p.part + ((size_t)attn_slot(blockIdx.x, share) * RB + r) * HD) + col0);
     }
     if (!whole && attn_arrive(p, share.first, share.last, &s_last, tid == 0, 0, THREADS)) {
 #pragma unroll 1

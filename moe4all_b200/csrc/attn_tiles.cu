@@ -607,12 +607,13 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
           __syncwarp();
         }
         if (mine_row && !whole && group == 0) __stcg(p.part_ml + slot, ml);
-        if (__any_sync(0xFFFFFFFFu, mine_row && odd && L == L)) {  // (the rows' stores above are seen by the lanes that put them right)
+        const bool put_right = mine_row && odd && L == L;
+        if (__any_sync(0xFFFFFFFFu, put_right)) {  // (the rows' stores above are seen by the lanes that put them right)
           __threadfence();
           __syncwarp();
-          if (mine_row && odd && L == L)
-            attn_odd_values(p, it.s, it.q0, it.head, it.key0, it.key0 + ((end - first) << Sh::LOG2_TILE), BK, it.full_lo, it.full_hi, it.pos0 + attn_row_token(p, row),
-                            col0, Sh::COLS, whole ? p.out + attn_row_offset(p, it.row0, it.head, row, p.out_stride) + col0 : p.part + slot * HD + col0);
+          attn_odd_values(p, it.s, it.q0, it.head, it.key0, it.key0 + ((end - first) << Sh::LOG2_TILE), BK, it.full_lo, it.full_hi, put_right,
+                          it.pos0 + attn_row_token(p, row), col0, Sh::COLS,
+                          whole ? p.out + attn_row_offset(p, it.row0, it.head, mine_row ? row : 0, p.out_stride) + col0 : p.part + slot * HD + col0);
         }
       }
       if (!whole) {  // the first and the last at most

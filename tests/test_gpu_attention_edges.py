@@ -4,7 +4,7 @@ import dataclasses
 
 import pytest
 
-from test_gpu_attention import Batch, Rope, check
+from test_gpu_attention import NAN, Batch, Rope, check
 
 pytestmark = pytest.mark.gpu
 
@@ -50,3 +50,64 @@ def test_widest_windows_where_rows_in_front_see_nothing(backend, path, window):
     assert bool((want[:4] == 0).all()) and bool((want[4:10] != 0).any(1).all())
     check(backend, Batch([1, 40, 7], [600, 20, 0], 8, 2, 64, page=16, seed=5), window=window, path=path)
     check(backend, Batch([30, 1, 200], [0, 0, 0], 8, 2, 64, seed=6), window=window, path=path)
+
+
+@pytest.mark.parametrize("path", [1, 2])
+@pytest.mark.parametrize("hd", [48, 80, 128])
+def test_values_rewritten_between_calls_that_put_odd_ones_together(backend, path, hd):
+    # infinities in other rows and columns every time, no wait between the calls: each sees its own
+    import torch
+    from moe4all_b200 import RopeKv
+
+    H, K, n, steps, w = 4, 2, [70, 9], 12, backend.wrap_tensor
+    b = Batch(n, [0, 0], H, K, hd, page=16, seed=hd)
+    g = torch.Generator(device="cuda").manual_seed(7)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda")
+    q, k = r(79, H * hd), r(79, K * hd)
+    vs, outs, ropes, ops, wants = [], [torch.zeros_like(b.out) for _ in range(steps)], [], [], []
+    for i in range(steps):
+        v = r(79, K * hd)
+        for row, col in ((i * 5 % 70, i * 7 % (K * hd)), (70 + i % 9, (i * 11 + 3) % (K * hd))):
+            v[row, col] = float("inf") if i % 3 else float("-inf")
+        vs.append(v)
+        ropes.append(RopeKv(q=w(q), k=w(k), v=w(v), q_out=w(b.q), k_cache=w(b.k), v_cache=w(b.v), **b.fields(backend)))
+        ops.append(b.op(backend, path=path, out=w(outs[i])))
+        torch.cuda.synchronize()
+        backend.rope_kv(ropes[i])
+        backend.sync()
+        wants.append(b.ref())
+    torch.cuda.synchronize()
+    for rope, op in zip(ropes, ops):
+        backend.rope_kv(rope)
+        backend.attention(op)
+    backend.sync()
+    for got, (want, tol) in zip(outs, wants):
+        assert torch.equal(got.isfinite(), want.isfinite())
+        assert float(torch.where(want.isfinite(), (got - want).abs(), 0.0).max()) <= tol and torch.equal(torch.where(want.isinf(), got.double(), 0.0), torch.where(want.isinf(), want, 0.0))
+
+
+@pytest.mark.parametrize("path,K,n,kv", [(2, 8, 40, 16384), (1, 8, 40, 16384), (2, 1, 1, 300_000), (1, 1, 1, 300_000)])
+def test_long_contexts_of_nothing_but_infinities_end_in_time(backend, path, K, n, kv):
+    # every value is infinite, of one sign per column or of both: put together for two items and more to a CTA while its other warps wait
+    import torch
+    from moe4all_b200 import Attention
+
+    hd, page, rows, w = 64, 256, 4, backend.wrap_tensor
+    g = torch.Generator(device="cuda").manual_seed(9)
+    pages = n * -(-kv // page)
+    k = torch.randn(pages, K, page, hd, generator=g, device="cuda", dtype=torch.float16)
+    v = torch.full_like(k, float("inf"))
+    v[..., 1::2] = float("-inf")
+    v[:, :, ::2, 10] = float("-inf")
+    v[:, :, ::2, 11] = NAN
+    q, out = torch.randn(n * rows, K * hd, generator=g, device="cuda"), torch.zeros(n * rows, K * hd, device="cuda")
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    cu, lens, table = i32([i * rows for i in range(n + 1)]), i32([kv] * n), i32(list(range(pages))).view(n, -1)
+    torch.cuda.synchronize()
+    backend.attention(Attention(q=w(q), k=w(k), v=w(v), out=w(out), scale=0.125, cu_q=w(cu), kv_len=w(lens), page_table=w(table), rows=n * rows, n_seq=n, n_head=K, n_kv=K,
+                                head_dim=hd, n_pages=pages, page_size=page, max_pages=pages // n, max_q=rows, path=path))
+    backend.sync()
+    want = torch.full((hd,), float("inf"), device="cuda")
+    want[1::2] = float("-inf")
+    want[10] = want[11] = NAN
+    assert torch.equal(out.view(-1, hd).nan_to_num(nan=7.0), want.expand(n * rows * K, hd).nan_to_num(nan=7.0))
