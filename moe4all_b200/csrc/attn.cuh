@@ -59,6 +59,19 @@ __device__ __forceinline__ bool attn_wait(uint64_t* bar, int phase) {
 }
 __device__ __forceinline__ bool wait_all(uint64_t* bar, int phase) { return __all_sync(0xFFFFFFFFu, attn_wait(bar, phase)); }
 
+// Where a role has given up, copies and MMAs that nobody waits for any more are in flight: two milliseconds for what takes microseconds, by the clock
+// (__nanosleep may return at once), before shared and tensor memory are somebody else's.
+static __device__ __noinline__ void attn_let_land() {
+  uint64_t begin, now;
+  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(begin)::"memory");
+#pragma unroll 1
+  for (uint32_t i = 0; i < (1u << 24); ++i) {
+    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(now)::"memory");
+    if (now - begin > 2000000) return;
+    __nanosleep(1000);
+  }
+}
+
 __device__ __forceinline__ AttnSeq attn_load_seq(const AttnParams& p, int s) {
   bool bad = false;
   const AttnSeq r = attn_seq(__ldcg(p.cu_q + s), __ldcg(p.cu_q + s + 1), p.kv_len != nullptr ? __ldcg(p.kv_len + s) : 0, p.kv_len == nullptr, p.rows, p.cap, &bad);

@@ -112,7 +112,7 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
   __shared__ long long s_scan[Sh::THREADS / 32];
   __shared__ AttnStart s_start;
   __shared__ uint32_t s_tmem;
-  __shared__ int s_last, s_odd[4 * RING];
+  __shared__ int s_last, s_gave_up, s_odd[4 * RING];
   unsigned char* s_q = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   unsigned char *s_k = s_q + 2 * Sh::QPIECE, *s_v = s_k + BUFS * TILE;
   unsigned char* s_out = s_v + BUFS * TILE;
@@ -134,6 +134,11 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
     mbar_fence_init();
   }
   if (tid < 4 * RING) s_odd[tid] = 0;
+  if (tid == 0) s_gave_up = 0;
+  auto gave_up = [&]() {  // a bounded wait ran out
+    atomicExch(&p.status->timeout, 11);
+    s_gave_up = 1;
+  };
   if (warp == 0) umma::tmem_alloc(&s_tmem);
   pdl_wait();
   attn_plan<Sh::THREADS, Sh::LOG2_TILE, Sh::EXTRA, Sh::JOIN>(p, reinterpret_cast<int*>(s_q), s_scan, &s_start);
@@ -197,8 +202,7 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
       }
       return at;
     };
-    int ks = 0, vs = 0;  // copies asked for
-    auto load = [&](const Place& at, int n, int& asked, const CUtensorMap* map, unsigned char* bufs, uint64_t* full, uint64_t* empty) {
+    auto load = [&](const Place& at, int n, const CUtensorMap* map, unsigned char* bufs, uint64_t* full, uint64_t* empty) {
       const int buf = n % BUFS;
       const int count = __popc(__ballot_sync(0xFFFFFFFFu, at.y >= 0));
       if (n >= BUFS) ok = wait_all(empty + buf, n / BUFS - 1);
@@ -212,29 +216,21 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
         for (int s = 0; s < SLABS; ++s) tma_load_4d(dst + s * (BK * 128), map, 64 * s, at.y, at.head, w, full);
       }
       __syncwarp();
-      asked = n + 1;
     };
     // V of tile n, K of tile n + 2: the order in which they are used, and in which buffers come free
     Place v0 = {}, v1 = {}, k = place(0);
 #pragma unroll 1
     for (int n = -2; n < N && ok; ++n) {
-      if (n >= 0) load(v0, n, vs, &vmap, s_v, bars.v_full + n % BUFS, bars.v_empty);
+      if (n >= 0) load(v0, n, &vmap, s_v, bars.v_full + n % BUFS, bars.v_empty);
       v0 = v1, v1 = k;
       if (n + 2 < N && ok) {
-        load(k, n + 2, ks, &kmap, s_k, n < 0 ? bars.k_first + n + 2 : bars.ready + (n & 3), bars.k_empty);
+        load(k, n + 2, &kmap, s_k, n < 0 ? bars.k_first + n + 2 : bars.ready + (n & 3), bars.k_empty);
         k = place(n + 3);
       } else if (ok && lane == 0) {
         mbar_arrive(bars.ready + (n & 3));
       }
     }
-    if (!ok) {
-      if (lane == 0) atomicExch(&p.status->timeout, 11);
-      // copies in flight land before the shared memory is somebody else's
-      for (int i = max(0, vs - BUFS); i < vs; ++i) attn_wait(bars.v_full + i % BUFS, i / BUFS);
-      for (int i = max(0, ks - BUFS); i < min(ks, 2); ++i) attn_wait(bars.k_first + i, 0);
-      // (K's land in barriers that wait for more than copies: their bytes are given the time that copies take at most)
-      __nanosleep(1000000);
-    }
+    if (!ok && lane == 0) gave_up();
   } else if (role == 4) {
     // ---- MMAs.  Scores run one tile ahead of the sums; their accumulators are free by then, since MMAs of one thread go in order
     const uint32_t idesc_s = umma::idesc_f16_f32(128, BK), idesc_o = umma::idesc_f16_f32(128, HD) | umma::IDESC_B_MN_MAJOR;
@@ -306,7 +302,7 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
         __syncwarp();
       }
     }
-    if (!ok && lane == 0) atomicExch(&p.status->timeout, 11);
+    if (!ok && lane == 0) gave_up();
   } else if (role > 4) {
     // ---- V tiles with hidden keys.  0 x value has to be 0 where a row does not see the key: keys that no row sees become zeros, and so do
     // values that are not finite; the item's end adds these to the rows that see them
@@ -364,7 +360,7 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(bars.ready + (n & 3));
     }
-    if (!ok && lane == 0) atomicExch(&p.status->timeout, 11);
+    if (!ok && lane == 0) gave_up();
   } else if (role == 0) {
     // ---- weights: thread = row, 64 keys of each tile
     set_regs<Sh::REG_W>();
@@ -427,9 +423,9 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
     };
     // an item's q is turned two tiles ahead of its first: its scores then follow the last item's without a break.  (Not earlier: the copies
     // know of an item three tiles ahead.)
-    int turned = 0;
+    int turned = 0, n = 0;
 #pragma unroll 1
-    for (int n = 0, item = 0; n < N && ok; ++item) {
+    for (int item = 0; n < N && ok; ++item) {
       ok = wait_all(bars.i_full + item % ITEMS, item / ITEMS);
       if (!ok) break;
       const TileItem& it = s_item[item % ITEMS];
@@ -521,7 +517,10 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
         stop = n1;
       }
     }
-    if (!ok && lane == 0) atomicExch(&p.status->timeout, 11);
+    if (!ok && lane == 0) gave_up();
+    if constexpr (GROUPS == 2)  // the other warp of these rows may give up later: it still waits for this one at the tiles until then
+#pragma unroll 1
+      for (; n < N; ++n) asm volatile("bar.sync %0, 64;" ::"r"(2 + (warp & 3)) : "memory");
   } else {
     // ---- sums: thread = row, COLS of its columns
     set_regs<Sh::REG_S>();
@@ -621,9 +620,11 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
         ++parts;
       }
     }
-    // ---- items that other CTAs have tiles of: whoever comes last joins them
+    // ---- items that other CTAs have tiles of: whoever comes last joins them.  All of these warps do or none does: one may have given up alone
+    uint32_t all = ok;
+    asm volatile("{\n\t.reg .pred a, b;\n\tsetp.ne.u32 a, %0, 0;\n\tbar.red.and.pred b, 1, %1, a;\n\tselp.u32 %0, 1, 0, b;\n\t}" : "+r"(all) : "n"(128 * Sh::S_GROUPS) : "memory");
 #pragma unroll 1
-    for (int i = 0; i < parts && ok; ++i) {
+    for (int i = 0; i < parts && all; ++i) {
       if (attn_arrive(p, s_parts[i].first_cta, s_parts[i].last_cta, &s_last, tid == 128 * Sh::W_GROUPS, 1, 128 * Sh::S_GROUPS)) {
         const TileItem& it = s_parts[i];
         const AttnShare share = {it.first_cta, it.last_cta};
@@ -687,11 +688,12 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
         asm volatile("bar.sync 1, %0;" ::"n"(128 * Sh::S_GROUPS) : "memory");
       }
     }
-    if (!ok && lane == 0) atomicExch(&p.status->timeout, 11);
+    if (!ok && lane == 0) gave_up();
   }
   umma::fence_before_sync();
   __syncthreads();
   umma::fence_after_sync();
+  if (s_gave_up) attn_let_land();
   if (warp == 0) umma::tmem_dealloc(tmem);
 }
 
