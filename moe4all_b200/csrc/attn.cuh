@@ -39,6 +39,10 @@ __device__ __forceinline__ float exp2_approx(float x) {
 // 2^(a - b) where a <= b, either possibly "no key yet" (-inf).
 __device__ __forceinline__ float exp2_rel(float a, float b) { return a == -CUDART_INF_F ? 0.f : exp2_approx(a - b); }
 
+// A part's sum x on its way into a join: where the part's weight has underflowed, what is not finite still arrives, so that a result does not
+// depend on how its keys were cut into parts.
+__device__ __forceinline__ float weighed(float w, float x) { return w != 0.f ? w * x : fabsf(x) < CUDART_INF_F ? 0.f : x; }
+
 __device__ __forceinline__ void tma_load_4d(void* smem_dst, const CUtensorMap* tm, int x, int y, int z, int w, uint64_t* bar) {
   asm volatile(
       "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(
@@ -377,7 +381,7 @@ __device__ __forceinline__ void attn_join_row(const AttnParams& p, const AttnSha
     if (c0 + lane < parts) {
       const float2 ml = __ldcg(&p.part_ml[(size_t)attn_slot(sh.first + c0 + lane, sh) * item_rows + r]);
       w = exp2_rel(ml.x, M);
-      if (w != 0.f) L += w * ml.y;  // (a part that saw nothing holds nothing)
+      L += w * ml.y;
     }
 #pragma unroll 1
     for (int k0 = 0; k0 < min(32, parts - c0); k0 += 8) {
@@ -391,9 +395,11 @@ __device__ __forceinline__ void attn_join_row(const AttnParams& p, const AttnSha
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         const float wk = __shfl_sync(0xFFFFFFFFu, w, k0 + k);
-        if (c0 + k0 + k < parts && wk != 0.f) {
+        if (c0 + k0 + k < parts) {
 #pragma unroll
-          for (int j = 0; j < V; ++j) o[j].x += wk * v[k][j].x, o[j].y += wk * v[k][j].y, o[j].z += wk * v[k][j].z, o[j].w += wk * v[k][j].w;
+          for (int j = 0; j < V; ++j)
+            if (4 * lane + 128 * j < HD)
+              o[j].x += weighed(wk, v[k][j].x), o[j].y += weighed(wk, v[k][j].y), o[j].z += weighed(wk, v[k][j].z), o[j].w += weighed(wk, v[k][j].w);
         }
       }
     }

@@ -352,7 +352,8 @@ __global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
       for (int j = 0; j < 2; ++j)
         if (m[n][j] == -CUDART_INF_F && l[n][j] != 0.f) m[n][j] = 0.f;  // nothing but NaN: a part that counts, not one without keys
     __syncthreads();  // the last item's parts have been read
-    // one half of the warps puts its sums down, the other adds its own to them, each brought to the higher maximum
+    // one half of the warps puts its sums down, the other adds its own to them, each brought to the higher maximum.  (No part is left out because its
+    // weight has underflowed: what is not finite in it stays that, here as NaN, and is put right below)
     if (lane < 4) {
 #pragma unroll
       for (int n = 0; n < NT; ++n)
@@ -383,8 +384,8 @@ __global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
 #pragma unroll
           for (int k = 0; k < KST; ++k) {
             float* at = mine + (8 * n + c0 + j) * PITCH + 16 * k;
-            at[0] = (a != 0.f ? a * o[k][n][j] : 0.f) + (b != 0.f ? b * at[0] : 0.f);
-            at[8] = (a != 0.f ? a * o[k][n][2 + j] : 0.f) + (b != 0.f ? b * at[8] : 0.f);
+            at[0] = a * o[k][n][j] + b * at[0];
+            at[8] = a * o[k][n][2 + j] + b * at[8];
           }
         }
     }
@@ -408,11 +409,10 @@ __global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
         const float m0 = s_m[w * RB + r], m1 = two ? s_m[(w + SLOTS) % WARPS * RB + r] : -CUDART_INF_F;
         const float wt = exp2_rel(fmaxf(m0, m1), M);
         const float4 v = *reinterpret_cast<const float4*>(s_o + (w * RB + r) * PITCH + i);
-        if (wt != 0.f) {
-          const float w0 = exp2_rel(m0, M), w1 = exp2_rel(m1, M);
-          L += (w0 != 0.f ? w0 * s_l[w * RB + r] : 0.f) + (w1 != 0.f ? w1 * s_l[(w + SLOTS) % WARPS * RB + r] : 0.f);
-          sum.x += wt * v.x, sum.y += wt * v.y, sum.z += wt * v.z, sum.w += wt * v.w;
-        }
+        L += exp2_rel(m0, M) * s_l[w * RB + r];
+        if (two) L += exp2_rel(m1, M) * s_l[(w + SLOTS) % WARPS * RB + r];
+        sum.x += wt * v.x, sum.y += wt * v.y, sum.z += wt * v.z, sum.w += wt * v.w;
+
       }
       if (whole) {
         const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);

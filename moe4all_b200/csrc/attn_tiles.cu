@@ -644,7 +644,7 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
 #pragma unroll 8
           for (int c = 0; c < n; ++c) {
             const float w = exp2_rel(s_w[c * 128 + at], M);
-            if (w != 0.f) L += w * __ldcg(&p.part_ml[(size_t)attn_slot(share.first + c, share) * 128 + at]).y;  // (a part that saw nothing holds nothing)
+            L += w * __ldcg(&p.part_ml[(size_t)attn_slot(share.first + c, share) * 128 + at]).y;
             s_w[c * 128 + at] = w;
           }
           const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);  // NaN stays
@@ -675,8 +675,9 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
             for (int c = 0; c < 4; ++c)
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
-                const float w = c0 + c < n ? s_w[(c0 + c) * 128 + row[i]] : 0.f;
-                if (w != 0.f) o[i].x += w * v[c][i].x, o[i].y += w * v[c][i].y, o[i].z += w * v[c][i].z, o[i].w += w * v[c][i].w;
+                if (c0 + c >= n) continue;
+                const float w = s_w[(c0 + c) * 128 + row[i]];
+                o[i].x += weighed(w, v[c][i].x), o[i].y += weighed(w, v[c][i].y), o[i].z += weighed(w, v[c][i].z), o[i].w += weighed(w, v[c][i].w);
               }
           }
 #pragma unroll

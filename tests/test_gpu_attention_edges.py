@@ -111,3 +111,29 @@ def test_long_contexts_of_nothing_but_infinities_end_in_time(backend, path, K, n
     want[1::2] = float("-inf")
     want[10] = want[11] = NAN
     assert torch.equal(out.view(-1, hd).nan_to_num(nan=7.0), want.expand(n * rows * K, hd).nan_to_num(nan=7.0))
+
+
+@pytest.mark.parametrize("H,K,hd,n", [(8, 2, 64, 1), (8, 1, 128, 2), (4, 1, 256, 1), (2, 1, 192, 5), (4, 1, 128, 100), (6, 2, 64, 30), (2, 1, 256, 40)])
+@pytest.mark.parametrize("path", [1, 2])
+@pytest.mark.parametrize("kv", [40, 9000])
+def test_what_is_not_finite_reaches_its_row_whatever_its_weight(backend, path, H, K, hd, n, kv):
+    # early keys hundreds of powers of two below the later ones: their parts' weights underflow where warps and CTAs join
+    b = Batch([n, 1], [kv, kv // 2], H, K, hd, page=16, seed=hd + n)
+    for s in range(2):
+        k, v = b.get(b.k, s).clone(), b.get(b.v, s).clone()
+        b.q[b.cu[s] : b.cu[s + 1], : H * hd] = b.q[b.cu[s] : b.cu[s + 1], : H * hd].abs() + 1.0
+        k[:] = k.abs() * 0.25
+        k[: kv // 3] -= 60.0
+        for key, col, x in ((0, 3, "inf"), (1, 4, "nan"), (5, 6, "-inf"), (11, 6, "inf"), (kv // 4, hd - 1, "-inf")):
+            v[key, :, col] = float(x)
+        b.put(b.k, s, k)
+        b.put(b.v, s, v)
+    want = check(backend, b, path=path)[:, : H * hd].view(-1, H, hd)
+    assert bool((want[:, :, 3] == float("inf")).all()) and bool(want[:, :, [4, 6]].isnan().all()) and bool((want[:, :, hd - 1] == float("-inf")).all())
+    assert bool(want[:, :, [0, 1, 2, 5]].isfinite().all())
+    # and a key without a score makes NaN of its rows, as early and as light as it is
+    k = b.get(b.k, 0).clone()
+    k[7, 0, 2] = NAN
+    b.put(b.k, 0, k)
+    want = check(backend, b, path=path)[:, : H * hd].view(-1, H, hd)
+    assert bool(want[:n, : H // K].isnan().all()) and bool(want[:n, H // K :, 0].isfinite().all()) and bool(want[n:, :, 0].isfinite().all())
