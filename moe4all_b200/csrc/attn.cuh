@@ -12,7 +12,7 @@ struct AttnParams {
   const float* q;
   float* out;
   const int *cu_q, *kv_len, *page_table;  // kv_len, page_table: null where the keys are packed rows
-  const __half* v;                        // for what the tiles' products leave out (values that are not finite)
+  const __half *k, *v;                    // for what the tiles' products of pieces get wrong (keys and values that are not finite)
   size_t page_pitch, head_pitch, row_pitch;  // of the cache, in values
   long long q_stride, out_stride;
   float* part;      // [2 CTAs][rows of an item][HD] sums, not yet divided
@@ -101,11 +101,11 @@ __device__ __forceinline__ size_t attn_row_offset(const AttnParams& p, int token
   return (size_t)(token0 + t) * stride + (size_t)(head * p.g + (r - t * p.g)) * p.hd;
 }
 
-// Where the values of a key and head begin; the keys behind it follow row_pitch apart up to its page's end.
-__device__ __forceinline__ const __half* attn_value(const AttnParams& p, int s, int q0, int head, int key) {
-  if (p.page_table == nullptr) return p.v + (size_t)(q0 + key) * p.row_pitch + (size_t)head * p.head_pitch;
+// Where the values of a key and head begin in K or V; the keys behind it follow row_pitch apart up to its page's end.
+__device__ __forceinline__ const __half* attn_value(const AttnParams& p, const __half* cache, int s, int q0, int head, int key) {
+  if (p.page_table == nullptr) return cache + (size_t)(q0 + key) * p.row_pitch + (size_t)head * p.head_pitch;
   const int page = attn_page_of(p, key);
-  return p.v + (size_t)attn_page(p, s, page) * p.page_pitch + (size_t)(key - page * p.page_size) * p.row_pitch + (size_t)head * p.head_pitch;
+  return cache + (size_t)attn_page(p, s, page) * p.page_pitch + (size_t)(key - page * p.page_size) * p.row_pitch + (size_t)head * p.head_pitch;
 }
 
 // Powers of two that bring a row whose largest magnitude is `big` to [2^7, 2^8), and back; both normal numbers.
@@ -273,6 +273,29 @@ struct AttnCursor {
   }
 };
 
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN where either is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// The score (times a positive number) of a visible key for which the products of q's pieces came out as NaN: the sum of q's products with the key's
+// components that are not finite, which is all that decides it (inf times a piece of the other sign, or of zero, made the NaN).  NaN where the key is
+// finite: then q is not.
+__device__ __forceinline__ float attn_odd_score(const AttnParams& p, int s, int q0, int head, int key, const float* q) {
+  const __half* k = attn_value(p, p.k, s, q0, head, key);
+  float sum = 0.f;
+  bool found = false;
+#pragma unroll 1
+  for (int i = 0; i < p.hd; ++i) {
+    const float x = __half2float(__ldcg(k + i));
+    if (fabsf(x) < CUDART_INF_F) continue;
+    sum += x * __ldcg(q + i);
+    found = true;
+  }
+  return found ? sum * p.scale_log2 : CUDART_NAN_F;
+}
+
 // Which of an f16 pair's values are +inf or NaN (bits 0 and 1), and -inf or NaN (bits 16 and 17).
 __device__ __forceinline__ uint32_t odd_pair(uint32_t x) {
   uint32_t r = 0;
@@ -310,7 +333,7 @@ static __device__ __forceinline__ void attn_odd_values(const AttnParams& p, int 
         const int key = k0 + lane;
         uint32_t mine_plus = 0, mine_minus = 0;
         if (key >= lo && key <= hi) {
-          const uint4* v = reinterpret_cast<const uint4*>(attn_value(p, s, q0, head, key) + col0 + c);
+          const uint4* v = reinterpret_cast<const uint4*>(attn_value(p, p.v, s, q0, head, key) + col0 + c);
 #pragma unroll 1
           for (int j = 0; 8 * j < n; ++j) {
             const uint4 x = __ldcg(v + j);  // past L1, as all that an earlier kernel wrote: this one may have started beside it

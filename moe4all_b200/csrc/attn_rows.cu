@@ -255,7 +255,7 @@ __global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
               if (key > to || key < from) s[n][j] = -CUDART_INF_F;
               if (key + 8 > to || key + 8 < from) s[n][2 + j] = -CUDART_INF_F;
             }
-            grows |= fmaxf(s[n][j], s[n][2 + j]) > m[n][j] + ATTN_SLACK;
+            grows |= !(max_nan(s[n][j], s[n][2 + j]) <= m[n][j] + ATTN_SLACK);  // (or there is none)
           }
         // (the maximum is looked for only where a score is past the slack: one vote instead of three rounds of shuffles)
         if (__any_sync(0xFFFFFFFFu, grows)) {
@@ -263,6 +263,13 @@ __global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
           for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
+              if (l[n][j] == l[n][j] && 8 * n + c0 + j < n_rows) {  // (a row that is NaN already stays that)
+#pragma unroll
+                for (int i = 0; i < 4; i += 2)
+                  if (s[n][i + j] != s[n][i + j])
+                    s[n][i + j] = attn_odd_score(p, cur.s, cur.seq.q0, cur.head, key + 4 * i,
+                                                 p.q + attn_row_offset(p, cur.seq.q0 + blk.t0, cur.head, 8 * n + c0 + j, p.q_stride));
+              }
               float mx = fmaxf(s[n][j], s[n][2 + j]);
 #pragma unroll
               for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, x));
@@ -471,6 +478,7 @@ bool attn_cache_map(CUtensorMap* tm, const __half* base, const AttnParams& p, in
 // max_rows: rows (tokens x heads of a kv head) that a sequence's new tokens make at most, as far as the caller knows; longer ones are
 // cut into more items.
 int32_t launch_attn_rows(infr_cuda_ctx* ctx, AttnParams p, const __half* k, int max_rows) {
+  p.k = k;
   CUtensorMap km, vm;
   if (!attn_cache_map(&km, k, p, 16) || !attn_cache_map(&vm, p.v, p, 16)) return fail(ctx, INFR_CUDA_ERR_CUDA, "attention: cuTensorMapEncodeTiled failed");
   const int nt = p.g <= 8 && max_rows <= 8 ? 1 : 2;

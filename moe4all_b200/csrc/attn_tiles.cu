@@ -101,6 +101,23 @@ __device__ __forceinline__ void hide(float (&s)[32], uint32_t seen) {
   for (int i = 0; i < 32; ++i) s[i] = (seen >> i) & 1u ? s[i] : -CUDART_INF_F;
 }
 
+// Scores of 64 keys at sa, some of which are NaN in this warp's rows: these are put right, and the row's maximum is given back.  (A column at a
+// time: all lanes take part.)
+static __device__ __noinline__ float tile_odd_scores(const AttnParams& p, const TileItem& it, int ks, int from, int to, int row, uint32_t sa, bool put_right, float top) {
+  const float* q = p.q + attn_row_offset(p, it.row0, it.head, put_right ? row : 0, p.q_stride);
+  if (put_right) top = -CUDART_INF_F;
+#pragma unroll 1
+  for (int i = 0; i < 64; ++i) {
+    float x = umma::tmem_ld_32x1(sa + i);
+    const bool seen = put_right && ks + i >= from && ks + i <= to;
+    if (seen && x != x) x = attn_odd_score(p, it.s, it.q0, it.head, ks + i, q);
+    if (seen) top = fmaxf(top, x);
+    __syncwarp();
+    umma::tmem_st_32x1(sa + i, x);
+  }
+  return top;
+}
+
 template <int HD>
 __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
     k_attn_tiles(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ AttnParams p, const int granule) {
@@ -460,9 +477,11 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
               if (masked) hide(s, seen);
               float t[2] = {top, -CUDART_INF_F};
 #pragma unroll
-              for (int i = 0; i < 32; i += 2) t[(i >> 1) & 1] = fmaxf(fmaxf(t[(i >> 1) & 1], s[i]), s[i + 1]);
-              top = fmaxf(t[0], t[1]);
+              for (int i = 0; i < 32; i += 2) t[(i >> 1) & 1] = max_nan(max_nan(t[(i >> 1) & 1], s[i]), s[i + 1]);
+              top = max_nan(t[0], t[1]);
             }
+            const bool put_right = top != top && row < n_rows && l == l;  // (a row that is NaN already stays that)
+            if (__any_sync(0xFFFFFFFFu, put_right)) top = tile_odd_scores(p, it, ks, from, to, row, sa, put_right, top);
           }
           if constexpr (GROUPS == 2) {
             float* at = s_max + (n & 1) * 256 + row;
@@ -712,6 +731,7 @@ int32_t launch_attn_tiles(infr_cuda_ctx* ctx, AttnParams p, const __half* k) {
   // a copy takes as many keys as lie side by side in every page
   int granule = p.hd <= 128 ? 128 : 64;
   while (p.page_table != nullptr && p.page_size % granule) granule >>= 1;
+  p.k = k;
   CUtensorMap km, vm;
   if (!attn_cache_map(&km, k, p, granule) || !attn_cache_map(&vm, p.v, p, granule)) return fail(ctx, INFR_CUDA_ERR_CUDA, "attention: cuTensorMapEncodeTiled failed");
   p.tb = ATTN_TILE_ROWS / p.g;

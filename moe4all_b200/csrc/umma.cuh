@@ -203,6 +203,15 @@ __device__ __forceinline__ void tmem_ld_wait(float (&r)[16]) {
                :
                : "memory");
 }
+// One column, with the waits (for what happens rarely).
+__device__ __forceinline__ float tmem_ld_32x1(uint32_t taddr) {
+  float r;
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\n\ttcgen05.wait::ld.sync.aligned;" : "=f"(r) : "r"(taddr) : "memory");
+  return r;
+}
+__device__ __forceinline__ void tmem_st_32x1(uint32_t taddr, float r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};\n\ttcgen05.wait::st.sync.aligned;" ::"r"(taddr), "f"(r) : "memory");
+}
 // 32 columns written, without the wait.
 __device__ __forceinline__ void tmem_st_32x32_async(uint32_t taddr, const uint32_t (&r)[32]) {
   asm volatile(

@@ -137,3 +137,35 @@ def test_what_is_not_finite_reaches_its_row_whatever_its_weight(backend, path, H
     b.put(b.k, 0, k)
     want = check(backend, b, path=path)[:, : H * hd].view(-1, H, hd)
     assert bool(want[:n, : H // K].isnan().all()) and bool(want[:n, H // K :, 0].isfinite().all()) and bool(want[n:, :, 0].isfinite().all())
+
+
+@pytest.mark.parametrize("H,K,hd,n", [(8, 2, 64, 1), (8, 1, 128, 2), (4, 1, 256, 1), (3, 3, 80, 9), (2, 1, 192, 7), (4, 1, 128, 200), (16, 1, 64, 30), (2, 1, 256, 140)])
+@pytest.mark.parametrize("path", [1, 2])
+@pytest.mark.parametrize("page", [0, 16])
+@pytest.mark.parametrize("scale", [1, -1])
+def test_infinite_keys_count_by_their_scores(backend, path, page, H, K, hd, n, scale):
+    # a key with an infinite component has a score of -inf (and no weight) or +inf (and its row is NaN), by q's sign there: the formula's, not
+    # that of q's pieces, the second of which may be zero or of the other sign
+    import torch
+
+    b = Batch([n, 3], [0, 0] if not page else [700, 40], H, K, hd, page=page, seed=hd + n)
+    b.q[: n + 3, 2 : H * hd : hd] = b.q[: n + 3, 2 : H * hd : hd].abs() * scale
+    b.q[: n + 3, 3 : H * hd : hd] = -b.q[: n + 3, 3 : H * hd : hd].abs() * scale
+    b.q[: n + 3 : 2, 2 : H * hd : hd] = b.q[: n + 3 : 2, 2 : H * hd : hd].half().float()  # (no second piece, or next to none)
+    inf = float("inf")
+    for s in range(2):  # (the first key is finite: every row sees a score)
+        k = b.get(b.k, s).clone()
+        for i, key in enumerate({1, b.kv[s] // 2, b.kv[s] - 2} & set(range(1, b.kv[s]))):
+            k[key, :, 2 if i % 2 else 3] = -inf if i % 2 else inf
+            if i == 2:
+                k[key, :, 2] = -inf  # two of them, of one sign
+        b.put(b.k, s, k)
+    want = check(backend, b, scale=scale * hd ** -0.5, path=path)
+    assert bool(want[:, : H * hd].isfinite().all())
+    # of the other sign, in one of the heads' keys: NaN from there on
+    t = b.kv[0] - n + n // 2
+    k = b.get(b.k, 0).clone()
+    k[t, 0, 2] = inf
+    b.put(b.k, 0, k)
+    want = check(backend, b, scale=scale * hd ** -0.5, path=path)[:, : H * hd].view(-1, H, hd)
+    assert bool(want[n // 2 : n, : H // K].isnan().all()) and (n // 2 < 3 or bool(want[2 : n // 2].isfinite().all()))
