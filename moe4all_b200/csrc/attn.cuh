@@ -27,9 +27,13 @@ struct AttnParams {
   int page_shift;    // log2(page_size), or -1
 };
 
-// Weights are 2^(x - reference + ATTN_BIAS): the reference follows the running maximum only when that has grown by ATTN_SLACK, so
-// they stay below 2^15 and fit f16; a weight of 2^-32 of the largest still has a bit in f16's subnormals.
-constexpr float ATTN_BIAS = 7.f, ATTN_SLACK = 8.f;
+// Weights are 2^(x - reference + bias), two f16 pieces each: at most 2^15.9, and known to 2^-25.  The reference is a whole number (sums are
+// brought to another one without error) that follows the keys' maximum up and, where that falls far enough, down again: what a weight is rounded by
+// stays small against its neighbours' weights, not only against the row's largest, whose value may be next to nothing (a sink).
+constexpr float ATTN_BIAS = 10.f;
+constexpr float ATTN_SLACK = 5.9f;  // few-rows kernel: how far scores may pass the reference before it follows,
+constexpr float ATTN_FALL = 14.f;   // and how far below it the largest of 16 keys may stay, looked at every fourth time: its weight is 2^-5 or more
+// (64 streams, us: 84.7 without looking, 86 so, 88 with a slack of 1.9; rounds of shuffles for every 16 keys cost more than either)
 
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;
@@ -273,9 +277,14 @@ struct AttnCursor {
   }
 };
 
-__device__ __forceinline__ float max_nan(float a, float b) {  // NaN where either is
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN where one is
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 

@@ -243,7 +243,7 @@ __global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
         }
         const bool masked = ks + 16 > full_hi || ks < full_lo;
         const int key = ks + (lane >> 2);
-        bool grows = false;
+        bool grows = false, falls = false;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -257,8 +257,18 @@ __global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
             }
             grows |= !(max_nan(s[n][j], s[n][2 + j]) <= m[n][j] + ATTN_SLACK);  // (or there is none)
           }
-        // (the maximum is looked for only where a score is past the slack: one vote instead of three rounds of shuffles)
-        if (__any_sync(0xFFFFFFFFu, grows)) {
+        if ((t & 3) == 0) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              uint32_t high = __ballot_sync(0xFFFFFFFFu, fmaxf(s[n][j], s[n][2 + j]) >= m[n][j] - ATTN_FALL);  // of each column's eight lanes
+              high |= high >> 16, high |= high >> 8, high |= high >> 4;
+              falls |= (high & 15u) != 15u;
+            }
+        }
+        // (the maximum is looked for only where a score is past the slack, or all of a column's are far below: votes instead of rounds of shuffles)
+        if (__any_sync(0xFFFFFFFFu, grows) || falls) {
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -270,10 +280,17 @@ __global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
                     s[n][i + j] = attn_odd_score(p, cur.s, cur.seq.q0, cur.head, key + 4 * i,
                                                  p.q + attn_row_offset(p, cur.seq.q0 + blk.t0, cur.head, 8 * n + c0 + j, p.q_stride));
               }
-              float mx = fmaxf(s[n][j], s[n][2 + j]);
+              float mx = fmaxf(s[n][j], s[n][2 + j]), lx = l[n][j];
 #pragma unroll
               for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, x));
-              const float to = mx > m[n][j] + ATTN_SLACK ? mx : m[n][j];
+              if (falls) {
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) lx = fmaxf(lx, __shfl_xor_sync(0xFFFFFFFFu, lx, x));
+              }
+              float to = m[n][j];
+              if (mx > to + ATTN_SLACK) to = ceilf(mx);
+              // (down only as far as leaves the sums in range: weights so far below 2^60)
+              else if (falls && mx < to - ATTN_FALL && mx > -CUDART_INF_F) to = fminf(to, fmaxf(ceilf(mx), to + (float)((int)(__float_as_uint(lx) >> 23) - 187)));
               const float w = to == m[n][j] ? 1.f : exp2_rel(m[n][j], to);
               m[n][j] = to;
               l[n][j] *= w;
@@ -288,9 +305,9 @@ __global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
           float e[4];
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            const float off = ATTN_BIAS - (m[n][j] == -CUDART_INF_F ? 0.f : m[n][j]);
-            e[j] = exp2_approx(s[n][j] + off);
-            e[2 + j] = exp2_approx(s[n][2 + j] + off);
+            const float ref = m[n][j] == -CUDART_INF_F ? 0.f : m[n][j];
+            e[j] = exp2_approx((s[n][j] - ref) + ATTN_BIAS);  // (in this order: scores of any size)
+            e[2 + j] = exp2_approx((s[n][2 + j] - ref) + ATTN_BIAS);
             l[n][j] += e[j] + e[2 + j];
           }
           split2(e[0], e[1], ph[n][0], pl[n][0]);

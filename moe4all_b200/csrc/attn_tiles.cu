@@ -26,7 +26,7 @@
 namespace infr {
 namespace {
 
-constexpr float TILE_BIAS = 15.f;  // weights are 2^(x - maximum + 15): below f16's limit, 2^-40 of the largest still has a bit
+constexpr float TILE_BIAS = 15.f, TILE_FALL = 8.f;  // see ATTN_BIAS; the reference is no less than a tile's maximum, and no more than 9 above it
 constexpr int JOIN_PARTS = 160;    // parts that an item can have: CTAs of a launch
 constexpr int RING = 4;            // tiles' and items' words in shared memory: the roles are never further apart
 
@@ -56,7 +56,7 @@ struct TilesShape {
   static constexpr int SMEM = 1024 + 2 * QPIECE + 2 * BUFS * TILE + OUT + SMALL;
   static_assert(SMEM + 2048 <= 232448, "more shared memory than a CTA has");
   // registers by role: together as many as the launch has
-  static constexpr int REG_W = HD <= 128 ? 104 : 112, REG_S = HD == 64 ? 168 : HD == 128 ? 208 : 160, REG_C = HD == 64 ? 128 : HD == 128 ? 96 : 80;
+  static constexpr int REG_W = HD == 128 ? 104 : 112, REG_S = HD == 64 ? 168 : HD == 128 ? 208 : 160, REG_C = HD == 64 ? 120 : HD == 128 ? 96 : 80;
   static_assert(REG_W * W_GROUPS + REG_S * S_GROUPS + REG_C <= 512, "more registers than the launch has");
 };
 
@@ -116,6 +116,12 @@ static __device__ __noinline__ float tile_odd_scores(const AttnParams& p, const 
     umma::tmem_st_32x1(sa + i, x);
   }
   return top;
+}
+
+// 64 scores at sa become what they are above the reference.
+static __device__ __noinline__ void tile_far_scores(uint32_t sa, float f, float ref) {
+#pragma unroll 1
+  for (int i = 0; i < 64; ++i) umma::tmem_st_32x1(sa + i, __fadd_rn(__fmul_rn(umma::tmem_ld_32x1(sa + i), f), -ref));
 }
 
 template <int HD>
@@ -454,7 +460,9 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
       const int to = it.pos0 + (row < n_rows ? attn_row_token(p, row) : 0);  // the row sees the keys from .. to
       const int from = attn_first_key(to, p.window);
       const bool busy = (warp & 3) * 32 < n_rows;  // (other rows' weights are whatever is there: they reach those rows' sums only)
-      float m = -CUDART_INF_F, l = 0.f;
+      float m = -CUDART_INF_F, l = 0.f;  // reference, weights
+      float* highest = s_l + ((item % Sh::ENDS) * GROUPS + wg) * 128 + row;  // of the references that it fell from: where the weights go at the end
+      *highest = m;
       int ks = it.key0 + 64 * wg;
       int stop = n1 < N ? max(n, n1 - 2) : n1;  // where the next item's q is turned
 #pragma unroll 1
@@ -477,7 +485,7 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
               if (masked) hide(s, seen);
               float t[2] = {top, -CUDART_INF_F};
 #pragma unroll
-              for (int i = 0; i < 32; i += 2) t[(i >> 1) & 1] = max_nan(max_nan(t[(i >> 1) & 1], s[i]), s[i + 1]);
+              for (int i = 0; i < 32; i += 2) t[(i >> 1) & 1] = max_nan(t[(i >> 1) & 1], s[i], s[i + 1]);
               top = max_nan(t[0], t[1]);
             }
             const bool put_right = top != top && row < n_rows && l == l;  // (a row that is NaN already stays that)
@@ -489,12 +497,22 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
             asm volatile("bar.sync %0, 64;" ::"r"(2 + (warp & 3)) : "memory");  // (the two warps of these rows)
             top = fmaxf(top, at[128 * (wg ^ 1)]);
           }
-          const float now = fmaxf(m, top * f);
+          const float t = top * f;  // (a NaN leaves the reference where it is)
+          float now = t > m ? ceilf(t) : m;
+          if (t < m - TILE_FALL && t > -CUDART_INF_F) {  // down, but only as far as leaves the sums in range
+            const float h = fmaxf(*highest, m);
+            *highest = h;
+            now = fmaxf(ceilf(t), h - 60.f);
+          }
           l *= exp2_rel(m, now);
           m = now;
           if (busy) {
-            const float off = TILE_BIAS - (now == -CUDART_INF_F ? 0.f : now);
-            const float2 f2 = make_float2(f, f), off2 = make_float2(off, off), minus = make_float2(-1.f, -1.f);
+            // Scores past 2^22 lose the bias in one step (and weights past 2^16 f16's range): product, difference and bias one after the other for them
+            const float ref = now == -CUDART_INF_F ? 0.f : now;
+            const bool far = __any_sync(0xFFFFFFFFu, fabsf(ref) > 4194304.f && row < n_rows);
+            const float ff = far ? 1.f : f, off = far ? TILE_BIAS : TILE_BIAS - ref;
+            if (far) tile_far_scores(sa, f, ref);
+            const float2 f2 = make_float2(ff, ff), off2 = make_float2(off, off), minus = make_float2(-1.f, -1.f);
             float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll 1
             for (int j = 0; j < 64; j += 32) {
@@ -524,7 +542,7 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
           umma::fence_before_sync();
           if (wg == 0) s_ref[(n & (RING - 1)) * 128 + row] = m;
           if (n + 1 == n1) {
-            s_l[((item % Sh::ENDS) * GROUPS + wg) * 128 + row] = l;
+            *highest = l;
             if (wg == 0) s_end[(item % Sh::ENDS) * 128 + row] = m;
           }
           __syncwarp();

@@ -1,6 +1,7 @@
 """GPU: rope_kv and attention at the ends of what their arguments may be, against the formulas in 64 bits (tolerances as in
 test_gpu_attention.py unless a test derives its own)."""
 import dataclasses
+import math
 
 import pytest
 
@@ -169,3 +170,94 @@ def test_infinite_keys_count_by_their_scores(backend, path, page, H, K, hd, n, s
     b.put(b.k, 0, k)
     want = check(backend, b, scale=scale * hd ** -0.5, path=path)[:, : H * hd].view(-1, H, hd)
     assert bool(want[n // 2 : n, : H // K].isnan().all()) and (n // 2 < 3 or bool(want[2 : n // 2].isfinite().all()))
+
+
+@pytest.mark.parametrize("H,K,hd,n,lens", [(4, 1, 64, 1, [4096] * 160), (4, 1, 64, 3, [131072]), (8, 1, 128, 1, [2500] * 150), (2, 1, 256, 1, [3000] * 150), (8, 2, 128, 40, [9000, 700]),
+                                           (2, 2, 192, 100, [3000]), (4, 1, 64, 130, [20000])])
+@pytest.mark.parametrize("path", [1, 2])
+@pytest.mark.parametrize("above", [5, 20, 33, 45, 70])
+def test_a_sink_leaves_the_others_their_accuracy(backend, path, H, K, hd, n, lens, above):
+    # one key 2^above times as heavy as any other, of value zero: what is left are the others.  A weight is known to 2^-25 and at least 2^-5 where the
+    # reference has fallen to its neighbours (2^-20 of it), the exponential to 2^-20; the sums have kv / 64 steps of the tensor cores in a warp, or of tiles, 2^-23
+    # each.  The keys that share the sink's reference are known to 2^-25 of its weight, which is all but the whole: the other 127 of its tile, 2^15, or those of four
+    # slices of 16 after which a warp looks down, 2^10; their values go up to 1.5.  (Otherwise all of a warp's or a part's keys were off by that.)
+    b = Batch([n] * len(lens), [x - n for x in lens], H, K, hd, page=64, seed=above)
+    b.q.zero_()
+    b.q[:, 0 : H * hd : hd] = 1.0
+    b.q[:, 1 : H * hd : hd] = 0.25
+    for s, kv in enumerate(lens):
+        k, v = b.get(b.k, s).clone(), b.get(b.v, s).clone()
+        k[:, :, 0] = 0.0
+        k[:, :, 1].clamp_(-2.0, 2.0)
+        v[:] = 1.0 + v.abs().clamp_(max=2.0) * 0.25
+        sink = (s * 37) % (kv - n)
+        k[sink, :, 0], k[sink, :, 1], v[sink] = above, 0.0, 0.0
+        b.put(b.k, s, k)
+        b.put(b.v, s, v)
+    want, _ = b.ref(scale=math.log(2.0))
+    backend.attention(b.op(backend, scale=math.log(2.0), path=path))
+    backend.sync()
+    off = ((b.out.double() - want).abs() - want * (2.0 ** -19 + max(lens) / 64 * 2.0 ** -23))[:, : H * hd].max()
+    assert float(off) <= 1.5 * (63 * 2.0 ** -35 if path == 1 else 127 * 2.0 ** -40), float(off)
+
+
+@pytest.mark.parametrize("H,K,hd,n,kv", [(8, 2, 64, 1, 900), (8, 1, 128, 2, 5000), (4, 1, 256, 1, 300), (8, 2, 128, 100, 700), (2, 1, 192, 150, 300)])
+@pytest.mark.parametrize("path", [1, 2])
+@pytest.mark.parametrize("e", [12, 13, 14, 15, 17, 20, 25, 60])
+@pytest.mark.parametrize("scale", [math.log(2.0), 0.37, -0.37])
+def test_scores_of_any_size(backend, path, H, K, hd, n, kv, e, scale):
+    # scores of 2047 x 2^e: keys that tie share the weight; those a step below have none, and where f32 still tells powers of two apart, theirs
+    import torch
+
+    b = Batch([n, 1], [kv, kv // 3], H, K, hd, page=16, seed=e)
+    b.q.zero_()
+    b.q[:, 0 : H * hd : hd] = 2.0 ** e
+    near = e == 12 and scale == math.log(2.0)
+    if near:
+        b.q[:, 1 : H * hd : hd] = 1.0
+    g = torch.Generator(device="cuda").manual_seed(3)
+    for s in range(2):
+        k = b.get(b.k, s).clone()
+        pick = torch.randint(0, 7, (b.kv[s], K), generator=g, device="cuda")
+        k[:, :, 0] = 2047.0 if near else torch.where(pick < 2, 2047.0, 2046.0 - pick).half()
+        k[:, :, 1] = -pick.half()
+        k[0, :, 0], k[0, :, 1] = 2047.0, 0.0
+        if scale < 0:
+            k[:, :, 0] *= -1
+        b.put(b.k, s, k)
+    want, _ = b.ref(scale=scale)
+    backend.attention(b.op(backend, scale=scale, path=path))
+    backend.sync()
+    # weights to 2^-20 and two pieces, kv / 64 steps of sums
+    off = (b.out.double() - want)[:, : H * hd].abs().max()
+    assert float(off) <= float(b.v.nan_to_num().abs().max()) * (2.0 ** -18 + kv / 64 * 2.0 ** -23), float(off)
+
+
+@pytest.mark.parametrize("kv,hd,n,H", [(2000, 64, 9, 12), (140_000, 64, 9, 12), (140_000, 64, 1, 4), (30_000, 128, 32, 4), (70_000, 192, 2, 20), (20_000, 256, 20, 6), (70_000, 16, 128, 1), (131_072, 128, 1, 8)])
+@pytest.mark.parametrize("path", [1, 2])
+def test_no_part_of_an_item_is_lost_or_weighed_wrong(backend, path, kv, hd, n, H):
+    # keys of 128 by 128 count in a column of their own, in turn, with weights of 2^-2 .. 2^2 by the 128: all of it powers of two, whose sums f32 holds without
+    # rounding within a part.  What is left: half a step at each of up to 160 parts' sums, the division, and the exponential's 2^-22 where they meet.
+    import torch
+
+    b = Batch([n], [kv - n], H, 1, hd, page=64, seed=hd)
+    b.q.zero_()
+    b.q[:, 0 : H * hd : hd] = 1.0
+    i = torch.arange(kv, device="cuda") // 128
+    level = (i * 7 + i // 5) % 5 - 2
+    k, v = torch.zeros(kv, 1, hd, device="cuda", dtype=torch.float16), torch.zeros(kv, 1, hd, device="cuda", dtype=torch.float16)
+    k[:, 0, 0] = level.half()
+    v[torch.arange(kv, device="cuda"), 0, i % hd] = 1.0
+    b.put(b.k, 0, k)
+    b.put(b.v, 0, v)
+    want, _ = b.ref(scale=math.log(2.0))
+    backend.attention(b.op(backend, scale=math.log(2.0), path=path))
+    backend.sync()
+    rel = 160 * 2.0 ** -24 + 2.0 ** -20
+    got, want = b.out.double()[:, : H * hd], want[:, : H * hd]
+    assert bool(((got - want).abs() <= rel * want).all()), float(((got - want).abs() / want.clamp(min=1e-9)).max())
+    # without any 128 of the keys: a hundred times the bound at least
+    weight = torch.pow(2.0, level.double())
+    column = torch.zeros(hd, dtype=torch.float64, device="cuda").index_add_(0, i % hd, weight)
+    part = torch.zeros(int(i[-1]) + 1, dtype=torch.float64, device="cuda").index_add_(0, i, weight)
+    assert float((part / column[torch.arange(len(part), device="cuda") % hd])[:-1].min()) > 100 * rel
