@@ -461,8 +461,9 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
       const int from = attn_first_key(to, p.window);
       const bool busy = (warp & 3) * 32 < n_rows;  // (other rows' weights are whatever is there: they reach those rows' sums only)
       float m = -CUDART_INF_F, l = 0.f;  // reference, weights
-      float* highest = s_l + ((item % Sh::ENDS) * GROUPS + wg) * 128 + row;  // of the references that it fell from: where the weights go at the end
-      *highest = m;
+      // of the references that it fell from: where the weights go at the end (written behind a wait for the item's scores, not before: the sums have
+      // read what an item ahead left there by then)
+      float* highest = s_l + ((item % Sh::ENDS) * GROUPS + wg) * 128 + row;
       int ks = it.key0 + 64 * wg;
       int stop = n1 < N ? max(n, n1 - 2) : n1;  // where the next item's q is turned
 #pragma unroll 1
@@ -497,6 +498,7 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
             asm volatile("bar.sync %0, 64;" ::"r"(2 + (warp & 3)) : "memory");  // (the two warps of these rows)
             top = fmaxf(top, at[128 * (wg ^ 1)]);
           }
+          if (m == -CUDART_INF_F) *highest = m;
           const float t = top * f;  // (a NaN leaves the reference where it is)
           float now = t > m ? ceilf(t) : m;
           if (t < m - TILE_FALL && t > -CUDART_INF_F) {  // down, but only as far as leaves the sums in range

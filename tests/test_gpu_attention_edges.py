@@ -240,6 +240,8 @@ def test_no_part_of_an_item_is_lost_or_weighed_wrong(backend, path, kv, hd, n, H
     # rounding within a part.  What is left: half a step at each of up to 160 parts' sums, the division, and the exponential's 2^-22 where they meet.
     import torch
 
+    if path == 1 and H > 16:
+        pytest.skip("more query heads to a kv head than the few-rows kernel takes")
     b = Batch([n], [kv - n], H, 1, hd, page=64, seed=hd)
     b.q.zero_()
     b.q[:, 0 : H * hd : hd] = 1.0
