@@ -351,8 +351,9 @@ int32_t infr_cuda_add(infr_cuda_ctx* ctx, const infr_cuda_buf* a, const infr_cud
  *
  * All of these arrays are read on the device when the call runs, so a recorded plan follows new lengths and tables written into the same
  * buffers.  What they say is checked there: a row number outside the call, a length past max_pages * page_size or a page outside
- * [0, n_pages) is forced into range (a page that is not there is read as page 0, and not written), and the next infr_cuda_sync /
- * download fails with INVALID_ARG.  Page table entries past a sequence's length are not read.
+ * [0, n_pages) is forced into range (a page that is not there is read as page 0, and not written), attention leaves a batch out whose cu_q is so far out of
+ * order that it makes more rows than the call has, and the next infr_cuda_sync / download fails with INVALID_ARG.  Page table entries past a
+ * sequence's length are not read.
  *
  * n_seq: up to 4096.  head_dim: a multiple of 16 up to 256.  n_head: a multiple of n_kv, up to 128 query heads to each; query head h reads kv head
  * h / (n_head / n_kv).  page_size: a multiple of 16.  Strides are in values between rows, a multiple of 4 up to 2^24, 0 for rows side by side
@@ -383,9 +384,13 @@ typedef struct infr_cuda_rope_kv_desc {
 int32_t infr_cuda_rope_kv(infr_cuda_ctx* ctx, const infr_cuda_rope_kv_desc* desc);
 
 /* out[r, h, :] = sum_j w_j v_j,  w = softmax_j(scale * q[r, h, :] . k_j)  over the keys j of the row's sequence with
- * position(r) - window < j <= position(r)  (window 0: all j <= position(r)); a row that sees no key gets zeros.
- * f32 accuracy: q and the weights enter the tensor cores as two f16 pieces each, sums are f32.  Keys and values that a row may not
- * see do not reach it, whatever bits they hold. */
+ * position(r) - window < j <= position(r)  (window 0: all j <= position(r)); a row that sees no key, or none whose score is above
+ * -inf, gets zeros.
+ * f32 accuracy: q and the weights enter the tensor cores as two f16 pieces each, sums are f32.  A weight is off by 2^-20 of itself or of
+ * the largest of the 16 keys that it stands among, and by 2^-34 at most of the largest of the few tens (or 128) that are worked on with it.
+ * Keys and values that a row may not see do not reach it, whatever bits they hold.  What it sees and is not finite counts as in the formula, however the call
+ * is cut into parts: a key whose score is -inf has no weight, one whose score is NaN or +inf makes the row NaN, and a value that is not finite makes its column that
+ * (NaN where there are infinities of both signs), however small its weight. */
 typedef struct infr_cuda_attention_desc {
   const infr_cuda_buf* q;            /* [rows, n_head, head_dim] f32, rows q_stride apart                     */
   const infr_cuda_buf *k, *v;        /* f16, pages or packed rows                                             */
@@ -394,8 +399,10 @@ typedef struct infr_cuda_attention_desc {
   uint32_t rows, n_seq, n_head, n_kv, head_dim;
   uint32_t n_pages, page_size, max_pages;              /* 0 for packed rows                                   */
   uint32_t q_stride, out_stride;
-  uint32_t max_q;                    /* rows of a sequence at most, as far as the caller knows (0: `rows`).  Only
-                                        the choice of kernel goes by it: results do not                       */
+  uint32_t max_q;                    /* rows of a sequence at most, as far as the caller knows.  0 stands for `rows`,
+                                        which single tokens of many sequences should not be taken for: give 1
+                                        for them.  Only the choice of kernel goes by it: results do not, but
+                                        for their rounding                                                    */
   uint32_t window;                   /* keys that a row sees at most; 0 = all before it                       */
   float scale;                       /* usually head_dim^-0.5                                                 */
   uint32_t path;                     /* 0 = choose; 1 = the few-rows kernel (up to 16 query heads to a kv head);

@@ -427,7 +427,7 @@ class Attention:
     max_pages: int = 0
     q_stride: int = 0
     out_stride: int = 0
-    max_q: int = 0  # longest sequence of new rows, as far as known: picks the kernel, not the results
+    max_q: int = 0  # longest sequence of new rows, as far as known (1 for a decode step; 0 counts as all rows): picks the kernel, not the results
     window: int = 0
     path: int = 0  # 0 auto, 1 few-rows kernel, 2 tensor-memory kernel
 

@@ -53,7 +53,7 @@ class StackAttention:
     page_table: torch.Tensor
     page_size: int
     caches: List[tuple]
-    max_q: int = 0
+    max_q: int = 0  # longest sequence of new rows, as far as known (1 for a decode step): picks the kernel
     window: int = 0
     rope_base: float = 1e4
     n_rot: Optional[int] = None  # whole heads unless given
@@ -165,6 +165,8 @@ class MoeStack:
             self.layer(li)
 
     def record(self) -> None:
+        """Records a step for `replay`.  Runs one first, on what `hidden` holds: with attention it writes keys and values into the caller's pages, as any step
+        does (of the tokens that kv_len and cu_q say; the step that is replayed for these writes the same places)."""
         self.step()  # scratch sized, kernels loaded
         self.be.sync()
         self.be.graph_begin()
