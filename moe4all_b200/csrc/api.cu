@@ -174,10 +174,13 @@ int32_t drain_and_poll(infr_cuda_ctx* ctx, const char* what) {
   if (tag || bad) {
     st->timeout = 0;
     st->bad_index = 0;
-    // a router launch that gave up may have left logits behind: every word back to "not written yet"
-    if (tag && ctx->route_logits) cudaMemset(ctx->route_logits, 0xFF, ROUTE_LOGIT_BYTES);
+    // a router launch that gave up may have left logits behind: every word back to "not written yet" (ahead of the next launch, which does not wait
+    // for what other streams do)
+    DeviceGuard g(ctx->device);
+    if (tag && ctx->route_logits) cudaMemsetAsync(ctx->route_logits, 0xFF, ROUTE_LOGIT_BYTES, ctx->stream);
     // and an attention launch join counters
-    if (tag && ctx->attn_count) cudaMemset(ctx->attn_count, 0, ATTN_MAX_CTAS * sizeof(int));
+    if (tag && ctx->attn_count) cudaMemsetAsync(ctx->attn_count, 0, ATTN_MAX_CTAS * sizeof(int), ctx->stream);
+    if (tag) cudaStreamSynchronize(ctx->stream);
     if (tag) {
       char msg[96];
       std::snprintf(msg, sizeof msg, "a bounded device-side wait ran out (kernel tag %d); outputs of that call are invalid", tag);
@@ -219,9 +222,10 @@ int32_t infr_cuda_create(int32_t device, infr_cuda_ctx** out) {
       cudaHostAlloc(reinterpret_cast<void**>(&ctx->status_host), HOST_WORDS_BYTES, cudaHostAllocMapped) != cudaSuccess ||
       cudaHostGetDevicePointer(reinterpret_cast<void**>(&ctx->status), ctx->status_host, 0) != cudaSuccess ||
       cudaMalloc(&ctx->route_logits, ROUTE_LOGIT_BYTES) != cudaSuccess ||
-      cudaMemset(ctx->route_logits, 0xFF, ROUTE_LOGIT_BYTES) != cudaSuccess ||
+      cudaMemsetAsync(ctx->route_logits, 0xFF, ROUTE_LOGIT_BYTES, ctx->own_stream) != cudaSuccess ||
       cudaMalloc(&ctx->attn_count, ATTN_MAX_CTAS * sizeof(int)) != cudaSuccess ||
-      cudaMemset(ctx->attn_count, 0, ATTN_MAX_CTAS * sizeof(int)) != cudaSuccess) {
+      cudaMemsetAsync(ctx->attn_count, 0, ATTN_MAX_CTAS * sizeof(int), ctx->own_stream) != cudaSuccess ||
+      cudaStreamSynchronize(ctx->own_stream) != cudaSuccess) {  // (whatever stream the first launch is on)
     infr_cuda_destroy(ctx);
     return INFR_CUDA_ERR_CUDA;
   }
