@@ -295,11 +295,15 @@ static __device__ __noinline__ float attn_odd_score(const AttnParams& p, int s, 
   const __half* k = attn_value(p, p.k, s, q0, head, key);
   float sum = 0.f;
   bool found = false;
+#pragma unroll 2
+  for (int i = 0; i < p.hd; i += 8) {
+    const uint4 x = __ldcg(reinterpret_cast<const uint4*>(k + i));
+    if (only_finite(x.x) == x.x && only_finite(x.y) == x.y && only_finite(x.z) == x.z && only_finite(x.w) == x.w) continue;
 #pragma unroll 1
-  for (int i = 0; i < p.hd; ++i) {
-    const float x = __half2float(__ldcg(k + i));
-    if (fabsf(x) < CUDART_INF_F) continue;
-    sum += x * __ldcg(q + i);
+    for (int j = i; j < i + 8; ++j) {
+      const float y = __half2float(__ldcg(k + j));
+      if (!(fabsf(y) < CUDART_INF_F)) sum += y * __ldcg(q + j);
+    }
     found = true;
   }
   return found ? sum * p.scale_log2 : CUDART_NAN_F;

@@ -263,3 +263,33 @@ def test_no_part_of_an_item_is_lost_or_weighed_wrong(backend, path, kv, hd, n, H
     column = torch.zeros(hd, dtype=torch.float64, device="cuda").index_add_(0, i % hd, weight)
     part = torch.zeros(int(i[-1]) + 1, dtype=torch.float64, device="cuda").index_add_(0, i, weight)
     assert float((part / column[torch.arange(len(part), device="cuda") % hd])[:-1].min()) > 100 * rel
+
+
+@pytest.mark.parametrize("path", [1, 2])
+@pytest.mark.parametrize("K,n,rows,kv", [(8, 40, 4, 8192), (1, 1, 8, 100_000)])
+def test_long_contexts_of_infinite_keys_end_in_time(backend, path, K, n, rows, kv):
+    # one component of every key but the first has overflowed: by q's sign there a row is NaN, or sees the first key alone
+    import torch
+    from moe4all_b200 import Attention
+
+    hd, page, w = 128, 256, backend.wrap_tensor
+    g = torch.Generator(device="cuda").manual_seed(10)
+    pages = n * -(-kv // page)
+    k, v = (torch.randn(pages, K, page, hd, generator=g, device="cuda", dtype=torch.float16) for _ in range(2))
+    first = torch.arange(0, pages, pages // n, device="cuda")
+    keep = k[first, :, 0, hd - 1].clone()
+    k[..., hd - 1] = float("inf")
+    k[first, :, 0, hd - 1] = keep
+    q, out = torch.randn(n * rows, K * hd, generator=g, device="cuda"), torch.zeros(n * rows, K * hd, device="cuda")
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    cu, lens, table = i32([i * rows for i in range(n + 1)]), i32([kv] * n), i32(list(range(pages))).view(n, -1)
+    torch.cuda.synchronize()
+    backend.attention(Attention(q=w(q), k=w(k), v=w(v), out=w(out), scale=0.09, cu_q=w(cu), kv_len=w(lens), page_table=w(table), rows=n * rows, n_seq=n, n_head=K, n_kv=K,
+                                head_dim=hd, n_pages=pages, page_size=page, max_pages=pages // n, max_q=rows, path=path))
+    backend.sync()
+    plus = q.view(n, rows, K, hd)[..., hd - 1] > 0
+    got = out.view(n, rows, K, hd)
+    assert bool(got[plus].isnan().all())
+    # (the one key's weight is the whole: its value, by two f16 pieces and a division)
+    want = v[first, :, 0].float()[:, None].expand(n, rows, K, hd)
+    assert float((got - want)[~plus].abs().max()) <= float(v[first, :, 0].float().abs().max()) * 2.0 ** -20
