@@ -79,6 +79,19 @@ class BoundAttention:
 
     def __init__(self, attn: StackAttention, be: CudaBackend, rows: int, ne: int, eps: float, hidden: Buffer, device):
         H, K, hd = attn.n_head, attn.n_kv, attn.head_dim
+        # (the library sees addresses and bytes: types and shapes are seen here or not at all)
+        n_seq = attn.kv_len.numel()
+        for name, t in (("cu_q", attn.cu_q), ("kv_len", attn.kv_len), ("page_table", attn.page_table)):
+            if t.dtype != torch.int32:
+                raise ValueError(f"StackAttention.{name} must be int32, not {t.dtype}")
+        if attn.cu_q.numel() != n_seq + 1 or attn.page_table.dim() != 2 or attn.page_table.shape[0] != n_seq:
+            raise ValueError("StackAttention: cu_q is [n_seq + 1], kv_len [n_seq], page_table [n_seq, max_pages]")
+        if len(attn.layers) != len(attn.caches) or not attn.layers:
+            raise ValueError("StackAttention: a (k, v) pair of caches for each layer")
+        shape = (attn.caches[0][0].shape[0], K, attn.page_size, hd)
+        for c in (c for kv in attn.caches for c in kv):
+            if c.dtype != torch.float16 or tuple(c.shape) != shape:
+                raise ValueError(f"StackAttention: caches are float16 [n_pages, n_kv, page_size, head_dim], {shape} here, not {c.dtype} {tuple(c.shape)}")
         wide, w = (H + 2 * K) * hd, be.wrap_tensor
         self._be, self._layers, self._shape, self._hidden = be, attn.layers, (rows, ne, eps, wide, H * hd), hidden
         self._rows = [torch.zeros(rows, n, device=device) for n in (ne, wide, H * hd, H * hd, ne)]
@@ -86,12 +99,11 @@ class BoundAttention:
         self._out = out
         # (the parts of the wide rows: their memory is _rows')
         part = lambda first: be.wrap(self._rows[1].data_ptr() + 4 * first, 4 * (rows * wide - first))
-        n_pages = attn.caches[0][0].shape[0]
-        batch = dict(cu_q=w(attn.cu_q), kv_len=w(attn.kv_len), page_table=w(attn.page_table), rows=rows, n_seq=attn.kv_len.numel(), n_head=H, n_kv=K,
-                     head_dim=hd, n_pages=n_pages, page_size=attn.page_size, max_pages=attn.page_table.shape[1])
+        batch = dict(cu_q=w(attn.cu_q), kv_len=w(attn.kv_len), page_table=w(attn.page_table), rows=rows, n_seq=n_seq, n_head=H, n_kv=K,
+                     head_dim=hd, n_pages=shape[0], page_size=attn.page_size, max_pages=attn.page_table.shape[1])
         parts = part(0), part(H * hd), part((H + K) * hd)
         self._ops = []
-        for L, (k, v) in zip(attn.layers, attn.caches, strict=True):
+        for L, (k, v) in zip(attn.layers, attn.caches):
             opt = lambda t: None if t is None else w(t)
             kc, vc = w(k), w(v)
             self._ops.append((w(L.norm), RopeKv(q=parts[0], k=parts[1], v=parts[2], q_stride=wide, k_stride=wide, v_stride=wide, q_out=q, k_cache=kc, v_cache=vc,
@@ -141,6 +153,8 @@ class MoeStack:
                                    sh_down=b.get("sh_down"), sh_gate_inp=b.get("sh_gate_inp"),
                                    sh_ff=sh_ff if "sh_gate" in b else 0, **fuse, **route_kw))
         self.plan = None
+        if attn is not None and len(attn.layers) != len(layers):
+            raise ValueError(f"MoeStack: {len(layers)} layers, and attention for {len(attn.layers)}")
         self.attn = attn
         self._attn = None if attn is None else attn.bind(be, rows, ne, eps, self.b_hidden, dev)
 

@@ -98,6 +98,20 @@ def test_layer_of_the_attention_itself():
         dataclasses.replace(attn, max_q=1).layer(0)
 
 
+def test_arrays_and_caches_that_are_something_else_are_refused():
+    be = Notes()
+    ok = attention(be)
+    stack(be, 4, ok)
+    z, f16 = torch.zeros, torch.float16
+    pair = lambda *s, dtype=f16: (z(*s, dtype=dtype), z(*s, dtype=dtype))
+    for match, kw in (("kv_len must be int32", dict(kv_len=ok.kv_len.long())), ("cu_q must be int32", dict(cu_q=ok.cu_q.float())), ("page_table must be int32", dict(page_table=ok.page_table.long())),
+                      (r"cu_q is \[n_seq", dict(cu_q=ok.cu_q[:2])), (r"page_table \[n_seq", dict(page_table=ok.page_table.view(-1))), (r"page_table \[n_seq", dict(page_table=ok.page_table[:1])),
+                      ("a .k, v. pair", dict(caches=ok.caches[:1])), ("float16", dict(caches=[ok.caches[0], pair(20, PAGE, KV, HD)])), ("float16", dict(caches=[pair(20, KV, PAGE, HD, dtype=torch.float32)] * 2)),
+                      ("float16", dict(caches=[ok.caches[0], pair(19, KV, PAGE, HD)])), ("attention for 1", dict(layers=ok.layers[:1], caches=ok.caches[:1]))):
+        with pytest.raises(ValueError, match=match):
+            stack(be, 4, dataclasses.replace(ok, **kw))
+
+
 @pytest.mark.gpu
 def test_chunks_and_steps_over_one_attention(backend):
     """A prompt by one stack, then tokens by another (fused or not, recorded or not) over the same `StackAttention`, in turns: bit for bit what
