@@ -293,3 +293,28 @@ def test_long_contexts_of_infinite_keys_end_in_time(backend, path, K, n, rows, k
     # (the one key's weight is the whole: its value, by two f16 pieces and a division)
     want = v[first, :, 0].float()[:, None].expand(n, rows, K, hd)
     assert float((got - want)[~plus].abs().max()) <= float(v[first, :, 0].float().abs().max()) * 2.0 ** -20
+
+
+@pytest.mark.parametrize("H,K,hd,kv,n", [(8, 1, 128, 65536, 150), (16, 1, 64, 65536, 150), (4, 1, 256, 32768, 150), (8, 1, 192, 40000, 150), (2, 1, 128, 300_000, 1)])
+@pytest.mark.parametrize("path", [1, 2])
+def test_long_sums_of_one_sign(backend, path, H, K, hd, kv, n):
+    # equal weights of values of one sign: whatever a step of the sums loses adds up.  A whole item's are kv / 128 additions in f32, half a step each, of slices or tiles
+    # that the tensor cores sum in sixteen steps from zero; then pieces, division, joins.
+    import torch
+    from moe4all_b200 import Attention
+
+    page, w = 256, backend.wrap_tensor
+    g = torch.Generator(device="cuda").manual_seed(12)
+    pages = -(-kv // page)
+    k = torch.randn(pages, K, page, hd, generator=g, device="cuda", dtype=torch.float16)
+    v = (1.0 + 0.25 * torch.rand(pages, K, page, hd, generator=g, device="cuda")).half()
+    q, out = torch.zeros(n, H * hd, device="cuda"), torch.zeros(n, H * hd, device="cuda")
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    cu, lens, table = i32(list(range(n + 1))), i32([kv] * n), i32(list(range(pages))).expand(n, -1).contiguous()  # (all of them read the same pages)
+    torch.cuda.synchronize()
+    backend.attention(Attention(q=w(q), k=w(k), v=w(v), out=w(out), scale=0.1, cu_q=w(cu), kv_len=w(lens), page_table=w(table), rows=n, n_seq=n, n_head=H, n_kv=K,
+                                head_dim=hd, n_pages=pages, page_size=page, max_pages=pages, max_q=1, path=path))
+    backend.sync()
+    want = v.double().permute(0, 2, 1, 3).reshape(-1, K, hd)[:kv].mean(0).repeat_interleave(H // K, 0).view(-1)
+    off = ((out.double() - want) / want).abs().max()
+    assert float(off) <= kv / 128 * 2.0 ** -24 + 2.0 ** -19, float(off)
