@@ -82,7 +82,8 @@ const char* infr_cuda_last_error(const infr_cuda_ctx* ctx);
 const char* infr_cuda_name(void);
 /* Use an existing CUDA stream (a `cudaStream_t` passed as void*) instead of the context's own;
  * NULL restores the context's stream.  Lets a host that owns streams (PyTorch, NCCL) order the
- * kernels with its own work.  No counterpart in the reference (Vulkan queues are internal). */
+ * kernels with its own work.  The context's workspaces are shared by what runs on either: the host orders what is still queued
+ * on the former stream ahead of what comes on the new one (an event, or infr_cuda_sync first).  No counterpart in the reference (Vulkan queues are internal). */
 int32_t infr_cuda_set_stream(infr_cuda_ctx* ctx, void* cuda_stream);
 
 /* Tuning switches of a context, a plain struct read and written as a whole (the reference folds its
@@ -338,7 +339,7 @@ int32_t infr_cuda_add(infr_cuda_ctx* ctx, const infr_cuda_buf* a, const infr_cud
  * infr_cuda_rope_kv rotates q and k and puts k and v into the cache, infr_cuda_attention reads the cache, Linear and
  * Add bring the result back to the residual stream.
  *
- * Rows are f32, as everywhere here; the cache is f16, in one of two layouts:
+ * Rows are f32, as everywhere here; the cache is f16 (what is past its range becomes infinite there), in one of two layouts:
  *   pages   k, v: [n_pages, n_kv, page_size, head_dim]; page_table: [n_seq, max_pages] i32, token i of sequence s is token
  *           i % page_size of page page_table[s, i / page_size].  Pages may be shared by sequences that read them.
  *   packed  k, v: [rows, n_kv, head_dim], the call's own rows in their order; page_table and kv_len are NULL.  For prompts

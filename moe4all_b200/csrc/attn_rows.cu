@@ -9,9 +9,10 @@
 // q scaled by a power of two per row so that f16's range holds it): f32 results stay f32 results.
 //
 // Measured (us; K and V at the measured 6538 GB/s): 64 tokens over 700 - 8000 keys each (32 / 4 heads of 128, 429 MB) 85 (66), one token over
-// 131072 keys (268 MB) 58.8 (41), 16 tokens over up to 16000 keys (16 / 2 heads of 256, 257 MB) 57.5 (39), one token over 513 keys 10.7: what is
+// 131072 keys (268 MB) 60 (41), 16 tokens over up to 16000 keys (16 / 2 heads of 256, 257 MB) 59 (39), one token over 513 keys 10.8: what is
 // left is the kernel's two ends, about 3 us until the plan of the call is known, 3 until the first tiles are there and 3 for the join of
-// an item's parts; and, with heads of 256, a warp's own chain from tile to tile.
+// an item's parts; and, with heads of 256, a warp's own chain from tile to tile.  Nine to sixteen rows of heads of 192 and 256 do not fit the registers: 107 and 194
+// words a thread are spilled.
 #include "attn.cuh"
 
 namespace infr {

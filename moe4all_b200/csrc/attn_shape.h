@@ -107,8 +107,9 @@ INFR_ATTN_HD int attn_ctas(long long units, int grid, int most, int join) {
 
 // Whether the few-rows kernel serves a call of up to max_rows rows (tokens x g heads) to a (sequence, kv head), of which there are `pairs`.  Its
 // time grows with the rows past eight, the tile kernel's does not; but that one's ends are longer, which counts while every pair has many CTAs.
-// Measured (us, few-rows / tile kernel, heads of 128): 32 rows, 4 pairs of 16000 keys 28.9 / 40.7, 8 of 8000 29.3 / 35.7, 16 of 8000 43.2 / 39.0;
-// 16 rows, 16 pairs 31.3 / 33.4, 32 49.2 / 44.7 (heads of 64: 30.8 / 34.9; of 1000 keys 20.3 / 21.8), 128 of 4000 79.3 / 69.6; 8 rows, 128 56.8 / 65.3.
+// Measured (us, few-rows / tile kernel, heads of 128, 8000 keys): 32 rows, 4 pairs 26.8 / 35.0, 8 30.4 / 33.8, 16 42.7 / 36.3; 16 rows, 16 pairs 31.8 / 33.8,
+// 64 74.9 / 66.0; 8 rows, 128 pairs of 4000 keys 56.8 / 65.3.  16 rows and 32 pairs are the border, and one number for all: there heads of 64 take 34.1 / 36.7, of
+// 256 100.1 / 104.1, 1000 keys 21.1 / 22.5, but heads of 128 over 8000 keys 51.1 / 44.3 (8 sequences) and 44.7 / 41.8 (16): these lose up to a seventh.
 inline bool attn_few_rows(uint64_t max_rows, uint32_t g, uint64_t pairs) {
   return g <= (uint32_t)ATTN_ROWS_LIMIT && max_rows <= (pairs <= 8 ? 32u : pairs <= 32 ? 16u : 8u);
 }

@@ -4,7 +4,7 @@
 // a pair (row, key) costs 8 hd operations at the f16 rate.
 //
 // One CTA per SM, roles by warpgroup:
-//   weights   a thread per row and 64 keys (two groups for tiles of 128): scores S from tensor memory -> running maximum -> weights P, back
+//   weights   a thread per row and 64 keys (two groups for tiles of 128): scores S from tensor memory -> maximum, reference -> weights P, back
 //             over S as f16 pieces.  Both groups on one tile: what the MMAs wait for is a tile's weights, and with a tile to each
 //             group these took twice as long (3.3 against 1.7 thousand cycles; the tensor cores' part of a tile is 2.1)
 //   sums      a thread per row: the f32 sums in registers.  Each tile's P V starts from zero in tensor memory and is added here, brought
@@ -14,8 +14,9 @@
 // S and P of two tiles, and the sums of two (one for heads wider than 64), fill tensor memory: while a tile's weights are made the
 // tensor cores work on the next tile's scores and the last one's sums.
 //
-// Measured (us; the tensor cores' floor at 2 x 4 hd operations a pair and the measured 1666 TFLOP/s): 8192 tokens of 32 / 4 heads of 128 1036 (660),
-// four chunks of 512 tokens over up to 16000 keys 576 (366), 8192 tokens in 16 sequences of 64 / 8 heads of 64 225 (51).  What bounds it is
+// Measured (us; the tensor cores' floor at 2 x 4 hd operations a pair and the measured 1666 TFLOP/s): 8192 tokens of 32 / 4 heads of 128 1050 (660),
+// four chunks of 512 tokens over up to 16000 keys 590 (366), 8192 tokens in 16 sequences of 64 / 8 heads of 64 234 (51); the same chunks with 16 / 2 heads
+// of 192 343 (221), of 256 462 (219: one buffer each for K and V, 32 words a thread spilled).  What bounds it is
 // the weights: 3.0 thousand cycles a tile of 128 keys (maxima 0.6, powers of two and pieces 1.7, the rest waits), against 2.1 - 2.3 of MMAs.  Short
 // sequences of narrow heads pay per item: q into pieces 3 - 4 thousand cycles, results out 4 - 5, masked tiles on the diagonal.
 // Loops are kept rolled, and waits short: the roles share one instruction cache, and with every tile's code straight-line it hit 60% of
@@ -82,7 +83,7 @@ struct TileBars {
   uint64_t ready[4];    // all that step n of the MMAs needs: weights of tile n, its V there and looked after, its sums' columns free, K of tile n + 2
   uint64_t k_first[2];  // K of the first two tiles
   uint64_t o_full[2];
-  uint64_t a_full[RING];       // a tile's maxima (and, at an item's end, weights)
+  uint64_t a_full[RING];       // a tile's references (and, at an item's end, weights)
   uint64_t f_full[RING];       // an item's score factors
   uint64_t q_full, q_empty[RING];
 };
@@ -139,9 +140,9 @@ __global__ void __launch_bounds__(TilesShape<HD>::THREADS, 1)
   unsigned char* s_q = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   unsigned char *s_k = s_q + 2 * Sh::QPIECE, *s_v = s_k + BUFS * TILE;
   unsigned char* s_out = s_v + BUFS * TILE;
-  float* s_ref = reinterpret_cast<float*>(s_out + Sh::OUT);   // [RING][128] running maximum after a tile
+  float* s_ref = reinterpret_cast<float*>(s_out + Sh::OUT);   // [RING][128] reference after a tile
   float* s_fac = s_ref + RING * 128;                          // [RING][128] score factors by item
-  float* s_end = s_fac + RING * 128;                          // [ENDS][128] running maximum at an item's end
+  float* s_end = s_fac + RING * 128;                          // [ENDS][128] reference at an item's end
   float* s_l = s_end + Sh::ENDS * 128;                        // [ENDS][W_GROUPS][128] weights then
   float* s_max = s_l + Sh::ENDS * Sh::W_GROUPS * 128;         // [2][W_GROUPS][128] a tile's maxima by group
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
