@@ -318,3 +318,19 @@ def test_long_sums_of_one_sign(backend, path, H, K, hd, kv, n):
     want = v.double().permute(0, 2, 1, 3).reshape(-1, K, hd)[:kv].mean(0).repeat_interleave(H // K, 0).view(-1)
     off = ((out.double() - want) / want).abs().max()
     assert float(off) <= kv / 128 * 2.0 ** -24 + 2.0 ** -19, float(off)
+
+
+@pytest.mark.parametrize("path", [1, 2])
+@pytest.mark.parametrize("n", [1, 3, 150])
+def test_rows_whose_every_score_is_minus_infinity_get_zeros(backend, path, n):
+    # a window of one key, and of every second row's key a component that has overflowed against q's sign there: there is no weight to divide by
+    b = Batch([n, 2], [500, 9], 8, 2, 64, page=16, seed=n)
+    b.q[:, 0 : 8 * 64 : 64] = b.q[:, 0 : 8 * 64 : 64].abs() + 0.01
+    k = b.get(b.k, 0).clone()
+    k[::2, :, 0] = float("-inf")
+    b.put(b.k, 0, k)
+    backend.attention(b.op(backend, window=1, path=path))
+    backend.sync()
+    own = b.get(b.v, 0).double()[b.kv[0] - n :].repeat_interleave(4, 1).view(n, -1)  # (of the other rows their own value)
+    own[(b.kv[0] - n) % 2 :: 2] = 0.0
+    assert float((b.out[:n].double() - own).abs().max()) <= float(own.abs().max()) * 2.0 ** -20
