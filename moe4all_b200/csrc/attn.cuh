@@ -324,7 +324,7 @@ __device__ __forceinline__ uint32_t odd_pair(uint32_t x) {
 // zero, is NaN), or left out, in columns col0 .. of the result or part at dst, is put right: the sum of such values, whatever their weights.
 // Columns that came out finite can only miss values of tiles with hidden keys, where they count as zeros.
 // All lanes take part; those with a row are active: `to` its last key.  Keys by lane, 32 columns at a time, what is found noted in two words: other
-// warps of the CTA wait meanwhile, and their waits have a limit.  (A row's lane by itself took 3 - 50 us a key.)
+// warps of the CTA wait meanwhile, and their waits have a limit.  (A row's lane by itself waits for memory at every key, and at every value found.)
 // key0 .. key1: the keys of this part; full_lo .. full_hi: tiles inside have no hidden keys.
 static __device__ __forceinline__ void attn_odd_values(const AttnParams& p, int s, int q0, int head, int key0, int key1, int tile, int full_lo, int full_hi, bool active,
                                                     int to, int col0, int cols, float* dst) {
