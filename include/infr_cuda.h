@@ -36,6 +36,8 @@ extern "C" {
 /* Element / block types (crates/infr-core/src/tensor.rs:7-57), numbered as in the GGUF file
  * format so a loader can pass a tensor's type through unchanged. */
 #define INFR_CUDA_DT_F32 0
+#define INFR_CUDA_DT_F16 1   /* token tables only (infr_cuda_embed) */
+#define INFR_CUDA_DT_BF16 30 /* token tables only                   */
 #define INFR_CUDA_DT_Q4K 12 /* 256 weights / 144 B, crates/infr-core/src/decode_spec.rs:327 */
 #define INFR_CUDA_DT_Q6K 14 /* 256 weights / 210 B, crates/infr-core/src/decode_spec.rs:331 */
 #define INFR_CUDA_DT_Q8_0 8 /* 32 weights / 34 B, crates/infr-core/src/decode_spec.rs:320   */
@@ -410,6 +412,74 @@ typedef struct infr_cuda_attention_desc {
                                         2 = the tensor-memory kernel                                          */
 } infr_cuda_attention_desc;
 int32_t infr_cuda_attention(infr_cuda_ctx* ctx, const infr_cuda_attention_desc* desc);
+
+/* The same two over pages of 8 bits, half an f16 cache and a sixteenth:
+ *   codes   k_cache, v_cache (k, v): u8 [n_pages, n_kv, page_size, head_dim]
+ *   scales  k_scale, v_scale: u8 [n_pages, n_kv, page_size, head_dim / 16], a byte for 16 values
+ * A scale byte s is the f16 number d with the bits s << 7 (four significant bits), a code c the value (c - 128) d, which is an f16 number.
+ * rope_kv takes the least d with 127 d >= the largest magnitude of the 16, and the nearest codes: a value is off by d / 2 at most.  16 values of
+ * which one is not finite, or past 60960, get the scale byte 0xFF: none of them is a number then.  (Any byte from 0xC0 on says that.)  What attention
+ * makes of such keys and values it sees: a NaN score, and NaN in the 16 columns.
+ * Attention of few rows reads the codes; for many rows (infr_cuda_attention_desc.path) the pages that are seen are unpacked into f16 ones of the context's
+ * own first, which takes room for n_pages or n_seq * max_pages pages, whichever are fewer: made when a larger call comes, and not while recording. */
+int32_t infr_cuda_rope_kv_q8(infr_cuda_ctx* ctx, const infr_cuda_rope_kv_desc* desc, infr_cuda_buf* k_scale, infr_cuda_buf* v_scale);
+int32_t infr_cuda_attention_q8(infr_cuda_ctx* ctx, const infr_cuda_attention_desc* desc, const infr_cuda_buf* k_scale, const infr_cuda_buf* v_scale);
+
+/* Keys and values of a batch's rows out of the cache's pages: row r of sequence s is the token that rope_kv put there for it (the last tokens of kv_len[s]; to
+ * read a sequence whole, give it kv_len[s] rows).  Rows that are of no sequence stay as they were, rows with a negative position become zeros.
+ * The values are the cache's own: exact in f16 and in f32. */
+typedef struct infr_cuda_kv_read_desc {
+  const infr_cuda_buf *k_cache, *v_cache;  /* f16 pages, or codes                                             */
+  const infr_cuda_buf *k_scale, *v_scale;  /* NULL, or the codes' scales                                      */
+  infr_cuda_buf *k, *v;                    /* [rows, n_kv, head_dim], rows k_stride and v_stride apart        */
+  const infr_cuda_buf *cu_q, *kv_len, *page_table;
+  uint32_t rows, n_seq, n_kv, head_dim;
+  uint32_t n_pages, page_size, max_pages;
+  uint32_t k_stride, v_stride;             /* in values, a multiple of 16 bytes; 0 = rows side by side        */
+  uint32_t f16;                            /* 1: k and v are f16 rows, 0: f32                                 */
+} infr_cuda_kv_read_desc;
+int32_t infr_cuda_kv_read(infr_cuda_ctx* ctx, const infr_cuda_kv_read_desc* desc);
+
+/* ---- the two ends of a step -------------------------------------------------------------------------
+ *
+ * What makes a recorded step go from tokens to tokens without the host (Capabilities::embed_gather and gpu_sample of the reference,
+ * crates/infr-core/src/backend.rs): the ids that infr_cuda_sample writes are the ones that the next step's infr_cuda_embed reads. */
+
+/* dst[r, :] = scale * table[ids[r], :].  An id outside [0, n_vocab) gives a row of zeros, and the next infr_cuda_sync / download fails with
+ * INVALID_ARG. */
+typedef struct infr_cuda_embed_desc {
+  const infr_cuda_buf* table;  /* [n_vocab, ne] of dtype, GGUF blocks as they are in the file               */
+  const infr_cuda_buf* ids;    /* [rows] i32                                                                  */
+  infr_cuda_buf* dst;          /* [rows, ne] f32, rows dst_stride apart                                       */
+  int32_t dtype;               /* F32, F16, BF16 or a block format that an expert bank may have               */
+  uint32_t rows, ne, n_vocab;  /* ne: a multiple of 16, and of the format's block                             */
+  uint32_t dst_stride;         /* in values, a multiple of 4; 0 = rows side by side                           */
+  float scale;                 /* 1, or what the model multiplies its embeddings by                           */
+} infr_cuda_embed_desc;
+int32_t infr_cuda_embed(infr_cuda_ctx* ctx, const infr_cuda_embed_desc* desc);
+
+/* A token of each row of logits, by the row's own settings and a random number that the caller gives:
+ *   w_i   = exp((x_i - max x) / temperature)
+ *   kept    the top_k largest (of equal ones the lowest ids), of these the shortest run from the largest that has top_p of their weight, of these
+ *           the ones with w_i >= min_p
+ *   ids[r]  the first kept id whose weight and the kept ones' of lower ids are more than u times the kept ones' together
+ * Weights and sums are f64; weights below 2^-64 count as none.
+ * temperature: 0 or less (or NaN) takes the largest logit, of equal ones the lowest id; NULL: 1.  top_k: 0 or less keeps all.  top_p: 1 and above (or NaN)
+ * keeps all, 0 and below the largest.  min_p: 0 and below (or NaN) keeps all, at most 1 counts.  u: in [0, 1); 1 and above the last kept one, NaN or below 0
+ * the first.  Logits of -inf are never taken; among +inf ones all count alike and the others do not.  A row with a NaN, or with nothing above -inf, gives -1
+ * (and prob 0).  Each row's result depends on nothing but the row. */
+typedef struct infr_cuda_sample_desc {
+  const infr_cuda_buf* logits;       /* [rows, n_vocab] f32, rows `stride` apart                              */
+  const infr_cuda_buf* u;            /* [rows] f32                                                            */
+  const infr_cuda_buf* temperature;  /* [rows] f32, or NULL                                                   */
+  const infr_cuda_buf* top_k;        /* [rows] i32, or NULL                                                   */
+  const infr_cuda_buf *top_p, *min_p; /* [rows] f32, or NULL                                                  */
+  infr_cuda_buf* ids;                /* [rows] i32                                                            */
+  infr_cuda_buf* prob;               /* [rows] f32: the token's weight over the kept ones' together, or NULL  */
+  uint32_t rows, n_vocab;
+  uint32_t stride;                   /* in values, any; 0 = rows side by side                                 */
+} infr_cuda_sample_desc;
+int32_t infr_cuda_sample(infr_cuda_ctx* ctx, const infr_cuda_sample_desc* desc);
 
 /* ---- expert parallelism (crates/infr-vulkan/src/ep.rs:1-53, 156-505) ---------------------------- */
 

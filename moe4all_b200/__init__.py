@@ -8,5 +8,5 @@ interface for that path: `CudaBackend` follows `infr_core::backend::Backend`
 every call raises.
 """
 from .backend import (  # noqa: F401
-    Activation, Attention, BackendError, Buffer, Config, CudaBackend, DType, MoeFfn, MoeGating, RopeKv, Unsupported, load_library,
+    Activation, Attention, BackendError, Buffer, Config, CudaBackend, DType, Embed, KvRead, MoeFfn, MoeGating, RopeKv, Sample, Unsupported, load_library,
 )

@@ -31,6 +31,7 @@ EXPORTS = [
     "infr_cuda_gguf_meta_u64", "infr_cuda_gguf_meta_f64", "infr_cuda_gguf_meta_str", "infr_cuda_gguf_upload",
     "infr_cuda_sync", "infr_cuda_moe_ffn", "infr_cuda_moe_route", "infr_cuda_linear",
     "infr_cuda_rope_kv", "infr_cuda_attention",
+    "infr_cuda_rope_kv_q8", "infr_cuda_attention_q8", "infr_cuda_kv_read", "infr_cuda_embed", "infr_cuda_sample",
     "infr_cuda_gated_act", "infr_cuda_moe_shared_add", "infr_cuda_rmsnorm", "infr_cuda_add",
     "infr_cuda_moe_expert_rows", "infr_cuda_launch_count", "infr_cuda_em_down_ctas_per_sm",
     "infr_cuda_graph_begin", "infr_cuda_graph_end", "infr_cuda_graph_launch", "infr_cuda_graph_free", "infr_cuda_set_trace", "infr_cuda_moe_route_noalloc", "infr_cuda_moe_combine", "infr_cuda_umma_selftest",
@@ -56,6 +57,8 @@ class Unsupported(BackendError):
 class DType(enum.IntEnum):
     """crates/infr-core/src/tensor.rs:7-57, numbered as in the GGUF file format."""
     F32 = 0
+    F16 = 1    # token tables only
+    BF16 = 30  # token tables only
     Q4_0 = 2
     Q4_1 = 3
     Q5_0 = 6
@@ -80,6 +83,8 @@ class DType(enum.IntEnum):
         """crates/infr-core/src/decode_spec.rs:315-335: elements and bytes per block."""
         if self is DType.F32:
             return n_elem * 4
+        if self in (DType.F16, DType.BF16):
+            return n_elem * 2
         elems, nbytes = {DType.Q8_0: (32, 34), DType.Q4K: (256, 144), DType.Q5K: (256, 176), DType.Q6K: (256, 210),
                          DType.IQ4NL: (32, 18), DType.IQ4XS: (256, 136), DType.Q4_0: (32, 18), DType.Q4_1: (32, 20),
                          DType.Q5_0: (32, 22), DType.Q5_1: (32, 24), DType.Q2K: (256, 84), DType.Q3K: (256, 110), DType.MXFP4: (32, 17),
@@ -135,6 +140,21 @@ class _AttentionDesc(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v", "out", "cu_q", "kv_len", "page_table")] + [
         (n, C.c_uint32) for n in ("rows", "n_seq", "n_head", "n_kv", "head_dim", "n_pages", "page_size", "max_pages", "q_stride", "out_stride", "max_q",
                                   "window")] + [("scale", C.c_float), ("path", C.c_uint32)]
+
+
+class _KvReadDesc(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("k_cache", "v_cache", "k_scale", "v_scale", "k", "v", "cu_q", "kv_len", "page_table")] + [
+        (n, C.c_uint32) for n in ("rows", "n_seq", "n_kv", "head_dim", "n_pages", "page_size", "max_pages", "k_stride", "v_stride", "f16")]
+
+
+class _EmbedDesc(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("table", "ids", "dst")] + [("dtype", C.c_int32)] + [(n, C.c_uint32) for n in ("rows", "ne", "n_vocab", "dst_stride")] + [
+        ("scale", C.c_float)]
+
+
+class _SampleDesc(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("logits", "u", "temperature", "top_k", "top_p", "min_p", "ids", "prob")] + [
+        (n, C.c_uint32) for n in ("rows", "n_vocab", "stride")]
 
 
 class Config(C.Structure):
@@ -200,6 +220,11 @@ def load_library(path: Optional[str] = None):
     L.infr_cuda_linear.argtypes = [vp, i32, vp, vp, vp, u32, u32, u32]
     L.infr_cuda_rope_kv.argtypes = [vp, C.POINTER(_RopeKvDesc)]
     L.infr_cuda_attention.argtypes = [vp, C.POINTER(_AttentionDesc)]
+    L.infr_cuda_rope_kv_q8.argtypes = [vp, C.POINTER(_RopeKvDesc), vp, vp]
+    L.infr_cuda_attention_q8.argtypes = [vp, C.POINTER(_AttentionDesc), vp, vp]
+    L.infr_cuda_kv_read.argtypes = [vp, C.POINTER(_KvReadDesc)]
+    L.infr_cuda_embed.argtypes = [vp, C.POINTER(_EmbedDesc)]
+    L.infr_cuda_sample.argtypes = [vp, C.POINTER(_SampleDesc)]
     L.infr_cuda_gated_act.argtypes = [vp, vp, vp, vp, sz]
     L.infr_cuda_moe_shared_add.argtypes = [vp, vp, vp, vp, vp, u32, u32]
     L.infr_cuda_rmsnorm.argtypes = [vp, vp, vp, vp, u32, u32, C.c_float]
@@ -364,11 +389,17 @@ def _fill(desc, op, names):
     return desc
 
 
+def _both_scales(op):
+    if (op.k_scale is None) != (op.v_scale is None):
+        raise ValueError(f"{type(op).__name__}: k_scale and v_scale come together")
+
+
 @dataclass(frozen=True)
 class RopeKv:
     """New q, k and v rows of a batch on their way to attention: per-head RmsNorm (where the weights are given), rotary embedding of q and k,
-    k and v into the f16 cache - pages where `page_table` is given, packed rows otherwise (`infr_cuda_rope_kv_desc` in
-    include/infr_cuda.h says what each field is).  Frozen: the descriptor is made once and serves every call."""
+    k and v into the f16 cache - pages where `page_table` is given, packed rows otherwise - or, with `k_scale` and `v_scale`, into pages of 8 bits
+    (`infr_cuda_rope_kv_desc` and `infr_cuda_rope_kv_q8` in include/infr_cuda.h say what each field is).  Frozen: the descriptor is made once and serves
+    every call."""
     q: Buffer
     k: Buffer
     v: Buffer
@@ -398,8 +429,11 @@ class RopeKv:
     q_norm: Optional[Buffer] = None
     k_norm: Optional[Buffer] = None
     norm_eps: float = 1e-6
+    k_scale: Optional[Buffer] = None  # u8 [n_pages, n_kv, page_size, head_dim / 16]: k_cache and v_cache are codes of 8 bits
+    v_scale: Optional[Buffer] = None
 
     def __post_init__(self):
+        _both_scales(self)
         d = _fill(_RopeKvDesc(), self, [n for n, _ in _RopeKvDesc._fields_ if n != "style"])
         d.style = int(bool(self.interleaved))
         object.__setattr__(self, "_desc", d)
@@ -407,8 +441,9 @@ class RopeKv:
 
 @dataclass(frozen=True)
 class Attention:
-    """Causal attention of a batch's new rows over its cache, or over packed f16 rows where `page_table` is not given
-    (`infr_cuda_attention_desc` in include/infr_cuda.h says what each field is).  Frozen: the descriptor is made once and serves every call."""
+    """Causal attention of a batch's new rows over its cache, or over packed f16 rows where `page_table` is not given; with `k_scale` and `v_scale` over
+    pages of 8 bits (`infr_cuda_attention_desc` and `infr_cuda_attention_q8` in include/infr_cuda.h say what each field is).  Frozen: the descriptor is made
+    once and serves every call."""
     q: Buffer
     k: Buffer
     v: Buffer
@@ -430,9 +465,80 @@ class Attention:
     max_q: int = 0  # longest sequence of new rows, as far as known (1 for a decode step; 0 counts as all rows): picks the kernel, not the results
     window: int = 0
     path: int = 0  # 0 auto, 1 few-rows kernel, 2 tensor-memory kernel
+    k_scale: Optional[Buffer] = None  # u8 [n_pages, n_kv, page_size, head_dim / 16]: k and v are codes of 8 bits
+    v_scale: Optional[Buffer] = None
 
     def __post_init__(self):
+        _both_scales(self)
         object.__setattr__(self, "_desc", _fill(_AttentionDesc(), self, [n for n, _ in _AttentionDesc._fields_]))
+
+
+@dataclass(frozen=True)
+class KvRead:
+    """Keys and values of a batch's rows out of pages, of f16 or (with `k_scale` and `v_scale`) of 8 bits, as f32 or f16 rows
+    (`infr_cuda_kv_read_desc` in include/infr_cuda.h says what each field is)."""
+    k_cache: Buffer
+    v_cache: Buffer
+    k: Buffer
+    v: Buffer
+    cu_q: Buffer
+    kv_len: Buffer
+    page_table: Buffer
+    rows: int
+    n_seq: int
+    n_kv: int
+    head_dim: int
+    n_pages: int
+    page_size: int
+    max_pages: int
+    k_scale: Optional[Buffer] = None
+    v_scale: Optional[Buffer] = None
+    k_stride: int = 0
+    v_stride: int = 0
+    f16: bool = False
+
+    def __post_init__(self):
+        d = _fill(_KvReadDesc(), self, [n for n, _ in _KvReadDesc._fields_ if n != "f16"])
+        d.f16 = int(bool(self.f16))
+        object.__setattr__(self, "_desc", d)
+
+
+@dataclass(frozen=True)
+class Embed:
+    """dst[r] = scale * table[ids[r]] (`infr_cuda_embed_desc` in include/infr_cuda.h)."""
+    table: Buffer
+    ids: Buffer
+    dst: Buffer
+    rows: int
+    ne: int
+    n_vocab: int
+    dtype: DType = DType.F32
+    scale: float = 1.0
+    dst_stride: int = 0
+
+    def __post_init__(self):
+        d = _fill(_EmbedDesc(), self, [n for n, _ in _EmbedDesc._fields_ if n != "dtype"])
+        d.dtype = int(self.dtype)
+        object.__setattr__(self, "_desc", d)
+
+
+@dataclass(frozen=True)
+class Sample:
+    """A token of each row of logits from given random numbers, settings by row (`infr_cuda_sample_desc` in include/infr_cuda.h)."""
+    logits: Buffer
+    u: Buffer
+    ids: Buffer
+    rows: int
+    n_vocab: int
+    temperature: Optional[Buffer] = None
+    top_k: Optional[Buffer] = None
+    top_p: Optional[Buffer] = None
+    min_p: Optional[Buffer] = None
+    prob: Optional[Buffer] = None
+    stride: int = 0
+
+    def __post_init__(self):
+        object.__setattr__(self, "_desc", _fill(_SampleDesc(), self, [n for n, _ in _SampleDesc._fields_]))
 
 
 class CudaBackend:
@@ -661,10 +767,25 @@ class CudaBackend:
         self._check(self._lib.infr_cuda_linear(self._ctx, int(dtype), w.handle, x.handle, y.handle, m, in_f, out_f))
 
     def rope_kv(self, op: RopeKv) -> None:
-        self._check(self._lib.infr_cuda_rope_kv(self._ctx, op._desc))
+        if op.k_scale is not None:
+            self._check(self._lib.infr_cuda_rope_kv_q8(self._ctx, op._desc, op.k_scale.handle, op.v_scale.handle))
+        else:
+            self._check(self._lib.infr_cuda_rope_kv(self._ctx, op._desc))
 
     def attention(self, op: Attention) -> None:
-        self._check(self._lib.infr_cuda_attention(self._ctx, op._desc))
+        if op.k_scale is not None:
+            self._check(self._lib.infr_cuda_attention_q8(self._ctx, op._desc, op.k_scale.handle, op.v_scale.handle))
+        else:
+            self._check(self._lib.infr_cuda_attention(self._ctx, op._desc))
+
+    def kv_read(self, op: KvRead) -> None:
+        self._check(self._lib.infr_cuda_kv_read(self._ctx, op._desc))
+
+    def embed(self, op: Embed) -> None:
+        self._check(self._lib.infr_cuda_embed(self._ctx, op._desc))
+
+    def sample(self, op: Sample) -> None:
+        self._check(self._lib.infr_cuda_sample(self._ctx, op._desc))
 
     def gated_act(self, gate: Buffer, up: Buffer, dst: Buffer, n: int) -> None:
         self._check(self._lib.infr_cuda_gated_act(self._ctx, gate.handle, up.handle, dst.handle, n))

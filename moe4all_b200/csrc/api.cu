@@ -186,6 +186,7 @@ int32_t drain_and_poll(infr_cuda_ctx* ctx, const char* what) {
       std::snprintf(msg, sizeof msg, "a bounded device-side wait ran out (kernel tag %d); outputs of that call are invalid", tag);
       return fail(ctx, INFR_CUDA_ERR_TIMEOUT, msg);
     }
+    if (bad == 3) return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "a token id outside [0, n_vocab) reached the embedding and got zeros; outputs of that call are invalid");
     if (bad == 2)
       return fail(ctx, INFR_CUDA_ERR_INVALID_ARG,
                   "a page, a row or a length outside its range reached an attention kernel and was forced into it; outputs of that call are invalid");
@@ -253,6 +254,8 @@ void infr_cuda_destroy(infr_cuda_ctx* ctx) {
   if (ctx->route_logits) cudaFree(ctx->route_logits);
   if (ctx->attn_count) cudaFree(ctx->attn_count);
   if (ctx->attn_parts) cudaFree(ctx->attn_parts);
+  if (ctx->kv_unpacked) cudaFree(ctx->kv_unpacked);
+  for (void* p : ctx->kv_unpacked_before) cudaFree(p);
   if (ctx->own_stream) cudaStreamDestroy(ctx->own_stream);
   delete ctx;
 }
@@ -1058,17 +1061,26 @@ AttnSizes attn_sizes(const Desc* d) {
   return {d->rows, d->n_seq, d->n_head, d->n_kv, d->head_dim, d->n_pages, d->page_size, d->max_pages, d->page_table != nullptr};
 }
 
-// What both calls check of a batch and its cache.
+// Scale bytes of a cache in 8 bits; both null: the cache is f16.
+struct KvScales {
+  const infr_cuda_buf *k, *v;
+  bool any() const { return k || v; }
+  uint32_t width() const { return any() ? 1 : 2; }  // bytes of a value
+};
+
+// What the calls check of a batch and its cache.
 template <class Desc>
-int32_t attn_check_batch(infr_cuda_ctx* ctx, const char* op, const Desc* d, const infr_cuda_buf* k, const infr_cuda_buf* v) {
-  const AttnSizes s = attn_sizes(d);
+int32_t attn_check_batch(infr_cuda_ctx* ctx, const char* op, const Desc* d, const AttnSizes& s, const infr_cuda_buf* k, const infr_cuda_buf* v, const KvScales& scales) {
   bool unsupported = false;
   const std::string name = std::string(op) + ": ";
   if (const char* why = attn_sizes_error(s, &unsupported)) return fail(ctx, unsupported ? INFR_CUDA_ERR_UNSUPPORTED : INFR_CUDA_ERR_INVALID_ARG, name + why);
   if ((d->kv_len != nullptr) != s.paged) return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, name + "kv_len and page_table come together");
+  if (scales.any() && !s.paged) return fail(ctx, INFR_CUDA_ERR_UNSUPPORTED, name + "a cache in 8 bits is one of pages");
   if (!fits(d->cu_q, ((size_t)d->n_seq + 1) * 4) || (s.paged && (!fits(d->kv_len, (size_t)d->n_seq * 4) || !fits(d->page_table, (size_t)d->n_seq * d->max_pages * 4))))
     return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, name + "cu_q, kv_len or page_table missing or too small");
-  if (!fits(k, attn_cache_bytes(s)) || !fits(v, attn_cache_bytes(s))) return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, name + "cache buffer missing or too small");
+  const uint64_t bytes = attn_cache_bytes(s, scales.width());
+  if (!fits(k, bytes) || !fits(v, bytes)) return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, name + "cache buffer missing or too small");
+  if (scales.any() && (!fits(scales.k, bytes / 16) || !fits(scales.v, bytes / 16))) return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, name + "scale buffer missing or too small");
   return INFR_CUDA_OK;
 }
 
@@ -1112,10 +1124,12 @@ void attn_batch_params(Params& p, infr_cuda_ctx* ctx, const Desc* d) {
 
 extern "C" {
 
-int32_t infr_cuda_rope_kv(infr_cuda_ctx* ctx, const infr_cuda_rope_kv_desc* d) {
-  if (!ctx) return INFR_CUDA_ERR_INVALID_ARG;
-  if (!d) return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "rope_kv: null descriptor");
-  int32_t rc = attn_check_batch(ctx, "rope_kv", d, d->k_cache, d->v_cache);
+}  // extern "C"
+
+namespace {
+
+int32_t rope_kv(infr_cuda_ctx* ctx, const infr_cuda_rope_kv_desc* d, const KvScales& scales) {
+  int32_t rc = attn_check_batch(ctx, "rope_kv", d, attn_sizes(d), d->k_cache, d->v_cache, scales);
   if (rc) return rc;
   if (d->n_rot % 8 || d->n_rot > d->head_dim) return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "rope_kv: n_rot must be a multiple of 8, at most head_dim");
   if (d->style > INFR_CUDA_ROPE_INTERLEAVED) return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "rope_kv: unknown style");
@@ -1134,7 +1148,7 @@ int32_t infr_cuda_rope_kv(infr_cuda_ctx* ctx, const infr_cuda_rope_kv_desc* d) {
       (rc = attn_check_rows(ctx, "rope_kv: q_out", d->q_out, d->rows, d->q_out_stride, wide_q, &p.qo_stride)))
     return rc;
   if (!d->rows) return INFR_CUDA_OK;
-  const uint64_t nq = attn_span(d->rows, p.qo_stride, wide_q) * 4, nc = attn_cache_bytes(attn_sizes(d));
+  const uint64_t nq = attn_span(d->rows, p.qo_stride, wide_q) * 4, nc = attn_cache_bytes(attn_sizes(d), scales.width());
   const bool in_place = d->q_out->ptr == d->q->ptr && p.qo_stride == p.q_stride;
   if (!in_place && (overlap(d->q_out, nq, d->q, attn_span(d->rows, p.q_stride, wide_q) * 4) || overlap(d->q_out, nq, d->k, attn_span(d->rows, p.k_stride, wide_kv) * 4) ||
                     overlap(d->q_out, nq, d->v, attn_span(d->rows, p.v_stride, wide_kv) * 4)))
@@ -1143,20 +1157,32 @@ int32_t infr_cuda_rope_kv(infr_cuda_ctx* ctx, const infr_cuda_rope_kv_desc* d) {
     for (const auto& [b, stride] : {std::pair{d->k, p.k_stride}, std::pair{d->v, p.v_stride}})
       if (attn_rows_meet(reinterpret_cast<uintptr_t>(d->q->ptr), wide_q * 4ull, p.q_stride * 4ull, reinterpret_cast<uintptr_t>(b->ptr), wide_kv * 4ull, stride * 4ull, d->rows))
         return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "rope_kv: q is rotated in place and k or v lies in its rows");
-  if (overlap(d->k_cache, nc, d->v_cache, nc) || overlap(d->k_cache, nc, d->q_out, nq) || overlap(d->v_cache, nc, d->q_out, nq))
-    return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "rope_kv: k_cache, v_cache and q_out must not overlap");
-  for (const infr_cuda_buf* c : {d->k_cache, d->v_cache})
-    if (overlap(c, nc, d->q, attn_span(d->rows, p.q_stride, wide_q) * 4) || overlap(c, nc, d->k, attn_span(d->rows, p.k_stride, wide_kv) * 4) ||
-        overlap(c, nc, d->v, attn_span(d->rows, p.v_stride, wide_kv) * 4))
+  const std::pair<const infr_cuda_buf*, uint64_t> written[4] = {{d->k_cache, nc}, {d->v_cache, nc}, {scales.k, nc / 16}, {scales.v, nc / 16}};
+  const int n_written = scales.any() ? 4 : 2;
+  for (int i = 0; i < n_written; ++i) {
+    const auto& [c, bytes] = written[i];
+    for (int j = 0; j < i; ++j)
+      if (overlap(c, bytes, written[j].first, written[j].second)) return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "rope_kv: the parts of the cache must not overlap");
+    if (overlap(c, bytes, d->q_out, nq)) return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "rope_kv: k_cache, v_cache and q_out must not overlap");
+    if (overlap(c, bytes, d->q, attn_span(d->rows, p.q_stride, wide_q) * 4) || overlap(c, bytes, d->k, attn_span(d->rows, p.k_stride, wide_kv) * 4) ||
+        overlap(c, bytes, d->v, attn_span(d->rows, p.v_stride, wide_kv) * 4))
       return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "rope_kv: a cache overlaps the rows that go into it");
+  }
   DeviceGuard g(ctx->device);
   attn_batch_params(p, ctx, d);
   p.q = static_cast<const float*>(d->q->ptr);
   p.k = static_cast<const float*>(d->k->ptr);
   p.v = static_cast<const float*>(d->v->ptr);
   p.q_out = static_cast<float*>(d->q_out->ptr);
-  p.k_cache = static_cast<__half*>(d->k_cache->ptr);
-  p.v_cache = static_cast<__half*>(d->v_cache->ptr);
+  if (scales.any()) {
+    p.k_codes = static_cast<uint8_t*>(d->k_cache->ptr);
+    p.v_codes = static_cast<uint8_t*>(d->v_cache->ptr);
+    p.k_scale = static_cast<uint8_t*>(scales.k->ptr);
+    p.v_scale = static_cast<uint8_t*>(scales.v->ptr);
+  } else {
+    p.k_cache = static_cast<__half*>(d->k_cache->ptr);
+    p.v_cache = static_cast<__half*>(d->v_cache->ptr);
+  }
   p.q_norm = d->q_norm ? static_cast<const float*>(d->q_norm->ptr) : nullptr;
   p.k_norm = d->k_norm ? static_cast<const float*>(d->k_norm->ptr) : nullptr;
   p.freq_factors = d->freq_factors ? static_cast<const float*>(d->freq_factors->ptr) : nullptr;
@@ -1169,10 +1195,38 @@ int32_t infr_cuda_rope_kv(infr_cuda_ctx* ctx, const infr_cuda_rope_kv_desc* d) {
   return launch_rope_kv(ctx, p);
 }
 
-int32_t infr_cuda_attention(infr_cuda_ctx* ctx, const infr_cuda_attention_desc* d) {
-  if (!ctx) return INFR_CUDA_ERR_INVALID_ARG;
-  if (!d) return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "attention: null descriptor");
-  int32_t rc = attn_check_batch(ctx, "attention", d, d->k, d->v);
+// The f16 pages of a call over pages of 8 bits: grown like the scratch, but what a recorded plan may read from stays.
+int32_t ensure_unpacked(infr_cuda_ctx* ctx, uint64_t bytes) {
+  if (bytes > ctx->kv_unpacked_bytes) {
+    if (ctx->capturing) return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "attention: its f16 pages would have to be made while recording: run the call once un-recorded first");
+    cudaError_t e = cudaStreamSynchronize(ctx->stream);
+    if (e != cudaSuccess) return check_cuda(ctx, e, "attention: f16 pages: sync");
+    if (ctx->kv_unpacked && ctx->kv_unpacked_recorded) {
+      try {
+        ctx->kv_unpacked_before.push_back(ctx->kv_unpacked);
+      } catch (const std::bad_alloc&) {
+        return fail(ctx, INFR_CUDA_ERR_OOM, "attention: host out of memory");
+      }
+    } else if (ctx->kv_unpacked) {
+      cudaFree(ctx->kv_unpacked);
+    }
+    ctx->kv_unpacked = nullptr;
+    ctx->kv_unpacked_bytes = 0;
+    ctx->kv_unpacked_recorded = false;
+    e = cudaMalloc(&ctx->kv_unpacked, bytes);
+    if (e != cudaSuccess) {
+      ctx->kv_unpacked = nullptr;
+      cudaGetLastError();
+      return check_cuda(ctx, e, "attention: f16 pages of a cache in 8 bits");
+    }
+    ctx->kv_unpacked_bytes = bytes;
+  }
+  if (ctx->capturing) ctx->kv_unpacked_recorded = true;
+  return INFR_CUDA_OK;
+}
+
+int32_t attention(infr_cuda_ctx* ctx, const infr_cuda_attention_desc* d, const KvScales& scales) {
+  int32_t rc = attn_check_batch(ctx, "attention", d, attn_sizes(d), d->k, d->v, scales);
   if (rc) return rc;
   if (!std::isfinite(d->scale)) return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "attention: scale must be finite");
   if (d->path > 2) return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "attention: unknown path");
@@ -1184,14 +1238,22 @@ int32_t infr_cuda_attention(infr_cuda_ctx* ctx, const infr_cuda_attention_desc* 
       (rc = attn_check_rows(ctx, "attention: out", d->out, d->rows, d->out_stride, wide, &p.out_stride)))
     return rc;
   if (!d->rows) return INFR_CUDA_OK;
-  const uint64_t no = attn_span(d->rows, p.out_stride, wide) * 4, nc = attn_cache_bytes(attn_sizes(d));
-  if (overlap(d->out, no, d->q, attn_span(d->rows, p.q_stride, wide) * 4) || overlap(d->out, no, d->k, nc) || overlap(d->out, no, d->v, nc))
+  const uint64_t no = attn_span(d->rows, p.out_stride, wide) * 4, nc = attn_cache_bytes(attn_sizes(d), scales.width());
+  if (overlap(d->out, no, d->q, attn_span(d->rows, p.q_stride, wide) * 4) || overlap(d->out, no, d->k, nc) || overlap(d->out, no, d->v, nc) ||
+      (scales.any() && (overlap(d->out, no, scales.k, nc / 16) || overlap(d->out, no, scales.v, nc / 16))))
     return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "attention: out must not overlap q, k or v");
   DeviceGuard guard(ctx->device);
   attn_batch_params(p, ctx, d);
   p.q = static_cast<const float*>(d->q->ptr);
   p.out = static_cast<float*>(d->out->ptr);
-  p.v = static_cast<const __half*>(d->v->ptr);
+  if (scales.any()) {
+    p.kq = static_cast<const uint8_t*>(d->k->ptr);
+    p.vq = static_cast<const uint8_t*>(d->v->ptr);
+    p.ks = static_cast<const uint8_t*>(scales.k->ptr);
+    p.vs = static_cast<const uint8_t*>(scales.v->ptr);
+  } else {
+    p.v = static_cast<const __half*>(d->v->ptr);
+  }
   p.g = (int)g;
   p.g_inv = (65536 + g - 1) / g;
   p.window = attn_window(d->window, p.kv_len != nullptr ? (uint32_t)p.cap : d->rows);
@@ -1215,8 +1277,137 @@ int32_t infr_cuda_attention(infr_cuda_ctx* ctx, const infr_cuda_attention_desc* 
   }
   p.part = reinterpret_cast<float*>(ctx->attn_parts);
   p.part_ml = reinterpret_cast<float2*>(ctx->attn_parts + part);
-  const __half* k = static_cast<const __half*>(d->k->ptr);
-  return few ? launch_attn_rows(ctx, p, k, (int)(max_rows < 1024 ? max_rows : 1024)) : launch_attn_tiles(ctx, p, k);
+  const __half* k = scales.any() ? nullptr : static_cast<const __half*>(d->k->ptr);
+  if (few) return launch_attn_rows(ctx, p, k, (int)(max_rows < 1024 ? max_rows : 1024));
+  if (scales.any()) {
+    AttnUnpacked u;
+    if (!attn_unpacked(attn_sizes(d), &u)) return fail(ctx, INFR_CUDA_ERR_OOM, "attention: f16 pages of a cache in 8 bits past 2^48 bytes");
+    if ((rc = ensure_unpacked(ctx, u.table + 2 * u.side))) return rc;
+    int* table = u.by_sequence ? reinterpret_cast<int*>(ctx->kv_unpacked) : nullptr;
+    __half *kf = reinterpret_cast<__half*>(ctx->kv_unpacked + u.table), *vf = reinterpret_cast<__half*>(ctx->kv_unpacked + u.table + u.side);
+    if ((rc = launch_kv_unpack(ctx, p, kf, vf, table))) return rc;
+    if (table) p.page_table = table, p.n_pages = (int)u.pages;
+    k = kf, p.v = vf;
+  }
+  return launch_attn_tiles(ctx, p, k);
+}
+
+}  // namespace
+
+extern "C" {
+
+int32_t infr_cuda_rope_kv(infr_cuda_ctx* ctx, const infr_cuda_rope_kv_desc* d) {
+  if (!ctx) return INFR_CUDA_ERR_INVALID_ARG;
+  if (!d) return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "rope_kv: null descriptor");
+  return rope_kv(ctx, d, {nullptr, nullptr});
+}
+
+int32_t infr_cuda_rope_kv_q8(infr_cuda_ctx* ctx, const infr_cuda_rope_kv_desc* d, infr_cuda_buf* k_scale, infr_cuda_buf* v_scale) {
+  if (!ctx) return INFR_CUDA_ERR_INVALID_ARG;
+  if (!d || !k_scale || !v_scale) return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "rope_kv_q8: null descriptor or scale buffer");
+  return rope_kv(ctx, d, {k_scale, v_scale});
+}
+
+int32_t infr_cuda_attention(infr_cuda_ctx* ctx, const infr_cuda_attention_desc* d) {
+  if (!ctx) return INFR_CUDA_ERR_INVALID_ARG;
+  if (!d) return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "attention: null descriptor");
+  return attention(ctx, d, {nullptr, nullptr});
+}
+
+int32_t infr_cuda_attention_q8(infr_cuda_ctx* ctx, const infr_cuda_attention_desc* d, const infr_cuda_buf* k_scale, const infr_cuda_buf* v_scale) {
+  if (!ctx) return INFR_CUDA_ERR_INVALID_ARG;
+  if (!d || !k_scale || !v_scale) return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "attention_q8: null descriptor or scale buffer");
+  return attention(ctx, d, {k_scale, v_scale});
+}
+
+int32_t infr_cuda_kv_read(infr_cuda_ctx* ctx, const infr_cuda_kv_read_desc* d) {
+  if (!ctx) return INFR_CUDA_ERR_INVALID_ARG;
+  if (!d) return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "kv_read: null descriptor");
+  const KvScales scales = {d->k_scale, d->v_scale};
+  const AttnSizes sizes = {d->rows, d->n_seq, d->n_kv, d->n_kv, d->head_dim, d->n_pages, d->page_size, d->max_pages, d->page_table != nullptr};
+  int32_t rc = attn_check_batch(ctx, "kv_read", d, sizes, d->k_cache, d->v_cache, scales);
+  if (rc) return rc;
+  if (!sizes.paged) return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "kv_read: page_table missing");
+  const uint32_t wide = d->n_kv * d->head_dim, width = d->f16 ? 2 : 4, align = 16 / width;
+  const uint32_t ks = d->k_stride ? d->k_stride : wide, vs = d->v_stride ? d->v_stride : wide;
+  if (ks < wide || vs < wide || ks % align || vs % align)
+    return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "kv_read: a row stride is a multiple of 16 bytes and at least a row");
+  if (ks > (1u << 24) || vs > (1u << 24)) return fail(ctx, INFR_CUDA_ERR_UNSUPPORTED, "kv_read: a row stride past 2^24 values");
+  const uint64_t nk = attn_span(d->rows, ks, wide) * width, nv = attn_span(d->rows, vs, wide) * width, nc = attn_cache_bytes(sizes, scales.width());
+  if (!fits(d->k, nk) || !fits(d->v, nv)) return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "kv_read: row buffer missing or too small");
+  if (!d->rows) return INFR_CUDA_OK;
+  if (attn_rows_meet(reinterpret_cast<uintptr_t>(d->k->ptr), (uint64_t)wide * width, (uint64_t)ks * width, reinterpret_cast<uintptr_t>(d->v->ptr), (uint64_t)wide * width,
+                     (uint64_t)vs * width, d->rows))
+    return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "kv_read: the rows of k and v overlap");
+  for (const auto& [rows, bytes] : {std::pair<const infr_cuda_buf*, uint64_t>{d->k, nk}, {d->v, nv}})
+    if (overlap(rows, bytes, d->k_cache, nc) || overlap(rows, bytes, d->v_cache, nc) ||
+        (scales.any() && (overlap(rows, bytes, d->k_scale, nc / 16) || overlap(rows, bytes, d->v_scale, nc / 16))))
+      return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "kv_read: rows overlap the cache");
+  DeviceGuard g(ctx->device);
+  KvReadParams p = {};
+  attn_batch_params(p, ctx, d);
+  p.k = d->k_cache->ptr;
+  p.v = d->v_cache->ptr;
+  p.ks = scales.any() ? static_cast<const uint8_t*>(d->k_scale->ptr) : nullptr;
+  p.vs = scales.any() ? static_cast<const uint8_t*>(d->v_scale->ptr) : nullptr;
+  p.k_out = d->k->ptr;
+  p.v_out = d->v->ptr;
+  p.ko_stride = ks;
+  p.vo_stride = vs;
+  p.f16 = d->f16 ? 1 : 0;
+  return launch_kv_read(ctx, p);
+}
+
+// ---- the two ends of a step: tokens to rows, logits to tokens --------------------------------------
+
+int32_t infr_cuda_embed(infr_cuda_ctx* ctx, const infr_cuda_embed_desc* d) {
+  if (!ctx) return INFR_CUDA_ERR_INVALID_ARG;
+  if (!d) return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "embed: null descriptor");
+  const bool plain = d->dtype == INFR_CUDA_DT_F32 || d->dtype == INFR_CUDA_DT_F16 || d->dtype == INFR_CUDA_DT_BF16;
+  if (!plain && !block_elems(d->dtype)) return fail(ctx, INFR_CUDA_ERR_UNSUPPORTED, "embed: table dtype not covered (F32, F16, BF16 and the block formats an expert bank may have)");
+  if (codebook_missing(ctx, d->dtype))
+    return fail(ctx, INFR_CUDA_ERR_UNSUPPORTED, "embed: the table is in a grid codebook format whose table has not been set (infr_cuda_set_codebook)");
+  if (!d->ne || !d->n_vocab) return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "embed: zero dimension");
+  if (!plain && d->ne % block_elems(d->dtype)) return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "embed: ne must be a whole number of blocks (32, 64 or 256 weights)");
+  if (d->ne % 16) return fail(ctx, INFR_CUDA_ERR_UNSUPPORTED, "embed: ne must be a multiple of 16");
+  if (d->ne > (1u << 20) || d->rows > (1u << 22) || d->n_vocab > (1u << 30)) return fail(ctx, INFR_CUDA_ERR_UNSUPPORTED, "embed: more than 2^20 values, 2^22 rows or 2^30 tokens");
+  if (!std::isfinite(d->scale)) return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "embed: scale must be finite");
+  long long stride = 0;
+  const int32_t rc = attn_check_rows(ctx, "embed: dst", d->dst, d->rows, d->dst_stride, d->ne, &stride);
+  if (rc) return rc;
+  const uint64_t rb = d->dtype == INFR_CUDA_DT_F16 || d->dtype == INFR_CUDA_DT_BF16 ? (uint64_t)d->ne * 2 : row_bytes(d->dtype, d->ne);
+  const uint64_t nt = rb * d->n_vocab, nd = attn_span(d->rows, stride, d->ne) * 4;
+  if (!fits(d->table, nt) || !fits(d->ids, (size_t)d->rows * 4)) return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "embed: table or ids missing or too small");
+  if (!d->rows) return INFR_CUDA_OK;
+  if (overlap(d->dst, nd, d->table, nt) || overlap(d->dst, nd, d->ids, (uint64_t)d->rows * 4)) return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "embed: dst overlaps table or ids");
+  DeviceGuard g(ctx->device);
+  return launch_embed(ctx, d->dtype, static_cast<const uint8_t*>(d->table->ptr), static_cast<const int*>(d->ids->ptr), static_cast<float*>(d->dst->ptr), (size_t)stride, (int)d->rows,
+                      (int)d->ne, (int)d->n_vocab, d->scale);
+}
+
+int32_t infr_cuda_sample(infr_cuda_ctx* ctx, const infr_cuda_sample_desc* d) {
+  if (!ctx) return INFR_CUDA_ERR_INVALID_ARG;
+  if (!d) return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "sample: null descriptor");
+  if (!d->n_vocab) return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "sample: zero dimension");
+  if (d->n_vocab > (1u << 24) || d->rows > (1u << 22)) return fail(ctx, INFR_CUDA_ERR_UNSUPPORTED, "sample: more than 2^24 tokens or 2^22 rows");
+  const uint32_t stride = d->stride ? d->stride : d->n_vocab;
+  if (stride < d->n_vocab) return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "sample: a row stride is at least a row");
+  const uint64_t nl = attn_span(d->rows, stride, d->n_vocab) * 4, nr = (uint64_t)d->rows * 4;
+  if (!fits(d->logits, nl) || !fits(d->u, nr) || !fits(d->ids, nr)) return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "sample: logits, u or ids missing or too small");
+  for (const infr_cuda_buf* b : {d->temperature, d->top_k, d->top_p, d->min_p, static_cast<const infr_cuda_buf*>(d->prob)})
+    if (b && !fits(b, nr)) return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "sample: a buffer of one word per row is too small");
+  if (!d->rows) return INFR_CUDA_OK;
+  for (const infr_cuda_buf* out : {d->ids, d->prob}) {
+    if (!out) continue;
+    if (overlap(out, nr, d->logits, nl)) return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "sample: ids or prob overlaps logits");
+    for (const infr_cuda_buf* b : {d->u, d->temperature, d->top_k, d->top_p, d->min_p})
+      if (b && overlap(out, nr, b, nr)) return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "sample: ids or prob overlaps a row's parameters");
+  }
+  if (d->prob && overlap(d->ids, nr, d->prob, nr)) return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "sample: ids and prob overlap");
+  DeviceGuard g(ctx->device);
+  auto f32 = [](const infr_cuda_buf* b) { return b ? static_cast<const float*>(b->ptr) : nullptr; };
+  return launch_sample(ctx, f32(d->logits), f32(d->u), f32(d->temperature), d->top_k ? static_cast<const int*>(d->top_k->ptr) : nullptr, f32(d->top_p), f32(d->min_p),
+                       static_cast<int*>(d->ids->ptr), d->prob ? static_cast<float*>(d->prob->ptr) : nullptr, stride, (int)d->rows, (int)d->n_vocab);
 }
 
 int32_t infr_cuda_moe_expert_rows(infr_cuda_ctx* ctx, const infr_cuda_buf* x_rows, const infr_cuda_buf* seg_off,

@@ -25,6 +25,7 @@ struct AttnParams {
   uint32_t g_inv;    // ceil(2^16 / g): r / g = r * g_inv >> 16 for the rows r of an item
   int cap;           // max_pages * page_size
   int page_shift;    // log2(page_size), or -1
+  const uint8_t *kq, *vq, *ks, *vs;  // pages of 8 bits (kv_q8.cuh): codes and scale bytes; the pitches are the codes', 16 to a scale byte.  Null: f16
 };
 
 // Weights are 2^(x - reference + bias), two f16 pieces each: at most 2^15.9, and known to 2^-25.  The reference is a whole number (sums are
@@ -461,10 +462,27 @@ struct RopeParams {
   double turns0, ratio;  // turns per token of pair 0, and of each pair relative to the one before
   float norm_eps;
   int rows, n_seq, n_head, n_kv, hd, page_size, max_pages, n_pages, cap, n_rot, interleaved;
+  uint8_t *k_codes, *v_codes, *k_scale, *v_scale;  // a cache of 8 bits in place of k_cache and v_cache, or null
 };
 int32_t launch_rope_kv(infr_cuda_ctx* ctx, const RopeParams& p);
 
 int32_t launch_attn_rows(infr_cuda_ctx* ctx, AttnParams p, const __half* k, int max_rows);
 int32_t launch_attn_tiles(infr_cuda_ctx* ctx, AttnParams p, const __half* k);
+
+// Rows of a batch out of the cache's pages (kv_read.cu).
+struct KvReadParams {
+  const void *k, *v;                 // f16 values, or codes
+  const uint8_t *ks, *vs;            // scale bytes, or null
+  void *k_out, *v_out;               // f16 or f32 rows
+  const int *cu_q, *kv_len, *page_table;
+  DeviceStatus* status;
+  size_t page_pitch, head_pitch, row_pitch;  // in values
+  long long ko_stride, vo_stride;
+  int rows, n_seq, n_kv, hd, page_size, max_pages, n_pages, cap, f16;
+};
+int32_t launch_kv_read(infr_cuda_ctx* ctx, const KvReadParams& p);
+// The pages of 8 bits that a call's rows see as f16 pages at k and v, each at its own number, or (table != null) the pages of sequence s from
+// s * max_pages on, which the table then says.
+int32_t launch_kv_unpack(infr_cuda_ctx* ctx, const AttnParams& p, __half* k, __half* v, int* table);
 
 }  // namespace infr

@@ -140,10 +140,27 @@ inline const char* attn_sizes_error(const AttnSizes& s, bool* unsupported) {
   return nullptr;
 }
 
-// Bytes of the cache that a call's pages or rows take; all ones where that is past 64 bits (accepted sizes go to 2^80).
-inline uint64_t attn_cache_bytes(const AttnSizes& s) {
-  const uint64_t tokens = s.paged ? (uint64_t)s.n_pages * s.page_size : s.rows, each = (uint64_t)s.n_kv * s.head_dim * 2;
+// Bytes of the cache that a call's pages or rows take, `width` to a value; all ones where that is past 64 bits (accepted sizes go to 2^80).
+inline uint64_t attn_cache_bytes(const AttnSizes& s, uint32_t width = 2) {
+  const uint64_t tokens = s.paged ? (uint64_t)s.n_pages * s.page_size : s.rows, each = (uint64_t)s.n_kv * s.head_dim * width;
   return tokens > ~0ull / each ? ~0ull : tokens * each;
+}
+
+// The f16 copy of what a call sees of pages in 8 bits: every page of the cache at its own number, or max_pages places to a sequence where these are fewer.
+struct AttnUnpacked {
+  bool by_sequence;
+  uint64_t pages, table, side;  // bytes ahead of the pages (the sequences' table), and of K or V
+};
+// false: past 2^48 bytes.
+inline bool attn_unpacked(const AttnSizes& s, AttnUnpacked* u) {
+  const uint64_t places = (uint64_t)s.n_seq * s.max_pages;
+  u->by_sequence = places < s.n_pages;
+  u->pages = u->by_sequence ? places : s.n_pages;
+  u->table = u->by_sequence ? (places * 4 + 255) / 256 * 256 : 0;
+  const uint64_t page = (uint64_t)s.page_size * s.n_kv * s.head_dim * 2;
+  if (u->pages > (1ull << 47) / page) return false;
+  u->side = u->pages * page;
+  return true;
 }
 
 // Values a buffer needs for `rows` rows of `wide` values that are `stride` apart.

@@ -26,7 +26,8 @@ constexpr uint32_t QK = 256;
 // Device-visible status word written by kernels whose bounded waits ran out.
 struct DeviceStatus {
   int timeout;      // != 0: a bounded wait gave up (value identifies the kernel)
-  int bad_index;    // 1: an expert id outside [0, n_expert) was clamped; 2: a page, row or length of an attention batch
+  int bad_index;    // 1: an expert id outside [0, n_expert) was clamped; 2: a page, row or length of an attention batch;
+                    // 3: a token outside the embedding table
 };
 
 }  // namespace infr
@@ -78,6 +79,10 @@ struct infr_cuda_ctx {
   int* attn_count = nullptr;                  // device memory: join counters of the attention kernels, zero between launches
   char* attn_parts = nullptr;                 // and their partial results: one block of its final size, so that a recorded
                                               // plan's address of it holds whatever is called later
+  char* kv_unpacked = nullptr;                // device memory: the f16 pages of attention of many rows over pages of 8 bits, grown on demand.  A block that
+  size_t kv_unpacked_bytes = 0;               // a recorded plan has the address of stays where it is until the context ends
+  bool kv_unpacked_recorded = false;
+  std::vector<void*> kv_unpacked_before;
   unsigned long long* trace = nullptr;        // optional phase stamps (see trace_stamp)
   infr_cuda_config cfg = {};                  // tuning switches (infr_cuda_set_config)
   infr::EpState* ep = nullptr;                // expert-parallel communicator and buffers, or null

@@ -136,6 +136,50 @@ __global__ void __launch_bounds__(256) k_linear_anyfmt(int dt, const unsigned ch
   if (lane == 0) y[(size_t)blockIdx.y * out_f + o] = acc;
 }
 
+// Rows of a token table by number, scaled: a thread per 16 weights.  An id outside the table gives zeros.
+template <int DT>
+__global__ void __launch_bounds__(128) k_embed(int dt, const unsigned char* __restrict__ table, const int* __restrict__ ids, float* __restrict__ dst, DeviceStatus* status, int ne,
+                                               int n_vocab, size_t rb, size_t dst_stride, float scale) {
+  pdl_trigger();
+  const int h = blockIdx.y * 128 + threadIdx.x;
+  pdl_wait();
+  const int id = __ldcg(ids + blockIdx.x);
+  if (16 * h >= ne) return;
+  float v[16];
+  if ((unsigned)id >= (unsigned)n_vocab) {
+    if (h == 0) status->bad_index = 3;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = 0.f;
+  } else {
+    const unsigned char* row = table + (size_t)id * rb;
+    if constexpr (DT == INFR_CUDA_DT_F32) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) *reinterpret_cast<float4*>(v + 4 * i) = __ldg(reinterpret_cast<const float4*>(row) + 4 * h + i);
+    } else if constexpr (DT == INFR_CUDA_DT_F16 || DT == INFR_CUDA_DT_BF16) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint4 x = __ldg(reinterpret_cast<const uint4*>(row) + 2 * h + i);
+        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          v[8 * i + 2 * j] = DT == INFR_CUDA_DT_F16 ? f16_bits_to_f32(w[j]) : __uint_as_float(w[j] << 16);
+          v[8 * i + 2 * j + 1] = DT == INFR_CUDA_DT_F16 ? f16_bits_to_f32(w[j] >> 16) : __uint_as_float(w[j] & 0xFFFF0000u);
+        }
+      }
+    } else {
+      uint32_t c[4];
+      float A, B;
+      int off;
+      fmt_codes16(DT < 0 ? dt : DT, row, h, c, A, B, off);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] = fmaf(A, (float)((int)((c[i >> 2] >> (8 * (i & 3))) & 0xFFu) - off), B);
+    }
+  }
+  float4* to = reinterpret_cast<float4*>(dst + (size_t)blockIdx.x * dst_stride + 16 * h);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) to[i] = make_float4(v[4 * i] * scale, v[4 * i + 1] * scale, v[4 * i + 2] * scale, v[4 * i + 3] * scale);
+}
+
 __global__ void k_gated_act(const float* __restrict__ g, const float* __restrict__ u, float* __restrict__ dst, size_t n) {
   const size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
   if (i < n) {
@@ -264,6 +308,21 @@ int32_t launch_linear(infr_cuda_ctx* ctx, int32_t dtype, const uint8_t* w, const
   }
   ctx->launches += 1;
   return check_cuda(ctx, cudaGetLastError(), "k_linear launch");
+}
+
+int32_t launch_embed(infr_cuda_ctx* ctx, int32_t dtype, const uint8_t* table, const int* ids, float* dst, size_t dst_stride, int rows, int ne, int n_vocab, float scale) {
+  const size_t rb = dtype == INFR_CUDA_DT_F16 || dtype == INFR_CUDA_DT_BF16 ? (size_t)ne * 2 : row_bytes(dtype, ne);
+  const auto kernel = dtype == INFR_CUDA_DT_F32    ? k_embed<INFR_CUDA_DT_F32>
+                      : dtype == INFR_CUDA_DT_F16  ? k_embed<INFR_CUDA_DT_F16>
+                      : dtype == INFR_CUDA_DT_BF16 ? k_embed<INFR_CUDA_DT_BF16>
+                      : dtype == INFR_CUDA_DT_Q8_0 ? k_embed<INFR_CUDA_DT_Q8_0>
+                      : dtype == INFR_CUDA_DT_Q4K  ? k_embed<INFR_CUDA_DT_Q4K>
+                      : dtype == INFR_CUDA_DT_Q6K  ? k_embed<INFR_CUDA_DT_Q6K>
+                                                   : k_embed<-1>;
+  const cudaError_t e = launch_ex(kernel, dim3(rows, (ne / 16 + 127) / 128), dim3(128), 0, ctx->stream, true, (int)dtype, table, ids, dst, ctx->status, ne, n_vocab, rb, dst_stride, scale);
+  if (e != cudaSuccess) return check_cuda(ctx, e, "k_embed launch");
+  ctx->launches += 1;
+  return check_cuda(ctx, cudaGetLastError(), "k_embed launch");
 }
 
 int32_t launch_gated_act(infr_cuda_ctx* ctx, const float* gate, const float* up, float* dst, size_t n) {

@@ -199,6 +199,11 @@ int32_t launch_anyfmt_decode(infr_cuda_ctx* ctx, const DecodeParams& p, bool pdl
 // y[m, out_f] = x[m, in_f] · Wᵀ for W of dtype F32 / Q4_K / Q6_K.
 int32_t launch_linear(infr_cuda_ctx* ctx, int32_t dtype, const uint8_t* w, const float* x, float* y, int m, int in_f,
                       int out_f);
+// dst[r] = scale * row ids[r] of a table [n_vocab, ne] of dtype F32 / F16 / BF16 or a block format.
+int32_t launch_embed(infr_cuda_ctx* ctx, int32_t dtype, const uint8_t* table, const int* ids, float* dst, size_t dst_stride, int rows, int ne, int n_vocab, float scale);
+// A token of each row of logits (sample.cu); parameters by row, null = that step is left out.
+int32_t launch_sample(infr_cuda_ctx* ctx, const float* logits, const float* u, const float* temperature, const int* top_k, const float* top_p, const float* min_p, int* ids,
+                      float* prob, size_t stride, int rows, int n_vocab);
 int32_t launch_gated_act(infr_cuda_ctx* ctx, const float* gate, const float* up, float* dst, size_t n);
 int32_t launch_shared_add(infr_cuda_ctx* ctx, const float* moe, const float* shexp, const float* gate, float* dst,
                           int rows, int n);

@@ -1,0 +1,170 @@
+// Keys and values out of the cache's pages: as rows of a batch for whoever asked (k_kv_read), or, of pages in 8 bits, as f16 pages for the
+// attention kernel that takes these (k_kv_unpack).  Every value is read once and written once: memory bounds both.
+#include "attn.cuh"
+#include "kv_q8.cuh"
+
+namespace infr {
+namespace {
+
+constexpr int READ_THREADS = 256, READ_ROWS = 8;
+
+// Eight values of a row to each thread: 8 bytes of codes in (16 of f16), 16 bytes of f16 out (32 of f32), neighbours side by side.
+template <bool Q8, bool F16>
+__global__ void __launch_bounds__(READ_THREADS) k_kv_read(const __grid_constant__ KvReadParams p) {
+  __shared__ long long s_at[READ_ROWS];  // where a row's token lies (-1: a row that is no token; -2: of no sequence)
+  __shared__ int s_first;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int r0 = (int)((long long)blockIdx.x * p.rows / gridDim.x), r1 = (int)((long long)(blockIdx.x + 1) * p.rows / gridDim.x);
+  const int chunks = p.hd / 8, side = p.n_kv * chunks;
+  pdl_trigger();
+  pdl_wait();
+  if (tid < 32) {
+    // the last sequence that begins at or before the first row (rows ahead of cu_q[0] belong to none): 32 places at a time
+    int lo = 0, hi = p.n_seq;
+#pragma unroll 1
+    while (hi - lo > 1) {
+      const int step = (hi - lo + 31) / 32, i = lo + lane * step;
+      const int n = __popc(__ballot_sync(0xFFFFFFFFu, i < hi && __ldcg(p.cu_q + i) <= r0));
+      lo += max(n - 1, 0) * step;
+      hi = min(hi, lo + step);
+    }
+    if (lane == 0) s_first = lo;
+  }
+  __syncthreads();
+  bool bad = false;
+  int s = s_first;
+  AttnSeq seq = {0, 0, 0};
+  auto load = [&](int i) { return attn_seq(__ldcg(p.cu_q + i), __ldcg(p.cu_q + i + 1), __ldcg(p.kv_len + i), false, p.rows, p.cap, &bad); };
+  if (tid < READ_ROWS) seq = load(s);
+#pragma unroll 1
+  for (int row0 = r0; row0 < r1; row0 += READ_ROWS) {
+    const int rows = min(READ_ROWS, r1 - row0);
+    if (tid < rows) {
+      const int r = row0 + tid;
+#pragma unroll 1
+      while (s + 1 < p.n_seq && r >= seq.q0 + seq.q_len) seq = load(++s);
+      const int pos = seq.past + r - seq.q0;
+      long long at = -2;
+      if (r >= seq.q0 && r < seq.q0 + seq.q_len) {
+        at = -1;
+        if (pos >= 0) {
+          const int page = pos / p.page_size;
+          int id = __ldcg(p.page_table + (size_t)s * p.max_pages + page);
+          if ((unsigned)id >= (unsigned)p.n_pages) bad = true, id = 0;  // read as page 0, reported at the next sync
+          at = (long long)((size_t)id * p.page_pitch + (size_t)(pos - page * p.page_size) * p.row_pitch);
+        }
+      }
+      s_at[tid] = at;
+    }
+    __syncthreads();
+#pragma unroll 2
+    for (int e = tid; e < rows * 2 * side; e += READ_THREADS) {
+      const int i = e / (2 * side), in = e - i * 2 * side;
+      const bool is_v = in >= side;
+      const int c = is_v ? in - side : in, head = c / chunks;
+      const long long at = s_at[i];
+      if (at == -2) continue;
+      const size_t from = (size_t)max(at, 0ll) + (size_t)head * p.head_pitch + (size_t)(c - head * chunks) * 8;
+      uint4 w = make_uint4(0, 0, 0, 0);  // eight f16 values
+      if (at >= 0) {
+        if constexpr (Q8) {
+          const uint2 codes = __ldcg(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(is_v ? p.v : p.k) + from));
+          const uint32_t d2 = q8_scale_pair(__ldcg((is_v ? p.vs : p.ks) + from / 16));
+          w = make_uint4(q8_lo(codes.x, d2), q8_hi(codes.x, d2), q8_lo(codes.y, d2), q8_hi(codes.y, d2));
+        } else {
+          w = __ldcg(reinterpret_cast<const uint4*>(static_cast<const __half*>(is_v ? p.v : p.k) + from));
+        }
+      }
+      const size_t to = (size_t)(row0 + i) * (is_v ? p.vo_stride : p.ko_stride) + (size_t)c * 8;
+      if constexpr (F16) {
+        *reinterpret_cast<uint4*>(static_cast<__half*>(is_v ? p.v_out : p.k_out) + to) = w;
+      } else {
+        const __half2* h = reinterpret_cast<const __half2*>(&w);
+        const float2 a = __half22float2(h[0]), b = __half22float2(h[1]), cc = __half22float2(h[2]), d = __half22float2(h[3]);
+        float4* dst = reinterpret_cast<float4*>(static_cast<float*>(is_v ? p.v_out : p.k_out) + to);
+        dst[0] = make_float4(a.x, a.y, b.x, b.y);
+        dst[1] = make_float4(cc.x, cc.y, d.x, d.y);
+      }
+    }
+    __syncthreads();
+  }
+  if (bad) p.status->bad_index = 2;
+}
+
+// The pages that some row of the call sees, one kv head of a page at a time.
+__global__ void __launch_bounds__(READ_THREADS) k_kv_unpack(const __grid_constant__ AttnParams p, __half* __restrict__ k, __half* __restrict__ v, int* __restrict__ table) {
+  extern __shared__ int s_pre[];  // pages ahead of each sequence, then the first page of each
+  __shared__ long long s_scan[READ_THREADS / 32];
+  const int tid = threadIdx.x;
+  int* s_page0 = s_pre + p.n_seq + 1;
+  pdl_trigger();
+  pdl_wait();
+  if (tid == 0) s_pre[0] = 0;
+  long long carry = 0;
+#pragma unroll 1
+  for (int s0 = 0; s0 < p.n_seq; s0 += READ_THREADS) {
+    const int s = s0 + tid;
+    int n = 0;
+    if (s < p.n_seq) {
+      const AttnSeq seq = attn_load_seq(p, s);
+      const int hi = seq.past + seq.q_len, lo = attn_first_key(seq.past, p.window);
+      const int first = lo / p.page_size;
+      s_page0[s] = first;
+      n = seq.q_len > 0 && hi > lo ? (hi - 1) / p.page_size + 1 - first : 0;
+    }
+    const long long sum = carry + block_scan<READ_THREADS>(n, s_scan);
+    if (s < p.n_seq) s_pre[s + 1] = (int)min(sum, 0x7FFFFFFFll);  // (4096 sequences of 2^31 / 16 pages and more: not in 180 GB)
+    __syncthreads();
+    carry = s_pre[min(s0 + READ_THREADS, p.n_seq)];
+  }
+  const long long units = carry * p.n_kv, u0 = units * blockIdx.x / gridDim.x, u1 = units * (blockIdx.x + 1) / gridDim.x;
+  const int blocks = p.hd / 16, per = p.page_size * blocks;  // 16 values to each thread
+#pragma unroll 1
+  for (long long u = u0; u < u1; ++u) {
+    const int page = (int)(u / p.n_kv), head = (int)(u - (long long)page * p.n_kv);
+    int s = 0;
+#pragma unroll 1
+    for (int hi = p.n_seq; hi - s > 1;) {  // the last sequence whose pages begin at or before this one
+      const int mid = (s + hi) / 2;
+      if (s_pre[mid] <= page) s = mid;
+      else hi = mid;
+    }
+    while (s_pre[s + 1] <= page) ++s;  // (past sequences without pages)
+    const int j = s_page0[s] + page - s_pre[s], id = attn_page(p, s, j);
+    const int to_page = table != nullptr ? s * p.max_pages + j : id;
+    if (table != nullptr && head == 0 && tid == 0) table[(size_t)s * p.max_pages + j] = to_page;
+    const size_t from = (size_t)id * p.page_pitch + (size_t)head * p.head_pitch, to = (size_t)to_page * p.page_pitch + (size_t)head * p.head_pitch;
+#pragma unroll 1
+    for (int e = tid; e < 2 * per; e += READ_THREADS) {
+      const bool is_v = e >= per;
+      const size_t at = (size_t)(is_v ? e - per : e) * 16;
+      const uint4 c = __ldcg(reinterpret_cast<const uint4*>((is_v ? p.vq : p.kq) + from + at));
+      const uint32_t d2 = q8_scale_pair(__ldcg((is_v ? p.vs : p.ks) + (from + at) / 16));
+      uint4* dst = reinterpret_cast<uint4*>((is_v ? v : k) + to + at);
+      dst[0] = make_uint4(q8_lo(c.x, d2), q8_hi(c.x, d2), q8_lo(c.y, d2), q8_hi(c.y, d2));
+      dst[1] = make_uint4(q8_lo(c.z, d2), q8_hi(c.z, d2), q8_lo(c.w, d2), q8_hi(c.w, d2));
+    }
+  }
+}
+
+}  // namespace
+
+int32_t launch_kv_read(infr_cuda_ctx* ctx, const KvReadParams& p) {
+  const int most = ctx->sm_count * 8;
+  const auto kernel = p.ks != nullptr ? (p.f16 ? k_kv_read<true, true> : k_kv_read<true, false>) : (p.f16 ? k_kv_read<false, true> : k_kv_read<false, false>);
+  const cudaError_t e = launch_ex(kernel, dim3(p.rows < most ? p.rows : most), dim3(READ_THREADS), 0, ctx->stream, true, p);
+  if (e != cudaSuccess) return check_cuda(ctx, e, "k_kv_read launch");
+  ctx->launches += 1;
+  return check_cuda(ctx, cudaGetLastError(), "k_kv_read launch");
+}
+
+int32_t launch_kv_unpack(infr_cuda_ctx* ctx, const AttnParams& p, __half* k, __half* v, int* table) {
+  const size_t smem = (2 * (size_t)p.n_seq + 1) * 4;
+  cudaError_t e = ensure_smem(reinterpret_cast<const void*>(&k_kv_unpack), smem);
+  if (e == cudaSuccess) e = launch_ex(k_kv_unpack, dim3(ctx->sm_count * 8), dim3(READ_THREADS), smem, ctx->stream, true, p, k, v, table);
+  if (e != cudaSuccess) return check_cuda(ctx, e, "k_kv_unpack launch");
+  ctx->launches += 1;
+  return check_cuda(ctx, cudaGetLastError(), "k_kv_unpack launch");
+}
+
+}  // namespace infr

@@ -1,5 +1,5 @@
 // What stands between a layer's q / k / v rows and its attention: per-head RMS norm and rotary embedding of q and k, k and v rounded to
-// f16 into the cache.  Every value is read once and written once: memory bounds it.
+// f16 into the cache, or quantised into one of 8 bits (kv_q8.cuh).  Every value is read once and written once: memory bounds it.
 //
 // Sixteen lanes own a head; a lane takes eight values at a time as two 16-byte words that hold four whole pairs (halves style: the words
 // are half the rotated range apart; interleaved: neighbours), so that a pair never leaves its lane.  The angles are products of a position
@@ -10,6 +10,7 @@
 // Measured: 8192 rows of 32 + 2 x 4 heads of 128 59.9 us, 5.3 TB/s of the rows and the cache (0.81 of the copy rate; 62.4 with heads divided
 // out of an index instead of counted on, 64.5 with five CTAs to an SM in place of four); 777 rows 9.9 us, 32 rows 4.8 us: launch, plan, one row's chain.
 #include "attn.cuh"
+#include "kv_q8.cuh"
 
 namespace infr {
 namespace {
@@ -33,9 +34,11 @@ __device__ __forceinline__ void store4_f16(__half* dst, const float4& v) {
   *reinterpret_cast<uint2*>(dst) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
 }
 
-// JS: eight-value chunks of a lane: 1 for heads up to 128, else 2.
-template <int JS>
+// JS: eight-value chunks of a lane: 1 for heads up to 128, else 2.  Q8: the cache is one of 8 bits.
+template <int JS, bool Q8>
 __global__ void __launch_bounds__(ROPE_THREADS) k_rope_kv(const __grid_constant__ RopeParams p) {
+  // a head on its way into 8 bits: what shares a scale lies in two to six lanes, as n_rot has it
+  __shared__ __align__(16) float s_head[Q8 ? ROPE_TEAMS * 128 * JS : 4];
   __shared__ __align__(16) float s_cos[ROPE_ROWS * ROPE_MAX_PAIRS], s_sin[ROPE_ROWS * ROPE_MAX_PAIRS];
   __shared__ int s_pos[ROPE_ROWS], s_first;
   __shared__ long long s_at[ROPE_ROWS];
@@ -142,6 +145,7 @@ __global__ void __launch_bounds__(ROPE_THREADS) k_rope_kv(const __grid_constant_
       if (!has) continue;
       const float k = w != nullptr ? rsqrtf(sq / (float)p.hd + p.norm_eps) : 1.f;
       const long long at = s_at[i];
+      float* head = s_head + (Q8 ? team * 128 * JS : 0);
 #pragma unroll
       for (int j = 0; j < JS; ++j) {
         const int c = tl + 16 * j;
@@ -165,11 +169,35 @@ __global__ void __launch_bounds__(ROPE_THREADS) k_rope_kv(const __grid_constant_
           float* dst = p.q_out + (size_t)r * p.qo_stride + (size_t)h * p.hd;
           *reinterpret_cast<float4*>(dst + oa[j]) = x[j];
           *reinterpret_cast<float4*>(dst + ob[j]) = y[j];
+        } else if constexpr (Q8) {
+          *reinterpret_cast<float4*>(head + oa[j]) = x[j];
+          *reinterpret_cast<float4*>(head + ob[j]) = y[j];
         } else if (at >= 0) {
           __half* dst = (is_v ? p.v_cache + (size_t)(h - p.n_head - p.n_kv) * p.head_pitch : p.k_cache + (size_t)(h - p.n_head) * p.head_pitch) + at;
           store4_f16(dst + oa[j], x[j]);
           store4_f16(dst + ob[j], y[j]);
         }
+      }
+      if (Q8 && !is_q) {  // (a team as one: it is half of a warp)
+        const uint32_t lanes = 0xFFFFu << (16 * (team & 1));
+        __syncwarp(lanes);
+        if (16 * tl < p.hd && at >= 0) {
+          float4 v[4];
+          float big = 0.f;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            v[k] = *reinterpret_cast<const float4*>(head + 16 * tl + 4 * k);
+            big = max_nan(max_nan(big, fabsf(v[k].x), fabsf(v[k].y)), fabsf(v[k].z), fabsf(v[k].w));
+          }
+          const uint32_t sb = q8_scale_byte(big);
+          const float r = q8_inverse(sb);
+          const uint4 codes = sb < Q8_ODD ? make_uint4(q8_codes4(v[0], r), q8_codes4(v[1], r), q8_codes4(v[2], r), q8_codes4(v[3], r))
+                                          : make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
+          const size_t to = (size_t)at + (size_t)(h - p.n_head - (is_v ? p.n_kv : 0)) * p.head_pitch + 16 * tl;
+          *reinterpret_cast<uint4*>((is_v ? p.v_codes : p.k_codes) + to) = codes;
+          (is_v ? p.v_scale : p.k_scale)[to / 16] = (uint8_t)sb;
+        }
+        __syncwarp(lanes);
       }
     }
     __syncthreads();  // the rows' words have been read
@@ -183,7 +211,7 @@ int32_t launch_rope_kv(infr_cuda_ctx* ctx, const RopeParams& p) {
   // Eight to an SM: its threads' worth.  Of these four are there at once (64 registers; three of heads past 128, 80), the rest follow: 8192 rows in two
   // waves 59.9 us.  Fewer rows than that have a CTA each.
   const int most = ctx->sm_count * 8;
-  const cudaError_t e = launch_ex(p.hd <= 128 ? k_rope_kv<1> : k_rope_kv<2>, dim3(p.rows < most ? p.rows : most), dim3(ROPE_THREADS), 0, ctx->stream, true, p);
+  const cudaError_t e = launch_ex(p.k_scale != nullptr ? (p.hd <= 128 ? k_rope_kv<1, true> : k_rope_kv<2, true>) : (p.hd <= 128 ? k_rope_kv<1, false> : k_rope_kv<2, false>), dim3(p.rows < most ? p.rows : most), dim3(ROPE_THREADS), 0, ctx->stream, true, p);
   if (e != cudaSuccess) return check_cuda(ctx, e, "k_rope_kv launch");
   ctx->launches += 1;
   return check_cuda(ctx, cudaGetLastError(), "k_rope_kv launch");
