@@ -22,16 +22,23 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int SAMPLE_CTAS = 8, SAMPLE_THREADS = 512, SAMPLE_WARPS = SAMPLE_THREADS / 32;
-constexpr int SAMPLE_BINS = 4 * SAMPLE_THREADS;  // a thread has four
-constexpr int SAMPLE_LIST = 2048;                // candidates that are sorted
-constexpr int SAMPLE_CAP = 40960;                // values of a row in a CTA's shared memory; what is behind them is read again from global memory
-constexpr double SAMPLE_REACH = 45.0;            // weights down to e^-45 < 2^-64
+constexpr int SAMPLE_CTAS = 8;
+constexpr int SAMPLE_BINS = 2048;
+constexpr int SAMPLE_LIST = 2048;     // candidates that are sorted
+constexpr int SAMPLE_FEW = 1024;      // so many largest ones are looked for among the threads' largest first
+constexpr int SAMPLE_CAP = 40960;     // values of a row in a CTA's shared memory at most
+constexpr double SAMPLE_REACH = 45.0; // weights down to e^-45 < 2^-64
 typedef unsigned long long u64;
+
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {  // NaN where one is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 
 // Values in order: larger ones have smaller numbers; with the index behind them, the order in which tokens are taken.
 __device__ __forceinline__ uint32_t rank_of(float x) {
-  const uint32_t b = __float_as_uint(x);
+  const uint32_t b = __float_as_uint(x + 0.f);  // (-0 is 0)
   return b & 0x80000000u ? b : 0x7FFFFFFFu - b;
 }
 __device__ __forceinline__ float value_of(uint32_t r) { return __uint_as_float(r & 0x80000000u ? r : 0x7FFFFFFFu - r); }
@@ -40,12 +47,12 @@ __device__ __forceinline__ u64 place_of(float x, int i) { return (u64)rank_of(x)
 struct SampleShared {
   uint32_t hist[SAMPLE_BINS];
   u64 list[SAMPLE_LIST];
-  double scan[2][SAMPLE_WARPS];
-  int scan_n[SAMPLE_WARPS];
+  double scan[2][16];
+  int scan_n[16];
+  float scan_f[2][16];
   // from every CTA, by rank
-  u64 best[SAMPLE_CTAS];
-  float low[SAMPLE_CTAS];
-  int odd[SAMPLE_CTAS];
+  float top[SAMPLE_CTAS], least[SAMPLE_CTAS];
+  int best[SAMPLE_CTAS];
   double sum[SAMPLE_CTAS], above[SAMPLE_CTAS], kept[SAMPLE_CTAS];
   uint32_t first[SAMPLE_CTAS], last[SAMPLE_CTAS];
   int equal[SAMPLE_CTAS];
@@ -57,16 +64,47 @@ struct SampleShared {
   int pick;
 };
 
+template <int THREADS>
 struct Sampler {
+  static constexpr int WARPS = THREADS / 32, PER = SAMPLE_BINS / THREADS;  // bins (and candidates) of a thread
   SampleShared& sh;
   cg::cluster_group cluster;
-  const float *xs, *gx;  // this CTA's values: in shared memory, and where they came from
-  int n, base, me, tid;  // how many, index of the first
+  // This CTA's values, four to a word that lies on a 16-byte boundary: in shared memory, or (xs null) where they came from.  The row begins within its first
+  // word as a rule; what is not of the row reads as -inf.
+  const float *xs, *row;
+  int words, base, n_vocab;  // index of the first value: may be negative
+  int me, tid;
   float top;             // the row's largest value
   double inv_t;
   float floor_x;         // values from here on have a weight
 
-  __device__ float x_at(int i) const { return i < SAMPLE_CAP ? xs[i] : __ldcg(gx + i) + 0.f; }
+  __device__ float4 from_row(int w) const {
+    const int i = base + 4 * w;
+    if (i >= 0 && i + 3 < n_vocab) return __ldcg(reinterpret_cast<const float4*>(row + i));
+    float x[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = i + j >= 0 && i + j < n_vocab ? __ldcg(row + i + j) : -CUDART_INF_F;
+    return make_float4(x[0], x[1], x[2], x[3]);
+  }
+  __device__ float4 word(int w) const { return xs != nullptr ? *reinterpret_cast<const float4*>(xs + 4 * w) : from_row(w); }
+  // f(value, index) for the values of the words from + k * step
+  template <class F>
+  __device__ __forceinline__ void each(int from, int to, int step, F f) const {
+#pragma unroll 1
+    for (int w0 = from; w0 < to; w0 += 4 * step) {
+      float4 v[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (w0 + k * step < to) v[k] = word(w0 + k * step);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int i = base + 4 * (w0 + k * step);
+        if (w0 + k * step < to) f(v[k].x, i), f(v[k].y, i + 1), f(v[k].z, i + 2), f(v[k].w, i + 3);
+      }
+    }
+  }
+  template <class F>
+  __device__ __forceinline__ void mine(F f) const { each(tid, words, THREADS, f); }
   __device__ double weight(float x) const { return x < floor_x ? 0.0 : x == top ? 1.0 : exp(((double)x - (double)top) * inv_t); }
 
   template <typename T>
@@ -91,7 +129,7 @@ struct Sampler {
     T ahead = 0;
     all = 0;
 #pragma unroll
-    for (int w = 0; w < SAMPLE_WARPS; ++w) {
+    for (int w = 0; w < WARPS; ++w) {
       if (w == warp) ahead = all;
       all += s[w];
     }
@@ -104,7 +142,7 @@ struct Sampler {
     if (tid < SAMPLE_CTAS) *cluster.map_shared_rank(array + me, tid) = v;
   }
   __device__ void clear_hist() {
-    for (int b = tid; b < SAMPLE_BINS; b += SAMPLE_THREADS) sh.hist[b] = 0;
+    for (int b = tid; b < SAMPLE_BINS; b += THREADS) sh.hist[b] = 0;
     if (tid == 0) sh.n_list = 0, sh.b1 = sh.b2 = SAMPLE_BINS;
     __syncthreads();
   }
@@ -119,30 +157,38 @@ struct Sampler {
   // (`slack`: by how much of a weight a bin's edges are off)
   template <class Edge>
   __device__ void bracket(bool by_weight, int k, double target, double slack, Edge edge) {
-    uint32_t c[4] = {0, 0, 0, 0};
+    uint32_t c[PER], sum_c = 0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) c[j] = 0;
 #pragma unroll
     for (int r = 0; r < SAMPLE_CTAS; ++r) {
-      const uint4 h = *reinterpret_cast<const uint4*>(cluster.map_shared_rank(sh.hist, r) + 4 * tid);
-      c[0] += h.x, c[1] += h.y, c[2] += h.z, c[3] += h.w;
-    }
-    int all = 0;
-    int ahead = before<int>((int)(c[0] + c[1] + c[2] + c[3]), sh.scan_n, all);
-    if (by_weight) {
-      double hi[4], lo[4], w = edge(4 * tid);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const double next = edge(4 * tid + j + 1);
-        hi[j] = c[j] * w * (1.0 + slack), lo[j] = c[j] * next * (1.0 - slack);
+      for (int j = 0; j < PER; j += 4) {
+        const uint4 h = *reinterpret_cast<const uint4*>(cluster.map_shared_rank(sh.hist, r) + PER * tid + j);
+        c[j] += h.x, c[j + 1] += h.y, c[j + 2] += h.z, c[j + 3] += h.w;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < PER; ++j) sum_c += c[j];
+    int all = 0;
+    int ahead = before<int>((int)sum_c, sh.scan_n, all);
+    if (by_weight) {
+      double hi[PER], lo[PER], sum_hi = 0, sum_lo = 0, w = edge(PER * tid);
+#pragma unroll
+      for (int j = 0; j < PER; ++j) {
+        const double next = edge(PER * tid + j + 1);
+        sum_hi += hi[j] = c[j] * w * (1.0 + slack);
+        sum_lo += lo[j] = c[j] * next * (1.0 - slack);
         w = next;
       }
       double sum;
-      double h = before<double>((hi[0] + hi[1]) + (hi[2] + hi[3]), sh.scan[0], sum), l = before<double>((lo[0] + lo[1]) + (lo[2] + lo[3]), sh.scan[1], sum);
+      double h = before<double>(sum_hi, sh.scan[0], sum), l = before<double>(sum_lo, sh.scan[1], sum);
       int b1 = SAMPLE_BINS, b2 = SAMPLE_BINS, end = -1;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < PER; ++j) {
         h += hi[j], l += lo[j];
         if (!c[j]) continue;
-        end = 4 * tid + j;
+        end = PER * tid + j;
         // (what sums in another order may differ by)
         if (b1 == SAMPLE_BINS && h * (1.0 + 1e-12) >= target) b1 = end;
         if (b2 == SAMPLE_BINS && l * (1.0 - 1e-12) >= target) b2 = end;
@@ -160,19 +206,19 @@ struct Sampler {
     } else {
       int at = ahead;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (at < k && k <= at + (int)c[j]) sh.b1 = sh.b2 = 4 * tid + j;
+      for (int j = 0; j < PER; ++j) {
+        if (at < k && k <= at + (int)c[j]) sh.b1 = sh.b2 = PER * tid + j;
         at += (int)c[j];
       }
-      if (tid == SAMPLE_THREADS - 1 && all < k) sh.b1 = sh.b2 = -1;  // all are kept
+      if (tid == THREADS - 1 && all < k) sh.b1 = sh.b2 = -1;  // all are kept
     }
     __syncthreads();
     const int b1 = sh.b1, b2 = sh.b2;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (4 * tid + j == b1) sh.ahead = ahead;
+    for (int j = 0; j < PER; ++j) {
+      if (PER * tid + j == b1) sh.ahead = ahead;
       ahead += (int)c[j];
-      if (4 * tid + j == b2) sh.upto = ahead;
+      if (PER * tid + j == b2) sh.upto = ahead;
     }
     __syncthreads();
   }
@@ -181,17 +227,118 @@ struct Sampler {
   __device__ void sort_list(int n) {
     int size = 32;
     while (size < n) size <<= 1;
-    for (int i = n + tid; i < size; i += SAMPLE_THREADS) sh.list[i] = ~0ull;
+    for (int i = n + tid; i < size; i += THREADS) sh.list[i] = ~0ull;
     __syncthreads();
+    const bool alone = size <= 64;  // a warp's pairs
+    if (alone && tid >= 32) size = 0;
     for (int k = 2; k <= size; k <<= 1)
       for (int j = k >> 1; j > 0; j >>= 1) {
-        for (int t = tid; t < size / 2; t += SAMPLE_THREADS) {
+        for (int t = tid; t < size / 2; t += THREADS) {
           const int a = 2 * t - (t & (j - 1)), b = a + j;
           const u64 x = sh.list[a], y = sh.list[b];
           if ((x > y) == ((a & k) == 0)) sh.list[a] = y, sh.list[b] = x;
         }
-        __syncthreads();
+        if (alone) __syncwarp();
+        else __syncthreads();
       }
+    __syncthreads();
+  }
+
+  // The weights of the list's first `count` candidates, the thread's own in w, and the sum ahead of them.
+  __device__ double list_weights(int count, bool by_index, double (&w)[PER], double& all) {
+    double sum = 0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const int e = PER * tid + j;
+      w[j] = e < count ? weight(value_of(by_index ? (uint32_t)sh.list[e] : (uint32_t)(sh.list[e] >> 32))) : 0.0;
+      sum += w[j];
+    }
+    return before<double>(sum, sh.scan[0], all);
+  }
+  // The first of them with which the sum from `at` on reaches the target, or passes it; the last one with a weight if none does.
+  __device__ int list_find(int count, const double (&w)[PER], double at, double target, bool passes) {
+    if (tid == 0) sh.pick = SAMPLE_LIST, sh.b1 = -1;
+    __syncthreads();
+    int found = SAMPLE_LIST, last = -1;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      at += w[j];
+      if (PER * tid + j >= count || w[j] <= 0) continue;
+      last = PER * tid + j;
+      if (found == SAMPLE_LIST && (passes ? at > target : at >= target)) found = last;
+    }
+    if (found < SAMPLE_LIST) atomicMin(&sh.pick, found);
+    if (last >= 0) atomicMax(&sh.b1, last);
+    __syncthreads();
+    const int to = sh.pick == SAMPLE_LIST ? sh.b1 : sh.pick;
+    __syncthreads();
+    return to;
+  }
+
+  // The k largest are in the first CTA's list: the token, by itself.
+  __device__ void from_list(int k, double p, double least, double u, int* id, float* prob) {
+    int count = min(sh.n_list, SAMPLE_LIST);
+    sort_list(count);
+    count = min(count, k);
+    double w[PER], all;
+    double at = list_weights(count, false, w, all);
+    if (p < 1.0) count = list_find(count, w, at, p * all, false) + 1;
+    // (those with no weight are at the end)
+    int n = 0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) n += PER * tid + j < count && w[j] > 0 && w[j] >= least;
+    before<int>(n, sh.scan_n, count);
+    u64 mine[PER];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) mine[j] = PER * tid + j < count ? sh.list[PER * tid + j] : 0;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < PER; ++j)
+      if (PER * tid + j < count) sh.list[PER * tid + j] = mine[j] << 32 | mine[j] >> 32;
+    __syncthreads();
+    sort_list(count);
+    at = list_weights(count, true, w, all);
+    const int e = list_find(count, w, at, u * all, true);
+    if (PER * tid <= e && e < PER * tid + PER) {
+      *id = (int)(sh.list[e] >> 32);
+      double we = 0;
+#pragma unroll
+      for (int j = 0; j < PER; ++j)
+        if (PER * tid + j == e) we = w[j];
+      if (prob != nullptr) *prob = (float)(we / all);
+    }
+  }
+
+  // Bins of one width from the largest value down to `low`: the nearest edge, so that a value is within half a bin (and f32's 2^-22 of its distance).
+  // (A difference of halves does not overflow.)
+  float bin_scale, bin_half;
+  __device__ void set_bins(float low) {
+    bin_scale = top > low ? (float)((double)(SAMPLE_BINS - 1) / (0.5 * ((double)top - (double)low))) : 0.f;
+    bin_half = 0.5f * top;
+  }
+  __device__ int bin(float x) const {
+    const float b = fminf(fmaf(fmaf(-0.5f, x, bin_half), bin_scale, 8388608.f), 8388608.f + (SAMPLE_BINS - 1));
+    return (int)(__float_as_uint(b) & (SAMPLE_BINS - 1));
+  }
+
+  // Whether the k largest are in the first CTA's list: those that share a bin with the k-th largest of the threads' largest, or are larger, if they are not
+  // too many.  Only the threads that have such a one look through their values again.
+  __device__ bool few_largest(int k, float my_top, float least_top) {
+    set_bins(least_top);
+    clear_hist();
+    if (my_top > -CUDART_INF_F) atomicAdd(&sh.hist[bin(my_top)], 1u);
+    cluster.sync();
+    bracket(false, k, 0.0, 0.0, [](int) { return 0.0; });
+    const int b2 = sh.b2;
+    if (b2 < 0) return false;
+    if (my_top > -CUDART_INF_F && bin(my_top) <= b2)
+      mine([&](float x, int i) {
+        if (x == -CUDART_INF_F || bin(x) > b2) return;
+        const int to = atomicAdd(cluster.map_shared_rank(&sh.n_list, 0), 1);
+        if (to < SAMPLE_LIST) *cluster.map_shared_rank(&sh.list[to], 0) = place_of(x, i);
+      });
+    cluster.sync();
+    return *cluster.map_shared_rank(&sh.n_list, 0) <= SAMPLE_LIST;
   }
 
   // The border among the values up to `within`: that of the k largest, or with p < 1 that of the run with p of the weight, or (k, then p) both where the
@@ -199,32 +346,26 @@ struct Sampler {
   __device__ u64 find(u64 within, int k, double p, bool* both) {
     const bool by_weight = k <= 0;
     *both = false;
-    // ---- bins of one width from the largest value down to the least that has a weight (a border of the k largest may lie behind: then nothing is left out)
-    float low = CUDART_INF_F;
-    for (int r = 0; r < SAMPLE_CTAS; ++r) low = fminf(low, sh.low[r]);
-    low = fmaxf(low, floor_x);
-    const float s = top > low ? (float)((double)(SAMPLE_BINS - 1) / (0.5 * ((double)top - (double)low))) : 0.f;
-    const float half = 0.5f * top;  // (a difference of halves does not overflow)
-    auto bin = [&](float x) { return min((int)((half - 0.5f * x) * s), SAMPLE_BINS - 1); };
+    // ---- bins down to the least value that has a weight (a border of the k largest may lie behind: then nothing is left out)
+    const float low = floor_x;
+    set_bins(low);
     clear_hist();
-    double mine = 0;
-#pragma unroll 4
-    for (int i = tid; i < n; i += SAMPLE_THREADS) {
-      const float x = x_at(i);
-      if (x < low || place_of(x, base + i) > within) continue;
+    double sum = 0;
+    mine([&](float x, int i) {
+      if (x < low || place_of(x, i) > within) return;
       atomicAdd(&sh.hist[bin(x)], 1u);
-      if (by_weight) mine += weight(x);
-    }
+      if (by_weight) sum += weight(x);
+    });
     if (by_weight) {
       double all;
-      before<double>(mine, sh.scan[0], all);
+      before<double>(sum, sh.scan[0], all);
       tell(sh.sum, all);
     }
     cluster.sync();
     double target = by_weight ? p * total(sh.sum) : 0;
-    const double width = s > 0.f ? 2.0 * inv_t / s : 0.0;
-    // f32 moves a bin's edges by 2^-22 of their distance from the largest, which is 45 in the exponent at most
-    bracket(by_weight, k, target, 2e-5, [&](int b) { return exp(-b * width); });
+    const double width = bin_scale > 0.f ? 2.0 * inv_t / bin_scale : 0.0;
+    // (f32 moves a bin's edges by 2^-22 of their distance from the largest, which is 45 in the exponent at most)
+    bracket(by_weight, k, target, 3e-5, [&](int b) { return exp((0.5 - b) * width); });
     int b1 = sh.b1, b2 = sh.b2, ahead = sh.ahead, upto = sh.upto;
     if (b1 < 0) return within;
     bool whole = !by_weight && upto <= SAMPLE_LIST;  // the list takes what lies ahead too
@@ -235,13 +376,12 @@ struct Sampler {
       if (n_list <= SAMPLE_LIST) break;
       // ---- too many: bins of ranks, 2^11 to the candidates' range; after three of these a bin is one value
       uint32_t lo = 0xFFFFFFFFu, hi = 0;
-      for (int i = tid; i < n; i += SAMPLE_THREADS) {
-        const float x = x_at(i);
-        if (x < low || place_of(x, base + i) > within) continue;
+      mine([&](float x, int i) {
+        if (x < low || place_of(x, i) > within) return;
         const uint32_t r = rank_of(x);
         const int b = by_rank ? 0 : bin(x);
         if (by_rank ? r >= r1 && r <= r2 : b >= b1 && b <= b2) lo = min(lo, r), hi = max(hi, r);
-      }
+      });
       lo = __reduce_min_sync(0xFFFFFFFFu, lo), hi = __reduce_max_sync(0xFFFFFFFFu, hi);
       if (tid == 0) sh.first[me] = 0xFFFFFFFFu, sh.last[me] = 0;
       __syncthreads();
@@ -257,13 +397,12 @@ struct Sampler {
       while (((r2 - r1) >> shift) >= SAMPLE_BINS) ++shift;
       clear_hist();
       double over = 0;
-      for (int i = tid; i < n; i += SAMPLE_THREADS) {
-        const float x = x_at(i);
+      mine([&](float x, int i) {
         const uint32_t r = rank_of(x);
-        if (x < low || place_of(x, base + i) > within || r > r2) continue;
+        if (x < low || place_of(x, i) > within || r > r2) return;
         if (r >= r1) atomicAdd(&sh.hist[(r - r1) >> shift], 1u);
         else if (by_weight) over += weight(x);
-      }
+      });
       if (by_weight) {
         double all;
         before<double>(over, sh.scan[0], all);
@@ -295,14 +434,13 @@ struct Sampler {
         const float x0 = value_of(r1);
         double over1 = 0;
         int equal = 0;
-        // (a thread's values side by side: in the order of their indices)
-        const int each = (n + SAMPLE_THREADS - 1) / SAMPLE_THREADS | 1, i0 = min(tid * each, n), i1 = min(i0 + each, n);
-        for (int i = i0; i < i1; ++i) {
-          const float x = x_at(i);
-          if (x < low || place_of(x, base + i) > within) continue;
+        // (a thread's words side by side: in the order of their indices)
+        const int own = (words + THREADS - 1) / THREADS, w0 = min(tid * own, words), w1 = min(w0 + own, words);
+        each(w0, w1, 1, [&](float x, int i) {
+          if (x < low || place_of(x, i) > within) return;
           if (x == x0) ++equal;
           else if (by_weight && x > x0) over1 += weight(x);
-        }
+        });
         double all = 0;
         int all_equal;
         if (by_weight) before<double>(over1, sh.scan[0], all);
@@ -323,32 +461,32 @@ struct Sampler {
         }
         keep = min(keep, there);
         off += before_me;
-        if (off < keep && keep <= off + equal)
-          for (int i = i0, at = off; i < i1; ++i) {
-            const float x = x_at(i);
-            if (x == x0 && place_of(x, base + i) <= within && ++at == keep)
-              for (int r = 0; r < SAMPLE_CTAS; ++r) *cluster.map_shared_rank(&sh.border, r) = place_of(x, base + i);
-          }
+        if (off < keep && keep <= off + equal) {
+          int at = off;
+          each(w0, w1, 1, [&](float x, int i) {
+            if (x == x0 && place_of(x, i) <= within && ++at == keep)
+              for (int r = 0; r < SAMPLE_CTAS; ++r) *cluster.map_shared_rank(&sh.border, r) = place_of(x, i);
+          });
+        }
         cluster.sync();
         return sh.border;
       }
     }
     // ---- the candidates into the first CTA's list
     double over = 0;
-    for (int i = tid; i < n; i += SAMPLE_THREADS) {
-      const float x = x_at(i);
-      const u64 at = place_of(x, base + i);
-      if (x < low || at > within) continue;
+    mine([&](float x, int i) {
+      const u64 at = place_of(x, i);
+      if (x < low || at > within) return;
       const uint32_t r = rank_of(x);
       const int b = by_rank ? 0 : bin(x);
-      if (by_rank ? r > r2 : b > b2) continue;
+      if (by_rank ? r > r2 : b > b2) return;
       if (whole || (by_rank ? r >= r1 : b >= b1)) {
         const int to = atomicAdd(cluster.map_shared_rank(&sh.n_list, 0), 1);
         if (to < SAMPLE_LIST) *cluster.map_shared_rank(&sh.list[to], 0) = at;  // (always)
       } else if (by_weight) {
         over += weight(x);
       }
-    }
+    });
     if (by_weight) {
       double all;
       before<double>(over, sh.scan[0], all);
@@ -362,28 +500,11 @@ struct Sampler {
       if (!by_weight) count = min(count, whole ? k : k - ahead);
       int last = count - 1;
       if (by_weight || (whole && p < 1.0)) {
-        double w[4], sum = 0, all;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int e = 4 * tid + j;
-          w[j] = e < count ? weight(value_of((uint32_t)(sh.list[e] >> 32))) : 0.0;
-          sum += w[j];
-        }
-        double at = before<double>(sum, sh.scan[0], all);
+        double w[PER], all;
+        double at = list_weights(count, false, w, all);
         if (by_weight) at += total(sh.above);
         else target = p * all;
-        if (tid == 0) sh.pick = count - 1;
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          at += w[j];
-          if (4 * tid + j < count && at >= target) {
-            atomicMin(&sh.pick, 4 * tid + j);
-            break;
-          }
-        }
-        __syncthreads();
-        last = sh.pick;
+        last = max(0, list_find(count, w, at, target, false));
       }
       if (tid < SAMPLE_CTAS) *cluster.map_shared_rank(&sh.border, tid) = sh.list[last];
     }
@@ -399,17 +520,21 @@ struct SampleParams {
   int* ids;
   float* prob;
   size_t stride;
-  int n_vocab;
+  int n_vocab, cached;
 };
 
-__global__ void __cluster_dims__(SAMPLE_CTAS, 1, 1) __launch_bounds__(SAMPLE_THREADS) k_sample(const __grid_constant__ SampleParams p) {
+template <int THREADS>
+__global__ void __cluster_dims__(SAMPLE_CTAS, 1, 1) __launch_bounds__(THREADS, 1024 / THREADS) k_sample(const __grid_constant__ SampleParams p) {
   extern __shared__ __align__(16) float s_x[];
   __shared__ SampleShared sh;
+  constexpr int WARPS = THREADS / 32;
   cg::cluster_group cluster = cg::this_cluster();
-  const int tid = threadIdx.x, me = (int)cluster.block_rank(), row = blockIdx.x / SAMPLE_CTAS;
-  // shares of the row that begin at a multiple of four
-  const int per = ((p.n_vocab + SAMPLE_CTAS - 1) / SAMPLE_CTAS + 3) & ~3, base = min(me * per, p.n_vocab), n = min(per, p.n_vocab - base);
-  const float* gx = p.logits + (size_t)row * p.stride + base;
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // waited for ahead of the first word to another CTA: all are there then
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, me = (int)cluster.block_rank(), row = blockIdx.x / SAMPLE_CTAS;
+  const float* x = p.logits + (size_t)row * p.stride;
+  const int lead = (int)((reinterpret_cast<uintptr_t>(x) >> 2) & 3);  // values of the row's first word that are not the row's
+  const int all_words = (p.n_vocab + lead + 3) / 4, per = (all_words + SAMPLE_CTAS - 1) / SAMPLE_CTAS, w0 = min(me * per, all_words);
+  Sampler<THREADS> s = {sh, cluster, p.cached ? s_x : nullptr, x, min(per, all_words - w0), 4 * w0 - lead, p.n_vocab, me, tid, 0.f, 0.0, 0.f, 0.f, 0.f};
   pdl_trigger();
   pdl_wait();
   const float T = p.temperature != nullptr ? __ldcg(p.temperature + row) : 1.f;
@@ -417,112 +542,167 @@ __global__ void __cluster_dims__(SAMPLE_CTAS, 1, 1) __launch_bounds__(SAMPLE_THR
   const float top_p = p.top_p != nullptr ? __ldcg(p.top_p + row) : 1.f, min_p = p.min_p != nullptr ? __ldcg(p.min_p + row) : 0.f;
   const float u = __ldcg(p.u + row);
 
-  // ---- the row into shared memory; its largest value, the least above -inf, and whether all are numbers
-  u64 best = ~0ull;
-  float low = CUDART_INF_F;
-  int odd = 0;
-#pragma unroll 8
-  for (int i = tid; i < n; i += SAMPLE_THREADS) {
-    const float x = __ldcg(gx + i) + 0.f;  // (-0 is 0)
-    if (i < SAMPLE_CAP) s_x[i] = x;
-    odd |= x != x;
-    if (x > -CUDART_INF_F) low = fminf(low, x);
-    best = min(best, place_of(x, base + i));
+  // ---- the row, once: its largest value (NaN where one is), and every thread's largest
+  float top = -CUDART_INF_F;
+#pragma unroll 1
+  for (int v0 = tid; v0 < s.words; v0 += 4 * THREADS) {
+    float4 v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (v0 + k * THREADS < s.words) v[k] = s.from_row(v0 + k * THREADS);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (v0 + k * THREADS >= s.words) break;
+      if (p.cached) *reinterpret_cast<float4*>(s_x + 4 * (v0 + k * THREADS)) = v[k];
+      top = max3_nan(max3_nan(top, v[k].x, v[k].y), v[k].z, v[k].w);
+    }
   }
+  const float my_top = top;
+  float least_top = my_top > -CUDART_INF_F ? my_top : CUDART_INF_F;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
-    best = min(best, __shfl_xor_sync(0xFFFFFFFFu, best, o));
-    low = fminf(low, __shfl_xor_sync(0xFFFFFFFFu, low, o));
+    top = max3_nan(top, top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    least_top = fminf(least_top, __shfl_xor_sync(0xFFFFFFFFu, least_top, o));
   }
-  if (tid == 0) sh.n_list = 0;
-  if ((tid & 31) == 0) sh.list[tid >> 5] = best, sh.scan[0][tid >> 5] = low;
-  odd = __syncthreads_or(odd);
-  for (int w = 0; w < SAMPLE_WARPS; ++w) best = min(best, sh.list[w]), low = fminf(low, (float)sh.scan[0][w]);
-  Sampler s = {sh, cluster, s_x, gx, n, base, me, tid, 0.f, 0.0, 0.f};
-  cluster.sync();  // every CTA is there: its memory may be written
-  s.tell(sh.best, best), s.tell(sh.low, low), s.tell(sh.odd, odd);
+  if (lane == 0) sh.scan_f[0][warp] = top, sh.scan_f[1][warp] = least_top;
+  if (tid == 0) sh.n_list = 0, sh.pick = 0x7FFFFFFF;
+  __syncthreads();
+  for (int w = 0; w < WARPS; ++w) top = max3_nan(top, top, sh.scan_f[0][w]), least_top = fminf(least_top, sh.scan_f[1][w]);
+  asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+  s.tell(sh.top, top), s.tell(sh.least, least_top);
   cluster.sync();
-  for (int r = 0; r < SAMPLE_CTAS; ++r) best = min(best, sh.best[r]), odd |= sh.odd[r];
-  s.top = value_of((uint32_t)(best >> 32));
-  const bool none = odd || s.top == -CUDART_INF_F, greedy = !(T > 0.f) || top_k == 1;
-  if (none || greedy) {
+  for (int r = 0; r < SAMPLE_CTAS; ++r) top = max3_nan(top, top, sh.top[r]), least_top = fminf(least_top, sh.least[r]);
+  s.top = top;
+  const bool none = !(top > -CUDART_INF_F);
+  if (none || !(T > 0.f) || top_k == 1 || top_p <= 0.f) {
+    // ---- nothing to take, or the first of the largest
+    if (my_top == top) s.mine([&](float y, int i) {
+      if (y == top) atomicMin(&sh.pick, i);
+    });
+    __syncthreads();
+    s.tell(sh.best, sh.pick);
+    cluster.sync();
     if (me == 0 && tid == 0) {
-      p.ids[row] = none ? -1 : (int)(uint32_t)best;
+      int id = sh.best[0];
+      for (int r = 1; r < SAMPLE_CTAS; ++r) id = min(id, sh.best[r]);
+      p.ids[row] = none ? -1 : id;
       if (p.prob != nullptr) p.prob[row] = none ? 0.f : 1.f;
     }
-    cluster.sync();
     return;
   }
   s.inv_t = 1.0 / (double)T;
   // (an infinite largest value leaves those like it; rounded down, never up)
-  const double reach = (double)s.top - SAMPLE_REACH * (double)T;
-  s.floor_x = s.top == CUDART_INF_F ? s.top : reach > -3.0e38 ? __double2float_rd(reach) : -3.402823466e38f;
+  const double reach = (double)top - SAMPLE_REACH * (double)T;
+  s.floor_x = top == CUDART_INF_F ? top : reach > -3.0e38 ? __double2float_rd(reach) : -3.402823466e38f;
+  const double least = min_p > 0.f ? fmin((double)min_p, 1.0) : 0.0, part = u > 0.f ? fmin((double)u, 1.0) : 0.0;
 
   u64 border = ~0ull;
   bool both = false;
-  if (top_k > 0 && top_k < p.n_vocab) border = s.find(border, top_k, (double)top_p, &both);
-  if (top_p < 1.f && !both) {
-    if (top_p > 0.f) {
-      bool done;
-      cluster.sync();
-      border = s.find(border, 0, (double)top_p, &done);
-    } else {
-      border = best;
+  if (top_k > 0 && top_k < p.n_vocab) {
+    if (top_k <= SAMPLE_FEW && s.few_largest(top_k, my_top, least_top)) {
+      cluster.sync();  // (all have read how many)
+      if (me == 0) s.from_list(top_k, (double)top_p, least, part, p.ids + row, p.prob != nullptr ? p.prob + row : nullptr);
+      return;
     }
+    if (top_k <= SAMPLE_FEW) cluster.sync();
+    border = s.find(border, top_k, (double)top_p, &both);
+  }
+  if (top_p < 1.f && !both) {
+    bool done;
+    cluster.sync();
+    border = s.find(border, 0, (double)top_p, &done);
   }
 
-  // ---- the kept weights in the order of the tokens: a thread's side by side
-  const double least = min_p > 0.f ? fmin((double)min_p, 1.0) : 0.0;
-  const int each = (n + SAMPLE_THREADS - 1) / SAMPLE_THREADS | 1, i0 = min(tid * each, n), i1 = min(i0 + each, n);
-  auto kept = [&](int i) {
-    const float x = s.x_at(i);
-    if (x < s.floor_x || place_of(x, base + i) > border) return 0.0;
-    const double w = s.weight(x);
+  // ---- the kept weights in the order of the tokens: a warp's words side by side
+  const float border_x = value_of((uint32_t)(border >> 32));
+  const int border_i = (int)(uint32_t)border;
+  const int own = (s.words + WARPS - 1) / WARPS, v0 = min(warp * own, s.words), v1 = min(v0 + own, s.words);
+  const bool cut = border != ~0ull;
+  auto kept = [&](float y, int i) {
+    if (y < s.floor_x || (cut && (y < border_x || (y == border_x && i > border_i)))) return 0.0;
+    const double w = s.weight(y);
     return w >= least ? w : 0.0;
   };
-  double sum = 0, all;
-  for (int i = i0; i < i1; ++i) sum += kept(i);
-  double at = s.before<double>(sum, sh.scan[0], all);
-  if (tid == 0) sh.pick = -1;
+  double sum = 0;
+  s.each(v0 + lane, v1, 32, [&](float y, int i) { sum += kept(y, i); });
+  sum = s.warp_total(sum);
+  __syncthreads();
+  if (lane == 0) sh.scan[0][warp] = sum;
+  __syncthreads();
+  double all = 0;
+  for (int w = 0; w < WARPS; ++w) all += sh.scan[0][w];
   s.tell(sh.kept, all);
   cluster.sync();
-  const double whole = s.total(sh.kept), want = (u > 0.f ? fmin((double)u, 1.0) : 0.0) * whole;
+  const double whole = s.total(sh.kept), want = part * whole;
   int owner = 0;
-  double off = 0, mine = 0;
+  double off = 0, at = 0;
   for (int r = 0; r < SAMPLE_CTAS; ++r) {  // the last CTA with weights that begins at or before it
-    if (sh.kept[r] > 0 && off <= want) owner = r, mine = off;
+    if (sh.kept[r] > 0 && off <= want) owner = r, at = off;
     off += sh.kept[r];
   }
-  if (owner == me) {
-    at += mine;
-    if (sum > 0 && at <= want) atomicMax(&sh.pick, tid);
-    __syncthreads();
-    if (tid == sh.pick) {
-      int id = -1;
-      double w = 0;
-      for (int i = i0; i < i1; ++i) {
-        const double x = kept(i);
-        if (x <= 0) continue;
-        id = i, w = x;
-        at += x;
-        if (at > want) break;
-      }
-      p.ids[row] = base + id;
-      if (p.prob != nullptr) p.prob[row] = (float)(w / whole);
-    }
+  if (owner != me) return;
+  int from = 0;
+  off = at;
+  for (int w = 0; w < WARPS; ++w) {  // and its last such warp
+    if (sh.scan[0][w] > 0 && off <= want) from = w, at = off;
+    off += sh.scan[0][w];
   }
-  cluster.sync();
+  if (from != warp) return;
+  // its words again, 32 at a time: the first value that passes, or the last with a weight
+  int id = -1;
+  double w_id = 0;
+#pragma unroll 1
+  for (int v = v0; v < v1; v += 32) {
+    double w[4] = {0, 0, 0, 0};
+    const int i = s.base + 4 * (v + lane);
+    if (v + lane < v1) {
+      const float4 y = s.word(v + lane);
+      w[0] = kept(y.x, i), w[1] = kept(y.y, i + 1), w[2] = kept(y.z, i + 2), w[3] = kept(y.w, i + 3);
+    }
+    double ahead = (w[0] + w[1]) + (w[2] + w[3]);
+    const double four = ahead;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double y = __shfl_up_sync(0xFFFFFFFFu, ahead, o);
+      if (lane >= o) ahead += y;
+    }
+    const double next = at + __shfl_sync(0xFFFFFFFFu, ahead, 31);
+    double here = at + (ahead - four);
+    int mine = -1, last = -1;
+    double w_mine = 0, w_last = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      here += w[j];
+      if (w[j] <= 0) continue;
+      last = i + j, w_last = w[j];
+      if (mine < 0 && here > want) mine = last, w_mine = w_last;
+    }
+    const uint32_t has = __ballot_sync(0xFFFFFFFFu, mine >= 0), any = __ballot_sync(0xFFFFFFFFu, last >= 0);
+    const int lane_at = has ? __ffs(has) - 1 : any ? 31 - __clz(any) : 0;
+    if (has || any) {
+      id = __shfl_sync(0xFFFFFFFFu, has ? mine : last, lane_at);
+      w_id = __shfl_sync(0xFFFFFFFFu, has ? w_mine : w_last, lane_at);
+    }
+    if (has) break;
+    at = next;
+  }
+  if (lane == 0) {
+    p.ids[row] = id;
+    if (p.prob != nullptr) p.prob[row] = (float)(w_id / whole);
+  }
 }
 
 }  // namespace
 
 int32_t launch_sample(infr_cuda_ctx* ctx, const float* logits, const float* u, const float* temperature, const int* top_k, const float* top_p, const float* min_p, int* ids,
                       float* prob, size_t stride, int rows, int n_vocab) {
-  const SampleParams p = {logits, u, temperature, top_p, min_p, top_k, ids, prob, stride, n_vocab};
-  const int per = ((n_vocab + SAMPLE_CTAS - 1) / SAMPLE_CTAS + 3) & ~3;
-  const size_t smem = (size_t)(per < SAMPLE_CAP ? per : SAMPLE_CAP) * 4;
-  cudaError_t e = ensure_smem(reinterpret_cast<const void*>(&k_sample), (size_t)SAMPLE_CAP * 4);
-  if (e == cudaSuccess) e = launch_ex(k_sample, dim3((unsigned)rows * SAMPLE_CTAS), dim3(SAMPLE_THREADS), smem, ctx->stream, true, p);
+  SampleParams p = {logits, u, temperature, top_p, min_p, top_k, ids, prob, stride, n_vocab, 0};
+  const int per = ((n_vocab + 3 + 3) / 4 + SAMPLE_CTAS - 1) / SAMPLE_CTAS * 4;
+  p.cached = rows <= 16 && per <= SAMPLE_CAP;
+  const size_t smem = p.cached ? (size_t)per * 4 : 0;
+  const auto kernel = p.cached ? k_sample<512> : k_sample<256>;
+  cudaError_t e = ensure_smem(reinterpret_cast<const void*>(kernel), p.cached ? (size_t)SAMPLE_CAP * 4 : 0);
+  if (e == cudaSuccess) e = launch_ex(kernel, dim3((unsigned)rows * SAMPLE_CTAS), dim3(p.cached ? 512 : 256), smem, ctx->stream, true, p);
   if (e != cudaSuccess) return check_cuda(ctx, e, "k_sample launch");
   ctx->launches += 1;
   return check_cuda(ctx, cudaGetLastError(), "k_sample launch");
