@@ -10,8 +10,8 @@
 // go by the order of the additions, and there are 10^5 borders to a row.  Weights below 2^-64 of the largest count as none: all of them together are 2^-46,
 // which an f32 u cannot tell from nothing.
 //
-// A cluster of eight CTAs has a row in its shared memory: the logits are read once.  Every decision is made from numbers that all eight have, in the same order,
-// so that they take the same steps; what is shared goes through distributed shared memory, a cluster barrier behind it.
+// A cluster of eight CTAs has a row.  Every decision is made from numbers that all eight have got from one of them, added up in the same order, so that they
+// take the same steps and meet at the same barriers whatever the row and its settings hold (and should somebody write them meanwhile).
 #include <cooperative_groups.h>
 #include <math_constants.h>
 
@@ -25,7 +25,9 @@ namespace cg = cooperative_groups;
 constexpr int SAMPLE_CTAS = 8;
 constexpr int SAMPLE_BINS = 2048;
 constexpr int SAMPLE_LIST = 2048;     // candidates that are sorted
-constexpr int SAMPLE_FEW = 1024;      // so many largest ones are looked for among the threads' largest first
+constexpr int SAMPLE_FEW = 192;       // so many largest ones are looked for among the threads' largest first,
+constexpr int SAMPLE_FEW_BINS = 256;  // by bins of these,
+constexpr int SAMPLE_SLOTS = 64;      // and so many candidates of a CTA looked at
 constexpr int SAMPLE_CAP = 40960;     // values of a row in a CTA's shared memory at most
 constexpr double SAMPLE_REACH = 45.0; // weights down to e^-45 < 2^-64
 typedef unsigned long long u64;
@@ -44,20 +46,31 @@ __device__ __forceinline__ uint32_t rank_of(float x) {
 __device__ __forceinline__ float value_of(uint32_t r) { return __uint_as_float(r & 0x80000000u ? r : 0x7FFFFFFFu - r); }
 __device__ __forceinline__ u64 place_of(float x, int i) { return (u64)rank_of(x) << 32 | (uint32_t)i; }
 
-struct SampleShared {
+struct __align__(16) SampleShared {
   uint32_t hist[SAMPLE_BINS];
-  u64 list[SAMPLE_LIST];
+  union {
+    u64 list[SAMPLE_LIST];
+    struct {
+      u64 few[SAMPLE_CTAS * SAMPLE_SLOTS];      // the candidates by CTA, then by rank
+      double few_weight[SAMPLE_CTAS * SAMPLE_SLOTS];
+      uint32_t few_hist[SAMPLE_CTAS][SAMPLE_FEW_BINS];
+    };
+  };
+  uint32_t sums[SAMPLE_BINS];  // of all CTAs' hist
+  double power[32];            // 2^(j / 32)
   double scan[2][16];
   int scan_n[16];
   float scan_f[2][16];
   // from every CTA, by rank
   float top[SAMPLE_CTAS], least[SAMPLE_CTAS];
-  int best[SAMPLE_CTAS];
+  float temperature, top_p, min_p, u;  // from the first CTA
+  int top_k;
+  int best[SAMPLE_CTAS], n_few[SAMPLE_CTAS];
   double sum[SAMPLE_CTAS], above[SAMPLE_CTAS], kept[SAMPLE_CTAS];
   uint32_t first[SAMPLE_CTAS], last[SAMPLE_CTAS];
   int equal[SAMPLE_CTAS];
   // the first CTA's
-  int n_list;
+  int n_list, done;
   u64 border;
   // of the bins
   int b1, b2, ahead, upto;
@@ -75,7 +88,7 @@ struct Sampler {
   int words, base, n_vocab;  // index of the first value: may be negative
   int me, tid;
   float top;             // the row's largest value
-  double inv_t;
+  double steps;          // thirty-seconds of an octave to a unit of the logits: 32 log2(e) / T
   float floor_x;         // values from here on have a weight
 
   __device__ float4 from_row(int w) const {
@@ -91,21 +104,49 @@ struct Sampler {
   template <class F>
   __device__ __forceinline__ void each(int from, int to, int step, F f) const {
 #pragma unroll 1
-    for (int w0 = from; w0 < to; w0 += 4 * step) {
-      float4 v[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (w0 + k * step < to) v[k] = word(w0 + k * step);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
+    for (int w0 = from; w0 < to; w0 += 2 * step) {
+      const bool two = w0 + step < to;
+      const float4 a = word(w0);
+      float4 b = make_float4(-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F);
+      if (two) b = word(w0 + step);
+#pragma unroll 1
+      for (int k = 0; k < 2; ++k) {
+        const float4 v = k == 0 ? a : b;
         const int i = base + 4 * (w0 + k * step);
-        if (w0 + k * step < to) f(v[k].x, i), f(v[k].y, i + 1), f(v[k].z, i + 2), f(v[k].w, i + 3);
+        f(v.x, i), f(v.y, i + 1), f(v.z, i + 2), f(v.w, i + 3);
       }
     }
   }
   template <class F>
   __device__ __forceinline__ void mine(F f) const { each(tid, words, THREADS, f); }
-  __device__ double weight(float x) const { return x < floor_x ? 0.0 : x == top ? 1.0 : exp(((double)x - (double)top) * inv_t); }
+  // 2^(t / 32) of 64 bits, t <= 0: a table and the exponent for the whole part, five terms of e^r behind the first for the rest, |r| <= log(2) / 64: 2e-15.
+  __device__ __forceinline__ double power32(double t) const {
+    const double m = t + 6755399441055744.0;  // 1.5 2^52: the sum's low word is t rounded
+    const int k = __double2loint(m);
+    const double r = (t - (m - 6755399441055744.0)) * (0.69314718055994531 / 32);
+    const double e = fma(r, fma(r, fma(r, fma(r, fma(r, 1.0 / 120, 1.0 / 24), 1.0 / 6), 0.5), 1.0), 1.0) * sh.power[k & 31];
+    return __hiloint2double(__double2hiint(e) + (k >> 5) * (1 << 20), __double2loint(e));
+  }
+  // exp((x - top) / T)
+  __device__ __forceinline__ double weight(float x) const { return x < floor_x ? 0.0 : x == top ? 1.0 : power32(((double)x - (double)top) * steps); }
+  // Whether a value is one of those up to a border.
+  struct Upto {
+    float x;
+    int i;
+    bool all;
+    __device__ explicit Upto(u64 border) : x(value_of((uint32_t)(border >> 32))), i((int)(uint32_t)border), all(border == ~0ull) {}
+    __device__ __forceinline__ bool has(float y, int j) const { return all || y > x || (y == x && j <= i); }
+  };
+  // The weight of all values into every CTA's sum; there behind the next cluster barrier.
+  __device__ void sum_up(u64 within) {
+    const Upto in(within);
+    double sum = 0, all;
+    mine([&](float x, int i) {
+      if (in.has(x, i)) sum += weight(x);
+    });
+    before<double>(sum, sh.scan[0], all);
+    tell(sh.sum, all);
+  }
 
   template <typename T>
   __device__ T warp_total(T v) const {
@@ -141,6 +182,10 @@ struct Sampler {
   __device__ void tell(T* array, T v) {
     if (tid < SAMPLE_CTAS) *cluster.map_shared_rank(array + me, tid) = v;
   }
+  // The first CTA's word to all.
+  __device__ void tell_one(int* word, int v) {
+    if (tid < SAMPLE_CTAS) *cluster.map_shared_rank(word, tid) = v;
+  }
   __device__ void clear_hist() {
     for (int b = tid; b < SAMPLE_BINS; b += THREADS) sh.hist[b] = 0;
     if (tid == 0) sh.n_list = 0, sh.b1 = sh.b2 = SAMPLE_BINS;
@@ -157,16 +202,26 @@ struct Sampler {
   // (`slack`: by how much of a weight a bin's edges are off)
   template <class Edge>
   __device__ void bracket(bool by_weight, int k, double target, double slack, Edge edge) {
+    // every CTA adds up an eighth of the bins, and tells the sums to all
+    constexpr int EIGHTH = SAMPLE_BINS / SAMPLE_CTAS / 4;
+    static_assert(EIGHTH * SAMPLE_CTAS % THREADS == 0, "every thread takes part in every round");
+#pragma unroll 1
+    for (int e = tid; e < EIGHTH * SAMPLE_CTAS; e += THREADS) {
+      const int at = me * EIGHTH + e / SAMPLE_CTAS;  // four bins, by eight neighbouring threads
+      uint4 h = reinterpret_cast<const uint4*>(cluster.map_shared_rank(sh.hist, e % SAMPLE_CTAS))[at];
+#pragma unroll
+      for (int o = 1; o < SAMPLE_CTAS; o <<= 1) {
+        h.x += __shfl_xor_sync(0xFFFFFFFFu, h.x, o), h.y += __shfl_xor_sync(0xFFFFFFFFu, h.y, o);
+        h.z += __shfl_xor_sync(0xFFFFFFFFu, h.z, o), h.w += __shfl_xor_sync(0xFFFFFFFFu, h.w, o);
+      }
+      reinterpret_cast<uint4*>(cluster.map_shared_rank(sh.sums, e % SAMPLE_CTAS))[at] = h;
+    }
+    cluster.sync();
     uint32_t c[PER], sum_c = 0;
 #pragma unroll
-    for (int j = 0; j < PER; ++j) c[j] = 0;
-#pragma unroll
-    for (int r = 0; r < SAMPLE_CTAS; ++r) {
-#pragma unroll
-      for (int j = 0; j < PER; j += 4) {
-        const uint4 h = *reinterpret_cast<const uint4*>(cluster.map_shared_rank(sh.hist, r) + PER * tid + j);
-        c[j] += h.x, c[j + 1] += h.y, c[j + 2] += h.z, c[j + 3] += h.w;
-      }
+    for (int j = 0; j < PER; j += 4) {
+      const uint4 h = *reinterpret_cast<const uint4*>(sh.sums + PER * tid + j);
+      c[j] = h.x, c[j + 1] = h.y, c[j + 2] = h.z, c[j + 3] = h.w;
     }
 #pragma unroll
     for (int j = 0; j < PER; ++j) sum_c += c[j];
@@ -275,40 +330,6 @@ struct Sampler {
     return to;
   }
 
-  // The k largest are in the first CTA's list: the token, by itself.
-  __device__ void from_list(int k, double p, double least, double u, int* id, float* prob) {
-    int count = min(sh.n_list, SAMPLE_LIST);
-    sort_list(count);
-    count = min(count, k);
-    double w[PER], all;
-    double at = list_weights(count, false, w, all);
-    if (p < 1.0) count = list_find(count, w, at, p * all, false) + 1;
-    // (those with no weight are at the end)
-    int n = 0;
-#pragma unroll
-    for (int j = 0; j < PER; ++j) n += PER * tid + j < count && w[j] > 0 && w[j] >= least;
-    before<int>(n, sh.scan_n, count);
-    u64 mine[PER];
-#pragma unroll
-    for (int j = 0; j < PER; ++j) mine[j] = PER * tid + j < count ? sh.list[PER * tid + j] : 0;
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < PER; ++j)
-      if (PER * tid + j < count) sh.list[PER * tid + j] = mine[j] << 32 | mine[j] >> 32;
-    __syncthreads();
-    sort_list(count);
-    at = list_weights(count, true, w, all);
-    const int e = list_find(count, w, at, u * all, true);
-    if (PER * tid <= e && e < PER * tid + PER) {
-      *id = (int)(sh.list[e] >> 32);
-      double we = 0;
-#pragma unroll
-      for (int j = 0; j < PER; ++j)
-        if (PER * tid + j == e) we = w[j];
-      if (prob != nullptr) *prob = (float)(we / all);
-    }
-  }
-
   // Bins of one width from the largest value down to `low`: the nearest edge, so that a value is within half a bin (and f32's 2^-22 of its distance).
   // (A difference of halves does not overflow.)
   float bin_scale, bin_half;
@@ -321,51 +342,130 @@ struct Sampler {
     return (int)(__float_as_uint(b) & (SAMPLE_BINS - 1));
   }
 
-  // Whether the k largest are in the first CTA's list: those that share a bin with the k-th largest of the threads' largest, or are larger, if they are not
-  // too many.  Only the threads that have such a one look through their values again.
-  __device__ bool few_largest(int k, float my_top, float least_top) {
-    set_bins(least_top);
-    clear_hist();
-    if (my_top > -CUDART_INF_F) atomicAdd(&sh.hist[bin(my_top)], 1u);
+  // The token where no more than the k largest are needed: they are among the values that share a bin with the k-th largest of the threads' largest, or are
+  // larger, and only the threads that have such a one look through their values again.  The first CTA sorts these by counting (a thread to each) and takes the
+  // token by itself.  all_weight > 0: the weight of the whole row, of which the run has p (and which may need more than these); else of the k largest.
+  // False: too many candidates, or too few.
+  __device__ bool few_largest(int k, bool of_all, double p, double least, double u, float my_top, float least_top, int* id, float* prob) {
+    const double width = top > least_top ? (SAMPLE_FEW_BINS - 1) / (0.5 * ((double)top - (double)least_top)) : 0.0;
+    const float scale = (float)width, half = 0.5f * top;
+    auto few_bin = [&](float x) { return min((int)(fmaf(-0.5f, x, half) * scale), SAMPLE_FEW_BINS - 1); };
+    if (tid < SAMPLE_FEW_BINS) sh.hist[tid] = 0;
+    if (tid == 0) sh.n_list = 0, sh.done = 0;
+    __syncthreads();
+    const bool has = my_top > -CUDART_INF_F;
+    const int my_bin = has ? few_bin(my_top) : SAMPLE_FEW_BINS;
+    if (has) atomicAdd(&sh.hist[my_bin], 1u);
+    __syncthreads();
+    for (int e = tid; e < SAMPLE_FEW_BINS * SAMPLE_CTAS; e += THREADS)
+      cluster.map_shared_rank(&sh.few_hist[me][0], e / SAMPLE_FEW_BINS)[e % SAMPLE_FEW_BINS] = sh.hist[e % SAMPLE_FEW_BINS];
     cluster.sync();
-    bracket(false, k, 0.0, 0.0, [](int) { return 0.0; });
-    const int b2 = sh.b2;
-    if (b2 < 0) return false;
-    if (my_top > -CUDART_INF_F && bin(my_top) <= b2)
-      mine([&](float x, int i) {
-        if (x == -CUDART_INF_F || bin(x) > b2) return;
-        const int to = atomicAdd(cluster.map_shared_rank(&sh.n_list, 0), 1);
-        if (to < SAMPLE_LIST) *cluster.map_shared_rank(&sh.list[to], 0) = place_of(x, i);
-      });
+    int c = 0, all;
+    if (tid < SAMPLE_FEW_BINS)
+      for (int r = 0; r < SAMPLE_CTAS; ++r) c += (int)sh.few_hist[r][tid];
+    const int ahead = before<int>(c, sh.scan_n, all);
+    if (ahead < k && k <= ahead + c) sh.b2 = tid;
+    __syncthreads();
+    const int b2 = all >= k ? sh.b2 : -1;
+    // a warp's lanes together for each of its threads that have candidates
+#pragma unroll 1
+    for (uint32_t ask = __ballot_sync(0xFFFFFFFFu, my_bin <= b2); ask; ask &= ask - 1) {
+      const int from = (tid & ~31) + __ffs(ask) - 1;
+#pragma unroll 1
+      for (int w = from + (tid & 31) * THREADS; w < words; w += 32 * THREADS) {
+        const float4 v = word(w);
+        const float x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (x[j] > -CUDART_INF_F && few_bin(x[j]) <= b2) {
+            const int to = atomicAdd(&sh.n_list, 1);
+            if (to < SAMPLE_SLOTS) *cluster.map_shared_rank(&sh.few[me * SAMPLE_SLOTS + to], 0) = place_of(x[j], base + 4 * w + j);
+          }
+      }
+    }
+    __syncthreads();
+    tell(sh.n_few, b2 < 0 ? SAMPLE_SLOTS + 1 : sh.n_list);
     cluster.sync();
-    return *cluster.map_shared_rank(&sh.n_list, 0) <= SAMPLE_LIST;
+    int n = 0;
+    for (int r = 0; r < SAMPLE_CTAS; ++r) {
+      if (sh.n_few[r] > SAMPLE_SLOTS) return false;
+      n += sh.n_few[r];
+    }
+    if (n > THREADS) return false;
+    bool done = true;
+    if (me == 0) {
+      // thread e has candidate e
+      u64 at = ~0ull;
+      int e = tid;
+      for (int r = 0; r < SAMPLE_CTAS; ++r) {
+        if (e >= 0 && e < sh.n_few[r]) at = sh.few[r * SAMPLE_SLOTS + e];
+        e -= sh.n_few[r];
+      }
+      double w = tid < n ? weight(value_of((uint32_t)(at >> 32))) : 0.0;
+      __syncthreads();
+      if (tid < n) sh.few[tid] = at;
+      __syncthreads();
+      int rank = 0;
+#pragma unroll 4
+      for (int i = 0; i < n; ++i) rank += sh.few[i] < at;
+      __syncthreads();
+      if (tid < n) sh.few[rank] = at, sh.few_weight[rank] = w;
+      __syncthreads();
+      // thread r has rank r
+      at = tid < n ? sh.few[tid] : ~0ull;
+      w = tid < n && (of_all || tid < k) ? sh.few_weight[tid] : 0.0;
+      int count = of_all ? n : min(n, k);
+      if (p < 1.0) {
+        double sum;
+        const double ahead_w = before<double>(w, sh.scan[0], sum), target = p * (of_all ? total(sh.sum) : sum);
+        // (as they are added one by one, the first with which the sum reaches the target is the last)
+        const int over = __syncthreads_count(tid < count && !(ahead_w + w >= target));
+        done = over < count || !of_all;
+        count = min(count, over + 1);
+      }
+      if (tid < count && (w <= 0 || w < least)) w = 0.0;
+      if (tid < count) sh.few_weight[tid] = w;
+      if (tid == 0) sh.pick = -1;
+      __syncthreads();
+      const int index = (int)(uint32_t)at;
+      double lower = 0, kept = 0;
+#pragma unroll 4
+      for (int i = 0; i < count; ++i) {
+        const double x = sh.few_weight[i];
+        kept += x;
+        if ((int)(uint32_t)sh.few[i] < index) lower += x;
+      }
+      if (tid < count && w > 0 && lower <= u * kept) atomicMax(&sh.pick, index);
+      __syncthreads();
+      if (done && tid < count && w > 0 && index == sh.pick) {
+        *id = index;
+        if (prob != nullptr) *prob = (float)(w / kept);
+      }
+    }
+    if (!of_all) return true;  // (nothing of another CTA is waited for)
+    if (me == 0) tell_one(&sh.done, done ? 1 : 0);
+    cluster.sync();
+    return sh.done != 0;
   }
 
   // The border among the values up to `within`: that of the k largest, or with p < 1 that of the run with p of the weight, or (k, then p) both where the
   // candidates hold all of the k; *both: whether they did.
-  __device__ u64 find(u64 within, int k, double p, bool* both) {
+  __device__ __noinline__ u64 find(u64 within, int k, double p, bool* both) {
     const bool by_weight = k <= 0;
+    const Upto in(within);
     *both = false;
     // ---- bins down to the least value that has a weight (a border of the k largest may lie behind: then nothing is left out)
     const float low = floor_x;
     set_bins(low);
     clear_hist();
-    double sum = 0;
     mine([&](float x, int i) {
-      if (x < low || place_of(x, i) > within) return;
-      atomicAdd(&sh.hist[bin(x)], 1u);
-      if (by_weight) sum += weight(x);
+      if (x >= low && in.has(x, i)) atomicAdd(&sh.hist[bin(x)], 1u);
     });
-    if (by_weight) {
-      double all;
-      before<double>(sum, sh.scan[0], all);
-      tell(sh.sum, all);
-    }
     cluster.sync();
     double target = by_weight ? p * total(sh.sum) : 0;
-    const double width = bin_scale > 0.f ? 2.0 * inv_t / bin_scale : 0.0;
+    const double width = bin_scale > 0.f ? 2.0 * steps / bin_scale : 0.0;
     // (f32 moves a bin's edges by 2^-22 of their distance from the largest, which is 45 in the exponent at most)
-    bracket(by_weight, k, target, 3e-5, [&](int b) { return exp((0.5 - b) * width); });
+    bracket(by_weight, k, target, 3e-5, [&](int b) { return power32((0.5 - b) * width); });
     int b1 = sh.b1, b2 = sh.b2, ahead = sh.ahead, upto = sh.upto;
     if (b1 < 0) return within;
     bool whole = !by_weight && upto <= SAMPLE_LIST;  // the list takes what lies ahead too
@@ -377,7 +477,7 @@ struct Sampler {
       // ---- too many: bins of ranks, 2^11 to the candidates' range; after three of these a bin is one value
       uint32_t lo = 0xFFFFFFFFu, hi = 0;
       mine([&](float x, int i) {
-        if (x < low || place_of(x, i) > within) return;
+        if (x < low || !in.has(x, i)) return;
         const uint32_t r = rank_of(x);
         const int b = by_rank ? 0 : bin(x);
         if (by_rank ? r >= r1 && r <= r2 : b >= b1 && b <= b2) lo = min(lo, r), hi = max(hi, r);
@@ -399,7 +499,7 @@ struct Sampler {
       double over = 0;
       mine([&](float x, int i) {
         const uint32_t r = rank_of(x);
-        if (x < low || place_of(x, i) > within || r > r2) return;
+        if (x < low || r > r2 || !in.has(x, i)) return;
         if (r >= r1) atomicAdd(&sh.hist[(r - r1) >> shift], 1u);
         else if (by_weight) over += weight(x);
       });
@@ -415,17 +515,15 @@ struct Sampler {
         const u64 r = r1 + ((u64)b << shift);
         return r > r2 ? 0.0 : weight(value_of((uint32_t)r));
       });
-      if (by_weight && (shift == 0 || level >= 8) && sh.b1 != sh.b2 && sh.upto - sh.ahead > SAMPLE_LIST) {
-        // bins of one value each: the sums are what they are, the first that passes the target is the one.  (And so that this ends whatever the values are.)
-        if (tid == 0) sh.b2 = sh.b1;
-        __syncthreads();
-        uint32_t c = 0;
-        for (int r = 0; r < SAMPLE_CTAS; ++r) c += cluster.map_shared_rank(sh.hist, r)[sh.b1];
-        if (tid == 0) sh.upto = sh.ahead + (int)c;
-        __syncthreads();
-      }
       b1 = sh.b1, b2 = sh.b2;
-      ahead = was + sh.ahead, upto = was + sh.upto;
+      if (b1 < 0 || level >= 16) return within;  // (not with values that stay as they are)
+      int in_bins = sh.upto - sh.ahead;
+      if (by_weight && (shift == 0 || level >= 8) && b1 != b2 && in_bins > SAMPLE_LIST) {
+        // bins of one value each: the sums are what they are, the first that passes the target is the one.  (And so that the range becomes a bin's at last.)
+        b2 = b1;
+        in_bins = (int)sh.sums[b1];
+      }
+      ahead = was + sh.ahead, upto = ahead + in_bins;
       r2 = (uint32_t)min((u64)r2, r1 + (((u64)b2 + 1) << shift) - 1);
       r1 = r1 + ((uint32_t)b1 << shift);
       whole = false;
@@ -437,7 +535,7 @@ struct Sampler {
         // (a thread's words side by side: in the order of their indices)
         const int own = (words + THREADS - 1) / THREADS, w0 = min(tid * own, words), w1 = min(w0 + own, words);
         each(w0, w1, 1, [&](float x, int i) {
-          if (x < low || place_of(x, i) > within) return;
+          if (x < low || !in.has(x, i)) return;
           if (x == x0) ++equal;
           else if (by_weight && x > x0) over1 += weight(x);
         });
@@ -464,7 +562,7 @@ struct Sampler {
         if (off < keep && keep <= off + equal) {
           int at = off;
           each(w0, w1, 1, [&](float x, int i) {
-            if (x == x0 && place_of(x, i) <= within && ++at == keep)
+            if (x == x0 && in.has(x, i) && ++at == keep)
               for (int r = 0; r < SAMPLE_CTAS; ++r) *cluster.map_shared_rank(&sh.border, r) = place_of(x, i);
           });
         }
@@ -475,14 +573,13 @@ struct Sampler {
     // ---- the candidates into the first CTA's list
     double over = 0;
     mine([&](float x, int i) {
-      const u64 at = place_of(x, i);
-      if (x < low || at > within) return;
+      if (x < low || !in.has(x, i)) return;
       const uint32_t r = rank_of(x);
       const int b = by_rank ? 0 : bin(x);
       if (by_rank ? r > r2 : b > b2) return;
       if (whole || (by_rank ? r >= r1 : b >= b1)) {
         const int to = atomicAdd(cluster.map_shared_rank(&sh.n_list, 0), 1);
-        if (to < SAMPLE_LIST) *cluster.map_shared_rank(&sh.list[to], 0) = at;  // (always)
+        if (to < SAMPLE_LIST) *cluster.map_shared_rank(&sh.list[to], 0) = place_of(x, i);  // (always)
       } else if (by_weight) {
         over += weight(x);
       }
@@ -498,7 +595,7 @@ struct Sampler {
       int count = min(sh.n_list, SAMPLE_LIST);
       sort_list(count);
       if (!by_weight) count = min(count, whole ? k : k - ahead);
-      int last = count - 1;
+      int last = max(0, count - 1);
       if (by_weight || (whole && p < 1.0)) {
         double w[PER], all;
         double at = list_weights(count, false, w, all);
@@ -535,12 +632,18 @@ __global__ void __cluster_dims__(SAMPLE_CTAS, 1, 1) __launch_bounds__(THREADS, 1
   const int lead = (int)((reinterpret_cast<uintptr_t>(x) >> 2) & 3);  // values of the row's first word that are not the row's
   const int all_words = (p.n_vocab + lead + 3) / 4, per = (all_words + SAMPLE_CTAS - 1) / SAMPLE_CTAS, w0 = min(me * per, all_words);
   Sampler<THREADS> s = {sh, cluster, p.cached ? s_x : nullptr, x, min(per, all_words - w0), 4 * w0 - lead, p.n_vocab, me, tid, 0.f, 0.0, 0.f, 0.f, 0.f};
+  if (tid < 32) sh.power[tid] = exp2(tid * 0.03125);
   pdl_trigger();
   pdl_wait();
-  const float T = p.temperature != nullptr ? __ldcg(p.temperature + row) : 1.f;
-  const int top_k = p.top_k != nullptr ? __ldcg(p.top_k + row) : 0;
-  const float top_p = p.top_p != nullptr ? __ldcg(p.top_p + row) : 1.f, min_p = p.min_p != nullptr ? __ldcg(p.min_p + row) : 0.f;
-  const float u = __ldcg(p.u + row);
+  float T = 1.f, top_p = 1.f, min_p = 0.f, u = 0.f;
+  int top_k = 0;
+  if (me == 0 && tid < SAMPLE_CTAS) {
+    if (p.temperature != nullptr) T = __ldcg(p.temperature + row);
+    if (p.top_k != nullptr) top_k = __ldcg(p.top_k + row);
+    if (p.top_p != nullptr) top_p = __ldcg(p.top_p + row);
+    if (p.min_p != nullptr) min_p = __ldcg(p.min_p + row);
+    u = __ldcg(p.u + row);
+  }
 
   // ---- the row, once: its largest value (NaN where one is), and every thread's largest
   float top = -CUDART_INF_F;
@@ -570,7 +673,12 @@ __global__ void __cluster_dims__(SAMPLE_CTAS, 1, 1) __launch_bounds__(THREADS, 1
   for (int w = 0; w < WARPS; ++w) top = max3_nan(top, top, sh.scan_f[0][w]), least_top = fminf(least_top, sh.scan_f[1][w]);
   asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
   s.tell(sh.top, top), s.tell(sh.least, least_top);
+  if (me == 0 && tid < SAMPLE_CTAS) {
+    SampleShared* to = cluster.map_shared_rank(&sh, tid);
+    to->temperature = T, to->top_p = top_p, to->min_p = min_p, to->u = u, to->top_k = top_k;
+  }
   cluster.sync();
+  T = sh.temperature, top_p = sh.top_p, min_p = sh.min_p, u = sh.u, top_k = sh.top_k;
   for (int r = 0; r < SAMPLE_CTAS; ++r) top = max3_nan(top, top, sh.top[r]), least_top = fminf(least_top, sh.least[r]);
   s.top = top;
   const bool none = !(top > -CUDART_INF_F);
@@ -590,7 +698,7 @@ __global__ void __cluster_dims__(SAMPLE_CTAS, 1, 1) __launch_bounds__(THREADS, 1
     }
     return;
   }
-  s.inv_t = 1.0 / (double)T;
+  s.steps = 46.166241308446828 / (double)T;  // 32 log2(e)
   // (an infinite largest value leaves those like it; rounded down, never up)
   const double reach = (double)top - SAMPLE_REACH * (double)T;
   s.floor_x = top == CUDART_INF_F ? top : reach > -3.0e38 ? __double2float_rd(reach) : -3.402823466e38f;
@@ -598,28 +706,30 @@ __global__ void __cluster_dims__(SAMPLE_CTAS, 1, 1) __launch_bounds__(THREADS, 1
 
   u64 border = ~0ull;
   bool both = false;
-  if (top_k > 0 && top_k < p.n_vocab) {
-    if (top_k <= SAMPLE_FEW && s.few_largest(top_k, my_top, least_top)) {
-      cluster.sync();  // (all have read how many)
-      if (me == 0) s.from_list(top_k, (double)top_p, least, part, p.ids + row, p.prob != nullptr ? p.prob + row : nullptr);
-      return;
-    }
-    if (top_k <= SAMPLE_FEW) cluster.sync();
-    border = s.find(border, top_k, (double)top_p, &both);
+  int* id_out = p.ids + row;
+  float* prob_out = p.prob != nullptr ? p.prob + row : nullptr;
+  const bool limited = top_k > 0 && top_k < p.n_vocab;
+  if (limited && top_k <= SAMPLE_FEW && s.few_largest(top_k, false, (double)top_p, least, part, my_top, least_top, id_out, prob_out)) return;
+  if (!limited && top_p < 1.f) {  // (mostly a short run)
+    s.sum_up(border);
+    if (s.few_largest(SAMPLE_FEW, true, (double)top_p, least, part, my_top, least_top, id_out, prob_out)) return;
   }
+  if (limited) border = s.find(border, top_k, (double)top_p, &both);
   if (top_p < 1.f && !both) {
     bool done;
     cluster.sync();
+    if (limited) {
+      s.sum_up(border);
+      cluster.sync();
+    }
     border = s.find(border, 0, (double)top_p, &done);
   }
 
   // ---- the kept weights in the order of the tokens: a warp's words side by side
-  const float border_x = value_of((uint32_t)(border >> 32));
-  const int border_i = (int)(uint32_t)border;
+  const typename Sampler<THREADS>::Upto in(border);
   const int own = (s.words + WARPS - 1) / WARPS, v0 = min(warp * own, s.words), v1 = min(v0 + own, s.words);
-  const bool cut = border != ~0ull;
   auto kept = [&](float y, int i) {
-    if (y < s.floor_x || (cut && (y < border_x || (y == border_x && i > border_i)))) return 0.0;
+    if (y < s.floor_x || !in.has(y, i)) return 0.0;
     const double w = s.weight(y);
     return w >= least ? w : 0.0;
   };
