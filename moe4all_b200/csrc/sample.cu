@@ -25,9 +25,10 @@ namespace cg = cooperative_groups;
 constexpr int SAMPLE_CTAS = 8;
 constexpr int SAMPLE_BINS = 2048;
 constexpr int SAMPLE_LIST = 2048;     // candidates that are sorted
-constexpr int SAMPLE_FEW = 192;       // so many largest ones are looked for among the threads' largest first,
+constexpr int SAMPLE_FEW = 192;       // a run of p of a row's weight is looked for among so many largest ones first
+constexpr int SAMPLE_MAXIMA = 1024;   // so many largest ones are looked for by the threads' largest,
 constexpr int SAMPLE_FEW_BINS = 256;  // by bins of these,
-constexpr int SAMPLE_SLOTS = 64;      // and so many candidates of a CTA looked at
+constexpr int SAMPLE_SLOTS = SAMPLE_LIST / SAMPLE_CTAS;  // and so many candidates of a CTA looked at
 constexpr int SAMPLE_CAP = 40960;     // values of a row in a CTA's shared memory at most
 constexpr double SAMPLE_REACH = 45.0; // weights down to e^-45 < 2^-64
 typedef unsigned long long u64;
@@ -47,16 +48,15 @@ __device__ __forceinline__ float value_of(uint32_t r) { return __uint_as_float(r
 __device__ __forceinline__ u64 place_of(float x, int i) { return (u64)rank_of(x) << 32 | (uint32_t)i; }
 
 struct __align__(16) SampleShared {
-  uint32_t hist[SAMPLE_BINS];
   union {
-    u64 list[SAMPLE_LIST];
-    struct {
-      u64 few[SAMPLE_CTAS * SAMPLE_SLOTS];      // the candidates by CTA, then by rank
-      double few_weight[SAMPLE_CTAS * SAMPLE_SLOTS];
-      uint32_t few_hist[SAMPLE_CTAS][SAMPLE_FEW_BINS];
-    };
+    uint32_t hist[SAMPLE_BINS];
+    double few_weight[512];  // a candidate's to a thread
   };
-  uint32_t sums[SAMPLE_BINS];  // of all CTAs' hist
+  u64 list[SAMPLE_LIST];
+  union {
+    uint32_t sums[SAMPLE_BINS];  // of all CTAs' hist
+    uint32_t few_hist[SAMPLE_CTAS][SAMPLE_FEW_BINS];
+  };
   double power[32];            // 2^(j / 32)
   double scan[2][16];
   int scan_n[16];
@@ -128,7 +128,10 @@ struct Sampler {
     return __hiloint2double(__double2hiint(e) + (k >> 5) * (1 << 20), __double2loint(e));
   }
   // exp((x - top) / T)
-  __device__ __forceinline__ double weight(float x) const { return x < floor_x ? 0.0 : x == top ? 1.0 : power32(((double)x - (double)top) * steps); }
+  __device__ __forceinline__ double weight(float x) const {  // (without branches: several at a time)
+    const double w = power32(((double)x - (double)top) * steps);
+    return x < floor_x ? 0.0 : x == top ? 1.0 : w;
+  }
   // Whether a value is one of those up to a border.
   struct Upto {
     float x;
@@ -142,7 +145,8 @@ struct Sampler {
     const Upto in(within);
     double sum = 0, all;
     mine([&](float x, int i) {
-      if (in.has(x, i)) sum += weight(x);
+      const double w = weight(x);
+      sum += in.has(x, i) ? w : 0.0;
     });
     before<double>(sum, sh.scan[0], all);
     tell(sh.sum, all);
@@ -300,18 +304,18 @@ struct Sampler {
   }
 
   // The weights of the list's first `count` candidates, the thread's own in w, and the sum ahead of them.
-  __device__ double list_weights(int count, bool by_index, double (&w)[PER], double& all) {
+  __device__ double list_weights(int count, double (&w)[PER], double& all) {
     double sum = 0;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
       const int e = PER * tid + j;
-      w[j] = e < count ? weight(value_of(by_index ? (uint32_t)sh.list[e] : (uint32_t)(sh.list[e] >> 32))) : 0.0;
+      w[j] = e < count ? weight(value_of((uint32_t)(sh.list[e] >> 32))) : 0.0;
       sum += w[j];
     }
     return before<double>(sum, sh.scan[0], all);
   }
-  // The first of them with which the sum from `at` on reaches the target, or passes it; the last one with a weight if none does.
-  __device__ int list_find(int count, const double (&w)[PER], double at, double target, bool passes) {
+  // The first of them with which the sum from `at` on reaches the target; the last one with a weight if none does.
+  __device__ int list_find(int count, const double (&w)[PER], double at, double target) {
     if (tid == 0) sh.pick = SAMPLE_LIST, sh.b1 = -1;
     __syncthreads();
     int found = SAMPLE_LIST, last = -1;
@@ -320,7 +324,7 @@ struct Sampler {
       at += w[j];
       if (PER * tid + j >= count || w[j] <= 0) continue;
       last = PER * tid + j;
-      if (found == SAMPLE_LIST && (passes ? at > target : at >= target)) found = last;
+      if (found == SAMPLE_LIST && at >= target) found = last;
     }
     if (found < SAMPLE_LIST) atomicMin(&sh.pick, found);
     if (last >= 0) atomicMax(&sh.b1, last);
@@ -342,11 +346,24 @@ struct Sampler {
     return (int)(__float_as_uint(b) & (SAMPLE_BINS - 1));
   }
 
+  // The border of the first CTA's n candidates, to all: that of the k largest and (p < 1) of the run with p of their weight.
+  __device__ void cut_list(int n, int k, double p) {
+    sort_list(n);
+    int last = max(0, min(n, k) - 1);
+    if (p < 1.0) {
+      double w[PER], all;
+      const double at = list_weights(last + 1, w, all);
+      last = max(0, list_find(last + 1, w, at, p * all));
+    }
+    if (tid < SAMPLE_CTAS) *cluster.map_shared_rank(&sh.border, tid) = sh.list[last];
+  }
+
   // The token where no more than the k largest are needed: they are among the values that share a bin with the k-th largest of the threads' largest, or are
-  // larger, and only the threads that have such a one look through their values again.  The first CTA sorts these by counting (a thread to each) and takes the
-  // token by itself.  all_weight > 0: the weight of the whole row, of which the run has p (and which may need more than these); else of the k largest.
-  // False: too many candidates, or too few.
-  __device__ bool few_largest(int k, bool of_all, double p, double least, double u, float my_top, float least_top, int* id, float* prob) {
+  // larger, and only the threads that have such a one look through their values again.  If these are few, the first CTA sorts them by counting (a thread to each)
+  // and takes the token by itself; of more it finds the border.  of_all: the run has p of the whole row's weight (and may need more than these), else of the k
+  // largest's.  NOTHING: too many candidates, or too few.
+  enum Found { NOTHING, TOKEN, BORDER };
+  __device__ Found few_largest(int k, bool of_all, double p, double least, double u, float my_top, float least_top, int* id, float* prob) {
     const double width = top > least_top ? (SAMPLE_FEW_BINS - 1) / (0.5 * ((double)top - (double)least_top)) : 0.0;
     const float scale = (float)width, half = 0.5f * top;
     auto few_bin = [&](float x) { return min((int)(fmaf(-0.5f, x, half) * scale), SAMPLE_FEW_BINS - 1); };
@@ -379,7 +396,7 @@ struct Sampler {
         for (int j = 0; j < 4; ++j)
           if (x[j] > -CUDART_INF_F && few_bin(x[j]) <= b2) {
             const int to = atomicAdd(&sh.n_list, 1);
-            if (to < SAMPLE_SLOTS) *cluster.map_shared_rank(&sh.few[me * SAMPLE_SLOTS + to], 0) = place_of(x[j], base + 4 * w + j);
+            if (to < SAMPLE_SLOTS) *cluster.map_shared_rank(&sh.list[me * SAMPLE_SLOTS + to], 0) = place_of(x[j], base + 4 * w + j);
           }
       }
     }
@@ -388,31 +405,54 @@ struct Sampler {
     cluster.sync();
     int n = 0;
     for (int r = 0; r < SAMPLE_CTAS; ++r) {
-      if (sh.n_few[r] > SAMPLE_SLOTS) return false;
+      if (sh.n_few[r] > SAMPLE_SLOTS) return NOTHING;
       n += sh.n_few[r];
     }
-    if (n > THREADS) return false;
+    if (n > THREADS) {
+      if (of_all) return NOTHING;
+      if (me == 0) {
+        u64 at[PER];
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+          int e = tid + j * THREADS;
+          at[j] = ~0ull;
+#pragma unroll 1
+          for (int r = 0; r < SAMPLE_CTAS; ++r) {
+            if (e >= 0 && e < sh.n_few[r]) at[j] = sh.list[r * SAMPLE_SLOTS + e];
+            e -= sh.n_few[r];
+          }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+          if (tid + j * THREADS < n) sh.list[tid + j * THREADS] = at[j];
+        __syncthreads();
+        cut_list(n, k, p);
+      }
+      cluster.sync();
+      return BORDER;
+    }
     bool done = true;
     if (me == 0) {
       // thread e has candidate e
       u64 at = ~0ull;
       int e = tid;
       for (int r = 0; r < SAMPLE_CTAS; ++r) {
-        if (e >= 0 && e < sh.n_few[r]) at = sh.few[r * SAMPLE_SLOTS + e];
+        if (e >= 0 && e < sh.n_few[r]) at = sh.list[r * SAMPLE_SLOTS + e];
         e -= sh.n_few[r];
       }
       double w = tid < n ? weight(value_of((uint32_t)(at >> 32))) : 0.0;
       __syncthreads();
-      if (tid < n) sh.few[tid] = at;
+      if (tid < n) sh.list[tid] = at;
       __syncthreads();
       int rank = 0;
 #pragma unroll 4
-      for (int i = 0; i < n; ++i) rank += sh.few[i] < at;
+      for (int i = 0; i < n; ++i) rank += sh.list[i] < at;
       __syncthreads();
-      if (tid < n) sh.few[rank] = at, sh.few_weight[rank] = w;
+      if (tid < n) sh.list[rank] = at, sh.few_weight[rank] = w;
       __syncthreads();
       // thread r has rank r
-      at = tid < n ? sh.few[tid] : ~0ull;
+      at = tid < n ? sh.list[tid] : ~0ull;
       w = tid < n && (of_all || tid < k) ? sh.few_weight[tid] : 0.0;
       int count = of_all ? n : min(n, k);
       if (p < 1.0) {
@@ -433,7 +473,7 @@ struct Sampler {
       for (int i = 0; i < count; ++i) {
         const double x = sh.few_weight[i];
         kept += x;
-        if ((int)(uint32_t)sh.few[i] < index) lower += x;
+        if ((int)(uint32_t)sh.list[i] < index) lower += x;
       }
       if (tid < count && w > 0 && lower <= u * kept) atomicMax(&sh.pick, index);
       __syncthreads();
@@ -442,10 +482,10 @@ struct Sampler {
         if (prob != nullptr) *prob = (float)(w / kept);
       }
     }
-    if (!of_all) return true;  // (nothing of another CTA is waited for)
+    if (!of_all) return TOKEN;  // (nothing of another CTA is waited for)
     if (me == 0) tell_one(&sh.done, done ? 1 : 0);
     cluster.sync();
-    return sh.done != 0;
+    return sh.done != 0 ? TOKEN : NOTHING;
   }
 
   // The border among the values up to `within`: that of the k largest, or with p < 1 that of the run with p of the weight, or (k, then p) both where the
@@ -462,7 +502,7 @@ struct Sampler {
       if (x >= low && in.has(x, i)) atomicAdd(&sh.hist[bin(x)], 1u);
     });
     cluster.sync();
-    double target = by_weight ? p * total(sh.sum) : 0;
+    const double target = by_weight ? p * total(sh.sum) : 0;
     const double width = bin_scale > 0.f ? 2.0 * steps / bin_scale : 0.0;
     // (f32 moves a bin's edges by 2^-22 of their distance from the largest, which is 45 in the exponent at most)
     bracket(by_weight, k, target, 3e-5, [&](int b) { return power32((0.5 - b) * width); });
@@ -592,18 +632,16 @@ struct Sampler {
     }
     cluster.sync();
     if (me == 0) {
-      int count = min(sh.n_list, SAMPLE_LIST);
-      sort_list(count);
-      if (!by_weight) count = min(count, whole ? k : k - ahead);
-      int last = max(0, count - 1);
-      if (by_weight || (whole && p < 1.0)) {
+      const int count = min(sh.n_list, SAMPLE_LIST);
+      if (!by_weight) {
+        cut_list(count, whole ? k : k - ahead, whole ? p : 1.0);
+      } else {
+        sort_list(count);
         double w[PER], all;
-        double at = list_weights(count, false, w, all);
-        if (by_weight) at += total(sh.above);
-        else target = p * all;
-        last = max(0, list_find(count, w, at, target, false));
+        const double at = list_weights(count, w, all);
+        const int last = max(0, list_find(count, w, at + total(sh.above), target));
+        if (tid < SAMPLE_CTAS) *cluster.map_shared_rank(&sh.border, tid) = sh.list[last];
       }
-      if (tid < SAMPLE_CTAS) *cluster.map_shared_rank(&sh.border, tid) = sh.list[last];
     }
     *both = whole;
     cluster.sync();
@@ -648,13 +686,13 @@ __global__ void __cluster_dims__(SAMPLE_CTAS, 1, 1) __launch_bounds__(THREADS, 1
   // ---- the row, once: its largest value (NaN where one is), and every thread's largest
   float top = -CUDART_INF_F;
 #pragma unroll 1
-  for (int v0 = tid; v0 < s.words; v0 += 4 * THREADS) {
-    float4 v[4];
+  for (int v0 = tid; v0 < s.words; v0 += 6 * THREADS) {
+    float4 v[6];
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
+    for (int k = 0; k < 6; ++k)
       if (v0 + k * THREADS < s.words) v[k] = s.from_row(v0 + k * THREADS);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < 6; ++k) {
       if (v0 + k * THREADS >= s.words) break;
       if (p.cached) *reinterpret_cast<float4*>(s_x + 4 * (v0 + k * THREADS)) = v[k];
       top = max3_nan(max3_nan(top, v[k].x, v[k].y), v[k].z, v[k].w);
@@ -709,12 +747,16 @@ __global__ void __cluster_dims__(SAMPLE_CTAS, 1, 1) __launch_bounds__(THREADS, 1
   int* id_out = p.ids + row;
   float* prob_out = p.prob != nullptr ? p.prob + row : nullptr;
   const bool limited = top_k > 0 && top_k < p.n_vocab;
-  if (limited && top_k <= SAMPLE_FEW && s.few_largest(top_k, false, (double)top_p, least, part, my_top, least_top, id_out, prob_out)) return;
+  if (limited && top_k <= SAMPLE_MAXIMA) {
+    const auto found = s.few_largest(top_k, false, (double)top_p, least, part, my_top, least_top, id_out, prob_out);
+    if (found == s.TOKEN) return;
+    if (found == s.BORDER) border = sh.border, both = true;
+  }
   if (!limited && top_p < 1.f) {  // (mostly a short run)
     s.sum_up(border);
-    if (s.few_largest(SAMPLE_FEW, true, (double)top_p, least, part, my_top, least_top, id_out, prob_out)) return;
+    if (s.few_largest(SAMPLE_FEW, true, (double)top_p, least, part, my_top, least_top, id_out, prob_out) == s.TOKEN) return;
   }
-  if (limited) border = s.find(border, top_k, (double)top_p, &both);
+  if (limited && !both) border = s.find(border, top_k, (double)top_p, &both);
   if (top_p < 1.f && !both) {
     bool done;
     cluster.sync();
