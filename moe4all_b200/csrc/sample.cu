@@ -123,8 +123,8 @@ struct Sampler {
   __device__ __forceinline__ double power32(double t) const {
     const double m = t + 6755399441055744.0;  // 1.5 2^52: the sum's low word is t rounded
     const int k = __double2loint(m);
-    const double r = (t - (m - 6755399441055744.0)) * (0.69314718055994531 / 32);
-    const double e = fma(r, fma(r, fma(r, fma(r, fma(r, 1.0 / 120, 1.0 / 24), 1.0 / 6), 0.5), 1.0), 1.0) * sh.power[k & 31];
+    constexpr double c = 0.69314718055994531 / 32;
+    const double f = t - (m - 6755399441055744.0), e = fma(f, fma(f, fma(f, fma(f, fma(f, c * c * c * c * c / 120, c * c * c * c / 24), c * c * c / 6), c * c / 2), c), 1.0) * sh.power[k & 31];
     return __hiloint2double(__double2hiint(e) + (k >> 5) * (1 << 20), __double2loint(e));
   }
   // exp((x - top) / T)
@@ -136,9 +136,12 @@ struct Sampler {
   struct Upto {
     float x;
     int i;
-    bool all;
-    __device__ explicit Upto(u64 border) : x(value_of((uint32_t)(border >> 32))), i((int)(uint32_t)border), all(border == ~0ull) {}
-    __device__ __forceinline__ bool has(float y, int j) const { return all || y > x || (y == x && j <= i); }
+    __device__ explicit Upto(u64 border) {
+      const bool all = border == ~0ull;
+      x = all ? -CUDART_INF_F : value_of((uint32_t)(border >> 32));
+      i = all ? 0x7FFFFFFF : (int)(uint32_t)border;
+    }
+    __device__ __forceinline__ bool has(float y, int j) const { return y > x || (y == x && j <= i); }
   };
   // The weight of all values into every CTA's sum; there behind the next cluster barrier.
   __device__ void sum_up(u64 within) {
@@ -770,13 +773,18 @@ __global__ void __cluster_dims__(SAMPLE_CTAS, 1, 1) __launch_bounds__(THREADS, 1
   // ---- the kept weights in the order of the tokens: a warp's words side by side
   const typename Sampler<THREADS>::Upto in(border);
   const int own = (s.words + WARPS - 1) / WARPS, v0 = min(warp * own, s.words), v1 = min(v0 + own, s.words);
+  const float cutoff = fmaxf(in.x, s.floor_x);
   auto kept = [&](float y, int i) {
-    if (y < s.floor_x || !in.has(y, i)) return 0.0;
+    if (y < cutoff) return 0.0;
     const double w = s.weight(y);
-    return w >= least ? w : 0.0;
+    return w >= least && in.has(y, i) ? w : 0.0;
   };
   double sum = 0;
-  s.each(v0 + lane, v1, 32, [&](float y, int i) { sum += kept(y, i); });
+  if (border == ~0ull && least == 0.0) {
+    s.each(v0 + lane, v1, 32, [&](float y, int) { sum += s.weight(y); });
+  } else {
+    s.each(v0 + lane, v1, 32, [&](float y, int i) { sum += kept(y, i); });
+  }
   sum = s.warp_total(sum);
   __syncthreads();
   if (lane == 0) sh.scan[0][warp] = sum;
