@@ -285,24 +285,54 @@ struct Sampler {
     __syncthreads();
   }
 
-  // The first CTA sorts the candidates: list[0 .. n - 1], padded to a power of two.
+  // The first CTA sorts the candidates, list[0 .. n - 1]: by counting into bins of one width, and within a bin (a few, unless values are equal) by counting
+  // again.  (With a network of exchanges 1100 of them took 30 us.)
   __device__ void sort_list(int n) {
-    int size = 32;
-    while (size < n) size <<= 1;
-    for (int i = n + tid; i < size; i += THREADS) sh.list[i] = ~0ull;
+    u64 at[PER];
+    float low = CUDART_INF_F;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const int e = tid + j * THREADS;
+      at[j] = e < n ? sh.list[e] : ~0ull;
+      if (e < n) low = fminf(low, value_of((uint32_t)(at[j] >> 32)));
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) low = fminf(low, __shfl_xor_sync(0xFFFFFFFFu, low, o));
+    for (int b = tid; b < SAMPLE_BINS; b += THREADS) sh.hist[b] = 0;
+    if ((tid & 31) == 0) sh.scan_f[0][tid >> 5] = low;
     __syncthreads();
-    const bool alone = size <= 64;  // a warp's pairs
-    if (alone && tid >= 32) size = 0;
-    for (int k = 2; k <= size; k <<= 1)
-      for (int j = k >> 1; j > 0; j >>= 1) {
-        for (int t = tid; t < size / 2; t += THREADS) {
-          const int a = 2 * t - (t & (j - 1)), b = a + j;
-          const u64 x = sh.list[a], y = sh.list[b];
-          if ((x > y) == ((a & k) == 0)) sh.list[a] = y, sh.list[b] = x;
-        }
-        if (alone) __syncwarp();
-        else __syncthreads();
+    for (int w = 0; w < WARPS; ++w) low = fminf(low, sh.scan_f[0][w]);
+    const float scale = top > low ? (float)((SAMPLE_BINS - 1) / (0.5 * ((double)top - (double)low))) : 0.f, half = 0.5f * top;
+    int bin[PER], order[PER];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      bin[j] = min((int)(fmaf(-0.5f, value_of((uint32_t)(at[j] >> 32)), half) * scale), SAMPLE_BINS - 1);
+      if (tid + j * THREADS < n) order[j] = atomicAdd(&sh.hist[bin[j]], 1u);
+    }
+    __syncthreads();
+    int sum = 0, all;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) sum += (int)sh.hist[PER * tid + j];
+    int ahead = before<int>(sum, sh.scan_n, all);
+#pragma unroll
+    for (int j = 0; j < PER; ++j) sh.sums[PER * tid + j] = ahead, ahead += (int)sh.hist[PER * tid + j];
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < PER; ++j)
+      if (tid + j * THREADS < n) sh.list[sh.sums[bin[j]] + order[j]] = at[j];
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < PER; ++j)
+      if (tid + j * THREADS < n) {
+        const int first = sh.sums[bin[j]], count = sh.hist[bin[j]];
+        order[j] = first;
+#pragma unroll 1
+        for (int i = first; i < first + count; ++i) order[j] += sh.list[i] < at[j];
       }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < PER; ++j)
+      if (tid + j * THREADS < n) sh.list[order[j]] = at[j];
     __syncthreads();
   }
 
@@ -514,6 +544,8 @@ struct Sampler {
     bool whole = !by_weight && upto <= SAMPLE_LIST;  // the list takes what lies ahead too
     uint32_t r1 = 0, r2 = 0;                          // the candidates as a range of ranks, once the bins are not enough
     bool by_rank = false;
+    double above = 0;          // by weight: of the values ahead of rank `from`, in all CTAs
+    uint32_t from = 0;
     for (int level = 0;; ++level) {
       const int n_list = whole ? upto : upto - ahead;
       if (n_list <= SAMPLE_LIST) break;
@@ -552,7 +584,8 @@ struct Sampler {
         tell(sh.above, all);
       }
       cluster.sync();
-      const double above = by_weight ? total(sh.above) : 0.0;
+      if (by_weight) above = total(sh.above);
+      from = r1;
       const int was = ahead;
       bracket(by_weight, k - was, target - above, 0.0, [&](int b) {
         const u64 r = r1 + ((u64)b << shift);
@@ -623,7 +656,7 @@ struct Sampler {
       if (whole || (by_rank ? r >= r1 : b >= b1)) {
         const int to = atomicAdd(cluster.map_shared_rank(&sh.n_list, 0), 1);
         if (to < SAMPLE_LIST) *cluster.map_shared_rank(&sh.list[to], 0) = place_of(x, i);  // (always)
-      } else if (by_weight) {
+      } else if (by_weight && r >= from) {
         over += weight(x);
       }
     });
@@ -642,7 +675,7 @@ struct Sampler {
         sort_list(count);
         double w[PER], all;
         const double at = list_weights(count, w, all);
-        const int last = max(0, list_find(count, w, at + total(sh.above), target));
+        const int last = max(0, list_find(count, w, at + (above + total(sh.above)), target));
         if (tid < SAMPLE_CTAS) *cluster.map_shared_rank(&sh.border, tid) = sh.list[last];
       }
     }
