@@ -496,23 +496,25 @@ struct Sampler {
         done = over < count || !of_all;
         count = min(count, over + 1);
       }
-      if (tid < count && (w <= 0 || w < least)) w = 0.0;
-      if (tid < count) sh.few_weight[tid] = w;
-      if (tid == 0) sh.pick = -1;
-      __syncthreads();
-      const int index = (int)(uint32_t)at;
-      double lower = 0, kept = 0;
+      if (done) {  // (else the candidates are not enough)
+        if (tid < count && (w <= 0 || w < least)) w = 0.0;
+        if (tid < count) sh.few_weight[tid] = w;
+        if (tid == 0) sh.pick = -1;
+        __syncthreads();
+        const int index = (int)(uint32_t)at;
+        double lower = 0, kept = 0;
 #pragma unroll 4
-      for (int i = 0; i < count; ++i) {
-        const double x = sh.few_weight[i];
-        kept += x;
-        if ((int)(uint32_t)sh.list[i] < index) lower += x;
-      }
-      if (tid < count && w > 0 && lower <= u * kept) atomicMax(&sh.pick, index);
-      __syncthreads();
-      if (done && tid < count && w > 0 && index == sh.pick) {
-        *id = index;
-        if (prob != nullptr) *prob = (float)(w / kept);
+        for (int i = 0; i < count; ++i) {
+          const double x = sh.few_weight[i];
+          kept += x;
+          if ((int)(uint32_t)sh.list[i] < index) lower += x;
+        }
+        if (tid < count && w > 0 && lower <= u * kept) atomicMax(&sh.pick, index);
+        __syncthreads();
+        if (done && tid < count && w > 0 && index == sh.pick) {
+          *id = index;
+          if (prob != nullptr) *prob = (float)(w / kept);
+        }
       }
     }
     if (!of_all) return TOKEN;  // (nothing of another CTA is waited for)
@@ -523,7 +525,7 @@ struct Sampler {
 
   // The border among the values up to `within`: that of the k largest, or with p < 1 that of the run with p of the weight, or (k, then p) both where the
   // candidates hold all of the k; *both: whether they did.
-  __device__ __noinline__ u64 find(u64 within, int k, double p, bool* both) {
+  __device__ u64 find(u64 within, int k, double p, bool* both) {
     const bool by_weight = k <= 0;
     const Upto in(within);
     *both = false;
