@@ -22,7 +22,7 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int SAMPLE_CTAS = 8;
+constexpr int SAMPLE_CTAS = 8, SAMPLE_THREADS = 512;
 constexpr int SAMPLE_BINS = 2048;
 constexpr int SAMPLE_LIST = 2048;     // candidates that are sorted
 constexpr int SAMPLE_FEW = 192;       // a run of p of a row's weight is looked for among so many largest ones first
@@ -50,7 +50,7 @@ __device__ __forceinline__ u64 place_of(float x, int i) { return (u64)rank_of(x)
 struct __align__(16) SampleShared {
   union {
     uint32_t hist[SAMPLE_BINS];
-    double few_weight[512];  // a candidate's to a thread
+    double few_weight[SAMPLE_THREADS];  // a candidate's to a thread
   };
   u64 list[SAMPLE_LIST];
   union {
@@ -77,9 +77,8 @@ struct __align__(16) SampleShared {
   int pick;
 };
 
-template <int THREADS>
 struct Sampler {
-  static constexpr int WARPS = THREADS / 32, PER = SAMPLE_BINS / THREADS;  // bins (and candidates) of a thread
+  static constexpr int THREADS = SAMPLE_THREADS, WARPS = THREADS / 32, PER = SAMPLE_BINS / THREADS;  // bins (and candidates) of a thread
   SampleShared& sh;
   cg::cluster_group cluster;
   // This CTA's values, four to a word that lies on a 16-byte boundary: in shared memory, or (xs null) where they came from.  The row begins within its first
@@ -696,18 +695,17 @@ struct SampleParams {
   int n_vocab, cached;
 };
 
-template <int THREADS>
-__global__ void __cluster_dims__(SAMPLE_CTAS, 1, 1) __launch_bounds__(THREADS, 1024 / THREADS) k_sample(const __grid_constant__ SampleParams p) {
+__global__ void __cluster_dims__(SAMPLE_CTAS, 1, 1) __launch_bounds__(SAMPLE_THREADS, 2) k_sample(const __grid_constant__ SampleParams p) {
   extern __shared__ __align__(16) float s_x[];
   __shared__ SampleShared sh;
-  constexpr int WARPS = THREADS / 32;
+  constexpr int THREADS = SAMPLE_THREADS, WARPS = THREADS / 32;
   cg::cluster_group cluster = cg::this_cluster();
   asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // waited for ahead of the first word to another CTA: all are there then
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, me = (int)cluster.block_rank(), row = blockIdx.x / SAMPLE_CTAS;
   const float* x = p.logits + (size_t)row * p.stride;
   const int lead = (int)((reinterpret_cast<uintptr_t>(x) >> 2) & 3);  // values of the row's first word that are not the row's
   const int all_words = (p.n_vocab + lead + 3) / 4, per = (all_words + SAMPLE_CTAS - 1) / SAMPLE_CTAS, w0 = min(me * per, all_words);
-  Sampler<THREADS> s = {sh, cluster, p.cached ? s_x : nullptr, x, min(per, all_words - w0), 4 * w0 - lead, p.n_vocab, me, tid, 0.f, 0.0, 0.f, 0.f, 0.f};
+  Sampler s = {sh, cluster, p.cached ? s_x : nullptr, x, min(per, all_words - w0), 4 * w0 - lead, p.n_vocab, me, tid, 0.f, 0.0, 0.f, 0.f, 0.f};
   if (tid < 32) sh.power[tid] = exp2(tid * 0.03125);
   pdl_trigger();
   pdl_wait();
@@ -806,7 +804,7 @@ __global__ void __cluster_dims__(SAMPLE_CTAS, 1, 1) __launch_bounds__(THREADS, 1
   }
 
   // ---- the kept weights in the order of the tokens: a warp's words side by side
-  const typename Sampler<THREADS>::Upto in(border);
+  const Sampler::Upto in(border);
   const int own = (s.words + WARPS - 1) / WARPS, v0 = min(warp * own, s.words), v1 = min(v0 + own, s.words);
   const float cutoff = fmaxf(in.x, s.floor_x);
   auto kept = [&](float y, int i) {
@@ -893,11 +891,12 @@ int32_t launch_sample(infr_cuda_ctx* ctx, const float* logits, const float* u, c
                       float* prob, size_t stride, int rows, int n_vocab) {
   SampleParams p = {logits, u, temperature, top_p, min_p, top_k, ids, prob, stride, n_vocab, 0};
   const int per = ((n_vocab + 3 + 3) / 4 + SAMPLE_CTAS - 1) / SAMPLE_CTAS * 4;
-  p.cached = rows <= 16 && per <= SAMPLE_CAP;
+  // A row that fits is kept in shared memory: 64 rows of 150000 with settings of all kinds 98 us, read again from L2 108, with 256 threads to a CTA (all rows at
+  // once then, but each of them slower) 141; rows that all take one of the 20 largest 25, 26 and 17.
+  p.cached = per <= SAMPLE_CAP;
   const size_t smem = p.cached ? (size_t)per * 4 : 0;
-  const auto kernel = p.cached ? k_sample<512> : k_sample<256>;
-  cudaError_t e = ensure_smem(reinterpret_cast<const void*>(kernel), p.cached ? (size_t)SAMPLE_CAP * 4 : 0);
-  if (e == cudaSuccess) e = launch_ex(kernel, dim3((unsigned)rows * SAMPLE_CTAS), dim3(p.cached ? 512 : 256), smem, ctx->stream, true, p);
+  cudaError_t e = ensure_smem(reinterpret_cast<const void*>(&k_sample), (size_t)SAMPLE_CAP * 4);
+  if (e == cudaSuccess) e = launch_ex(k_sample, dim3((unsigned)rows * SAMPLE_CTAS), dim3(SAMPLE_THREADS), smem, ctx->stream, true, p);
   if (e != cudaSuccess) return check_cuda(ctx, e, "k_sample launch");
   ctx->launches += 1;
   return check_cuda(ctx, cudaGetLastError(), "k_sample launch");
