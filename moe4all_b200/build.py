@@ -13,7 +13,7 @@ LIB = os.path.join(OUT_DIR, "libinfr_cuda.so")
 
 SOURCES = ["api.cu", "router_topk.cu", "decode_ffn.cu", "dense_ops.cu", "grouped_ffn.cu", "grouped_tmem.cu", "umma_selftest.cu",
            "gguf_ingest.cu", "ep.cu", "expert_major.cu", "anyfmt_ffn.cu",
-           "attn_rows.cu", "attn_tiles.cu", "rope_kv.cu", "kv_read.cu", "sample.cu"]
+           "attn_rows.cu", "attn_rows_q8.cu", "attn_tiles.cu", "rope_kv.cu", "kv_read.cu", "sample.cu"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

@@ -14,86 +14,33 @@
 // an item's parts; and, with heads of 256, a warp's own chain from tile to tile.  Nine to sixteen rows of heads of 192 and 256 do not fit the registers: 107 and 194
 // words a thread are spilled.
 #include "attn.cuh"
-#include "kv_q8.cuh"
 
 namespace infr {
 namespace {
 
-__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
-__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
-// Two 16 x 16 matrices of bytes transposed: r[0], r[1] are rows lane / 4 and 8 more of the first, columns 4 (lane % 4) .. + 3.
-__device__ __forceinline__ void ldsm2_t8(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m16n16.x2.trans.shared.b8 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-}
-__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ uint32_t movm(uint32_t a) {
-  uint32_t d;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
-  return d;
-}
 constexpr int ROWS_EXTRA = 3;  // tiles' time that an item's beginning and end take (64 streams: 1 93.7, 3 86.1, 6 87.0 us)
 
-template <int HD, int NT, bool Q8>
+template <int HD, int NT>
 struct RowsShape {
   static constexpr int WARPS = 8, THREADS = WARPS * 32, RB = 8 * NT;
   static constexpr int LOG2_TILE = 7;              // 16 keys a warp
-  static constexpr int SIDE = 16 * HD * (Q8 ? 1 : 2);  // bytes of 16 keys of K, or of V
-  static constexpr int SCALES = Q8 ? 2 * HD : 0;       // bytes of a unit's scales, which lie apart
+  static constexpr int SIDE = 16 * HD * 2;         // bytes of 16 keys of K, or of V
   // A unit of the ring is both where eight warps' rings hold two of them or more, else (heads wider than 128) one of the two: K's place is
   // asked for again while V is used.  (Apart, heads of 128 lose: 93 -> 106 us for 64 streams.)
-  static constexpr bool PAIRED = Q8 || HD <= 128;
+  static constexpr bool PAIRED = HD <= 128;
   static constexpr int UNIT = PAIRED ? 2 * SIDE : SIDE;
   static constexpr int PITCH = HD + 4;             // words: the fragments' columns fall on different banks
-  static constexpr int SLOTS = HD <= 128 ? WARPS : WARPS / 2;  // wide heads: half of the warps add theirs to the others' first
+  static constexpr int SLOTS = PAIRED ? WARPS : WARPS / 2;  // wide heads: half of the warps add theirs to the others' first
   static constexpr int MERGE = SLOTS * RB * PITCH * 4, STATS = 2 * WARPS * RB * 4;
-  static constexpr int FIT = (232448 - 1024 - 1024 - MERGE - STATS) / (WARPS * (UNIT + SCALES));
-  static constexpr int MOST = Q8 ? 8 : 6, UNITS = FIT > MOST ? MOST : FIT;
-  static constexpr int SMEM = 1024 + WARPS * UNITS * (UNIT + SCALES) + MERGE + STATS + WARPS * UNITS * 8;
-  static_assert(WARPS * UNITS * UNIT >= 16 * ATTN_MAX_SEQ + 4, "what is known of the sequences fits where the keys go later");
+  static constexpr int FIT = (232448 - 1024 - 1024 - MERGE - STATS) / (WARPS * UNIT);
+  static constexpr int UNITS = FIT > 6 ? 6 : FIT;
+  static constexpr int SMEM = 1024 + WARPS * UNITS * UNIT + MERGE + STATS + WARPS * UNITS * 8;
 };
 
-// Pages of 8 bits: columns of rows of the item, the part of it that lies here, where 16 values of V that a row sees are not numbers, become NaN.  All of
-// the warp's lanes take part, a row to each of the first ones; `active`: not NaN already.  Blocks of 16 from block0 on, every `step`-th.
-static __device__ __noinline__ void attn_odd_blocks(const AttnParams& p, int s, int head, int key0, int key1, bool active, int to, int block0, int step, float* dst) {
-  const int lane = threadIdx.x & 31, from = attn_first_key(to, p.window);
-  const int lo = max(key0, __reduce_min_sync(0xFFFFFFFFu, active ? from : 0x7FFFFFFF)), hi = min(key1 - 1, __reduce_max_sync(0xFFFFFFFFu, active ? to : -1));
-#pragma unroll 1
-  for (int b = block0; b < p.hd / 16; b += step) {
-    bool sees = false;
-#pragma unroll 1
-    for (int k0 = lo & ~31; k0 <= hi; k0 += 32) {
-      const int key = k0 + lane;
-      bool odd = false;
-      if (key >= lo && key <= hi) {
-        const int page = attn_page_of(p, key);
-        odd = __ldcg(p.vs + ((size_t)attn_page(p, s, page) * p.page_pitch + (size_t)head * p.head_pitch + (size_t)(key - page * p.page_size) * p.row_pitch) / 16 + b) >= Q8_ODD;
-      }
-#pragma unroll 1
-      for (uint32_t found = __ballot_sync(0xFFFFFFFFu, odd); found; found &= found - 1) {
-        const int key = k0 + __ffs(found) - 1;
-        sees |= active && key >= from && key <= to;
-      }
-    }
-    if (sees)
-      for (int i = 0; i < 16; i += 4) __stcg(reinterpret_cast<float4*>(dst + 16 * b + i), make_float4(CUDART_NAN_F, CUDART_NAN_F, CUDART_NAN_F, CUDART_NAN_F));
-  }
-}
-
-// Q8: pages of 8 bits.  The tensor cores' inner dimensions may go in any order that both operands have, so a lane takes for K 16 neighbouring values of a key
-// at once (one scale, one 16-byte word: four steps of the product), and the 16 keys stand in the order in which a transposing load of bytes gives V's:
-// row i of the scores is key 4 (i / 2) + i % 2 of the slice, row 8 + i two behind it.
-template <int HD, int NT, bool Q8>
-__global__ void __launch_bounds__(RowsShape<HD, NT, Q8>::THREADS, 1)
+template <int HD, int NT>
+__global__ void __launch_bounds__(RowsShape<HD, NT>::THREADS, 1)
     k_attn_rows(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ AttnParams p) {
-  using Sh = RowsShape<HD, NT, Q8>;
+  using Sh = RowsShape<HD, NT>;
   constexpr int WARPS = Sh::WARPS, THREADS = Sh::THREADS, RB = Sh::RB, UNITS = Sh::UNITS, UNIT = Sh::UNIT, SIDE = Sh::SIDE, PITCH = Sh::PITCH, SLOTS = Sh::SLOTS;
   constexpr int SLABS = HD / 64, KST = HD / 16;
   constexpr int AHEAD = 4;  // sums under way (one or two at a time 60.5 us for 16 streams of heads of 256, so 58.8)
@@ -104,8 +51,7 @@ __global__ void __launch_bounds__(RowsShape<HD, NT, Q8>::THREADS, 1)
   __shared__ int s_last;
   __shared__ float s_weight[RB], s_factor[RB];
   unsigned char* ring_all = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  unsigned char* scales = ring_all + WARPS * UNITS * UNIT + (threadIdx.x >> 5) * UNITS * Sh::SCALES;
-  float* s_o = reinterpret_cast<float*>(ring_all + WARPS * UNITS * (UNIT + Sh::SCALES));
+  float* s_o = reinterpret_cast<float*>(ring_all + WARPS * UNITS * UNIT);
   uint4* s_q = reinterpret_cast<uint4*>(s_o);  // [NT][KST][32]
   float* s_m = s_o + SLOTS * RB * PITCH;
   float* s_l = s_m + WARPS * RB;
@@ -161,18 +107,13 @@ __global__ void __launch_bounds__(RowsShape<HD, NT, Q8>::THREADS, 1)
     if (lane == 0) {
       const int at = asked % UNITS;
       unsigned char* dst = ring + at * UNIT;
-      mbar_arrive_expect_tx(full + at, Q8 ? UNIT + 2 * p.hd : UNIT);
+      mbar_arrive_expect_tx(full + at, UNIT);
       const int y = a_y, w = packed ? 0 : attn_page_checked(p, a_page);
-      if constexpr (Q8) {
-        const size_t first = ((size_t)w * p.page_pitch + (size_t)ahead.head * p.head_pitch + (size_t)y * p.row_pitch) / 16;
-        bulk_g2s(scales + at * Sh::SCALES, p.ks + first, p.hd, full + at);  // (16 keys' hd / 16 bytes)
-        bulk_g2s(scales + at * Sh::SCALES + HD, p.vs + first, p.hd, full + at);
-      }
       const CUtensorMap* map = Sh::PAIRED || !(asked & 1) ? &kmap : &vmap;
 #pragma unroll
       for (int s = 0; s < SLABS; ++s) {
-        tma_load_4d(dst + s * (SIDE / SLABS), map, 64 * s, y, ahead.head, w, full + at);
-        if (Sh::PAIRED) tma_load_4d(dst + SIDE + s * (SIDE / SLABS), &vmap, 64 * s, y, ahead.head, w, full + at);
+        tma_load_4d(dst + s * 2048, map, 64 * s, y, ahead.head, w, full + at);
+        if (Sh::PAIRED) tma_load_4d(dst + SIDE + s * 2048, &vmap, 64 * s, y, ahead.head, w, full + at);
       }
     }
     ++asked;
@@ -188,9 +129,6 @@ __global__ void __launch_bounds__(RowsShape<HD, NT, Q8>::THREADS, 1)
   uint32_t used = 0;
   bool alive = true;
   const int c0 = 2 * (lane & 3);  // this thread's columns (rows of the item): c0, c0 + 1 of every eight
-  const int key1 = Q8 ? 4 * (lane >> 3) + ((lane >> 2) & 1) : lane >> 2;  // and its keys of a slice: this one and
-  constexpr int NEXT = Q8 ? 2 : 8;                                        // the one so far behind it
-  const int nb = p.hd / 16;       // Q8: scales of a key
   long long left = st.until - st.before;  // tiles
 #pragma unroll 1
   for (;; cur.next(p)) {
@@ -213,7 +151,7 @@ __global__ void __launch_bounds__(RowsShape<HD, NT, Q8>::THREADS, 1)
       for (int k = 0; k < KST; ++k)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const int i = Q8 ? 64 * (k >> 2) + 8 * c0 + 4 * (k & 3) + 2 * j : 16 * k + 8 * j + c0;
+          const int i = 16 * k + 8 * j + c0;
           v[k][j] = has && i < p.hd ? __ldcg(reinterpret_cast<const float2*>(src + i)) : make_float2(0.f, 0.f);
           big = fmaxf(big, fmaxf(fabsf(v[k][j].x), fabsf(v[k][j].y)));
         }
@@ -269,26 +207,9 @@ __global__ void __launch_bounds__(RowsShape<HD, NT, Q8>::THREADS, 1)
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int i = 0; i < 4; ++i) s[n][i] = part[n][0][i] = part[n][1][i] = part[n][2][i] = 0.f;
-        uint4 kw[2];     // Q8: this lane's 16 values of both keys
-        uint32_t kd[2];  // and their scales
 #pragma unroll
         for (int k = 0; k < KST; ++k) {
           uint32_t a[4];
-          if constexpr (Q8) {
-            if ((k & 3) == 0) {
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const int key = key1 + NEXT * h, b = k + (lane & 3);
-                const unsigned char* row = ring + (used % UNITS) * UNIT + (k >> 2) * 1024 + key * 64;
-                kw[h] = *reinterpret_cast<const uint4*>(row + (((lane & 3) ^ ((key >> 1) & 3)) << 4));
-                // (behind the head's end q is 0 and the codes' values are finite)
-                kd[h] = q8_scale_pair(HD % 64 == 0 && b >= nb ? 0u : scales[(used % UNITS) * Sh::SCALES + key * nb + b]);
-              }
-            }
-            const uint32_t w0 = (k & 3) == 0 ? kw[0].x : (k & 3) == 1 ? kw[0].y : (k & 3) == 2 ? kw[0].z : kw[0].w;
-            const uint32_t w1 = (k & 3) == 0 ? kw[1].x : (k & 3) == 1 ? kw[1].y : (k & 3) == 2 ? kw[1].z : kw[1].w;
-            a[0] = q8_lo(w0, kd[0]), a[1] = q8_lo(w1, kd[1]), a[2] = q8_hi(w0, kd[0]), a[3] = q8_hi(w1, kd[1]);
-          } else
           ldsm4(a, kb + (k >> 2) * 2048 + ((i4 & 1) * 8 + r8) * 128 + (((2 * (k & 3) + (i4 >> 1)) ^ r8) << 4));
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
@@ -307,7 +228,7 @@ __global__ void __launch_bounds__(RowsShape<HD, NT, Q8>::THREADS, 1)
           ask_next();
         }
         const bool masked = ks + 16 > full_hi || ks < full_lo;
-        const int key = ks + key1;
+        const int key = ks + (lane >> 2);
         bool grows = false, falls = false;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -318,7 +239,7 @@ __global__ void __launch_bounds__(RowsShape<HD, NT, Q8>::THREADS, 1)
             if (masked) {
               const int to = lim[n][j], from = attn_first_key(to, p.window);
               if (key > to || key < from) s[n][j] = -CUDART_INF_F;
-              if (key + NEXT > to || key + NEXT < from) s[n][2 + j] = -CUDART_INF_F;
+              if (key + 8 > to || key + 8 < from) s[n][2 + j] = -CUDART_INF_F;
             }
             grows |= !(max_nan(s[n][j], s[n][2 + j]) <= m[n][j] + ATTN_SLACK);  // (or there is none)
           }
@@ -338,7 +259,7 @@ __global__ void __launch_bounds__(RowsShape<HD, NT, Q8>::THREADS, 1)
           for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-              if (!Q8 && l[n][j] == l[n][j] && 8 * n + c0 + j < n_rows) {  // (a row that is NaN already stays that)
+              if (l[n][j] == l[n][j] && 8 * n + c0 + j < n_rows) {  // (a row that is NaN already stays that)
 #pragma unroll
                 for (int i = 0; i < 4; i += 2)
                   if (s[n][i + j] != s[n][i + j])
@@ -392,7 +313,7 @@ __global__ void __launch_bounds__(RowsShape<HD, NT, Q8>::THREADS, 1)
         }
         unsigned char* vs = ring + (used % UNITS) * UNIT + (Sh::PAIRED ? SIDE : 0);
         const uint32_t vb = smem_u32(vs);
-        if (!Q8 && masked) {
+        if (masked) {
 #pragma unroll 1
           for (int e = lane; e < 16 * SLABS * 8; e += 32) {  // 16-byte words, 128 bytes of a key after the other
             const int kk = ks + ((e >> 3) & 15);
@@ -410,48 +331,9 @@ __global__ void __launch_bounds__(RowsShape<HD, NT, Q8>::THREADS, 1)
         for (int k0 = 0; k0 < KST; k0 += AHEAD) {
           uint32_t a[AHEAD][4];
           float sum[AHEAD][NT][4];
-          if constexpr (Q8) {
-            // scales of this lane's keys 4 c .. 4 c + 3 and the four blocks, a word to each key; those that are no numbers count as zeros and wait
-            // for the item's end
-            static_assert(AHEAD == 4, "a word of scales");
-            const unsigned char* vd = scales + (used % UNITS) * Sh::SCALES + HD + 2 * c0 * nb + k0;
-            uint32_t w[4], bad = 0;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              if ((nb & 3) == 0) {
-                w[i] = k0 < nb ? *reinterpret_cast<const uint32_t*>(vd + i * nb) : 0u;
-              } else {  // (one byte after the other: those behind the head's end are the next key's)
-                w[i] = 0;
-#pragma unroll
-                for (int b = 0; b < 4; ++b)
-                  if (k0 + b < nb) w[i] |= (uint32_t)vd[i * nb + b] << (8 * b);
-              }
-              bad |= w[i] & (w[i] << 1);
-            }
-            if (bad & 0x80808080u) {
-              odd = true;
-#pragma unroll
-              for (int i = 0; i < 4; ++i) w[i] &= ~(((w[i] & (w[i] << 1) & 0x80808080u) >> 7) * 0xFFu);
-            }
-            uint32_t ab[2][2];  // blocks 0 and 1, and 2 and 3: of the first two keys, of the other two
-            ab[0][0] = __byte_perm(w[0], w[1], 0x5140), ab[1][0] = __byte_perm(w[0], w[1], 0x7362);
-            ab[0][1] = __byte_perm(w[2], w[3], 0x5140), ab[1][1] = __byte_perm(w[2], w[3], 0x7362);
-#pragma unroll
-            for (int k = 0; k < AHEAD; k += 2) {
-              uint32_t r[4];
-              const int c = k + (lane >> 4), kk = lane & 15;
-              ldsm2_t8(r, vb + (k0 >> 2) * 1024 + kk * 64 + ((c ^ ((kk >> 1) & 3)) << 4));
-#pragma unroll
-              for (int i = 0; i < 2; ++i) {
-                const uint32_t d01 = __byte_perm(ab[k >> 1][0], 0, i ? 0x3424 : 0x1404) >> 1, d23 = __byte_perm(ab[k >> 1][1], 0, i ? 0x3424 : 0x1404) >> 1;
-                a[k + i][0] = q8_lo(r[2 * i], d01), a[k + i][1] = q8_lo(r[2 * i + 1], d01);
-                a[k + i][2] = q8_hi(r[2 * i], d23), a[k + i][3] = q8_hi(r[2 * i + 1], d23);
-              }
-            }
-          }
 #pragma unroll
           for (int k = 0; k < AHEAD; ++k) {
-            if constexpr (!Q8) ldsm4_t(a[k], vb + ((k0 + k) >> 2) * 2048 + ((i4 >> 1) * 8 + r8) * 128 + (((2 * ((k0 + k) & 3) + (i4 & 1)) ^ r8) << 4));
+            ldsm4_t(a[k], vb + ((k0 + k) >> 2) * 2048 + ((i4 >> 1) * 8 + r8) * 128 + (((2 * ((k0 + k) & 3) + (i4 & 1)) ^ r8) << 4));
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -476,14 +358,12 @@ __global__ void __launch_bounds__(RowsShape<HD, NT, Q8>::THREADS, 1)
       }
     }
 
-    if constexpr (!Q8) {
 #pragma unroll
-      for (int k = 0; k < KST; ++k)
+    for (int k = 0; k < KST; ++k)
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+      for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) odd |= !(fabsf(o[k][n][i]) < CUDART_INF_F);
-    }
+        for (int i = 0; i < 4; ++i) odd |= !(fabsf(o[k][n][i]) < CUDART_INF_F);
 
     // ---- the warps' parts of the item
 #pragma unroll
@@ -574,11 +454,6 @@ __global__ void __launch_bounds__(RowsShape<HD, NT, Q8>::THREADS, 1)
       __threadfence();
       __syncthreads();
       const int r = lane < n_rows ? lane : 0;
-      if constexpr (Q8) {
-        attn_odd_blocks(p, cur.s, cur.head, (blk.tile0 + first_tile) << Sh::LOG2_TILE, (blk.tile0 + end_tile) << Sh::LOG2_TILE, lane < n_rows && s_weight[r] == s_weight[r],
-                        cur.seq.past + blk.t0 + attn_row_token(p, r), warp, WARPS,
-                        whole ? p.out + attn_row_offset(p, cur.seq.q0 + blk.t0, cur.head, r, p.out_stride) : p.part + ((size_t)attn_slot(blockIdx.x, share) * RB + r) * HD);
-      } else
 #pragma unroll 1
       for (int col0 = 32 * warp; col0 < p.hd; col0 += 32 * WARPS)
         attn_odd_values(p, cur.s, cur.seq.q0, cur.head, (blk.tile0 + first_tile) << Sh::LOG2_TILE, (blk.tile0 + end_tile) << Sh::LOG2_TILE, 1 << Sh::LOG2_TILE, full_lo,
@@ -598,29 +473,12 @@ __global__ void __launch_bounds__(RowsShape<HD, NT, Q8>::THREADS, 1)
     for (; used < asked; ++used) attn_wait(full + used % UNITS, used / UNITS);
 }
 
-template <int HD, int NT, bool Q8>
+template <int HD, int NT>
 cudaError_t run_rows(infr_cuda_ctx* ctx, const CUtensorMap& km, const CUtensorMap& vm, const AttnParams& p) {
-  using Sh = RowsShape<HD, NT, Q8>;
-  const cudaError_t e = ensure_smem(reinterpret_cast<const void*>(&k_attn_rows<HD, NT, Q8>), Sh::SMEM);
+  using Sh = RowsShape<HD, NT>;
+  const cudaError_t e = ensure_smem(reinterpret_cast<const void*>(&k_attn_rows<HD, NT>), Sh::SMEM);
   if (e != cudaSuccess) return e;
-  return launch_ex(k_attn_rows<HD, NT, Q8>, dim3(ctx->sm_count < ATTN_MAX_CTAS ? ctx->sm_count : ATTN_MAX_CTAS), dim3(Sh::THREADS), Sh::SMEM, ctx->stream, true, km, vm, p);
-}
-
-template <int HD>
-cudaError_t run_rows_of(infr_cuda_ctx* ctx, const CUtensorMap& km, const CUtensorMap& vm, const AttnParams& p, int nt) {
-  if (p.kq != nullptr) return nt == 1 ? run_rows<HD, 1, true>(ctx, km, vm, p) : run_rows<HD, 2, true>(ctx, km, vm, p);
-  return nt == 1 ? run_rows<HD, 1, false>(ctx, km, vm, p) : run_rows<HD, 2, false>(ctx, km, vm, p);
-}
-
-// Codes of 16 keys of a head, 64 values wide.
-bool attn_codes_map(CUtensorMap* tm, const uint8_t* base, const AttnParams& p) {
-  EncodeTiledFn enc = encode_tiled_fn();
-  if (!enc) return false;
-  const cuuint64_t dims[4] = {(cuuint64_t)p.hd, (cuuint64_t)p.page_size, (cuuint64_t)p.n_kv, (cuuint64_t)p.n_pages};
-  const cuuint64_t strides[3] = {p.row_pitch, p.head_pitch, p.page_pitch};
-  const cuuint32_t box[4] = {64, 16, 1, 1}, estr[4] = {1, 1, 1, 1};
-  return enc(tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<uint8_t*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B,
-             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return launch_ex(k_attn_rows<HD, NT>, dim3(ctx->sm_count < ATTN_MAX_CTAS ? ctx->sm_count : ATTN_MAX_CTAS), dim3(Sh::THREADS), Sh::SMEM, ctx->stream, true, km, vm, p);
 }
 
 }  // namespace
@@ -639,16 +497,17 @@ bool attn_cache_map(CUtensorMap* tm, const __half* base, const AttnParams& p, in
 // max_rows: rows (tokens x heads of a kv head) that a sequence's new tokens make at most, as far as the caller knows; longer ones are
 // cut into more items.
 int32_t launch_attn_rows(infr_cuda_ctx* ctx, AttnParams p, const __half* k, int max_rows) {
+  if (p.kq != nullptr) return launch_attn_rows_q8(ctx, p, max_rows);
   p.k = k;
   CUtensorMap km, vm;
-  if (p.kq != nullptr ? !attn_codes_map(&km, p.kq, p) || !attn_codes_map(&vm, p.vq, p) : !attn_cache_map(&km, k, p, 16) || !attn_cache_map(&vm, p.v, p, 16)) return fail(ctx, INFR_CUDA_ERR_CUDA, "attention: cuTensorMapEncodeTiled failed");
+  if (!attn_cache_map(&km, k, p, 16) || !attn_cache_map(&vm, p.v, p, 16)) return fail(ctx, INFR_CUDA_ERR_CUDA, "attention: cuTensorMapEncodeTiled failed");
   const int nt = p.g <= 8 && max_rows <= 8 ? 1 : 2;
   p.tb = 8 * nt / p.g;
   cudaError_t e;
-  if (p.hd <= 64) e = run_rows_of<64>(ctx, km, vm, p, nt);
-  else if (p.hd <= 128) e = run_rows_of<128>(ctx, km, vm, p, nt);
-  else if (p.hd <= 192) e = run_rows_of<192>(ctx, km, vm, p, nt);
-  else e = run_rows_of<256>(ctx, km, vm, p, nt);
+  if (p.hd <= 64) e = nt == 1 ? run_rows<64, 1>(ctx, km, vm, p) : run_rows<64, 2>(ctx, km, vm, p);
+  else if (p.hd <= 128) e = nt == 1 ? run_rows<128, 1>(ctx, km, vm, p) : run_rows<128, 2>(ctx, km, vm, p);
+  else if (p.hd <= 192) e = nt == 1 ? run_rows<192, 1>(ctx, km, vm, p) : run_rows<192, 2>(ctx, km, vm, p);
+  else e = nt == 1 ? run_rows<256, 1>(ctx, km, vm, p) : run_rows<256, 2>(ctx, km, vm, p);
   if (e != cudaSuccess) return check_cuda(ctx, e, "k_attn_rows launch");
   ctx->launches += 1;
   return check_cuda(ctx, cudaGetLastError(), "k_attn_rows launch");

@@ -1,0 +1,560 @@
+// Attention of a few rows per (sequence, kv head) over pages of 8 bits (kv_q8.cuh): the form of attn_rows.cu - a warp streams slices of its own through a ring of its
+// own, both products transposed, q and the weights as two f16 pieces each, results f32 - with the codes turned into f16 fragments in registers.
+//
+//   S^T[16 keys, 8 rows] = K[16, hd] q^T[hd, 8],    O^T[hd, 8 rows] += V^T[hd, 16 keys] P^T[16 keys, 8 rows]
+//
+// What a product sums over may go in any order that both operands have.  A lane takes for K 16 neighbouring values of a key at once: one 16-byte word and one
+// scale are four steps of the product.  And the 16 keys stand in the order in which a transposing load of bytes gives V's, four neighbouring keys to a lane: row i
+// of the scores is key 4 (i / 2) + i % 2, row 8 + i two behind it.  A block of 16 values of V is one product's 16 rows, so its scales are one number to each key.
+//
+// Half the bytes of f16 pages leave the instructions as the bound: a code costs one and a half of them on its way to f16 (byte behind the exponent of 1024, minus
+// 1152, times the scale: all exact).  So a warp works on 32 keys at a time where the registers hold it: the checks of the running maximum, the ring and the additions of
+// sums come once for these, and two chains of products run beside each other.
+#include "attn.cuh"
+#include "kv_q8.cuh"
+
+namespace infr {
+namespace {
+
+constexpr int ROWS_EXTRA = 3;  // tiles' time that an item's beginning and end take
+
+// Two 16 x 16 matrices of bytes transposed: r[0], r[1] are rows lane / 4 and 8 more of the first, columns 4 (lane % 4) .. + 3.
+__device__ __forceinline__ void ldsm2_t8(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m16n16.x2.trans.shared.b8 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+
+template <int HD, int NT>
+struct Q8Shape {
+  static constexpr int WARPS = 8, THREADS = WARPS * 32, RB = 8 * NT;
+  static constexpr int HALVES = HD <= 128 ? 2 : 1, KEYS = 16 * HALVES;  // keys of a slice
+  static constexpr int LOG2_TILE = HALVES == 2 ? 8 : 7;
+  static constexpr int SIDE = KEYS * HD;                // bytes of a slice of K, or of V
+  static constexpr int UNIT = 2 * SIDE, SCALES = 2 * KEYS * HD / 16;
+  static constexpr int PITCH = HD + 4;                  // words: the fragments' columns fall on different banks
+  static constexpr int SLOTS = HD == 64 ? WARPS : WARPS / 2;  // half of the warps add theirs to the others' first
+  static constexpr int MERGE = SLOTS * RB * PITCH * 4, STATS = 2 * WARPS * RB * 4;
+  static constexpr int FIT = (232448 - 1024 - 1024 - MERGE - STATS) / (WARPS * (UNIT + SCALES));
+  static constexpr int UNITS = FIT > 4 ? 4 : FIT;
+  static constexpr int SMEM = 1024 + WARPS * UNITS * (UNIT + SCALES) + MERGE + STATS + WARPS * UNITS * 8;
+  static_assert(UNITS >= 2, "one to work on, one on its way");
+  static_assert(WARPS * UNITS * UNIT >= 16 * ATTN_MAX_SEQ + 4, "what is known of the sequences fits where the keys go later");
+};
+
+// Columns of rows of the item, the part of it that lies here, where 16 values of V that a row sees are not numbers, become NaN.  All of the warp's lanes take
+// part, a row to each of the first ones; `active`: not NaN already.  Blocks of 16 from block0 on, every `step`-th.
+static __device__ __noinline__ void attn_odd_blocks(const AttnParams& p, int s, int head, int key0, int key1, bool active, int to, int block0, int step, float* dst) {
+  const int lane = threadIdx.x & 31, from = attn_first_key(to, p.window);
+  const int lo = max(key0, __reduce_min_sync(0xFFFFFFFFu, active ? from : 0x7FFFFFFF)), hi = min(key1 - 1, __reduce_max_sync(0xFFFFFFFFu, active ? to : -1));
+#pragma unroll 1
+  for (int b = block0; b < p.hd / 16; b += step) {
+    bool sees = false;
+#pragma unroll 1
+    for (int k0 = lo & ~31; k0 <= hi; k0 += 32) {
+      const int key = k0 + lane;
+      bool odd = false;
+      if (key >= lo && key <= hi) {
+        const int page = attn_page_of(p, key);
+        odd = __ldcg(p.vs + ((size_t)attn_page(p, s, page) * p.page_pitch + (size_t)head * p.head_pitch + (size_t)(key - page * p.page_size) * p.row_pitch) / 16 + b) >= Q8_ODD;
+      }
+#pragma unroll 1
+      for (uint32_t found = __ballot_sync(0xFFFFFFFFu, odd); found; found &= found - 1) {
+        const int key = k0 + __ffs(found) - 1;
+        sees |= active && key >= from && key <= to;
+      }
+    }
+    if (sees)
+      for (int i = 0; i < 16; i += 4) __stcg(reinterpret_cast<float4*>(dst + 16 * b + i), make_float4(CUDART_NAN_F, CUDART_NAN_F, CUDART_NAN_F, CUDART_NAN_F));
+  }
+}
+
+template <int HD, int NT>
+__global__ void __launch_bounds__(Q8Shape<HD, NT>::THREADS, 1)
+    k_attn_rows_q8(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ AttnParams p, const int box) {
+  using Sh = Q8Shape<HD, NT>;
+  constexpr int WARPS = Sh::WARPS, THREADS = Sh::THREADS, RB = Sh::RB, UNITS = Sh::UNITS, UNIT = Sh::UNIT, SIDE = Sh::SIDE, PITCH = Sh::PITCH, SLOTS = Sh::SLOTS;
+  constexpr int SLABS = HD / 64, KST = HD / 16, HALVES = Sh::HALVES, KEYS = Sh::KEYS, SLAB = KEYS * 64;
+  constexpr int AHEAD = 4;  // sums under way, and a word of scales
+  static_assert(NT * KST * 512 <= Sh::MERGE, "q's pieces lie where the sums go");
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ long long s_scan[WARPS];
+  __shared__ AttnStart s_start;
+  __shared__ int s_last;
+  __shared__ float s_weight[RB], s_factor[RB];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  unsigned char* ring_all = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  unsigned char *ring = ring_all + warp * UNITS * UNIT, *scales = ring_all + WARPS * UNITS * UNIT + warp * UNITS * Sh::SCALES;
+  float* s_o = reinterpret_cast<float*>(ring_all + WARPS * UNITS * (UNIT + Sh::SCALES));
+  uint4* s_q = reinterpret_cast<uint4*>(s_o);  // [NT][KST][32]
+  float* s_m = s_o + SLOTS * RB * PITCH;
+  float* s_l = s_m + WARPS * RB;
+  uint64_t* full = reinterpret_cast<uint64_t*>(s_l + WARPS * RB) + warp * UNITS;
+
+  pdl_trigger();  // the next kernel may take the SMs that this one leaves free, and do what needs no input of its
+  if (lane == 0)
+    for (int i = 0; i < UNITS; ++i) mbar_init(full + i, 1);
+  mbar_fence_init();
+  pdl_wait();
+  attn_plan<THREADS, Sh::LOG2_TILE, ROWS_EXTRA, 0>(p, reinterpret_cast<int*>(ring_all), s_scan, &s_start);
+  const AttnStart st = s_start;
+  if (st.until == st.before) return;
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the plan's words lay where the copies go
+  __syncthreads();
+
+  const int nb = p.hd / 16;  // scales of a key
+  // ---- what the warp asks for: its slices of the CTA's tiles, one after the other, as many as its ring holds
+  AttnCursor<Sh::LOG2_TILE, ROWS_EXTRA> ahead;
+  ahead.start(p, st);
+  AttnCursor<Sh::LOG2_TILE, ROWS_EXTRA> cur = ahead;  // what it works on
+  int at = ahead.first(st);  // tile of its item to look at next
+  int a_key = -1;            // first key of the slice to ask for (-1: none left),
+  int a_page[HALVES];        // its pages' numbers (-1: none of these 16 keys is seen)
+  uint32_t asked = 0;
+  auto find = [&]() {        // the next tile of which this warp has keys
+#pragma unroll 1
+    while (ahead.ub < st.u1) {
+      if (at >= ahead.end(st)) {
+        ahead.next(p);
+        at = 0;
+        continue;
+      }
+      const int ks = ((ahead.blk.tile0 + at) << Sh::LOG2_TILE) + warp * KEYS;
+      if (ks < ahead.blk.hi && ks + KEYS > ahead.blk.lo) {
+        a_key = ks;
+#pragma unroll
+        for (int h = 0; h < HALVES; ++h) {
+          // (a page that holds the whole slice is asked for once)
+          const int key = box == KEYS ? max(ks, ahead.blk.lo & ~15) : ks + 16 * h;
+          a_page[h] = (h == 0 || box < KEYS) && key < ahead.blk.hi && key + 16 > ahead.blk.lo ? attn_page_entry(p, ahead.s, attn_page_of(p, key)) : -1;
+          if (a_page[h] < 0 && (h == 0 || box < KEYS) && key < ahead.blk.hi && key + 16 > ahead.blk.lo) a_page[h] = 0x7FFFFFFF;  // (not a page: reported below)
+        }
+        return;
+      }
+      ++at;
+    }
+    a_key = -1;
+  };
+  auto ask_next = [&]() {
+    if (a_key < 0) return;
+    if (lane == 0) {
+      const int to = asked % UNITS;
+      unsigned char *dst = ring + to * UNIT, *sc = scales + to * Sh::SCALES;
+      int parts = 0;
+#pragma unroll
+      for (int h = 0; h < HALVES; ++h) parts += a_page[h] >= 0;
+      mbar_arrive_expect_tx(full + to, parts * box * (2 * HD + 2 * nb));
+#pragma unroll
+      for (int h = 0; h < HALVES; ++h) {
+        if (a_page[h] < 0) continue;
+        const int key = a_key + 16 * h, page = attn_page_of(p, key), y = key - page * p.page_size, w = attn_page_checked(p, a_page[h]);
+        const size_t first = ((size_t)w * p.page_pitch + (size_t)ahead.head * p.head_pitch + (size_t)y * p.row_pitch) / 16;
+        bulk_g2s(sc + 16 * h * nb, p.ks + first, box * nb, full + to);
+        bulk_g2s(sc + Sh::SCALES / 2 + 16 * h * nb, p.vs + first, box * nb, full + to);
+#pragma unroll
+        for (int s = 0; s < SLABS; ++s) {
+          tma_load_4d(dst + s * SLAB + h * 1024, &kmap, 64 * s, y, ahead.head, w, full + to);
+          tma_load_4d(dst + SIDE + s * SLAB + h * 1024, &vmap, 64 * s, y, ahead.head, w, full + to);
+        }
+      }
+    }
+    ++asked;
+    ++at;
+    find();
+  };
+  find();
+#pragma unroll 1
+  for (int i = 0; i < UNITS; ++i) ask_next();
+
+  uint32_t used = 0;
+  bool alive = true;
+  const int c0 = 2 * (lane & 3);  // this thread's columns (rows of the item): c0, c0 + 1 of every eight
+  const int key1 = 4 * (lane >> 3) + ((lane >> 2) & 1);  // and its keys of every 16: this one, and two behind it
+  long long left = st.until - st.before;  // tiles
+#pragma unroll 1
+  for (;; cur.next(p)) {
+    const AttnBlock& blk = cur.blk;
+    const int first_tile = cur.first(st), end_tile = cur.end(st), n_rows = blk.nt * p.g;
+
+    // ---- q: B fragments of q^T, rows scaled by a power of two, as two f16 pieces, put down by one warp per eight rows where the sums go
+    // at the item's end; of 64 values step k has 16 c + 4 k .. + 3 of lane c
+    float f[NT][2];  // of the thread's columns: score -> log2 units
+    int lim[NT][2];  // and the last key their row sees
+    __syncthreads();  // the last item's sums have been read
+    if (warp < NT) {
+      const int r = 8 * warp + (lane >> 2);
+      const bool has = r < n_rows;
+      const float* src = p.q + attn_row_offset(p, cur.seq.q0 + blk.t0, cur.head, has ? r : 0, p.q_stride);
+      float4 v[KST];
+      float big = 0.f;
+#pragma unroll
+      for (int k = 0; k < KST; ++k) {
+        const int i = 64 * (k >> 2) + 8 * c0 + 4 * (k & 3);
+        v[k] = has && i < p.hd ? __ldcg(reinterpret_cast<const float4*>(src + i)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        big = fmaxf(big, fmaxf(fmaxf(fabsf(v[k].x), fabsf(v[k].y)), fmaxf(fabsf(v[k].z), fabsf(v[k].w))));
+      }
+      big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 1));
+      big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 2));
+      float down, up;
+      attn_row_scale(big, down, up);
+#pragma unroll
+      for (int k = 0; k < KST; ++k) {
+        uint4 w;
+        split2(v[k].x * down, v[k].y * down, w.x, w.z);
+        split2(v[k].z * down, v[k].w * down, w.y, w.w);
+        s_q[(warp * KST + k) * 32 + lane] = w;
+      }
+      if ((lane & 3) == 0) s_factor[r] = up * p.scale_log2;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int rr = 8 * n + c0 + j;
+        f[n][j] = s_factor[rr];
+        lim[n][j] = cur.seq.past + blk.t0 + (rr < n_rows ? attn_row_token(p, rr) : blk.nt - 1);
+      }
+    const int full_hi = attn_full_hi(cur.seq, blk), full_lo = attn_full_lo(cur.seq, blk, p.window);
+
+    float o[KST][NT][4], m[NT][2], l[NT][2];
+#pragma unroll
+    for (int k = 0; k < KST; ++k)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[k][n][i] = 0.f;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) m[n][0] = m[n][1] = -CUDART_INF_F, l[n][0] = l[n][1] = 0.f;
+
+    bool odd = false;  // values that are no numbers were left out
+#pragma unroll 1
+    for (int t = first_tile; t < end_tile; ++t) {
+      const int ks = ((blk.tile0 + t) << Sh::LOG2_TILE) + warp * KEYS;
+      if (ks >= blk.hi || ks + KEYS <= blk.lo) continue;
+      if (alive) {
+        alive = wait_all(full + used % UNITS, used / UNITS);
+        if (!alive && lane == 0) atomicExch(&p.status->timeout, 10);
+      }
+      if (!alive) continue;
+      const unsigned char *kb = ring + (used % UNITS) * UNIT, *sc = scales + (used % UNITS) * Sh::SCALES;
+      // ---- scores: pieces and even and odd steps apart
+      float s[HALVES][NT][4];
+#pragma unroll
+      for (int h = 0; h < HALVES; ++h) {
+        float part[NT][3][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[h][n][i] = part[n][0][i] = part[n][1][i] = part[n][2][i] = 0.f;
+#pragma unroll
+        for (int b = 0; b < SLABS; ++b) {
+          uint4 kw[2];     // this lane's 16 values of both keys
+          uint32_t kd[2];  // and their scales (behind the head's end q is 0 and the codes' values are finite)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int key = 16 * h + key1 + 2 * j, blk16 = 4 * b + (lane & 3);
+            kw[j] = *reinterpret_cast<const uint4*>(kb + b * SLAB + key * 64 + (((lane & 3) ^ ((key >> 1) & 3)) << 4));
+            kd[j] = q8_scale_pair(blk16 < nb ? sc[key * nb + blk16] : 0u);
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t w0 = k == 0 ? kw[0].x : k == 1 ? kw[0].y : k == 2 ? kw[0].z : kw[0].w;
+            const uint32_t w1 = k == 0 ? kw[1].x : k == 1 ? kw[1].y : k == 2 ? kw[1].z : kw[1].w;
+            const uint32_t a[4] = {q8_lo(w0, kd[0]), q8_lo(w1, kd[1]), q8_hi(w0, kd[0]), q8_hi(w1, kd[1])};
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              const uint4 w = s_q[(n * KST + 4 * b + k) * 32 + lane];
+              mma16816(k & 1 ? part[n][0] : s[h][n], a, w.x, w.y);
+              mma16816(k & 1 ? part[n][2] : part[n][1], a, w.z, w.w);
+            }
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[h][n][i] = (s[h][n][i] + part[n][0][i]) + (part[n][1][i] + part[n][2][i]);
+      }
+      const bool masked = ks + KEYS > full_hi || ks < full_lo;
+      bool grows = false, falls = false;
+      float top[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+#pragma unroll
+          for (int h = 0; h < HALVES; ++h) {
+            s[h][n][j] *= f[n][j];
+            s[h][n][2 + j] *= f[n][j];
+            if (masked) {
+              const int to = lim[n][j], from = attn_first_key(to, p.window), key = ks + 16 * h + key1;
+              if (key > to || key < from) s[h][n][j] = -CUDART_INF_F;
+              if (key + 2 > to || key + 2 < from) s[h][n][2 + j] = -CUDART_INF_F;
+            }
+          }
+          top[n][j] = max_nan(s[0][n][j], s[0][n][2 + j]);
+          if (HALVES == 2) top[n][j] = max_nan(top[n][j], s[HALVES - 1][n][j], s[HALVES - 1][n][2 + j]);
+          grows |= !(top[n][j] <= m[n][j] + ATTN_SLACK);  // (or there is none)
+        }
+      if ((t & 3) == 0) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            uint32_t high = __ballot_sync(0xFFFFFFFFu, !(top[n][j] < m[n][j] - ATTN_FALL));  // of each column's eight lanes
+            high |= high >> 16, high |= high >> 8, high |= high >> 4;
+            falls |= (high & 15u) != 15u;
+          }
+      }
+      // (the maximum is looked for only where a score is past the slack, or all of a column's are far below: votes instead of rounds of shuffles)
+      if (__any_sync(0xFFFFFFFFu, grows) || falls) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            float mx = -CUDART_INF_F, lx = l[n][j];
+#pragma unroll
+            for (int h = 0; h < HALVES; ++h) mx = fmaxf(mx, fmaxf(s[h][n][j], s[h][n][2 + j]));  // (a NaN leaves the reference where it is)
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, x));
+            if (falls) {
+#pragma unroll
+              for (int x = 4; x < 32; x <<= 1) lx = fmaxf(lx, __shfl_xor_sync(0xFFFFFFFFu, lx, x));
+            }
+            float to = m[n][j];
+            if (mx > to + ATTN_SLACK) to = ceilf(mx);
+            // (down only as far as leaves the sums in range: weights so far below 2^60)
+            else if (falls && mx < to - ATTN_FALL && mx > -CUDART_INF_F) to = fminf(to, fmaxf(ceilf(mx), to + (float)((int)(__float_as_uint(lx) >> 23) - 187)));
+            const float w = to == m[n][j] ? 1.f : exp2_rel(m[n][j], to);
+            m[n][j] = to;
+            l[n][j] *= w;
+#pragma unroll
+            for (int k = 0; k < KST; ++k) o[k][n][j] *= w, o[k][n][2 + j] *= w;
+          }
+      }
+      // ---- weights, transposed into B fragments
+      uint32_t ph[HALVES][NT][2], pl[HALVES][NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int h = 0; h < HALVES; ++h) {
+          float e[4];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float ref = m[n][j] == -CUDART_INF_F ? 0.f : m[n][j];
+            e[j] = exp2_approx((s[h][n][j] - ref) + ATTN_BIAS);  // (in this order: scores of any size)
+            e[2 + j] = exp2_approx((s[h][n][2 + j] - ref) + ATTN_BIAS);
+            l[n][j] += e[j] + e[2 + j];
+          }
+          split2(e[0], e[1], ph[h][n][0], pl[h][n][0]);
+          split2(e[2], e[3], ph[h][n][1], pl[h][n][1]);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) ph[h][n][i] = movm(ph[h][n][i]), pl[h][n][i] = movm(pl[h][n][i]);
+        }
+      // ---- sums, from zero for every slice and added here: the tensor cores truncate, and a running sum would lose 2^-23 of itself to every slice.
+      // (0 x value is 0 whatever the codes; scales that are no numbers, and those of keys that no row sees, count as zeros.)
+      const uint32_t vb = smem_u32(kb + SIDE);
+#pragma unroll
+      for (int k0 = 0; k0 < KST; k0 += AHEAD) {
+        float sum[AHEAD][NT][4];
+#pragma unroll
+        for (int h = 0; h < HALVES; ++h) {
+          uint32_t w[4], bad = 0;  // scales of the keys 4 c .. 4 c + 3 of these 16, a byte to each of the four blocks
+          const unsigned char* vd = sc + Sh::SCALES / 2 + (16 * h + 2 * c0) * nb + k0;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if ((nb & 3) == 0) {
+              w[i] = k0 < nb ? *reinterpret_cast<const uint32_t*>(vd + i * nb) : 0u;
+            } else {  // (one byte after the other: those behind the head's end are the next key's)
+              w[i] = 0;
+#pragma unroll
+              for (int b = 0; b < 4; ++b)
+                if (k0 + b < nb) w[i] |= (uint32_t)vd[i * nb + b] << (8 * b);
+            }
+            if (masked) {
+              const int key = ks + 16 * h + 2 * c0 + i;
+              if (key >= blk.hi || key < blk.lo) w[i] = 0;
+            }
+            bad |= w[i] & (w[i] << 1);
+          }
+          if (bad & 0x80808080u) {
+            odd = true;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] &= ~(((w[i] & (w[i] << 1) & 0x80808080u) >> 7) * 0xFFu);
+          }
+          uint32_t ab[2][2];  // blocks 0 and 1, and 2 and 3: of the first two keys, of the other two
+          ab[0][0] = __byte_perm(w[0], w[1], 0x5140), ab[1][0] = __byte_perm(w[0], w[1], 0x7362);
+          ab[0][1] = __byte_perm(w[2], w[3], 0x5140), ab[1][1] = __byte_perm(w[2], w[3], 0x7362);
+#pragma unroll
+          for (int k = 0; k < AHEAD; k += 2) {
+            uint32_t r[4];
+            const int c = k + (lane >> 4), kk = 16 * h + (lane & 15);
+            ldsm2_t8(r, vb + (k0 >> 2) * SLAB + kk * 64 + ((c ^ ((kk >> 1) & 3)) << 4));
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const uint32_t d01 = __byte_perm(ab[k >> 1][0], 0, i ? 0x3424 : 0x1404) >> 1, d23 = __byte_perm(ab[k >> 1][1], 0, i ? 0x3424 : 0x1404) >> 1;
+              const uint32_t a[4] = {q8_lo(r[2 * i], d01), q8_lo(r[2 * i + 1], d01), q8_hi(r[2 * i], d23), q8_hi(r[2 * i + 1], d23)};
+#pragma unroll
+              for (int n = 0; n < NT; ++n) {
+                float(&to)[4] = sum[k + i][n];
+                if (h == 0) to[0] = to[1] = to[2] = to[3] = 0.f;
+                mma16816(to, a, pl[h][n][0], pl[h][n][1]);
+                mma16816(to, a, ph[h][n][0], ph[h][n][1]);
+              }
+            }
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k)
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[k0 + k][n][i] += sum[k][n][i];
+      }
+      __syncwarp();
+      ++used;
+      ask_next();
+    }
+
+    // ---- the warps' parts of the item
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) l[n][j] += __shfl_xor_sync(0xFFFFFFFFu, l[n][j], x);
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        if (m[n][j] == -CUDART_INF_F && l[n][j] != 0.f) m[n][j] = 0.f;  // nothing but NaN: a part that counts, not one without keys
+    __syncthreads();  // the last item's parts have been read, and q's pieces
+    // one half of the warps puts its sums down, the other adds its own to them, each brought to the higher maximum
+    if (lane < 4) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) s_m[warp * RB + 8 * n + c0 + j] = m[n][j], s_l[warp * RB + 8 * n + c0 + j] = l[n][j];
+    }
+    float* mine = s_o + (warp & (SLOTS - 1)) * RB * PITCH + (lane >> 2);
+    if (SLOTS == WARPS || warp >= SLOTS) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int k = 0; k < KST; ++k) {
+            float* to = mine + (8 * n + c0 + j) * PITCH + 16 * k;
+            to[0] = o[k][n][j];
+            to[8] = o[k][n][2 + j];
+          }
+    }
+    if constexpr (SLOTS < WARPS) __syncthreads();
+    if (SLOTS < WARPS && warp < SLOTS) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float other = s_m[(warp + SLOTS) % WARPS * RB + 8 * n + c0 + j], to = fmaxf(m[n][j], other);
+          const float a = exp2_rel(m[n][j], to), b = exp2_rel(other, to);
+#pragma unroll
+          for (int k = 0; k < KST; ++k) {
+            float* x = mine + (8 * n + c0 + j) * PITCH + 16 * k;
+            x[0] = a * o[k][n][j] + b * x[0];
+            x[8] = a * o[k][n][2 + j] + b * x[8];
+          }
+        }
+    }
+    const bool any_odd = __syncthreads_or(odd) != 0;
+    const bool whole = first_tile == 0 && end_tile == blk.ntile;
+    AttnShare share = {0, 0};
+    if (!whole) share = attn_share(cur.ub, blk.ntile, st);
+#pragma unroll 1
+    for (int e = tid; e < RB * (HD / 4); e += THREADS) {
+      const int r = e / (HD / 4), i = 4 * (e % (HD / 4));
+      if (r >= n_rows) continue;
+      float M = -CUDART_INF_F, L = 0.f;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) M = fmaxf(M, s_m[w * RB + r]);
+      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < SLOTS; ++w) {
+        constexpr bool two = SLOTS < WARPS;  // this slot holds two warps' sums
+        const float m0 = s_m[w * RB + r], m1 = two ? s_m[(w + SLOTS) % WARPS * RB + r] : -CUDART_INF_F;
+        const float wt = exp2_rel(fmaxf(m0, m1), M);
+        const float4 v = *reinterpret_cast<const float4*>(s_o + (w * RB + r) * PITCH + i);
+        L += exp2_rel(m0, M) * s_l[w * RB + r];
+        if (two) L += exp2_rel(m1, M) * s_l[(w + SLOTS) % WARPS * RB + r];
+        sum.x += wt * v.x, sum.y += wt * v.y, sum.z += wt * v.z, sum.w += wt * v.w;
+      }
+      if (whole) {
+        const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
+        if (i < p.hd)
+          *reinterpret_cast<float4*>(p.out + attn_row_offset(p, cur.seq.q0 + blk.t0, cur.head, r, p.out_stride) + i) = make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
+      } else {
+        const size_t to = (size_t)attn_slot(blockIdx.x, share) * RB + r;
+        __stcg(reinterpret_cast<float4*>(p.part + to * HD + i), sum);
+        if (i == 0) __stcg(p.part_ml + to, make_float2(M, L));
+      }
+      if (i == 0) s_weight[r] = L;
+    }
+    if (any_odd) {  // some row may see values that are no numbers
+      __threadfence();
+      __syncthreads();
+      const int r = lane < n_rows ? lane : 0;
+      attn_odd_blocks(p, cur.s, cur.head, (blk.tile0 + first_tile) << Sh::LOG2_TILE, (blk.tile0 + end_tile) << Sh::LOG2_TILE, lane < n_rows && s_weight[r] == s_weight[r],
+                      cur.seq.past + blk.t0 + attn_row_token(p, r), warp, WARPS,
+                      whole ? p.out + attn_row_offset(p, cur.seq.q0 + blk.t0, cur.head, r, p.out_stride) : p.part + ((size_t)attn_slot(blockIdx.x, share) * RB + r) * HD);
+    }
+    if (!whole && attn_arrive(p, share.first, share.last, &s_last, tid == 0, 0, THREADS)) {
+#pragma unroll 1
+      for (int r = warp; r < n_rows; r += WARPS)
+        attn_join_row<HD>(p, share, RB, r, p.out + attn_row_offset(p, cur.seq.q0 + blk.t0, cur.head, r, p.out_stride));
+    }
+    left -= end_tile - first_tile;
+    if (left <= 0) break;
+  }
+  // a warp that gave up has copies in flight: they land before its shared memory is somebody else's
+  if (!alive)
+    for (; used < asked; ++used) attn_wait(full + used % UNITS, used / UNITS);
+}
+
+// Codes of `box` keys of a head, 64 values wide.
+bool attn_codes_map(CUtensorMap* tm, const uint8_t* base, const AttnParams& p, int box) {
+  EncodeTiledFn enc = encode_tiled_fn();
+  if (!enc) return false;
+  const cuuint64_t dims[4] = {(cuuint64_t)p.hd, (cuuint64_t)p.page_size, (cuuint64_t)p.n_kv, (cuuint64_t)p.n_pages};
+  const cuuint64_t strides[3] = {p.row_pitch, p.head_pitch, p.page_pitch};
+  const cuuint32_t sizes[4] = {64, (cuuint32_t)box, 1, 1}, estr[4] = {1, 1, 1, 1};
+  return enc(tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<uint8_t*>(base), dims, strides, sizes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int HD, int NT>
+int32_t run_rows_q8(infr_cuda_ctx* ctx, const AttnParams& p) {
+  using Sh = Q8Shape<HD, NT>;
+  const int box = p.page_size % Sh::KEYS == 0 ? Sh::KEYS : 16;
+  CUtensorMap km, vm;
+  if (!attn_codes_map(&km, p.kq, p, box) || !attn_codes_map(&vm, p.vq, p, box)) return fail(ctx, INFR_CUDA_ERR_CUDA, "attention: cuTensorMapEncodeTiled failed");
+  cudaError_t e = ensure_smem(reinterpret_cast<const void*>(&k_attn_rows_q8<HD, NT>), Sh::SMEM);
+  if (e == cudaSuccess)
+    e = launch_ex(k_attn_rows_q8<HD, NT>, dim3(ctx->sm_count < ATTN_MAX_CTAS ? ctx->sm_count : ATTN_MAX_CTAS), dim3(Sh::THREADS), Sh::SMEM, ctx->stream, true, km, vm, p, box);
+  if (e != cudaSuccess) return check_cuda(ctx, e, "k_attn_rows_q8 launch");
+  ctx->launches += 1;
+  return check_cuda(ctx, cudaGetLastError(), "k_attn_rows_q8 launch");
+}
+
+template <int HD>
+int32_t run_rows_q8_of(infr_cuda_ctx* ctx, const AttnParams& p, int nt) { return nt == 1 ? run_rows_q8<HD, 1>(ctx, p) : run_rows_q8<HD, 2>(ctx, p); }
+
+}  // namespace
+
+// max_rows: see launch_attn_rows.
+int32_t launch_attn_rows_q8(infr_cuda_ctx* ctx, AttnParams p, int max_rows) {
+  const int nt = p.g <= 8 && max_rows <= 8 ? 1 : 2;
+  p.tb = 8 * nt / p.g;
+  if (p.hd <= 64) return run_rows_q8_of<64>(ctx, p, nt);
+  if (p.hd <= 128) return run_rows_q8_of<128>(ctx, p, nt);
+  if (p.hd <= 192) return run_rows_q8_of<192>(ctx, p, nt);
+  return run_rows_q8_of<256>(ctx, p, nt);
+}
+
+}  // namespace infr
