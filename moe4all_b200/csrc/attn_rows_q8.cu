@@ -1,5 +1,5 @@
-// Attention of a few rows per (sequence, kv head) over pages of 8 bits (kv_q8.cuh): the form of attn_rows.cu - a warp streams slices of its own through a ring of its
-// own, both products transposed, q and the weights as two f16 pieces each, results f32 - with the codes turned into f16 fragments in registers.
+// Attention of a few rows per (sequence, kv head) over pages of 8 bits (kv_q8.cuh): the form of attn_rows.cu - a warp to 16 keys of a tile, both products transposed, q
+// and the weights as two f16 pieces each, results f32 - with the codes turned into f16 fragments in registers.
 //
 //   S^T[16 keys, 8 rows] = K[16, hd] q^T[hd, 8],    O^T[hd, 8 rows] += V^T[hd, 16 keys] P^T[16 keys, 8 rows]
 //
@@ -8,8 +8,8 @@
 // of the scores is key 4 (i / 2) + i % 2, row 8 + i two behind it.  A block of 16 values of V is one product's 16 rows, so its scales are one number to each key.
 //
 // Half the bytes of f16 pages leave the instructions as the bound: a code costs one and a half of them on its way to f16 (byte behind the exponent of 1024, minus
-// 1152, times the scale: all exact).  So a warp works on 32 keys at a time where the registers hold it: the checks of the running maximum, the ring and the additions of
-// sums come once for these, and two chains of products run beside each other.
+// 1152, times the scale: all exact).  So there are sixteen warps where the registers hold that, in two groups that take tiles of 128 keys in turn; and one warp of a
+// group asks for a whole tile, each in its turn (by every warp for itself the copies were a third of all instructions, and a warp more would take registers from all).
 #include "attn.cuh"
 #include "kv_q8.cuh"
 
@@ -18,6 +18,12 @@ namespace {
 
 constexpr int ROWS_EXTRA = 3;  // tiles' time that an item's beginning and end take
 
+__device__ __forceinline__ void mma16816_zero(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {  // (no moves of zeros ahead of it)
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+
 // Two 16 x 16 matrices of bytes transposed: r[0], r[1] are rows lane / 4 and 8 more of the first, columns 4 (lane % 4) .. + 3.
 __device__ __forceinline__ void ldsm2_t8(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m16n16.x2.trans.shared.b8 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
@@ -25,19 +31,19 @@ __device__ __forceinline__ void ldsm2_t8(uint32_t (&r)[4], uint32_t addr) {
 
 template <int HD, int NT>
 struct Q8Shape {
-  static constexpr int WARPS = 8, THREADS = WARPS * 32, RB = 8 * NT;
-  static constexpr int HALVES = HD <= 128 ? 2 : 1, KEYS = 16 * HALVES;  // keys of a slice
-  static constexpr int LOG2_TILE = HALVES == 2 ? 8 : 7;
-  static constexpr int SIDE = KEYS * HD;                // bytes of a slice of K, or of V
-  static constexpr int UNIT = 2 * SIDE, SCALES = 2 * KEYS * HD / 16;
+  static constexpr int WARPS = HD <= 128 && NT == 1 ? 16 : 8, GROUPS = WARPS / 8;  // that do the products
+  static constexpr int THREADS = WARPS * 32, RB = 8 * NT;
+  static constexpr int LOG2_TILE = 7, KEYS = 1 << LOG2_TILE;
+  static constexpr int SIDE = KEYS * HD;                // bytes of a tile of K, or of V
+  static constexpr int STAGE = 2 * SIDE, SCALES = 2 * KEYS * HD / 16;
   static constexpr int PITCH = HD + 4;                  // words: the fragments' columns fall on different banks
-  static constexpr int SLOTS = HD == 64 ? WARPS : WARPS / 2;  // half of the warps add theirs to the others' first
+  static constexpr int SLOTS = HD == 64 && WARPS == 8 ? WARPS : WARPS / 2;  // half of the warps add theirs to the others' first
   static constexpr int MERGE = SLOTS * RB * PITCH * 4, STATS = 2 * WARPS * RB * 4;
-  static constexpr int FIT = (232448 - 1024 - 1024 - MERGE - STATS) / (WARPS * (UNIT + SCALES));
-  static constexpr int UNITS = FIT > 4 ? 4 : FIT;
-  static constexpr int SMEM = 1024 + WARPS * UNITS * (UNIT + SCALES) + MERGE + STATS + WARPS * UNITS * 8;
-  static_assert(UNITS >= 2, "one to work on, one on its way");
-  static_assert(WARPS * UNITS * UNIT >= 16 * ATTN_MAX_SEQ + 4, "what is known of the sequences fits where the keys go later");
+  // Twice the groups: what asks for a group's tile n + STAGES - GROUPS then has waited for the tile that the group asked for ahead of it, tile n itself.
+  static constexpr int STAGES = 2 * GROUPS;
+  static constexpr int SMEM = 1024 + STAGES * (STAGE + SCALES) + MERGE + STATS;
+  static_assert(SMEM + 2048 <= 232448, "more shared memory than a CTA has");
+  static_assert(SMEM - 1024 >= 16 * ATTN_MAX_SEQ + 4, "what is known of the sequences fits where keys and sums go later");
 };
 
 // Columns of rows of the item, the part of it that lies here, where 16 values of V that a row sees are not numbers, become NaN.  All of the warp's lanes take
@@ -67,111 +73,111 @@ static __device__ __noinline__ void attn_odd_blocks(const AttnParams& p, int s, 
   }
 }
 
+// Where a group's copies are in the CTA's line.
+template <class Cursor>
+struct AskState {
+  Cursor c;
+  int t;  // the tile of its item to ask for next
+};
+
 template <int HD, int NT>
 __global__ void __launch_bounds__(Q8Shape<HD, NT>::THREADS, 1)
-    k_attn_rows_q8(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ AttnParams p, const int box) {
+    k_attn_rows_q8(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ AttnParams p, const int granule) {
   using Sh = Q8Shape<HD, NT>;
-  constexpr int WARPS = Sh::WARPS, THREADS = Sh::THREADS, RB = Sh::RB, UNITS = Sh::UNITS, UNIT = Sh::UNIT, SIDE = Sh::SIDE, PITCH = Sh::PITCH, SLOTS = Sh::SLOTS;
-  constexpr int SLABS = HD / 64, KST = HD / 16, HALVES = Sh::HALVES, KEYS = Sh::KEYS, SLAB = KEYS * 64;
-  constexpr int AHEAD = 4;  // sums under way, and a word of scales
+  constexpr int WARPS = Sh::WARPS, GROUPS = Sh::GROUPS, THREADS = Sh::THREADS, RB = Sh::RB, STAGES = Sh::STAGES, STAGE = Sh::STAGE, SIDE = Sh::SIDE, PITCH = Sh::PITCH, SLOTS = Sh::SLOTS;
+  constexpr int SLABS = HD / 64, KST = HD / 16, SLAB = Sh::KEYS * 64;
+  constexpr int AHEAD = WARPS == 16 ? 2 : 4;  // sums under way
   static_assert(NT * KST * 512 <= Sh::MERGE, "q's pieces lie where the sums go");
+  using Cursor = AttnCursor<Sh::LOG2_TILE, ROWS_EXTRA>;
   extern __shared__ unsigned char smem_raw[];
+  __shared__ uint64_t full[STAGES], empty[STAGES];
   __shared__ long long s_scan[WARPS];
   __shared__ AttnStart s_start;
+  __shared__ Cursor s_cur;  // the item that is worked on
+  __shared__ AskState<Cursor> s_ask[GROUPS];
   __shared__ int s_last;
   __shared__ float s_weight[RB], s_factor[RB];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  unsigned char* ring_all = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  unsigned char *ring = ring_all + warp * UNITS * UNIT, *scales = ring_all + WARPS * UNITS * UNIT + warp * UNITS * Sh::SCALES;
-  float* s_o = reinterpret_cast<float*>(ring_all + WARPS * UNITS * (UNIT + Sh::SCALES));
+  unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  unsigned char* scales = ring + STAGES * STAGE;
+  float* s_o = reinterpret_cast<float*>(scales + STAGES * Sh::SCALES);
   uint4* s_q = reinterpret_cast<uint4*>(s_o);  // [NT][KST][32]
   float* s_m = s_o + SLOTS * RB * PITCH;
   float* s_l = s_m + WARPS * RB;
-  uint64_t* full = reinterpret_cast<uint64_t*>(s_l + WARPS * RB) + warp * UNITS;
 
   pdl_trigger();  // the next kernel may take the SMs that this one leaves free, and do what needs no input of its
-  if (lane == 0)
-    for (int i = 0; i < UNITS; ++i) mbar_init(full + i, 1);
+  if (tid == 0)
+    for (int i = 0; i < STAGES; ++i) mbar_init(full + i, 1), mbar_init(empty + i, 8);
   mbar_fence_init();
   pdl_wait();
-  attn_plan<THREADS, Sh::LOG2_TILE, ROWS_EXTRA, 0>(p, reinterpret_cast<int*>(ring_all), s_scan, &s_start);
-  const AttnStart st = s_start;
-  if (st.until == st.before) return;
+  attn_plan<THREADS, Sh::LOG2_TILE, ROWS_EXTRA, 0>(p, reinterpret_cast<int*>(ring), s_scan, &s_start);
+  if (s_start.until == s_start.before) return;
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the plan's words lay where the copies go
+  if (tid == 0) {
+    s_cur.start(p, s_start);
+    for (int g = 0; g < GROUPS; ++g) s_ask[g].c = s_cur, s_ask[g].t = s_cur.first(s_start) + g;
+  }
   __syncthreads();
 
   const int nb = p.hd / 16;  // scales of a key
-  // ---- what the warp asks for: its slices of the CTA's tiles, one after the other, as many as its ring holds
-  AttnCursor<Sh::LOG2_TILE, ROWS_EXTRA> ahead;
-  ahead.start(p, st);
-  AttnCursor<Sh::LOG2_TILE, ROWS_EXTRA> cur = ahead;  // what it works on
-  int at = ahead.first(st);  // tile of its item to look at next
-  int a_key = -1;            // first key of the slice to ask for (-1: none left),
-  int a_page[HALVES];        // its pages' numbers (-1: none of these 16 keys is seen)
-  uint32_t asked = 0;
-  auto find = [&]() {        // the next tile of which this warp has keys
-#pragma unroll 1
-    while (ahead.ub < st.u1) {
-      if (at >= ahead.end(st)) {
-        ahead.next(p);
-        at = 0;
-        continue;
-      }
-      const int ks = ((ahead.blk.tile0 + at) << Sh::LOG2_TILE) + warp * KEYS;
-      if (ks < ahead.blk.hi && ks + KEYS > ahead.blk.lo) {
-        a_key = ks;
-#pragma unroll
-        for (int h = 0; h < HALVES; ++h) {
-          // (a page that holds the whole slice is asked for once)
-          const int key = box == KEYS ? max(ks, ahead.blk.lo & ~15) : ks + 16 * h;
-          a_page[h] = (h == 0 || box < KEYS) && key < ahead.blk.hi && key + 16 > ahead.blk.lo ? attn_page_entry(p, ahead.s, attn_page_of(p, key)) : -1;
-          if (a_page[h] < 0 && (h == 0 || box < KEYS) && key < ahead.blk.hi && key + 16 > ahead.blk.lo) a_page[h] = 0x7FFFFFFF;  // (not a page: reported below)
-        }
-        return;
-      }
-      ++at;
-    }
-    a_key = -1;
-  };
-  auto ask_next = [&]() {
-    if (a_key < 0) return;
+  const int N = (int)(s_start.until - s_start.before);  // tiles of this CTA
+  // Tile n, by a warp: as many keys at once as lie side by side in every page, by lane.  (A group's state is in shared memory: in registers all warps would pay for
+  // it.  What asks for the group's next tile has waited for this one's copies, and with them for what was written ahead of these.)
+  auto ask = [&](int n) {
+    AskState<Cursor>& a = s_ask[n & (GROUPS - 1)];
     if (lane == 0) {
-      const int to = asked % UNITS;
-      unsigned char *dst = ring + to * UNIT, *sc = scales + to * Sh::SCALES;
-      int parts = 0;
-#pragma unroll
-      for (int h = 0; h < HALVES; ++h) parts += a_page[h] >= 0;
-      mbar_arrive_expect_tx(full + to, parts * box * (2 * HD + 2 * nb));
-#pragma unroll
-      for (int h = 0; h < HALVES; ++h) {
-        if (a_page[h] < 0) continue;
-        const int key = a_key + 16 * h, page = attn_page_of(p, key), y = key - page * p.page_size, w = attn_page_checked(p, a_page[h]);
-        const size_t first = ((size_t)w * p.page_pitch + (size_t)ahead.head * p.head_pitch + (size_t)y * p.row_pitch) / 16;
-        bulk_g2s(sc + 16 * h * nb, p.ks + first, box * nb, full + to);
-        bulk_g2s(sc + Sh::SCALES / 2 + 16 * h * nb, p.vs + first, box * nb, full + to);
-#pragma unroll
-        for (int s = 0; s < SLABS; ++s) {
-          tma_load_4d(dst + s * SLAB + h * 1024, &kmap, 64 * s, y, ahead.head, w, full + to);
-          tma_load_4d(dst + SIDE + s * SLAB + h * 1024, &vmap, 64 * s, y, ahead.head, w, full + to);
-        }
+      int t = a.t;
+      while (t >= a.c.end(s_start)) {
+        t -= a.c.end(s_start);
+        a.c.next(p);
       }
+      a.t = t;
     }
-    ++asked;
-    ++at;
-    find();
+    __syncwarp();
+    const int key = ((a.c.blk.tile0 + a.t) << Sh::LOG2_TILE) + lane * granule, head = a.c.head, stage = n % STAGES;
+    const bool seen = lane * granule < Sh::KEYS && key < a.c.blk.hi && key + granule > a.c.blk.lo;
+    int y = 0, w = 0;
+    if (seen) {
+      const int page = attn_page_of(p, key);
+      w = attn_page(p, a.c.s, page);
+      y = key - page * p.page_size;
+    }
+    const int count = __popc(__ballot_sync(0xFFFFFFFFu, seen));
+    if (n >= STAGES && !wait_all(empty + stage, n / STAGES - 1)) {
+      if (lane == 0) atomicExch(&p.status->timeout, 10);
+      return;
+    }
+    if (lane == 0) {
+      a.t += GROUPS;
+      mbar_arrive_expect_tx(full + stage, (uint32_t)(count * granule * (2 * HD + 2 * nb)));
+    }
+    __syncwarp();
+    if (seen) {
+      const size_t first = ((size_t)w * p.page_pitch + (size_t)head * p.head_pitch + (size_t)y * p.row_pitch) / 16;
+      unsigned char *dst = ring + stage * STAGE + lane * granule * 64, *sc = scales + stage * Sh::SCALES + lane * granule * nb;
+#pragma unroll
+      for (int s = 0; s < SLABS; ++s) tma_load_4d(dst + s * SLAB, &kmap, 64 * s, y, head, w, full + stage);
+      bulk_g2s(sc, p.ks + first, granule * nb, full + stage);
+#pragma unroll
+      for (int s = 0; s < SLABS; ++s) tma_load_4d(dst + SIDE + s * SLAB, &vmap, 64 * s, y, head, w, full + stage);
+      bulk_g2s(sc + Sh::SCALES / 2, p.vs + first, granule * nb, full + stage);
+    }
+    __syncwarp();
   };
-  find();
+  if (warp == 0)
 #pragma unroll 1
-  for (int i = 0; i < UNITS; ++i) ask_next();
+    for (int n = 0; n < STAGES && n < N; ++n) ask(n);
 
-  uint32_t used = 0;
   bool alive = true;
   const int c0 = 2 * (lane & 3);  // this thread's columns (rows of the item): c0, c0 + 1 of every eight
-  const int key1 = 4 * (lane >> 3) + ((lane >> 2) & 1);  // and its keys of every 16: this one, and two behind it
-  long long left = st.until - st.before;  // tiles
+  const int key1 = 4 * (lane >> 3) + ((lane >> 2) & 1);  // and its keys of the warp's 16: this one, and two behind it
+  const int key0 = 16 * (warp & 7), group = warp >> 3;   // the warp's keys of a tile, and its tiles: those of this parity
+  int done = 0;                                          // tiles of the items ahead
 #pragma unroll 1
-  for (;; cur.next(p)) {
+  while (true) {
+    const Cursor& cur = s_cur;
     const AttnBlock& blk = cur.blk;
+    const AttnStart& st = s_start;
     const int first_tile = cur.first(st), end_tile = cur.end(st), n_rows = blk.nt * p.g;
 
     // ---- q: B fragments of q^T, rows scaled by a power of two, as two f16 pieces, put down by one warp per eight rows where the sums go
@@ -227,31 +233,30 @@ __global__ void __launch_bounds__(Q8Shape<HD, NT>::THREADS, 1)
 
     bool odd = false;  // values that are no numbers were left out
 #pragma unroll 1
-    for (int t = first_tile; t < end_tile; ++t) {
-      const int ks = ((blk.tile0 + t) << Sh::LOG2_TILE) + warp * KEYS;
-      if (ks >= blk.hi || ks + KEYS <= blk.lo) continue;
+    for (int t = first_tile + ((done ^ group) & (GROUPS - 1)); t < end_tile; t += GROUPS) {
+      const int n = done + t - first_tile, stage = n % STAGES, ks = ((blk.tile0 + t) << Sh::LOG2_TILE) + key0;
       if (alive) {
-        alive = wait_all(full + used % UNITS, used / UNITS);
+        alive = wait_all(full + stage, n / STAGES);
         if (!alive && lane == 0) atomicExch(&p.status->timeout, 10);
       }
-      if (!alive) continue;
-      const unsigned char *kb = ring + (used % UNITS) * UNIT, *sc = scales + (used % UNITS) * Sh::SCALES;
+      // what the group's last tile has left, for the next one but
+      if (alive && (warp & 7) == ((n / GROUPS) & 7) && n >= GROUPS && n - GROUPS + STAGES < N) ask(n - GROUPS + STAGES);
+      if (!alive || ks >= blk.hi || ks + 16 <= blk.lo) {
+        if (lane == 0) mbar_arrive(empty + stage);
+        continue;
+      }
+      const unsigned char *kb = ring + stage * STAGE + key0 * 64, *sc = scales + stage * Sh::SCALES + key0 * nb;
       // ---- scores: pieces and even and odd steps apart
-      float s[HALVES][NT][4];
-#pragma unroll
-      for (int h = 0; h < HALVES; ++h) {
+      float s[NT][4];
+      {
         float part[NT][3][4];
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) s[h][n][i] = part[n][0][i] = part[n][1][i] = part[n][2][i] = 0.f;
 #pragma unroll
         for (int b = 0; b < SLABS; ++b) {
           uint4 kw[2];     // this lane's 16 values of both keys
           uint32_t kd[2];  // and their scales (behind the head's end q is 0 and the codes' values are finite)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            const int key = 16 * h + key1 + 2 * j, blk16 = 4 * b + (lane & 3);
+            const int key = key1 + 2 * j, blk16 = 4 * b + (lane & 3);
             kw[j] = *reinterpret_cast<const uint4*>(kb + b * SLAB + key * 64 + (((lane & 3) ^ ((key >> 1) & 3)) << 4));
             kd[j] = q8_scale_pair(blk16 < nb ? sc[key * nb + blk16] : 0u);
           }
@@ -263,35 +268,36 @@ __global__ void __launch_bounds__(Q8Shape<HD, NT>::THREADS, 1)
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
               const uint4 w = s_q[(n * KST + 4 * b + k) * 32 + lane];
-              mma16816(k & 1 ? part[n][0] : s[h][n], a, w.x, w.y);
-              mma16816(k & 1 ? part[n][2] : part[n][1], a, w.z, w.w);
+              if (b == 0 && k < 2) {
+                mma16816_zero(k & 1 ? part[n][0] : s[n], a, w.x, w.y);
+                mma16816_zero(k & 1 ? part[n][2] : part[n][1], a, w.z, w.w);
+              } else {
+                mma16816(k & 1 ? part[n][0] : s[n], a, w.x, w.y);
+                mma16816(k & 1 ? part[n][2] : part[n][1], a, w.z, w.w);
+              }
             }
           }
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[h][n][i] = (s[h][n][i] + part[n][0][i]) + (part[n][1][i] + part[n][2][i]);
+          for (int i = 0; i < 4; ++i) s[n][i] = (s[n][i] + part[n][0][i]) + (part[n][1][i] + part[n][2][i]);
       }
-      const bool masked = ks + KEYS > full_hi || ks < full_lo;
+      const bool masked = ks + 16 > full_hi || ks < full_lo;
       bool grows = false, falls = false;
       float top[NT][2];
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-#pragma unroll
-          for (int h = 0; h < HALVES; ++h) {
-            s[h][n][j] *= f[n][j];
-            s[h][n][2 + j] *= f[n][j];
-            if (masked) {
-              const int to = lim[n][j], from = attn_first_key(to, p.window), key = ks + 16 * h + key1;
-              if (key > to || key < from) s[h][n][j] = -CUDART_INF_F;
-              if (key + 2 > to || key + 2 < from) s[h][n][2 + j] = -CUDART_INF_F;
-            }
+          s[n][j] *= f[n][j];
+          s[n][2 + j] *= f[n][j];
+          if (masked) {
+            const int to = lim[n][j], from = attn_first_key(to, p.window), key = ks + key1;
+            if (key > to || key < from) s[n][j] = -CUDART_INF_F;
+            if (key + 2 > to || key + 2 < from) s[n][2 + j] = -CUDART_INF_F;
           }
-          top[n][j] = max_nan(s[0][n][j], s[0][n][2 + j]);
-          if (HALVES == 2) top[n][j] = max_nan(top[n][j], s[HALVES - 1][n][j], s[HALVES - 1][n][2 + j]);
+          top[n][j] = max_nan(s[n][j], s[n][2 + j]);
           grows |= !(top[n][j] <= m[n][j] + ATTN_SLACK);  // (or there is none)
         }
       if ((t & 3) == 0) {
@@ -310,9 +316,7 @@ __global__ void __launch_bounds__(Q8Shape<HD, NT>::THREADS, 1)
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            float mx = -CUDART_INF_F, lx = l[n][j];
-#pragma unroll
-            for (int h = 0; h < HALVES; ++h) mx = fmaxf(mx, fmaxf(s[h][n][j], s[h][n][2 + j]));  // (a NaN leaves the reference where it is)
+            float mx = fmaxf(s[n][j], s[n][2 + j]), lx = l[n][j];  // (a NaN leaves the reference where it is)
 #pragma unroll
             for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, x));
             if (falls) {
@@ -331,34 +335,31 @@ __global__ void __launch_bounds__(Q8Shape<HD, NT>::THREADS, 1)
           }
       }
       // ---- weights, transposed into B fragments
-      uint32_t ph[HALVES][NT][2], pl[HALVES][NT][2];
+      uint32_t ph[NT][2], pl[NT][2];
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int h = 0; h < HALVES; ++h) {
+      for (int n = 0; n < NT; ++n) {
           float e[4];
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             const float ref = m[n][j] == -CUDART_INF_F ? 0.f : m[n][j];
-            e[j] = exp2_approx((s[h][n][j] - ref) + ATTN_BIAS);  // (in this order: scores of any size)
-            e[2 + j] = exp2_approx((s[h][n][2 + j] - ref) + ATTN_BIAS);
+            e[j] = exp2_approx((s[n][j] - ref) + ATTN_BIAS);  // (in this order: scores of any size)
+            e[2 + j] = exp2_approx((s[n][2 + j] - ref) + ATTN_BIAS);
             l[n][j] += e[j] + e[2 + j];
           }
-          split2(e[0], e[1], ph[h][n][0], pl[h][n][0]);
-          split2(e[2], e[3], ph[h][n][1], pl[h][n][1]);
+          split2(e[0], e[1], ph[n][0], pl[n][0]);
+          split2(e[2], e[3], ph[n][1], pl[n][1]);
 #pragma unroll
-          for (int i = 0; i < 2; ++i) ph[h][n][i] = movm(ph[h][n][i]), pl[h][n][i] = movm(pl[h][n][i]);
+          for (int i = 0; i < 2; ++i) ph[n][i] = movm(ph[n][i]), pl[n][i] = movm(pl[n][i]);
         }
       // ---- sums, from zero for every slice and added here: the tensor cores truncate, and a running sum would lose 2^-23 of itself to every slice.
       // (0 x value is 0 whatever the codes; scales that are no numbers, and those of keys that no row sees, count as zeros.)
       const uint32_t vb = smem_u32(kb + SIDE);
 #pragma unroll
-      for (int k0 = 0; k0 < KST; k0 += AHEAD) {
-        float sum[AHEAD][NT][4];
-#pragma unroll
-        for (int h = 0; h < HALVES; ++h) {
-          uint32_t w[4], bad = 0;  // scales of the keys 4 c .. 4 c + 3 of these 16, a byte to each of the four blocks
-          const unsigned char* vd = sc + Sh::SCALES / 2 + (16 * h + 2 * c0) * nb + k0;
+      for (int k0 = 0; k0 < KST; k0 += 4) {
+        uint32_t ab[2][2];  // scales of blocks 0 and 1, and 2 and 3, of these four: of the lane's first two keys of every 16, and of the other two
+        {
+          uint32_t w[4], bad = 0;  // of the keys 4 c .. 4 c + 3, a byte to each of the four blocks
+          const unsigned char* vd = sc + Sh::SCALES / 2 + 2 * c0 * nb + k0;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             if ((nb & 3) == 0) {
@@ -370,7 +371,7 @@ __global__ void __launch_bounds__(Q8Shape<HD, NT>::THREADS, 1)
                 if (k0 + b < nb) w[i] |= (uint32_t)vd[i * nb + b] << (8 * b);
             }
             if (masked) {
-              const int key = ks + 16 * h + 2 * c0 + i;
+              const int key = ks + 2 * c0 + i;
               if (key >= blk.hi || key < blk.lo) w[i] = 0;
             }
             bad |= w[i] & (w[i] << 1);
@@ -380,39 +381,40 @@ __global__ void __launch_bounds__(Q8Shape<HD, NT>::THREADS, 1)
 #pragma unroll
             for (int i = 0; i < 4; ++i) w[i] &= ~(((w[i] & (w[i] << 1) & 0x80808080u) >> 7) * 0xFFu);
           }
-          uint32_t ab[2][2];  // blocks 0 and 1, and 2 and 3: of the first two keys, of the other two
           ab[0][0] = __byte_perm(w[0], w[1], 0x5140), ab[1][0] = __byte_perm(w[0], w[1], 0x7362);
           ab[0][1] = __byte_perm(w[2], w[3], 0x5140), ab[1][1] = __byte_perm(w[2], w[3], 0x7362);
-#pragma unroll
-          for (int k = 0; k < AHEAD; k += 2) {
-            uint32_t r[4];
-            const int c = k + (lane >> 4), kk = 16 * h + (lane & 15);
-            ldsm2_t8(r, vb + (k0 >> 2) * SLAB + kk * 64 + ((c ^ ((kk >> 1) & 3)) << 4));
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const uint32_t d01 = __byte_perm(ab[k >> 1][0], 0, i ? 0x3424 : 0x1404) >> 1, d23 = __byte_perm(ab[k >> 1][1], 0, i ? 0x3424 : 0x1404) >> 1;
-              const uint32_t a[4] = {q8_lo(r[2 * i], d01), q8_lo(r[2 * i + 1], d01), q8_hi(r[2 * i], d23), q8_hi(r[2 * i + 1], d23)};
-#pragma unroll
-              for (int n = 0; n < NT; ++n) {
-                float(&to)[4] = sum[k + i][n];
-                if (h == 0) to[0] = to[1] = to[2] = to[3] = 0.f;
-                mma16816(to, a, pl[h][n][0], pl[h][n][1]);
-                mma16816(to, a, ph[h][n][0], ph[h][n][1]);
-              }
-            }
-          }
         }
 #pragma unroll
-        for (int k = 0; k < AHEAD; ++k)
+        for (int k1 = 0; k1 < 4; k1 += AHEAD) {
+          float sum[AHEAD][NT][4];
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
+            for (int k = 0; k < AHEAD; k += 2) {
+              uint32_t r[4];
+              const int c = k1 + k + (lane >> 4), kk = lane & 15;
+              ldsm2_t8(r, vb + (k0 >> 2) * SLAB + kk * 64 + ((c ^ ((kk >> 1) & 3)) << 4));
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[k0 + k][n][i] += sum[k][n][i];
+              for (int i = 0; i < 2; ++i) {
+                const uint32_t *two = ab[(k1 + k) >> 1], d01 = __byte_perm(two[0], 0, i ? 0x3424 : 0x1404) >> 1, d23 = __byte_perm(two[1], 0, i ? 0x3424 : 0x1404) >> 1;
+                const uint32_t a[4] = {q8_lo(r[2 * i], d01), q8_lo(r[2 * i + 1], d01), q8_hi(r[2 * i], d23), q8_hi(r[2 * i + 1], d23)};
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                  mma16816_zero(sum[k + i][n], a, pl[n][0], pl[n][1]);
+                  mma16816(sum[k + i][n], a, ph[n][0], ph[n][1]);
+                }
+              }
+            }
+#pragma unroll
+          for (int k = 0; k < AHEAD; ++k)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) o[k0 + k1 + k][n][i] += sum[k][n][i];
+        }
       }
       __syncwarp();
-      ++used;
-      ask_next();
+      if (lane == 0) mbar_arrive(empty + stage);
     }
+    done += end_tile - first_tile;
 
     // ---- the warps' parts of the item
 #pragma unroll
@@ -426,7 +428,7 @@ __global__ void __launch_bounds__(Q8Shape<HD, NT>::THREADS, 1)
 #pragma unroll
       for (int j = 0; j < 2; ++j)
         if (m[n][j] == -CUDART_INF_F && l[n][j] != 0.f) m[n][j] = 0.f;  // nothing but NaN: a part that counts, not one without keys
-    __syncthreads();  // the last item's parts have been read, and q's pieces
+    __syncthreads();  // q's pieces have been read
     // one half of the warps puts its sums down, the other adds its own to them, each brought to the higher maximum
     if (lane < 4) {
 #pragma unroll
@@ -509,12 +511,12 @@ __global__ void __launch_bounds__(Q8Shape<HD, NT>::THREADS, 1)
       for (int r = warp; r < n_rows; r += WARPS)
         attn_join_row<HD>(p, share, RB, r, p.out + attn_row_offset(p, cur.seq.q0 + blk.t0, cur.head, r, p.out_stride));
     }
-    left -= end_tile - first_tile;
-    if (left <= 0) break;
+    if (done >= N) break;
+    __syncthreads();  // all have done with the item
+    if (tid == 0) s_cur.next(p);
+    __syncthreads();
   }
-  // a warp that gave up has copies in flight: they land before its shared memory is somebody else's
-  if (!alive)
-    for (; used < asked; ++used) attn_wait(full + used % UNITS, used / UNITS);
+  if (!alive) attn_let_land();  // copies are in flight: they land before this shared memory is somebody else's
 }
 
 // Codes of `box` keys of a head, 64 values wide.
@@ -531,12 +533,13 @@ bool attn_codes_map(CUtensorMap* tm, const uint8_t* base, const AttnParams& p, i
 template <int HD, int NT>
 int32_t run_rows_q8(infr_cuda_ctx* ctx, const AttnParams& p) {
   using Sh = Q8Shape<HD, NT>;
-  const int box = p.page_size % Sh::KEYS == 0 ? Sh::KEYS : 16;
+  int granule = Sh::KEYS;
+  while (p.page_size % granule) granule >>= 1;
   CUtensorMap km, vm;
-  if (!attn_codes_map(&km, p.kq, p, box) || !attn_codes_map(&vm, p.vq, p, box)) return fail(ctx, INFR_CUDA_ERR_CUDA, "attention: cuTensorMapEncodeTiled failed");
+  if (!attn_codes_map(&km, p.kq, p, granule) || !attn_codes_map(&vm, p.vq, p, granule)) return fail(ctx, INFR_CUDA_ERR_CUDA, "attention: cuTensorMapEncodeTiled failed");
   cudaError_t e = ensure_smem(reinterpret_cast<const void*>(&k_attn_rows_q8<HD, NT>), Sh::SMEM);
   if (e == cudaSuccess)
-    e = launch_ex(k_attn_rows_q8<HD, NT>, dim3(ctx->sm_count < ATTN_MAX_CTAS ? ctx->sm_count : ATTN_MAX_CTAS), dim3(Sh::THREADS), Sh::SMEM, ctx->stream, true, km, vm, p, box);
+    e = launch_ex(k_attn_rows_q8<HD, NT>, dim3(ctx->sm_count < ATTN_MAX_CTAS ? ctx->sm_count : ATTN_MAX_CTAS), dim3(Sh::THREADS), Sh::SMEM, ctx->stream, true, km, vm, p, granule);
   if (e != cudaSuccess) return check_cuda(ctx, e, "k_attn_rows_q8 launch");
   ctx->launches += 1;
   return check_cuda(ctx, cudaGetLastError(), "k_attn_rows_q8 launch");
