@@ -80,7 +80,8 @@ struct AskState {
   int t;  // the tile of its item to ask for next
 };
 
-template <int HD, int NT>
+// WHOLE: heads of HD values, not fewer: the places of scales are known then (873 -> 760 instructions to 16 keys of heads of 128).
+template <int HD, int NT, bool WHOLE>
 __global__ void __launch_bounds__(Q8Shape<HD, NT>::THREADS, 1)
     k_attn_rows_q8(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ AttnParams p, const int granule) {
   using Sh = Q8Shape<HD, NT>;
@@ -119,7 +120,7 @@ __global__ void __launch_bounds__(Q8Shape<HD, NT>::THREADS, 1)
   }
   __syncthreads();
 
-  const int nb = p.hd / 16;  // scales of a key
+  const int nb = WHOLE ? HD / 16 : p.hd / 16;  // scales of a key
   const int N = (int)(s_start.until - s_start.before);  // tiles of this CTA
   // Tile n, by a warp: as many keys at once as lie side by side in every page, by lane.  (A group's state is in shared memory: in registers all warps would pay for
   // it.  What asks for the group's next tile has waited for this one's copies, and with them for what was written ahead of these.)
@@ -258,7 +259,7 @@ __global__ void __launch_bounds__(Q8Shape<HD, NT>::THREADS, 1)
           for (int j = 0; j < 2; ++j) {
             const int key = key1 + 2 * j, blk16 = 4 * b + (lane & 3);
             kw[j] = *reinterpret_cast<const uint4*>(kb + b * SLAB + key * 64 + (((lane & 3) ^ ((key >> 1) & 3)) << 4));
-            kd[j] = q8_scale_pair(blk16 < nb ? sc[key * nb + blk16] : 0u);
+            kd[j] = q8_scale_pair(WHOLE || blk16 < nb ? sc[key * nb + blk16] : 0u);
           }
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
@@ -362,8 +363,8 @@ __global__ void __launch_bounds__(Q8Shape<HD, NT>::THREADS, 1)
           const unsigned char* vd = sc + Sh::SCALES / 2 + 2 * c0 * nb + k0;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            if ((nb & 3) == 0) {
-              w[i] = k0 < nb ? *reinterpret_cast<const uint32_t*>(vd + i * nb) : 0u;
+            if constexpr (WHOLE) {
+              w[i] = *reinterpret_cast<const uint32_t*>(vd + i * nb);
             } else {  // (one byte after the other: those behind the head's end are the next key's)
               w[i] = 0;
 #pragma unroll
@@ -530,23 +531,26 @@ bool attn_codes_map(CUtensorMap* tm, const uint8_t* base, const AttnParams& p, i
              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int HD, int NT>
+template <int HD, int NT, bool WHOLE>
 int32_t run_rows_q8(infr_cuda_ctx* ctx, const AttnParams& p) {
   using Sh = Q8Shape<HD, NT>;
   int granule = Sh::KEYS;
   while (p.page_size % granule) granule >>= 1;
   CUtensorMap km, vm;
   if (!attn_codes_map(&km, p.kq, p, granule) || !attn_codes_map(&vm, p.vq, p, granule)) return fail(ctx, INFR_CUDA_ERR_CUDA, "attention: cuTensorMapEncodeTiled failed");
-  cudaError_t e = ensure_smem(reinterpret_cast<const void*>(&k_attn_rows_q8<HD, NT>), Sh::SMEM);
+  cudaError_t e = ensure_smem(reinterpret_cast<const void*>(&k_attn_rows_q8<HD, NT, WHOLE>), Sh::SMEM);
   if (e == cudaSuccess)
-    e = launch_ex(k_attn_rows_q8<HD, NT>, dim3(ctx->sm_count < ATTN_MAX_CTAS ? ctx->sm_count : ATTN_MAX_CTAS), dim3(Sh::THREADS), Sh::SMEM, ctx->stream, true, km, vm, p, granule);
+    e = launch_ex(k_attn_rows_q8<HD, NT, WHOLE>, dim3(ctx->sm_count < ATTN_MAX_CTAS ? ctx->sm_count : ATTN_MAX_CTAS), dim3(Sh::THREADS), Sh::SMEM, ctx->stream, true, km, vm, p, granule);
   if (e != cudaSuccess) return check_cuda(ctx, e, "k_attn_rows_q8 launch");
   ctx->launches += 1;
   return check_cuda(ctx, cudaGetLastError(), "k_attn_rows_q8 launch");
 }
 
 template <int HD>
-int32_t run_rows_q8_of(infr_cuda_ctx* ctx, const AttnParams& p, int nt) { return nt == 1 ? run_rows_q8<HD, 1>(ctx, p) : run_rows_q8<HD, 2>(ctx, p); }
+int32_t run_rows_q8_of(infr_cuda_ctx* ctx, const AttnParams& p, int nt) {
+  if (p.hd == HD) return nt == 1 ? run_rows_q8<HD, 1, true>(ctx, p) : run_rows_q8<HD, 2, true>(ctx, p);
+  return nt == 1 ? run_rows_q8<HD, 1, false>(ctx, p) : run_rows_q8<HD, 2, false>(ctx, p);
+}
 
 }  // namespace
 
