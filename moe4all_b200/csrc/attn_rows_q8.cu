@@ -24,6 +24,23 @@ __device__ __forceinline__ void mma16816_zero(float (&d)[4], const uint32_t (&a)
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 
+// (Through pointers that come from the aligned beginning the compiler reads generic addresses: 26 loads of 16 keys, and 64-bit sums for them.)
+__device__ __forceinline__ uint4 lds128(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t at) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t lds8(uint32_t at) {
+  uint32_t v;
+  asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+  return v;
+}
+
 // Two 16 x 16 matrices of bytes transposed: r[0], r[1] are rows lane / 4 and 8 more of the first, columns 4 (lane % 4) .. + 3.
 __device__ __forceinline__ void ldsm2_t8(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m16n16.x2.trans.shared.b8 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
@@ -173,6 +190,7 @@ __global__ void __launch_bounds__(Q8Shape<HD, NT>::THREADS, 1)
   const int c0 = 2 * (lane & 3);  // this thread's columns (rows of the item): c0, c0 + 1 of every eight
   const int key1 = 4 * (lane >> 3) + ((lane >> 2) & 1);  // and its keys of the warp's 16: this one, and two behind it
   const int key0 = 16 * (warp & 7), group = warp >> 3;   // the warp's keys of a tile, and its tiles: those of this parity
+  const uint32_t ring_at = smem_u32(ring), scales_at = smem_u32(scales), q_at = smem_u32(s_q) + 16 * lane;
   int done = 0;                                          // tiles of the items ahead
 #pragma unroll 1
   while (true) {
@@ -246,7 +264,28 @@ __global__ void __launch_bounds__(Q8Shape<HD, NT>::THREADS, 1)
         if (lane == 0) mbar_arrive(empty + stage);
         continue;
       }
-      const unsigned char *kb = ring + stage * STAGE + key0 * 64, *sc = scales + stage * Sh::SCALES + key0 * nb;
+      const uint32_t kb = ring_at + stage * STAGE + key0 * 64, sc = scales_at + stage * Sh::SCALES + key0 * nb;
+      const bool masked = ks + 16 > full_hi || ks < full_lo;
+      // scales that are no numbers: in K's place one that is NaN in f16 too, in V's zeros that wait for the item's end.  Zeros too for keys that no row sees: 0 x value is 0
+      // whatever the codes.  (Seldom: looked for a word to a lane, and written where they lie.)
+      uint32_t bad = 0;
+      for (int e = lane; e < 4 * nb; e += 32) {
+        const uint32_t a = lds32(sc + 4 * e), b = lds32(sc + Sh::SCALES / 2 + 4 * e);
+        bad |= (a & (a << 1)) | (b & (b << 1));
+      }
+      if (__any_sync(0xFFFFFFFFu, (bad & 0x80808080u) != 0) || masked) {
+        unsigned char* w = scales + stage * Sh::SCALES + key0 * nb;
+#pragma unroll 1
+        for (int e = lane; e < 16 * nb; e += 32) {
+          const int key = ks + e / nb;
+          const bool seen = key >= blk.lo && key < blk.hi, k_odd = w[e] >= Q8_ODD, v_odd = w[Sh::SCALES / 2 + e] >= Q8_ODD;
+          if (k_odd) w[e] = 0xFF;
+          if (v_odd || !seen) w[Sh::SCALES / 2 + e] = 0;
+          odd |= v_odd && seen;
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // (ahead of the next copy to here)
+        __syncwarp();
+      }
       // ---- scores: pieces and even and odd steps apart
       float s[NT][4];
       {
@@ -258,8 +297,8 @@ __global__ void __launch_bounds__(Q8Shape<HD, NT>::THREADS, 1)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             const int key = key1 + 2 * j, blk16 = 4 * b + (lane & 3);
-            kw[j] = *reinterpret_cast<const uint4*>(kb + b * SLAB + key * 64 + (((lane & 3) ^ ((key >> 1) & 3)) << 4));
-            kd[j] = q8_scale_pair(WHOLE || blk16 < nb ? sc[key * nb + blk16] : 0u);
+            kw[j] = lds128(kb + b * SLAB + key * 64 + (((lane & 3) ^ ((key >> 1) & 3)) << 4));
+            kd[j] = WHOLE || blk16 < nb ? lds8(sc + key * nb + blk16) * 0x00800080u : 0u;  // (both halves of a pair: << 7)
           }
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
@@ -268,7 +307,7 @@ __global__ void __launch_bounds__(Q8Shape<HD, NT>::THREADS, 1)
             const uint32_t a[4] = {q8_lo(w0, kd[0]), q8_lo(w1, kd[1]), q8_hi(w0, kd[0]), q8_hi(w1, kd[1])};
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-              const uint4 w = s_q[(n * KST + 4 * b + k) * 32 + lane];
+              const uint4 w = lds128(q_at + (n * KST + 4 * b + k) * 512);
               if (b == 0 && k < 2) {
                 mma16816_zero(k & 1 ? part[n][0] : s[n], a, w.x, w.y);
                 mma16816_zero(k & 1 ? part[n][2] : part[n][1], a, w.z, w.w);
@@ -284,7 +323,6 @@ __global__ void __launch_bounds__(Q8Shape<HD, NT>::THREADS, 1)
 #pragma unroll
           for (int i = 0; i < 4; ++i) s[n][i] = (s[n][i] + part[n][0][i]) + (part[n][1][i] + part[n][2][i]);
       }
-      const bool masked = ks + 16 > full_hi || ks < full_lo;
       bool grows = false, falls = false;
       float top[NT][2];
 #pragma unroll
@@ -352,35 +390,24 @@ __global__ void __launch_bounds__(Q8Shape<HD, NT>::THREADS, 1)
 #pragma unroll
           for (int i = 0; i < 2; ++i) ph[n][i] = movm(ph[n][i]), pl[n][i] = movm(pl[n][i]);
         }
-      // ---- sums, from zero for every slice and added here: the tensor cores truncate, and a running sum would lose 2^-23 of itself to every slice.
-      // (0 x value is 0 whatever the codes; scales that are no numbers, and those of keys that no row sees, count as zeros.)
-      const uint32_t vb = smem_u32(kb + SIDE);
+      // ---- sums, from zero for every slice and added here: the tensor cores truncate, and a running sum would lose 2^-23 of itself to every slice
+      const uint32_t vb = kb + SIDE;
 #pragma unroll
       for (int k0 = 0; k0 < KST; k0 += 4) {
         uint32_t ab[2][2];  // scales of blocks 0 and 1, and 2 and 3, of these four: of the lane's first two keys of every 16, and of the other two
         {
-          uint32_t w[4], bad = 0;  // of the keys 4 c .. 4 c + 3, a byte to each of the four blocks
-          const unsigned char* vd = sc + Sh::SCALES / 2 + 2 * c0 * nb + k0;
+          uint32_t w[4];  // of the keys 4 c .. 4 c + 3, a byte to each of the four blocks
+          const uint32_t vd = sc + Sh::SCALES / 2 + 2 * c0 * nb + k0;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             if constexpr (WHOLE) {
-              w[i] = *reinterpret_cast<const uint32_t*>(vd + i * nb);
+              w[i] = lds32(vd + i * nb);
             } else {  // (one byte after the other: those behind the head's end are the next key's)
               w[i] = 0;
 #pragma unroll
               for (int b = 0; b < 4; ++b)
-                if (k0 + b < nb) w[i] |= (uint32_t)vd[i * nb + b] << (8 * b);
+                if (k0 + b < nb) w[i] |= lds8(vd + i * nb + b) << (8 * b);
             }
-            if (masked) {
-              const int key = ks + 2 * c0 + i;
-              if (key >= blk.hi || key < blk.lo) w[i] = 0;
-            }
-            bad |= w[i] & (w[i] << 1);
-          }
-          if (bad & 0x80808080u) {
-            odd = true;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] &= ~(((w[i] & (w[i] << 1) & 0x80808080u) >> 7) * 0xFFu);
           }
           ab[0][0] = __byte_perm(w[0], w[1], 0x5140), ab[1][0] = __byte_perm(w[0], w[1], 0x7362);
           ab[0][1] = __byte_perm(w[2], w[3], 0x5140), ab[1][1] = __byte_perm(w[2], w[3], 0x7362);
