@@ -10,6 +10,7 @@
 // Half the bytes of f16 pages leave the instructions as the bound: a code costs one and a half of them on its way to f16 (byte behind the exponent of 1024, minus
 // 1152, times the scale: all exact).  So there are sixteen warps where the registers hold that, in two groups that take tiles of 128 keys in turn; and one warp of a
 // group asks for a whole tile, each in its turn (by every warp for itself the copies were a third of all instructions, and a warp more would take registers from all).
+// Between items stands one barrier of the CTA, behind which all add up the warps' sums; an item's q and its other words are made ready two items ahead.
 #include "attn.cuh"
 #include "kv_q8.cuh"
 
@@ -54,11 +55,11 @@ struct Q8Shape {
   static constexpr int SIDE = KEYS * HD;                // bytes of a tile of K, or of V
   static constexpr int STAGE = 2 * SIDE, SCALES = 2 * KEYS * HD / 16;
   static constexpr int PITCH = HD + 4;                  // words: the fragments' columns fall on different banks
-  static constexpr int SLOTS = HD == 64 && WARPS == 8 ? WARPS : WARPS / 2;  // half of the warps add theirs to the others' first
-  static constexpr int MERGE = SLOTS * RB * PITCH * 4, STATS = 2 * WARPS * RB * 4;
+  static constexpr int SUMS = WARPS * RB * PITCH * 4, STATS = 2 * WARPS * RB * 4;
+  static constexpr int Q = NT * HD / 16 * 512;          // an item's q, as fragments
   // Twice the groups: what asks for a group's tile n + STAGES - GROUPS then has waited for the tile that the group asked for ahead of it, tile n itself.
   static constexpr int STAGES = 2 * GROUPS;
-  static constexpr int SMEM = 1024 + STAGES * (STAGE + SCALES) + MERGE + STATS;
+  static constexpr int SMEM = 1024 + STAGES * (STAGE + SCALES) + SUMS + STATS + 2 * Q;
   static_assert(SMEM + 2048 <= 232448, "more shared memory than a CTA has");
   static_assert(SMEM - 1024 >= 16 * ATTN_MAX_SEQ + 4, "what is known of the sequences fits where keys and sums go later");
 };
@@ -97,48 +98,103 @@ struct AskState {
   int t;  // the tile of its item to ask for next
 };
 
+// An item as the warps see it.
+struct Q8Item {
+  int tiles, key0;               // tiles of it here, and the first one's first key
+  int lo, hi, full_lo, full_hi;  // keys that some row sees; that every row sees
+  int row0, nt, n_rows, pos0;    // its first row of the call, tokens, rows (tokens x heads), position of its first token
+  int head, s;
+  int whole, first_cta, last_cta;  // no other CTA has tiles of it; the CTAs that have
+};
+
+// The item at the cursor, and its q as B fragments of q^T: rows scaled by a power of two, as two f16 pieces; of 64 values step k has 16 c + 4 k .. + 3 of lane c.
+// By a warp.
+template <int HD, int NT, class Cursor>
+static __device__ __noinline__ void q8_item(const AttnParams& p, const AttnStart& st, const Cursor& c, Q8Item* item, uint4* q, float* factor) {
+  const int lane = threadIdx.x & 31;
+  const int row0 = c.seq.q0 + c.blk.t0, n_rows = c.blk.nt * p.g, head = c.head;
+  if (lane == 0) {
+    const int first = c.first(st), end = c.end(st);
+    const AttnShare share = attn_share(c.ub, c.blk.ntile, st);
+    item->tiles = end - first, item->key0 = (c.blk.tile0 + first) << Q8Shape<HD, NT>::LOG2_TILE;
+    item->lo = c.blk.lo, item->hi = c.blk.hi, item->full_lo = attn_full_lo(c.seq, c.blk, p.window), item->full_hi = attn_full_hi(c.seq, c.blk);
+    item->row0 = row0, item->nt = c.blk.nt, item->n_rows = n_rows, item->pos0 = c.seq.past + c.blk.t0;
+    item->head = head, item->s = c.s;
+    item->whole = first == 0 && end == c.blk.ntile, item->first_cta = share.first, item->last_cta = share.last;
+  }
+#pragma unroll 1
+  for (int n = 0; n < NT; ++n) {
+    const int r = 8 * n + (lane >> 2);
+    const bool has = r < n_rows;
+    const float* src = p.q + attn_row_offset(p, row0, head, has ? r : 0, p.q_stride);
+    float4 v[HD / 16];
+    float big = 0.f;
+#pragma unroll
+    for (int k = 0; k < HD / 16; ++k) {
+      const int i = 64 * (k >> 2) + 16 * (lane & 3) + 4 * (k & 3);
+      v[k] = has && i < p.hd ? __ldcg(reinterpret_cast<const float4*>(src + i)) : make_float4(0.f, 0.f, 0.f, 0.f);
+      big = fmaxf(big, fmaxf(fmaxf(fabsf(v[k].x), fabsf(v[k].y)), fmaxf(fabsf(v[k].z), fabsf(v[k].w))));
+    }
+    big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 1));
+    big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 2));
+    float down, up;
+    attn_row_scale(big, down, up);
+#pragma unroll
+    for (int k = 0; k < HD / 16; ++k) {
+      uint4 w;
+      split2(v[k].x * down, v[k].y * down, w.x, w.z);
+      split2(v[k].z * down, v[k].w * down, w.y, w.w);
+      q[(n * (HD / 16) + k) * 32 + lane] = w;
+    }
+    if ((lane & 3) == 0) factor[r] = up * p.scale_log2;
+  }
+}
+
 // WHOLE: heads of HD values, not fewer: the places of scales are known then (873 -> 760 instructions to 16 keys of heads of 128).
 template <int HD, int NT, bool WHOLE>
 __global__ void __launch_bounds__(Q8Shape<HD, NT>::THREADS, 1)
     k_attn_rows_q8(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ AttnParams p, const int granule) {
   using Sh = Q8Shape<HD, NT>;
-  constexpr int WARPS = Sh::WARPS, GROUPS = Sh::GROUPS, THREADS = Sh::THREADS, RB = Sh::RB, STAGES = Sh::STAGES, STAGE = Sh::STAGE, SIDE = Sh::SIDE, PITCH = Sh::PITCH, SLOTS = Sh::SLOTS;
+  constexpr int WARPS = Sh::WARPS, GROUPS = Sh::GROUPS, THREADS = Sh::THREADS, RB = Sh::RB, STAGES = Sh::STAGES, STAGE = Sh::STAGE, SIDE = Sh::SIDE, PITCH = Sh::PITCH;
   constexpr int SLABS = HD / 64, KST = HD / 16, SLAB = Sh::KEYS * 64;
   constexpr int AHEAD = WARPS == 16 ? 2 : 4;  // sums under way
-  static_assert(NT * KST * 512 <= Sh::MERGE, "q's pieces lie where the sums go");
   using Cursor = AttnCursor<Sh::LOG2_TILE, ROWS_EXTRA>;
   extern __shared__ unsigned char smem_raw[];
-  __shared__ uint64_t full[STAGES], empty[STAGES];
+  __shared__ uint64_t full[STAGES], empty[STAGES], item_ready[2], sums_read;
   __shared__ long long s_scan[WARPS];
   __shared__ AttnStart s_start;
-  __shared__ Cursor s_cur;  // the item that is worked on
   __shared__ AskState<Cursor> s_ask[GROUPS];
-  __shared__ int s_last;
-  __shared__ float s_weight[RB], s_factor[RB];
+  __shared__ Cursor s_walk;    // the last item that has been made ready
+  __shared__ Q8Item s_item[2], s_part[2];
+  __shared__ int s_described, s_parts, s_last, s_gave_up[2];
+  __shared__ float s_factor[2][RB], s_weight[RB];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   unsigned char* scales = ring + STAGES * STAGE;
   float* s_o = reinterpret_cast<float*>(scales + STAGES * Sh::SCALES);
-  uint4* s_q = reinterpret_cast<uint4*>(s_o);  // [NT][KST][32]
-  float* s_m = s_o + SLOTS * RB * PITCH;
+  float* s_m = s_o + WARPS * RB * PITCH;
   float* s_l = s_m + WARPS * RB;
+  uint4* s_q = reinterpret_cast<uint4*>(s_l + WARPS * RB);  // [2][NT][KST][32]
 
   pdl_trigger();  // the next kernel may take the SMs that this one leaves free, and do what needs no input of its
-  if (tid == 0)
+  if (tid == 0) {
     for (int i = 0; i < STAGES; ++i) mbar_init(full + i, 1), mbar_init(empty + i, 8);
+    mbar_init(item_ready, 1), mbar_init(item_ready + 1, 1), mbar_init(&sums_read, WARPS);
+    s_parts = s_gave_up[0] = s_gave_up[1] = 0;
+  }
   mbar_fence_init();
   pdl_wait();
   attn_plan<THREADS, Sh::LOG2_TILE, ROWS_EXTRA, 0>(p, reinterpret_cast<int*>(ring), s_scan, &s_start);
   if (s_start.until == s_start.before) return;
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the plan's words lay where the copies go
-  if (tid == 0) {
-    s_cur.start(p, s_start);
-    for (int g = 0; g < GROUPS; ++g) s_ask[g].c = s_cur, s_ask[g].t = s_cur.first(s_start) + g;
+  const int N = (int)(s_start.until - s_start.before);  // tiles of this CTA
+  if (tid < GROUPS) {
+    s_ask[tid].c.start(p, s_start);
+    s_ask[tid].t = s_ask[tid].c.first(s_start) + tid;
   }
   __syncthreads();
 
   const int nb = WHOLE ? HD / 16 : p.hd / 16;  // scales of a key
-  const int N = (int)(s_start.until - s_start.before);  // tiles of this CTA
   // Tile n, by a warp: as many keys at once as lie side by side in every page, by lane.  (A group's state is in shared memory: in registers all warps would pay for
   // it.  What asks for the group's next tile has waited for this one's copies, and with them for what was written ahead of these.)
   auto ask = [&](int n) {
@@ -182,63 +238,46 @@ __global__ void __launch_bounds__(Q8Shape<HD, NT>::THREADS, 1)
     }
     __syncwarp();
   };
-  if (warp == 0)
+  // the first tiles, and the first two items
+  if (warp == 2) {
 #pragma unroll 1
     for (int n = 0; n < STAGES && n < N; ++n) ask(n);
+  } else if (warp < 2) {
+    Cursor c;
+    c.start(p, s_start);
+    int ahead = 0;
+    if (warp == 1) ahead = c.end(s_start) - c.first(s_start);
+    if (warp == 1 && ahead < N) c.next(p);
+    if (warp == 0 || ahead < N) q8_item<HD, NT>(p, s_start, c, s_item + warp, s_q + warp * (Sh::Q / 16), s_factor[warp]);
+    if (warp == 1 && lane == 0) {
+      s_walk = c;
+      s_described = ahead + (ahead < N ? c.end(s_start) - c.first(s_start) : 0);
+    }
+  }
+  __syncthreads();
 
   bool alive = true;
   const int c0 = 2 * (lane & 3);  // this thread's columns (rows of the item): c0, c0 + 1 of every eight
   const int key1 = 4 * (lane >> 3) + ((lane >> 2) & 1);  // and its keys of the warp's 16: this one, and two behind it
   const int key0 = 16 * (warp & 7), group = warp >> 3;   // the warp's keys of a tile, and its tiles: those of this parity
-  const uint32_t ring_at = smem_u32(ring), scales_at = smem_u32(scales), q_at = smem_u32(s_q) + 16 * lane;
-  int done = 0;                                          // tiles of the items ahead
+  const uint32_t ring_at = smem_u32(ring), scales_at = smem_u32(scales);
+  int done = 0;  // tiles of the items ahead
 #pragma unroll 1
-  while (true) {
-    const Cursor& cur = s_cur;
-    const AttnBlock& blk = cur.blk;
-    const AttnStart& st = s_start;
-    const int first_tile = cur.first(st), end_tile = cur.end(st), n_rows = blk.nt * p.g;
-
-    // ---- q: B fragments of q^T, rows scaled by a power of two, as two f16 pieces, put down by one warp per eight rows where the sums go
-    // at the item's end; of 64 values step k has 16 c + 4 k .. + 3 of lane c
+  for (int item = 0; done < N; ++item) {
+    const Q8Item& it = s_item[item & 1];
+    if (item >= 2 && alive) alive = wait_all(item_ready + (item & 1), (item >> 1) - 1);
+    const uint32_t q_at = smem_u32(s_q) + (item & 1) * Sh::Q + 16 * lane;
     float f[NT][2];  // of the thread's columns: score -> log2 units
     int lim[NT][2];  // and the last key their row sees
-    __syncthreads();  // the last item's sums have been read
-    if (warp < NT) {
-      const int r = 8 * warp + (lane >> 2);
-      const bool has = r < n_rows;
-      const float* src = p.q + attn_row_offset(p, cur.seq.q0 + blk.t0, cur.head, has ? r : 0, p.q_stride);
-      float4 v[KST];
-      float big = 0.f;
-#pragma unroll
-      for (int k = 0; k < KST; ++k) {
-        const int i = 64 * (k >> 2) + 8 * c0 + 4 * (k & 3);
-        v[k] = has && i < p.hd ? __ldcg(reinterpret_cast<const float4*>(src + i)) : make_float4(0.f, 0.f, 0.f, 0.f);
-        big = fmaxf(big, fmaxf(fmaxf(fabsf(v[k].x), fabsf(v[k].y)), fmaxf(fabsf(v[k].z), fabsf(v[k].w))));
-      }
-      big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 1));
-      big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 2));
-      float down, up;
-      attn_row_scale(big, down, up);
-#pragma unroll
-      for (int k = 0; k < KST; ++k) {
-        uint4 w;
-        split2(v[k].x * down, v[k].y * down, w.x, w.z);
-        split2(v[k].z * down, v[k].w * down, w.y, w.w);
-        s_q[(warp * KST + k) * 32 + lane] = w;
-      }
-      if ((lane & 3) == 0) s_factor[r] = up * p.scale_log2;
-    }
-    __syncthreads();
+    const int tiles = it.tiles, lo = it.lo, hi = it.hi, full_lo = it.full_lo, full_hi = it.full_hi, first_key = it.key0 + key0;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const int rr = 8 * n + c0 + j;
-        f[n][j] = s_factor[rr];
-        lim[n][j] = cur.seq.past + blk.t0 + (rr < n_rows ? attn_row_token(p, rr) : blk.nt - 1);
+        f[n][j] = s_factor[item & 1][rr];
+        lim[n][j] = it.pos0 + (rr < it.n_rows ? attn_row_token(p, rr) : it.nt - 1);
       }
-    const int full_hi = attn_full_hi(cur.seq, blk), full_lo = attn_full_lo(cur.seq, blk, p.window);
 
     float o[KST][NT][4], m[NT][2], l[NT][2];
 #pragma unroll
@@ -252,15 +291,12 @@ __global__ void __launch_bounds__(Q8Shape<HD, NT>::THREADS, 1)
 
     bool odd = false;  // values that are no numbers were left out
 #pragma unroll 1
-    for (int t = first_tile + ((done ^ group) & (GROUPS - 1)); t < end_tile; t += GROUPS) {
-      const int n = done + t - first_tile, stage = n % STAGES, ks = ((blk.tile0 + t) << Sh::LOG2_TILE) + key0;
-      if (alive) {
-        alive = wait_all(full + stage, n / STAGES);
-        if (!alive && lane == 0) atomicExch(&p.status->timeout, 10);
-      }
+    for (int t = (done ^ group) & (GROUPS - 1); t < tiles; t += GROUPS) {
+      const int n = done + t, stage = n % STAGES, ks = first_key + (t << Sh::LOG2_TILE);
+      if (alive) alive = wait_all(full + stage, n / STAGES);
       // what the group's last tile has left, for the next one but
       if (alive && (warp & 7) == ((n / GROUPS) & 7) && n >= GROUPS && n - GROUPS + STAGES < N) ask(n - GROUPS + STAGES);
-      if (!alive || ks >= blk.hi || ks + 16 <= blk.lo) {
+      if (!alive || ks >= hi || ks + 16 <= lo) {
         if (lane == 0) mbar_arrive(empty + stage);
         continue;
       }
@@ -278,7 +314,7 @@ __global__ void __launch_bounds__(Q8Shape<HD, NT>::THREADS, 1)
 #pragma unroll 1
         for (int e = lane; e < 16 * nb; e += 32) {
           const int key = ks + e / nb;
-          const bool seen = key >= blk.lo && key < blk.hi, k_odd = w[e] >= Q8_ODD, v_odd = w[Sh::SCALES / 2 + e] >= Q8_ODD;
+          const bool seen = key >= lo && key < hi, k_odd = w[e] >= Q8_ODD, v_odd = w[Sh::SCALES / 2 + e] >= Q8_ODD;
           if (k_odd) w[e] = 0xFF;
           if (v_odd || !seen) w[Sh::SCALES / 2 + e] = 0;
           odd |= v_odd && seen;
@@ -442,7 +478,7 @@ __global__ void __launch_bounds__(Q8Shape<HD, NT>::THREADS, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(empty + stage);
     }
-    done += end_tile - first_tile;
+    done += tiles;
 
     // ---- the warps' parts of the item
 #pragma unroll
@@ -456,16 +492,18 @@ __global__ void __launch_bounds__(Q8Shape<HD, NT>::THREADS, 1)
 #pragma unroll
       for (int j = 0; j < 2; ++j)
         if (m[n][j] == -CUDART_INF_F && l[n][j] != 0.f) m[n][j] = 0.f;  // nothing but NaN: a part that counts, not one without keys
-    __syncthreads();  // q's pieces have been read
-    // one half of the warps puts its sums down, the other adds its own to them, each brought to the higher maximum
+    if (item >= 1 && alive) alive = wait_all(&sums_read, item - 1);  // the last item's sums have been read
+    bool keys = false;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) keys |= m[n][0] > -CUDART_INF_F || m[n][1] > -CUDART_INF_F;
     if (lane < 4) {
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int j = 0; j < 2; ++j) s_m[warp * RB + 8 * n + c0 + j] = m[n][j], s_l[warp * RB + 8 * n + c0 + j] = l[n][j];
     }
-    float* mine = s_o + (warp & (SLOTS - 1)) * RB * PITCH + (lane >> 2);
-    if (SLOTS == WARPS || warp >= SLOTS) {
+    if (__any_sync(0xFFFFFFFFu, keys)) {  // (without keys a part's weight is 0, and its sums are not read)
+      float* mine = s_o + warp * RB * PITCH + (lane >> 2);
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -477,48 +515,32 @@ __global__ void __launch_bounds__(Q8Shape<HD, NT>::THREADS, 1)
             to[8] = o[k][n][2 + j];
           }
     }
-    if constexpr (SLOTS < WARPS) __syncthreads();
-    if (SLOTS < WARPS && warp < SLOTS) {
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const float other = s_m[(warp + SLOTS) % WARPS * RB + 8 * n + c0 + j], to = fmaxf(m[n][j], other);
-          const float a = exp2_rel(m[n][j], to), b = exp2_rel(other, to);
-#pragma unroll
-          for (int k = 0; k < KST; ++k) {
-            float* x = mine + (8 * n + c0 + j) * PITCH + 16 * k;
-            x[0] = a * o[k][n][j] + b * x[0];
-            x[8] = a * o[k][n][2 + j] + b * x[8];
-          }
-        }
+    if (!alive && lane == 0) s_gave_up[item & 1] = 1;
+    const bool any_odd = __syncthreads_or(odd) != 0, whole = it.whole;
+    if (s_gave_up[item & 1]) {  // (all leave at the same barrier)
+      if (tid == 0) atomicExch(&p.status->timeout, 10);
+      attn_let_land();  // copies are in flight: they land before this shared memory is somebody else's
+      return;
     }
-    const bool any_odd = __syncthreads_or(odd) != 0;
-    const bool whole = first_tile == 0 && end_tile == blk.ntile;
-    AttnShare share = {0, 0};
-    if (!whole) share = attn_share(cur.ub, blk.ntile, st);
+    const AttnShare share = {it.first_cta, it.last_cta};
 #pragma unroll 1
-    for (int e = tid; e < RB * (HD / 4); e += THREADS) {
+    for (int e = tid; e < it.n_rows * (HD / 4); e += THREADS) {
       const int r = e / (HD / 4), i = 4 * (e % (HD / 4));
-      if (r >= n_rows) continue;
       float M = -CUDART_INF_F, L = 0.f;
 #pragma unroll
       for (int w = 0; w < WARPS; ++w) M = fmaxf(M, s_m[w * RB + r]);
       float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int w = 0; w < SLOTS; ++w) {
-        constexpr bool two = SLOTS < WARPS;  // this slot holds two warps' sums
-        const float m0 = s_m[w * RB + r], m1 = two ? s_m[(w + SLOTS) % WARPS * RB + r] : -CUDART_INF_F;
-        const float wt = exp2_rel(fmaxf(m0, m1), M);
+#pragma unroll 4
+      for (int w = 0; w < WARPS; ++w) {
+        const float wt = exp2_rel(s_m[w * RB + r], M);
+        L += wt * s_l[w * RB + r];
+        if (wt == 0.f) continue;
         const float4 v = *reinterpret_cast<const float4*>(s_o + (w * RB + r) * PITCH + i);
-        L += exp2_rel(m0, M) * s_l[w * RB + r];
-        if (two) L += exp2_rel(m1, M) * s_l[(w + SLOTS) % WARPS * RB + r];
         sum.x += wt * v.x, sum.y += wt * v.y, sum.z += wt * v.z, sum.w += wt * v.w;
       }
       if (whole) {
         const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
-        if (i < p.hd)
-          *reinterpret_cast<float4*>(p.out + attn_row_offset(p, cur.seq.q0 + blk.t0, cur.head, r, p.out_stride) + i) = make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
+        if (i < p.hd) *reinterpret_cast<float4*>(p.out + attn_row_offset(p, it.row0, it.head, r, p.out_stride) + i) = make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
       } else {
         const size_t to = (size_t)attn_slot(blockIdx.x, share) * RB + r;
         __stcg(reinterpret_cast<float4*>(p.part + to * HD + i), sum);
@@ -529,22 +551,39 @@ __global__ void __launch_bounds__(Q8Shape<HD, NT>::THREADS, 1)
     if (any_odd) {  // some row may see values that are no numbers
       __threadfence();
       __syncthreads();
-      const int r = lane < n_rows ? lane : 0;
-      attn_odd_blocks(p, cur.s, cur.head, (blk.tile0 + first_tile) << Sh::LOG2_TILE, (blk.tile0 + end_tile) << Sh::LOG2_TILE, lane < n_rows && s_weight[r] == s_weight[r],
-                      cur.seq.past + blk.t0 + attn_row_token(p, r), warp, WARPS,
-                      whole ? p.out + attn_row_offset(p, cur.seq.q0 + blk.t0, cur.head, r, p.out_stride) : p.part + ((size_t)attn_slot(blockIdx.x, share) * RB + r) * HD);
+      const int r = lane < it.n_rows ? lane : 0;
+      attn_odd_blocks(p, it.s, it.head, it.key0, it.key0 + (tiles << Sh::LOG2_TILE), lane < it.n_rows && s_weight[r] == s_weight[r], it.pos0 + attn_row_token(p, r), warp, WARPS,
+                      whole ? p.out + attn_row_offset(p, it.row0, it.head, r, p.out_stride) : p.part + ((size_t)attn_slot(blockIdx.x, share) * RB + r) * HD);
     }
-    if (!whole && attn_arrive(p, share.first, share.last, &s_last, tid == 0, 0, THREADS)) {
-#pragma unroll 1
-      for (int r = warp; r < n_rows; r += WARPS)
-        attn_join_row<HD>(p, share, RB, r, p.out + attn_row_offset(p, cur.seq.q0 + blk.t0, cur.head, r, p.out_stride));
+    if (tid == 0 && !whole && s_parts < 2) s_part[s_parts++] = it;
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sums_read);
+    if (warp == WARPS - 1 && s_described < N) {  // the item after the next, in this one's place
+      if (alive) alive = wait_all(&sums_read, item);
+      if (lane == 0) s_walk.next(p);
+      __syncwarp();
+      q8_item<HD, NT>(p, s_start, s_walk, s_item + (item & 1), s_q + (item & 1) * (Sh::Q / 16), s_factor[item & 1]);
+      __syncwarp();
+      if (lane == 0) s_described += s_item[item & 1].tiles;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(item_ready + (item & 1));
     }
-    if (done >= N) break;
-    __syncthreads();  // all have done with the item
-    if (tid == 0) s_cur.next(p);
-    __syncthreads();
   }
-  if (!alive) attn_let_land();  // copies are in flight: they land before this shared memory is somebody else's
+  if (__syncthreads_or(!alive)) {
+    if (tid == 0) atomicExch(&p.status->timeout, 10);
+    attn_let_land();
+    return;
+  }
+  // ---- items that other CTAs have tiles of, the first and the last at most: whoever comes last joins them
+#pragma unroll 1
+  for (int i = 0; i < s_parts; ++i) {
+    const Q8Item& it = s_part[i];
+    if (attn_arrive(p, it.first_cta, it.last_cta, &s_last, tid == 0, 0, THREADS)) {
+      const AttnShare share = {it.first_cta, it.last_cta};
+#pragma unroll 1
+      for (int r = warp; r < it.n_rows; r += WARPS) attn_join_row<HD>(p, share, RB, r, p.out + attn_row_offset(p, it.row0, it.head, r, p.out_stride));
+    }
+  }
 }
 
 // Codes of `box` keys of a head, 64 values wide.
@@ -575,15 +614,16 @@ int32_t run_rows_q8(infr_cuda_ctx* ctx, const AttnParams& p) {
 
 template <int HD>
 int32_t run_rows_q8_of(infr_cuda_ctx* ctx, const AttnParams& p, int nt) {
-  if (p.hd == HD) return nt == 1 ? run_rows_q8<HD, 1, true>(ctx, p) : run_rows_q8<HD, 2, true>(ctx, p);
-  return nt == 1 ? run_rows_q8<HD, 1, false>(ctx, p) : run_rows_q8<HD, 2, false>(ctx, p);
+  if constexpr (HD <= 128)
+    if (nt == 2) return p.hd == HD ? run_rows_q8<HD, 2, true>(ctx, p) : run_rows_q8<HD, 2, false>(ctx, p);
+  return p.hd == HD ? run_rows_q8<HD, 1, true>(ctx, p) : run_rows_q8<HD, 1, false>(ctx, p);
 }
 
 }  // namespace
 
-// max_rows: see launch_attn_rows.
+// max_rows: see launch_attn_rows.  Heads wider than 128 have items of eight rows (attn_q8_rows_limit): of sixteen the sums do not fit beside the tiles.
 int32_t launch_attn_rows_q8(infr_cuda_ctx* ctx, AttnParams p, int max_rows) {
-  const int nt = p.g <= 8 && max_rows <= 8 ? 1 : 2;
+  const int nt = p.hd > 128 || (p.g <= 8 && max_rows <= 8) ? 1 : 2;
   p.tb = 8 * nt / p.g;
   if (p.hd <= 64) return run_rows_q8_of<64>(ctx, p, nt);
   if (p.hd <= 128) return run_rows_q8_of<128>(ctx, p, nt);

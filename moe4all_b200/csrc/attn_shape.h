@@ -114,6 +114,9 @@ inline bool attn_few_rows(uint64_t max_rows, uint32_t g, uint64_t pairs) {
   return g <= (uint32_t)ATTN_ROWS_LIMIT && max_rows <= (pairs <= 8 ? 32u : pairs <= 32 ? 16u : 8u);
 }
 
+// Query heads to a kv head that the few-rows kernel over pages of 8 bits takes.
+inline uint32_t attn_q8_rows_limit(uint32_t head_dim) { return head_dim > 128 ? 8u : (uint32_t)ATTN_ROWS_LIMIT; }
+
 // What a call gives, as numbers.
 struct AttnSizes {
   uint32_t rows, n_seq, n_head, n_kv, head_dim;
