@@ -322,10 +322,10 @@ __global__ void __launch_bounds__(Q8Shape<HD, NT>::THREADS, 1)
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // (ahead of the next copy to here)
         __syncwarp();
       }
-      // ---- scores: pieces and even and odd steps apart
+      // ---- scores, q's pieces apart
       float s[NT][4];
       {
-        float part[NT][3][4];
+        float part[NT][4];
 #pragma unroll
         for (int b = 0; b < SLABS; ++b) {
           uint4 kw[2];     // this lane's 16 values of both keys
@@ -344,12 +344,12 @@ __global__ void __launch_bounds__(Q8Shape<HD, NT>::THREADS, 1)
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
               const uint4 w = lds128(q_at + (n * KST + 4 * b + k) * 512);
-              if (b == 0 && k < 2) {
-                mma16816_zero(k & 1 ? part[n][0] : s[n], a, w.x, w.y);
-                mma16816_zero(k & 1 ? part[n][2] : part[n][1], a, w.z, w.w);
+              if (b == 0 && k == 0) {
+                mma16816_zero(s[n], a, w.x, w.y);
+                mma16816_zero(part[n], a, w.z, w.w);
               } else {
-                mma16816(k & 1 ? part[n][0] : s[n], a, w.x, w.y);
-                mma16816(k & 1 ? part[n][2] : part[n][1], a, w.z, w.w);
+                mma16816(s[n], a, w.x, w.y);
+                mma16816(part[n], a, w.z, w.w);
               }
             }
           }
@@ -357,7 +357,7 @@ __global__ void __launch_bounds__(Q8Shape<HD, NT>::THREADS, 1)
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[n][i] = (s[n][i] + part[n][0][i]) + (part[n][1][i] + part[n][2][i]);
+          for (int i = 0; i < 4; ++i) s[n][i] += part[n][i];
       }
       bool grows = false, falls = false;
       float top[NT][2];
