@@ -91,11 +91,12 @@ static __device__ __noinline__ void attn_odd_blocks(const AttnParams& p, int s, 
   }
 }
 
-// Where a group's copies are in the CTA's line.
+// The tile that a group asks for next.
 template <class Cursor>
 struct AskState {
   Cursor c;
-  int t;  // the tile of its item to ask for next
+  int t;           // which one of its item it is
+  int2 place[8];   // by copy: its first key's place in the page (-1: no row sees any of its keys), and the page
 };
 
 // An item as the warps see it.
@@ -113,15 +114,6 @@ template <int HD, int NT, class Cursor>
 static __device__ __noinline__ void q8_item(const AttnParams& p, const AttnStart& st, const Cursor& c, Q8Item* item, uint4* q, float* factor) {
   const int lane = threadIdx.x & 31;
   const int row0 = c.seq.q0 + c.blk.t0, n_rows = c.blk.nt * p.g, head = c.head;
-  if (lane == 0) {
-    const int first = c.first(st), end = c.end(st);
-    const AttnShare share = attn_share(c.ub, c.blk.ntile, st);
-    item->tiles = end - first, item->key0 = (c.blk.tile0 + first) << Q8Shape<HD, NT>::LOG2_TILE;
-    item->lo = c.blk.lo, item->hi = c.blk.hi, item->full_lo = attn_full_lo(c.seq, c.blk, p.window), item->full_hi = attn_full_hi(c.seq, c.blk);
-    item->row0 = row0, item->nt = c.blk.nt, item->n_rows = n_rows, item->pos0 = c.seq.past + c.blk.t0;
-    item->head = head, item->s = c.s;
-    item->whole = first == 0 && end == c.blk.ntile, item->first_cta = share.first, item->last_cta = share.last;
-  }
 #pragma unroll 1
   for (int n = 0; n < NT; ++n) {
     const int r = 8 * n + (lane >> 2);
@@ -133,8 +125,18 @@ static __device__ __noinline__ void q8_item(const AttnParams& p, const AttnStart
     for (int k = 0; k < HD / 16; ++k) {
       const int i = 64 * (k >> 2) + 16 * (lane & 3) + 4 * (k & 3);
       v[k] = has && i < p.hd ? __ldcg(reinterpret_cast<const float4*>(src + i)) : make_float4(0.f, 0.f, 0.f, 0.f);
-      big = fmaxf(big, fmaxf(fmaxf(fabsf(v[k].x), fabsf(v[k].y)), fmaxf(fabsf(v[k].z), fabsf(v[k].w))));
     }
+    if (n == 0 && lane == 0) {  // (while these are on their way)
+      const int first = c.first(st), end = c.end(st);
+      const AttnShare share = attn_share(c.ub, c.blk.ntile, st);
+      item->tiles = end - first, item->key0 = (c.blk.tile0 + first) << Q8Shape<HD, NT>::LOG2_TILE;
+      item->lo = c.blk.lo, item->hi = c.blk.hi, item->full_lo = attn_full_lo(c.seq, c.blk, p.window), item->full_hi = attn_full_hi(c.seq, c.blk);
+      item->row0 = row0, item->nt = c.blk.nt, item->n_rows = n_rows, item->pos0 = c.seq.past + c.blk.t0;
+      item->head = head, item->s = c.s;
+      item->whole = first == 0 && end == c.blk.ntile, item->first_cta = share.first, item->last_cta = share.last;
+    }
+#pragma unroll
+    for (int k = 0; k < HD / 16; ++k) big = fmaxf(big, fmaxf(fmaxf(fabsf(v[k].x), fabsf(v[k].y)), fmaxf(fabsf(v[k].z), fabsf(v[k].w))));
     big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 1));
     big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 2));
     float down, up;
@@ -188,70 +190,61 @@ __global__ void __launch_bounds__(Q8Shape<HD, NT>::THREADS, 1)
   if (s_start.until == s_start.before) return;
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the plan's words lay where the copies go
   const int N = (int)(s_start.until - s_start.before);  // tiles of this CTA
-  if (tid < GROUPS) {
-    s_ask[tid].c.start(p, s_start);
-    s_ask[tid].t = s_ask[tid].c.first(s_start) + tid;
-  }
-  __syncthreads();
-
   const int nb = WHOLE ? HD / 16 : p.hd / 16;  // scales of a key
-  // Tile n, by a warp: as many keys at once as lie side by side in every page, by lane.  (A group's state is in shared memory: in registers all warps would pay for
-  // it.  What asks for the group's next tile has waited for this one's copies, and with them for what was written ahead of these.)
-  auto ask = [&](int n) {
-    AskState<Cursor>& a = s_ask[n & (GROUPS - 1)];
-    if (lane == 0) {
-      int t = a.t;
-      while (t >= a.c.end(s_start)) {
-        t -= a.c.end(s_start);
-        a.c.next(p);
-      }
-      a.t = t;
+  // A tile's copies take as many keys at once as lie side by side in every page, one to a lane.  The tile t of the cursor's item, or of those behind it:
+  auto look = [&](Cursor& c, int& t) {
+    while (t >= c.end(s_start)) {
+      t -= c.end(s_start);
+      c.next(p);
     }
-    __syncwarp();
-    const int key = ((a.c.blk.tile0 + a.t) << Sh::LOG2_TILE) + lane * granule, head = a.c.head, stage = n % STAGES;
-    const bool seen = lane * granule < Sh::KEYS && key < a.c.blk.hi && key + granule > a.c.blk.lo;
-    int y = 0, w = 0;
-    if (seen) {
+    const int key = ((c.blk.tile0 + t) << Sh::LOG2_TILE) + lane * granule;
+    int2 at = make_int2(-1, 0);
+    if (lane * granule < Sh::KEYS && key < c.blk.hi && key + granule > c.blk.lo) {
       const int page = attn_page_of(p, key);
-      w = attn_page(p, a.c.s, page);
-      y = key - page * p.page_size;
+      at = make_int2(key - page * p.page_size, attn_page_entry(p, c.s, page));
     }
-    const int count = __popc(__ballot_sync(0xFFFFFFFFu, seen));
-    if (n >= STAGES && !wait_all(empty + stage, n / STAGES - 1)) {
-      if (lane == 0) atomicExch(&p.status->timeout, 10);
-      return;
-    }
-    if (lane == 0) {
-      a.t += GROUPS;
-      mbar_arrive_expect_tx(full + stage, (uint32_t)(count * granule * (2 * HD + 2 * nb)));
-    }
+    return at;
+  };
+  auto copy = [&](int n, int2 at, int head) {
+    const int stage = n % STAGES, count = __popc(__ballot_sync(0xFFFFFFFFu, at.x >= 0));
+    if (lane == 0) mbar_arrive_expect_tx(full + stage, (uint32_t)(count * granule * (2 * HD + 2 * nb)));
     __syncwarp();
-    if (seen) {
-      const size_t first = ((size_t)w * p.page_pitch + (size_t)head * p.head_pitch + (size_t)y * p.row_pitch) / 16;
+    if (at.x >= 0) {
+      const int w = attn_page_checked(p, at.y);
+      const size_t first = ((size_t)w * p.page_pitch + (size_t)head * p.head_pitch + (size_t)at.x * p.row_pitch) / 16;
       unsigned char *dst = ring + stage * STAGE + lane * granule * 64, *sc = scales + stage * Sh::SCALES + lane * granule * nb;
 #pragma unroll
-      for (int s = 0; s < SLABS; ++s) tma_load_4d(dst + s * SLAB, &kmap, 64 * s, y, head, w, full + stage);
+      for (int s = 0; s < SLABS; ++s) tma_load_4d(dst + s * SLAB, &kmap, 64 * s, at.x, head, w, full + stage);
       bulk_g2s(sc, p.ks + first, granule * nb, full + stage);
 #pragma unroll
-      for (int s = 0; s < SLABS; ++s) tma_load_4d(dst + SIDE + s * SLAB, &vmap, 64 * s, y, head, w, full + stage);
+      for (int s = 0; s < SLABS; ++s) tma_load_4d(dst + SIDE + s * SLAB, &vmap, 64 * s, at.x, head, w, full + stage);
       bulk_g2s(sc + Sh::SCALES / 2, p.vs + first, granule * nb, full + stage);
     }
     __syncwarp();
   };
-  // the first tiles, and the first two items
-  if (warp == 2) {
-#pragma unroll 1
-    for (int n = 0; n < STAGES && n < N; ++n) ask(n);
-  } else if (warp < 2) {
+  // the first two items, the first tiles, and where the groups' next ones are: a warp to each
+  static_assert(2 + STAGES + GROUPS <= WARPS, "a warp to each");
+  if (warp < 2 + STAGES + GROUPS) {
     Cursor c;
     c.start(p, s_start);
-    int ahead = 0;
-    if (warp == 1) ahead = c.end(s_start) - c.first(s_start);
-    if (warp == 1 && ahead < N) c.next(p);
-    if (warp == 0 || ahead < N) q8_item<HD, NT>(p, s_start, c, s_item + warp, s_q + warp * (Sh::Q / 16), s_factor[warp]);
-    if (warp == 1 && lane == 0) {
-      s_walk = c;
-      s_described = ahead + (ahead < N ? c.end(s_start) - c.first(s_start) : 0);
+    if (warp < 2) {
+      int ahead = 0;
+      if (warp == 1) ahead = c.end(s_start) - c.first(s_start);
+      if (warp == 1 && ahead < N) c.next(p);
+      if (warp == 0 || ahead < N) q8_item<HD, NT>(p, s_start, c, s_item + warp, s_q + warp * (Sh::Q / 16), s_factor[warp]);
+      if (warp == 1 && lane == 0) {
+        s_walk = c;
+        s_described = ahead + (ahead < N ? c.end(s_start) - c.first(s_start) : 0);
+      }
+    } else {
+      const int n = warp - 2;
+      int t = c.first(s_start) + n;
+      if (n < N) {
+        const int2 at = look(c, t);
+        if (n < STAGES) copy(n, at, c.head);
+        else if (lane < 8) s_ask[n - STAGES].place[lane] = at;
+      }
+      if (n >= STAGES && lane == 0) s_ask[n - STAGES].c = c, s_ask[n - STAGES].t = t;
     }
   }
   __syncthreads();
@@ -294,9 +287,30 @@ __global__ void __launch_bounds__(Q8Shape<HD, NT>::THREADS, 1)
     for (int t = (done ^ group) & (GROUPS - 1); t < tiles; t += GROUPS) {
       const int n = done + t, stage = n % STAGES, ks = first_key + (t << Sh::LOG2_TILE);
       if (alive) alive = wait_all(full + stage, n / STAGES);
-      // what the group's last tile has left, for the next one but
-      if (alive && (warp & 7) == ((n / GROUPS) & 7) && n >= GROUPS && n - GROUPS + STAGES < N) ask(n - GROUPS + STAGES);
+      // The place that the group's last tile has left, for the next one but: by one warp, each in its turn.  The wait for it is one for the group's last asker too, and
+      // for what that left.  (In shared memory: in registers all warps would pay for it.)  Where the tile after that one is comes behind the scores.
+      const bool asks = alive && (warp & 7) == ((n / GROUPS) & 7) && n >= GROUPS && n - GROUPS + STAGES < N;
+      int2 next = make_int2(-1, 0);
+      if (asks) {
+        AskState<Cursor>& a = s_ask[group];
+        alive = wait_all(empty + (n - GROUPS) % STAGES, (n - GROUPS) / STAGES);
+        if (alive) copy(n - GROUPS + STAGES, lane < 8 ? a.place[lane] : next, a.c.head);
+        if (n + STAGES < N) {
+          if (lane == 0) {
+            a.t += GROUPS;
+            while (a.t >= a.c.end(s_start)) {
+              a.t -= a.c.end(s_start);
+              a.c.next(p);
+            }
+          }
+          __syncwarp();
+          int t = a.t;
+          next = look(a.c, t);
+        }
+      }
       if (!alive || ks >= hi || ks + 16 <= lo) {
+        if (asks && lane < 8) s_ask[group].place[lane] = next;
+        __syncwarp();
         if (lane == 0) mbar_arrive(empty + stage);
         continue;
       }
@@ -409,6 +423,7 @@ __global__ void __launch_bounds__(Q8Shape<HD, NT>::THREADS, 1)
             for (int k = 0; k < KST; ++k) o[k][n][j] *= w, o[k][n][2 + j] *= w;
           }
       }
+      if (asks && lane < 8) s_ask[group].place[lane] = next;
       // ---- weights, transposed into B fragments
       uint32_t ph[NT][2], pl[NT][2];
 #pragma unroll
