@@ -1232,9 +1232,9 @@ int32_t attention(infr_cuda_ctx* ctx, const infr_cuda_attention_desc* d, const K
   if (d->path > 2) return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "attention: unknown path");
   if (d->window > 0x7FFFFFFFu) return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "attention: window is past 31 bits");
   const uint32_t g = d->n_head / d->n_kv, wide = d->n_head * d->head_dim;
-  const uint32_t rows_limit = scales.any() ? attn_q8_rows_limit(d->head_dim) : (uint32_t)ATTN_ROWS_LIMIT;
   if (d->path == 1 && g > (uint32_t)ATTN_ROWS_LIMIT) return fail(ctx, INFR_CUDA_ERR_UNSUPPORTED, "attention: path 1 takes up to 16 query heads to a kv head");
-  if (d->path == 1 && g > rows_limit) return fail(ctx, INFR_CUDA_ERR_UNSUPPORTED, "attention: over pages of 8 bits path 1 takes up to 8 query heads of more than 128 values to a kv head");
+  if (d->path == 1 && scales.any() && g > attn_q8_rows_limit(d->head_dim))
+    return fail(ctx, INFR_CUDA_ERR_UNSUPPORTED, "attention: over pages of 8 bits path 1 takes up to 8 query heads of more than 128 values to a kv head");
   AttnParams p = {};
   if ((rc = attn_check_rows(ctx, "attention: q", d->q, d->rows, d->q_stride, wide, &p.q_stride)) ||
       (rc = attn_check_rows(ctx, "attention: out", d->out, d->rows, d->out_stride, wide, &p.out_stride)))
@@ -1265,7 +1265,9 @@ int32_t attention(infr_cuda_ctx* ctx, const infr_cuda_attention_desc* d, const K
   for (int i = 4; i < 31; ++i)
     if (d->page_size == (1u << i)) p.page_shift = i;
   const uint64_t max_rows = (uint64_t)(d->max_q && d->max_q < d->rows ? d->max_q : d->rows) * g;
-  const bool few = d->path ? d->path == 1 : g <= rows_limit && attn_few_rows(max_rows, g, (uint64_t)d->n_seq * d->n_kv);
+  const bool few = d->path ? d->path == 1
+                   : scales.any() ? attn_q8_few_rows(max_rows, g, d->head_dim, (uint64_t)d->n_seq * d->n_kv)
+                                  : attn_few_rows(max_rows, g, (uint64_t)d->n_seq * d->n_kv);
   // two partial results of 128 rows of 256 values for each CTA, their maxima and weights behind them
   const size_t part = align_up(2 * (size_t)ctx->sm_count * ATTN_TILE_ROWS * 256 * 4, 256);
   if (!ctx->attn_parts) {
