@@ -136,48 +136,71 @@ __global__ void __launch_bounds__(256) k_linear_anyfmt(int dt, const unsigned ch
   if (lane == 0) y[(size_t)blockIdx.y * out_f + o] = acc;
 }
 
-// Rows of a token table by number, scaled: a thread per 16 weights.  An id outside the table gives zeros.
+// Rows of a token table by number, scaled: 16 weights to each of a thread's units.  An id outside the table gives zeros.
 template <int DT>
-__global__ void __launch_bounds__(128) k_embed(int dt, const unsigned char* __restrict__ table, const int* __restrict__ ids, float* __restrict__ dst, DeviceStatus* status, int ne,
-                                               int n_vocab, size_t rb, size_t dst_stride, float scale) {
+__device__ __forceinline__ void embed_unit(int dt, const unsigned char* row, int h, float (&v)[16]) {
+  if constexpr (DT == INFR_CUDA_DT_F32) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) *reinterpret_cast<float4*>(v + 4 * i) = __ldg(reinterpret_cast<const float4*>(row) + 4 * h + i);
+  } else if constexpr (DT == INFR_CUDA_DT_F16 || DT == INFR_CUDA_DT_BF16) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint4 x = __ldg(reinterpret_cast<const uint4*>(row) + 2 * h + i);
+      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        v[8 * i + 2 * j] = DT == INFR_CUDA_DT_F16 ? f16_bits_to_f32(w[j]) : __uint_as_float(w[j] << 16);
+        v[8 * i + 2 * j + 1] = DT == INFR_CUDA_DT_F16 ? f16_bits_to_f32(w[j] >> 16) : __uint_as_float(w[j] & 0xFFFF0000u);
+      }
+    }
+  } else {
+    uint32_t c[4];
+    float A, B;
+    int off;
+    fmt_codes16(DT < 0 ? dt : DT, row, h, c, A, B, off);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = fmaf(A, (float)((int)((c[i >> 2] >> (8 * (i & 3))) & 0xFFu) - off), B);
+  }
+}
+
+constexpr int EMBED_THREADS = 128, EMBED_UNITS = 4;
+
+// Memory bounds it: the rows' bytes and their f32 values, once each.  A warp's values go through shared memory and out in whole lines (each thread's 64 bytes by
+// itself were half a sector to a store: 8191 rows of 7168 from Q8_0 67 us).
+template <int DT>
+__global__ void __launch_bounds__(EMBED_THREADS) k_embed(int dt, const unsigned char* __restrict__ table, const int* __restrict__ ids, float* __restrict__ dst, DeviceStatus* status, int ne,
+                                                         int n_vocab, size_t rb, size_t dst_stride, float scale) {
+  __shared__ __align__(16) float s_v[EMBED_THREADS * 16];
+  const int lane = threadIdx.x & 31, warp0 = threadIdx.x - lane;
+  float* s_w = s_v + warp0 * 16;
   pdl_trigger();
-  const int h = blockIdx.y * 128 + threadIdx.x;
   pdl_wait();
   const int id = __ldcg(ids + blockIdx.x);
-  if (16 * h >= ne) return;
-  float v[16];
-  if ((unsigned)id >= (unsigned)n_vocab) {
-    if (h == 0) status->bad_index = 3;
+  const bool has = (unsigned)id < (unsigned)n_vocab;
+  if (!has && threadIdx.x == 0 && blockIdx.y == 0) status->bad_index = 3;
+  const unsigned char* row = table + (has ? (size_t)id * rb : 0);
+  float* to = dst + (size_t)blockIdx.x * dst_stride;
+#pragma unroll 1
+  for (int k = 0; k < EMBED_UNITS; ++k) {
+    const int h0 = (blockIdx.y * EMBED_UNITS + k) * EMBED_THREADS + warp0, h = h0 + lane;
+    if (16 * h0 >= ne) return;
+    float v[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) v[i] = 0.f;
-  } else {
-    const unsigned char* row = table + (size_t)id * rb;
-    if constexpr (DT == INFR_CUDA_DT_F32) {
+    if (has && 16 * h < ne) embed_unit<DT>(dt, row, h, v);
+    // (a 16-byte word of a lane where four lanes' words of one store meet four different ones)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) *reinterpret_cast<float4*>(v + 4 * i) = __ldg(reinterpret_cast<const float4*>(row) + 4 * h + i);
-    } else if constexpr (DT == INFR_CUDA_DT_F16 || DT == INFR_CUDA_DT_BF16) {
+    for (int i = 0; i < 4; ++i)
+      *reinterpret_cast<float4*>(s_w + 16 * lane + 4 * (i ^ ((lane >> 1) & 3))) = make_float4(v[4 * i] * scale, v[4 * i + 1] * scale, v[4 * i + 2] * scale, v[4 * i + 3] * scale);
+    __syncwarp();
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const uint4 x = __ldg(reinterpret_cast<const uint4*>(row) + 2 * h + i);
-        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          v[8 * i + 2 * j] = DT == INFR_CUDA_DT_F16 ? f16_bits_to_f32(w[j]) : __uint_as_float(w[j] << 16);
-          v[8 * i + 2 * j + 1] = DT == INFR_CUDA_DT_F16 ? f16_bits_to_f32(w[j] >> 16) : __uint_as_float(w[j] & 0xFFFF0000u);
-        }
-      }
-    } else {
-      uint32_t c[4];
-      float A, B;
-      int off;
-      fmt_codes16(DT < 0 ? dt : DT, row, h, c, A, B, off);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = fmaf(A, (float)((int)((c[i >> 2] >> (8 * (i & 3))) & 0xFFu) - off), B);
+    for (int i = 0; i < 4; ++i) {
+      const int word = 32 * i + lane, l = word >> 2;
+      const float4 x = *reinterpret_cast<const float4*>(s_w + 16 * l + 4 * ((word & 3) ^ ((l >> 1) & 3)));
+      if (16 * h0 + 4 * word < ne) *reinterpret_cast<float4*>(to + 16 * h0 + 4 * word) = x;
     }
+    __syncwarp();
   }
-  float4* to = reinterpret_cast<float4*>(dst + (size_t)blockIdx.x * dst_stride + 16 * h);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) to[i] = make_float4(v[4 * i] * scale, v[4 * i + 1] * scale, v[4 * i + 2] * scale, v[4 * i + 3] * scale);
 }
 
 __global__ void k_gated_act(const float* __restrict__ g, const float* __restrict__ u, float* __restrict__ dst, size_t n) {
@@ -319,7 +342,7 @@ int32_t launch_embed(infr_cuda_ctx* ctx, int32_t dtype, const uint8_t* table, co
                       : dtype == INFR_CUDA_DT_Q4K  ? k_embed<INFR_CUDA_DT_Q4K>
                       : dtype == INFR_CUDA_DT_Q6K  ? k_embed<INFR_CUDA_DT_Q6K>
                                                    : k_embed<-1>;
-  const cudaError_t e = launch_ex(kernel, dim3(rows, (ne / 16 + 127) / 128), dim3(128), 0, ctx->stream, true, (int)dtype, table, ids, dst, ctx->status, ne, n_vocab, rb, dst_stride, scale);
+  const cudaError_t e = launch_ex(kernel, dim3(rows, (ne / 16 + EMBED_THREADS * EMBED_UNITS - 1) / (EMBED_THREADS * EMBED_UNITS)), dim3(EMBED_THREADS), 0, ctx->stream, true, (int)dtype, table, ids, dst, ctx->status, ne, n_vocab, rb, dst_stride, scale);
   if (e != cudaSuccess) return check_cuda(ctx, e, "k_embed launch");
   ctx->launches += 1;
   return check_cuda(ctx, cudaGetLastError(), "k_embed launch");

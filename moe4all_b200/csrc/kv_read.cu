@@ -8,14 +8,30 @@ namespace {
 
 constexpr int READ_THREADS = 256, READ_ROWS = 8;
 
-// Eight values of a row to each thread: 8 bytes of codes in (16 of f16), 16 bytes of f16 out (32 of f32), neighbours side by side.
-template <bool Q8, bool F16>
+template <int N>
+__device__ __forceinline__ void load_words(uint32_t (&w)[N], const unsigned char* from) {
+  static_assert(N == 1 || N == 2 || N == 4, "a load's words");
+  if constexpr (N == 4) {
+    const uint4 x = __ldcg(reinterpret_cast<const uint4*>(from));
+    w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+  } else if constexpr (N == 2) {
+    const uint2 x = __ldcg(reinterpret_cast<const uint2*>(from));
+    w[0] = x.x, w[1] = x.y;
+  } else {
+    w[0] = __ldcg(reinterpret_cast<const uint32_t*>(from));
+  }
+}
+
+// 16 bytes of the result to each thread, neighbours side by side (two of these to a thread were half a sector to each store: 332 MB 66 us); its place in a row
+// worked out once, the rows behind each other.
+template <bool Q8, bool F16, int ROWS>
 __global__ void __launch_bounds__(READ_THREADS) k_kv_read(const __grid_constant__ KvReadParams p) {
-  __shared__ long long s_at[READ_ROWS];  // where a row's token lies (-1: a row that is no token; -2: of no sequence)
+  __shared__ long long s_at[ROWS];  // where a row's token lies (-1: a row that is no token; -2: of no sequence)
   __shared__ int s_first;
   const int tid = threadIdx.x, lane = tid & 31;
   const int r0 = (int)((long long)blockIdx.x * p.rows / gridDim.x), r1 = (int)((long long)(blockIdx.x + 1) * p.rows / gridDim.x);
-  const int chunks = p.hd / 8, side = p.n_kv * chunks;
+  constexpr int VALUES = F16 ? 8 : 4, WORDS = VALUES * (Q8 ? 1 : 2) / 4;  // of a thread in a row
+  const int chunks = p.hd / VALUES, side = p.n_kv * chunks;
   pdl_trigger();
   pdl_wait();
   if (tid < 32) {
@@ -35,10 +51,11 @@ __global__ void __launch_bounds__(READ_THREADS) k_kv_read(const __grid_constant_
   int s = s_first;
   AttnSeq seq = {0, 0, 0};
   auto load = [&](int i) { return attn_seq(__ldcg(p.cu_q + i), __ldcg(p.cu_q + i + 1), __ldcg(p.kv_len + i), false, p.rows, p.cap, &bad); };
-  if (tid < READ_ROWS) seq = load(s);
+  if (tid < ROWS) seq = load(s);
 #pragma unroll 1
-  for (int row0 = r0; row0 < r1; row0 += READ_ROWS) {
-    const int rows = min(READ_ROWS, r1 - row0);
+  for (int row0 = r0; row0 < r1; row0 += ROWS) {
+    const int rows = min(ROWS, r1 - row0);
+    if (tid < ROWS && tid >= rows) s_at[tid] = -2;
     if (tid < rows) {
       const int r = row0 + tid;
 #pragma unroll 1
@@ -57,33 +74,49 @@ __global__ void __launch_bounds__(READ_THREADS) k_kv_read(const __grid_constant_
       s_at[tid] = at;
     }
     __syncthreads();
-#pragma unroll 2
-    for (int e = tid; e < rows * 2 * side; e += READ_THREADS) {
-      const int i = e / (2 * side), in = e - i * 2 * side;
-      const bool is_v = in >= side;
-      const int c = is_v ? in - side : in, head = c / chunks;
-      const long long at = s_at[i];
-      if (at == -2) continue;
-      const size_t from = (size_t)max(at, 0ll) + (size_t)head * p.head_pitch + (size_t)(c - head * chunks) * 8;
-      uint4 w = make_uint4(0, 0, 0, 0);  // eight f16 values
-      if (at >= 0) {
-        if constexpr (Q8) {
-          const uint2 codes = __ldcg(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(is_v ? p.v : p.k) + from));
-          const uint32_t d2 = q8_scale_pair(__ldcg((is_v ? p.vs : p.ks) + from / 16));
-          w = make_uint4(q8_lo(codes.x, d2), q8_hi(codes.x, d2), q8_lo(codes.y, d2), q8_hi(codes.y, d2));
-        } else {
-          w = __ldcg(reinterpret_cast<const uint4*>(static_cast<const __half*>(is_v ? p.v : p.k) + from));
+#pragma unroll 1
+    for (int u = tid; u < 2 * side; u += READ_THREADS) {
+      const bool is_v = u >= side;
+      const int c = is_v ? u - side : u, head = c / chunks;
+      const size_t in = (size_t)head * p.head_pitch + (size_t)(c - head * chunks) * VALUES;
+      const void* from = is_v ? p.v : p.k;
+      const uint8_t* scales = is_v ? p.vs : p.ks;
+      const size_t stride = is_v ? p.vo_stride : p.ko_stride;
+      void* to = is_v ? p.v_out : p.k_out;
+      // all rows' words first, none behind another's use
+      uint32_t w[ROWS][WORDS], scale[ROWS];
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i) {
+        const long long at = s_at[i];
+        const size_t x = (size_t)at + in;
+        scale[i] = 0;
+#pragma unroll
+        for (int j = 0; j < WORDS; ++j) w[i][j] = Q8 ? 0x80808080u : 0;
+        if (at >= 0) {
+          if constexpr (Q8) scale[i] = __ldcg(scales + x / 16);
+          load_words(w[i], static_cast<const unsigned char*>(from) + (Q8 ? x : 2 * x));
         }
       }
-      const size_t to = (size_t)(row0 + i) * (is_v ? p.vo_stride : p.ko_stride) + (size_t)c * 8;
-      if constexpr (F16) {
-        *reinterpret_cast<uint4*>(static_cast<__half*>(is_v ? p.v_out : p.k_out) + to) = w;
-      } else {
-        const __half2* h = reinterpret_cast<const __half2*>(&w);
-        const float2 a = __half22float2(h[0]), b = __half22float2(h[1]), cc = __half22float2(h[2]), d = __half22float2(h[3]);
-        float4* dst = reinterpret_cast<float4*>(static_cast<float*>(is_v ? p.v_out : p.k_out) + to);
-        dst[0] = make_float4(a.x, a.y, b.x, b.y);
-        dst[1] = make_float4(cc.x, cc.y, d.x, d.y);
+#pragma unroll
+      for (int i = 0; i < ROWS; ++i) {
+        const long long at = s_at[i];
+        if (at == -2) continue;
+        uint32_t f[VALUES / 2];  // f16 pairs
+        if constexpr (Q8) {
+          const uint32_t d2 = q8_scale_pair(scale[i]);
+#pragma unroll
+          for (int j = 0; j < WORDS; ++j) f[2 * j] = q8_lo(w[i][j], d2), f[2 * j + 1] = q8_hi(w[i][j], d2);
+        } else {
+#pragma unroll
+          for (int j = 0; j < WORDS; ++j) f[j] = w[i][j];
+        }
+        const size_t y = (size_t)(row0 + i) * stride + (size_t)c * VALUES;
+        if constexpr (F16) {
+          *reinterpret_cast<uint4*>(static_cast<__half*>(to) + y) = make_uint4(f[0], f[1], f[2], f[3]);
+        } else {
+          const float2 a = __half22float2(*reinterpret_cast<const __half2*>(f)), b = __half22float2(*reinterpret_cast<const __half2*>(f + 1));
+          *reinterpret_cast<float4*>(static_cast<float*>(to) + y) = make_float4(a.x, a.y, b.x, b.y);
+        }
       }
     }
     __syncthreads();
@@ -149,10 +182,16 @@ __global__ void __launch_bounds__(READ_THREADS) k_kv_unpack(const __grid_constan
 
 }  // namespace
 
+template <bool Q8, bool F16>
+static cudaError_t launch_read(infr_cuda_ctx* ctx, const KvReadParams& p) {
+  // A row to each CTA while all of them are there at once, then eight: 777 rows of 8 x 128 values as f16 3.0 us for 4.3 with eight rows' instructions in the way, 32000
+  // rows of 8 x 128 as f32 58.9 us for 64.9 with 27 rows in a loop, 65.0 with four.
+  if (p.rows <= ctx->sm_count * 8) return launch_ex(k_kv_read<Q8, F16, 1>, dim3(p.rows), dim3(READ_THREADS), 0, ctx->stream, true, p);
+  return launch_ex(k_kv_read<Q8, F16, READ_ROWS>, dim3((p.rows + READ_ROWS - 1) / READ_ROWS), dim3(READ_THREADS), 0, ctx->stream, true, p);
+}
+
 int32_t launch_kv_read(infr_cuda_ctx* ctx, const KvReadParams& p) {
-  const int most = ctx->sm_count * 8;
-  const auto kernel = p.ks != nullptr ? (p.f16 ? k_kv_read<true, true> : k_kv_read<true, false>) : (p.f16 ? k_kv_read<false, true> : k_kv_read<false, false>);
-  const cudaError_t e = launch_ex(kernel, dim3(p.rows < most ? p.rows : most), dim3(READ_THREADS), 0, ctx->stream, true, p);
+  const cudaError_t e = p.ks != nullptr ? (p.f16 ? launch_read<true, true>(ctx, p) : launch_read<true, false>(ctx, p)) : (p.f16 ? launch_read<false, true>(ctx, p) : launch_read<false, false>(ctx, p));
   if (e != cudaSuccess) return check_cuda(ctx, e, "k_kv_read launch");
   ctx->launches += 1;
   return check_cuda(ctx, cudaGetLastError(), "k_kv_read launch");

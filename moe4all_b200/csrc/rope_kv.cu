@@ -36,7 +36,7 @@ __device__ __forceinline__ void store4_f16(__half* dst, const float4& v) {
 
 // JS: eight-value chunks of a lane: 1 for heads up to 128, else 2.  Q8: the cache is one of 8 bits.
 template <int JS, bool Q8>
-__global__ void __launch_bounds__(ROPE_THREADS) k_rope_kv(const __grid_constant__ RopeParams p) {
+__global__ void __launch_bounds__(ROPE_THREADS, Q8 ? 4 : 1) k_rope_kv(const __grid_constant__ RopeParams p) {
   // a head on its way into 8 bits: what shares a scale lies in two to six lanes, as n_rot has it
   __shared__ __align__(16) float s_head[Q8 ? ROPE_TEAMS * 128 * JS : 4];
   __shared__ __align__(16) float s_cos[ROPE_ROWS * ROPE_MAX_PAIRS], s_sin[ROPE_ROWS * ROPE_MAX_PAIRS];
@@ -56,8 +56,13 @@ __global__ void __launch_bounds__(ROPE_THREADS) k_rope_kv(const __grid_constant_
 #pragma unroll
   for (int j = 0; j < JS; ++j) {
     const int c = tl + 16 * j;
-    oa[j] = !p.interleaved && c < rot ? 4 * c : 8 * c;
-    ob[j] = !p.interleaved && c < rot ? p.n_rot / 2 + 4 * c : 8 * c + 4;
+    if constexpr (Q8) {  // half of what is turned apart, or of what is not: neighbours' words side by side, whole pairs in each where they are interleaved
+      oa[j] = c < rot ? 4 * c : p.n_rot + 4 * (c - rot);
+      ob[j] = oa[j] + (c < rot ? p.n_rot : p.hd - p.n_rot) / 2;
+    } else {
+      oa[j] = !p.interleaved && c < rot ? 4 * c : 8 * c;
+      ob[j] = !p.interleaved && c < rot ? p.n_rot / 2 + 4 * c : 8 * c + 4;
+    }
   }
   const int r0 = (int)((long long)blockIdx.x * p.rows / gridDim.x), r1 = (int)((long long)(blockIdx.x + 1) * p.rows / gridDim.x);
   pdl_wait();
@@ -156,7 +161,15 @@ __global__ void __launch_bounds__(ROPE_THREADS) k_rope_kv(const __grid_constant_
           y[j].x *= k * wb.x, y[j].y *= k * wb.y, y[j].z *= k * wb.z, y[j].w *= k * wb.w;
         }
         if (!is_v && c < rot) {
-          const float4 cs = *reinterpret_cast<const float4*>(s_cos + i * ROPE_MAX_PAIRS + 4 * c), sn = *reinterpret_cast<const float4*>(s_sin + i * ROPE_MAX_PAIRS + 4 * c);
+          const float *row_cos = s_cos + i * ROPE_MAX_PAIRS, *row_sin = s_sin + i * ROPE_MAX_PAIRS;
+          float4 cs, sn;
+          if (Q8 && p.interleaved) {
+            const float2 ca = *reinterpret_cast<const float2*>(row_cos + oa[j] / 2), cb = *reinterpret_cast<const float2*>(row_cos + ob[j] / 2);
+            const float2 sa = *reinterpret_cast<const float2*>(row_sin + oa[j] / 2), sb = *reinterpret_cast<const float2*>(row_sin + ob[j] / 2);
+            cs = make_float4(ca.x, ca.y, cb.x, cb.y), sn = make_float4(sa.x, sa.y, sb.x, sb.y);
+          } else {
+            cs = *reinterpret_cast<const float4*>(row_cos + 4 * c), sn = *reinterpret_cast<const float4*>(row_sin + 4 * c);
+          }
           if (p.interleaved) {
             turn(x[j].x, x[j].y, cs.x, sn.x), turn(x[j].z, x[j].w, cs.y, sn.y);
             turn(y[j].x, y[j].y, cs.z, sn.z), turn(y[j].z, y[j].w, cs.w, sn.w);
