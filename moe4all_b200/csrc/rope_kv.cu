@@ -9,6 +9,8 @@
 //
 // Measured: 8192 rows of 32 + 2 x 4 heads of 128 59.9 us, 5.3 TB/s of the rows and the cache (0.81 of the copy rate; 62.4 with heads divided
 // out of an index instead of counted on, 64.5 with five CTAs to an SM in place of four); 777 rows 9.9 us, 32 rows 4.8 us: launch, plan, one row's chain.
+// Into 8 bits: 4099 rows of 16 + 2 x 2 heads of 256, a quarter turned, pairs interleaved 36.5 us, 4.6 TB/s (0.70; 41 with a lane's two words neighbours, half a sector to
+// each, 39 of these with three CTAs to an SM in place of four).
 #include "attn.cuh"
 #include "kv_q8.cuh"
 
@@ -51,7 +53,8 @@ __global__ void __launch_bounds__(ROPE_THREADS, Q8 ? 4 : 1) k_rope_kv(const __gr
 #pragma unroll 1
   for (int b = my_pair; b; b >>= 1, x *= x)
     if (b & 1) turns *= x;
-  const int n_vec = p.n_head + 2 * p.n_kv, chunks = p.hd / 8, rot = p.n_rot / 8;
+  const int all = p.n_head + 2 * p.n_kv, chunks = p.hd / 8, rot = p.n_rot / 8;
+  const int vec0 = Q8 ? all * (int)blockIdx.y / (int)gridDim.y : 0, n_vec = Q8 ? all * ((int)blockIdx.y + 1) / (int)gridDim.y - vec0 : all;  // heads of this CTA's rows
   int oa[JS], ob[JS];
 #pragma unroll
   for (int j = 0; j < JS; ++j) {
@@ -92,7 +95,7 @@ __global__ void __launch_bounds__(ROPE_THREADS, Q8 ? 4 : 1) k_rope_kv(const __gr
   int fi = 0, fh = 0;   // its row of the batch and its number
   auto fetch = [&](int row0, int rows) {
     while (fh >= n_vec) fh -= n_vec, ++fi;
-    const int i = fi, h = fh, r = row0 + i;
+    const int i = fi, h = vec0 + fh, r = row0 + i;
     const bool is_q = h < p.n_head, is_v = h >= p.n_head + p.n_kv;
     const float* src = is_q ? p.q + (size_t)r * p.q_stride + (size_t)h * p.hd
                             : (is_v ? p.v + (size_t)r * p.v_stride + (size_t)(h - p.n_head - p.n_kv) * p.hd : p.k + (size_t)r * p.k_stride + (size_t)(h - p.n_head) * p.hd);
@@ -134,7 +137,7 @@ __global__ void __launch_bounds__(ROPE_THREADS, Q8 ? 4 : 1) k_rope_kv(const __gr
     __syncthreads();
 #pragma unroll 1
     for (int e0 = 0; e0 < rows * n_vec; e0 += ROPE_TEAMS) {
-      const int i = min(fi, rows - 1), h = fh, r = row0 + i;
+      const int i = min(fi, rows - 1), h = vec0 + fh, r = row0 + i;
       const bool is_q = h < p.n_head, is_v = h >= p.n_head + p.n_kv, has = fi < rows && s_pos[i] >= 0;
       const float* w = is_v ? nullptr : (is_q ? p.q_norm : p.k_norm);
       float4 x[JS], y[JS];
@@ -224,7 +227,15 @@ int32_t launch_rope_kv(infr_cuda_ctx* ctx, const RopeParams& p) {
   // Eight to an SM: its threads' worth.  Of these four are there at once (64 registers; three of heads past 128, 80), the rest follow: 8192 rows in two
   // waves 59.9 us.  Fewer rows than that have a CTA each.
   const int most = ctx->sm_count * 8;
-  const cudaError_t e = launch_ex(p.k_scale != nullptr ? (p.hd <= 128 ? k_rope_kv<1, true> : k_rope_kv<2, true>) : (p.hd <= 128 ? k_rope_kv<1, false> : k_rope_kv<2, false>), dim3(p.rows < most ? p.rows : most), dim3(ROPE_THREADS), 0, ctx->stream, true, p);
+  if (p.k_scale != nullptr) {
+    // Fewer rows than SMs: a row's heads over several CTAs, a turn's worth each (32 rows of 32 + 2 x 4 heads 6.5 us for 8.2 with a CTA to a row).
+    const int n_vec = p.n_head + 2 * p.n_kv, turns = (n_vec + ROPE_TEAMS - 1) / ROPE_TEAMS, parts = p.rows >= ctx->sm_count ? 1 : (turns < ctx->sm_count / p.rows ? turns : ctx->sm_count / p.rows);
+    const cudaError_t e = launch_ex(p.hd <= 128 ? k_rope_kv<1, true> : k_rope_kv<2, true>, dim3(p.rows < most ? p.rows : most, parts), dim3(ROPE_THREADS), 0, ctx->stream, true, p);
+    if (e != cudaSuccess) return check_cuda(ctx, e, "k_rope_kv launch");
+    ctx->launches += 1;
+    return check_cuda(ctx, cudaGetLastError(), "k_rope_kv launch");
+  }
+  const cudaError_t e = launch_ex(p.hd <= 128 ? k_rope_kv<1, false> : k_rope_kv<2, false>, dim3(p.rows < most ? p.rows : most), dim3(ROPE_THREADS), 0, ctx->stream, true, p);
   if (e != cudaSuccess) return check_cuda(ctx, e, "k_rope_kv launch");
   ctx->launches += 1;
   return check_cuda(ctx, cudaGetLastError(), "k_rope_kv launch");
