@@ -26,6 +26,8 @@ pub const ERR_NCCL: i32 = -5;
 pub const ERR_TIMEOUT: i32 = -6;
 
 pub const DT_F32: i32 = 0;
+pub const DT_F16: i32 = 1; // token tables only
+pub const DT_BF16: i32 = 30; // token tables only
 pub const DT_Q4K: i32 = 12;
 pub const DT_Q6K: i32 = 14;
 pub const DT_Q8_0: i32 = 8;
@@ -178,6 +180,78 @@ impl Default for infr_cuda_attention_desc {
 }
 
 #[repr(C)]
+#[derive(Clone, Copy)]
+pub struct infr_cuda_kv_read_desc {
+    pub k_cache: *const infr_cuda_buf,
+    pub v_cache: *const infr_cuda_buf,
+    pub k_scale: *const infr_cuda_buf,
+    pub v_scale: *const infr_cuda_buf,
+    pub k: *mut infr_cuda_buf,
+    pub v: *mut infr_cuda_buf,
+    pub cu_q: *const infr_cuda_buf,
+    pub kv_len: *const infr_cuda_buf,
+    pub page_table: *const infr_cuda_buf,
+    pub rows: u32,
+    pub n_seq: u32,
+    pub n_kv: u32,
+    pub head_dim: u32,
+    pub n_pages: u32,
+    pub page_size: u32,
+    pub max_pages: u32,
+    pub k_stride: u32,
+    pub v_stride: u32,
+    pub f16: u32,
+}
+
+impl Default for infr_cuda_kv_read_desc {
+    fn default() -> Self {
+        unsafe { std::mem::zeroed() }
+    }
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct infr_cuda_embed_desc {
+    pub table: *const infr_cuda_buf,
+    pub ids: *const infr_cuda_buf,
+    pub dst: *mut infr_cuda_buf,
+    pub dtype: i32,
+    pub rows: u32,
+    pub ne: u32,
+    pub n_vocab: u32,
+    pub dst_stride: u32,
+    pub scale: f32,
+}
+
+impl Default for infr_cuda_embed_desc {
+    fn default() -> Self {
+        unsafe { std::mem::zeroed() }
+    }
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct infr_cuda_sample_desc {
+    pub logits: *const infr_cuda_buf,
+    pub u: *const infr_cuda_buf,
+    pub temperature: *const infr_cuda_buf,
+    pub top_k: *const infr_cuda_buf,
+    pub top_p: *const infr_cuda_buf,
+    pub min_p: *const infr_cuda_buf,
+    pub ids: *mut infr_cuda_buf,
+    pub prob: *mut infr_cuda_buf,
+    pub rows: u32,
+    pub n_vocab: u32,
+    pub stride: u32,
+}
+
+impl Default for infr_cuda_sample_desc {
+    fn default() -> Self {
+        unsafe { std::mem::zeroed() }
+    }
+}
+
+#[repr(C)]
 #[derive(Clone, Copy, Default)]
 pub struct infr_cuda_config {
     pub gu_warps: u32,
@@ -230,6 +304,11 @@ extern "C" {
                                     gate: *const infr_cuda_buf, dst: *mut infr_cuda_buf, rows: u32, n: u32) -> i32;
     pub fn infr_cuda_rope_kv(ctx: *mut infr_cuda_ctx, desc: *const infr_cuda_rope_kv_desc) -> i32;
     pub fn infr_cuda_attention(ctx: *mut infr_cuda_ctx, desc: *const infr_cuda_attention_desc) -> i32;
+    pub fn infr_cuda_rope_kv_q8(ctx: *mut infr_cuda_ctx, desc: *const infr_cuda_rope_kv_desc, k_scale: *mut infr_cuda_buf, v_scale: *mut infr_cuda_buf) -> i32;
+    pub fn infr_cuda_attention_q8(ctx: *mut infr_cuda_ctx, desc: *const infr_cuda_attention_desc, k_scale: *const infr_cuda_buf, v_scale: *const infr_cuda_buf) -> i32;
+    pub fn infr_cuda_kv_read(ctx: *mut infr_cuda_ctx, desc: *const infr_cuda_kv_read_desc) -> i32;
+    pub fn infr_cuda_embed(ctx: *mut infr_cuda_ctx, desc: *const infr_cuda_embed_desc) -> i32;
+    pub fn infr_cuda_sample(ctx: *mut infr_cuda_ctx, desc: *const infr_cuda_sample_desc) -> i32;
     pub fn infr_cuda_rmsnorm(ctx: *mut infr_cuda_ctx, x: *const infr_cuda_buf, weight: *const infr_cuda_buf,
                              dst: *mut infr_cuda_buf, rows: u32, dim: u32, eps: f32) -> i32;
     pub fn infr_cuda_add(ctx: *mut infr_cuda_ctx, a: *const infr_cuda_buf, b: *const infr_cuda_buf, dst: *mut infr_cuda_buf, n: usize) -> i32;

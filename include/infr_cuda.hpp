@@ -41,7 +41,8 @@ struct Result {
 // crates/infr-core/src/tensor.rs:7-57, numbered as in the GGUF file format.
 enum class DType : int32_t { F32 = INFR_CUDA_DT_F32, Q4_0 = INFR_CUDA_DT_Q4_0, Q4_1 = INFR_CUDA_DT_Q4_1, Q5_0 = INFR_CUDA_DT_Q5_0,
                              Q5_1 = INFR_CUDA_DT_Q5_1, Q2K = INFR_CUDA_DT_Q2K, Q3K = INFR_CUDA_DT_Q3K, Q8_0 = INFR_CUDA_DT_Q8_0, Q4K = INFR_CUDA_DT_Q4K, Q5K = INFR_CUDA_DT_Q5K, Q6K = INFR_CUDA_DT_Q6K, IQ4NL = INFR_CUDA_DT_IQ4NL, IQ4XS = INFR_CUDA_DT_IQ4XS, MXFP4 = INFR_CUDA_DT_MXFP4, NVFP4 = INFR_CUDA_DT_NVFP4, Q2_0 = INFR_CUDA_DT_Q2_0,
-                             IQ2XS = INFR_CUDA_DT_IQ2XS, IQ2S = INFR_CUDA_DT_IQ2S, IQ3XXS = INFR_CUDA_DT_IQ3XXS, IQ3S = INFR_CUDA_DT_IQ3S };
+                             IQ2XS = INFR_CUDA_DT_IQ2XS, IQ2S = INFR_CUDA_DT_IQ2S, IQ3XXS = INFR_CUDA_DT_IQ3XXS, IQ3S = INFR_CUDA_DT_IQ3S,
+                             F16 = INFR_CUDA_DT_F16, BF16 = INFR_CUDA_DT_BF16 };  // (these two: token tables only)
 // crates/infr-core/src/graph.rs:73-85
 enum class MoeGating : uint32_t {
   Softmax = INFR_CUDA_GATING_SOFTMAX,
@@ -151,6 +152,8 @@ struct RopeKv {
   Buffer* q_out = nullptr;
   Buffer* k_cache = nullptr;
   Buffer* v_cache = nullptr;
+  Buffer* k_scale = nullptr;  // with these k_cache and v_cache are codes of 8 bits
+  Buffer* v_scale = nullptr;
   const Buffer* q_norm = nullptr;
   const Buffer* k_norm = nullptr;
   const Buffer* freq_factors = nullptr;
@@ -178,6 +181,8 @@ struct Attention {
   const Buffer* q = nullptr;
   const Buffer* k = nullptr;
   const Buffer* v = nullptr;
+  const Buffer* k_scale = nullptr;  // with these k and v are codes of 8 bits
+  const Buffer* v_scale = nullptr;
   Buffer* out = nullptr;
   uint32_t q_stride = 0, out_stride = 0, max_q = 0, window = 0, path = 0;
   float scale = 0.f;
@@ -189,6 +194,72 @@ struct Attention {
     batch.fill(d);
     d.q = h(q), d.k = h(k), d.v = h(v), d.out = h(out);
     d.q_stride = q_stride, d.out_stride = out_stride, d.max_q = max_q, d.window = window, d.scale = scale, d.path = path;
+    return d;
+  }
+};
+
+// Keys and values of a batch's rows out of the cache's pages (batch.n_head is not looked at).
+struct KvRead {
+  SeqBatch batch;
+  const Buffer* k_cache = nullptr;
+  const Buffer* v_cache = nullptr;
+  const Buffer* k_scale = nullptr;  // of pages of 8 bits
+  const Buffer* v_scale = nullptr;
+  Buffer* k = nullptr;
+  Buffer* v = nullptr;
+  uint32_t k_stride = 0, v_stride = 0;
+  bool f16 = false;
+
+  infr_cuda_kv_read_desc to_desc() const {
+    infr_cuda_kv_read_desc d;
+    std::memset(&d, 0, sizeof d);
+    auto h = [](const Buffer* b) -> infr_cuda_buf* { return b ? b->handle() : nullptr; };
+    d.k_cache = h(k_cache), d.v_cache = h(v_cache), d.k_scale = h(k_scale), d.v_scale = h(v_scale), d.k = h(k), d.v = h(v);
+    d.cu_q = h(batch.cu_q), d.kv_len = h(batch.kv_len), d.page_table = h(batch.page_table);
+    d.rows = batch.rows, d.n_seq = batch.n_seq, d.n_kv = batch.n_kv, d.head_dim = batch.head_dim;
+    d.n_pages = batch.n_pages, d.page_size = batch.page_size, d.max_pages = batch.max_pages;
+    d.k_stride = k_stride, d.v_stride = v_stride, d.f16 = f16;
+    return d;
+  }
+};
+
+// Rows of a token table by number, scaled.
+struct Embed {
+  const Buffer* table = nullptr;
+  const Buffer* ids = nullptr;
+  Buffer* dst = nullptr;
+  DType dtype = DType::F32;
+  uint32_t rows = 0, ne = 0, n_vocab = 0, dst_stride = 0;
+  float scale = 1.f;
+
+  infr_cuda_embed_desc to_desc() const {
+    infr_cuda_embed_desc d;
+    std::memset(&d, 0, sizeof d);
+    auto h = [](const Buffer* b) -> infr_cuda_buf* { return b ? b->handle() : nullptr; };
+    d.table = h(table), d.ids = h(ids), d.dst = h(dst), d.dtype = static_cast<int32_t>(dtype);
+    d.rows = rows, d.ne = ne, d.n_vocab = n_vocab, d.dst_stride = dst_stride, d.scale = scale;
+    return d;
+  }
+};
+
+// A token of each row of logits from given random numbers, settings by row (null: that setting is off).
+struct Sample {
+  const Buffer* logits = nullptr;
+  const Buffer* u = nullptr;
+  const Buffer* temperature = nullptr;
+  const Buffer* top_k = nullptr;
+  const Buffer* top_p = nullptr;
+  const Buffer* min_p = nullptr;
+  Buffer* ids = nullptr;
+  Buffer* prob = nullptr;
+  uint32_t rows = 0, n_vocab = 0, stride = 0;
+
+  infr_cuda_sample_desc to_desc() const {
+    infr_cuda_sample_desc d;
+    std::memset(&d, 0, sizeof d);
+    auto h = [](const Buffer* b) -> infr_cuda_buf* { return b ? b->handle() : nullptr; };
+    d.logits = h(logits), d.u = h(u), d.temperature = h(temperature), d.top_k = h(top_k), d.top_p = h(top_p), d.min_p = h(min_p), d.ids = h(ids), d.prob = h(prob);
+    d.rows = rows, d.n_vocab = n_vocab, d.stride = stride;
     return d;
   }
 };
@@ -347,11 +418,25 @@ class Backend {
   }
   Status rope_kv(const RopeKv& op) {
     const infr_cuda_rope_kv_desc d = op.to_desc();
+    if (op.k_scale || op.v_scale) return st(infr_cuda_rope_kv_q8(ctx_, &d, op.k_scale ? op.k_scale->handle() : nullptr, op.v_scale ? op.v_scale->handle() : nullptr));
     return st(infr_cuda_rope_kv(ctx_, &d));
   }
   Status attention(const Attention& op) {
     const infr_cuda_attention_desc d = op.to_desc();
+    if (op.k_scale || op.v_scale) return st(infr_cuda_attention_q8(ctx_, &d, op.k_scale ? op.k_scale->handle() : nullptr, op.v_scale ? op.v_scale->handle() : nullptr));
     return st(infr_cuda_attention(ctx_, &d));
+  }
+  Status kv_read(const KvRead& op) {
+    const infr_cuda_kv_read_desc d = op.to_desc();
+    return st(infr_cuda_kv_read(ctx_, &d));
+  }
+  Status embed(const Embed& op) {
+    const infr_cuda_embed_desc d = op.to_desc();
+    return st(infr_cuda_embed(ctx_, &d));
+  }
+  Status sample(const Sample& op) {
+    const infr_cuda_sample_desc d = op.to_desc();
+    return st(infr_cuda_sample(ctx_, &d));
   }
   Status gated_act(const Buffer& gate, const Buffer& up, Buffer& dst, size_t n) { return st(infr_cuda_gated_act(ctx_, gate.handle(), up.handle(), dst.handle(), n)); }
   Status moe_shared_expert_add(const Buffer& moe, const Buffer& shexp, const Buffer& gate, Buffer& dst, uint32_t rows, uint32_t n) {
