@@ -11,6 +11,10 @@
 // 1152, times the scale: all exact).  So there are sixteen warps where the registers hold that, in two groups that take tiles of 128 keys in turn; and one warp of a
 // group asks for a whole tile, each in its turn (by every warp for itself the copies were a third of all instructions, and a warp more would take registers from all).
 // Between items stands one barrier of the CTA, behind which all add up the warps' sums; an item's q and its other words are made ready two items ahead.
+//
+// Measured (heads of 128, 32 to 4 kv heads): single tokens of 64 sequences of 700 to 8000 keys 77 us (f16 pages 85), one of 131072 keys 51.6 (60; 143 MB, 2.8 TB/s), one
+// of 513 12.7 (10.8), of which the plan and the first item take 8 to 10.  What bounds it is issue: 570 to 700 instructions to a warp's 16 keys, half of them on the way
+// from codes to f16 fragments.
 #include "attn.cuh"
 #include "kv_q8.cuh"
 
@@ -152,7 +156,7 @@ static __device__ __noinline__ void q8_item(const AttnParams& p, const AttnStart
   }
 }
 
-// WHOLE: heads of HD values, not fewer: the places of scales are known then (873 -> 760 instructions to 16 keys of heads of 128).
+// WHOLE: heads of HD values, not fewer: the places of scales are known then (an eighth fewer instructions to 16 keys of heads of 128).
 template <int HD, int NT, bool WHOLE>
 __global__ void __launch_bounds__(Q8Shape<HD, NT>::THREADS, 1)
     k_attn_rows_q8(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ AttnParams p, const int granule) {
@@ -337,42 +341,39 @@ __global__ void __launch_bounds__(Q8Shape<HD, NT>::THREADS, 1)
         __syncwarp();
       }
       // ---- scores, q's pieces apart
-      float s[NT][4];
-      {
-        float part[NT][4];
+      float s[NT][4], part[NT][4];
 #pragma unroll
-        for (int b = 0; b < SLABS; ++b) {
-          uint4 kw[2];     // this lane's 16 values of both keys
-          uint32_t kd[2];  // and their scales (behind the head's end q is 0 and the codes' values are finite)
+      for (int b = 0; b < SLABS; ++b) {
+        uint4 kw[2];     // this lane's 16 values of both keys
+        uint32_t kd[2];  // and their scales (behind the head's end q is 0 and the codes' values are finite)
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int key = key1 + 2 * j, blk16 = 4 * b + (lane & 3);
-            kw[j] = lds128(kb + b * SLAB + key * 64 + (((lane & 3) ^ ((key >> 1) & 3)) << 4));
-            kd[j] = WHOLE || blk16 < nb ? lds8(sc + key * nb + blk16) * 0x00800080u : 0u;  // (both halves of a pair: << 7)
-          }
+        for (int j = 0; j < 2; ++j) {
+          const int key = key1 + 2 * j, blk16 = 4 * b + (lane & 3);
+          kw[j] = lds128(kb + b * SLAB + key * 64 + (((lane & 3) ^ ((key >> 1) & 3)) << 4));
+          kd[j] = WHOLE || blk16 < nb ? lds8(sc + key * nb + blk16) * 0x00800080u : 0u;  // (both halves of a pair: << 7)
+        }
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const uint32_t w0 = k == 0 ? kw[0].x : k == 1 ? kw[0].y : k == 2 ? kw[0].z : kw[0].w;
-            const uint32_t w1 = k == 0 ? kw[1].x : k == 1 ? kw[1].y : k == 2 ? kw[1].z : kw[1].w;
-            const uint32_t a[4] = {q8_lo(w0, kd[0]), q8_lo(w1, kd[1]), q8_hi(w0, kd[0]), q8_hi(w1, kd[1])};
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t w0 = k == 0 ? kw[0].x : k == 1 ? kw[0].y : k == 2 ? kw[0].z : kw[0].w;
+          const uint32_t w1 = k == 0 ? kw[1].x : k == 1 ? kw[1].y : k == 2 ? kw[1].z : kw[1].w;
+          const uint32_t a[4] = {q8_lo(w0, kd[0]), q8_lo(w1, kd[1]), q8_hi(w0, kd[0]), q8_hi(w1, kd[1])};
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              const uint4 w = lds128(q_at + (n * KST + 4 * b + k) * 512);
-              if (b == 0 && k == 0) {
-                mma16816_zero(s[n], a, w.x, w.y);
-                mma16816_zero(part[n], a, w.z, w.w);
-              } else {
-                mma16816(s[n], a, w.x, w.y);
-                mma16816(part[n], a, w.z, w.w);
-              }
+          for (int n = 0; n < NT; ++n) {
+            const uint4 w = lds128(q_at + (n * KST + 4 * b + k) * 512);
+            if (b == 0 && k == 0) {
+              mma16816_zero(s[n], a, w.x, w.y);
+              mma16816_zero(part[n], a, w.z, w.w);
+            } else {
+              mma16816(s[n], a, w.x, w.y);
+              mma16816(part[n], a, w.z, w.w);
             }
           }
         }
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) s[n][i] += part[n][i];
       }
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[n][i] += part[n][i];
       bool grows = false, falls = false;
       float top[NT][2];
 #pragma unroll
@@ -428,19 +429,19 @@ __global__ void __launch_bounds__(Q8Shape<HD, NT>::THREADS, 1)
       uint32_t ph[NT][2], pl[NT][2];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-          float e[4];
+        float e[4];
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const float ref = m[n][j] == -CUDART_INF_F ? 0.f : m[n][j];
-            e[j] = exp2_approx((s[n][j] - ref) + ATTN_BIAS);  // (in this order: scores of any size)
-            e[2 + j] = exp2_approx((s[n][2 + j] - ref) + ATTN_BIAS);
-            l[n][j] += e[j] + e[2 + j];
-          }
-          split2(e[0], e[1], ph[n][0], pl[n][0]);
-          split2(e[2], e[3], ph[n][1], pl[n][1]);
-#pragma unroll
-          for (int i = 0; i < 2; ++i) ph[n][i] = movm(ph[n][i]), pl[n][i] = movm(pl[n][i]);
+        for (int j = 0; j < 2; ++j) {
+          const float ref = m[n][j] == -CUDART_INF_F ? 0.f : m[n][j];
+          e[j] = exp2_approx((s[n][j] - ref) + ATTN_BIAS);  // (in this order: scores of any size)
+          e[2 + j] = exp2_approx((s[n][2 + j] - ref) + ATTN_BIAS);
+          l[n][j] += e[j] + e[2 + j];
         }
+        split2(e[0], e[1], ph[n][0], pl[n][0]);
+        split2(e[2], e[3], ph[n][1], pl[n][1]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) ph[n][i] = movm(ph[n][i]), pl[n][i] = movm(pl[n][i]);
+      }
       // ---- sums, from zero for every slice and added here: the tensor cores truncate, and a running sum would lose 2^-23 of itself to every slice
       const uint32_t vb = kb + SIDE;
 #pragma unroll
@@ -467,21 +468,21 @@ __global__ void __launch_bounds__(Q8Shape<HD, NT>::THREADS, 1)
         for (int k1 = 0; k1 < 4; k1 += AHEAD) {
           float sum[AHEAD][NT][4];
 #pragma unroll
-            for (int k = 0; k < AHEAD; k += 2) {
-              uint32_t r[4];
-              const int c = k1 + k + (lane >> 4), kk = lane & 15;
-              ldsm2_t8(r, vb + (k0 >> 2) * SLAB + kk * 64 + ((c ^ ((kk >> 1) & 3)) << 4));
+          for (int k = 0; k < AHEAD; k += 2) {
+            uint32_t r[4];
+            const int c = k1 + k + (lane >> 4), kk = lane & 15;
+            ldsm2_t8(r, vb + (k0 >> 2) * SLAB + kk * 64 + ((c ^ ((kk >> 1) & 3)) << 4));
 #pragma unroll
-              for (int i = 0; i < 2; ++i) {
-                const uint32_t *two = ab[(k1 + k) >> 1], d01 = __byte_perm(two[0], 0, i ? 0x3424 : 0x1404) >> 1, d23 = __byte_perm(two[1], 0, i ? 0x3424 : 0x1404) >> 1;
-                const uint32_t a[4] = {q8_lo(r[2 * i], d01), q8_lo(r[2 * i + 1], d01), q8_hi(r[2 * i], d23), q8_hi(r[2 * i + 1], d23)};
+            for (int i = 0; i < 2; ++i) {
+              const uint32_t *two = ab[(k1 + k) >> 1], d01 = __byte_perm(two[0], 0, i ? 0x3424 : 0x1404) >> 1, d23 = __byte_perm(two[1], 0, i ? 0x3424 : 0x1404) >> 1;
+              const uint32_t a[4] = {q8_lo(r[2 * i], d01), q8_lo(r[2 * i + 1], d01), q8_hi(r[2 * i], d23), q8_hi(r[2 * i + 1], d23)};
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                  mma16816_zero(sum[k + i][n], a, pl[n][0], pl[n][1]);
-                  mma16816(sum[k + i][n], a, ph[n][0], ph[n][1]);
-                }
+              for (int n = 0; n < NT; ++n) {
+                mma16816_zero(sum[k + i][n], a, pl[n][0], pl[n][1]);
+                mma16816(sum[k + i][n], a, ph[n][0], ph[n][1]);
               }
             }
+          }
 #pragma unroll
           for (int k = 0; k < AHEAD; ++k)
 #pragma unroll

@@ -550,3 +550,45 @@ def test_refusals(backend):
         call(op)
         call(dataclasses.replace(op, rows=0))
     be.sync()
+
+
+@pytest.mark.parametrize("H,K,hd", [(9, 1, 144), (16, 1, 256), (32, 2, 192), (17, 1, 64)])
+def test_more_heads_than_the_few_rows_kernel_takes(backend, H, K, hd):
+    """The choice by itself goes to the tiles; the few-rows kernel asked for by name is refused."""
+    from moe4all_b200 import Unsupported
+
+    b = Q8Batch([1, 3, 1], [70, 0, 400], H, K, hd, page=16, seed=H)
+    check(backend, b)
+    with pytest.raises(Unsupported):
+        backend.attention(b.op(backend, path=1))
+
+
+@pytest.mark.parametrize("n,K,rows", [(2, 4, 64), (2, 4, 65), (4, 4, 48), (4, 4, 49), (9, 4, 32), (9, 4, 33)])
+def test_both_sides_of_the_choice(backend, n, K, rows):
+    check(backend, Q8Batch([rows] + [1] * (n - 1), [100 + i for i in range(n)], 2 * K, K, 64, page=32, seed=rows))
+
+
+def test_two_contexts_side_by_side(backend):
+    """Two contexts over one cache, calls of both under way at once: each has f16 pages and partial sums of its own."""
+    import torch
+
+    from moe4all_b200 import CudaBackend
+
+    b = Q8Batch([70, 1, 90], [300, 2000, 0], 8, 2, 128, page=64, seed=90)
+    want, tol = b.ref()
+    other = CudaBackend(0)
+    try:
+        outs = [torch.full_like(b.out, 7.5) for _ in range(2)]
+        ops = [[b.op(be, out=be.wrap_tensor(o), path=path) for path in (2, 1)] for be, o in zip((backend, other), outs)]
+        torch.cuda.synchronize()
+        for path in range(2):
+            for _ in range(5):
+                for be, op in zip((backend, other), ops):
+                    be.attention(op[path])
+            backend.sync(), other.sync()
+            for o in outs:
+                assert float((o - want).abs().max()) <= tol
+                o.fill_(7.5)
+            torch.cuda.synchronize()
+    finally:
+        other.close()

@@ -342,3 +342,41 @@ def test_sample_refusals(backend):
     be.sample(dataclasses.replace(ok, rows=0))
     be.sample(dataclasses.replace(ok, prob=None, temperature=None, top_k=None, top_p=None, min_p=None))
     be.sync()
+
+
+@pytest.mark.parametrize("k", [2, 63, 64, 65, 1023, 1024, 1025, 4096, 4097])
+@pytest.mark.parametrize("order", ["up", "down", "one_part", "mixed"])
+def test_where_the_largest_lie(backend, k, order):
+    """Sorted logits, and the largest all in one stretch of the row: what a CTA or a thread finds of them is anything from none to all."""
+    V = 60000
+    x = np.sort(logits(np.random.default_rng(k), 1, V)[0])
+    if order == "down":
+        x = x[::-1]
+    elif order == "one_part":
+        x = np.concatenate([x[: V // 3], x[V - 5000 :], x[V // 3 : V - 5000]])
+    elif order == "mixed":
+        x = np.random.default_rng(k + 1).permutation(x)
+    x = np.tile(x, (4, 1)).astype(np.float32)
+    compare(backend, x, u=np.array([0.0, 0.31, 0.77, 0.999]), top_k=[k, k, k, k], top_p=[1.0, 0.9, 1.0, 0.5], temperature=[1.0, 1.0, 3.0, 30.0])
+
+
+def test_samplers_of_two_contexts(backend):
+    import torch
+
+    from moe4all_b200 import CudaBackend
+
+    rng = np.random.default_rng(77)
+    x = logits(rng, 3, 90001)
+    kw = dict(u=rng.random(3), top_k=[0, 50, 2000], top_p=[0.9, 1.0, 0.8])
+    want, _, _, op = run(backend, x, **kw)
+    other = CudaBackend(0)
+    try:
+        got, _, _, op2 = run(other, x, **kw)
+        assert (got == want).all()
+        for _ in range(10):
+            backend.sample(op), other.sample(op2)
+        backend.sync(), other.sync()
+        torch.cuda.synchronize()
+        assert (run(backend, x, **kw)[0] == want).all()
+    finally:
+        other.close()
