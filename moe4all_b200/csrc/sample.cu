@@ -12,6 +12,10 @@
 //
 // A cluster of eight CTAs has a row.  Every decision is made from numbers that all eight have got from one of them, added up in the same order, so that they
 // take the same steps and meet at the same barriers whatever the row and its settings hold (and should somebody write them meanwhile).
+//
+// Measured, of 150000: one row of which the largest is taken 5.2 us, of the 20 largest 7.1, of all 12.2, of the 1000 largest those with 0.95 25.7, of all with 0.9, spread over
+// thousands, 45; 64 rows 17, 25, 41, 66, 137, with settings of all kinds 79.  One pass over the row reads it (2.6 us of the 45); what bounds the rest is the f64 of a
+// weight - thirteen operations to a value, in four passes - and the barriers of the cluster, a microsecond each.
 #include <cooperative_groups.h>
 #include <math_constants.h>
 
@@ -52,7 +56,13 @@ struct __align__(16) SampleShared {
     uint32_t hist[SAMPLE_BINS];
     double few_weight[SAMPLE_THREADS];  // a candidate's to a thread
   };
-  u64 list[SAMPLE_LIST];
+  union {
+    u64 list[SAMPLE_LIST];
+    struct {
+      uint32_t place[SAMPLE_BINS];   // 64ths of a bin that its values lie behind its beginning, together
+      uint32_t places[SAMPLE_BINS];  // and those of all CTAs
+    };
+  };
   union {
     uint32_t sums[SAMPLE_BINS];  // of all CTAs' hist
     uint32_t few_hist[SAMPLE_CTAS][SAMPLE_FEW_BINS];
@@ -142,16 +152,17 @@ struct Sampler {
     }
     __device__ __forceinline__ bool has(float y, int j) const { return y > x || (y == x && j <= i); }
   };
-  // The weight of all values into every CTA's sum; there behind the next cluster barrier.
-  __device__ void sum_up(u64 within) {
+  // The weight of all values into every CTA's sum, and that of the threads' largest into `above`; there behind the next cluster barrier.
+  __device__ void sum_up(u64 within, float my_top) {
     const Upto in(within);
-    double sum = 0, all;
+    double sum = 0, all, largest;
     mine([&](float x, int i) {
       const double w = weight(x);
       sum += in.has(x, i) ? w : 0.0;
     });
     before<double>(sum, sh.scan[0], all);
-    tell(sh.sum, all);
+    before<double>(weight(my_top), sh.scan[1], largest);
+    tell(sh.sum, all), tell(sh.above, largest);
   }
 
   template <typename T>
@@ -192,8 +203,11 @@ struct Sampler {
   __device__ void tell_one(int* word, int v) {
     if (tid < SAMPLE_CTAS) *cluster.map_shared_rank(word, tid) = v;
   }
-  __device__ void clear_hist() {
-    for (int b = tid; b < SAMPLE_BINS; b += THREADS) sh.hist[b] = 0;
+  __device__ void clear_hist(bool places) {
+    for (int b = tid; b < SAMPLE_BINS; b += THREADS) {
+      sh.hist[b] = 0;
+      if (places) sh.place[b] = 0;
+    }
     if (tid == 0) sh.n_list = 0, sh.b1 = sh.b2 = SAMPLE_BINS;
     __syncthreads();
   }
@@ -205,9 +219,10 @@ struct Sampler {
 
   // The bins b1 .. b2 that the border lies in, how many values lie ahead of them and up to their end.  By count: the bin of the k-th value; by weight: those
   // that may have the value with which the sum passes `target`, by the weights `hi` and `lo` that a bin's values have at most and at least.
-  // (`slack`: by how much of a weight a bin's edges are off)
+  // (`slack`: by how much of a weight a bin's edges are off.  `places`: how far in their bins the values lie is known: a weight is a convex function of that,
+  // at most the chord between the edges, at least a `gap` of the first one's below it)
   template <class Edge>
-  __device__ void bracket(bool by_weight, int k, double target, double slack, Edge edge) {
+  __device__ void bracket(bool by_weight, int k, double target, double slack, bool places, double gap, Edge edge) {
     // every CTA adds up an eighth of the bins, and tells the sums to all
     constexpr int EIGHTH = SAMPLE_BINS / SAMPLE_CTAS / 4;
     static_assert(EIGHTH * SAMPLE_CTAS % THREADS == 0, "every thread takes part in every round");
@@ -221,6 +236,15 @@ struct Sampler {
         h.z += __shfl_xor_sync(0xFFFFFFFFu, h.z, o), h.w += __shfl_xor_sync(0xFFFFFFFFu, h.w, o);
       }
       reinterpret_cast<uint4*>(cluster.map_shared_rank(sh.sums, e % SAMPLE_CTAS))[at] = h;
+      if (places) {
+        h = reinterpret_cast<const uint4*>(cluster.map_shared_rank(sh.place, e % SAMPLE_CTAS))[at];
+#pragma unroll
+        for (int o = 1; o < SAMPLE_CTAS; o <<= 1) {
+          h.x += __shfl_xor_sync(0xFFFFFFFFu, h.x, o), h.y += __shfl_xor_sync(0xFFFFFFFFu, h.y, o);
+          h.z += __shfl_xor_sync(0xFFFFFFFFu, h.z, o), h.w += __shfl_xor_sync(0xFFFFFFFFu, h.w, o);
+        }
+        reinterpret_cast<uint4*>(cluster.map_shared_rank(sh.places, e % SAMPLE_CTAS))[at] = h;
+      }
     }
     cluster.sync();
     uint32_t c[PER], sum_c = 0;
@@ -238,8 +262,9 @@ struct Sampler {
 #pragma unroll
       for (int j = 0; j < PER; ++j) {
         const double next = edge(PER * tid + j + 1);
-        sum_hi += hi[j] = c[j] * w * (1.0 + slack);
-        sum_lo += lo[j] = c[j] * next * (1.0 - slack);
+        const double far = places ? (w - next) * (sh.places[PER * tid + j] * 0.015625) : 0.0;
+        sum_hi += hi[j] = (c[j] * w - far) * (1.0 + slack);
+        sum_lo += lo[j] = (places ? c[j] * (w - (w - next) * 0.015625 - w * gap) - far : c[j] * next) * (1.0 - slack);
         w = next;
       }
       double sum;
@@ -366,16 +391,32 @@ struct Sampler {
     return to;
   }
 
-  // Bins of one width from the largest value down to `low`: the nearest edge, so that a value is within half a bin (and f32's 2^-22 of its distance).
+  // Bins of one width from the largest value down to `low`, in 64 places each: the nearest place (a half of one behind, and f32's 2^-22 of the distance).
   // (A difference of halves does not overflow.)
-  float bin_scale, bin_half;
+  float place_scale, bin_half;
   __device__ void set_bins(float low) {
-    bin_scale = top > low ? (float)((double)(SAMPLE_BINS - 1) / (0.5 * ((double)top - (double)low))) : 0.f;
+    place_scale = top > low ? (float)((double)(64 * (SAMPLE_BINS - 1)) / (0.5 * ((double)top - (double)low))) : 0.f;
     bin_half = 0.5f * top;
   }
-  __device__ int bin(float x) const {
-    const float b = fminf(fmaf(fmaf(-0.5f, x, bin_half), bin_scale, 8388608.f), 8388608.f + (SAMPLE_BINS - 1));
-    return (int)(__float_as_uint(b) & (SAMPLE_BINS - 1));
+  __device__ uint32_t place(float x) const {  // from half a bin ahead of the largest value on
+    const float b = fminf(fmaf(fmaf(-0.5f, x, bin_half), place_scale, 8388608.f), 8388608.f + (64 * (SAMPLE_BINS - 1) + 31));
+    return (__float_as_uint(b) & 0x7FFFFFu) + 32;
+  }
+  __device__ int bin(float x) const { return (int)(place(x) >> 6); }
+
+  // The first rank from `first` on (up to the one of `low`, or one more) whose value is in bin b or one behind it: a warp's lanes at 32 places at a time.
+  __device__ uint32_t rank_of_bin(int b, float low) const {
+    u64 lo = rank_of(top), hi = (u64)rank_of(low) + 1;
+#pragma unroll 1
+    while (lo < hi) {
+      const u64 step = (hi - lo + 31) / 32, at = lo + (tid & 31) * step;
+      const bool ahead = at < hi && bin(value_of((uint32_t)at)) < b;
+      const int n = __popc(__ballot_sync(0xFFFFFFFFu, ahead));  // (the lanes ahead are the first ones)
+      if (n == 0) break;
+      lo += (n - 1) * step + 1;
+      hi = min(hi, lo + step - 1);
+    }
+    return (uint32_t)lo;
   }
 
   // The border of the first CTA's n candidates, to all: that of the k largest and (p < 1) of the run with p of their weight.
@@ -529,17 +570,26 @@ struct Sampler {
     const Upto in(within);
     *both = false;
     // ---- bins down to the least value that has a weight (a border of the k largest may lie behind: then nothing is left out)
-    const float low = floor_x;
+    float low = floor_x;
+    if (by_weight) {
+      // (or could be the border: from it on lies more than 1 - p of the weight, in n_vocab values at most, none of them above it)
+      const double least = (double)top + 32.0 * log2(0.999 * (1.0 - p) * total(sh.sum) / n_vocab) / steps;
+      if (least > (double)low) low = __double2float_rd(least);
+    }
     set_bins(low);
-    clear_hist();
+    clear_hist(by_weight);
     mine([&](float x, int i) {
-      if (x >= low && in.has(x, i)) atomicAdd(&sh.hist[bin(x)], 1u);
+      if (x >= low && in.has(x, i)) {
+        const uint32_t at = place(x);
+        atomicAdd(&sh.hist[at >> 6], 1u);
+        if (by_weight) atomicAdd(&sh.place[at >> 6], at & 63);
+      }
     });
     cluster.sync();
     const double target = by_weight ? p * total(sh.sum) : 0;
-    const double width = bin_scale > 0.f ? 2.0 * steps / bin_scale : 0.0;
+    const double width = place_scale > 0.f ? 128.0 * steps / place_scale : 0.0, gap = (width * (0.69314718055994531 / 32)) * (width * (0.69314718055994531 / 32)) / 8;
     // (f32 moves a bin's edges by 2^-22 of their distance from the largest, which is 45 in the exponent at most)
-    bracket(by_weight, k, target, 3e-5, [&](int b) { return power32((0.5 - b) * width); });
+    bracket(by_weight, k, target, 3e-5, by_weight, gap, [&](int b) { return power32((0.5 + 1.0 / 128 - b) * width); });
     int b1 = sh.b1, b2 = sh.b2, ahead = sh.ahead, upto = sh.upto;
     if (b1 < 0) return within;
     bool whole = !by_weight && upto <= SAMPLE_LIST;  // the list takes what lies ahead too
@@ -571,7 +621,7 @@ struct Sampler {
       by_rank = true;
       int shift = 0;
       while (((r2 - r1) >> shift) >= SAMPLE_BINS) ++shift;
-      clear_hist();
+      clear_hist(false);
       double over = 0;
       mine([&](float x, int i) {
         const uint32_t r = rank_of(x);
@@ -588,7 +638,7 @@ struct Sampler {
       if (by_weight) above = total(sh.above);
       from = r1;
       const int was = ahead;
-      bracket(by_weight, k - was, target - above, 0.0, [&](int b) {
+      bracket(by_weight, k - was, target - above, 0.0, false, 0.0, [&](int b) {
         const u64 r = r1 + ((u64)b << shift);
         return r > r2 ? 0.0 : weight(value_of((uint32_t)r));
       });
@@ -647,18 +697,19 @@ struct Sampler {
         return sh.border;
       }
     }
-    // ---- the candidates into the first CTA's list
+    // ---- the candidates into a list of this CTA's, from which the first one fetches them (one by one into its list they waited a microsecond each)
+    if (!by_rank) r1 = rank_of_bin(b1, low), r2 = rank_of_bin(b2 + 1, low) - 1;
+    const float x1 = whole ? CUDART_INF_F : value_of(r1), x2 = value_of(r2), x0 = by_rank ? value_of(from) : CUDART_INF_F;
     double over = 0;
     mine([&](float x, int i) {
-      if (x < low || !in.has(x, i)) return;
-      const uint32_t r = rank_of(x);
-      const int b = by_rank ? 0 : bin(x);
-      if (by_rank ? r > r2 : b > b2) return;
-      if (whole || (by_rank ? r >= r1 : b >= b1)) {
-        const int to = atomicAdd(cluster.map_shared_rank(&sh.n_list, 0), 1);
-        if (to < SAMPLE_LIST) *cluster.map_shared_rank(&sh.list[to], 0) = place_of(x, i);  // (always)
-      } else if (by_weight && r >= from) {
-        over += weight(x);
+      const bool has = x >= x2 && in.has(x, i), listed = has && x <= x1;
+      if (by_weight) {  // (a weight to all: several at a time, without branches)
+        const double w = weight(x);
+        over += has && !listed && x <= x0 ? w : 0.0;
+      }
+      if (listed) {
+        const int to = atomicAdd(&sh.n_list, 1);
+        if (to < SAMPLE_LIST) sh.list[to] = place_of(x, i);  // (always)
       }
     });
     if (by_weight) {
@@ -667,9 +718,19 @@ struct Sampler {
       if (by_rank) cluster.sync();  // (the last level's words have been read)
       tell(sh.above, all);
     }
+    __syncthreads();
+    tell(sh.n_few, sh.n_list);
     cluster.sync();
     if (me == 0) {
-      const int count = min(sh.n_list, SAMPLE_LIST);
+      int count = 0;
+#pragma unroll 1
+      for (int r = 0; r < SAMPLE_CTAS; ++r) {
+        const int n = min(sh.n_few[r], SAMPLE_LIST - count);
+        if (r > 0)
+          for (int e = tid; e < n; e += THREADS) sh.list[count + e] = cluster.map_shared_rank(sh.list, r)[e];
+        count += n;
+      }
+      __syncthreads();
       if (!by_weight) {
         cut_list(count, whole ? k : k - ahead, whole ? p : 1.0);
       } else {
@@ -789,15 +850,17 @@ __global__ void __cluster_dims__(SAMPLE_CTAS, 1, 1) __launch_bounds__(SAMPLE_THR
     if (found == s.BORDER) border = sh.border, both = true;
   }
   if (!limited && top_p < 1.f) {  // (mostly a short run)
-    s.sum_up(border);
-    if (s.few_largest(SAMPLE_FEW, true, (double)top_p, least, part, my_top, least_top, id_out, prob_out) == s.TOKEN) return;
+    s.sum_up(border, my_top);
+    cluster.sync();
+    // (where the threads' largest together are less than the run, as good as never)
+    if (s.total(sh.above) >= (double)top_p * s.total(sh.sum) && s.few_largest(SAMPLE_FEW, true, (double)top_p, least, part, my_top, least_top, id_out, prob_out) == s.TOKEN) return;
   }
   if (limited && !both) border = s.find(border, top_k, (double)top_p, &both);
   if (top_p < 1.f && !both) {
     bool done;
     cluster.sync();
     if (limited) {
-      s.sum_up(border);
+      s.sum_up(border, my_top);
       cluster.sync();
     }
     border = s.find(border, 0, (double)top_p, &done);
@@ -891,8 +954,8 @@ int32_t launch_sample(infr_cuda_ctx* ctx, const float* logits, const float* u, c
                       float* prob, size_t stride, int rows, int n_vocab) {
   SampleParams p = {logits, u, temperature, top_p, min_p, top_k, ids, prob, stride, n_vocab, 0};
   const int per = ((n_vocab + 3 + 3) / 4 + SAMPLE_CTAS - 1) / SAMPLE_CTAS * 4;
-  // A row that fits is kept in shared memory: 64 rows of 150000 with settings of all kinds 98 us, read again from L2 108, with 256 threads to a CTA (all rows at
-  // once then, but each of them slower) 141; rows that all take one of the 20 largest 25, 26 and 17.
+  // A row that fits is kept in shared memory: 64 rows of 150000 with settings of all kinds 98 us (79 since), read again from L2 108, with 256 threads to a CTA (all rows at
+  // once then, but each of them slower) 141, with four CTAs to a row 128; rows that all take one of the 20 largest 25, 26 and 17.
   p.cached = per <= SAMPLE_CAP;
   const size_t smem = p.cached ? (size_t)per * 4 : 0;
   cudaError_t e = ensure_smem(reinterpret_cast<const void*>(&k_sample), (size_t)SAMPLE_CAP * 4);
