@@ -7,8 +7,8 @@
 // scale are four steps of the product.  And the 16 keys stand in the order in which a transposing load of bytes gives V's, four neighbouring keys to a lane: row i
 // of the scores is key 4 (i / 2) + i % 2, row 8 + i two behind it.  A block of 16 values of V is one product's 16 rows, so its scales are one number to each key.
 //
-// Half the bytes of f16 pages leave the instructions as the bound: a code costs one and a half of them on its way to f16 (byte behind the exponent of 1024, minus
-// 1152, times the scale: all exact).  So there are sixteen warps where the registers hold that, in two groups that take tiles of 128 keys in turn; and one warp of a
+// Half the bytes of f16 pages leave the instructions as the bound: a code costs one of them on its way to f16 (byte behind the exponent of 1024, times
+// the scale and minus 1152 times it: exact; as 32nds, so that no product is past f16).  So there are sixteen warps where the registers hold that, in two groups that take tiles of 128 keys in turn; and one warp of a
 // group asks for a whole tile, each in its turn (by every warp for itself the copies were a third of all instructions, and a warp more would take registers from all).
 // Between items stands one barrier of the CTA, behind which all add up the warps' sums; an item's q and its other words are made ready two items ahead.
 //
@@ -152,7 +152,7 @@ static __device__ __noinline__ void q8_item(const AttnParams& p, const AttnStart
       split2(v[k].z * down, v[k].w * down, w.y, w.w);
       q[(n * (HD / 16) + k) * 32 + lane] = w;
     }
-    if ((lane & 3) == 0) factor[r] = up * p.scale_log2;
+    if ((lane & 3) == 0) factor[r] = 32.f * up * p.scale_log2;  // (keys come as 32nds)
   }
 }
 
@@ -345,18 +345,18 @@ __global__ void __launch_bounds__(Q8Shape<HD, NT>::THREADS, 1)
 #pragma unroll
       for (int b = 0; b < SLABS; ++b) {
         uint4 kw[2];     // this lane's 16 values of both keys
-        uint32_t kd[2];  // and their scales (behind the head's end q is 0 and the codes' values are finite)
+        uint32_t kd[2], ko[2];  // and their scales (behind the head's end q is 0 and the codes' values are finite)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const int key = key1 + 2 * j, blk16 = 4 * b + (lane & 3);
           kw[j] = lds128(kb + b * SLAB + key * 64 + (((lane & 3) ^ ((key >> 1) & 3)) << 4));
-          kd[j] = WHOLE || blk16 < nb ? lds8(sc + key * nb + blk16) * 0x00800080u : 0u;  // (both halves of a pair: << 7)
+          q8_32nds(WHOLE || blk16 < nb ? lds8(sc + key * nb + blk16) * 0x00800080u : 0u, kd[j], ko[j]);  // (both halves of a pair: << 7)
         }
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const uint32_t w0 = k == 0 ? kw[0].x : k == 1 ? kw[0].y : k == 2 ? kw[0].z : kw[0].w;
           const uint32_t w1 = k == 0 ? kw[1].x : k == 1 ? kw[1].y : k == 2 ? kw[1].z : kw[1].w;
-          const uint32_t a[4] = {q8_lo(w0, kd[0]), q8_lo(w1, kd[1]), q8_hi(w0, kd[0]), q8_hi(w1, kd[1])};
+          const uint32_t a[4] = {q8_lo32(w0, kd[0], ko[0]), q8_lo32(w1, kd[1], ko[1]), q8_hi32(w0, kd[0], ko[0]), q8_hi32(w1, kd[1], ko[1])};
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             const uint4 w = lds128(q_at + (n * KST + 4 * b + k) * 512);
@@ -475,7 +475,9 @@ __global__ void __launch_bounds__(Q8Shape<HD, NT>::THREADS, 1)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
               const uint32_t *two = ab[(k1 + k) >> 1], d01 = __byte_perm(two[0], 0, i ? 0x3424 : 0x1404) >> 1, d23 = __byte_perm(two[1], 0, i ? 0x3424 : 0x1404) >> 1;
-              const uint32_t a[4] = {q8_lo(r[2 * i], d01), q8_lo(r[2 * i + 1], d01), q8_hi(r[2 * i], d23), q8_hi(r[2 * i + 1], d23)};
+              uint32_t a01, a23, o01, o23;
+              q8_32nds(d01, a01, o01), q8_32nds(d23, a23, o23);
+              const uint32_t a[4] = {q8_lo32(r[2 * i], a01, o01), q8_lo32(r[2 * i + 1], a01, o01), q8_hi32(r[2 * i], a23, o23), q8_hi32(r[2 * i + 1], a23, o23)};
 #pragma unroll
               for (int n = 0; n < NT; ++n) {
                 mma16816_zero(sum[k + i][n], a, pl[n][0], pl[n][1]);
@@ -527,8 +529,8 @@ __global__ void __launch_bounds__(Q8Shape<HD, NT>::THREADS, 1)
 #pragma unroll
           for (int k = 0; k < KST; ++k) {
             float* to = mine + (8 * n + c0 + j) * PITCH + 16 * k;
-            to[0] = o[k][n][j];
-            to[8] = o[k][n][2 + j];
+            to[0] = 32.f * o[k][n][j];  // (values come as 32nds)
+            to[8] = 32.f * o[k][n][2 + j];
           }
     }
     if (!alive && lane == 0) s_gave_up[item & 1] = 1;
