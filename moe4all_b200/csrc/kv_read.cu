@@ -124,11 +124,13 @@ __global__ void __launch_bounds__(READ_THREADS) k_kv_read(const __grid_constant_
   if (bad) p.status->bad_index = 2;
 }
 
-// The pages that some row of the call sees, one kv head of a page at a time.
-__global__ void __launch_bounds__(READ_THREADS) k_kv_unpack(const __grid_constant__ AttnParams p, __half* __restrict__ k, __half* __restrict__ v, int* __restrict__ table) {
+// The pages that some row of the call sees: a warp to 128 blocks of 16 values, which are a part of a kv head of a page (a CTA to all of such a head were ten in a row for
+// pages of 16 tokens, each with its own wait for the page's number).
+constexpr int UNPACK_PIECE = 128;
+__global__ void __launch_bounds__(READ_THREADS) k_kv_unpack(const __grid_constant__ AttnParams p, __half* __restrict__ k_out, __half* __restrict__ v, int* __restrict__ table) {
   extern __shared__ int s_pre[];  // pages ahead of each sequence, then the first page of each
   __shared__ long long s_scan[READ_THREADS / 32];
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid & 31;
   int* s_page0 = s_pre + p.n_seq + 1;
   pdl_trigger();
   pdl_wait();
@@ -150,11 +152,13 @@ __global__ void __launch_bounds__(READ_THREADS) k_kv_unpack(const __grid_constan
     __syncthreads();
     carry = s_pre[min(s0 + READ_THREADS, p.n_seq)];
   }
-  const long long units = carry * p.n_kv, u0 = units * blockIdx.x / gridDim.x, u1 = units * (blockIdx.x + 1) / gridDim.x;
-  const int blocks = p.hd / 16, per = p.page_size * blocks;  // 16 values to each thread
+  const int blocks = p.hd / 16, per = p.page_size * blocks, pieces = (2 * per + UNPACK_PIECE - 1) / UNPACK_PIECE;  // 16 values to each of a unit's places
+  const long long units = carry * p.n_kv * pieces, warps = (long long)gridDim.x * (READ_THREADS / 32), w = (long long)blockIdx.x * (READ_THREADS / 32) + (tid >> 5);
+  const long long u0 = units * w / warps, u1 = units * (w + 1) / warps;
 #pragma unroll 1
   for (long long u = u0; u < u1; ++u) {
-    const int page = (int)(u / p.n_kv), head = (int)(u - (long long)page * p.n_kv);
+    const long long side = u / pieces;
+    const int piece = (int)(u - side * pieces), page = (int)(side / p.n_kv), head = (int)(side - (long long)page * p.n_kv);
     int s = 0;
 #pragma unroll 1
     for (int hi = p.n_seq; hi - s > 1;) {  // the last sequence whose pages begin at or before this one
@@ -165,17 +169,26 @@ __global__ void __launch_bounds__(READ_THREADS) k_kv_unpack(const __grid_constan
     while (s_pre[s + 1] <= page) ++s;  // (past sequences without pages)
     const int j = s_page0[s] + page - s_pre[s], id = attn_page(p, s, j);
     const int to_page = table != nullptr ? s * p.max_pages + j : id;
-    if (table != nullptr && head == 0 && tid == 0) table[(size_t)s * p.max_pages + j] = to_page;
+    if (table != nullptr && head == 0 && piece == 0 && lane == 0) table[(size_t)s * p.max_pages + j] = to_page;
     const size_t from = (size_t)id * p.page_pitch + (size_t)head * p.head_pitch, to = (size_t)to_page * p.page_pitch + (size_t)head * p.head_pitch;
-#pragma unroll 1
-    for (int e = tid; e < 2 * per; e += READ_THREADS) {
-      const bool is_v = e >= per;
-      const size_t at = (size_t)(is_v ? e - per : e) * 16;
-      const uint4 c = __ldcg(reinterpret_cast<const uint4*>((is_v ? p.vq : p.kq) + from + at));
-      const uint32_t d2 = q8_scale_pair(__ldcg((is_v ? p.vs : p.ks) + (from + at) / 16));
-      uint4* dst = reinterpret_cast<uint4*>((is_v ? v : k) + to + at);
-      dst[0] = make_uint4(q8_lo(c.x, d2), q8_hi(c.x, d2), q8_lo(c.y, d2), q8_hi(c.y, d2));
-      dst[1] = make_uint4(q8_lo(c.z, d2), q8_hi(c.z, d2), q8_lo(c.w, d2), q8_hi(c.w, d2));
+    uint4 c[UNPACK_PIECE / 32];
+    uint32_t d2[UNPACK_PIECE / 32];
+#pragma unroll
+    for (int k = 0; k < UNPACK_PIECE / 32; ++k) {
+      const int e = piece * UNPACK_PIECE + 32 * k + lane;
+      const size_t at = from + (size_t)(e >= per ? e - per : e) * 16;
+      if (e < 2 * per) {
+        c[k] = __ldcg(reinterpret_cast<const uint4*>((e >= per ? p.vq : p.kq) + at));
+        d2[k] = q8_scale_pair(__ldcg((e >= per ? p.vs : p.ks) + at / 16));
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < UNPACK_PIECE / 32; ++k) {
+      const int e = piece * UNPACK_PIECE + 32 * k + lane;
+      if (e >= 2 * per) continue;
+      uint4* dst = reinterpret_cast<uint4*>((e >= per ? v : k_out) + to + (size_t)(e >= per ? e - per : e) * 16);
+      dst[0] = make_uint4(q8_lo(c[k].x, d2[k]), q8_hi(c[k].x, d2[k]), q8_lo(c[k].y, d2[k]), q8_hi(c[k].y, d2[k]));
+      dst[1] = make_uint4(q8_lo(c[k].z, d2[k]), q8_hi(c[k].z, d2[k]), q8_lo(c[k].w, d2[k]), q8_hi(c[k].w, d2[k]));
     }
   }
 }
