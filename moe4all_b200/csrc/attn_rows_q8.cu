@@ -12,9 +12,9 @@
 // group asks for a whole tile, each in its turn (by every warp for itself the copies were a third of all instructions, and a warp more would take registers from all).
 // Between items stands one barrier of the CTA, behind which all add up the warps' sums; an item's q and its other words are made ready two items ahead.
 //
-// Measured (heads of 128, 32 to 4 kv heads): single tokens of 64 sequences of 700 to 8000 keys 77 us (f16 pages 85), one of 131072 keys 51.6 (60; 143 MB, 2.8 TB/s), one
-// of 513 12.7 (10.8), of which the plan and the first item take 8 to 10.  What bounds it is issue: 570 to 700 instructions to a warp's 16 keys, half of them on the way
-// from codes to f16 fragments.
+// Measured (heads of 128, 32 to 4 kv heads): single tokens of 64 sequences of 700 to 8000 keys 76.9 us (f16 pages 85), one of 131072 keys 51.5 (60; 143 MB, 2.8 TB/s), one
+// of 513 12.7 (10.8), of which the plan and the first item take 8 to 10.  What bounds it is latency: four warps to a scheduler, 550 to 680 instructions to 16 keys, issue 0.43;
+// an operation less to every pair of codes was half a per cent.
 #include "attn.cuh"
 #include "kv_q8.cuh"
 
