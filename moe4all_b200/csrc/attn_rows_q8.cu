@@ -148,11 +148,11 @@ static __device__ __noinline__ void q8_item(const AttnParams& p, const AttnStart
 #pragma unroll
     for (int k = 0; k < HD / 16; ++k) {
       uint4 w;
-      split2(v[k].x * down, v[k].y * down, w.x, w.z);
-      split2(v[k].z * down, v[k].w * down, w.y, w.w);
+      split2(v[k].x * down * 32.f, v[k].y * down * 32.f, w.x, w.z);  // (keys come as 32nds; 32 down may be past f32)
+      split2(v[k].z * down * 32.f, v[k].w * down * 32.f, w.y, w.w);
       q[(n * (HD / 16) + k) * 32 + lane] = w;
     }
-    if ((lane & 3) == 0) factor[r] = 32.f * up * p.scale_log2;  // (keys come as 32nds)
+    if ((lane & 3) == 0) factor[r] = up * p.scale_log2;
   }
 }
 

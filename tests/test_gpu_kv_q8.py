@@ -592,3 +592,25 @@ def test_two_contexts_side_by_side(backend):
             torch.cuda.synchronize()
     finally:
         other.close()
+
+
+@pytest.mark.parametrize("path", [1, 2])
+@pytest.mark.parametrize("size", [3.0e38, 1.0e-38, 1.0e-44])
+def test_rows_of_any_size(backend, path, size):
+    """q near both ends of f32, and a scale that brings the scores back (both powers of two but for rounding of the rows themselves)."""
+    import torch
+
+    b = Q8Batch([1, 2], [60, 200], 4, 2, 64, page=16, seed=95)
+    q = b.q.clone()
+    s = 2.0 ** np.floor(np.log2(size / float(q.abs().max())))
+    scale = float(np.clip(64 ** -0.5 / s, 2e-38, 1e37))
+    b.q.copy_((q.double() * s).float())
+    torch.cuda.synchronize()
+    got = b.out.clone()
+    op = b.op(backend, path=path, scale=scale, out=backend.wrap_tensor(got))
+    backend.attention(op)
+    backend.sync()
+    # the plain scale over rows that are the same numbers (those that f32 rounded near its lower end among them)
+    b.q.copy_((b.q.double() * (scale / 64 ** -0.5)).float())
+    want, tol = b.ref()
+    assert bool(got.isfinite().all()) and float((got - want).abs().max()) <= tol
