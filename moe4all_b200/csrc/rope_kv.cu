@@ -38,7 +38,7 @@ __device__ __forceinline__ void store4_f16(__half* dst, const float4& v) {
 
 // JS: eight-value chunks of a lane: 1 for heads up to 128, else 2.  Q8: the cache is one of 8 bits.
 template <int JS, bool Q8>
-__global__ void __launch_bounds__(ROPE_THREADS, Q8 ? 4 : 1) k_rope_kv(const __grid_constant__ RopeParams p) {
+__global__ void __launch_bounds__(ROPE_THREADS, JS == 2 && !Q8 ? 3 : 4) k_rope_kv(const __grid_constant__ RopeParams p) {
   // a head on its way into 8 bits: what shares a scale lies in two to six lanes, as n_rot has it
   __shared__ __align__(16) float s_head[Q8 ? ROPE_TEAMS * 128 * JS : 4];
   __shared__ __align__(16) float s_cos[ROPE_ROWS * ROPE_MAX_PAIRS], s_sin[ROPE_ROWS * ROPE_MAX_PAIRS];
