@@ -115,8 +115,8 @@ inline bool attn_few_rows(uint64_t max_rows, uint32_t g, uint64_t pairs) {
 }
 
 // Over pages of 8 bits: query heads to a kv head that the few-rows kernel takes, and whether it serves a call.  The tile kernel has the pages unpacked first.  Measured
-// (us, few-rows / tile kernel, 8000 keys, heads of 64; 128; 256): 64 rows, 8 pairs 34.8 / 38.5; 47.3 / 55.1; 83.4 / 105.8; 48 rows, 16 pairs 48.3 / 43.8; 60.8 / 68.8;
-// 119.5 / 134.8; 32 rows, 64 pairs 110.1 / 105.1; 140.5 / 161.2; 285.8 / 360.0, 256 pairs of heads of 128 530 / 547; 48 rows, 64 pairs 155 / 110; 198 / 166; 419 / 364.
+// (us, few-rows / tile kernel, 8000 keys, heads of 64; 128; 256): 64 rows, 8 pairs 35.0 / 40.6; 47.9 / 56.7; 82.9 / 102.8; 48 rows, 16 pairs 48.9 / 45.9; 61.2 / 68.0;
+// 118.8 / 134.3; 32 rows, 64 pairs 109.2 / 108.1; 141.5 / 167.3; 282.9 / 361.5, 256 pairs of heads of 128 529 / 553; 48 rows, 64 pairs 154 / 113; 197 / 172; 414 / 367.
 inline uint32_t attn_q8_rows_limit(uint32_t head_dim) { return head_dim > 128 ? 8u : (uint32_t)ATTN_ROWS_LIMIT; }
 inline bool attn_q8_few_rows(uint64_t max_rows, uint32_t g, uint32_t head_dim, uint64_t pairs) {
   return g <= attn_q8_rows_limit(head_dim) && max_rows <= (pairs <= 8 ? 64u : pairs <= 16 ? 48u : 32u);
