@@ -20,6 +20,7 @@
 #include <math_constants.h>
 
 #include "kernels.cuh"
+#include "sample_shape.h"
 
 namespace infr {
 namespace {
@@ -34,7 +35,6 @@ constexpr int SAMPLE_MAXIMA = 1024;   // so many largest ones are looked for by 
 constexpr int SAMPLE_FEW_BINS = 256;  // by bins of these,
 constexpr int SAMPLE_SLOTS = SAMPLE_LIST / SAMPLE_CTAS;  // and so many candidates of a CTA looked at
 constexpr int SAMPLE_CAP = 40960;     // values of a row in a CTA's shared memory at most
-constexpr double SAMPLE_REACH = 45.0; // weights down to e^-45 < 2^-64
 typedef unsigned long long u64;
 
 __device__ __forceinline__ float max3_nan(float a, float b, float c) {  // NaN where one is
@@ -834,9 +834,7 @@ __global__ void __cluster_dims__(SAMPLE_CTAS, 1, 1) __launch_bounds__(SAMPLE_THR
     return;
   }
   s.steps = 46.166241308446828 / (double)T;  // 32 log2(e)
-  // (an infinite largest value leaves those like it; rounded down, never up)
-  const double reach = (double)top - SAMPLE_REACH * (double)T;
-  s.floor_x = top == CUDART_INF_F ? top : reach > -3.0e38 ? __double2float_rd(reach) : -3.402823466e38f;
+  s.floor_x = sample_floor(top, T);
   const double least = min_p > 0.f ? fmin((double)min_p, 1.0) : 0.0, part = u > 0.f ? fmin((double)u, 1.0) : 0.0;
 
   u64 border = ~0ull;
