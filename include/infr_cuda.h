@@ -421,7 +421,9 @@ int32_t infr_cuda_attention(infr_cuda_ctx* ctx, const infr_cuda_attention_desc* 
  * which one is not finite, or past 60960, get the scale byte 0xFF: none of them is a number then.  (Any byte from 0xC0 on says that.)  What attention
  * makes of such keys and values it sees: a NaN score, and NaN in the 16 columns.
  * Attention of few rows reads the codes; for many rows (infr_cuda_attention_desc.path) the pages that are seen are unpacked into f16 ones of the context's
- * own first, which takes room for n_pages or n_seq * max_pages pages, whichever are fewer: made when a larger call comes, and not while recording.
+ * own first, which takes room for n_pages or n_seq * max_pages pages, whichever are fewer: made when a larger call comes, and not while recording.  Where the
+ * device has no room for them (nearly twice the layer's cache where it is given whole), path 0 takes the few-rows kernel if the heads allow it, recorded too
+ * once a call has found that out; path 2 fails with OOM.
  * Path 1 takes up to 8 query heads to a kv head here where they have more than 128 values. */
 int32_t infr_cuda_rope_kv_q8(infr_cuda_ctx* ctx, const infr_cuda_rope_kv_desc* desc, infr_cuda_buf* k_scale, infr_cuda_buf* v_scale);
 int32_t infr_cuda_attention_q8(infr_cuda_ctx* ctx, const infr_cuda_attention_desc* desc, const infr_cuda_buf* k_scale, const infr_cuda_buf* v_scale);

@@ -1195,33 +1195,53 @@ int32_t rope_kv(infr_cuda_ctx* ctx, const infr_cuda_rope_kv_desc* d, const KvSca
   return launch_rope_kv(ctx, p);
 }
 
-// The f16 pages of a call over pages of 8 bits: grown like the scratch, but what a recorded plan may read from stays.
+// The f16 pages of a call over pages of 8 bits: grown like the scratch, but what a recorded plan may read from stays, and a block is given up only for a larger one
+// that there is: what had room keeps it.
 int32_t ensure_unpacked(infr_cuda_ctx* ctx, uint64_t bytes) {
-  if (bytes > ctx->kv_unpacked_bytes) {
-    if (ctx->capturing) return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "attention: its f16 pages would have to be made while recording: run the call once un-recorded first");
-    cudaError_t e = cudaStreamSynchronize(ctx->stream);
-    if (e != cudaSuccess) return check_cuda(ctx, e, "attention: f16 pages: sync");
-    if (ctx->kv_unpacked && ctx->kv_unpacked_recorded) {
-      try {
-        ctx->kv_unpacked_before.push_back(ctx->kv_unpacked);
-      } catch (const std::bad_alloc&) {
-        return fail(ctx, INFR_CUDA_ERR_OOM, "attention: host out of memory");
-      }
-    } else if (ctx->kv_unpacked) {
-      cudaFree(ctx->kv_unpacked);
-    }
-    ctx->kv_unpacked = nullptr;
-    ctx->kv_unpacked_bytes = 0;
-    ctx->kv_unpacked_recorded = false;
-    e = cudaMalloc(&ctx->kv_unpacked, bytes);
-    if (e != cudaSuccess) {
-      ctx->kv_unpacked = nullptr;
-      cudaGetLastError();
-      return check_cuda(ctx, e, "attention: f16 pages of a cache in 8 bits");
-    }
-    ctx->kv_unpacked_bytes = bytes;
+  if (bytes <= ctx->kv_unpacked_bytes) {
+    if (ctx->capturing) ctx->kv_unpacked_recorded = true;
+    return INFR_CUDA_OK;
   }
-  if (ctx->capturing) ctx->kv_unpacked_recorded = true;
+  if (ctx->capturing) {
+    if (bytes >= ctx->kv_unpacked_refused) return fail(ctx, INFR_CUDA_ERR_OOM, "attention: f16 pages of a cache in 8 bits: the device had no room for them");
+    return fail(ctx, INFR_CUDA_ERR_INVALID_ARG, "attention: its f16 pages would have to be made while recording: run the call once un-recorded first");
+  }
+  cudaError_t e = cudaStreamSynchronize(ctx->stream);
+  if (e != cudaSuccess) return check_cuda(ctx, e, "attention: f16 pages: sync");
+  if (ctx->kv_unpacked && ctx->kv_unpacked_recorded) {
+    try {
+      ctx->kv_unpacked_before.reserve(ctx->kv_unpacked_before.size() + 1);
+    } catch (const std::bad_alloc&) {
+      return fail(ctx, INFR_CUDA_ERR_OOM, "attention: host out of memory");
+    }
+  }
+  char* made = nullptr;
+  e = cudaMalloc(&made, bytes);
+  if (e == cudaErrorMemoryAllocation && ctx->kv_unpacked && !ctx->kv_unpacked_recorded) {  // (there may be room where the old ones lie)
+    cudaGetLastError();
+    cudaFree(ctx->kv_unpacked);
+    ctx->kv_unpacked = nullptr;
+    e = cudaMalloc(&made, bytes);
+    if (e != cudaSuccess) {
+      cudaGetLastError();
+      if (cudaMalloc(&ctx->kv_unpacked, ctx->kv_unpacked_bytes) != cudaSuccess) {
+        cudaGetLastError();
+        ctx->kv_unpacked = nullptr;
+        ctx->kv_unpacked_bytes = 0;
+      }
+    }
+  }
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    if (e == cudaErrorMemoryAllocation && bytes < ctx->kv_unpacked_refused) ctx->kv_unpacked_refused = bytes;
+    return check_cuda(ctx, e, "attention: f16 pages of a cache in 8 bits");
+  }
+  if (ctx->kv_unpacked && ctx->kv_unpacked_recorded) ctx->kv_unpacked_before.push_back(ctx->kv_unpacked);
+  else if (ctx->kv_unpacked) cudaFree(ctx->kv_unpacked);
+  ctx->kv_unpacked = made;
+  ctx->kv_unpacked_bytes = bytes;
+  ctx->kv_unpacked_recorded = false;
+  if (bytes >= ctx->kv_unpacked_refused) ctx->kv_unpacked_refused = ~0ull;
   return INFR_CUDA_OK;
 }
 
@@ -1284,9 +1304,11 @@ int32_t attention(infr_cuda_ctx* ctx, const infr_cuda_attention_desc* d, const K
   const __half* k = scales.any() ? nullptr : static_cast<const __half*>(d->k->ptr);
   if (few) return launch_attn_rows(ctx, p, k, (int)(max_rows < 1024 ? max_rows : 1024));
   if (scales.any()) {
-    AttnUnpacked u;
-    if (!attn_unpacked(attn_sizes(d), &u)) return fail(ctx, INFR_CUDA_ERR_OOM, "attention: f16 pages of a cache in 8 bits past 2^48 bytes");
-    if ((rc = ensure_unpacked(ctx, u.table + 2 * u.side))) return rc;
+    AttnUnpacked u = {};
+    rc = attn_unpacked(attn_sizes(d), &u) ? ensure_unpacked(ctx, u.table + 2 * u.side) : fail(ctx, INFR_CUDA_ERR_OOM, "attention: f16 pages of a cache in 8 bits past 2^48 bytes");
+    // (no room: the few-rows kernel, which needs none, is slower for many rows, but serves them)
+    if (rc == INFR_CUDA_ERR_OOM && !d->path && g <= attn_q8_rows_limit(d->head_dim)) return launch_attn_rows(ctx, p, k, (int)(max_rows < 1024 ? max_rows : 1024));
+    if (rc) return rc;
     int* table = u.by_sequence ? reinterpret_cast<int*>(ctx->kv_unpacked) : nullptr;
     __half *kf = reinterpret_cast<__half*>(ctx->kv_unpacked + u.table), *vf = reinterpret_cast<__half*>(ctx->kv_unpacked + u.table + u.side);
     if ((rc = launch_kv_unpack(ctx, p, kf, vf, table))) return rc;

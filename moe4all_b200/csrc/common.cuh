@@ -82,6 +82,7 @@ struct infr_cuda_ctx {
   char* kv_unpacked = nullptr;                // device memory: the f16 pages of attention of many rows over pages of 8 bits, grown on demand.  A block that
   size_t kv_unpacked_bytes = 0;               // a recorded plan has the address of stays where it is until the context ends
   bool kv_unpacked_recorded = false;
+  unsigned long long kv_unpacked_refused = ~0ull;  // the least size that the device had no room for, since a larger one fitted
   std::vector<void*> kv_unpacked_before;
   unsigned long long* trace = nullptr;        // optional phase stamps (see trace_stamp)
   infr_cuda_config cfg = {};                  // tuning switches (infr_cuda_set_config)
