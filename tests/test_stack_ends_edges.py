@@ -1,0 +1,20 @@
+"""Ends of a `MoeStack` that could not be served are refused before a step runs."""
+import dataclasses
+
+import pytest
+import torch
+
+from test_stack_attention_bind import NE, Notes, stack
+from test_stack_ends import ends
+
+from moe4all_b200 import DType
+
+
+@pytest.mark.parametrize("dtype", [DType.F16, DType.BF16])
+def test_a_head_of_16_bits_is_refused_before_a_step(dtype):
+    """`linear` has no weights of 16 bits: a step would end at its last op, its keys and values written."""
+    be = Notes()
+    with pytest.raises(ValueError, match="head_dtype"):
+        stack(be, 2, None, ends=dataclasses.replace(ends(be, 2), head_dtype=dtype))
+    # (a table of them is fine)
+    stack(be, 2, None, ends=dataclasses.replace(ends(be, 2), table_dtype=dtype))
