@@ -169,6 +169,8 @@ class BoundEnds:
                 raise ValueError(f"StackEnds.{name} is {want} of the {rows} rows, not {t.dtype} {tuple(t.shape)}")
         if ends.head is not None and (ends.norm is None or ends.u is None):
             raise ValueError("StackEnds: a head needs the norm ahead of it, and random numbers")
+        if ends.norm is not None and (ends.norm.dtype != torch.float32 or ends.norm.numel() != ne or not ends.norm.is_contiguous()):
+            raise ValueError(f"StackEnds.norm is float32 of the {ne} values of a row, not {ends.norm.dtype} {tuple(ends.norm.shape)}")
         if ends.head is not None and DType(ends.head_dtype) in (DType.F16, DType.BF16):
             raise ValueError(f"StackEnds.head_dtype: a Linear has no weights of 16 bits ({DType(ends.head_dtype).name}): F32 or a block format")
         if ends.head is None and (ends.u is not None or settings):

@@ -18,3 +18,11 @@ def test_a_head_of_16_bits_is_refused_before_a_step(dtype):
         stack(be, 2, None, ends=dataclasses.replace(ends(be, 2), head_dtype=dtype))
     # (a table of them is fine)
     stack(be, 2, None, ends=dataclasses.replace(ends(be, 2), table_dtype=dtype))
+
+
+def test_a_norm_that_is_something_else_is_refused():
+    """The library sees its bytes only: one of f64 would be read as f32, one of 16 bits refused behind the layers."""
+    be = Notes()
+    for norm in (torch.ones(NE).double(), torch.ones(NE).half(), torch.ones(NE - 1), torch.ones(2 * NE)[::2]):
+        with pytest.raises(ValueError, match="norm"):
+            stack(be, 2, None, ends=dataclasses.replace(ends(be, 2), norm=norm))
