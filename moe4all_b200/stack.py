@@ -234,6 +234,10 @@ class MoeStack:
         self.attn = attn
         self._attn = None if attn is None else attn.bind(be, rows, ne, eps, self.b_hidden, dev)
         self.ends = None if ends is None else BoundEnds(ends, be, rows, ne, eps, self.b_hidden, self.b_hn, dev)
+        if dev.type == "cuda":
+            # The buffers above are torch's, in the order of its stream: they may still be somebody else's there, and their zeros on the way.  The first step's ops
+            # run on the backend's.
+            torch.cuda.current_stream(dev).synchronize()
 
     def attn_layer(self, li: int) -> None:
         """The attention sub-layer of one layer in place on `hidden`."""
