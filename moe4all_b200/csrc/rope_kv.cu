@@ -132,7 +132,17 @@ __global__ void __launch_bounds__(ROPE_THREADS, JS == 2 && !Q8 ? 3 : 4) k_rope_k
     __syncthreads();
     if (turns_one && my_row < rows) {
       const double t = (double)s_pos[my_row] * turns;
-      sincospif(2.f * (float)(t - rint(t)), s_sin + my_row * ROPE_MAX_PAIRS + my_pair, s_cos + my_row * ROPE_MAX_PAIRS + my_pair);
+      float *to_sin = s_sin + my_row * ROPE_MAX_PAIRS + my_pair, *to_cos = s_cos + my_row * ROPE_MAX_PAIRS + my_pair;
+      if constexpr (Q8) {
+        // What f32 leaves of the angle, up to 2^-26 of a turn, is as much as the sine's own rounding and would carry more values past a code's border: by the derivatives.
+        const double part = t - rint(t);
+        const float near = (float)part, rest = 6.2831853f * (float)(part - (double)near);
+        float sn, cs;
+        sincospif(2.f * near, &sn, &cs);
+        *to_sin = fmaf(rest, cs, sn), *to_cos = fmaf(-rest, sn, cs);
+      } else {
+        sincospif(2.f * (float)(t - rint(t)), to_sin, to_cos);
+      }
     }
     __syncthreads();
 #pragma unroll 1
