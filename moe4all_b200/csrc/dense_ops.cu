@@ -137,15 +137,16 @@ __global__ void __launch_bounds__(256) k_linear_anyfmt(int dt, const unsigned ch
 }
 
 // Rows of a token table by number, scaled: 16 weights to each of a thread's units.  An id outside the table gives zeros.
+// (Plain loads: the table may be what a kernel has written beside whose end this one has started, and the read-only path is for what stays as it is all the while.)
 template <int DT>
 __device__ __forceinline__ void embed_unit(int dt, const unsigned char* row, int h, float (&v)[16]) {
   if constexpr (DT == INFR_CUDA_DT_F32) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) *reinterpret_cast<float4*>(v + 4 * i) = __ldg(reinterpret_cast<const float4*>(row) + 4 * h + i);
+    for (int i = 0; i < 4; ++i) *reinterpret_cast<float4*>(v + 4 * i) = reinterpret_cast<const float4*>(row)[4 * h + i];
   } else if constexpr (DT == INFR_CUDA_DT_F16 || DT == INFR_CUDA_DT_BF16) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const uint4 x = __ldg(reinterpret_cast<const uint4*>(row) + 2 * h + i);
+      const uint4 x = reinterpret_cast<const uint4*>(row)[2 * h + i];
       const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -157,7 +158,7 @@ __device__ __forceinline__ void embed_unit(int dt, const unsigned char* row, int
     uint32_t c[4];
     float A, B;
     int off;
-    fmt_codes16(DT < 0 ? dt : DT, row, h, c, A, B, off);
+    fmt_codes16<false>(DT < 0 ? dt : DT, row, h, c, A, B, off);
 #pragma unroll
     for (int i = 0; i < 16; ++i) v[i] = fmaf(A, (float)((int)((c[i >> 2] >> (8 * (i & 3))) & 0xFFu) - off), B);
   }
@@ -168,7 +169,7 @@ constexpr int EMBED_THREADS = 128, EMBED_UNITS = 4;
 // Memory bounds it: the rows' bytes and their f32 values, once each.  A warp's values go through shared memory and out in whole lines (each thread's 64 bytes by
 // itself were half a sector to a store: 8191 rows of 7168 from Q8_0 67 us, now 50.3, 0.90 of the copy rate).
 template <int DT>
-__global__ void __launch_bounds__(EMBED_THREADS) k_embed(int dt, const unsigned char* __restrict__ table, const int* __restrict__ ids, float* __restrict__ dst, DeviceStatus* status, int ne,
+__global__ void __launch_bounds__(EMBED_THREADS) k_embed(int dt, const unsigned char* table, const int* ids, float* dst, DeviceStatus* status, int ne,
                                                          int n_vocab, size_t rb, size_t dst_stride, float scale) {
   __shared__ __align__(16) float s_v[EMBED_THREADS * 16];
   const int lane = threadIdx.x & 31, warp0 = threadIdx.x - lane;
@@ -178,7 +179,7 @@ __global__ void __launch_bounds__(EMBED_THREADS) k_embed(int dt, const unsigned 
   const int id = __ldcg(ids + blockIdx.x);
   const bool has = (unsigned)id < (unsigned)n_vocab;
   if (!has && threadIdx.x == 0 && blockIdx.y == 0) status->bad_index = 3;
-  const unsigned char* row = table + (has ? (size_t)id * rb : 0);
+  const unsigned char* row = after_wait(table) + (has ? (size_t)id * rb : 0);
   float* to = dst + (size_t)blockIdx.x * dst_stride;
 #pragma unroll 1
   for (int k = 0; k < EMBED_UNITS; ++k) {
