@@ -212,10 +212,14 @@ def moe_layer_op(be: CudaBackend, gg, layer: int, arch: Optional[str] = None) ->
     n_used = gg.meta_u64(f"{arch}.expert_used_count") if arch else None
     if not n_used:
         raise BackendError(ERR_INVALID_ARG, "GGUF: no expert_used_count in the metadata")
+    dtype = {k: DType(t.dtype) for k, t in info.items()}
+    for k, t in dtype.items():
+        if t in (DType.F16, DType.BF16):  # (types of token tables, which `embed` takes)
+            raise ValueError(f"GGUF: {need[k]} is {t.name}: not a type that a MoE layer's tensors may have")
     b = {k: gg.upload(be, n) for k, n in need.items()}
     op = MoeFfn(x=None, router=b["router"], gate_exps=b["gate"], up_exps=b["up"], down_exps=b["down"], dst=None, rows=0, ne=ne,
-                n_expert=n_expert, n_used=int(n_used), n_ff_exp=n_ff, router_dtype=DType(info["router"].dtype),
-                gate_dtype=DType(info["gate"].dtype), up_dtype=DType(info["up"].dtype), down_dtype=DType(info["down"].dtype))
+                n_expert=n_expert, n_used=int(n_used), n_ff_exp=n_ff, router_dtype=dtype["router"],
+                gate_dtype=dtype["gate"], up_dtype=dtype["up"], down_dtype=dtype["down"])
     if gg.find(p + "exp_probs_b.bias") is not None:
         b["bias"] = gg.upload(be, p + "exp_probs_b.bias")
         op.exp_probs_b = b["bias"]
