@@ -417,7 +417,9 @@ int32_t infr_cuda_attention(infr_cuda_ctx* ctx, const infr_cuda_attention_desc* 
  *   codes   k_cache, v_cache (k, v): u8 [n_pages, n_kv, page_size, head_dim]
  *   scales  k_scale, v_scale: u8 [n_pages, n_kv, page_size, head_dim / 16], a byte for 16 values
  * A scale byte s is the f16 number d with the bits s << 7 (four significant bits), a code c the value (c - 128) d, which is an f16 number.
- * rope_kv takes the least d with 127 d >= the largest magnitude of the 16, and the nearest codes: a value is off by d / 2 at most.  16 values of
+ * rope_kv takes the least d with 127 d >= the largest magnitude of the 16, and the nearest codes: a value is off by d / 2 at most (and by what f32 rounds of
+ * the row and of its quotient by d).  Below 2^-14 these numbers are 2^-17 apart: 16 values whose largest is less than 7.8e-3 have fewer than 113 codes to a side,
+ * 65 where it is 1e-3, 13 at 1e-4, and their error does not fall below 2^-18.  16 values of
  * which one is not finite, or past 60960, get the scale byte 0xFF: none of them is a number then.  (Any byte from 0xC0 on says that.)  What attention
  * makes of such keys and values it sees: a NaN score, and NaN in the 16 columns.
  * Attention of few rows reads the codes; for many rows (infr_cuda_attention_desc.path) the pages that are seen are unpacked into f16 ones of the context's
@@ -466,7 +468,8 @@ int32_t infr_cuda_embed(infr_cuda_ctx* ctx, const infr_cuda_embed_desc* desc);
  *   kept    the top_k largest (of equal ones the lowest ids), of these the shortest run from the largest that has top_p of their weight, of these
  *           the ones with w_i >= min_p
  *   ids[r]  the first kept id whose weight and the kept ones' of lower ids are more than u times the kept ones' together
- * Weights and sums are f64; weights below 2^-64 count as none.
+ * Weights and sums are f64.  Tokens more than 45 temperatures below the largest (weights below e^-45) count as none: together they have n_vocab 2^-64 of the weight
+ * at most, and only a u below that can tell: u = 0 takes the first kept token with a weight.
  * temperature: 0 or less (or NaN) takes the largest logit, of equal ones the lowest id; NULL: 1.  top_k: 0 or less keeps all.  top_p: 1 and above (or NaN)
  * keeps all, 0 and below the largest.  min_p: 0 and below (or NaN) keeps all, at most 1 counts.  u: in [0, 1); 1 and above the last kept one, NaN or below 0
  * the first.  Logits of -inf are never taken; among +inf ones all count alike and the others do not.  A row with a NaN, or with nothing above -inf, gives -1

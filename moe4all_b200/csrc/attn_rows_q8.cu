@@ -12,9 +12,10 @@
 // group asks for a whole tile, each in its turn (by every warp for itself the copies were a third of all instructions, and a warp more would take registers from all).
 // Between items stands one barrier of the CTA, behind which all add up the warps' sums; an item's q and its other words are made ready two items ahead.
 //
-// Measured (heads of 128, 32 to 4 kv heads): single tokens of 64 sequences of 700 to 8000 keys 76.9 us (f16 pages 85), one of 131072 keys 51.5 (60; 143 MB, 2.8 TB/s), one
-// of 513 12.7 (10.8), of which the plan and the first item take 8 to 10.  What bounds it is latency: four warps to a scheduler, 550 to 680 instructions to 16 keys, issue 0.43;
-// an operation less to every pair of codes was half a per cent.
+// Measured (heads of 128, 32 to 4 kv heads; f16 pages in turn): single tokens of 64 sequences of 700 to 8000 keys 76.3 us (83.2), one of 131072 keys 51.3 (59.5; 143 MB, 2.8
+// TB/s), one of 513 13.0 (11.0), of which the plan and the first item take 8 to 10.  What bounds it is latency: four warps to a scheduler, 550 to 680 instructions to 16 keys,
+// issue 0.43.  By stamps, of a warp's 133 thousand cycles in a CTA with five items the tiles' work takes 39 to 45, waits for them 11 to 26, asking for the next ones 8 to 11,
+// the barrier and the warps' sums at items' ends 11 to 33, the plan and the first item 7 to 19; an operation less to every pair of codes was half a per cent.
 #include "attn.cuh"
 #include "kv_q8.cuh"
 

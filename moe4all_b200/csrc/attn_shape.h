@@ -117,6 +117,10 @@ inline bool attn_few_rows(uint64_t max_rows, uint32_t g, uint64_t pairs) {
 // Over pages of 8 bits: query heads to a kv head that the few-rows kernel takes, and whether it serves a call.  The tile kernel has the pages unpacked first.  Measured
 // (us, few-rows / tile kernel, 8000 keys, heads of 64; 128; 256): 64 rows, 8 pairs 35.0 / 40.6; 47.9 / 56.7; 82.9 / 102.8; 48 rows, 16 pairs 48.9 / 45.9; 61.2 / 68.0;
 // 118.8 / 134.3; 32 rows, 64 pairs 109.2 / 108.1; 141.5 / 167.3; 282.9 / 361.5, 256 pairs of heads of 128 529 / 553; 48 rows, 64 pairs 154 / 113; 197 / 172; 414 / 367.
+// One rule for all heads, so it loses at some: 48 rows, 16 pairs of heads of 64 6 %, 32 rows, 256 pairs of these 5 % (372 / 354); 64 rows, 16 pairs of heads of 128
+// 75.8 / 85.8, which go to the tiles, 13 % (over 1000 keys 24.6 / 34.6).
+// Nine to sixteen query heads of more than 128 values to a kv head go to the tiles even with single tokens, as the few-rows kernel's sums of 16 such rows have no room beside
+// its key tiles: 64 tokens over 700 - 8000 keys, 12 heads of 256 159 us (f16 pages 84), 16 of 192 110 (51); one token over 8000 keys, 16 of 256 55 (39).
 inline uint32_t attn_q8_rows_limit(uint32_t head_dim) { return head_dim > 128 ? 8u : (uint32_t)ATTN_ROWS_LIMIT; }
 inline bool attn_q8_few_rows(uint64_t max_rows, uint32_t g, uint32_t head_dim, uint64_t pairs) {
   return g <= attn_q8_rows_limit(head_dim) && max_rows <= (pairs <= 8 ? 64u : pairs <= 16 ? 48u : 32u);

@@ -167,7 +167,7 @@ __device__ __forceinline__ void embed_unit(int dt, const unsigned char* row, int
 constexpr int EMBED_THREADS = 128, EMBED_UNITS = 4;
 
 // Memory bounds it: the rows' bytes and their f32 values, once each.  A warp's values go through shared memory and out in whole lines (each thread's 64 bytes by
-// itself were half a sector to a store: 8191 rows of 7168 from Q8_0 67 us, now 50.3, 0.90 of the copy rate).
+// itself were half a sector to a store: 8191 rows of 7168 from Q8_0 67 us, now 49.8, 0.91 of the copy rate).
 template <int DT>
 __global__ void __launch_bounds__(EMBED_THREADS) k_embed(int dt, const unsigned char* table, const int* ids, float* dst, DeviceStatus* status, int ne,
                                                          int n_vocab, size_t rb, size_t dst_stride, float scale) {

@@ -7,14 +7,14 @@
 //
 // What is kept is always a run from the largest, so it is one border: a value and an index.  Finding it needs no sort of the row: a histogram of the values says
 // between which of them it lies, and the few that lie there are sorted.  Weights and their sums are f64: with f32 sums the token next to a border would
-// go by the order of the additions, and there are 10^5 borders to a row.  Weights below 2^-64 of the largest count as none: all of them together are 2^-46,
-// which an f32 u cannot tell from nothing.
+// go by the order of the additions, and there are 10^5 borders to a row.  Weights below e^-45 of the largest count as none (sample_shape.h): all of them together are
+// 2^-47 of 150000 tokens, 2^-40 of the 2^24 that a row may have.  A u below that, 0 among them, would tell: it takes the first kept token with a weight.
 //
 // A cluster of eight CTAs has a row.  Every decision is made from numbers that all eight have got from one of them, added up in the same order, so that they
 // take the same steps and meet at the same barriers whatever the row and its settings hold (and should somebody write them meanwhile).
 //
-// Measured, of 150000: one row of which the largest is taken 5.2 us, of the 20 largest 7.1, of all 12.2, of the 1000 largest those with 0.95 25.7, of all with 0.9, spread over
-// thousands, 45; 64 rows 17, 25, 41, 66, 137, with settings of all kinds 79.  One pass over the row reads it (2.6 us of the 45); what bounds the rest is the f64 of a
+// Measured, of 150000: one row of which the largest is taken 5.1 us, of the 20 largest 7.1, of all 12, of the 1000 largest those with 0.95 25.5, of all with 0.9, spread over
+// thousands, 45; 64 rows 17, 25, 40, 65, 137, with settings of all kinds 74.  One pass over the row reads it (2.6 us of the 45); what bounds the rest is the f64 of a
 // weight - thirteen operations to a value, in four passes - and the barriers of the cluster, a microsecond each.
 #include <cooperative_groups.h>
 #include <math_constants.h>
@@ -952,8 +952,9 @@ int32_t launch_sample(infr_cuda_ctx* ctx, const float* logits, const float* u, c
                       float* prob, size_t stride, int rows, int n_vocab) {
   SampleParams p = {logits, u, temperature, top_p, min_p, top_k, ids, prob, stride, n_vocab, 0};
   const int per = ((n_vocab + 3 + 3) / 4 + SAMPLE_CTAS - 1) / SAMPLE_CTAS * 4;
-  // A row that fits is kept in shared memory: 64 rows of 150000 with settings of all kinds 98 us (79 since), read again from L2 108, with 256 threads to a CTA (all rows at
-  // once then, but each of them slower) 141, with four CTAs to a row 128; rows that all take one of the 20 largest 25, 26 and 17.
+  // A row that fits is kept in shared memory, which leaves room for 37 rows at a time.  That was measured with 64 rows of 150000, settings of all kinds: kept 98 us, read
+  // again from L2 108, with 256 threads to a CTA (all rows at once then, but each of them slower) 141, with four CTAs to a row 128.  Where all 64 take one of the 20 largest
+  // the choice loses: 25 us, 26 from L2, but 17 with 256 threads.
   p.cached = per <= SAMPLE_CAP;
   const size_t smem = p.cached ? (size_t)per * 4 : 0;
   cudaError_t e = ensure_smem(reinterpret_cast<const void*>(&k_sample), (size_t)SAMPLE_CAP * 4);

@@ -149,8 +149,8 @@ class StackEnds:
     n_vocab: int
     table_dtype: DType = DType.F32
     scale: float = 1.0  # of the table's rows
-    norm: Optional[torch.Tensor] = None
-    head: Optional[Buffer] = None  # [n_vocab, ne] of head_dtype
+    norm: Optional[torch.Tensor] = None  # [ne] f32
+    head: Optional[Buffer] = None  # [n_vocab, ne] of head_dtype: F32 or a block format, as a Linear has it
     head_dtype: DType = DType.F32
     u: Optional[torch.Tensor] = None
     temperature: Optional[torch.Tensor] = None
