@@ -61,5 +61,6 @@ def test_f16_pages_that_do_not_fit(backend):
     with pytest.raises(BackendError, match="f16 pages"):
         be.attention(b.op(be, **big, path=2))
     right(small, lambda: be.execute(plan))
-    del plan, small_op, op, big
+    del plan, small_op, op, big, codes, scales
     be.close()
+    torch.cuda.empty_cache()  # (tens of GB)
